@@ -205,6 +205,59 @@ int s2v_loss_acc_f32(s2v_ctx* ctx, s2v_stream stream, int64_t num_graphs, int nu
                      const int32_t* label_row_ptr, const int32_t* label_col_idx, const float* label_val, int topk,
                      float* loss_mean, float* acc_mean, float* per_graph_loss);
 
+/* ---- dense layers with 8-bit weights (no counterpart in the reference, whose tensors are fp32) ----
+ * Matrices of these entry points are row-major with a leading dimension in ELEMENTS of its own; with one row (or none) it is not read. */
+typedef enum s2v_dtype { S2V_F32 = 0, S2V_F16 = 1, S2V_BF16 = 2 } s2v_dtype;
+/* Rows to 8-bit integers: with a_i = max_j |x_ij|,
+ *     q_ij = the integer nearest to x_ij * (127 / a_i), ties to even, both operations in fp32;   scale_i = a_i / 127,
+ * so that x_ij is about scale_i * q_ij and |q_ij| <= 127.  Tokens of an activation matrix, or channels of a weight matrix stored a
+ * channel a row.  A row without a value of 2^-110 or more gets q = 0 and scale = 0; a row with an infinity or NaN gets q = 0 and
+ * scale = NaN, which makes its products NaN.  x : [rows x cols] of x_type; q : int8 [rows x cols]; scale : [rows].  Columns of q between
+ * cols and ldq are left as they were.  x and q must not overlap. */
+int s2v_quantize_rows_i8(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t cols, int x_type, const void* x, int64_t ldx,
+                         int8_t* q, int64_t ldq, float* scale);
+/* C_ij = act((a_scale_i * b_scale_j) * sum_l A_il * B_jl + bias_j), act = ReLU where relu != 0 (NaN stays NaN).  The sum is exact (32-bit
+ * integers, k <= 131,071), the rest fp32, rounded once to c_type.  A : int8 [m x k], a row per token; B : int8 [n x k], a row per output
+ * channel (every value from -128 to 127 is allowed); a_scale [m], b_scale [n]; bias [n] or NULL; C : [m x n] of c_type, which overlaps no
+ * input.  Rows of A and B start on 16-byte boundaries: pointers and leading dimensions (of matrices of more than one row) are multiples of 16. */
+int s2v_gemm_i8(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, int64_t k, const int8_t* A, int64_t lda, const float* a_scale,
+                const int8_t* B, int64_t ldb, const float* b_scale, const float* bias, int relu, int c_type, void* C, int64_t ldc);
+/* The layer as a model calls it: s2v_quantize_rows_i8 on x : [m x k] of x_type, then s2v_gemm_i8 with W : int8 [n x k] and w_scale [n] as
+ * above into y : [m x n] of y_type; the same values as the two calls give.  `workspace` (16-byte aligned) takes the 8-bit rows and their
+ * scales; calls that share one must be ordered, those inside captured graphs among them. */
+size_t s2v_linear_i8_workspace_bytes(int64_t m, int64_t k);
+int s2v_linear_i8(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, int64_t k, int x_type, const void* x, int64_t ldx,
+                  const int8_t* W, int64_t ldw, const float* w_scale, const float* bias, int relu, void* workspace, size_t workspace_bytes,
+                  int y_type, void* y, int64_t ldy);
+
+/* ---- distillation: the loss of a student's logits against a teacher's top logits, and its gradient (no counterpart in the reference;
+ * it stands beside s2v_cross_entropy_f32, which takes labels) ----
+ * Row i of z : [rows x cols] of z_type holds the student's logits.  idx and t : [rows x top], leading dimension ldt, list up to 256 classes
+ * of the row with the teacher's logits (t of t_type), in any order; an entry with idx < 0 is not there.  With T = temperature (1e-30 to 1e30),
+ * over the entries that are there:
+ *     t_lse == NULL:  p_k = softmax of t_k / T over the list;  rest = 0
+ *     t_lse given:    p_k = exp(t_k / T - t_lse_i), t_lse_i = log-sum-exp of ALL the teacher's logits / T;  rest = max(0, 1 - sum p_k)
+ *     q_j = softmax of z_ij / T over all columns;  s = sum of q_j over the columns that no entry names
+ *     loss_i = row_weight_i * ( sum_k p_k (log p_k - log q_idx_k) + rest (log rest - log s) )
+ *     dz_ij  = row_weight_i / T * ( q_j (sum p + rest) - sum of p_k over the entries of column j - [no entry names j] q_j rest / s )
+ * i.e. the Kullback-Leibler divergence of the listed classes, with t_lse all others as one class, and its gradient.  (Training often scales
+ * it by T^2: put that into row_weight, which is 1 where NULL.)  Entries with p_k = 0 add nothing.  A class listed twice counts with each of its
+ * entries' p, and once in s.  Where s = 0 the rest's term is left out if rest <= 2^-16 (the rounding of t_lse) and infinite otherwise.
+ * A row whose list is empty, whose p are all zero without t_lse (every t is -infinity), or whose row_weight is 0 has loss 0 and gradient 0,
+ * whatever z holds there: its z is not read (for a weight of 0: unless stats are asked for).  -infinity in z is a class that the student excludes (q = 0); a row of z with NaN or +infinity, or
+ * without a finite value, has NaN as its loss and gradient, and so has a row with NaN or +infinity among its entries' t.  An entry with idx >= cols is left out and reported through the status word (S2V_ERR_INVALID_ARG).
+ *   loss : [rows];  stats : float [rows x 4], 16-byte aligned, or NULL, for s2v_distill_topk_grad;  dz : [rows x cols] of z_type or NULL: the gradient in the same
+ *   call.  dz may be z itself (with lddz = ldz); else it overlaps no input.  At most
+ *   1,048,576 columns. */
+int s2v_distill_topk(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t cols, int z_type, const void* z, int64_t ldz, int top,
+                     const int32_t* idx, int t_type, const void* t, int64_t ldt, const float* t_lse, float temperature,
+                     const float* row_weight, float* loss, float* stats, void* dz, int64_t lddz);
+/* The gradient alone, of sum_i row_weight_i * KL_i, from the `stats` that s2v_distill_topk wrote for the same z, list, t_lse and temperature;
+ * row_weight is that of this call (the gradient that arrives at each row's loss). */
+int s2v_distill_topk_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t cols, int z_type, const void* z, int64_t ldz, int top,
+                          const int32_t* idx, int t_type, const void* t, int64_t ldt, const float* t_lse, float temperature,
+                          const float* row_weight, const float* stats, void* dz, int64_t lddz);
+
 /* ---- graph pooling: Y[g,:] = sum of H[n,:] over n in [seg_ptr[g], seg_ptr[g+1]).
  * Replaces MatMul(SubgraphMsgPass CSR, H) (kernel_mean_field.cpp:44,
  * src/nn/msg_pass.cpp:156-177) for the batcher's layout, where graph g owns a
