@@ -1,0 +1,287 @@
+// C = act((a_scale x b_scale) * (A B^T) + bias) for 8-bit A [m x k] and B [n x k]: tcgen05 matrix instructions with 32-bit integer accumulators.
+//
+// A persistent CTA per SM walks over tiles of 128 x BN outputs.  One warp copies panels of 128 bytes along k (tensor maps, 128-byte swizzle; zeros
+// outside the matrices) into a ring, one issues the products, eight take finished accumulators out of tensor memory, of which there are two, so
+// that a tile's outputs are written under the next tile's products.
+#include <cstring>
+#include <type_traits>
+
+#include "gemm_i8.cuh"
+#include "tcgen05.cuh"
+#include "tma.cuh"
+
+namespace
+{
+
+constexpr int GI_EPI = 8;                              // epilogue warps
+constexpr int GI_THREADS = 32 * (2 + GI_EPI);
+constexpr int GI_PIECE = 64, GI_PITCH = 80;             // bytes of a row that an epilogue warp stages at a time; bytes between the staged rows (no bank conflicts)
+
+template <int BN> struct GiCfg {
+    static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr uint32_t TM_COLS = 2 * BN;
+    static constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);   // s32 <- s8 x s8, M = 128, N = BN
+    static constexpr uint32_t OFF_OUT = STAGES * STAGE;                       // per epilogue warp: 32 rows
+    static constexpr uint32_t OFF_SCALE = OFF_OUT + GI_EPI * 32 * GI_PITCH;   // per epilogue warp: 32 channels' scales, then their biases
+    static constexpr uint32_t OFF_BAR = OFF_SCALE + GI_EPI * 2 * 32 * 4;
+    enum { FULL = 0, EMPTY = FULL + STAGES, DONE = EMPTY + STAGES, READ = DONE + 2, BARS = READ + 2 };
+    static constexpr uint32_t OFF_MISC = OFF_BAR + 8 * BARS;
+    static constexpr uint32_t SMEM = OFF_MISC + 16 + 1024;                    // + slack to align the base to 1024 bytes
+    static_assert(SMEM <= 227 * 1024, "shared memory");
+};
+
+struct GiArgs {
+    int64_t m, n, ldc;
+    int kblocks, last_steps;        // panels along k; matrix instructions of the last one (32 bytes each)
+    int m_tiles, n_tiles;
+    const float* a_scale;
+    const float* b_scale;
+    const float* bias;
+    void* C;
+    int relu, wide;                 // wide: 16-byte stores of whole rows' pieces are aligned
+    s2v_device_status* status;
+};
+
+__device__ __forceinline__ void gi_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        :
+        : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// two fp32 values to one register of two 16-bit ones
+template <typename T> __device__ __forceinline__ uint32_t gi_pack(float a, float b)
+{
+    uint32_t r;
+    if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+
+// Tiles in columns of 16 row tiles, so that the tiles of one moment share panels of both matrices in L2.
+__device__ __forceinline__ void gi_tile(int tile, int m_tiles, int n_tiles, int& tm, int& tn)
+{
+    constexpr int G = 16;
+    const int per = G * n_tiles, g = tile / per, first = g * G, rows = min(G, m_tiles - first), at = tile - g * per;
+    tm = first + at % rows;
+    tn = at / rows;
+}
+
+// The outputs of 32 rows (lanes) by COLS columns, staged so that the store instructions write whole sectors.
+template <typename T>
+__device__ __forceinline__ void gi_write(const GiArgs& a, unsigned char* stage, const float* chan, int64_t row0, int64_t col0, float sa, uint32_t tmem, bool any)
+{
+    constexpr int COLS = GI_PIECE / sizeof(T), PER = 16 / sizeof(T);
+    const int lane = threadIdx.x & 31;
+    unsigned char* const mine = stage + lane * GI_PITCH;
+    uint32_t v[COLS];
+    if (any) {
+#pragma unroll
+        for (int h = 0; h < COLS; h += 16) tc_ld_cols16(tmem + h, v + h);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    } else {
+#pragma unroll
+        for (int j = 0; j < COLS; ++j) v[j] = 0;
+    }
+#pragma unroll
+    for (int j = 0; j < COLS; j += 4) {
+        const float4 s = *reinterpret_cast<const float4*>(chan + j), b = *reinterpret_cast<const float4*>(chan + 32 + j);
+        float y[4] = {fmaf(__fmul_rn(sa, s.x), (float)(int)v[j], b.x), fmaf(__fmul_rn(sa, s.y), (float)(int)v[j + 1], b.y),
+                      fmaf(__fmul_rn(sa, s.z), (float)(int)v[j + 2], b.z), fmaf(__fmul_rn(sa, s.w), (float)(int)v[j + 3], b.w)};
+        if (a.relu) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) y[u] = relu_ref(y[u]);
+        }
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(mine + 4 * j) = make_float4(y[0], y[1], y[2], y[3]);
+        else *reinterpret_cast<uint2*>(mine + 2 * j) = make_uint2(gi_pack<T>(y[0], y[1]), gi_pack<T>(y[2], y[3]));
+    }
+    __syncwarp();
+    T* const C = static_cast<T*>(a.C);
+    const int seg = lane & 3;
+    const int64_t c = col0 + seg * PER;
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+        const int r = it * 8 + (lane >> 2);
+        if (row0 + r < a.m && c < a.n) {
+            const T* const from = reinterpret_cast<const T*>(stage + r * GI_PITCH + 16 * seg);
+            T* const to = C + (row0 + r) * a.ldc + c;
+            if (a.wide && c + PER <= a.n) {
+                *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+            } else {
+#pragma unroll
+                for (int u = 0; u < PER; ++u)
+                    if (c + u < a.n) to[u] = from[u];
+            }
+        }
+    }
+    __syncwarp();
+}
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GiArgs a)
+{
+    using Cfg = GiCfg<BN>;
+    constexpr int STAGES = Cfg::STAGES;
+    extern __shared__ unsigned char gi_raw[];
+    unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(gi_raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t smem0 = smem_u32(smem);
+    const auto bar = [&](int i) { return smem0 + Cfg::OFF_BAR + 8u * (uint32_t)i; };
+    volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + Cfg::OFF_MISC);
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_MISC + 8);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tiles = a.m_tiles * a.n_tiles;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) tc_mbar_init(bar(Cfg::FULL + i), 1), tc_mbar_init(bar(Cfg::EMPTY + i), 1);
+        for (int i = 0; i < 2; ++i) tc_mbar_init(bar(Cfg::DONE + i), 1), tc_mbar_init(bar(Cfg::READ + i), GI_EPI);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (a.kblocks > 0) tma_prefetch_map(&map_a), tma_prefetch_map(&map_b);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(Cfg::TM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {   // copies
+        int it = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+            int tm, tn;
+            gi_tile(tile, a.m_tiles, a.n_tiles, tm, tn);
+            for (int kb = 0; kb < a.kblocks; ++kb, ++it) {
+                const int s = it % STAGES;
+                if (it >= STAGES && !(ok = tc_wait(bar(Cfg::EMPTY + s), (uint32_t)(it / STAGES - 1) & 1u, abort_flag, a.status, 70))) break;
+                if (tc_elect()) {
+                    const uint32_t at = smem0 + (uint32_t)s * Cfg::STAGE, b = bar(Cfg::FULL + s);
+                    mbar_expect(b, Cfg::STAGE);
+                    tma_load_2d(at, &map_a, kb * 128, tm * 128, b);
+                    tma_load_2d(at + Cfg::A_BYTES, &map_b, kb * 128, tn * BN, b);
+                }
+                __syncwarp();
+            }
+        }
+        // no copy may arrive once the CTA has gone: where a wait gave up, the ones under way are waited for here (bounded like every wait)
+        if (!ok || *abort_flag)
+            for (int i = max(0, it - STAGES); i < it; ++i) {
+                int spins = 0;
+                while (!tc_mbar_try(bar(Cfg::FULL + i % STAGES), (uint32_t)(i / STAGES) & 1u))
+                    if (++spins > TC_WAIT_LIMIT) break;
+            }
+    } else if (warp == 1) {   // products
+        int it = 0, t = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++t) {
+            const int acc = t & 1;
+            if (t >= 2 && !(ok = tc_wait(bar(Cfg::READ + acc), (uint32_t)(t / 2 - 1) & 1u, abort_flag, a.status, 71))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int kb = 0; kb < a.kblocks; ++kb, ++it) {
+                const int s = it % STAGES;
+                if (!(ok = tc_wait(bar(Cfg::FULL + s), (uint32_t)(it / STAGES) & 1u, abort_flag, a.status, 72))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (tc_elect()) {
+                    const uint64_t da = tc_b_desc(smem0 + (uint32_t)s * Cfg::STAGE), db = tc_b_desc(smem0 + (uint32_t)s * Cfg::STAGE + Cfg::A_BYTES);
+                    const int steps = kb + 1 == a.kblocks ? a.last_steps : 4;
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks)
+                        if (ks < steps) gi_mma(tmem + (uint32_t)(acc * BN), da + 2u * ks, db + 2u * ks, Cfg::IDESC, kb > 0 || ks > 0);
+                    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar(Cfg::EMPTY + s)) : "memory");
+                    if (kb + 1 == a.kblocks)
+                        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar(Cfg::DONE + acc)) : "memory");
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok || *abort_flag)   // products under way read shared memory and write tensor memory
+            for (int i = max(0, it - STAGES); i < it; ++i) {
+                int spins = 0;
+                while (!tc_mbar_try(bar(Cfg::EMPTY + i % STAGES), (uint32_t)(i / STAGES) & 1u))
+                    if (++spins > TC_WAIT_LIMIT) break;
+            }
+    } else {   // outputs: two warps per quarter of the accumulator's lanes, half of the columns each
+        constexpr int COLS = GI_PIECE / sizeof(T), HALF = BN / 2;
+        static_assert(HALF % COLS == 0 && COLS <= 32, "pieces of half a tile's rows");
+        const int e = warp - 2, quarter = warp & 3, half = e >> 2;
+        unsigned char* const stage = smem + Cfg::OFF_OUT + e * 32 * GI_PITCH;
+        float* const chan = reinterpret_cast<float*>(smem + Cfg::OFF_SCALE) + e * 64;
+        int t = 0;
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++t) {
+            int tm, tn;
+            gi_tile(tile, a.m_tiles, a.n_tiles, tm, tn);
+            const int acc = t & 1;
+            const int64_t row0 = (int64_t)tm * 128 + quarter * 32;
+            const float sa = row0 + lane < a.m ? __ldg(a.a_scale + row0 + lane) : 0.0f;
+            if (a.kblocks > 0 && !tc_wait(bar(Cfg::DONE + acc), (uint32_t)(t / 2) & 1u, abort_flag, a.status, 73)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int c = half * HALF; c < (half + 1) * HALF; c += COLS) {
+                const int64_t col0 = (int64_t)tn * BN + c;
+                if (row0 >= a.m || col0 >= a.n) break;   // (the same for the warp)
+                if (lane < COLS) {
+                    const int64_t col = col0 + lane;
+                    chan[lane] = col < a.n ? __ldg(a.b_scale + col) : 0.0f;
+                    chan[32 + lane] = a.bias && col < a.n ? __ldg(a.bias + col) : 0.0f;
+                }
+                __syncwarp();
+                gi_write<T>(a, stage, chan, row0, col0, sa, tmem + (uint32_t)(acc * BN + c) + ((uint32_t)quarter << 21), a.kblocks > 0);
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            if (lane == 0) tc_mbar_arrive(bar(Cfg::READ + acc));
+            __syncwarp();
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::TM_COLS) : "memory");
+}
+
+template <typename T, int BN> int gi_launch(s2v_ctx* ctx, cudaStream_t st, const s2v_gemm_i8_args& g)
+{
+    using Cfg = GiCfg<BN>;
+    CUtensorMap map_a, map_b;
+    if (g.k > 0) {
+        // (the leading dimension of a single row is not the caller's to get right)
+        const int64_t up = (g.k + 15) / 16 * 16;
+        if (!s2v_byte_matrix_map(&map_a, g.A, g.m, g.k, g.m > 1 ? g.lda : up, 128) || !s2v_byte_matrix_map(&map_b, g.B, g.n, g.k, g.n > 1 ? g.ldb : up, BN))
+            return s2v_fail(ctx, S2V_ERR_CUDA, "gemm_i8: the driver did not take a matrix's tensor map");
+    } else {
+        memset(&map_a, 0, sizeof(map_a));
+        memset(&map_b, 0, sizeof(map_b));
+    }
+    GiArgs a;
+    a.m = g.m, a.n = g.n, a.ldc = g.ldc;
+    a.kblocks = (int)((g.k + 127) / 128);
+    a.last_steps = g.k > 0 ? (int)((g.k - 128 * (int64_t)(a.kblocks - 1) + 31) / 32) : 0;
+    const int64_t mt = (g.m + 127) / 128, nt = (g.n + BN - 1) / BN;
+    if (mt * nt > INT32_MAX / 2) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, "gemm_i8: more than 2^30 tiles of outputs");
+    a.m_tiles = (int)mt, a.n_tiles = (int)nt;
+    a.a_scale = g.a_scale, a.b_scale = g.b_scale, a.bias = g.bias, a.C = g.C, a.relu = g.relu;
+    a.wide = s2v_aligned16(g.C) && (g.m == 1 || g.ldc * (int64_t)sizeof(T) % 16 == 0);
+    a.status = ctx->dstatus_dev;
+    S2V_CUDA_OK(ctx, s2v_allow_shared(gemm_i8_kernel<T, BN>, Cfg::SMEM));
+    const int64_t tiles = mt * nt;
+    const unsigned grid = (unsigned)(tiles < ctx->sm_count ? tiles : ctx->sm_count);
+    gemm_i8_kernel<T, BN><<<grid, GI_THREADS, Cfg::SMEM, st>>>(map_a, map_b, a);
+    S2V_CHECK_LAUNCH(ctx, "gemm_i8_kernel");
+    return S2V_OK;
+}
+
+}  // namespace
+
+int s2v_launch_gemm_i8(s2v_ctx* ctx, cudaStream_t st, const s2v_gemm_i8_args& g)
+{
+    return s2v_by_dtype(g.c_type, [&](auto type) {
+        using T = decltype(type);
+        const int64_t mt = (g.m + 127) / 128;
+        if (mt * ((g.n + 255) / 256) >= ctx->sm_count) return gi_launch<T, 256>(ctx, st, g);
+        if (mt * ((g.n + 127) / 128) >= ctx->sm_count) return gi_launch<T, 128>(ctx, st, g);
+        return gi_launch<T, 64>(ctx, st, g);
+    });
+}

@@ -1,6 +1,6 @@
-// Dense layers with 8-bit weights: rows to 8-bit integers with a scale each, and the product of two such matrices with the scales,
-// bias and ReLU in its epilogue.
-#include "elem_types.cuh"
+// Dense layers with 8-bit weights: rows to 8-bit integers with a scale each, and the entry points of the
+// product of two such matrices (gemm_i8.cu).
+#include "gemm_i8.cuh"
 
 namespace
 {
@@ -25,48 +25,6 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(int64_t rows, int64_
         const float f = finite && amax >= Q_LEAST ? __fdiv_rn(127.0f, amax) : 0.0f;
         for (int64_t c = lane; c < cols; c += 32) qr[c] = f == 0.0f ? 0 : (int8_t)__float2int_rn(__fmul_rn(to_f32(xr[c]), f));
         if (lane == 0) scale[r] = !finite ? __uint_as_float(0x7fffffffu) : f == 0.0f ? 0.0f : __fdiv_rn(amax, 127.0f);
-    }
-}
-
-// 64 x 64 outputs per CTA, 4 x 4 per thread, panels of 64 bytes along k in shared memory, four products an instruction.
-constexpr int GT = 64, GK = 64;
-template <typename T>
-__global__ void __launch_bounds__(256) gemm_i8_kernel(int64_t m, int64_t n, int64_t k, const int8_t* __restrict__ A, int64_t lda, const float* __restrict__ sa,
-                                                      const int8_t* __restrict__ B, int64_t ldb, const float* __restrict__ sb, const float* __restrict__ bias,
-                                                      int relu, T* __restrict__ C, int64_t ldc)
-{
-    __shared__ int as[GK / 4][GT + 1], bs[GK / 4][GT + 1];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int64_t col0 = (int64_t)blockIdx.x * GT;
-    for (int64_t row0 = (int64_t)blockIdx.y * GT; row0 < m; row0 += (int64_t)gridDim.y * GT) {
-        int acc[4][4] = {};
-        for (int64_t k0 = 0; k0 < k; k0 += GK) {
-            for (int e = threadIdx.x; e < GT * GK / 4; e += 256) {
-                const int r = e / (GK / 4), w = e % (GK / 4);
-                int va = 0, vb = 0;
-                for (int u = 0; u < 4; ++u) {
-                    const int64_t kk = k0 + 4 * w + u;
-                    if (kk < k && row0 + r < m) va |= (int)(uint8_t)A[(row0 + r) * lda + kk] << (8 * u);
-                    if (kk < k && col0 + r < n) vb |= (int)(uint8_t)B[(col0 + r) * ldb + kk] << (8 * u);
-                }
-                as[w][r] = va;
-                bs[w][r] = vb;
-            }
-            __syncthreads();
-            for (int w = 0; w < GK / 4; ++w)
-                for (int i = 0; i < 4; ++i)
-                    for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(as[w][ty + 16 * i], bs[w][tx + 16 * j], acc[i][j]);
-            __syncthreads();
-        }
-        for (int i = 0; i < 4; ++i) {
-            const int64_t r = row0 + ty + 16 * i;
-            for (int j = 0; j < 4; ++j) {
-                const int64_t c = col0 + tx + 16 * j;
-                if (r >= m || c >= n) continue;
-                const float v = fmaf(__fmul_rn(sa[r], sb[c]), (float)acc[i][j], bias ? bias[c] : 0.0f);
-                C[r * ldc + c] = from_f32<T>(relu ? relu_ref(v) : v);
-            }
-        }
     }
 }
 
@@ -126,15 +84,8 @@ int s2v_gemm_i8(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, int64_t k
     if (!a_scale || (k > 0 && !A)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "gemm_i8: NULL pointer");
     if (m > 1 && k > 0 && (lda < k || lda % 16 != 0)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "gemm_i8: lda below k or no multiple of 16");
     if (!s2v_aligned16(A)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "gemm_i8: 8-bit matrices must be 16-byte aligned");
-    cudaStream_t st = s2v_pick_stream(ctx, stream);
-    const int64_t gy = (m + GT - 1) / GT;
-    const dim3 grid((unsigned)((n + GT - 1) / GT), (unsigned)(gy > 65535 ? 65535 : gy));
-    return s2v_by_dtype(c_type, [&](auto type) {
-        using T = decltype(type);
-        gemm_i8_kernel<T><<<grid, 256, 0, st>>>(m, n, k, A, lda, a_scale, B, ldb, b_scale, bias, relu, static_cast<T*>(C), ldc);
-        S2V_CHECK_LAUNCH(ctx, "gemm_i8_kernel");
-        return (int)S2V_OK;
-    });
+    const s2v_gemm_i8_args g{m, n, k, lda, ldb, ldc, A, B, a_scale, b_scale, bias, relu, c_type, C};
+    return s2v_launch_gemm_i8(ctx, s2v_pick_stream(ctx, stream), g);
 }
 
 size_t s2v_linear_i8_workspace_bytes(int64_t m, int64_t k)
