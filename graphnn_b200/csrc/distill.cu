@@ -12,8 +12,7 @@ namespace
 {
 
 constexpr int DT_TOP = 256;            // most entries of a list
-constexpr int DT_THREADS = 256;        // at least DT_TOP: a thread per entry
-constexpr int64_t DT_COLS = 1 << 20;   // a bit per column in shared memory
+constexpr int64_t DT_COLS = 1 << 20;   // most columns
 constexpr int DT_SITE = 7;             // status word: a class outside the row
 
 struct DtArgs {
@@ -31,14 +30,6 @@ struct DtArgs {
     int top, t_type;
 };
 
-struct DtShared {
-    double sum[8];
-    float zk[DT_TOP], mx[8], sm[8];
-    double p[DT_TOP];
-    int idx[DT_TOP];   // -1: no entry
-    int any;
-};
-
 __device__ __forceinline__ float dt_exp2(float x)
 {
     float y;
@@ -47,181 +38,571 @@ __device__ __forceinline__ float dt_exp2(float x)
 }
 __device__ __forceinline__ float dt_finite_or_zero(float m) { return m == -INFINITY ? 0.0f : m; }   // so that a difference from it is no NaN
 
-__device__ __forceinline__ double dt_block_sum(double v, DtShared& s)
+template <typename V> __device__ __forceinline__ V dt_warp_sum(V v)
 {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if (lane == 0) s.sum[warp] = v;
-    __syncthreads();
-    double r = 0.0;
-    for (int w = 0; w < DT_THREADS / 32; ++w) r += s.sum[w];
-    return r;
+    return v;
 }
-__device__ __forceinline__ float dt_block_max(float v, DtShared& s)
+__device__ __forceinline__ float dt_warp_max(float v)
 {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
     for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if (lane == 0) s.mx[warp] = v;
-    __syncthreads();
-    float r = s.mx[0];
-    for (int w = 1; w < DT_THREADS / 32; ++w) r = fmaxf(r, s.mx[w]);
-    return r;
+    return v;
 }
 
-// what follows from a row's two sums
-struct DtRow {
-    double M, out, total, log_s;   // out: exp((M_out - M) / T)
-    __device__ __forceinline__ DtRow(float m_in, double s_in, float m_out, double s_out, float temperature)
+// ---------------------------------------------------------------- the list
+// What a row's list adds up to, over any part of its entries; P_k = exp((t_k - t_max) / T), or exp(t_k / T - t_lse) where that is given:
+//     Z = sum P,  A = sum P log P,  B = sum P (z_idx - m) / T,  s = sum of exp((z_idx - m) / T) over the columns,  m = the largest z_idx
+struct DtList {
+    double Z, A, B, s;
+    float m;
+};
+__device__ __forceinline__ int dt_load_id(const DtArgs& a, int64_t r, int k)
+{
+    const int id = k < a.top ? __ldg(a.idx + r * a.ldt + k) : -1;
+    if (id < a.cols) return id < 0 ? -1 : id;
+    a.status->code = S2V_ERR_INVALID_ARG;
+    a.status->where = DT_SITE;
+    return -1;
+}
+__device__ __forceinline__ float dt_load_t(const DtArgs& a, int64_t r, int k)
+{
+    const int64_t at = r * a.ldt + k;
+    return a.t_type == S2V_F32 ? __ldg(static_cast<const float*>(a.t) + at) : a.t_type == S2V_F16 ? to_f32(static_cast<const __half*>(a.t)[at])
+                                                                                                   : to_f32(static_cast<const __nv_bfloat16*>(a.t)[at]);
+}
+// log P of an entry
+__device__ __forceinline__ double dt_log_p(const DtArgs& a, float tv, float tmax, double t_lse, double inv_t)
+{
+    return a.t_lse ? (double)tv * inv_t - t_lse : ((double)tv - (double)dt_finite_or_zero(tmax)) * inv_t;
+}
+
+// ---------------------------------------------------------------- a row, once its sums are known
+struct DtCoef {
+    float M;            // the larger maximum (0 where there is none)
+    float given, rest;  // sum p, 1 - sum p; p = P * p_scale
+    float p_scale;
+    float inner;        // a listed column's gradient: inner * exp((z - M) / T) - scale * p
+    float outer;        // any other's: outer * exp((z - m_out) / T)
+    float scale;        // row_weight / T
+};
+__device__ __forceinline__ DtCoef dt_coefficients(const DtArgs& a, double Z, float m_in, float s_in, float m_out, float s_out, float weight, float c)
+{
+    DtCoef k;
+    const float m = fmaxf(m_in, m_out);
+    k.M = dt_finite_or_zero(m);
+    const float e_out = s_out == 0.0f ? 0.0f : dt_exp2((m_out - k.M) * c), e_in = s_in == 0.0f ? 0.0f : dt_exp2((m_in - k.M) * c);
+    const float total = m == -INFINITY ? NAN : s_in * e_in + s_out * e_out;
+    if (a.t_lse) {
+        k.given = (float)Z;
+        k.rest = Z > 1.0 ? 0.0f : (float)(1.0 - Z);
+        k.p_scale = 1.0f;
+    } else {
+        k.given = (float)(Z - Z + 1.0);   // one, and NaN where the list holds NaN or +infinity
+        k.rest = 0.0f;
+        k.p_scale = (float)(1.0 / Z);
+    }
+    k.scale = weight / a.temperature;
+    const float both = __fdividef(k.given + k.rest, total);
+    k.inner = k.scale * both;
+    k.outer = k.scale * (s_out == 0.0f && total == total ? 0.0f : both * e_out - __fdividef(k.rest, s_out));
+    return k;
+}
+__device__ __forceinline__ float dt_loss(const DtArgs& a, const DtList& l, float m_out, double s_out, float weight, double inv_t)
+{
+    const float mf = fmaxf(l.m, m_out);
+    if (mf == -INFINITY) return NAN;
+    const double M = (double)mf;
+    const double total = (l.s == 0.0 ? 0.0 : l.s * exp(((double)l.m - M) * inv_t)) + (s_out == 0.0 ? 0.0 : s_out * exp(((double)m_out - M) * inv_t));
+    const double lse = log(total);   // above M / T
+    // sum of p (log p - log q), log q = (z - M) / T - lse; B is relative to l.m
+    const double from = l.m == -INFINITY ? 0.0 : ((double)l.m - M) * inv_t;
+    double kl, rest = 0.0;
+    if (a.t_lse) {
+        kl = l.A - (l.B + l.Z * from) + l.Z * lse;
+        rest = l.Z > 1.0 ? 0.0 : 1.0 - l.Z;
+    } else {
+        kl = (l.A - (l.B + l.Z * from)) / l.Z - log(l.Z) + lse;
+    }
+    if (rest != 0.0) {
+        if (s_out != 0.0) {
+            const double d = l.s == 0.0 ? -INFINITY : log(l.s / s_out) + ((double)l.m - (double)m_out) * inv_t;
+            kl += rest * (log1p(-l.Z) + (d > 0.0 ? d + log1p(exp(-d)) : log1p(exp(d))));
+        } else if (rest > 1.0 / 65536.0) {
+            kl = INFINITY;
+        }
+    }
+    return (float)(kl * weight);
+}
+
+// ---------------------------------------------------------------- pieces of 16 bytes
+template <typename T> constexpr int DT_PER = 16 / (int)sizeof(T);
+
+__device__ __forceinline__ void dt_unpack(const uint4& v, float* x, float)
+{
+    x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
+}
+__device__ __forceinline__ void dt_unpack(const uint4& v, float* x, __half)
+{
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void dt_unpack(const uint4& v, float* x, __nv_bfloat16)
+{
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+__device__ __forceinline__ uint4 dt_pack(const float* y, float) { return make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])); }
+template <typename T> __device__ __forceinline__ uint4 dt_pack(const float* y, T)
+{
+    return make_uint4(pack_16bit<T>(y[0], y[1]), pack_16bit<T>(y[2], y[3]), pack_16bit<T>(y[4], y[5]), pack_16bit<T>(y[6], y[7]));
+}
+
+// A row's columns: `head` in front of the first 16-byte boundary, `pieces` of 16 bytes, `tail` behind them.
+template <typename T> struct DtRowShape {
+    int head, pieces, tail;
+    __device__ __forceinline__ DtRowShape(const T* z, int64_t cols)
     {
-        M = (double)fmaxf(m_in, m_out);
-        out = s_out == 0.0 ? 0.0 : exp(((double)m_out - M) / temperature);
-        total = M == -INFINITY ? NAN : (s_in == 0.0 ? 0.0 : s_in * exp(((double)m_in - M) / temperature)) + s_out * out;
-        const double d = s_in == 0.0 ? -INFINITY : log(s_in / s_out) + ((double)m_in - (double)m_out) / temperature;
-        log_s = d > 0.0 ? -d - log1p(exp(-d)) : -log1p(exp(d));
+        const int off = (int)((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / (int)sizeof(T);
+        head = off < cols ? off : (int)cols;
+        pieces = (int)((cols - head) / DT_PER<T>);
+        tail = (int)(cols - head) - pieces * DT_PER<T>;
     }
 };
 
-// A CTA per row.
-template <typename T, bool GRAD_ONLY>
-__global__ void __launch_bounds__(DT_THREADS) distill_rows_kernel(const DtArgs a)
+struct DtSum {   // of exp((z - m) / T), relative to the largest z
+    float m, s;
+    template <int N> __device__ __forceinline__ void add(const float* x, uint32_t listed, float c)
+    {
+        float top = m;
+#pragma unroll
+        for (int e = 0; e < N; ++e) top = fmaxf(top, listed >> e & 1 ? -INFINITY : x[e]);
+        if (top > m) {
+            s *= dt_exp2((m - top) * c);   // (m = -infinity: no sum yet)
+            m = top;
+        }
+        const float base = dt_finite_or_zero(m);
+        float part = 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) part += listed >> e & 1 ? 0.0f : dt_exp2((x[e] - base) * c);
+        s += part;
+    }
+    __device__ __forceinline__ void join(float om, float os, float c)
+    {
+        const float top = fmaxf(m, om), base = dt_finite_or_zero(top);
+        s = s * dt_exp2((m - base) * c) + os * dt_exp2((om - base) * c);
+        m = top;
+    }
+    __device__ __forceinline__ void join_warp(float c)
+    {
+        const float top = dt_warp_max(m);
+        s = dt_warp_sum(s * dt_exp2((m - dt_finite_or_zero(top)) * c));
+        m = top;
+    }
+};
+
+// zeros in the columns of a row that falls to this thread, one of `threads`
+template <typename T> __device__ __forceinline__ void dt_zero_row(T* dz, int64_t cols, int at, int threads)
 {
-    extern __shared__ uint32_t listed[];   // a bit per column: whether an entry names it
-    __shared__ DtShared s;
-    const int tid = threadIdx.x;
-    const float c = 1.4426950408889634f / a.temperature;
-    for (int64_t w = tid; w < (a.cols + 31) / 32; w += DT_THREADS) listed[w] = 0;
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const T* const z = static_cast<const T*>(a.z) + r * a.ldz;
-        T* const dz = a.dz ? static_cast<T*>(a.dz) + r * a.lddz : nullptr;
-        const float weight = a.row_weight ? a.row_weight[r] : 1.0f;
-        // the list: entries, p, their sum
-        int id = -1;
-        float tv = -INFINITY;
-        if (tid < a.top) {
-            id = a.idx[r * a.ldt + tid];
-            if (id >= a.cols) {
-                a.status->code = S2V_ERR_INVALID_ARG;
-                a.status->where = DT_SITE;
-                id = -1;
-            }
-            const int64_t at = r * a.ldt + tid;
-            if (id >= 0)
-                tv = a.t_type == S2V_F32 ? static_cast<const float*>(a.t)[at] : a.t_type == S2V_F16 ? to_f32(static_cast<const __half*>(a.t)[at])
-                                                                                                   : to_f32(static_cast<const __nv_bfloat16*>(a.t)[at]);
-        }
-        const bool some = __syncthreads_or(id >= 0);
-        const float tmax = dt_block_max(tv, s);
-        double p = 0.0, given, rest = 0.0;
-        if (a.t_lse) {
-            if (id >= 0) p = exp((double)tv / a.temperature - (double)a.t_lse[r]);
-            given = dt_block_sum(p, s);
-            rest = given > 1.0 ? 0.0 : 1.0 - given;
-        } else {
-            if (id >= 0) p = exp(((double)tv - (double)dt_finite_or_zero(tmax)) / a.temperature);
-            const double total = dt_block_sum(p, s);
-            p /= total;
-            given = total - total + 1.0;   // one, and NaN where the list holds NaN or +infinity
-        }
-        const bool skip = !some || (!a.t_lse && tmax == -INFINITY);
-        if (skip || (weight == 0.0f && !a.stats) || (GRAD_ONLY && weight == 0.0f)) {   // (the same for the whole CTA)
-            if (!GRAD_ONLY && tid == 0) a.loss[r] = 0.0f;
-            if (!GRAD_ONLY && a.stats && tid < 4) a.stats[4 * r + tid] = 0.0f;
-            if (dz)
-                for (int64_t j = tid; j < a.cols; j += DT_THREADS) dz[j] = from_f32<T>(0.0f);
-            __syncthreads();
-            continue;
-        }
-        __syncthreads();
-        if (tid < a.top) {
-            s.idx[tid] = id;
-            s.p[tid] = p;
-            if (id >= 0) atomicOr(&listed[id >> 5], 1u << (id & 31));
-        }
-        const float zk = id >= 0 ? to_f32(z[id]) : -INFINITY;
-        __syncthreads();
-        // the first entry of a column stands for it; p of all its entries
-        bool first = id >= 0;
-        double p_all = 0.0;
-        if (id >= 0)
-            for (int k = 0; k < a.top; ++k)
-                if (s.idx[k] == id) {
-                    p_all += s.p[k];
-                    if (k < tid) first = false;
-                }
-        float m_in, m_out;
-        double s_in, s_out;
-        if constexpr (GRAD_ONLY) {
-            m_out = a.stats[4 * r], s_out = (double)a.stats[4 * r + 1];
-            m_in = a.stats[4 * r + 2], s_in = (double)a.stats[4 * r + 3];
-        } else {
-            float m = -INFINITY, sum = 0.0f;
-            for (int64_t j = tid; j < a.cols; j += DT_THREADS) {
-                if (listed[j >> 5] >> (j & 31) & 1) continue;
-                const float v = to_f32(z[j]);
-                if (v > m) {
-                    sum *= dt_exp2((m - v) * c);   // (m = -infinity: no sum yet)
-                    m = v;
-                }
-                sum += dt_exp2((v - dt_finite_or_zero(m)) * c);
-            }
-            m_out = dt_block_max(m, s);
-            s_out = dt_block_sum((double)(sum * dt_exp2((m - dt_finite_or_zero(m_out)) * c)), s);
-            m_in = dt_block_max(zk, s);
-            s_in = dt_block_sum(first ? exp(((double)zk - (double)dt_finite_or_zero(m_in)) / a.temperature) : 0.0, s);
-        }
-        const DtRow row(m_in, s_in, m_out, s_out, a.temperature);
-        if constexpr (!GRAD_ONLY) {
-            double kl = 0.0;
-            if (id >= 0 && p != 0.0) kl = p * (log(p) - (((double)zk - row.M) / a.temperature - log(row.total)));
-            kl = dt_block_sum(kl, s);
-            if (rest != 0.0) {
-                if (s_out != 0.0) kl += rest * (log1p(-given) - row.log_s);
-                else if (rest > 1.0 / 65536.0) kl = INFINITY;
-            }
-            if (!(row.total > 0.0)) kl = NAN;
-            if (tid == 0) {
-                a.loss[r] = weight == 0.0f ? 0.0f : (float)(kl * weight);
-                if (a.stats) *reinterpret_cast<float4*>(a.stats + 4 * r) = make_float4(m_out, (float)s_out, m_in, (float)s_in);
-            }
-        }
-        if (dz) {
-            const double scale = (double)weight / a.temperature;
-            const float out = weight == 0.0f ? 0.0f : !(row.total > 0.0) ? NAN : s_out == 0.0 ? 0.0f : (float)(scale * ((given + rest) * row.out / row.total - rest / s_out));
-            const float base = dt_finite_or_zero(m_out);
-            __syncthreads();   // every listed z has been read
-            for (int64_t j = tid; j < a.cols; j += DT_THREADS) {
-                if (listed[j >> 5] >> (j & 31) & 1) continue;
-                dz[j] = from_f32<T>(out == 0.0f ? 0.0f : dt_exp2((to_f32(z[j]) - base) * c) * out);
-            }
-            if (first) dz[id] = from_f32<T>(weight == 0.0f ? 0.0f : (float)(scale * ((given + rest) * exp(((double)zk - row.M) / a.temperature) / row.total - p_all)));
-        }
-        __syncthreads();
-        if (id >= 0) listed[id >> 5] = 0;   // (a word, by all its entries)
-        __syncthreads();
+    const DtRowShape<T> row(dz, cols);
+    if (at < row.head) dz[at] = from_f32<T>(0.0f);
+    if (at < row.tail) dz[cols - 1 - at] = from_f32<T>(0.0f);
+    uint4* const to = reinterpret_cast<uint4*>(dz + row.head);
+    for (int p = at; p < row.pieces; p += threads) to[p] = make_uint4(0, 0, 0, 0);
+}
+
+// gradient of a piece; listed columns are written by their entries
+template <typename T> __device__ __forceinline__ void dt_store(T* to, bool whole, const uint4& v, uint32_t listed, float base, float outer, float c)
+{
+    constexpr int N = DT_PER<T>;
+    float x[N];
+    dt_unpack(v, x, T());
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = outer == 0.0f ? 0.0f : dt_exp2((x[e] - base) * c) * outer;
+    if (whole && listed == 0) {
+        __stcs(reinterpret_cast<uint4*>(to), dt_pack(x, T()));
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (!(listed >> e & 1)) to[e] = from_f32<T>(x[e]);
     }
 }
 
+// ---------------------------------------------------------------- rows of up to 256 pieces: a warp each
+// The row stays in registers between the sums and the gradient.
+constexpr int DW_WARPS = 4, DW_PIECES = 8;   // pieces a lane
+struct DwShared {
+    double P[DT_TOP];
+    int id[DT_TOP];
+    float z[DT_TOP];
+    uint32_t mask[(DW_PIECES * 32 + 4 + 31) / 32 * 8 + 1];   // a byte per piece, then one for the head and one for the tail
+};
+
+template <typename T, int NV, bool GRAD_ONLY>
+__global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArgs a)
+{
+    __shared__ DwShared shared[DW_WARPS];
+    DwShared& s = shared[threadIdx.x >> 5];
+    constexpr int N = DT_PER<T>, EDGE = DW_PIECES * 32;   // mask bytes of the head and the tail: EDGE, EDGE + 1
+    const int lane = threadIdx.x & 31;
+    const double inv_t = 1.0 / (double)a.temperature;
+    const float c = 1.4426950408889634f / a.temperature;
+    const uint8_t* const mask = reinterpret_cast<const uint8_t*>(s.mask);
+    for (int w = lane; w < (int)(sizeof(s.mask) / 4); w += 32) s.mask[w] = 0;
+    __syncwarp();
+    const int64_t step = (int64_t)gridDim.x * DW_WARPS;
+    for (int64_t r = (int64_t)blockIdx.x * DW_WARPS + (threadIdx.x >> 5); r < a.rows; r += step) {
+        const T* const z = static_cast<const T*>(a.z) + r * a.ldz;
+        T* const dz = a.dz ? static_cast<T*>(a.dz) + r * a.lddz : nullptr;
+        const float weight = a.row_weight ? __ldg(a.row_weight + r) : 1.0f;
+        const DtRowShape<T> row(z, a.cols);
+        float tmax = -INFINITY;
+        bool some = false;
+        for (int k = lane; k < a.top; k += 32) {
+            const int id = dt_load_id(a, r, k);
+            s.id[k] = id;
+            if (id < 0) continue;
+            some = true;
+            tmax = fmaxf(tmax, dt_load_t(a, r, k));
+        }
+        some = __any_sync(0xffffffffu, some);
+        tmax = dt_warp_max(tmax);
+        if (!some || (!a.t_lse && tmax == -INFINITY) || (weight == 0.0f && (GRAD_ONLY || !a.stats))) {
+            if (!GRAD_ONLY && lane == 0) a.loss[r] = 0.0f;
+            if (!GRAD_ONLY && a.stats && lane < 4) a.stats[4 * r + lane] = 0.0f;
+            if (dz) dt_zero_row(dz, a.cols, lane, 32);
+            __syncwarp();
+            continue;
+        }
+        uint4 v[NV];
+        const uint4* const zp = reinterpret_cast<const uint4*>(z + row.head);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * 32 + lane < row.pieces) v[j] = zp[j * 32 + lane];
+        // the scalar columns: the head's to the first lanes, the tail's to the last
+        const bool in_head = lane < row.head, in_tail = lane >= 32 - row.tail;
+        const int edge_at = in_head ? lane : (int)a.cols - 32 + lane, edge_bit = in_head ? lane : lane - (32 - row.tail);
+        float edge = in_head || in_tail ? to_f32(z[edge_at]) : -INFINITY;
+        // the list
+        const double t_lse = a.t_lse ? (double)__ldg(a.t_lse + r) : 0.0;
+        DtList l{0.0, 0.0, 0.0, 0.0, -INFINITY};
+        bool twice = false;
+        for (int k = lane; k < a.top; k += 32) {
+            const int id = s.id[k];
+            if (id < 0) continue;
+            const float zk = to_f32(z[id]);
+            const double lp = dt_log_p(a, dt_load_t(a, r, k), tmax, t_lse, inv_t), P = exp(lp);
+            s.z[k] = zk;
+            s.P[k] = P;
+            l.Z += P;
+            if (P != 0.0) l.A += P * lp;
+            l.m = fmaxf(l.m, zk);
+            const int at = id - row.head, byte = at < 0 ? EDGE : at >= row.pieces * N ? EDGE + 1 : at / N, bit = at < 0 ? id : at >= row.pieces * N ? at - row.pieces * N : at % N;
+            const uint32_t b = 1u << (8 * (byte & 3) + bit);
+            twice |= (atomicOr(&s.mask[byte >> 2], b) & b) != 0;
+        }
+        twice = __any_sync(0xffffffffu, twice);
+        __syncwarp();
+        l.Z = dt_warp_sum(l.Z);
+        l.A = dt_warp_sum(l.A);
+        l.m = dt_warp_max(l.m);
+        const auto first = [&](int k, double* all) {   // whether entry k is the first of its column; P of all the column's entries
+            *all = s.P[k];
+            if (!twice) return true;
+            bool f = true;
+            double sum = 0.0;
+            for (int i = 0; i < a.top; ++i)
+                if (s.id[i] == s.id[k]) {
+                    sum += s.P[i];
+                    if (i < k) f = false;
+                }
+            *all = sum;
+            return f;
+        };
+        DtSum d{-INFINITY, 0.0f};
+        uint32_t edge_listed = in_head || in_tail ? mask[in_head ? EDGE : EDGE + 1] >> edge_bit & 1u : 1u;
+        if constexpr (GRAD_ONLY) {
+            const float4 st = __ldg(reinterpret_cast<const float4*>(a.stats) + r);
+            d.m = st.x, d.s = st.y, l.m = st.z, l.s = (double)st.w;
+        } else {
+            for (int k = lane; k < a.top; k += 32) {
+                if (s.id[k] < 0) continue;
+                const double x = ((double)s.z[k] - (double)dt_finite_or_zero(l.m)) * inv_t;
+                double all;
+                if (first(k, &all)) l.s += exp(x);
+                if (s.P[k] != 0.0) l.B += s.P[k] * x;
+            }
+            l.B = dt_warp_sum(l.B);
+            l.s = dt_warp_sum(l.s);
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (j * 32 + lane < row.pieces) {
+                    float x[N];
+                    dt_unpack(v[j], x, T());
+                    d.template add<N>(x, mask[j * 32 + lane], c);
+                }
+            if (in_head || in_tail) d.template add<1>(&edge, edge_listed, c);
+            d.join_warp(c);
+            if (a.stats && lane == 0) reinterpret_cast<float4*>(a.stats)[r] = make_float4(d.m, d.s, l.m, (float)l.s);
+            const float loss = dt_loss(a, l, d.m, (double)d.s, weight, inv_t);
+            if (lane == 0) a.loss[r] = weight == 0.0f ? 0.0f : loss;
+        }
+        if (dz) {
+            const DtCoef k = dt_coefficients(a, l.Z, l.m, (float)l.s, d.m, d.s, weight, c);
+            const float outer = weight == 0.0f ? 0.0f : k.outer, base = dt_finite_or_zero(d.m);
+            T* const dp = dz + row.head;
+            const bool whole = (reinterpret_cast<uintptr_t>(dp) & 15) == 0;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (j * 32 + lane < row.pieces) dt_store(dp + (j * 32 + lane) * N, whole, v[j], mask[j * 32 + lane], base, outer, c);
+            if (!edge_listed) dz[edge_at] = from_f32<T>(outer == 0.0f ? 0.0f : dt_exp2((edge - base) * c) * outer);
+            for (int i = lane; i < a.top; i += 32) {
+                double all;
+                if (s.id[i] >= 0 && first(i, &all))
+                    dz[s.id[i]] = from_f32<T>(weight == 0.0f ? 0.0f : k.inner * expf((s.z[i] - k.M) / a.temperature) - k.scale * ((float)all * k.p_scale));
+            }
+        }
+        __syncwarp();
+        for (int k = lane; k < a.top; k += 32)
+            if (s.id[k] >= 0) {
+                const int at = s.id[k] - row.head, byte = at < 0 ? EDGE : at >= row.pieces * N ? EDGE + 1 : at / N;
+                s.mask[byte >> 2] = 0;
+            }
+        __syncwarp();
+    }
+}
+
+// ---------------------------------------------------------------- longer rows: a cluster of CTAs each
+// Every CTA has an equal run of the row's pieces: the first NV of each thread stay in registers between the sums and the gradient, what a very
+// long row has more is read again.  All CTAs work through the list (a thread an entry), each counts and writes the listed columns of its own run.
+constexpr int DC_THREADS = 512, DC_WARPS = DC_THREADS / 32, DC_LISTERS = DT_TOP / 32, DC_CTAS = 8;
+struct DcShared {
+    double P[DT_TOP];
+    double Z[DC_LISTERS], A[DC_LISTERS], B[DC_LISTERS], s_in[DC_LISTERS];
+    float4 peer[2][DC_CTAS];            // m_out, s_out, s_in of the cluster's CTAs, two rows by turns
+    float2 sum[DC_WARPS];               // dense sums of the warps
+    float tmax[DC_LISTERS], zmax[DC_LISTERS];
+    int id[DT_TOP];
+    uint32_t edge;                      // listed columns of the head (bits 0 to 7) and the tail (8 to 15)
+};
+
+template <typename T, int NV, bool GRAD_ONLY>
+__global__ void __launch_bounds__(DC_THREADS, 2) distill_cluster_kernel(const DtArgs a, int ctas)
+{
+    extern __shared__ uint32_t dc_mask[];   // a byte per piece of this CTA
+    __shared__ DcShared s;
+    constexpr int N = DT_PER<T>;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = (int)(blockIdx.x % (unsigned)ctas);
+    const double inv_t = 1.0 / (double)a.temperature;
+    const float c = 1.4426950408889634f / a.temperature;
+    const uint8_t* const mask = reinterpret_cast<const uint8_t*>(dc_mask);
+    const int most = (int)((a.cols / N + ctas - 1) / ctas);   // pieces of a CTA, at most
+    for (int w = tid; w < (most + 3) / 4; w += DC_THREADS) dc_mask[w] = 0;
+    if (tid == 0) s.edge = 0;
+    int turn = 0;
+    for (int64_t r = blockIdx.x / (unsigned)ctas; r < a.rows; r += gridDim.x / (unsigned)ctas) {
+        const T* const z = static_cast<const T*>(a.z) + r * a.ldz;
+        T* const dz = a.dz ? static_cast<T*>(a.dz) + r * a.lddz : nullptr;
+        const float weight = a.row_weight ? __ldg(a.row_weight + r) : 1.0f;
+        const DtRowShape<T> row(z, a.cols);
+        const int first_piece = rank * most, pieces = max(0, min(most, row.pieces - first_piece));
+        const uint4* const zp = reinterpret_cast<const uint4*>(z + row.head) + first_piece;
+        const int id = dt_load_id(a, r, tid);
+        const float tv = id >= 0 ? dt_load_t(a, r, tid) : -INFINITY;
+        const bool skip_weight = weight == 0.0f && (GRAD_ONLY || !a.stats);
+        uint4 v[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * DC_THREADS + tid < pieces && !skip_weight) v[j] = zp[j * DC_THREADS + tid];
+        if (warp < DC_LISTERS) {
+            const float m = dt_warp_max(tv);
+            if (lane == 0) s.tmax[warp] = m;
+        }
+        const bool some = __syncthreads_or(id >= 0);
+        float tmax = s.tmax[0];
+#pragma unroll
+        for (int w = 1; w < DC_LISTERS; ++w) tmax = fmaxf(tmax, s.tmax[w]);
+        if (!some || (!a.t_lse && tmax == -INFINITY) || skip_weight) {   // (the same for all CTAs of the row)
+            if (!GRAD_ONLY && rank == 0) {
+                if (tid == 0) a.loss[r] = 0.0f;
+                if (a.stats && tid < 4) a.stats[4 * r + tid] = 0.0f;
+            }
+            if (dz) dt_zero_row(dz, a.cols, rank * DC_THREADS + tid, ctas * DC_THREADS);
+            __syncthreads();
+            continue;
+        }
+        // the list: a thread an entry
+        const int at = id - row.head, piece = at < 0 ? -1 : at / N - first_piece;   // (of this CTA's)
+        const bool edge_entry = id >= 0 && (at < 0 || at >= row.pieces * N);
+        const bool mine = edge_entry ? rank == (at < 0 ? 0 : ctas - 1) : id >= 0 && piece >= 0 && piece < pieces;
+        uint32_t* const word = edge_entry ? &s.edge : &dc_mask[mine ? piece >> 2 : 0];
+        float zk = -INFINITY;
+        double P = 0.0, lp = 0.0;
+        bool twice = false;
+        if (warp < DC_LISTERS) {
+            if (id >= 0) {
+                if (mine || !GRAD_ONLY) zk = to_f32(z[id]);
+                lp = dt_log_p(a, tv, tmax, a.t_lse ? (double)__ldg(a.t_lse + r) : 0.0, inv_t);
+                P = exp(lp);
+            }
+            s.id[tid] = id;
+            s.P[tid] = P;
+            if (mine) {
+                const uint32_t b = 1u << (!edge_entry ? 8 * (piece & 3) + at % N : at < 0 ? id : 8 + at - row.pieces * N);
+                twice = (atomicOr(word, b) & b) != 0;
+            }
+            const float m = dt_warp_max(zk);
+            if (lane == 0) s.zmax[warp] = m;
+        }
+        bool first = mine;   // the first entry of its column; P of all the column's entries
+        double P_all = P;
+        if (__syncthreads_or(twice) && mine) {
+            P_all = 0.0;
+            for (int k = 0; k < a.top; ++k)
+                if (s.id[k] == id) {
+                    P_all += s.P[k];
+                    if (k < tid) first = false;
+                }
+        }
+        float m_in = s.zmax[0];
+#pragma unroll
+        for (int w = 1; w < DC_LISTERS; ++w) m_in = fmaxf(m_in, s.zmax[w]);
+        if (warp < DC_LISTERS) {
+            const double x = ((double)zk - (double)dt_finite_or_zero(m_in)) * inv_t;
+            const double Z = dt_warp_sum(P);
+            if (lane == 0) s.Z[warp] = Z;
+            if constexpr (!GRAD_ONLY) {
+                const double A = dt_warp_sum(P != 0.0 ? P * lp : 0.0), B = dt_warp_sum(P != 0.0 ? P * x : 0.0), s_in = dt_warp_sum(first ? exp(x) : 0.0);
+                if (lane == 0) s.A[warp] = A, s.B[warp] = B, s.s_in[warp] = s_in;
+            }
+        }
+        // the scalar columns: the head's to the first CTA, the tail's to the last
+        const bool in_head = rank == 0 && tid < row.head, in_tail = rank == ctas - 1 && tid >= 32 && tid < 32 + row.tail;
+        const int edge_at = in_head ? tid : (int)a.cols - row.tail + tid - 32;
+        const float edge = in_head || in_tail ? to_f32(z[edge_at]) : -INFINITY;
+        const uint32_t edge_listed = in_head ? s.edge >> tid & 1u : in_tail ? s.edge >> (8 + tid - 32) & 1u : 1u;
+        DtSum d{-INFINITY, 0.0f};
+        float s_in;
+        if constexpr (GRAD_ONLY) {
+            const float4 st = __ldg(reinterpret_cast<const float4*>(a.stats) + r);
+            d.m = st.x, d.s = st.y, m_in = st.z, s_in = st.w;
+            __syncthreads();
+        } else {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (j * DC_THREADS + tid < pieces) {
+                    float x[N];
+                    dt_unpack(v[j], x, T());
+                    d.template add<N>(x, mask[j * DC_THREADS + tid], c);
+                }
+            for (int p = NV * DC_THREADS + tid; p < pieces; p += DC_THREADS) {
+                float x[N];
+                dt_unpack(zp[p], x, T());
+                d.template add<N>(x, mask[p], c);
+            }
+            if (in_head || in_tail) d.template add<1>(&edge, edge_listed, c);
+            d.join_warp(c);
+            if (lane == 0) s.sum[warp] = make_float2(d.m, d.s);
+            __syncthreads();
+            // (every warp joins the warps' sums for itself)
+            d = lane < DC_WARPS ? DtSum{s.sum[lane].x, s.sum[lane].y} : DtSum{-INFINITY, 0.0f};
+            d.join_warp(c);
+            s_in = (float)dt_warp_sum(lane < DC_LISTERS ? s.s_in[lane] : 0.0);
+            if (ctas > 1) {
+                if (warp == 0 && lane < ctas) {
+                    uint32_t to;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&s.peer[turn][rank])), "r"(lane));
+                    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %3};" ::"r"(to), "f"(d.m), "f"(d.s), "f"(s_in) : "memory");
+                }
+                asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+                const float4 o = lane < ctas ? s.peer[turn][lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+                d = DtSum{o.x, o.y};
+                d.join_warp(c);
+                s_in = dt_warp_sum(o.z);
+                turn ^= 1;
+            }
+        }
+        const double Z = dt_warp_sum(lane < DC_LISTERS ? s.Z[lane] : 0.0);
+        if (!GRAD_ONLY && rank == 0 && warp == DC_WARPS - 1) {
+            const DtList l{Z, dt_warp_sum(lane < DC_LISTERS ? s.A[lane] : 0.0), dt_warp_sum(lane < DC_LISTERS ? s.B[lane] : 0.0), (double)s_in, m_in};
+            const float loss = dt_loss(a, l, d.m, (double)d.s, weight, inv_t);
+            if (lane == 0) {
+                a.loss[r] = weight == 0.0f ? 0.0f : loss;
+                if (a.stats) reinterpret_cast<float4*>(a.stats)[r] = make_float4(d.m, d.s, m_in, s_in);
+            }
+        }
+        if (dz) {
+            const DtCoef k = dt_coefficients(a, Z, m_in, s_in, d.m, d.s, weight, c);
+            const float outer = weight == 0.0f ? 0.0f : k.outer, base = dt_finite_or_zero(d.m);
+            T* const dp = dz + row.head + (int64_t)first_piece * N;
+            const bool whole = (reinterpret_cast<uintptr_t>(dp) & 15) == 0;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (j * DC_THREADS + tid < pieces) dt_store(dp + (j * DC_THREADS + tid) * N, whole, v[j], mask[j * DC_THREADS + tid], base, outer, c);
+            for (int p = NV * DC_THREADS + tid; p < pieces; p += DC_THREADS) dt_store(dp + (int64_t)p * N, whole, zp[p], mask[p], base, outer, c);
+            if (!edge_listed) dz[edge_at] = from_f32<T>(outer == 0.0f ? 0.0f : dt_exp2((edge - base) * c) * outer);
+            if (first) dz[id] = from_f32<T>(weight == 0.0f ? 0.0f : k.inner * expf((zk - k.M) / a.temperature) - k.scale * ((float)P_all * k.p_scale));
+        }
+        __syncthreads();
+        if (mine) *word = 0;   // (a whole word, by each of its entries)
+    }
+}
+
+template <typename T, int NV, bool GRAD_ONLY> int dc_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a, int ctas)
+{
+    const int64_t most = (a.cols / DT_PER<T> + ctas - 1) / ctas;
+    int64_t rows = a.rows;
+    if (rows > (1 << 20)) rows = 1 << 20;   // (clusters; further rows in turns)
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * ctas));
+    cfg.blockDim = dim3(DC_THREADS);
+    cfg.dynamicSmemBytes = (size_t)((most + 3) / 4 * 4);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = GRAD_ONLY ? 0 : 1;
+    S2V_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, distill_cluster_kernel<T, NV, GRAD_ONLY>, a, ctas));
+    S2V_CHECK_LAUNCH(ctx, "distill_cluster_kernel");
+    return S2V_OK;
+}
+template <typename T, int NV, bool GRAD_ONLY> int dw_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a)
+{
+    int64_t blocks = (a.rows + DW_WARPS - 1) / DW_WARPS;
+    const int64_t cap = (int64_t)ctx->sm_count * 16;
+    if (blocks > cap) blocks = cap;
+    distill_warp_kernel<T, NV, GRAD_ONLY><<<(unsigned)blocks, 32 * DW_WARPS, 0, st>>>(a);
+    S2V_CHECK_LAUNCH(ctx, "distill_warp_kernel");
+    return S2V_OK;
+}
+
+template <typename T, bool GRAD_ONLY> int dt_launch_type(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a)
+{
+    const int64_t pieces = a.cols / DT_PER<T>;
+    if (pieces <= 32) return dw_launch<T, 1, GRAD_ONLY>(ctx, st, a);
+    if (pieces <= 32 * DW_PIECES) return dw_launch<T, DW_PIECES, GRAD_ONLY>(ctx, st, a);
+    int ctas = 1;
+    while (ctas < DC_CTAS && (pieces > (int64_t)ctas * 8 * DC_THREADS || (a.rows * ctas < 2 * ctx->sm_count && pieces >= (int64_t)ctas * 2 * DC_THREADS))) ctas *= 2;
+    const int64_t most = (pieces + ctas - 1) / ctas;
+    if (most <= 2 * DC_THREADS) return dc_launch<T, 2, GRAD_ONLY>(ctx, st, a, ctas);
+    if (most <= 4 * DC_THREADS) return dc_launch<T, 4, GRAD_ONLY>(ctx, st, a, ctas);
+    return dc_launch<T, 8, GRAD_ONLY>(ctx, st, a, ctas);
+}
 int dt_launch(s2v_ctx* ctx, s2v_stream stream, int z_type, bool grad_only, const DtArgs& a)
 {
     cudaStream_t st = s2v_pick_stream(ctx, stream);
-    const size_t bits = (size_t)((a.cols + 31) / 32) * 4;
-    const int64_t cap = (int64_t)ctx->sm_count * 8;
-    const unsigned grid = (unsigned)(a.rows < cap ? a.rows : cap);
     return s2v_by_dtype(z_type, [&](auto type) {
         using T = decltype(type);
-        if (grad_only) {
-            S2V_CUDA_OK(ctx, s2v_allow_shared(distill_rows_kernel<T, true>, DT_COLS / 8));
-            distill_rows_kernel<T, true><<<grid, DT_THREADS, bits, st>>>(a);
-        } else {
-            S2V_CUDA_OK(ctx, s2v_allow_shared(distill_rows_kernel<T, false>, DT_COLS / 8));
-            distill_rows_kernel<T, false><<<grid, DT_THREADS, bits, st>>>(a);
-        }
-        S2V_CHECK_LAUNCH(ctx, "distill_rows_kernel");
-        return (int)S2V_OK;
+        return grad_only ? dt_launch_type<T, true>(ctx, st, a) : dt_launch_type<T, false>(ctx, st, a);
     });
 }
 

@@ -4,7 +4,6 @@
 // outside the matrices) into a ring, one issues the products, eight take finished accumulators out of tensor memory, of which there are two, so
 // that a tile's outputs are written under the next tile's products.
 #include <cstring>
-#include <type_traits>
 
 #include "gemm_i8.cuh"
 #include "tcgen05.cuh"
@@ -53,15 +52,6 @@ __device__ __forceinline__ void gi_mma(uint32_t d_tmem, uint64_t a_desc, uint64_
         : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// two fp32 values to one register of two 16-bit ones
-template <typename T> __device__ __forceinline__ uint32_t gi_pack(float a, float b)
-{
-    uint32_t r;
-    if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-    return r;
-}
-
 // Tiles in columns of 16 row tiles, so that the tiles of one moment share panels of both matrices in L2.
 __device__ __forceinline__ void gi_tile(int tile, int m_tiles, int n_tiles, int& tm, int& tn)
 {
@@ -97,7 +87,7 @@ __device__ __forceinline__ void gi_write(const GiArgs& a, unsigned char* stage, 
             for (int u = 0; u < 4; ++u) y[u] = relu_ref(y[u]);
         }
         if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(mine + 4 * j) = make_float4(y[0], y[1], y[2], y[3]);
-        else *reinterpret_cast<uint2*>(mine + 2 * j) = make_uint2(gi_pack<T>(y[0], y[1]), gi_pack<T>(y[2], y[3]));
+        else *reinterpret_cast<uint2*>(mine + 2 * j) = make_uint2(pack_16bit<T>(y[0], y[1]), pack_16bit<T>(y[2], y[3]));
     }
     __syncwarp();
     T* const C = static_cast<T*>(a.C);
