@@ -207,24 +207,28 @@ def _refuse(text: str):
     raise S2VError(-1, f"invalid argument: {text}")
 
 
-def _matrix(name: str, t, device: int, rows: int | None = None, cols: int | None = None, dtype=None) -> int:
+def _matrix(name: str, t, device: int, rows: int, cols: int, dtype) -> int:
     """The leading dimension of a 2-d device matrix with adjacent columns; raises for any other tensor."""
-    if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
-        _refuse(f"{name} has shape {tuple(t.shape)}, wanted ({'any' if rows is None else rows}, {'any' if cols is None else cols})")
-    if (t.dtype not in _DTYPES) if dtype is None else (t.dtype != dtype):
-        _refuse(f"{name} is {t.dtype}")
-    if t.get_device() != device:
-        _refuse(f"{name} is on {t.device}, the context on cuda:{device}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        _refuse(f"the columns of {name} are not adjacent")
-    # (of a single row or column torch may give any stride; a row repeated by expand() has stride 0 and is refused by the library)
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    shape = t.shape
+    if len(shape) == 2 and shape[0] == rows and shape[1] == cols and t.dtype is dtype and t.get_device() == device:
+        ld, step = t.stride()
+        if step == 1 or cols <= 1:
+            # (of a single row or column torch may give any stride; a row repeated by expand() has stride 0 and is refused by the library)
+            return ld if rows > 1 else max(ld, cols)
+    _refuse(f"{name} is no {rows} x {cols} matrix of {dtype} with adjacent columns on cuda:{device}, but {tuple(shape)} of {t.dtype} on {t.device} with strides {t.stride()}")
 
 
 def _vector(name: str, t, device: int, length: int):
     """Checks an fp32 device vector (or None)."""
-    if t is not None and (t.dim() != 1 or t.shape[0] != length or t.dtype != torch.float32 or (length > 1 and t.stride(0) != 1) or t.get_device() != device):
-        _refuse(f"{name} is no contiguous fp32 vector of {length} on cuda:{device}: {tuple(t.shape)} {t.dtype} on {t.device}")
+    if t is not None and not (t.dtype is torch.float32 and t.get_device() == device and t.shape == (length,) and t.is_contiguous()):
+        _refuse(f"{name} is no contiguous fp32 vector of {length} on cuda:{device}, but {tuple(t.shape)} of {t.dtype} on {t.device}")
+
+
+def _sizes(name: str, t):
+    """Rows, columns and element type of a matrix that the others go by."""
+    if len(t.shape) != 2 or t.dtype not in _DTYPES:
+        _refuse(f"{name} is no matrix of fp32, fp16 or bf16 numbers, but {tuple(t.shape)} of {t.dtype}")
+    return (*t.shape, t.dtype)
 
 
 COMM_ID_BYTES = 128
@@ -409,22 +413,23 @@ class Context:
     # -- dense layers with 8-bit weights (types: fp32, fp16, bf16; matrices may have a leading dimension of their own)
     def quantize_rows_i8(self, x, q, scale, stream=None):
         """s2v_quantize_rows_i8: rows of x to int8 q and fp32 scale, x ~ scale[:, None] * q."""
-        rows, cols = x.shape
-        ldx, ldq = _matrix("x", x, self.device), _matrix("q", q, self.device, rows, cols, torch.int8)
-        _vector("scale", scale, self.device, rows)
-        self.call("s2v_quantize_rows_i8", stream, rows, cols, _DTYPES[x.dtype], _ptr(x), ldx, _ptr(q), ldq, _ptr(scale))
+        rows, cols, dtype = _sizes("x", x)
+        dev = self.device
+        ldx, ldq = _matrix("x", x, dev, rows, cols, dtype), _matrix("q", q, dev, rows, cols, torch.int8)
+        _vector("scale", scale, dev, rows)
+        self.call("s2v_quantize_rows_i8", stream, rows, cols, _DTYPES[dtype], x.data_ptr(), ldx, q.data_ptr(), ldq, scale.data_ptr())
         return q, scale
 
     def gemm_i8(self, A, a_scale, B, b_scale, C_out, bias=None, relu=False, stream=None):
         """s2v_gemm_i8: C = act((a_scale x b_scale) * (A B^T) + bias) with int8 A [m x k] and B [n x k], rows on 16-byte boundaries."""
-        (m, k), n = A.shape, B.shape[0]
-        lda, ldb = _matrix("A", A, self.device, dtype=torch.int8), _matrix("B", B, self.device, n, k, torch.int8)
-        ldc = _matrix("C_out", C_out, self.device, m, n)
-        _vector("a_scale", a_scale, self.device, m)
-        _vector("b_scale", b_scale, self.device, n)
-        _vector("bias", bias, self.device, n)
-        self.call("s2v_gemm_i8", stream, m, n, k, _ptr(A), lda, _ptr(a_scale), _ptr(B), ldb, _ptr(b_scale), _ptr(bias), int(relu),
-                  _DTYPES[C_out.dtype], _ptr(C_out), ldc)
+        m, n, dtype = _sizes("C_out", C_out)
+        k, dev = A.shape[-1], self.device
+        lda, ldb, ldc = _matrix("A", A, dev, m, k, torch.int8), _matrix("B", B, dev, n, k, torch.int8), _matrix("C_out", C_out, dev, m, n, dtype)
+        _vector("a_scale", a_scale, dev, m)
+        _vector("b_scale", b_scale, dev, n)
+        _vector("bias", bias, dev, n)
+        self.call("s2v_gemm_i8", stream, m, n, k, A.data_ptr(), lda, a_scale.data_ptr(), B.data_ptr(), ldb, b_scale.data_ptr(), _ptr(bias),
+                  1 if relu else 0, _DTYPES[dtype], C_out.data_ptr(), ldc)
         return C_out
 
     def linear_i8_workspace_bytes(self, m: int, k: int) -> int:
@@ -432,45 +437,40 @@ class Context:
 
     def linear_i8(self, x, W, w_scale, y, workspace, bias=None, relu=False, stream=None):
         """s2v_linear_i8: y = act(x W^T + bias) with x quantised row by row on the way; W int8 [n x k] with a scale per row."""
-        (m, k), n = x.shape, W.shape[0]
-        ldx, ldw = _matrix("x", x, self.device), _matrix("W", W, self.device, n, k, torch.int8)
-        ldy = _matrix("y", y, self.device, m, n)
-        _vector("w_scale", w_scale, self.device, n)
-        _vector("bias", bias, self.device, n)
-        if workspace.get_device() != self.device or not workspace.is_contiguous():
+        (m, k, xtype), (rows, n, ytype), dev = _sizes("x", x), _sizes("y", y), self.device
+        ldx, ldw, ldy = _matrix("x", x, dev, m, k, xtype), _matrix("W", W, dev, n, k, torch.int8), _matrix("y", y, dev, m, n, ytype)
+        _vector("w_scale", w_scale, dev, n)
+        _vector("bias", bias, dev, n)
+        if workspace.get_device() != dev or not workspace.is_contiguous():
             _refuse("workspace is not contiguous or on another device")
-        self.call("s2v_linear_i8", stream, m, n, k, _DTYPES[x.dtype], _ptr(x), ldx, _ptr(W), ldw, _ptr(w_scale), _ptr(bias), int(relu),
-                  _ptr(workspace), workspace.numel() * workspace.element_size(), _DTYPES[y.dtype], _ptr(y), ldy)
+        self.call("s2v_linear_i8", stream, m, n, k, _DTYPES[xtype], x.data_ptr(), ldx, W.data_ptr(), ldw, w_scale.data_ptr(), _ptr(bias), 1 if relu else 0,
+                  workspace.data_ptr(), workspace.numel() * workspace.element_size(), _DTYPES[ytype], y.data_ptr(), ldy)
         return y
 
     # -- distillation from a teacher's top logits
-    def _distill_args(self, z, idx, t, temperature, t_lse, row_weight, dz):
-        (rows, cols), top = z.shape, idx.shape[1]
-        ldz, ldt = _matrix("z", z, self.device), _matrix("idx", idx, self.device, rows, top, torch.int32)
-        if _matrix("t", t, self.device, rows, top) != ldt and rows > 1:
+    def _distill_args(self, z, idx, t, temperature, t_lse, row_weight, stats, dz):
+        (rows, cols, dtype), (_, top, ttype), dev = _sizes("z", z), _sizes("t", t), self.device
+        ldz, ldt = _matrix("z", z, dev, rows, cols, dtype), _matrix("t", t, dev, rows, top, ttype)
+        if _matrix("idx", idx, dev, rows, top, torch.int32) != ldt and rows > 1:
             _refuse("idx and t need the same leading dimension")
-        _vector("t_lse", t_lse, self.device, rows)
-        _vector("row_weight", row_weight, self.device, rows)
-        lddz = 0 if dz is None else _matrix("dz", dz, self.device, rows, cols, z.dtype)
-        return (rows, cols, _DTYPES[z.dtype], _ptr(z), ldz, top, _ptr(idx), _DTYPES[t.dtype], _ptr(t), ldt, _ptr(t_lse), temperature, _ptr(row_weight)), lddz
-
-    def _distill_stats(self, stats, rows):
-        if stats is not None and _matrix("stats", stats, self.device, rows, 4, torch.float32) != 4 and rows > 1:
+        _vector("t_lse", t_lse, dev, rows)
+        _vector("row_weight", row_weight, dev, rows)
+        if stats is not None and _matrix("stats", stats, dev, rows, 4, torch.float32) != 4 and rows > 1:
             _refuse("stats is not contiguous")
+        lddz = 0 if dz is None else _matrix("dz", dz, dev, rows, cols, dtype)
+        return (rows, cols, _DTYPES[dtype], z.data_ptr(), ldz, top, idx.data_ptr(), _DTYPES[ttype], t.data_ptr(), ldt, _ptr(t_lse), temperature, _ptr(row_weight)), lddz
 
     def distill_topk(self, z, idx, t, loss, temperature=1.0, t_lse=None, row_weight=None, stats=None, dz=None, stream=None):
         """s2v_distill_topk: loss[i] = row_weight[i] * KL(teacher's top logits || student's row z[i]); dz (may be z): its gradient;
         stats: float [rows x 4] kept for distill_topk_grad."""
-        args, lddz = self._distill_args(z, idx, t, temperature, t_lse, row_weight, dz)
-        _vector("loss", loss, self.device, z.shape[0])
-        self._distill_stats(stats, z.shape[0])
-        self.call("s2v_distill_topk", stream, *args, _ptr(loss), _ptr(stats), _ptr(dz), lddz)
+        args, lddz = self._distill_args(z, idx, t, temperature, t_lse, row_weight, stats, dz)
+        _vector("loss", loss, self.device, args[0])
+        self.call("s2v_distill_topk", stream, *args, loss.data_ptr(), _ptr(stats), _ptr(dz), lddz)
         return loss
 
     def distill_topk_grad(self, z, idx, t, stats, dz, temperature=1.0, t_lse=None, row_weight=None, stream=None):
         """s2v_distill_topk_grad: the gradient of sum(row_weight * KL) from the stats of distill_topk."""
-        args, lddz = self._distill_args(z, idx, t, temperature, t_lse, row_weight, dz)
-        self._distill_stats(stats, z.shape[0])
+        args, lddz = self._distill_args(z, idx, t, temperature, t_lse, row_weight, stats, dz)
         self.call("s2v_distill_topk_grad", stream, *args, _ptr(stats), _ptr(dz), lddz)
         return dz
 

@@ -136,46 +136,7 @@ __device__ __forceinline__ float dt_loss(const DtArgs& a, const DtList& l, float
     return (float)(kl * weight);
 }
 
-// ---------------------------------------------------------------- pieces of 16 bytes
-template <typename T> constexpr int DT_PER = 16 / (int)sizeof(T);
-
-__device__ __forceinline__ void dt_unpack(const uint4& v, float* x, float)
-{
-    x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
-}
-__device__ __forceinline__ void dt_unpack(const uint4& v, float* x, __half)
-{
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        x[2 * i] = f.x, x[2 * i + 1] = f.y;
-    }
-}
-__device__ __forceinline__ void dt_unpack(const uint4& v, float* x, __nv_bfloat16)
-{
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-}
-__device__ __forceinline__ uint4 dt_pack(const float* y, float) { return make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])); }
-template <typename T> __device__ __forceinline__ uint4 dt_pack(const float* y, T)
-{
-    return make_uint4(pack_16bit<T>(y[0], y[1]), pack_16bit<T>(y[2], y[3]), pack_16bit<T>(y[4], y[5]), pack_16bit<T>(y[6], y[7]));
-}
-
-// A row's columns: `head` in front of the first 16-byte boundary, `pieces` of 16 bytes, `tail` behind them.
-template <typename T> struct DtRowShape {
-    int head, pieces, tail;
-    __device__ __forceinline__ DtRowShape(const T* z, int64_t cols)
-    {
-        const int off = (int)((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / (int)sizeof(T);
-        head = off < cols ? off : (int)cols;
-        pieces = (int)((cols - head) / DT_PER<T>);
-        tail = (int)(cols - head) - pieces * DT_PER<T>;
-    }
-};
-
+// ---------------------------------------------------------------- sums and gradients of pieces of 16 bytes
 struct DtSum {   // of exp((z - m) / T), relative to the largest z
     float m, s;
     template <int N> __device__ __forceinline__ void add(const float* x, uint32_t listed, float c)
@@ -210,7 +171,7 @@ struct DtSum {   // of exp((z - m) / T), relative to the largest z
 // zeros in the columns of a row that falls to this thread, one of `threads`
 template <typename T> __device__ __forceinline__ void dt_zero_row(T* dz, int64_t cols, int at, int threads)
 {
-    const DtRowShape<T> row(dz, cols);
+    const row_pieces<T> row(dz, cols);
     if (at < row.head) dz[at] = from_f32<T>(0.0f);
     if (at < row.tail) dz[cols - 1 - at] = from_f32<T>(0.0f);
     uint4* const to = reinterpret_cast<uint4*>(dz + row.head);
@@ -220,13 +181,13 @@ template <typename T> __device__ __forceinline__ void dt_zero_row(T* dz, int64_t
 // gradient of a piece; listed columns are written by their entries
 template <typename T> __device__ __forceinline__ void dt_store(T* to, bool whole, const uint4& v, uint32_t listed, float base, float outer, float c)
 {
-    constexpr int N = DT_PER<T>;
+    constexpr int N = PIECE<T>;
     float x[N];
-    dt_unpack(v, x, T());
+    unpack_piece(v, x, T());
 #pragma unroll
     for (int e = 0; e < N; ++e) x[e] = outer == 0.0f ? 0.0f : dt_exp2((x[e] - base) * c) * outer;
     if (whole && listed == 0) {
-        __stcs(reinterpret_cast<uint4*>(to), dt_pack(x, T()));
+        __stcs(reinterpret_cast<uint4*>(to), pack_piece(x, T()));
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e)
@@ -249,7 +210,7 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
 {
     __shared__ DwShared shared[DW_WARPS];
     DwShared& s = shared[threadIdx.x >> 5];
-    constexpr int N = DT_PER<T>, EDGE = DW_PIECES * 32;   // mask bytes of the head and the tail: EDGE, EDGE + 1
+    constexpr int N = PIECE<T>, EDGE = DW_PIECES * 32;   // mask bytes of the head and the tail: EDGE, EDGE + 1
     const int lane = threadIdx.x & 31;
     const double inv_t = 1.0 / (double)a.temperature;
     const float c = 1.4426950408889634f / a.temperature;
@@ -261,7 +222,7 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
         const T* const z = static_cast<const T*>(a.z) + r * a.ldz;
         T* const dz = a.dz ? static_cast<T*>(a.dz) + r * a.lddz : nullptr;
         const float weight = a.row_weight ? __ldg(a.row_weight + r) : 1.0f;
-        const DtRowShape<T> row(z, a.cols);
+        const row_pieces<T> row(z, a.cols);
         float tmax = -INFINITY;
         bool some = false;
         for (int k = lane; k < a.top; k += 32) {
@@ -344,7 +305,7 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
             for (int j = 0; j < NV; ++j)
                 if (j * 32 + lane < row.pieces) {
                     float x[N];
-                    dt_unpack(v[j], x, T());
+                    unpack_piece(v[j], x, T());
                     d.template add<N>(x, mask[j * 32 + lane], c);
                 }
             if (in_head || in_tail) d.template add<1>(&edge, edge_listed, c);
@@ -397,7 +358,7 @@ __global__ void __launch_bounds__(DC_THREADS, 2) distill_cluster_kernel(const Dt
 {
     extern __shared__ uint32_t dc_mask[];   // a byte per piece of this CTA
     __shared__ DcShared s;
-    constexpr int N = DT_PER<T>;
+    constexpr int N = PIECE<T>;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)(blockIdx.x % (unsigned)ctas);
     const double inv_t = 1.0 / (double)a.temperature;
@@ -411,7 +372,7 @@ __global__ void __launch_bounds__(DC_THREADS, 2) distill_cluster_kernel(const Dt
         const T* const z = static_cast<const T*>(a.z) + r * a.ldz;
         T* const dz = a.dz ? static_cast<T*>(a.dz) + r * a.lddz : nullptr;
         const float weight = a.row_weight ? __ldg(a.row_weight + r) : 1.0f;
-        const DtRowShape<T> row(z, a.cols);
+        const row_pieces<T> row(z, a.cols);
         const int first_piece = rank * most, pieces = max(0, min(most, row.pieces - first_piece));
         const uint4* const zp = reinterpret_cast<const uint4*>(z + row.head) + first_piece;
         const int id = dt_load_id(a, r, tid);
@@ -499,12 +460,12 @@ __global__ void __launch_bounds__(DC_THREADS, 2) distill_cluster_kernel(const Dt
             for (int j = 0; j < NV; ++j)
                 if (j * DC_THREADS + tid < pieces) {
                     float x[N];
-                    dt_unpack(v[j], x, T());
+                    unpack_piece(v[j], x, T());
                     d.template add<N>(x, mask[j * DC_THREADS + tid], c);
                 }
             for (int p = NV * DC_THREADS + tid; p < pieces; p += DC_THREADS) {
                 float x[N];
-                dt_unpack(zp[p], x, T());
+                unpack_piece(zp[p], x, T());
                 d.template add<N>(x, mask[p], c);
             }
             if (in_head || in_tail) d.template add<1>(&edge, edge_listed, c);
@@ -557,7 +518,7 @@ __global__ void __launch_bounds__(DC_THREADS, 2) distill_cluster_kernel(const Dt
 
 template <typename T, int NV, bool GRAD_ONLY> int dc_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a, int ctas)
 {
-    const int64_t most = (a.cols / DT_PER<T> + ctas - 1) / ctas;
+    const int64_t most = (a.cols / PIECE<T> + ctas - 1) / ctas;
     int64_t rows = a.rows;
     if (rows > (1 << 20)) rows = 1 << 20;   // (clusters; further rows in turns)
     cudaLaunchConfig_t cfg = {};
@@ -587,7 +548,7 @@ template <typename T, int NV, bool GRAD_ONLY> int dw_launch(s2v_ctx* ctx, cudaSt
 
 template <typename T, bool GRAD_ONLY> int dt_launch_type(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a)
 {
-    const int64_t pieces = a.cols / DT_PER<T>;
+    const int64_t pieces = a.cols / PIECE<T>;
     if (pieces <= 32) return dw_launch<T, 1, GRAD_ONLY>(ctx, st, a);
     if (pieces <= 32 * DW_PIECES) return dw_launch<T, DW_PIECES, GRAD_ONLY>(ctx, st, a);
     int ctas = 1;

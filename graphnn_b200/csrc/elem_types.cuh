@@ -36,6 +36,46 @@ template <typename T> __device__ __forceinline__ uint32_t pack_16bit(float a, fl
     else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
     return r;
 }
+// ---- pieces of 16 bytes
+template <typename T> constexpr int PIECE = 16 / (int)sizeof(T);   // elements of one
+
+__device__ __forceinline__ void unpack_piece(const uint4& v, float* x, float)
+{
+    x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
+}
+__device__ __forceinline__ void unpack_piece(const uint4& v, float* x, __half)
+{
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void unpack_piece(const uint4& v, float* x, __nv_bfloat16)
+{
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+__device__ __forceinline__ uint4 pack_piece(const float* y, float) { return make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])); }
+template <typename T> __device__ __forceinline__ uint4 pack_piece(const float* y, T)
+{
+    return make_uint4(pack_16bit<T>(y[0], y[1]), pack_16bit<T>(y[2], y[3]), pack_16bit<T>(y[4], y[5]), pack_16bit<T>(y[6], y[7]));
+}
+
+// A row's columns: `head` in front of the first 16-byte boundary, `pieces` of 16 bytes, `tail` behind them.
+template <typename T> struct row_pieces {
+    int head, tail;
+    int pieces;
+    __device__ __forceinline__ row_pieces(const T* z, int64_t cols)
+    {
+        const int off = (int)((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / (int)sizeof(T);
+        head = off < cols ? off : (int)cols;
+        pieces = (int)((cols - head) / PIECE<T>);
+        tail = (int)(cols - head - (int64_t)pieces * PIECE<T>);
+    }
+};
 
 }  // namespace
 

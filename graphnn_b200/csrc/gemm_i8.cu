@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
 
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // A and its scales may come from a kernel in front
     if (warp == 0) {   // copies
         int it = 0;
         bool ok = true;
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
             gi_tile(tile, a.m_tiles, a.n_tiles, tm, tn);
             const int acc = t & 1;
             const int64_t row0 = (int64_t)tm * 128 + quarter * 32;
-            const float sa = row0 + lane < a.m ? __ldg(a.a_scale + row0 + lane) : 0.0f;
+            const float sa = row0 + lane < a.m ? a.a_scale[row0 + lane] : 0.0f;
             if (a.kblocks > 0 && !tc_wait(bar(Cfg::DONE + acc), (uint32_t)(t / 2) & 1u, abort_flag, a.status, 73)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (int c = half * HALF; c < (half + 1) * HALF; c += COLS) {
@@ -232,7 +233,7 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::TM_COLS) : "memory");
 }
 
-template <typename T, int BN> int gi_launch(s2v_ctx* ctx, cudaStream_t st, const s2v_gemm_i8_args& g)
+template <typename T, int BN> int gi_launch(s2v_ctx* ctx, cudaStream_t st, const s2v_gemm_i8_args& g, bool dependent)
 {
     using Cfg = GiCfg<BN>;
     CUtensorMap map_a, map_b;
@@ -258,20 +259,32 @@ template <typename T, int BN> int gi_launch(s2v_ctx* ctx, cudaStream_t st, const
     S2V_CUDA_OK(ctx, s2v_allow_shared(gemm_i8_kernel<T, BN>, Cfg::SMEM));
     const int64_t tiles = mt * nt;
     const unsigned grid = (unsigned)(tiles < ctx->sm_count ? tiles : ctx->sm_count);
-    gemm_i8_kernel<T, BN><<<grid, GI_THREADS, Cfg::SMEM, st>>>(map_a, map_b, a);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(GI_THREADS);
+    cfg.dynamicSmemBytes = Cfg::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = dependent ? 1 : 0;
+    S2V_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, gemm_i8_kernel<T, BN>, map_a, map_b, a));
     S2V_CHECK_LAUNCH(ctx, "gemm_i8_kernel");
     return S2V_OK;
 }
 
 }  // namespace
 
-int s2v_launch_gemm_i8(s2v_ctx* ctx, cudaStream_t st, const s2v_gemm_i8_args& g)
+int s2v_launch_gemm_i8(s2v_ctx* ctx, cudaStream_t st, const s2v_gemm_i8_args& g, bool dependent)
 {
+    if (s2v_gemv_i8_takes(g.m, g.n, g.k)) return s2v_launch_gemv_i8(ctx, st, -1, g);
+    const int64_t mt = (g.m + 127) / 128;
+    if (g.k > 0 && (g.m <= 64 || mt * ((g.n + 63) / 64) < ctx->sm_count)) return s2v_launch_gemm_i8_split(ctx, st, g, dependent);
     return s2v_by_dtype(g.c_type, [&](auto type) {
         using T = decltype(type);
-        const int64_t mt = (g.m + 127) / 128;
-        if (mt * ((g.n + 255) / 256) >= ctx->sm_count) return gi_launch<T, 256>(ctx, st, g);
-        if (mt * ((g.n + 127) / 128) >= ctx->sm_count) return gi_launch<T, 128>(ctx, st, g);
-        return gi_launch<T, 64>(ctx, st, g);
+        if (mt * ((g.n + 255) / 256) >= ctx->sm_count) return gi_launch<T, 256>(ctx, st, g, dependent);
+        if (mt * ((g.n + 127) / 128) >= ctx->sm_count) return gi_launch<T, 128>(ctx, st, g, dependent);
+        return gi_launch<T, 64>(ctx, st, g, dependent);
     });
 }

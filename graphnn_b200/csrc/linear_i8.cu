@@ -1,31 +1,88 @@
 // Dense layers with 8-bit weights: rows to 8-bit integers with a scale each, and the entry points of the
 // product of two such matrices (gemm_i8.cu).
 #include "gemm_i8.cuh"
+#include "quantize.cuh"
 
 namespace
 {
 
-constexpr float Q_LEAST = 7.703719777548943e-34f;   // 2^-110: below it 127 / a comes near the end of fp32
+constexpr int QR_CTA = 256;
 
-// A warp per row, two passes over it: the largest magnitude, then the integers.
-template <typename T>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(int64_t rows, int64_t cols, const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q,
-                                                            int64_t ldq, float* __restrict__ scale)
+// A row by a warp (THREADS = 32) or by a CTA: 16-byte pieces, the first NV of each thread kept in registers between the largest magnitude and the
+// integers (a longer row's others are read again), single columns in front of the first 16-byte boundary and behind the last piece.
+template <typename T, int NV, int THREADS>
+__global__ void __launch_bounds__(QR_CTA) quantize_rows_kernel(int64_t rows, int64_t cols, const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q,
+                                                               int64_t ldq, float* __restrict__ scale)
 {
-    const int lane = threadIdx.x & 31;
-    const int64_t warps = ((int64_t)gridDim.x * blockDim.x) >> 5;
-    for (int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; r < rows; r += warps) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (a product behind this kernel waits for its end by itself)
+    constexpr int N = PIECE<T>;
+    __shared__ uint32_t part[QR_CTA / 32];
+    const int at = THREADS == 32 ? threadIdx.x & 31 : threadIdx.x;
+    const int64_t own = THREADS == 32 ? (int64_t)blockIdx.x * (QR_CTA / 32) + (threadIdx.x >> 5) : blockIdx.x, step = (int64_t)gridDim.x * (QR_CTA / THREADS);
+    for (int64_t r = own; r < rows; r += step) {
         const T* const xr = x + r * ldx;
         int8_t* const qr = q + r * ldq;
-        uint32_t a = 0;   // magnitudes as bit patterns: infinities and NaN are the largest
-        for (int64_t c = lane; c < cols; c += 32) a = max(a, __float_as_uint(to_f32(xr[c])) & 0x7fffffffu);
+        const row_pieces<T> row(xr, cols);
+        const uint4* const xp = reinterpret_cast<const uint4*>(xr + row.head);
+        uint4 v[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * THREADS + at < row.pieces) v[j] = __ldg(xp + j * THREADS + at);
+        const bool single = at < row.head || (at >= THREADS - row.tail);
+        const int64_t single_at = at < row.head ? at : cols - THREADS + at;
+        const float xs = single ? to_f32(xr[single_at]) : 0.0f;
+        uint32_t a = __float_as_uint(xs) & 0x7fffffffu;   // magnitudes as bit patterns: infinities and NaN are the largest
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * THREADS + at < row.pieces) a = max(a, q_largest<T>(v[j]));
+        for (int64_t p = NV * THREADS + at; p < row.pieces; p += THREADS) a = max(a, q_largest<T>(__ldg(xp + p)));
         a = __reduce_max_sync(0xffffffffu, a);
-        const float amax = __uint_as_float(a);
-        const bool finite = a < 0x7f800000u;
-        const float f = finite && amax >= Q_LEAST ? __fdiv_rn(127.0f, amax) : 0.0f;
-        for (int64_t c = lane; c < cols; c += 32) qr[c] = f == 0.0f ? 0 : (int8_t)__float2int_rn(__fmul_rn(to_f32(xr[c]), f));
-        if (lane == 0) scale[r] = !finite ? __uint_as_float(0x7fffffffu) : f == 0.0f ? 0.0f : __fdiv_rn(amax, 127.0f);
+        if constexpr (THREADS > 32) {
+            __syncthreads();   // (the row before has been read)
+            if ((at & 31) == 0) part[at >> 5] = a;
+            __syncthreads();
+            a = __reduce_max_sync(0xffffffffu, part[at & (QR_CTA / 32 - 1)]);
+        }
+        const q_row k(a);
+        int8_t* const qp = qr + row.head;
+        const bool whole = (reinterpret_cast<uintptr_t>(qp) & (N - 1)) == 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * THREADS + at < row.pieces) q_store<T>(qp + (j * THREADS + at) * N, whole, v[j], k);
+        for (int64_t p = NV * THREADS + at; p < row.pieces; p += THREADS) q_store<T>(qp + p * N, whole, __ldg(xp + p), k);
+        if (single) qr[single_at] = (int8_t)k.integer(xs);
+        if (at == 0) scale[r] = k.scale;
     }
+}
+
+template <typename T> int quantize_launch(s2v_ctx* ctx, cudaStream_t st, int64_t rows, int64_t cols, const T* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale)
+{
+    const int64_t pieces = cols / PIECE<T>;
+    const auto go = [&](auto kernel, int64_t blocks) {
+        const int64_t cap = (int64_t)1 << 20;
+        kernel<<<(unsigned)(blocks < cap ? blocks : cap), QR_CTA, 0, st>>>(rows, cols, x, ldx, q, ldq, scale);
+        S2V_CHECK_LAUNCH(ctx, "quantize_rows_kernel");
+        return (int)S2V_OK;
+    };
+    const int64_t per_warp = (rows + QR_CTA / 32 - 1) / (QR_CTA / 32);
+    if (pieces <= 32) return go(quantize_rows_kernel<T, 1, 32>, per_warp);
+    if (pieces <= 128) return go(quantize_rows_kernel<T, 4, 32>, per_warp);
+    if (pieces <= 2 * QR_CTA) return go(quantize_rows_kernel<T, 2, QR_CTA>, rows);
+    if (pieces <= 4 * QR_CTA) return go(quantize_rows_kernel<T, 4, QR_CTA>, rows);
+    return go(quantize_rows_kernel<T, 8, QR_CTA>, rows);
+}
+
+int check_quantize(s2v_ctx* ctx, const char* name, int64_t rows, int64_t cols, int x_type, const void* x, int64_t ldx)
+{
+    const std::string who(name);
+    if (rows < 0 || cols < 0) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": negative size");
+    if (!s2v_dtype_ok(x_type)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": unknown element type");
+    if (rows == 0) return S2V_OK;
+    if (cols > INT32_MAX) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, who + ": more than 2^31 - 1 columns");
+    if (cols > 0 && !x) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": NULL pointer");
+    if (rows > 1 && ldx < cols) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": leading dimension below the number of columns");
+    if (reinterpret_cast<uintptr_t>(x) % s2v_dtype_bytes(x_type)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": misaligned x");
+    return S2V_OK;
 }
 
 size_t workspace_scale_offset(int64_t m, int64_t k)
@@ -58,20 +115,14 @@ int s2v_quantize_rows_i8(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t 
                          float* scale)
 {
     S2V_ENTER(ctx);
-    if (rows < 0 || cols < 0) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "quantize_rows: negative size");
-    if (!s2v_dtype_ok(x_type)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "quantize_rows: unknown element type");
-    if (rows == 0) return S2V_OK;
-    if (!scale || (cols > 0 && (!x || !q))) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "quantize_rows: NULL pointer");
-    if (rows > 1 && (ldx < cols || ldq < cols)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "quantize_rows: leading dimension below the number of columns");
-    if (reinterpret_cast<uintptr_t>(x) % s2v_dtype_bytes(x_type)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "quantize_rows: misaligned x");
+    const int rc = check_quantize(ctx, "quantize_rows", rows, cols, x_type, x, ldx);
+    if (rc != S2V_OK || rows == 0) return rc;
+    if (!scale || (cols > 0 && !q)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "quantize_rows: NULL pointer");
+    if (rows > 1 && ldq < cols) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "quantize_rows: leading dimension below the number of columns");
     cudaStream_t st = s2v_pick_stream(ctx, stream);
-    int64_t blocks = (rows + 7) / 8;
-    if (blocks > (int64_t)ctx->sm_count * 8) blocks = (int64_t)ctx->sm_count * 8;
     return s2v_by_dtype(x_type, [&](auto type) {
         using T = decltype(type);
-        quantize_rows_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(rows, cols, static_cast<const T*>(x), ldx, q, ldq, scale);
-        S2V_CHECK_LAUNCH(ctx, "quantize_rows_kernel");
-        return (int)S2V_OK;
+        return quantize_launch<T>(ctx, st, rows, cols, static_cast<const T*>(x), ldx, q, ldq, scale);
     });
 }
 
@@ -85,7 +136,7 @@ int s2v_gemm_i8(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, int64_t k
     if (m > 1 && k > 0 && (lda < k || lda % 16 != 0)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "gemm_i8: lda below k or no multiple of 16");
     if (!s2v_aligned16(A)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "gemm_i8: 8-bit matrices must be 16-byte aligned");
     const s2v_gemm_i8_args g{m, n, k, lda, ldb, ldc, A, B, a_scale, b_scale, bias, relu, c_type, C};
-    return s2v_launch_gemm_i8(ctx, s2v_pick_stream(ctx, stream), g);
+    return s2v_launch_gemm_i8(ctx, s2v_pick_stream(ctx, stream), g, false);
 }
 
 size_t s2v_linear_i8_workspace_bytes(int64_t m, int64_t k)
@@ -106,9 +157,15 @@ int s2v_linear_i8(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, int64_t
     int8_t* const q = static_cast<int8_t*>(workspace);
     float* const scale = reinterpret_cast<float*>(q + workspace_scale_offset(m, k));
     const int64_t ldq = (k + 15) / 16 * 16;
-    const int done = s2v_quantize_rows_i8(ctx, stream, m, k, x_type, x, ldx, q, ldq, scale);
-    if (done != S2V_OK) return done;
-    return s2v_gemm_i8(ctx, stream, m, n, k, q, ldq, scale, W, ldw, w_scale, bias, relu, y_type, y, ldy);
+    const int bad = check_quantize(ctx, "linear_i8", m, k, x_type, x, ldx);
+    if (bad != S2V_OK) return bad;
+    s2v_gemm_i8_args g{m, n, k, ldx, ldw, ldy, x, W, nullptr, w_scale, bias, relu, y_type, y};
+    cudaStream_t st = s2v_pick_stream(ctx, stream);
+    if (s2v_gemv_i8_takes(m, n, k)) return s2v_launch_gemv_i8(ctx, st, x_type, g);
+    const int quantized = s2v_by_dtype(x_type, [&](auto type) { return quantize_launch<decltype(type)>(ctx, st, m, k, static_cast<const decltype(type)*>(x), ldx, q, ldq, scale); });
+    if (quantized != S2V_OK) return quantized;
+    g.lda = ldq, g.A = q, g.a_scale = scale;
+    return s2v_launch_gemm_i8(ctx, st, g, true);
 }
 
 }  // extern "C"
