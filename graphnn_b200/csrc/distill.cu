@@ -51,6 +51,90 @@ __device__ __forceinline__ float dt_warp_max(float v)
     return v;
 }
 
+// ---------------------------------------------------------------- sums and gradients of pieces of 16 bytes
+// e[i] = exp2((x[i] + minus_m) * c), two at a time
+template <int N> __device__ __forceinline__ void dt_exps(const float* x, float minus_m, float c, float* e)
+{
+    if constexpr (N == 1) {
+        e[0] = dt_exp2((x[0] + minus_m) * c);
+    } else {
+        uint64_t m2, c2;
+        asm("mov.b64 %0, {%1, %1};" : "=l"(m2) : "f"(minus_m));
+        asm("mov.b64 %0, {%1, %1};" : "=l"(c2) : "f"(c));
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            uint64_t v;
+            asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x[i]), "f"(x[i + 1]));
+            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(m2));
+            asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(c2));
+            asm("mov.b64 {%0, %1}, %2;" : "=f"(e[i]), "=f"(e[i + 1]) : "l"(v));
+            e[i] = dt_exp2(e[i]);
+            e[i + 1] = dt_exp2(e[i + 1]);
+        }
+    }
+}
+
+struct DtSum {   // of exp((z - m) / T), relative to the largest z
+    float m, s;
+    // (x is overwritten where columns are listed: few pieces have any)
+    template <int N> __device__ __forceinline__ void add(float* x, uint32_t listed, float c)
+    {
+        if (listed) {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (listed >> e & 1) x[e] = -INFINITY;
+        }
+        float top = x[0];
+#pragma unroll
+        for (int e = 1; e < N; ++e) top = fmaxf(top, x[e]);
+        if (top > m) {
+            s *= dt_exp2((m - top) * c);   // (m = -infinity: no sum yet)
+            m = top;
+        }
+        float e[N];
+        dt_exps<N>(x, -dt_finite_or_zero(m), c, e);
+#pragma unroll
+        for (int w = N / 2; w; w >>= 1)
+#pragma unroll
+            for (int i = 0; i < w; ++i) e[i] += e[i + w];
+        s += e[0];
+    }
+    __device__ __forceinline__ void join_warp(float c)
+    {
+        const float top = dt_warp_max(m);
+        s = dt_warp_sum(s * dt_exp2((m - dt_finite_or_zero(top)) * c));
+        m = top;
+    }
+};
+
+// zeros in the columns of a row that falls to this thread, one of `threads`
+template <typename T> __device__ __forceinline__ void dt_zero_row(T* dz, int64_t cols, int at, int threads)
+{
+    const row_pieces<T> row(dz, cols);
+    if (at < row.head) dz[at] = from_f32<T>(0.0f);
+    if (at < row.tail) dz[cols - 1 - at] = from_f32<T>(0.0f);
+    uint4* const to = reinterpret_cast<uint4*>(dz + row.head);
+    for (int p = at; p < row.pieces; p += threads) to[p] = make_uint4(0, 0, 0, 0);
+}
+
+// gradient of a piece; listed columns are written by their entries
+template <typename T> __device__ __forceinline__ void dt_store(T* to, bool whole, const uint4& v, uint32_t listed, float base, float outer, float c)
+{
+    constexpr int N = PIECE<T>;
+    float x[N], e[N];
+    unpack_piece(v, x, T());
+    dt_exps<N>(x, -base, c, e);
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] *= outer;
+    if (whole && listed == 0) {
+        __stcs(reinterpret_cast<uint4*>(to), pack_piece(e, T()));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (!(listed >> i & 1)) to[i] = from_f32<T>(e[i]);
+    }
+}
+
 // ---------------------------------------------------------------- the list
 // What a row's list adds up to, over any part of its entries; P_k = exp((t_k - t_max) / T), or exp(t_k / T - t_lse) where that is given:
 //     Z = sum P,  A = sum P log P,  B = sum P (z_idx - m) / T,  s = sum of exp((z_idx - m) / T) over the columns,  m = the largest z_idx
@@ -78,35 +162,46 @@ __device__ __forceinline__ double dt_log_p(const DtArgs& a, float tv, float tmax
     return a.t_lse ? (double)tv * inv_t - t_lse : ((double)tv - (double)dt_finite_or_zero(tmax)) * inv_t;
 }
 
+// an entry's part of Z, A and B (B relative to l.m, the largest listed z)
+__device__ __forceinline__ void dt_count(const DtArgs& a, DtList& l, float tv, float tmax, double t_lse, float zk, double inv_t)
+{
+    const double lp = dt_log_p(a, tv, tmax, t_lse, inv_t), P = exp(lp);
+    l.Z += P;
+    if (P != 0.0) {
+        l.A += P * lp;
+        l.B += P * (((double)zk - (double)dt_finite_or_zero(l.m)) * inv_t);
+    }
+}
+
 // ---------------------------------------------------------------- a row, once its sums are known
 struct DtCoef {
     float M;            // the larger maximum (0 where there is none)
-    float given, rest;  // sum p, 1 - sum p; p = P * p_scale
-    float p_scale;
+    float p_scale;      // p = P * p_scale
     float inner;        // a listed column's gradient: inner * exp((z - M) / T) - scale * p
     float outer;        // any other's: outer * exp((z - m_out) / T)
     float scale;        // row_weight / T
 };
-__device__ __forceinline__ DtCoef dt_coefficients(const DtArgs& a, double Z, float m_in, float s_in, float m_out, float s_out, float weight, float c)
+__device__ __forceinline__ DtCoef dt_coefficients(const DtArgs& a, double Z, const DtSum& in, const DtSum& out, float weight, float c)
 {
     DtCoef k;
-    const float m = fmaxf(m_in, m_out);
+    const float m = fmaxf(in.m, out.m);
     k.M = dt_finite_or_zero(m);
-    const float e_out = s_out == 0.0f ? 0.0f : dt_exp2((m_out - k.M) * c), e_in = s_in == 0.0f ? 0.0f : dt_exp2((m_in - k.M) * c);
-    const float total = m == -INFINITY ? NAN : s_in * e_in + s_out * e_out;
+    const float e_out = out.s == 0.0f ? 0.0f : dt_exp2((out.m - k.M) * c), e_in = in.s == 0.0f ? 0.0f : dt_exp2((in.m - k.M) * c);
+    const float total = m == -INFINITY ? NAN : in.s * e_in + out.s * e_out;
+    float given, rest;
     if (a.t_lse) {
-        k.given = (float)Z;
-        k.rest = Z > 1.0 ? 0.0f : (float)(1.0 - Z);
+        given = (float)Z;
+        rest = Z > 1.0 ? 0.0f : (float)(1.0 - Z);
         k.p_scale = 1.0f;
     } else {
-        k.given = (float)(Z - Z + 1.0);   // one, and NaN where the list holds NaN or +infinity
-        k.rest = 0.0f;
-        k.p_scale = (float)(1.0 / Z);
+        given = (float)(Z - Z + 1.0);   // one, and NaN where the list holds NaN or +infinity
+        rest = 0.0f;
+        k.p_scale = 1.0f / (float)Z;
     }
     k.scale = weight / a.temperature;
-    const float both = __fdividef(k.given + k.rest, total);
+    const float both = (given + rest) / total;
     k.inner = k.scale * both;
-    k.outer = k.scale * (s_out == 0.0f && total == total ? 0.0f : both * e_out - __fdividef(k.rest, s_out));
+    k.outer = k.scale * (out.s == 0.0f && total == total ? 0.0f : both * e_out - rest / out.s);
     return k;
 }
 __device__ __forceinline__ float dt_loss(const DtArgs& a, const DtList& l, float m_out, double s_out, float weight, double inv_t)
@@ -136,72 +231,13 @@ __device__ __forceinline__ float dt_loss(const DtArgs& a, const DtList& l, float
     return (float)(kl * weight);
 }
 
-// ---------------------------------------------------------------- sums and gradients of pieces of 16 bytes
-struct DtSum {   // of exp((z - m) / T), relative to the largest z
-    float m, s;
-    template <int N> __device__ __forceinline__ void add(const float* x, uint32_t listed, float c)
-    {
-        float top = m;
-#pragma unroll
-        for (int e = 0; e < N; ++e) top = fmaxf(top, listed >> e & 1 ? -INFINITY : x[e]);
-        if (top > m) {
-            s *= dt_exp2((m - top) * c);   // (m = -infinity: no sum yet)
-            m = top;
-        }
-        const float base = dt_finite_or_zero(m);
-        float part = 0.0f;
-#pragma unroll
-        for (int e = 0; e < N; ++e) part += listed >> e & 1 ? 0.0f : dt_exp2((x[e] - base) * c);
-        s += part;
-    }
-    __device__ __forceinline__ void join(float om, float os, float c)
-    {
-        const float top = fmaxf(m, om), base = dt_finite_or_zero(top);
-        s = s * dt_exp2((m - base) * c) + os * dt_exp2((om - base) * c);
-        m = top;
-    }
-    __device__ __forceinline__ void join_warp(float c)
-    {
-        const float top = dt_warp_max(m);
-        s = dt_warp_sum(s * dt_exp2((m - dt_finite_or_zero(top)) * c));
-        m = top;
-    }
-};
-
-// zeros in the columns of a row that falls to this thread, one of `threads`
-template <typename T> __device__ __forceinline__ void dt_zero_row(T* dz, int64_t cols, int at, int threads)
-{
-    const row_pieces<T> row(dz, cols);
-    if (at < row.head) dz[at] = from_f32<T>(0.0f);
-    if (at < row.tail) dz[cols - 1 - at] = from_f32<T>(0.0f);
-    uint4* const to = reinterpret_cast<uint4*>(dz + row.head);
-    for (int p = at; p < row.pieces; p += threads) to[p] = make_uint4(0, 0, 0, 0);
-}
-
-// gradient of a piece; listed columns are written by their entries
-template <typename T> __device__ __forceinline__ void dt_store(T* to, bool whole, const uint4& v, uint32_t listed, float base, float outer, float c)
-{
-    constexpr int N = PIECE<T>;
-    float x[N];
-    unpack_piece(v, x, T());
-#pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = outer == 0.0f ? 0.0f : dt_exp2((x[e] - base) * c) * outer;
-    if (whole && listed == 0) {
-        __stcs(reinterpret_cast<uint4*>(to), pack_piece(x, T()));
-    } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-            if (!(listed >> e & 1)) to[e] = from_f32<T>(x[e]);
-    }
-}
-
 // ---------------------------------------------------------------- rows of up to 256 pieces: a warp each
 // The row stays in registers between the sums and the gradient.
 constexpr int DW_WARPS = 4, DW_PIECES = 8;   // pieces a lane
 struct DwShared {
     double P[DT_TOP];
-    int id[DT_TOP];
     float z[DT_TOP];
+    int id[DT_TOP];
     uint32_t mask[(DW_PIECES * 32 + 4 + 31) / 32 * 8 + 1];   // a byte per piece, then one for the head and one for the tail
 };
 
@@ -212,8 +248,8 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
     DwShared& s = shared[threadIdx.x >> 5];
     constexpr int N = PIECE<T>, EDGE = DW_PIECES * 32;   // mask bytes of the head and the tail: EDGE, EDGE + 1
     const int lane = threadIdx.x & 31;
-    const double inv_t = 1.0 / (double)a.temperature;
-    const float c = 1.4426950408889634f / a.temperature;
+    const double inv = 1.0 / (double)a.temperature;
+    const float inv_t = 1.0f / a.temperature, c = 1.4426950408889634f / a.temperature;
     const uint8_t* const mask = reinterpret_cast<const uint8_t*>(s.mask);
     for (int w = lane; w < (int)(sizeof(s.mask) / 4); w += 32) s.mask[w] = 0;
     __syncwarp();
@@ -249,21 +285,21 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
         // the scalar columns: the head's to the first lanes, the tail's to the last
         const bool in_head = lane < row.head, in_tail = lane >= 32 - row.tail;
         const int edge_at = in_head ? lane : (int)a.cols - 32 + lane, edge_bit = in_head ? lane : lane - (32 - row.tail);
-        float edge = in_head || in_tail ? to_f32(z[edge_at]) : -INFINITY;
+        const float edge = in_head || in_tail ? to_f32(z[edge_at]) : -INFINITY;
         // the list
-        const double t_lse = a.t_lse ? (double)__ldg(a.t_lse + r) : 0.0;
+        const float t_lse = a.t_lse ? __ldg(a.t_lse + r) : 0.0f;
         DtList l{0.0, 0.0, 0.0, 0.0, -INFINITY};
+        DtSum inner{-INFINITY, 0.0f};
         bool twice = false;
         for (int k = lane; k < a.top; k += 32) {
             const int id = s.id[k];
             if (id < 0) continue;
             const float zk = to_f32(z[id]);
-            const double lp = dt_log_p(a, dt_load_t(a, r, k), tmax, t_lse, inv_t), P = exp(lp);
-            s.z[k] = zk;
-            s.P[k] = P;
+            const double lp = dt_log_p(a, dt_load_t(a, r, k), tmax, (double)t_lse, inv), P = exp(lp);
+            s.z[k] = zk, s.P[k] = P;
             l.Z += P;
-            if (P != 0.0) l.A += P * lp;
-            l.m = fmaxf(l.m, zk);
+            if (!GRAD_ONLY && P != 0.0) l.A += P * lp;
+            inner.m = fmaxf(inner.m, zk);
             const int at = id - row.head, byte = at < 0 ? EDGE : at >= row.pieces * N ? EDGE + 1 : at / N, bit = at < 0 ? id : at >= row.pieces * N ? at - row.pieces * N : at % N;
             const uint32_t b = 1u << (8 * (byte & 3) + bit);
             twice |= (atomicOr(&s.mask[byte >> 2], b) & b) != 0;
@@ -271,8 +307,7 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
         twice = __any_sync(0xffffffffu, twice);
         __syncwarp();
         l.Z = dt_warp_sum(l.Z);
-        l.A = dt_warp_sum(l.A);
-        l.m = dt_warp_max(l.m);
+        inner.m = dt_warp_max(inner.m);
         const auto first = [&](int k, double* all) {   // whether entry k is the first of its column; P of all the column's entries
             *all = s.P[k];
             if (!twice) return true;
@@ -286,47 +321,51 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
             *all = sum;
             return f;
         };
-        DtSum d{-INFINITY, 0.0f};
-        uint32_t edge_listed = in_head || in_tail ? mask[in_head ? EDGE : EDGE + 1] >> edge_bit & 1u : 1u;
+        DtSum outer{-INFINITY, 0.0f};
+        const uint32_t edge_listed = in_head || in_tail ? mask[in_head ? EDGE : EDGE + 1] >> edge_bit & 1u : 1u;
         if constexpr (GRAD_ONLY) {
             const float4 st = __ldg(reinterpret_cast<const float4*>(a.stats) + r);
-            d.m = st.x, d.s = st.y, l.m = st.z, l.s = (double)st.w;
+            outer = DtSum{st.x, st.y}, inner = DtSum{st.z, st.w};
         } else {
             for (int k = lane; k < a.top; k += 32) {
                 if (s.id[k] < 0) continue;
-                const double x = ((double)s.z[k] - (double)dt_finite_or_zero(l.m)) * inv_t;
                 double all;
+                const double x = ((double)s.z[k] - (double)dt_finite_or_zero(inner.m)) * inv;
                 if (first(k, &all)) l.s += exp(x);
                 if (s.P[k] != 0.0) l.B += s.P[k] * x;
             }
-            l.B = dt_warp_sum(l.B);
+            l.A = dt_warp_sum(l.A), l.B = dt_warp_sum(l.B);
             l.s = dt_warp_sum(l.s);
+            inner.s = (float)l.s, l.m = inner.m;
 #pragma unroll
             for (int j = 0; j < NV; ++j)
                 if (j * 32 + lane < row.pieces) {
                     float x[N];
                     unpack_piece(v[j], x, T());
-                    d.template add<N>(x, mask[j * 32 + lane], c);
+                    outer.template add<N>(x, mask[j * 32 + lane], c);
                 }
-            if (in_head || in_tail) d.template add<1>(&edge, edge_listed, c);
-            d.join_warp(c);
-            if (a.stats && lane == 0) reinterpret_cast<float4*>(a.stats)[r] = make_float4(d.m, d.s, l.m, (float)l.s);
-            const float loss = dt_loss(a, l, d.m, (double)d.s, weight, inv_t);
+            float edge_sum = edge;
+            if (in_head || in_tail) outer.template add<1>(&edge_sum, edge_listed, c);
+            outer.join_warp(c);
+            if (a.stats && lane == 0) reinterpret_cast<float4*>(a.stats)[r] = make_float4(outer.m, outer.s, inner.m, inner.s);
+            const float loss = dt_loss(a, l, outer.m, (double)outer.s, weight, inv);
             if (lane == 0) a.loss[r] = weight == 0.0f ? 0.0f : loss;
         }
-        if (dz) {
-            const DtCoef k = dt_coefficients(a, l.Z, l.m, (float)l.s, d.m, d.s, weight, c);
-            const float outer = weight == 0.0f ? 0.0f : k.outer, base = dt_finite_or_zero(d.m);
+        if (dz && weight == 0.0f) {   // (for the stats alone)
+            __syncwarp();
+            dt_zero_row(dz, a.cols, lane, 32);
+        } else if (dz) {
+            const DtCoef k = dt_coefficients(a, l.Z, inner, outer, weight, c);
+            const float base = dt_finite_or_zero(outer.m);
             T* const dp = dz + row.head;
             const bool whole = (reinterpret_cast<uintptr_t>(dp) & 15) == 0;
 #pragma unroll
             for (int j = 0; j < NV; ++j)
-                if (j * 32 + lane < row.pieces) dt_store(dp + (j * 32 + lane) * N, whole, v[j], mask[j * 32 + lane], base, outer, c);
-            if (!edge_listed) dz[edge_at] = from_f32<T>(outer == 0.0f ? 0.0f : dt_exp2((edge - base) * c) * outer);
+                if (j * 32 + lane < row.pieces) dt_store(dp + (j * 32 + lane) * N, whole, v[j], mask[j * 32 + lane], base, k.outer, c);
+            if (!edge_listed) dz[edge_at] = from_f32<T>(dt_exp2((edge - base) * c) * k.outer);
             for (int i = lane; i < a.top; i += 32) {
                 double all;
-                if (s.id[i] >= 0 && first(i, &all))
-                    dz[s.id[i]] = from_f32<T>(weight == 0.0f ? 0.0f : k.inner * expf((s.z[i] - k.M) / a.temperature) - k.scale * ((float)all * k.p_scale));
+                if (s.id[i] >= 0 && first(i, &all)) dz[s.id[i]] = from_f32<T>(k.inner * expf((s.z[i] - k.M) * inv_t) - k.scale * ((float)all * k.p_scale));
             }
         }
         __syncwarp();
@@ -341,28 +380,30 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
 
 // ---------------------------------------------------------------- longer rows: a cluster of CTAs each
 // Every CTA has an equal run of the row's pieces: the first NV of each thread stay in registers between the sums and the gradient, what a very
-// long row has more is read again.  All CTAs work through the list (a thread an entry), each counts and writes the listed columns of its own run.
-constexpr int DC_THREADS = 512, DC_WARPS = DC_THREADS / 32, DC_LISTERS = DT_TOP / 32, DC_CTAS = 8;
+// long row has more is read again.  All CTAs take the list (a thread an entry) and count and write the listed columns of their own run, in fp32;
+// the first CTA's first warp adds up the loss in 64 bits while the others write the gradient.
+constexpr int DC_THREADS = 256, DC_WARPS = DC_THREADS / 32, DC_CTAS = 8;
+static_assert(DC_THREADS == DT_TOP, "a thread an entry");
 struct DcShared {
-    double P[DT_TOP];
-    double Z[DC_LISTERS], A[DC_LISTERS], B[DC_LISTERS], s_in[DC_LISTERS];
-    float4 peer[2][DC_CTAS];            // m_out, s_out, s_in of the cluster's CTAs, two rows by turns
-    float2 sum[DC_WARPS];               // dense sums of the warps
-    float tmax[DC_LISTERS], zmax[DC_LISTERS];
+    float P[DT_TOP], t[DT_TOP], z[DT_TOP];
     int id[DT_TOP];
+    float4 peer[2][DC_CTAS];            // outer and inner sums of the cluster's CTAs, two rows by turns
+    float2 outer[DC_WARPS], inner[DC_WARPS];
+    double Z[DC_WARPS];
+    float tmax[DC_WARPS];
     uint32_t edge;                      // listed columns of the head (bits 0 to 7) and the tail (8 to 15)
 };
 
 template <typename T, int NV, bool GRAD_ONLY>
-__global__ void __launch_bounds__(DC_THREADS, 2) distill_cluster_kernel(const DtArgs a, int ctas)
+__global__ void __launch_bounds__(DC_THREADS, 3) distill_cluster_kernel(const DtArgs a, int ctas)
 {
     extern __shared__ uint32_t dc_mask[];   // a byte per piece of this CTA
     __shared__ DcShared s;
     constexpr int N = PIECE<T>;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)(blockIdx.x % (unsigned)ctas);
-    const double inv_t = 1.0 / (double)a.temperature;
-    const float c = 1.4426950408889634f / a.temperature;
+    const double inv = 1.0 / (double)a.temperature;
+    const float inv_t = 1.0f / a.temperature, c = 1.4426950408889634f / a.temperature;
     const uint8_t* const mask = reinterpret_cast<const uint8_t*>(dc_mask);
     const int most = (int)((a.cols / N + ctas - 1) / ctas);   // pieces of a CTA, at most
     for (int w = tid; w < (most + 3) / 4; w += DC_THREADS) dc_mask[w] = 0;
@@ -371,25 +412,28 @@ __global__ void __launch_bounds__(DC_THREADS, 2) distill_cluster_kernel(const Dt
     for (int64_t r = blockIdx.x / (unsigned)ctas; r < a.rows; r += gridDim.x / (unsigned)ctas) {
         const T* const z = static_cast<const T*>(a.z) + r * a.ldz;
         T* const dz = a.dz ? static_cast<T*>(a.dz) + r * a.lddz : nullptr;
-        const float weight = a.row_weight ? __ldg(a.row_weight + r) : 1.0f;
+        const float weight = a.row_weight ? __ldg(a.row_weight + r) : 1.0f, t_lse = a.t_lse ? __ldg(a.t_lse + r) : 0.0f;
+        const int id = dt_load_id(a, r, tid);
+        float tv = tid < a.top ? dt_load_t(a, r, tid) : -INFINITY;
+        if (id < 0) tv = -INFINITY;
         const row_pieces<T> row(z, a.cols);
         const int first_piece = rank * most, pieces = max(0, min(most, row.pieces - first_piece));
         const uint4* const zp = reinterpret_cast<const uint4*>(z + row.head) + first_piece;
-        const int id = dt_load_id(a, r, tid);
-        const float tv = id >= 0 ? dt_load_t(a, r, tid) : -INFINITY;
         const bool skip_weight = weight == 0.0f && (GRAD_ONLY || !a.stats);
         uint4 v[NV];
+        if (!skip_weight) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-            if (j * DC_THREADS + tid < pieces && !skip_weight) v[j] = zp[j * DC_THREADS + tid];
-        if (warp < DC_LISTERS) {
+            for (int j = 0; j < NV; ++j)
+                if (j * DC_THREADS + tid < pieces) v[j] = zp[j * DC_THREADS + tid];
+        }
+        {
             const float m = dt_warp_max(tv);
             if (lane == 0) s.tmax[warp] = m;
         }
         const bool some = __syncthreads_or(id >= 0);
         float tmax = s.tmax[0];
 #pragma unroll
-        for (int w = 1; w < DC_LISTERS; ++w) tmax = fmaxf(tmax, s.tmax[w]);
+        for (int w = 1; w < DC_WARPS; ++w) tmax = fmaxf(tmax, s.tmax[w]);
         if (!some || (!a.t_lse && tmax == -INFINITY) || skip_weight) {   // (the same for all CTAs of the row)
             if (!GRAD_ONLY && rank == 0) {
                 if (tid == 0) a.loss[r] = 0.0f;
@@ -404,112 +448,106 @@ __global__ void __launch_bounds__(DC_THREADS, 2) distill_cluster_kernel(const Dt
         const bool edge_entry = id >= 0 && (at < 0 || at >= row.pieces * N);
         const bool mine = edge_entry ? rank == (at < 0 ? 0 : ctas - 1) : id >= 0 && piece >= 0 && piece < pieces;
         uint32_t* const word = edge_entry ? &s.edge : &dc_mask[mine ? piece >> 2 : 0];
-        float zk = -INFINITY;
-        double P = 0.0, lp = 0.0;
+        const float zk = mine || (!GRAD_ONLY && rank == 0 && id >= 0) ? to_f32(z[id]) : -INFINITY;
+        // (in 64 bits: what the list leaves to the others, 1 - Z, may be small)
+        const double P = id >= 0 ? exp(dt_log_p(a, tv, tmax, (double)t_lse, inv)) : 0.0;
         bool twice = false;
-        if (warp < DC_LISTERS) {
-            if (id >= 0) {
-                if (mine || !GRAD_ONLY) zk = to_f32(z[id]);
-                lp = dt_log_p(a, tv, tmax, a.t_lse ? (double)__ldg(a.t_lse + r) : 0.0, inv_t);
-                P = exp(lp);
-            }
-            s.id[tid] = id;
-            s.P[tid] = P;
-            if (mine) {
-                const uint32_t b = 1u << (!edge_entry ? 8 * (piece & 3) + at % N : at < 0 ? id : 8 + at - row.pieces * N);
-                twice = (atomicOr(word, b) & b) != 0;
-            }
-            const float m = dt_warp_max(zk);
-            if (lane == 0) s.zmax[warp] = m;
+        s.id[tid] = id;
+        s.P[tid] = (float)P;
+        s.t[tid] = tv;
+        if (mine) {
+            const uint32_t b = 1u << (!edge_entry ? 8 * (piece & 3) + at % N : at < 0 ? id : 8 + at - row.pieces * N);
+            twice = (atomicOr(word, b) & b) != 0;
+        }
+        {
+            const double Z = dt_warp_sum(P);
+            if (lane == 0) s.Z[warp] = Z;
         }
         bool first = mine;   // the first entry of its column; P of all the column's entries
-        double P_all = P;
+        float P_all = (float)P;
         if (__syncthreads_or(twice) && mine) {
-            P_all = 0.0;
+            P_all = 0.0f;
             for (int k = 0; k < a.top; ++k)
                 if (s.id[k] == id) {
                     P_all += s.P[k];
                     if (k < tid) first = false;
                 }
         }
-        float m_in = s.zmax[0];
-#pragma unroll
-        for (int w = 1; w < DC_LISTERS; ++w) m_in = fmaxf(m_in, s.zmax[w]);
-        if (warp < DC_LISTERS) {
-            const double x = ((double)zk - (double)dt_finite_or_zero(m_in)) * inv_t;
-            const double Z = dt_warp_sum(P);
-            if (lane == 0) s.Z[warp] = Z;
-            if constexpr (!GRAD_ONLY) {
-                const double A = dt_warp_sum(P != 0.0 ? P * lp : 0.0), B = dt_warp_sum(P != 0.0 ? P * x : 0.0), s_in = dt_warp_sum(first ? exp(x) : 0.0);
-                if (lane == 0) s.A[warp] = A, s.B[warp] = B, s.s_in[warp] = s_in;
-            }
-        }
         // the scalar columns: the head's to the first CTA, the tail's to the last
         const bool in_head = rank == 0 && tid < row.head, in_tail = rank == ctas - 1 && tid >= 32 && tid < 32 + row.tail;
         const int edge_at = in_head ? tid : (int)a.cols - row.tail + tid - 32;
         const float edge = in_head || in_tail ? to_f32(z[edge_at]) : -INFINITY;
         const uint32_t edge_listed = in_head ? s.edge >> tid & 1u : in_tail ? s.edge >> (8 + tid - 32) & 1u : 1u;
-        DtSum d{-INFINITY, 0.0f};
-        float s_in;
+        DtSum outer{-INFINITY, 0.0f}, inner{first ? zk : -INFINITY, first ? 1.0f : 0.0f};
         if constexpr (GRAD_ONLY) {
             const float4 st = __ldg(reinterpret_cast<const float4*>(a.stats) + r);
-            d.m = st.x, d.s = st.y, m_in = st.z, s_in = st.w;
-            __syncthreads();
+            outer = DtSum{st.x, st.y}, inner = DtSum{st.z, st.w};
         } else {
+            // (a listed z of -infinity or NaN: 0 and NaN, as exp gives them)
+            if (first && !(zk > -INFINITY)) inner.s = zk == -INFINITY ? 0.0f : NAN;
+            if (zk == INFINITY && first) inner.s = NAN;
+            s.z[tid] = zk;
 #pragma unroll
             for (int j = 0; j < NV; ++j)
                 if (j * DC_THREADS + tid < pieces) {
                     float x[N];
                     unpack_piece(v[j], x, T());
-                    d.template add<N>(x, mask[j * DC_THREADS + tid], c);
+                    outer.template add<N>(x, mask[j * DC_THREADS + tid], c);
                 }
             for (int p = NV * DC_THREADS + tid; p < pieces; p += DC_THREADS) {
                 float x[N];
                 unpack_piece(zp[p], x, T());
-                d.template add<N>(x, mask[p], c);
+                outer.template add<N>(x, mask[p], c);
             }
-            if (in_head || in_tail) d.template add<1>(&edge, edge_listed, c);
-            d.join_warp(c);
-            if (lane == 0) s.sum[warp] = make_float2(d.m, d.s);
+            float edge_sum = edge;
+            if (in_head || in_tail) outer.template add<1>(&edge_sum, edge_listed, c);
+            outer.join_warp(c);
+            inner.join_warp(c);
+            if (lane == 0) s.outer[warp] = make_float2(outer.m, outer.s), s.inner[warp] = make_float2(inner.m, inner.s);
             __syncthreads();
             // (every warp joins the warps' sums for itself)
-            d = lane < DC_WARPS ? DtSum{s.sum[lane].x, s.sum[lane].y} : DtSum{-INFINITY, 0.0f};
-            d.join_warp(c);
-            s_in = (float)dt_warp_sum(lane < DC_LISTERS ? s.s_in[lane] : 0.0);
+            outer = lane < DC_WARPS ? DtSum{s.outer[lane].x, s.outer[lane].y} : DtSum{-INFINITY, 0.0f};
+            inner = lane < DC_WARPS ? DtSum{s.inner[lane].x, s.inner[lane].y} : DtSum{-INFINITY, 0.0f};
+            outer.join_warp(c);
+            inner.join_warp(c);
             if (ctas > 1) {
                 if (warp == 0 && lane < ctas) {
                     uint32_t to;
                     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&s.peer[turn][rank])), "r"(lane));
-                    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %3};" ::"r"(to), "f"(d.m), "f"(d.s), "f"(s_in) : "memory");
+                    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(outer.m), "f"(outer.s), "f"(inner.m), "f"(inner.s) : "memory");
                 }
                 asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-                const float4 o = lane < ctas ? s.peer[turn][lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-                d = DtSum{o.x, o.y};
-                d.join_warp(c);
-                s_in = dt_warp_sum(o.z);
+                const float4 o = lane < ctas ? s.peer[turn][lane] : make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
+                outer = DtSum{o.x, o.y}, inner = DtSum{o.z, o.w};
+                outer.join_warp(c);
+                inner.join_warp(c);
                 turn ^= 1;
             }
+            if (a.stats && rank == 0 && tid == DC_THREADS - 1) reinterpret_cast<float4*>(a.stats)[r] = make_float4(outer.m, outer.s, inner.m, inner.s);
         }
-        const double Z = dt_warp_sum(lane < DC_LISTERS ? s.Z[lane] : 0.0);
-        if (!GRAD_ONLY && rank == 0 && warp == DC_WARPS - 1) {
-            const DtList l{Z, dt_warp_sum(lane < DC_LISTERS ? s.A[lane] : 0.0), dt_warp_sum(lane < DC_LISTERS ? s.B[lane] : 0.0), (double)s_in, m_in};
-            const float loss = dt_loss(a, l, d.m, (double)d.s, weight, inv_t);
-            if (lane == 0) {
-                a.loss[r] = weight == 0.0f ? 0.0f : loss;
-                if (a.stats) reinterpret_cast<float4*>(a.stats)[r] = make_float4(d.m, d.s, m_in, s_in);
-            }
-        }
-        if (dz) {
-            const DtCoef k = dt_coefficients(a, Z, m_in, s_in, d.m, d.s, weight, c);
-            const float outer = weight == 0.0f ? 0.0f : k.outer, base = dt_finite_or_zero(d.m);
+        if (dz && weight == 0.0f) {   // (for the stats alone; the cluster has read the row)
+            if (ctas == 1) __syncthreads();
+            dt_zero_row(dz, a.cols, rank * DC_THREADS + tid, ctas * DC_THREADS);
+        } else if (dz) {
+            const double Z = dt_warp_sum(lane < DC_WARPS ? s.Z[lane] : 0.0);
+            const DtCoef k = dt_coefficients(a, Z, inner, outer, weight, c);
+            const float base = dt_finite_or_zero(outer.m);
             T* const dp = dz + row.head + (int64_t)first_piece * N;
             const bool whole = (reinterpret_cast<uintptr_t>(dp) & 15) == 0;
 #pragma unroll
             for (int j = 0; j < NV; ++j)
-                if (j * DC_THREADS + tid < pieces) dt_store(dp + (j * DC_THREADS + tid) * N, whole, v[j], mask[j * DC_THREADS + tid], base, outer, c);
-            for (int p = NV * DC_THREADS + tid; p < pieces; p += DC_THREADS) dt_store(dp + (int64_t)p * N, whole, zp[p], mask[p], base, outer, c);
-            if (!edge_listed) dz[edge_at] = from_f32<T>(outer == 0.0f ? 0.0f : dt_exp2((edge - base) * c) * outer);
-            if (first) dz[id] = from_f32<T>(weight == 0.0f ? 0.0f : k.inner * expf((zk - k.M) / a.temperature) - k.scale * ((float)P_all * k.p_scale));
+                if (j * DC_THREADS + tid < pieces) dt_store(dp + (j * DC_THREADS + tid) * N, whole, v[j], mask[j * DC_THREADS + tid], base, k.outer, c);
+            for (int p = NV * DC_THREADS + tid; p < pieces; p += DC_THREADS) dt_store(dp + (int64_t)p * N, whole, zp[p], mask[p], base, k.outer, c);
+            if (!edge_listed) dz[edge_at] = from_f32<T>(dt_exp2((edge - base) * c) * k.outer);
+            if (first) dz[id] = from_f32<T>(k.inner * expf((zk - k.M) * inv_t) - k.scale * (P_all * k.p_scale));
+        }
+        if (!GRAD_ONLY && rank == 0 && warp == 0) {
+            DtList l{0.0, 0.0, 0.0, (double)inner.s, inner.m};
+            for (int k = lane; k < a.top; k += 32)
+                if (s.id[k] >= 0) dt_count(a, l, s.t[k], tmax, (double)t_lse, s.z[k], inv);
+            l.Z = dt_warp_sum(l.Z), l.A = dt_warp_sum(l.A), l.B = dt_warp_sum(l.B);
+            const float loss = dt_loss(a, l, outer.m, (double)outer.s, weight, inv);
+            if (lane == 0) a.loss[r] = weight == 0.0f ? 0.0f : loss;
         }
         __syncthreads();
         if (mine) *word = 0;   // (a whole word, by each of its entries)
