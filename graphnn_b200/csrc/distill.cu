@@ -12,7 +12,7 @@ namespace
 {
 
 constexpr int DT_TOP = 256;            // most entries of a list
-constexpr int64_t DT_COLS = 1 << 20;   // most columns
+constexpr int64_t DT_ROW_BYTES = 1536 << 10;   // a row fits the shared memory of 8 CTAs
 constexpr int DT_SITE = 7;             // status word: a class outside the row
 
 struct DtArgs {
@@ -52,58 +52,119 @@ __device__ __forceinline__ float dt_warp_max(float v)
 }
 
 // ---------------------------------------------------------------- sums and gradients of pieces of 16 bytes
-// e[i] = exp2((x[i] + minus_m) * c), two at a time
-template <int N> __device__ __forceinline__ void dt_exps(const float* x, float minus_m, float c, float* e)
+__device__ __forceinline__ uint64_t dt_two(float a, float b)
 {
-    if constexpr (N == 1) {
-        e[0] = dt_exp2((x[0] + minus_m) * c);
-    } else {
-        uint64_t m2, c2;
-        asm("mov.b64 %0, {%1, %1};" : "=l"(m2) : "f"(minus_m));
-        asm("mov.b64 %0, {%1, %1};" : "=l"(c2) : "f"(c));
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ void dt_halves(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t dt_add2(uint64_t a, uint64_t b)
+{
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ uint64_t dt_mul2(uint64_t a, uint64_t b)
+{
+    uint64_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+// exp2((x + minus_m) * c) of two numbers
+__device__ __forceinline__ uint64_t dt_exp_two(float x0, float x1, uint64_t minus_m, uint64_t c)
+{
+    float a, b;
+    dt_halves(dt_mul2(dt_add2(dt_two(x0, x1), minus_m), c), a, b);
+    return dt_two(dt_exp2(a), dt_exp2(b));
+}
+
+// The largest elements of pieces, lane by lane of the register; then of a register's own.  (NaN loses here and shows in the sums.)
+__device__ __forceinline__ uint32_t dt_max_word(uint32_t a, uint32_t b, float) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+__device__ __forceinline__ uint32_t dt_max_word(uint32_t a, uint32_t b, __half)
+{
+    const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t dt_max_word(uint32_t a, uint32_t b, __nv_bfloat16)
+{
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+template <typename T> __device__ __forceinline__ uint32_t dt_max_piece(const uint4& v) { return dt_max_word(dt_max_word(v.x, v.y, T()), dt_max_word(v.z, v.w, T()), T()); }
+__device__ __forceinline__ float dt_max_of_word(uint32_t a, float) { return __uint_as_float(a); }
+__device__ __forceinline__ float dt_max_of_word(uint32_t a, __half) { return fmaxf(__half2float(__ushort_as_half((unsigned short)a)), __half2float(__ushort_as_half((unsigned short)(a >> 16)))); }
+__device__ __forceinline__ float dt_max_of_word(uint32_t a, __nv_bfloat16) { return fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u)); }
+template <typename T> __device__ __forceinline__ uint32_t dt_lowest()   // a register of -infinity
+{
+    return sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+}
+// -infinity in the place of the listed elements
+template <typename T> __device__ __forceinline__ void dt_take_out(uint4& v, uint32_t listed)
+{
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            uint64_t v;
-            asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x[i]), "f"(x[i + 1]));
-            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(m2));
-            asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(c2));
-            asm("mov.b64 {%0, %1}, %2;" : "=f"(e[i]), "=f"(e[i + 1]) : "l"(v));
-            e[i] = dt_exp2(e[i]);
-            e[i + 1] = dt_exp2(e[i + 1]);
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            if (listed >> i & 1) w[i] = dt_lowest<T>();
+        } else {
+            if (listed >> (2 * i) & 1) w[i] = (w[i] & 0xffff0000u) | (dt_lowest<T>() & 0xffffu);
+            if (listed >> (2 * i + 1) & 1) w[i] = (w[i] & 0xffffu) | (dt_lowest<T>() & 0xffff0000u);
         }
     }
+    v = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 struct DtSum {   // of exp((z - m) / T), relative to the largest z
     float m, s;
-    // (x is overwritten where columns are listed: few pieces have any)
-    template <int N> __device__ __forceinline__ void add(float* x, uint32_t listed, float c)
+    __device__ __forceinline__ void reach(float top, float c)
     {
-        if (listed) {
-#pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (listed >> e & 1) x[e] = -INFINITY;
-        }
-        float top = x[0];
-#pragma unroll
-        for (int e = 1; e < N; ++e) top = fmaxf(top, x[e]);
         if (top > m) {
             s *= dt_exp2((m - top) * c);   // (m = -infinity: no sum yet)
             m = top;
         }
-        float e[N];
-        dt_exps<N>(x, -dt_finite_or_zero(m), c, e);
-#pragma unroll
-        for (int w = N / 2; w; w >>= 1)
-#pragma unroll
-            for (int i = 0; i < w; ++i) e[i] += e[i + w];
-        s += e[0];
     }
-    __device__ __forceinline__ void join_warp(float c)
+    template <typename T> __device__ __forceinline__ void add_piece(const uint4& v, uint64_t minus_m, uint64_t c, uint64_t& sum)   // (m is reached)
     {
-        const float top = dt_warp_max(m);
-        s = dt_warp_sum(s * dt_exp2((m - dt_finite_or_zero(top)) * c));
+        constexpr int N = PIECE<T>;
+        float x[N];
+        unpack_piece(v, x, T());
+#pragma unroll
+        for (int i = 0; i < N; i += 2) sum = dt_add2(sum, dt_exp_two(x[i], x[i + 1], minus_m, c));
+    }
+    // pieces in registers, one of their own at a time for the others (`n` of them in all)
+    template <typename T, int NV> __device__ __forceinline__ void add_pieces(const uint4 (&v)[NV], int at, int step, int n, float c)
+    {
+        uint32_t top = dt_lowest<T>();
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * step + at < n) top = dt_max_word(top, dt_max_piece<T>(v[j]), T());
+        reach(dt_max_of_word(top, T()), c);
+        const float base = -dt_finite_or_zero(m);
+        const uint64_t base2 = dt_two(base, base), c2 = dt_two(c, c);
+        uint64_t sum[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * step + at < n) add_piece<T>(v[j], base2, c2, sum[j & 1]);
+        float a, b;
+        dt_halves(dt_add2(sum[0], sum[1]), a, b);
+        s += a + b;
+    }
+    __device__ __forceinline__ void add_one(float x, float c)
+    {
+        reach(x, c);
+        s += dt_exp2((x - dt_finite_or_zero(m)) * c);
+    }
+    // joined over groups of LANES lanes
+    template <int LANES> __device__ __forceinline__ void join(float c)
+    {
+        float top = m;
+#pragma unroll
+        for (int o = LANES / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        s *= dt_exp2((m - dt_finite_or_zero(top)) * c);
         m = top;
+#pragma unroll
+        for (int o = LANES / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     }
 };
 
@@ -118,14 +179,13 @@ template <typename T> __device__ __forceinline__ void dt_zero_row(T* dz, int64_t
 }
 
 // gradient of a piece; listed columns are written by their entries
-template <typename T> __device__ __forceinline__ void dt_store(T* to, bool whole, const uint4& v, uint32_t listed, float base, float outer, float c)
+template <typename T> __device__ __forceinline__ void dt_store(T* to, bool whole, const uint4& v, uint32_t listed, uint64_t minus_m, uint64_t outer, uint64_t c)
 {
     constexpr int N = PIECE<T>;
     float x[N], e[N];
     unpack_piece(v, x, T());
-    dt_exps<N>(x, -base, c, e);
 #pragma unroll
-    for (int i = 0; i < N; ++i) e[i] *= outer;
+    for (int i = 0; i < N; i += 2) dt_halves(dt_mul2(dt_exp_two(x[i], x[i + 1], minus_m, c), outer), e[i], e[i + 1]);
     if (whole && listed == 0) {
         __stcs(reinterpret_cast<uint4*>(to), pack_piece(e, T()));
     } else {
@@ -181,7 +241,7 @@ struct DtCoef {
     float outer;        // any other's: outer * exp((z - m_out) / T)
     float scale;        // row_weight / T
 };
-__device__ __forceinline__ DtCoef dt_coefficients(const DtArgs& a, double Z, const DtSum& in, const DtSum& out, float weight, float c)
+__device__ __forceinline__ DtCoef dt_coefficients(const DtArgs& a, double Z, const DtSum& in, const DtSum& out, float weight, float inv_t, float c)
 {
     DtCoef k;
     const float m = fmaxf(in.m, out.m);
@@ -198,10 +258,10 @@ __device__ __forceinline__ DtCoef dt_coefficients(const DtArgs& a, double Z, con
         rest = 0.0f;
         k.p_scale = 1.0f / (float)Z;
     }
-    k.scale = weight / a.temperature;
-    const float both = (given + rest) / total;
+    k.scale = weight * inv_t;
+    const float both = __fdividef(given + rest, total);
     k.inner = k.scale * both;
-    k.outer = k.scale * (out.s == 0.0f && total == total ? 0.0f : both * e_out - rest / out.s);
+    k.outer = k.scale * (out.s == 0.0f && total == total ? 0.0f : both * e_out - __fdividef(rest, out.s));
     return k;
 }
 __device__ __forceinline__ float dt_loss(const DtArgs& a, const DtList& l, float m_out, double s_out, float weight, double inv_t)
@@ -339,14 +399,11 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
             inner.s = (float)l.s, l.m = inner.m;
 #pragma unroll
             for (int j = 0; j < NV; ++j)
-                if (j * 32 + lane < row.pieces) {
-                    float x[N];
-                    unpack_piece(v[j], x, T());
-                    outer.template add<N>(x, mask[j * 32 + lane], c);
-                }
-            float edge_sum = edge;
-            if (in_head || in_tail) outer.template add<1>(&edge_sum, edge_listed, c);
-            outer.join_warp(c);
+                if (j * 32 + lane < row.pieces)
+                    if (const uint32_t listed = mask[j * 32 + lane]) dt_take_out<T>(v[j], listed);
+            outer.template add_pieces<T, NV>(v, lane, 32, row.pieces, c);
+            if (!edge_listed) outer.add_one(edge, c);
+            outer.template join<32>(c);
             if (a.stats && lane == 0) reinterpret_cast<float4*>(a.stats)[r] = make_float4(outer.m, outer.s, inner.m, inner.s);
             const float loss = dt_loss(a, l, outer.m, (double)outer.s, weight, inv);
             if (lane == 0) a.loss[r] = weight == 0.0f ? 0.0f : loss;
@@ -355,13 +412,13 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
             __syncwarp();
             dt_zero_row(dz, a.cols, lane, 32);
         } else if (dz) {
-            const DtCoef k = dt_coefficients(a, l.Z, inner, outer, weight, c);
+            const DtCoef k = dt_coefficients(a, l.Z, inner, outer, weight, inv_t, c);
             const float base = dt_finite_or_zero(outer.m);
             T* const dp = dz + row.head;
             const bool whole = (reinterpret_cast<uintptr_t>(dp) & 15) == 0;
 #pragma unroll
             for (int j = 0; j < NV; ++j)
-                if (j * 32 + lane < row.pieces) dt_store(dp + (j * 32 + lane) * N, whole, v[j], mask[j * 32 + lane], base, k.outer, c);
+                if (j * 32 + lane < row.pieces) dt_store(dp + (j * 32 + lane) * N, whole, v[j], mask[j * 32 + lane], dt_two(-base, -base), dt_two(k.outer, k.outer), dt_two(c, c));
             if (!edge_listed) dz[edge_at] = from_f32<T>(dt_exp2((edge - base) * c) * k.outer);
             for (int i = lane; i < a.top; i += 32) {
                 double all;
@@ -379,199 +436,297 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
 }
 
 // ---------------------------------------------------------------- longer rows: a cluster of CTAs each
-// Every CTA has an equal run of the row's pieces: the first NV of each thread stay in registers between the sums and the gradient, what a very
-// long row has more is read again.  All CTAs take the list (a thread an entry) and count and write the listed columns of their own run, in fp32;
-// the first CTA's first warp adds up the loss in 64 bits while the others write the gradient.
+// Every CTA has an equal run of the row's pieces, which lies in shared memory between the sums and the gradient: the row is read once, while the
+// list is worked through.  Listed columns of the run become -infinity there, so that the loops over it know nothing of them; their gradients are
+// written over what those loops wrote.  The first CTA's first warp adds up the loss while the others write the gradient.
 constexpr int DC_THREADS = 256, DC_WARPS = DC_THREADS / 32, DC_CTAS = 8;
-static_assert(DC_THREADS == DT_TOP, "a thread an entry");
+constexpr int DC_RUN = 64 << 10, DC_RUN_MOST = 192 << 10;   // bytes of a run: three CTAs an SM; one
+static_assert(DC_THREADS == DT_TOP && DC_WARPS == 8 && DC_CTAS == 8, "a thread an entry; the joins go over 8 lanes");
 struct DcShared {
     float P[DT_TOP], t[DT_TOP], z[DT_TOP];
-    int id[DT_TOP];
-    float4 peer[2][DC_CTAS];            // outer and inner sums of the cluster's CTAs, two rows by turns
+    alignas(16) int id[DT_TOP];
+    float4 peer[2][DC_CTAS];   // outer and inner sums of the cluster's CTAs, two rows by turns
     float2 outer[DC_WARPS], inner[DC_WARPS];
     double Z[DC_WARPS];
     float tmax[DC_WARPS];
-    uint32_t edge;                      // listed columns of the head (bits 0 to 7) and the tail (8 to 15)
 };
 
-template <typename T, int NV, bool GRAD_ONLY>
-__global__ void __launch_bounds__(DC_THREADS, 3) distill_cluster_kernel(const DtArgs a, int ctas)
+// What every thread with an entry knows of it, before z is looked at.  All threads of the CTA come here.
+struct DcEntry {
+    int id;
+    float t, tmax, P_all;   // P of all the column's entries
+    bool some, first;       // whether the row's list has any entry; whether this is the first of its column
+};
+__device__ __forceinline__ DcEntry dc_entry(const DtArgs& a, int64_t r, float t_lse, double inv, DcShared& s)
 {
-    extern __shared__ uint32_t dc_mask[];   // a byte per piece of this CTA
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const bool lister = warp * 32 < a.top;   // warps with entries
+    DcEntry e{-1, -INFINITY, -INFINITY, 0.0f, false, false};
+    if (lister) {
+        if (tid < a.top) {
+            e.id = dt_load_id(a, r, tid);
+            e.t = dt_load_t(a, r, tid);
+            if (e.id < 0) e.t = -INFINITY;
+        }
+        s.id[tid] = e.id;
+        s.t[tid] = e.t;
+        const float m = dt_warp_max(e.t);
+        if (lane == 0) s.tmax[warp] = m;
+    }
+    e.some = __syncthreads_or(e.id >= 0);
+    for (int w = 0; w * 32 < a.top; ++w) e.tmax = fmaxf(e.tmax, s.tmax[w]);
+    if (lister) {
+        // (in 64 bits: what the list leaves to the others, 1 - Z, may be small)
+        const double P = e.id >= 0 ? exp(dt_log_p(a, e.t, e.tmax, (double)t_lse, inv)) : 0.0;
+        e.P_all = (float)P;
+        s.P[tid] = e.P_all;
+        const double Z = dt_warp_sum(P);
+        if (lane == 0) s.Z[warp] = Z;
+        int before = 0, same = 0;   // entries of the same column
+        for (int k = 0; k < a.top; k += 4) {
+            const int4 o = *reinterpret_cast<const int4*>(s.id + k);   // (a list warp has written all of its 32)
+            same += (o.x == e.id) + (o.y == e.id) + (o.z == e.id) + (o.w == e.id);
+            if (k <= tid) before += (o.x == e.id && k < tid) + (o.y == e.id && k + 1 < tid) + (o.z == e.id && k + 2 < tid) + (o.w == e.id && k + 3 < tid);
+        }
+        e.first = e.id >= 0 && before == 0;
+        if (e.first && same > 1) {   // (rare: P of the others)
+            e.P_all = 0.0f;
+            for (int k = 0; k < a.top; ++k)
+                if (s.id[k] == e.id) e.P_all += (float)exp(dt_log_p(a, s.t[k], e.tmax, (double)t_lse, inv));
+        }
+    }
+    return e;
+}
+__device__ __forceinline__ double dc_Z(const DtArgs& a, const DcShared& s)
+{
+    double Z = 0.0;
+    for (int w = 0; w * 32 < a.top; ++w) Z += s.Z[w];
+    return Z;
+}
+__device__ __forceinline__ bool dc_skipped(const DtArgs& a, const DcEntry& e) { return !e.some || (!a.t_lse && e.tmax == -INFINITY); }
+
+// where a CTA's run lies
+template <typename T> struct DcRun {
+    row_pieces<T> row;
+    int first, pieces;   // pieces of the run
+    __device__ __forceinline__ DcRun(const T* z, int64_t cols, int rank, int ctas) : row(z, cols)
+    {
+        const int most = (int)((cols / PIECE<T> + ctas - 1) / ctas);
+        first = rank * most;
+        pieces = max(0, min(most, row.pieces - first));
+    }
+    // whether a column belongs to this CTA (the head to the first, the tail to the last), and its place among the run's elements, or -1 (head, tail)
+    __device__ __forceinline__ bool has(int id, int rank, int ctas, int& at) const
+    {
+        const int e = id - row.head;
+        at = -1;
+        if (id < 0) return false;
+        if (e < 0) return rank == 0;
+        if (e >= row.pieces * PIECE<T>) return rank == ctas - 1;
+        at = e - first * PIECE<T>;
+        return at >= 0 && at < pieces * PIECE<T>;
+    }
+};
+
+template <typename T> __global__ void __launch_bounds__(DC_THREADS, 3) distill_cluster_kernel(const DtArgs a, int ctas)
+{
+    extern __shared__ __align__(16) unsigned char dc_run[];
     __shared__ DcShared s;
+    uint4* const run = reinterpret_cast<uint4*>(dc_run);
     constexpr int N = PIECE<T>;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)(blockIdx.x % (unsigned)ctas);
     const double inv = 1.0 / (double)a.temperature;
     const float inv_t = 1.0f / a.temperature, c = 1.4426950408889634f / a.temperature;
-    const uint8_t* const mask = reinterpret_cast<const uint8_t*>(dc_mask);
-    const int most = (int)((a.cols / N + ctas - 1) / ctas);   // pieces of a CTA, at most
-    for (int w = tid; w < (most + 3) / 4; w += DC_THREADS) dc_mask[w] = 0;
-    if (tid == 0) s.edge = 0;
+    if (tid < DC_WARPS) s.inner[tid] = make_float2(-INFINITY, 0.0f);   // (of the warps without entries, once and for all)
     int turn = 0;
     for (int64_t r = blockIdx.x / (unsigned)ctas; r < a.rows; r += gridDim.x / (unsigned)ctas) {
         const T* const z = static_cast<const T*>(a.z) + r * a.ldz;
         T* const dz = a.dz ? static_cast<T*>(a.dz) + r * a.lddz : nullptr;
         const float weight = a.row_weight ? __ldg(a.row_weight + r) : 1.0f, t_lse = a.t_lse ? __ldg(a.t_lse + r) : 0.0f;
-        const int id = dt_load_id(a, r, tid);
-        float tv = tid < a.top ? dt_load_t(a, r, tid) : -INFINITY;
-        if (id < 0) tv = -INFINITY;
-        const row_pieces<T> row(z, a.cols);
-        const int first_piece = rank * most, pieces = max(0, min(most, row.pieces - first_piece));
-        const uint4* const zp = reinterpret_cast<const uint4*>(z + row.head) + first_piece;
-        const bool skip_weight = weight == 0.0f && (GRAD_ONLY || !a.stats);
-        uint4 v[NV];
+        const DcRun<T> my(z, a.cols, rank, ctas);
+        const bool skip_weight = weight == 0.0f && !a.stats;
         if (!skip_weight) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-                if (j * DC_THREADS + tid < pieces) v[j] = zp[j * DC_THREADS + tid];
+            const uint4* const zp = reinterpret_cast<const uint4*>(z + my.row.head) + my.first;
+            for (int p = tid; p < my.pieces; p += DC_THREADS)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(run + p)), "l"(zp + p) : "memory");
         }
-        {
-            const float m = dt_warp_max(tv);
-            if (lane == 0) s.tmax[warp] = m;
-        }
-        const bool some = __syncthreads_or(id >= 0);
-        float tmax = s.tmax[0];
-#pragma unroll
-        for (int w = 1; w < DC_WARPS; ++w) tmax = fmaxf(tmax, s.tmax[w]);
-        if (!some || (!a.t_lse && tmax == -INFINITY) || skip_weight) {   // (the same for all CTAs of the row)
-            if (!GRAD_ONLY && rank == 0) {
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        const DcEntry e = dc_entry(a, r, t_lse, inv, s);
+        if (skip_weight || dc_skipped(a, e)) {   // (the same for all CTAs of the row)
+            if (rank == 0) {
                 if (tid == 0) a.loss[r] = 0.0f;
                 if (a.stats && tid < 4) a.stats[4 * r + tid] = 0.0f;
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncthreads();   // (dz may be z)
             if (dz) dt_zero_row(dz, a.cols, rank * DC_THREADS + tid, ctas * DC_THREADS);
-            __syncthreads();
             continue;
         }
-        // the list: a thread an entry
-        const int at = id - row.head, piece = at < 0 ? -1 : at / N - first_piece;   // (of this CTA's)
-        const bool edge_entry = id >= 0 && (at < 0 || at >= row.pieces * N);
-        const bool mine = edge_entry ? rank == (at < 0 ? 0 : ctas - 1) : id >= 0 && piece >= 0 && piece < pieces;
-        uint32_t* const word = edge_entry ? &s.edge : &dc_mask[mine ? piece >> 2 : 0];
-        const float zk = mine || (!GRAD_ONLY && rank == 0 && id >= 0) ? to_f32(z[id]) : -INFINITY;
-        // (in 64 bits: what the list leaves to the others, 1 - Z, may be small)
-        const double P = id >= 0 ? exp(dt_log_p(a, tv, tmax, (double)t_lse, inv)) : 0.0;
-        bool twice = false;
-        s.id[tid] = id;
-        s.P[tid] = (float)P;
-        s.t[tid] = tv;
-        if (mine) {
-            const uint32_t b = 1u << (!edge_entry ? 8 * (piece & 3) + at % N : at < 0 ? id : 8 + at - row.pieces * N);
-            twice = (atomicOr(word, b) & b) != 0;
-        }
-        {
-            const double Z = dt_warp_sum(P);
-            if (lane == 0) s.Z[warp] = Z;
-        }
-        bool first = mine;   // the first entry of its column; P of all the column's entries
-        float P_all = (float)P;
-        if (__syncthreads_or(twice) && mine) {
-            P_all = 0.0f;
-            for (int k = 0; k < a.top; ++k)
-                if (s.id[k] == id) {
-                    P_all += s.P[k];
-                    if (k < tid) first = false;
-                }
-        }
+        int at;
+        const bool mine = my.has(e.id, rank, ctas, at) && e.first;
+        float zk = (mine && at < 0) || (rank == 0 && e.id >= 0) ? to_f32(z[e.id]) : -INFINITY;
         // the scalar columns: the head's to the first CTA, the tail's to the last
-        const bool in_head = rank == 0 && tid < row.head, in_tail = rank == ctas - 1 && tid >= 32 && tid < 32 + row.tail;
-        const int edge_at = in_head ? tid : (int)a.cols - row.tail + tid - 32;
+        const bool in_head = rank == 0 && tid < my.row.head, in_tail = rank == ctas - 1 && tid >= 32 && tid < 32 + my.row.tail;
+        const int edge_at = in_head ? tid : (int)a.cols - my.row.tail + tid - 32;
         const float edge = in_head || in_tail ? to_f32(z[edge_at]) : -INFINITY;
-        const uint32_t edge_listed = in_head ? s.edge >> tid & 1u : in_tail ? s.edge >> (8 + tid - 32) & 1u : 1u;
-        DtSum outer{-INFINITY, 0.0f}, inner{first ? zk : -INFINITY, first ? 1.0f : 0.0f};
-        if constexpr (GRAD_ONLY) {
-            const float4 st = __ldg(reinterpret_cast<const float4*>(a.stats) + r);
-            outer = DtSum{st.x, st.y}, inner = DtSum{st.z, st.w};
-        } else {
-            // (a listed z of -infinity or NaN: 0 and NaN, as exp gives them)
-            if (first && !(zk > -INFINITY)) inner.s = zk == -INFINITY ? 0.0f : NAN;
-            if (zk == INFINITY && first) inner.s = NAN;
-            s.z[tid] = zk;
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-                if (j * DC_THREADS + tid < pieces) {
-                    float x[N];
-                    unpack_piece(v[j], x, T());
-                    outer.template add<N>(x, mask[j * DC_THREADS + tid], c);
-                }
-            for (int p = NV * DC_THREADS + tid; p < pieces; p += DC_THREADS) {
-                float x[N];
-                unpack_piece(zp[p], x, T());
-                outer.template add<N>(x, mask[p], c);
-            }
-            float edge_sum = edge;
-            if (in_head || in_tail) outer.template add<1>(&edge_sum, edge_listed, c);
-            outer.join_warp(c);
-            inner.join_warp(c);
-            if (lane == 0) s.outer[warp] = make_float2(outer.m, outer.s), s.inner[warp] = make_float2(inner.m, inner.s);
-            __syncthreads();
-            // (every warp joins the warps' sums for itself)
-            outer = lane < DC_WARPS ? DtSum{s.outer[lane].x, s.outer[lane].y} : DtSum{-INFINITY, 0.0f};
-            inner = lane < DC_WARPS ? DtSum{s.inner[lane].x, s.inner[lane].y} : DtSum{-INFINITY, 0.0f};
-            outer.join_warp(c);
-            inner.join_warp(c);
-            if (ctas > 1) {
-                if (warp == 0 && lane < ctas) {
-                    uint32_t to;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&s.peer[turn][rank])), "r"(lane));
-                    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(outer.m), "f"(outer.s), "f"(inner.m), "f"(inner.s) : "memory");
-                }
-                asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-                const float4 o = lane < ctas ? s.peer[turn][lane] : make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
-                outer = DtSum{o.x, o.y}, inner = DtSum{o.z, o.w};
-                outer.join_warp(c);
-                inner.join_warp(c);
-                turn ^= 1;
-            }
-            if (a.stats && rank == 0 && tid == DC_THREADS - 1) reinterpret_cast<float4*>(a.stats)[r] = make_float4(outer.m, outer.s, inner.m, inner.s);
+        bool edge_out = in_head || in_tail;   // not listed
+        if (edge_out)
+            for (int k = 0; k < a.top; ++k) edge_out &= s.id[k] != edge_at;
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();
+        if (mine && at >= 0) {   // (one thread an element)
+            T* const held = reinterpret_cast<T*>(run) + at;
+            zk = to_f32(*held);
+            *held = from_f32<T>(-INFINITY);
         }
+        DtSum outer{-INFINITY, 0.0f}, inner{-INFINITY, 0.0f};
+        if (warp * 32 < a.top) {
+            s.z[tid] = zk;
+            // (a listed z of -infinity adds nothing, +infinity and NaN make the sum NaN)
+            if (mine) inner = DtSum{zk, zk < INFINITY ? zk > -INFINITY ? 1.0f : 0.0f : NAN};
+            inner.template join<32>(c);
+            if (lane == 0) s.inner[warp] = make_float2(inner.m, inner.s);
+        }
+        __syncthreads();
+        for (int p = tid; p < my.pieces; p += 4 * DC_THREADS) {
+            uint4 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (p + j * DC_THREADS < my.pieces) v[j] = run[p + j * DC_THREADS];
+            outer.template add_pieces<T, 4>(v, p, DC_THREADS, my.pieces, c);
+        }
+        if (edge_out) outer.add_one(edge, c);
+        outer.template join<32>(c);
+        if (lane == 0) s.outer[warp] = make_float2(outer.m, outer.s);
+        __syncthreads();
+        if (warp == 0) {   // the CTA's sums: lanes 0 to 7 the outer ones, 8 to 15 the inner ones (and again)
+            const float2 o = (lane & 8 ? s.inner : s.outer)[lane & 7];
+            DtSum d{o.x, o.y};
+            d.template join<8>(c);
+            const float m_in = __shfl_sync(0xffffffffu, d.m, 8), s_in = __shfl_sync(0xffffffffu, d.s, 8);
+            if (lane < ctas) {
+                uint32_t to;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&s.peer[turn][rank])), "r"(lane));
+                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(d.m), "f"(d.s), "f"(m_in), "f"(s_in) : "memory");
+            }
+            __syncwarp();
+        }
+        if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        else __syncthreads();
+        {
+            const float4 o = (lane & 7) < ctas ? s.peer[turn][lane & 7] : make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
+            DtSum d = lane & 8 ? DtSum{o.z, o.w} : DtSum{o.x, o.y};
+            d.template join<8>(c);
+            outer = DtSum{__shfl_sync(0xffffffffu, d.m, 0), __shfl_sync(0xffffffffu, d.s, 0)};
+            inner = DtSum{__shfl_sync(0xffffffffu, d.m, 8), __shfl_sync(0xffffffffu, d.s, 8)};
+        }
+        turn ^= 1;
+        if (a.stats && rank == 0 && tid == DC_THREADS - 1) reinterpret_cast<float4*>(a.stats)[r] = make_float4(outer.m, outer.s, inner.m, inner.s);
         if (dz && weight == 0.0f) {   // (for the stats alone; the cluster has read the row)
-            if (ctas == 1) __syncthreads();
             dt_zero_row(dz, a.cols, rank * DC_THREADS + tid, ctas * DC_THREADS);
         } else if (dz) {
-            const double Z = dt_warp_sum(lane < DC_WARPS ? s.Z[lane] : 0.0);
-            const DtCoef k = dt_coefficients(a, Z, inner, outer, weight, c);
+            const DtCoef k = dt_coefficients(a, dc_Z(a, s), inner, outer, weight, inv_t, c);
             const float base = dt_finite_or_zero(outer.m);
-            T* const dp = dz + row.head + (int64_t)first_piece * N;
-            const bool whole = (reinterpret_cast<uintptr_t>(dp) & 15) == 0;
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-                if (j * DC_THREADS + tid < pieces) dt_store(dp + (j * DC_THREADS + tid) * N, whole, v[j], mask[j * DC_THREADS + tid], base, k.outer, c);
-            for (int p = NV * DC_THREADS + tid; p < pieces; p += DC_THREADS) dt_store(dp + (int64_t)p * N, whole, zp[p], mask[p], base, k.outer, c);
-            if (!edge_listed) dz[edge_at] = from_f32<T>(dt_exp2((edge - base) * c) * k.outer);
-            if (first) dz[id] = from_f32<T>(k.inner * expf((zk - k.M) * inv_t) - k.scale * (P_all * k.p_scale));
+            const uint64_t base2 = dt_two(-base, -base), outer2 = dt_two(k.outer, k.outer), c2 = dt_two(c, c);
+            T* const dp = dz + my.row.head + (int64_t)my.first * N;
+            if ((reinterpret_cast<uintptr_t>(dp) & 15) == 0) {
+#pragma unroll 4
+                for (int p = tid; p < my.pieces; p += DC_THREADS) dt_store(dp + p * N, true, run[p], 0u, base2, outer2, c2);
+            } else {
+                for (int p = tid; p < my.pieces; p += DC_THREADS) dt_store(dp + p * N, false, run[p], 0u, base2, outer2, c2);
+            }
+            if (edge_out) dz[edge_at] = from_f32<T>(dt_exp2((edge - base) * c) * k.outer);
+            __syncthreads();   // the listed columns have been written as the others
+            if (mine) dz[e.id] = from_f32<T>(k.inner * expf((zk - k.M) * inv_t) - k.scale * (e.P_all * k.p_scale));
         }
-        if (!GRAD_ONLY && rank == 0 && warp == 0) {
+        if (rank == 0 && warp == 0) {
             DtList l{0.0, 0.0, 0.0, (double)inner.s, inner.m};
             for (int k = lane; k < a.top; k += 32)
-                if (s.id[k] >= 0) dt_count(a, l, s.t[k], tmax, (double)t_lse, s.z[k], inv);
+                if (s.id[k] >= 0) dt_count(a, l, s.t[k], e.tmax, (double)t_lse, s.z[k], inv);
             l.Z = dt_warp_sum(l.Z), l.A = dt_warp_sum(l.A), l.B = dt_warp_sum(l.B);
             const float loss = dt_loss(a, l, outer.m, (double)outer.s, weight, inv);
             if (lane == 0) a.loss[r] = weight == 0.0f ? 0.0f : loss;
         }
         __syncthreads();
-        if (mine) *word = 0;   // (a whole word, by each of its entries)
     }
 }
 
-template <typename T, int NV, bool GRAD_ONLY> int dc_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a, int ctas)
+// The gradient from kept sums: nothing to wait for but the list.
+template <typename T> __global__ void __launch_bounds__(DC_THREADS) distill_grad_kernel(const DtArgs a, int ctas)
 {
-    const int64_t most = (a.cols / PIECE<T> + ctas - 1) / ctas;
-    int64_t rows = a.rows;
-    if (rows > (1 << 20)) rows = 1 << 20;   // (clusters; further rows in turns)
+    __shared__ DcShared s;
+    constexpr int N = PIECE<T>;
+    const int tid = threadIdx.x;
+    const int rank = (int)(blockIdx.x % (unsigned)ctas);
+    const double inv = 1.0 / (double)a.temperature;
+    const float inv_t = 1.0f / a.temperature, c = 1.4426950408889634f / a.temperature;
+    for (int64_t r = blockIdx.x / (unsigned)ctas; r < a.rows; r += gridDim.x / (unsigned)ctas) {
+        const T* const z = static_cast<const T*>(a.z) + r * a.ldz;
+        T* const dz = static_cast<T*>(a.dz) + r * a.lddz;
+        const float weight = a.row_weight ? __ldg(a.row_weight + r) : 1.0f, t_lse = a.t_lse ? __ldg(a.t_lse + r) : 0.0f;
+        const float4 st = __ldg(reinterpret_cast<const float4*>(a.stats) + r);
+        const DcRun<T> my(z, a.cols, rank, ctas);
+        const DcEntry e = dc_entry(a, r, t_lse, inv, s);
+        int at;
+        const bool mine = my.has(e.id, rank, ctas, at) && e.first;
+        const float zk = mine ? to_f32(z[e.id]) : 0.0f;
+        const bool in_head = rank == 0 && tid < my.row.head, in_tail = rank == ctas - 1 && tid >= 32 && tid < 32 + my.row.tail;
+        const int edge_at = in_head ? tid : (int)a.cols - my.row.tail + tid - 32;
+        const float edge = in_head || in_tail ? to_f32(z[edge_at]) : 0.0f;
+        __syncthreads();   // every listed z has been read (dz may be z)
+        if (weight == 0.0f || dc_skipped(a, e)) {
+            dt_zero_row(dz, a.cols, rank * DC_THREADS + tid, ctas * DC_THREADS);
+            __syncthreads();
+            continue;
+        }
+        const DtSum outer{st.x, st.y}, inner{st.z, st.w};
+        const DtCoef k = dt_coefficients(a, dc_Z(a, s), inner, outer, weight, inv_t, c);
+        const float base = dt_finite_or_zero(outer.m);
+        const uint64_t base2 = dt_two(-base, -base), outer2 = dt_two(k.outer, k.outer), c2 = dt_two(c, c);
+        const uint4* const zp = reinterpret_cast<const uint4*>(z + my.row.head) + my.first;
+        T* const dp = dz + my.row.head + (int64_t)my.first * N;
+        const bool whole = (reinterpret_cast<uintptr_t>(dp) & 15) == 0;
+        for (int p = tid; p < my.pieces; p += 4 * DC_THREADS) {
+            uint4 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (p + j * DC_THREADS < my.pieces) v[j] = zp[p + j * DC_THREADS];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (p + j * DC_THREADS < my.pieces) dt_store(dp + (p + j * DC_THREADS) * N, whole, v[j], 0u, base2, outer2, c2);
+        }
+        if (in_head || in_tail) dz[edge_at] = from_f32<T>(dt_exp2((edge - base) * c) * k.outer);
+        __syncthreads();   // the listed columns have been written as the others
+        if (mine) dz[e.id] = from_f32<T>(k.inner * expf((zk - k.M) * inv_t) - k.scale * (e.P_all * k.p_scale));
+        __syncthreads();
+    }
+}
+
+template <typename T> int dc_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a, int ctas)
+{
+    const int64_t most = (a.cols / PIECE<T> + ctas - 1) / ctas, rows = a.rows < (1 << 20) ? a.rows : 1 << 20;   // (clusters; further rows by turns)
+    S2V_CUDA_OK(ctx, s2v_allow_shared(distill_cluster_kernel<T>, DC_RUN_MOST));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * ctas));
     cfg.blockDim = dim3(DC_THREADS);
-    cfg.dynamicSmemBytes = (size_t)((most + 3) / 4 * 4);
+    cfg.dynamicSmemBytes = (size_t)most * 16;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)ctas;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = GRAD_ONLY ? 0 : 1;
-    S2V_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, distill_cluster_kernel<T, NV, GRAD_ONLY>, a, ctas));
+    cfg.numAttrs = 1;
+    S2V_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, distill_cluster_kernel<T>, a, ctas));
     S2V_CHECK_LAUNCH(ctx, "distill_cluster_kernel");
+    return S2V_OK;
+}
+template <typename T> int dg_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a, int ctas)
+{
+    const int64_t rows = a.rows < (1 << 20) ? a.rows : 1 << 20;
+    distill_grad_kernel<T><<<(unsigned)(rows * ctas), DC_THREADS, 0, st>>>(a, ctas);
+    S2V_CHECK_LAUNCH(ctx, "distill_grad_kernel");
     return S2V_OK;
 }
 template <typename T, int NV, bool GRAD_ONLY> int dw_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a)
@@ -590,11 +745,8 @@ template <typename T, bool GRAD_ONLY> int dt_launch_type(s2v_ctx* ctx, cudaStrea
     if (pieces <= 32) return dw_launch<T, 1, GRAD_ONLY>(ctx, st, a);
     if (pieces <= 32 * DW_PIECES) return dw_launch<T, DW_PIECES, GRAD_ONLY>(ctx, st, a);
     int ctas = 1;
-    while (ctas < DC_CTAS && (pieces > (int64_t)ctas * 8 * DC_THREADS || (a.rows * ctas < 2 * ctx->sm_count && pieces >= (int64_t)ctas * 2 * DC_THREADS))) ctas *= 2;
-    const int64_t most = (pieces + ctas - 1) / ctas;
-    if (most <= 2 * DC_THREADS) return dc_launch<T, 2, GRAD_ONLY>(ctx, st, a, ctas);
-    if (most <= 4 * DC_THREADS) return dc_launch<T, 4, GRAD_ONLY>(ctx, st, a, ctas);
-    return dc_launch<T, 8, GRAD_ONLY>(ctx, st, a, ctas);
+    while (ctas < DC_CTAS && (pieces * 16 > (int64_t)ctas * DC_RUN || (a.rows * ctas < 2 * ctx->sm_count && pieces >= (int64_t)ctas * 2 * DC_THREADS))) ctas *= 2;
+    return GRAD_ONLY ? dg_launch<T>(ctx, st, a, ctas) : dc_launch<T>(ctx, st, a, ctas);
 }
 int dt_launch(s2v_ctx* ctx, s2v_stream stream, int z_type, bool grad_only, const DtArgs& a)
 {
@@ -614,7 +766,7 @@ int dt_check(s2v_ctx* ctx, const char* name, int z_type, const DtArgs& a)
     if (a.rows == 0) return S2V_OK;
     if (!a.z || !a.idx || !a.t) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": NULL pointer");
     if (a.top > DT_TOP) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, who + ": more than 256 entries a row");
-    if (a.cols > DT_COLS) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, who + ": more than 1,048,576 columns");
+    if (a.cols * (int64_t)s2v_dtype_bytes(z_type) > DT_ROW_BYTES) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, who + ": rows of more than 1,572,864 bytes");
     if (a.rows > 1 && (a.ldz < a.cols || a.ldt < a.top || (a.dz && a.lddz < a.cols)))
         return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": leading dimension below the number of columns");
     const size_t es = s2v_dtype_bytes(z_type);

@@ -348,7 +348,7 @@ def test_refusals(gpu_ctx):
     for got, want in [(call(rows=-1), -1), (call(cols=0), -1), (call(top=0), -1), (call(zt=3), -1), (call(tt=-1), -1), (call(z=None), -1), (call(idx=None), -1), (call(t=None), -1),
                       (call(loss=None), -1), (call(ldz=9), -1), (call(lddz=9), -1), (call(ldt=2), -1), (call(temp=0.0), -1), (call(temp=-1.0), -1), (call(temp=INF), -1),
                       (call(temp=float("nan")), -1), (call(temp=1e-35), -1), (call(z=p + 2), -1), (call(dz=p + 2), -1), (call(t=p + 1, tt=1), -1), (call(dz=p, lddz=11), -1),
-                      (call(top=257, ldt=257), -2), (call(cols=(1 << 20) + 1, ldz=1 << 21, lddz=1 << 21), -2),
+                      (call(top=257, ldt=257), -2), (call(cols=393217, ldz=1 << 20, lddz=1 << 20), -2), (call(cols=786433, zt=1, ldz=1 << 20, lddz=1 << 20), -2),
                       (grad(stats=None), -1), (grad(dz=None), -1), (grad(temp=0.0), -1), (grad(ldz=9), -1), (grad(rows=-1), -1), (grad(cols=0), -1)]:
         assert got == want, lib.s2v_last_error(h)
     assert call(rows=0, z=None) == 0 and grad(rows=0) == 0
