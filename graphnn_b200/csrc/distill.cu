@@ -12,7 +12,7 @@ namespace
 {
 
 constexpr int DT_TOP = 256;            // most entries of a list
-constexpr int64_t DT_ROW_BYTES = 1536 << 10;   // a row fits the shared memory of 8 CTAs
+constexpr int64_t DT_ROW_BYTES = 1536 << 10;   // longest rows
 constexpr int DT_SITE = 7;             // status word: a class outside the row
 
 struct DtArgs {
@@ -28,6 +28,8 @@ struct DtArgs {
     s2v_device_status* status;
     float temperature;
     int top, t_type;
+    double inv;       // 1 / temperature
+    float inv_t, c;   // the same; log2 e / temperature
 };
 
 __device__ __forceinline__ float dt_exp2(float x)
@@ -178,20 +180,19 @@ template <typename T> __device__ __forceinline__ void dt_zero_row(T* dz, int64_t
     for (int p = at; p < row.pieces; p += threads) to[p] = make_uint4(0, 0, 0, 0);
 }
 
-// gradient of a piece; listed columns are written by their entries
-template <typename T> __device__ __forceinline__ void dt_store(T* to, bool whole, const uint4& v, uint32_t listed, uint64_t minus_m, uint64_t outer, uint64_t c)
+// gradient of a piece; what is listed of it is written over by its entry
+template <typename T> __device__ __forceinline__ void dt_store(T* to, bool whole, const uint4& v, uint64_t minus_m, uint64_t outer, uint64_t c)
 {
     constexpr int N = PIECE<T>;
     float x[N], e[N];
     unpack_piece(v, x, T());
 #pragma unroll
     for (int i = 0; i < N; i += 2) dt_halves(dt_mul2(dt_exp_two(x[i], x[i + 1], minus_m, c), outer), e[i], e[i + 1]);
-    if (whole && listed == 0) {
+    if (whole) {
         __stcs(reinterpret_cast<uint4*>(to), pack_piece(e, T()));
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (!(listed >> i & 1)) to[i] = from_f32<T>(e[i]);
+        for (int i = 0; i < N; ++i) to[i] = from_f32<T>(e[i]);
     }
 }
 
@@ -264,30 +265,27 @@ __device__ __forceinline__ DtCoef dt_coefficients(const DtArgs& a, double Z, con
     k.outer = k.scale * (out.s == 0.0f && total == total ? 0.0f : both * e_out - __fdividef(rest, out.s));
     return k;
 }
-__device__ __forceinline__ float dt_loss(const DtArgs& a, const DtList& l, float m_out, double s_out, float weight, double inv_t)
+// (A warp's work, all lanes with the same arguments: its logarithms are taken side by side in three lanes.)
+__device__ __forceinline__ float dt_loss(const DtArgs& a, const DtList& l, const DtSum& out, float weight, double inv_t, float c)
 {
-    const float mf = fmaxf(l.m, m_out);
-    if (mf == -INFINITY) return NAN;
-    const double M = (double)mf;
-    const double total = (l.s == 0.0 ? 0.0 : l.s * exp(((double)l.m - M) * inv_t)) + (s_out == 0.0 ? 0.0 : s_out * exp(((double)m_out - M) * inv_t));
-    const double lse = log(total);   // above M / T
+    const float mf = fmaxf(l.m, out.m), M = dt_finite_or_zero(mf);
+    const double in_part = l.s == 0.0 ? 0.0 : l.s * (double)dt_exp2((l.m - M) * c), out_part = out.s == 0.0f ? 0.0 : (double)out.s * (double)dt_exp2((out.m - M) * c);
+    const double total = in_part + out_part;   // at least one, where there is a finite z
+    const double rest = !a.t_lse || l.Z > 1.0 ? 0.0 : 1.0 - l.Z;
+    const double odds = in_part / out_part;    // of the list against the others: log s = -log(1 + odds)
+    const int lane = threadIdx.x & 31;
+    const double log1 = log1p(lane == 0 ? total - 1.0 : lane == 1 ? odds : a.t_lse ? -l.Z : l.Z - 1.0);
+    const double lse = __shfl_sync(0xffffffffu, log1, 0), log_z = __shfl_sync(0xffffffffu, log1, 2);
+    double minus_log_s = __shfl_sync(0xffffffffu, log1, 1);
     // sum of p (log p - log q), log q = (z - M) / T - lse; B is relative to l.m
-    const double from = l.m == -INFINITY ? 0.0 : ((double)l.m - M) * inv_t;
-    double kl, rest = 0.0;
-    if (a.t_lse) {
-        kl = l.A - (l.B + l.Z * from) + l.Z * lse;
-        rest = l.Z > 1.0 ? 0.0 : 1.0 - l.Z;
-    } else {
-        kl = (l.A - (l.B + l.Z * from)) / l.Z - log(l.Z) + lse;
-    }
+    const double from = l.m == -INFINITY ? 0.0 : ((double)l.m - (double)M) * inv_t, B = l.B + l.Z * from;
+    double kl = a.t_lse ? l.A - B + l.Z * lse : (l.A - B) / l.Z - log_z + lse;
     if (rest != 0.0) {
-        if (s_out != 0.0) {
-            const double d = l.s == 0.0 ? -INFINITY : log(l.s / s_out) + ((double)l.m - (double)m_out) * inv_t;
-            kl += rest * (log1p(-l.Z) + (d > 0.0 ? d + log1p(exp(-d)) : log1p(exp(d))));
-        } else if (rest > 1.0 / 65536.0) {
-            kl = INFINITY;
-        }
+        if (!(odds < 1e30)) minus_log_s = log(l.s / (double)out.s) + ((double)l.m - (double)out.m) * inv_t;   // (too far apart for fp32; 1 / odds is nothing)
+        if (out.s != 0.0f) kl += rest * (log_z + minus_log_s);
+        else if (rest > 1.0 / 65536.0) kl = INFINITY;
     }
+    if (mf == -INFINITY) kl = NAN;
     return (float)(kl * weight);
 }
 
@@ -308,8 +306,8 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
     DwShared& s = shared[threadIdx.x >> 5];
     constexpr int N = PIECE<T>, EDGE = DW_PIECES * 32;   // mask bytes of the head and the tail: EDGE, EDGE + 1
     const int lane = threadIdx.x & 31;
-    const double inv = 1.0 / (double)a.temperature;
-    const float inv_t = 1.0f / a.temperature, c = 1.4426950408889634f / a.temperature;
+    const double inv = a.inv;
+    const float inv_t = a.inv_t, c = a.c;
     const uint8_t* const mask = reinterpret_cast<const uint8_t*>(s.mask);
     for (int w = lane; w < (int)(sizeof(s.mask) / 4); w += 32) s.mask[w] = 0;
     __syncwarp();
@@ -405,7 +403,7 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
             if (!edge_listed) outer.add_one(edge, c);
             outer.template join<32>(c);
             if (a.stats && lane == 0) reinterpret_cast<float4*>(a.stats)[r] = make_float4(outer.m, outer.s, inner.m, inner.s);
-            const float loss = dt_loss(a, l, outer.m, (double)outer.s, weight, inv);
+            const float loss = dt_loss(a, l, outer, weight, inv, c);
             if (lane == 0) a.loss[r] = weight == 0.0f ? 0.0f : loss;
         }
         if (dz && weight == 0.0f) {   // (for the stats alone)
@@ -418,8 +416,9 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
             const bool whole = (reinterpret_cast<uintptr_t>(dp) & 15) == 0;
 #pragma unroll
             for (int j = 0; j < NV; ++j)
-                if (j * 32 + lane < row.pieces) dt_store(dp + (j * 32 + lane) * N, whole, v[j], mask[j * 32 + lane], dt_two(-base, -base), dt_two(k.outer, k.outer), dt_two(c, c));
+                if (j * 32 + lane < row.pieces) dt_store(dp + (j * 32 + lane) * N, whole, v[j], dt_two(-base, -base), dt_two(k.outer, k.outer), dt_two(c, c));
             if (!edge_listed) dz[edge_at] = from_f32<T>(dt_exp2((edge - base) * c) * k.outer);
+            __syncwarp();   // the listed columns have been written as the others
             for (int i = lane; i < a.top; i += 32) {
                 double all;
                 if (s.id[i] >= 0 && first(i, &all)) dz[s.id[i]] = from_f32<T>(k.inner * expf((s.z[i] - k.M) * inv_t) - k.scale * ((float)all * k.p_scale));
@@ -435,75 +434,99 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
     }
 }
 
-// ---------------------------------------------------------------- longer rows: a cluster of CTAs each
-// Every CTA has an equal run of the row's pieces, which lies in shared memory between the sums and the gradient: the row is read once, while the
-// list is worked through.  Listed columns of the run become -infinity there, so that the loops over it know nothing of them; their gradients are
-// written over what those loops wrote.  The first CTA's first warp adds up the loss while the others write the gradient.
-constexpr int DC_THREADS = 256, DC_WARPS = DC_THREADS / 32, DC_CTAS = 8;
-constexpr int DC_RUN = 64 << 10, DC_RUN_MOST = 192 << 10;   // bytes of a run: three CTAs an SM; one
-static_assert(DC_THREADS == DT_TOP && DC_WARPS == 8 && DC_CTAS == 8, "a thread an entry; the joins go over 8 lanes");
+// ---------------------------------------------------------------- longer rows: a CTA or a cluster of CTAs each
+// Every CTA has an equal run of the row's pieces.  The first DC_HELD of them lie in shared memory between the sums and the gradient, the others are
+// read once more, from L2: two CTAs an SM, so that one moves data while the other joins sums or waits.  Listed columns become -infinity in shared
+// memory; the others' are named by a byte per piece.  Their gradients are written over what the loops over the run wrote.  The first CTA's first
+// warp adds up the loss while the others write the gradient.
+constexpr int DC_THREADS = 512, DC_WARPS = DC_THREADS / 32, DC_CTAS = 8, DC_LISTERS = DT_TOP / 32;
+constexpr int DC_SMEM = 104 << 10;                   // bytes of a CTA's pieces and marks
+constexpr int DC_HELD = 5600, DC_RUN = 16384;        // pieces held, and of a run, at most
+static_assert(DC_HELD * 16 + (DC_RUN - DC_HELD) <= DC_SMEM, "a byte for each piece that is not held");
+constexpr int DC_SLOTS = 512;                        // of the table that finds columns listed twice
 struct DcShared {
     float P[DT_TOP], t[DT_TOP], z[DT_TOP];
-    alignas(16) int id[DT_TOP];
+    int id[DT_TOP], slot[DC_SLOTS];
     float4 peer[2][DC_CTAS];   // outer and inner sums of the cluster's CTAs, two rows by turns
-    float2 outer[DC_WARPS], inner[DC_WARPS];
-    double Z[DC_WARPS];
-    float tmax[DC_WARPS];
+    float2 outer[DC_WARPS], inner[DC_LISTERS];
+    float Z[DC_LISTERS], tmax[DC_LISTERS];
+    int has[DC_LISTERS];       // bit 0: an entry; bit 1: a column that is listed twice
 };
 
-// What every thread with an entry knows of it, before z is looked at.  All threads of the CTA come here.
-struct DcEntry {
+// what a row's threads load first: their entry, the row's weight and normaliser
+struct DcHead {
     int id;
-    float t, tmax, P_all;   // P of all the column's entries
-    bool some, first;       // whether the row's list has any entry; whether this is the first of its column
+    float t, weight, t_lse;
+    __device__ __forceinline__ DcHead(const DtArgs& a, int64_t r) : id(-1), t(-INFINITY)
+    {
+        weight = a.row_weight ? __ldg(a.row_weight + r) : 1.0f;
+        t_lse = a.t_lse ? __ldg(a.t_lse + r) : 0.0f;
+        if (threadIdx.x < a.top) {
+            id = dt_load_id(a, r, threadIdx.x);
+            t = dt_load_t(a, r, threadIdx.x);
+        }
+    }
 };
-__device__ __forceinline__ DcEntry dc_entry(const DtArgs& a, int64_t r, float t_lse, double inv, DcShared& s)
+// What every thread with an entry knows of it, before z is looked at.  P in fp32: the gradient's rest, 1 - sum P, is off by 2^-23 at most.
+struct DcEntry {
+    float t, tmax, P;
+    int slot;     // its column's place in the table
+    bool twice;   // whether another entry of this column was there first
+};
+__device__ __forceinline__ DcEntry dc_entry(const DtArgs& a, const DcHead& h, DcShared& s)
 {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const bool lister = warp * 32 < a.top;   // warps with entries
-    DcEntry e{-1, -INFINITY, -INFINITY, 0.0f, false, false};
-    if (lister) {
-        if (tid < a.top) {
-            e.id = dt_load_id(a, r, tid);
-            e.t = dt_load_t(a, r, tid);
-            if (e.id < 0) e.t = -INFINITY;
+    DcEntry e{h.id >= 0 ? h.t : -INFINITY, -INFINITY, 0.0f, 0, false};
+    if (!a.t_lse) {
+        if (lister) {
+            const float m = dt_warp_max(e.t);
+            if (lane == 0) s.tmax[warp] = m;
         }
-        s.id[tid] = e.id;
-        s.t[tid] = e.t;
-        const float m = dt_warp_max(e.t);
-        if (lane == 0) s.tmax[warp] = m;
+        __syncthreads();
+        for (int w = 0; w * 32 < a.top; ++w) e.tmax = fmaxf(e.tmax, s.tmax[w]);
     }
-    e.some = __syncthreads_or(e.id >= 0);
-    for (int w = 0; w * 32 < a.top; ++w) e.tmax = fmaxf(e.tmax, s.tmax[w]);
     if (lister) {
-        // (in 64 bits: what the list leaves to the others, 1 - Z, may be small)
-        const double P = e.id >= 0 ? exp(dt_log_p(a, e.t, e.tmax, (double)t_lse, inv)) : 0.0;
-        e.P_all = (float)P;
-        s.P[tid] = e.P_all;
-        const double Z = dt_warp_sum(P);
-        if (lane == 0) s.Z[warp] = Z;
-        int before = 0, same = 0;   // entries of the same column
-        for (int k = 0; k < a.top; k += 4) {
-            const int4 o = *reinterpret_cast<const int4*>(s.id + k);   // (a list warp has written all of its 32)
-            same += (o.x == e.id) + (o.y == e.id) + (o.z == e.id) + (o.w == e.id);
-            if (k <= tid) before += (o.x == e.id && k < tid) + (o.y == e.id && k + 1 < tid) + (o.z == e.id && k + 2 < tid) + (o.w == e.id && k + 3 < tid);
+        if (h.id >= 0) {
+            e.P = expf(a.t_lse ? e.t * a.inv_t - h.t_lse : (e.t - dt_finite_or_zero(e.tmax)) * a.inv_t);
+            int was;
+            for (e.slot = h.id & (DC_SLOTS - 1); (was = atomicCAS(&s.slot[e.slot], -1, h.id)) != -1 && was != h.id; e.slot = (e.slot + 1) & (DC_SLOTS - 1)) {}
+            e.twice = was == h.id;
         }
-        e.first = e.id >= 0 && before == 0;
-        if (e.first && same > 1) {   // (rare: P of the others)
-            e.P_all = 0.0f;
-            for (int k = 0; k < a.top; ++k)
-                if (s.id[k] == e.id) e.P_all += (float)exp(dt_log_p(a, s.t[k], e.tmax, (double)t_lse, inv));
-        }
+        s.id[tid] = h.id;
+        s.t[tid] = e.t;
+        s.P[tid] = e.P;
+        const float Z = dt_warp_sum(e.P);
+        const int has = (__any_sync(0xffffffffu, h.id >= 0) ? 1 : 0) | (__any_sync(0xffffffffu, e.twice) ? 2 : 0);
+        if (lane == 0) s.Z[warp] = Z, s.has[warp] = has;
     }
     return e;
 }
-__device__ __forceinline__ double dc_Z(const DtArgs& a, const DcShared& s)
+// (after a barrier) bit 0: the row's list has an entry that counts; bit 1: a column is listed twice
+__device__ __forceinline__ int dc_has(const DtArgs& a, const DcEntry& e, const DcShared& s)
 {
-    double Z = 0.0;
+    int has = 0;
+    for (int w = 0; w * 32 < a.top; ++w) has |= s.has[w];
+    return !a.t_lse && e.tmax == -INFINITY ? has & 2 : has;
+}
+// Where some column is listed twice: whether an entry is the first of its column; P of all of the column's.
+__device__ __forceinline__ bool dc_first(const DtArgs& a, int id, const DcShared& s, float& P)
+{
+    bool first = true;
+    P = 0.0f;
+    for (int k = 0; k < a.top; ++k)
+        if (s.id[k] == id) {
+            P += s.P[k];
+            if (k < (int)threadIdx.x) first = false;
+        }
+    return first;
+}
+__device__ __forceinline__ float dc_Z(const DtArgs& a, const DcShared& s)
+{
+    float Z = 0.0f;
     for (int w = 0; w * 32 < a.top; ++w) Z += s.Z[w];
     return Z;
 }
-__device__ __forceinline__ bool dc_skipped(const DtArgs& a, const DcEntry& e) { return !e.some || (!a.t_lse && e.tmax == -INFINITY); }
 
 // where a CTA's run lies
 template <typename T> struct DcRun {
@@ -528,59 +551,82 @@ template <typename T> struct DcRun {
     }
 };
 
-template <typename T> __global__ void __launch_bounds__(DC_THREADS, 3) distill_cluster_kernel(const DtArgs a, int ctas)
+template <typename T> __global__ void __launch_bounds__(DC_THREADS, 2) distill_cluster_kernel(const DtArgs a, int ctas, int held)
 {
-    extern __shared__ __align__(16) unsigned char dc_run[];
+    extern __shared__ __align__(16) unsigned char dc_raw[];
     __shared__ DcShared s;
-    uint4* const run = reinterpret_cast<uint4*>(dc_run);
     constexpr int N = PIECE<T>;
+    uint4* const run = reinterpret_cast<uint4*>(dc_raw);
+    uint32_t* const marks = reinterpret_cast<uint32_t*>(run + held);           // a byte for each piece behind the held ones
+    const uint8_t* const mark = reinterpret_cast<const uint8_t*>(marks) - held;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)(blockIdx.x % (unsigned)ctas);
-    const double inv = 1.0 / (double)a.temperature;
-    const float inv_t = 1.0f / a.temperature, c = 1.4426950408889634f / a.temperature;
-    if (tid < DC_WARPS) s.inner[tid] = make_float2(-INFINITY, 0.0f);   // (of the warps without entries, once and for all)
+    const double inv = a.inv;
+    const float inv_t = a.inv_t, c = a.c;
+    const int most = (int)((a.cols / N + ctas - 1) / ctas);
+    for (int w = tid; w < (most - held + 3) / 4; w += DC_THREADS) marks[w] = 0;
+    for (int w = tid; w < DC_SLOTS; w += DC_THREADS) s.slot[w] = -1;
+    if (tid < DC_LISTERS) s.inner[tid] = make_float2(-INFINITY, 0.0f);   // (of the warps without entries, once and for all)
     int turn = 0;
     for (int64_t r = blockIdx.x / (unsigned)ctas; r < a.rows; r += gridDim.x / (unsigned)ctas) {
         const T* const z = static_cast<const T*>(a.z) + r * a.ldz;
         T* const dz = a.dz ? static_cast<T*>(a.dz) + r * a.lddz : nullptr;
-        const float weight = a.row_weight ? __ldg(a.row_weight + r) : 1.0f, t_lse = a.t_lse ? __ldg(a.t_lse + r) : 0.0f;
+        const DcHead head(a, r);
+        const float weight = head.weight;
         const DcRun<T> my(z, a.cols, rank, ctas);
+        const uint4* const zp = reinterpret_cast<const uint4*>(z + my.row.head) + my.first;
         const bool skip_weight = weight == 0.0f && !a.stats;
-        if (!skip_weight) {
-            const uint4* const zp = reinterpret_cast<const uint4*>(z + my.row.head) + my.first;
-            for (int p = tid; p < my.pieces; p += DC_THREADS)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(run + p)), "l"(zp + p) : "memory");
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        const DcEntry e = dc_entry(a, r, t_lse, inv, s);
-        if (skip_weight || dc_skipped(a, e)) {   // (the same for all CTAs of the row)
+        const int kept = min(held, my.pieces);
+        if (!skip_weight)
+            for (int p = tid; p < kept; p += DC_THREADS) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(run + p)), "l"(zp + p) : "memory");
+        const DcEntry e = dc_entry(a, head, s);
+        int at;
+        const bool here = my.has(head.id, rank, ctas, at), held_entry = here && at >= 0 && at < held * N;
+        bool mine = here && !e.twice;
+        float P_all = e.P, zk = (here && !held_entry) || (rank == 0 && head.id >= 0) ? to_f32(z[head.id]) : -INFINITY;
+        if (here && at >= held * N) atomicOr(&marks[(at / N - held) >> 2], 1u << (8 * ((at / N - held) & 3) + at % N));
+        // the scalar columns: the head's to the first CTA, the tail's to the last
+        const bool in_head = rank == 0 && tid < my.row.head, in_tail = rank == ctas - 1 && tid >= 32 && tid < 32 + my.row.tail;
+        const int edge_at = in_head ? tid : (int)a.cols - my.row.tail + tid - 32;
+        const float edge = in_head || in_tail ? to_f32(z[edge_at]) : -INFINITY;
+        __syncthreads();
+        const int has = dc_has(a, e, s);
+        if (skip_weight || !(has & 1)) {   // (the same for all CTAs of the row)
             if (rank == 0) {
                 if (tid == 0) a.loss[r] = 0.0f;
                 if (a.stats && tid < 4) a.stats[4 * r + tid] = 0.0f;
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             __syncthreads();   // (dz may be z)
+            if (head.id >= 0) s.slot[e.slot] = -1;
+            if (here && at >= held * N) marks[(at / N - held) >> 2] = 0;
             if (dz) dt_zero_row(dz, a.cols, rank * DC_THREADS + tid, ctas * DC_THREADS);
             continue;
         }
-        int at;
-        const bool mine = my.has(e.id, rank, ctas, at) && e.first;
-        float zk = (mine && at < 0) || (rank == 0 && e.id >= 0) ? to_f32(z[e.id]) : -INFINITY;
-        // the scalar columns: the head's to the first CTA, the tail's to the last
-        const bool in_head = rank == 0 && tid < my.row.head, in_tail = rank == ctas - 1 && tid >= 32 && tid < 32 + my.row.tail;
-        const int edge_at = in_head ? tid : (int)a.cols - my.row.tail + tid - 32;
-        const float edge = in_head || in_tail ? to_f32(z[edge_at]) : -INFINITY;
         bool edge_out = in_head || in_tail;   // not listed
         if (edge_out)
             for (int k = 0; k < a.top; ++k) edge_out &= s.id[k] != edge_at;
+        if ((has & 2) && here) mine = dc_first(a, head.id, s, P_all);
+        DtSum outer{-INFINITY, 0.0f}, inner{-INFINITY, 0.0f};
+        // what is not held, while the rest is on its way
+        for (int p = held + tid; p < my.pieces; p += 4 * DC_THREADS) {
+            uint4 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (p + j * DC_THREADS < my.pieces) v[j] = zp[p + j * DC_THREADS];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (p + j * DC_THREADS < my.pieces)
+                    if (const uint32_t listed = mark[p + j * DC_THREADS]) dt_take_out<T>(v[j], listed);
+            outer.template add_pieces<T, 4>(v, p, DC_THREADS, my.pieces, c);
+        }
         asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();
-        if (mine && at >= 0) {   // (one thread an element)
-            T* const held = reinterpret_cast<T*>(run) + at;
-            zk = to_f32(*held);
-            *held = from_f32<T>(-INFINITY);
+        if (mine && held_entry) {   // (one thread an element)
+            T* const element = reinterpret_cast<T*>(run) + at;
+            zk = to_f32(*element);
+            *element = from_f32<T>(-INFINITY);
         }
-        DtSum outer{-INFINITY, 0.0f}, inner{-INFINITY, 0.0f};
         if (warp * 32 < a.top) {
             s.z[tid] = zk;
             // (a listed z of -infinity adds nothing, +infinity and NaN make the sum NaN)
@@ -589,22 +635,22 @@ template <typename T> __global__ void __launch_bounds__(DC_THREADS, 3) distill_c
             if (lane == 0) s.inner[warp] = make_float2(inner.m, inner.s);
         }
         __syncthreads();
-        for (int p = tid; p < my.pieces; p += 4 * DC_THREADS) {
+        for (int p = tid; p < kept; p += 4 * DC_THREADS) {
             uint4 v[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (p + j * DC_THREADS < my.pieces) v[j] = run[p + j * DC_THREADS];
-            outer.template add_pieces<T, 4>(v, p, DC_THREADS, my.pieces, c);
+                if (p + j * DC_THREADS < kept) v[j] = run[p + j * DC_THREADS];
+            outer.template add_pieces<T, 4>(v, p, DC_THREADS, kept, c);
         }
         if (edge_out) outer.add_one(edge, c);
         outer.template join<32>(c);
         if (lane == 0) s.outer[warp] = make_float2(outer.m, outer.s);
         __syncthreads();
-        if (warp == 0) {   // the CTA's sums: lanes 0 to 7 the outer ones, 8 to 15 the inner ones (and again)
-            const float2 o = (lane & 8 ? s.inner : s.outer)[lane & 7];
+        if (warp == 0) {   // the CTA's sums: lanes 0 to 15 the outer ones, 16 to 23 the inner ones
+            const float2 o = lane < DC_WARPS ? s.outer[lane] : lane >= 16 && lane < 16 + DC_LISTERS ? s.inner[lane - 16] : make_float2(-INFINITY, 0.0f);
             DtSum d{o.x, o.y};
-            d.template join<8>(c);
-            const float m_in = __shfl_sync(0xffffffffu, d.m, 8), s_in = __shfl_sync(0xffffffffu, d.s, 8);
+            d.template join<16>(c);
+            const float m_in = __shfl_sync(0xffffffffu, d.m, 16), s_in = __shfl_sync(0xffffffffu, d.s, 16);
             if (lane < ctas) {
                 uint32_t to;
                 asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&s.peer[turn][rank])), "r"(lane));
@@ -630,52 +676,71 @@ template <typename T> __global__ void __launch_bounds__(DC_THREADS, 3) distill_c
             const float base = dt_finite_or_zero(outer.m);
             const uint64_t base2 = dt_two(-base, -base), outer2 = dt_two(k.outer, k.outer), c2 = dt_two(c, c);
             T* const dp = dz + my.row.head + (int64_t)my.first * N;
-            if ((reinterpret_cast<uintptr_t>(dp) & 15) == 0) {
+            const bool whole = (reinterpret_cast<uintptr_t>(dp) & 15) == 0;
+            for (int p = held + tid; p < my.pieces; p += 4 * DC_THREADS) {
+                uint4 v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (p + j * DC_THREADS < my.pieces) v[j] = zp[p + j * DC_THREADS];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (p + j * DC_THREADS < my.pieces) dt_store(dp + (p + j * DC_THREADS) * N, whole, v[j], base2, outer2, c2);
+            }
+            if (whole) {
 #pragma unroll 4
-                for (int p = tid; p < my.pieces; p += DC_THREADS) dt_store(dp + p * N, true, run[p], 0u, base2, outer2, c2);
+                for (int p = tid; p < kept; p += DC_THREADS) dt_store(dp + p * N, true, run[p], base2, outer2, c2);
             } else {
-                for (int p = tid; p < my.pieces; p += DC_THREADS) dt_store(dp + p * N, false, run[p], 0u, base2, outer2, c2);
+                for (int p = tid; p < kept; p += DC_THREADS) dt_store(dp + p * N, false, run[p], base2, outer2, c2);
             }
             if (edge_out) dz[edge_at] = from_f32<T>(dt_exp2((edge - base) * c) * k.outer);
             __syncthreads();   // the listed columns have been written as the others
-            if (mine) dz[e.id] = from_f32<T>(k.inner * expf((zk - k.M) * inv_t) - k.scale * (e.P_all * k.p_scale));
+            if (mine) dz[head.id] = from_f32<T>(k.inner * expf((zk - k.M) * inv_t) - k.scale * (P_all * k.p_scale));
         }
         if (rank == 0 && warp == 0) {
             DtList l{0.0, 0.0, 0.0, (double)inner.s, inner.m};
             for (int k = lane; k < a.top; k += 32)
-                if (s.id[k] >= 0) dt_count(a, l, s.t[k], e.tmax, (double)t_lse, s.z[k], inv);
+                if (s.id[k] >= 0) dt_count(a, l, s.t[k], e.tmax, (double)head.t_lse, s.z[k], inv);
             l.Z = dt_warp_sum(l.Z), l.A = dt_warp_sum(l.A), l.B = dt_warp_sum(l.B);
-            const float loss = dt_loss(a, l, outer.m, (double)outer.s, weight, inv);
+            const float loss = dt_loss(a, l, outer, weight, inv, c);
             if (lane == 0) a.loss[r] = weight == 0.0f ? 0.0f : loss;
         }
         __syncthreads();
+        if (head.id >= 0) s.slot[e.slot] = -1;
+        if (here && at >= held * N) marks[(at / N - held) >> 2] = 0;   // (a whole word, by each of its entries)
     }
 }
 
 // The gradient from kept sums: nothing to wait for but the list.
-template <typename T> __global__ void __launch_bounds__(DC_THREADS) distill_grad_kernel(const DtArgs a, int ctas)
+template <typename T> __global__ void __launch_bounds__(DC_THREADS, 2) distill_grad_kernel(const DtArgs a, int ctas)
 {
     __shared__ DcShared s;
     constexpr int N = PIECE<T>;
     const int tid = threadIdx.x;
     const int rank = (int)(blockIdx.x % (unsigned)ctas);
-    const double inv = 1.0 / (double)a.temperature;
-    const float inv_t = 1.0f / a.temperature, c = 1.4426950408889634f / a.temperature;
+    const float inv_t = a.inv_t, c = a.c;
+    for (int w = tid; w < DC_SLOTS; w += DC_THREADS) s.slot[w] = -1;
     for (int64_t r = blockIdx.x / (unsigned)ctas; r < a.rows; r += gridDim.x / (unsigned)ctas) {
         const T* const z = static_cast<const T*>(a.z) + r * a.ldz;
         T* const dz = static_cast<T*>(a.dz) + r * a.lddz;
-        const float weight = a.row_weight ? __ldg(a.row_weight + r) : 1.0f, t_lse = a.t_lse ? __ldg(a.t_lse + r) : 0.0f;
+        const DcHead head(a, r);
+        const float weight = head.weight;
         const float4 st = __ldg(reinterpret_cast<const float4*>(a.stats) + r);
         const DcRun<T> my(z, a.cols, rank, ctas);
-        const DcEntry e = dc_entry(a, r, t_lse, inv, s);
+        const DcEntry e = dc_entry(a, head, s);
         int at;
-        const bool mine = my.has(e.id, rank, ctas, at) && e.first;
-        const float zk = mine ? to_f32(z[e.id]) : 0.0f;
+        const bool here = my.has(head.id, rank, ctas, at);
+        bool mine = here && !e.twice;
+        float P_all = e.P;
+        const float zk = here ? to_f32(z[head.id]) : 0.0f;
         const bool in_head = rank == 0 && tid < my.row.head, in_tail = rank == ctas - 1 && tid >= 32 && tid < 32 + my.row.tail;
         const int edge_at = in_head ? tid : (int)a.cols - my.row.tail + tid - 32;
         const float edge = in_head || in_tail ? to_f32(z[edge_at]) : 0.0f;
-        __syncthreads();   // every listed z has been read (dz may be z)
-        if (weight == 0.0f || dc_skipped(a, e)) {
+        // (the barrier also stands between the reads of listed columns and the writes: dz may be z)
+        __syncthreads();
+        const int has = dc_has(a, e, s);
+        if ((has & 2) && here) mine = dc_first(a, head.id, s, P_all);
+        if (head.id >= 0) s.slot[e.slot] = -1;
+        if (weight == 0.0f || !(has & 1)) {
             dt_zero_row(dz, a.cols, rank * DC_THREADS + tid, ctas * DC_THREADS);
             __syncthreads();
             continue;
@@ -694,11 +759,11 @@ template <typename T> __global__ void __launch_bounds__(DC_THREADS) distill_grad
                 if (p + j * DC_THREADS < my.pieces) v[j] = zp[p + j * DC_THREADS];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (p + j * DC_THREADS < my.pieces) dt_store(dp + (p + j * DC_THREADS) * N, whole, v[j], 0u, base2, outer2, c2);
+                if (p + j * DC_THREADS < my.pieces) dt_store(dp + (p + j * DC_THREADS) * N, whole, v[j], base2, outer2, c2);
         }
         if (in_head || in_tail) dz[edge_at] = from_f32<T>(dt_exp2((edge - base) * c) * k.outer);
         __syncthreads();   // the listed columns have been written as the others
-        if (mine) dz[e.id] = from_f32<T>(k.inner * expf((zk - k.M) * inv_t) - k.scale * (e.P_all * k.p_scale));
+        if (mine) dz[head.id] = from_f32<T>(k.inner * expf((zk - k.M) * inv_t) - k.scale * (P_all * k.p_scale));
         __syncthreads();
     }
 }
@@ -706,11 +771,12 @@ template <typename T> __global__ void __launch_bounds__(DC_THREADS) distill_grad
 template <typename T> int dc_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a, int ctas)
 {
     const int64_t most = (a.cols / PIECE<T> + ctas - 1) / ctas, rows = a.rows < (1 << 20) ? a.rows : 1 << 20;   // (clusters; further rows by turns)
-    S2V_CUDA_OK(ctx, s2v_allow_shared(distill_cluster_kernel<T>, DC_RUN_MOST));
+    const int held = (int)(most < DC_HELD ? most : DC_HELD);
+    S2V_CUDA_OK(ctx, s2v_allow_shared(distill_cluster_kernel<T>, DC_SMEM));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * ctas));
     cfg.blockDim = dim3(DC_THREADS);
-    cfg.dynamicSmemBytes = (size_t)most * 16;
+    cfg.dynamicSmemBytes = (size_t)(held * 16 + (most - held + 3) / 4 * 4);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -718,7 +784,7 @@ template <typename T> int dc_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs&
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    S2V_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, distill_cluster_kernel<T>, a, ctas));
+    S2V_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, distill_cluster_kernel<T>, a, ctas, held));
     S2V_CHECK_LAUNCH(ctx, "distill_cluster_kernel");
     return S2V_OK;
 }
@@ -745,7 +811,7 @@ template <typename T, bool GRAD_ONLY> int dt_launch_type(s2v_ctx* ctx, cudaStrea
     if (pieces <= 32) return dw_launch<T, 1, GRAD_ONLY>(ctx, st, a);
     if (pieces <= 32 * DW_PIECES) return dw_launch<T, DW_PIECES, GRAD_ONLY>(ctx, st, a);
     int ctas = 1;
-    while (ctas < DC_CTAS && (pieces * 16 > (int64_t)ctas * DC_RUN || (a.rows * ctas < 2 * ctx->sm_count && pieces >= (int64_t)ctas * 2 * DC_THREADS))) ctas *= 2;
+    while (ctas < DC_CTAS && (pieces > (int64_t)ctas * DC_RUN || (a.rows * ctas < 2 * ctx->sm_count && pieces >= (int64_t)ctas * 2 * DC_THREADS))) ctas *= 2;
     return GRAD_ONLY ? dg_launch<T>(ctx, st, a, ctas) : dc_launch<T>(ctx, st, a, ctas);
 }
 int dt_launch(s2v_ctx* ctx, s2v_stream stream, int z_type, bool grad_only, const DtArgs& a)
@@ -786,7 +852,7 @@ int s2v_distill_topk(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t cols
                      void* dz, int64_t lddz)
 {
     S2V_ENTER(ctx);
-    const DtArgs a{rows, cols, ldz, ldt, lddz, z, idx, t, t_lse, row_weight, loss, stats, dz, ctx->dstatus_dev, temperature, top, t_type};
+    const DtArgs a{rows, cols, ldz, ldt, lddz, z, idx, t, t_lse, row_weight, loss, stats, dz, ctx->dstatus_dev, temperature, top, t_type, 1.0 / (double)temperature, 1.0f / temperature, 1.4426950408889634f / temperature};
     const int rc = dt_check(ctx, "distill_topk", z_type, a);
     if (rc != S2V_OK || rows == 0) return rc;
     if (!loss) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "distill_topk: NULL loss");
@@ -798,7 +864,7 @@ int s2v_distill_topk_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t
                           void* dz, int64_t lddz)
 {
     S2V_ENTER(ctx);
-    const DtArgs a{rows, cols, ldz, ldt, lddz, z, idx, t, t_lse, row_weight, nullptr, const_cast<float*>(stats), dz, ctx->dstatus_dev, temperature, top, t_type};
+    const DtArgs a{rows, cols, ldz, ldt, lddz, z, idx, t, t_lse, row_weight, nullptr, const_cast<float*>(stats), dz, ctx->dstatus_dev, temperature, top, t_type, 1.0 / (double)temperature, 1.0f / temperature, 1.4426950408889634f / temperature};
     const int rc = dt_check(ctx, "distill_topk_grad", z_type, a);
     if (rc != S2V_OK || rows == 0) return rc;
     if (!stats || !dz) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "distill_topk_grad: NULL pointer");
