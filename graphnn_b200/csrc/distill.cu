@@ -12,7 +12,7 @@ namespace
 {
 
 constexpr int DT_TOP = 256;            // most entries of a list
-constexpr int64_t DT_ROW_BYTES = 1536 << 10;   // longest rows
+constexpr int64_t DT_ROW_BYTES = 1 << 20;   // longest rows: eight runs
 constexpr int DT_SITE = 7;             // status word: a class outside the row
 
 struct DtArgs {
@@ -436,19 +436,22 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
 
 // ---------------------------------------------------------------- longer rows: a CTA or a cluster of CTAs each
 // Every CTA has an equal run of the row's pieces.  The first DC_HELD of them lie in shared memory between the sums and the gradient, the others are
-// read once more, from L2: two CTAs an SM, so that one moves data while the other joins sums or waits.  Listed columns become -infinity in shared
+// read once more, from L2.  Several CTAs share an SM, so that some move data while others join sums or wait.  Listed columns become -infinity in shared
 // memory; the others' are named by a byte per piece.  Their gradients are written over what the loops over the run wrote.  The first CTA's first
 // warp adds up the loss while the others write the gradient.
-constexpr int DC_THREADS = 512, DC_WARPS = DC_THREADS / 32, DC_CTAS = 8, DC_LISTERS = DT_TOP / 32;
-constexpr int DC_SMEM = 104 << 10;                   // bytes of a CTA's pieces and marks
-constexpr int DC_HELD = 5600, DC_RUN = 16384;        // pieces held, and of a run, at most
-static_assert(DC_HELD * 16 + (DC_RUN - DC_HELD) <= DC_SMEM, "a byte for each piece that is not held");
+constexpr int DC_CTAS = 8, DC_LISTERS = DT_TOP / 32;
+// Rows of up to DC_SHORT pieces: six CTAs of 128 threads an SM (the steps of a row are a chain of latencies: 16384 rows of 9000 bf16 199 us, with
+// CTAs of 256 threads 311), lists of more than 128 entries apart.  Longer ones: three of 256 (4096 rows of 131072 bf16 490 us; six of 128
+// 562, two of 512 620 to 650, all pieces held by a cluster of four 504).
+constexpr int DC_SHORT = 2048, DC_HELD = 4000, DC_RUN = 8192;   // pieces: of a short row; held, and of a run, at most
+constexpr int DC_SMEM = 72 << 10;
+static_assert(DC_HELD * 16 + (DC_RUN - DC_HELD) <= DC_SMEM && DC_SHORT <= DC_HELD, "a byte for each piece that is not held");
 constexpr int DC_SLOTS = 512;                        // of the table that finds columns listed twice
 struct DcShared {
     float P[DT_TOP], t[DT_TOP], z[DT_TOP];
     int id[DT_TOP], slot[DC_SLOTS];
     float4 peer[2][DC_CTAS];   // outer and inner sums of the cluster's CTAs, two rows by turns
-    float2 outer[DC_WARPS], inner[DC_LISTERS];
+    float2 outer[16], inner[DC_LISTERS];
     float Z[DC_LISTERS], tmax[DC_LISTERS];
     int has[DC_LISTERS];       // bit 0: an entry; bit 1: a column that is listed twice
 };
@@ -551,11 +554,12 @@ template <typename T> struct DcRun {
     }
 };
 
-template <typename T> __global__ void __launch_bounds__(DC_THREADS, 2) distill_cluster_kernel(const DtArgs a, int ctas, int held)
+template <typename T, int DC_THREADS, int CTAS_SM>
+__global__ void __launch_bounds__(DC_THREADS, CTAS_SM) distill_cluster_kernel(const DtArgs a, int ctas, int held)
 {
     extern __shared__ __align__(16) unsigned char dc_raw[];
     __shared__ DcShared s;
-    constexpr int N = PIECE<T>;
+    constexpr int N = PIECE<T>, DC_WARPS = DC_THREADS / 32;
     uint4* const run = reinterpret_cast<uint4*>(dc_raw);
     uint32_t* const marks = reinterpret_cast<uint32_t*>(run + held);           // a byte for each piece behind the held ones
     const uint8_t* const mark = reinterpret_cast<const uint8_t*>(marks) - held;
@@ -711,14 +715,15 @@ template <typename T> __global__ void __launch_bounds__(DC_THREADS, 2) distill_c
 }
 
 // The gradient from kept sums: nothing to wait for but the list.
-template <typename T> __global__ void __launch_bounds__(DC_THREADS, 2) distill_grad_kernel(const DtArgs a, int ctas)
+// (A CTA of 512 threads a long row: 4096 x 131072 bf16 345 us, 6.2 TB/s; with clusters of four such CTAs 454.)
+template <typename T, int DG_THREADS> __global__ void __launch_bounds__(DG_THREADS, 1024 / DG_THREADS) distill_grad_kernel(const DtArgs a, int ctas)
 {
     __shared__ DcShared s;
     constexpr int N = PIECE<T>;
     const int tid = threadIdx.x;
     const int rank = (int)(blockIdx.x % (unsigned)ctas);
     const float inv_t = a.inv_t, c = a.c;
-    for (int w = tid; w < DC_SLOTS; w += DC_THREADS) s.slot[w] = -1;
+    for (int w = tid; w < DC_SLOTS; w += DG_THREADS) s.slot[w] = -1;
     for (int64_t r = blockIdx.x / (unsigned)ctas; r < a.rows; r += gridDim.x / (unsigned)ctas) {
         const T* const z = static_cast<const T*>(a.z) + r * a.ldz;
         T* const dz = static_cast<T*>(a.dz) + r * a.lddz;
@@ -741,7 +746,7 @@ template <typename T> __global__ void __launch_bounds__(DC_THREADS, 2) distill_g
         if ((has & 2) && here) mine = dc_first(a, head.id, s, P_all);
         if (head.id >= 0) s.slot[e.slot] = -1;
         if (weight == 0.0f || !(has & 1)) {
-            dt_zero_row(dz, a.cols, rank * DC_THREADS + tid, ctas * DC_THREADS);
+            dt_zero_row(dz, a.cols, rank * DG_THREADS + tid, ctas * DG_THREADS);
             __syncthreads();
             continue;
         }
@@ -752,14 +757,14 @@ template <typename T> __global__ void __launch_bounds__(DC_THREADS, 2) distill_g
         const uint4* const zp = reinterpret_cast<const uint4*>(z + my.row.head) + my.first;
         T* const dp = dz + my.row.head + (int64_t)my.first * N;
         const bool whole = (reinterpret_cast<uintptr_t>(dp) & 15) == 0;
-        for (int p = tid; p < my.pieces; p += 4 * DC_THREADS) {
+        for (int p = tid; p < my.pieces; p += 4 * DG_THREADS) {
             uint4 v[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (p + j * DC_THREADS < my.pieces) v[j] = zp[p + j * DC_THREADS];
+                if (p + j * DG_THREADS < my.pieces) v[j] = zp[p + j * DG_THREADS];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (p + j * DC_THREADS < my.pieces) dt_store(dp + (p + j * DC_THREADS) * N, whole, v[j], base2, outer2, c2);
+                if (p + j * DG_THREADS < my.pieces) dt_store(dp + (p + j * DG_THREADS) * N, whole, v[j], base2, outer2, c2);
         }
         if (in_head || in_tail) dz[edge_at] = from_f32<T>(dt_exp2((edge - base) * c) * k.outer);
         __syncthreads();   // the listed columns have been written as the others
@@ -768,14 +773,15 @@ template <typename T> __global__ void __launch_bounds__(DC_THREADS, 2) distill_g
     }
 }
 
-template <typename T> int dc_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a, int ctas)
+template <typename T, int THREADS, int CTAS_SM> int dc_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a, int ctas)
 {
     const int64_t most = (a.cols / PIECE<T> + ctas - 1) / ctas, rows = a.rows < (1 << 20) ? a.rows : 1 << 20;   // (clusters; further rows by turns)
     const int held = (int)(most < DC_HELD ? most : DC_HELD);
-    S2V_CUDA_OK(ctx, s2v_allow_shared(distill_cluster_kernel<T>, DC_SMEM));
+    const auto kernel = distill_cluster_kernel<T, THREADS, CTAS_SM>;
+    S2V_CUDA_OK(ctx, s2v_allow_shared(kernel, DC_SMEM));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * ctas));
-    cfg.blockDim = dim3(DC_THREADS);
+    cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = (size_t)(held * 16 + (most - held + 3) / 4 * 4);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -784,14 +790,14 @@ template <typename T> int dc_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs&
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    S2V_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, distill_cluster_kernel<T>, a, ctas, held));
+    S2V_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, kernel, a, ctas, held));
     S2V_CHECK_LAUNCH(ctx, "distill_cluster_kernel");
     return S2V_OK;
 }
-template <typename T> int dg_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a, int ctas)
+template <typename T, int THREADS> int dg_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a, int ctas)
 {
     const int64_t rows = a.rows < (1 << 20) ? a.rows : 1 << 20;
-    distill_grad_kernel<T><<<(unsigned)(rows * ctas), DC_THREADS, 0, st>>>(a, ctas);
+    distill_grad_kernel<T, THREADS><<<(unsigned)(rows * ctas), THREADS, 0, st>>>(a, ctas);
     S2V_CHECK_LAUNCH(ctx, "distill_grad_kernel");
     return S2V_OK;
 }
@@ -811,8 +817,14 @@ template <typename T, bool GRAD_ONLY> int dt_launch_type(s2v_ctx* ctx, cudaStrea
     if (pieces <= 32) return dw_launch<T, 1, GRAD_ONLY>(ctx, st, a);
     if (pieces <= 32 * DW_PIECES) return dw_launch<T, DW_PIECES, GRAD_ONLY>(ctx, st, a);
     int ctas = 1;
-    while (ctas < DC_CTAS && (pieces > (int64_t)ctas * DC_RUN || (a.rows * ctas < 2 * ctx->sm_count && pieces >= (int64_t)ctas * 2 * DC_THREADS))) ctas *= 2;
-    return GRAD_ONLY ? dg_launch<T>(ctx, st, a, ctas) : dc_launch<T>(ctx, st, a, ctas);
+    const bool small = pieces <= DC_SHORT && a.top <= 128;
+    if constexpr (GRAD_ONLY) {
+        while (ctas < DC_CTAS && a.rows * ctas < 2 * ctx->sm_count && pieces >= (int64_t)ctas * 1024) ctas *= 2;
+        return small ? dg_launch<T, 128>(ctx, st, a, ctas) : dg_launch<T, 512>(ctx, st, a, ctas);
+    } else {
+        while (ctas < DC_CTAS && (pieces > (int64_t)ctas * DC_RUN || (a.rows * ctas < 2 * ctx->sm_count && pieces >= (int64_t)ctas * 512))) ctas *= 2;
+        return small ? dc_launch<T, 128, 6>(ctx, st, a, ctas) : dc_launch<T, 256, 3>(ctx, st, a, ctas);
+    }
 }
 int dt_launch(s2v_ctx* ctx, s2v_stream stream, int z_type, bool grad_only, const DtArgs& a)
 {
@@ -832,7 +844,7 @@ int dt_check(s2v_ctx* ctx, const char* name, int z_type, const DtArgs& a)
     if (a.rows == 0) return S2V_OK;
     if (!a.z || !a.idx || !a.t) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": NULL pointer");
     if (a.top > DT_TOP) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, who + ": more than 256 entries a row");
-    if (a.cols * (int64_t)s2v_dtype_bytes(z_type) > DT_ROW_BYTES) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, who + ": rows of more than 1,572,864 bytes");
+    if (a.cols * (int64_t)s2v_dtype_bytes(z_type) > DT_ROW_BYTES) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, who + ": rows of more than 1,048,576 bytes");
     if (a.rows > 1 && (a.ldz < a.cols || a.ldt < a.top || (a.dz && a.lddz < a.cols)))
         return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": leading dimension below the number of columns");
     const size_t es = s2v_dtype_bytes(z_type);

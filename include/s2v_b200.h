@@ -248,7 +248,7 @@ int s2v_linear_i8(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, int64_t
  * without a finite value, has NaN as its loss and gradient, and so has a row with NaN or +infinity among its entries' t.  An entry with idx >= cols is left out and reported through the status word (S2V_ERR_INVALID_ARG).
  *   loss : [rows];  stats : float [rows x 4], 16-byte aligned, or NULL, for s2v_distill_topk_grad;  dz : [rows x cols] of z_type or NULL: the gradient in the same
  *   call.  dz may be z itself (with lddz = ldz); else it overlaps no input.  Rows of
- *   at most 1,572,864 bytes (393,216 columns of fp32, 786,432 of 16 bits). */
+ *   at most 1,048,576 bytes (262,144 columns of fp32, 524,288 of 16 bits). */
 int s2v_distill_topk(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t cols, int z_type, const void* z, int64_t ldz, int top,
                      const int32_t* idx, int t_type, const void* t, int64_t ldt, const float* t_lse, float temperature,
                      const float* row_weight, float* loss, float* stats, void* dz, int64_t lddz);

@@ -174,7 +174,7 @@ def test_the_formula_of_the_gradient_is_the_losses_derivative():
 
 # ---------------------------------------------------------------- loss and gradient
 SIZES = [(1, 1, 1), (3, 2, 1), (64, 6, 3), (5, 7, 16), (40, 33, 33), (9, 100, 256), (17, 255, 8), (6, 1000, 10), (130, 1023, 20), (3, 1025, 64), (5, 4097, 100), (2, 8192, 128), (4, 20011, 50),
-         (1, 50021, 200), (2, 131072, 64)]
+         (1, 50021, 200), (2, 131072, 64), (300, 9001, 40), (3, 262144, 7), (302, 40003, 9)]
 
 
 @gpu
@@ -187,6 +187,14 @@ def test_loss_and_gradient(gpu_ctx, rows, cols, top, dtype, tail):
     loss, dz = both_ways(gpu_ctx, z, idx, t, temp, lse, w)
     assert_matches(loss, dz, z, idx, t, temp, lse, w)
     assert float(loss[rows // 2]) == 0 or rows <= 2
+
+
+@gpu
+def test_the_longest_rows(gpu_ctx):
+    for dtype, cols in (("bf16", 524288), ("f16", 524283)):
+        z, idx, t, lse, w = inputs(2, cols, 30, dtype, 5, True, 1.0)
+        loss, dz = both_ways(gpu_ctx, z, idx, t, 1.0, lse, w)
+        assert_matches(loss, dz, z, idx, t, 1.0, lse, w)
 
 
 @gpu
@@ -348,7 +356,7 @@ def test_refusals(gpu_ctx):
     for got, want in [(call(rows=-1), -1), (call(cols=0), -1), (call(top=0), -1), (call(zt=3), -1), (call(tt=-1), -1), (call(z=None), -1), (call(idx=None), -1), (call(t=None), -1),
                       (call(loss=None), -1), (call(ldz=9), -1), (call(lddz=9), -1), (call(ldt=2), -1), (call(temp=0.0), -1), (call(temp=-1.0), -1), (call(temp=INF), -1),
                       (call(temp=float("nan")), -1), (call(temp=1e-35), -1), (call(z=p + 2), -1), (call(dz=p + 2), -1), (call(t=p + 1, tt=1), -1), (call(dz=p, lddz=11), -1),
-                      (call(top=257, ldt=257), -2), (call(cols=393217, ldz=1 << 20, lddz=1 << 20), -2), (call(cols=786433, zt=1, ldz=1 << 20, lddz=1 << 20), -2),
+                      (call(top=257, ldt=257), -2), (call(cols=262145, ldz=1 << 20, lddz=1 << 20), -2), (call(cols=524289, zt=1, ldz=1 << 20, lddz=1 << 20), -2),
                       (grad(stats=None), -1), (grad(dz=None), -1), (grad(temp=0.0), -1), (grad(ldz=9), -1), (grad(rows=-1), -1), (grad(cols=0), -1)]:
         assert got == want, lib.s2v_last_error(h)
     assert call(rows=0, z=None) == 0 and grad(rows=0) == 0
