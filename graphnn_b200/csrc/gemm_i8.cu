@@ -22,8 +22,8 @@ template <int BN> struct GiCfg {
     static constexpr uint32_t TM_COLS = 2 * BN;
     static constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);   // s32 <- s8 x s8, M = 128, N = BN
     static constexpr uint32_t OFF_OUT = STAGES * STAGE;                       // per epilogue warp: 32 rows
-    static constexpr uint32_t OFF_SCALE = OFF_OUT + GI_EPI * 32 * GI_PITCH;   // per epilogue warp: 32 channels' scales, then their biases
-    static constexpr uint32_t OFF_BAR = OFF_SCALE + GI_EPI * 2 * 32 * 4;
+    static constexpr uint32_t OFF_SCALE = OFF_OUT + GI_EPI * 32 * GI_PITCH;   // per epilogue warp: the scales of half a tile's channels, then their biases
+    static constexpr uint32_t OFF_BAR = OFF_SCALE + GI_EPI * BN * 4;
     enum { FULL = 0, EMPTY = FULL + STAGES, DONE = EMPTY + STAGES, READ = DONE + 2, BARS = READ + 2 };
     static constexpr uint32_t OFF_MISC = OFF_BAR + 8 * BARS;
     static constexpr uint32_t SMEM = OFF_MISC + 16 + 1024;                    // + slack to align the base to 1024 bytes
@@ -62,24 +62,15 @@ __device__ __forceinline__ void gi_tile(int tile, int m_tiles, int n_tiles, int&
 }
 
 // The outputs of 32 rows (lanes) by COLS columns, staged so that the store instructions write whole sectors.
-template <typename T>
-__device__ __forceinline__ void gi_write(const GiArgs& a, unsigned char* stage, const float* chan, int64_t row0, int64_t col0, float sa, uint32_t tmem, bool any)
+template <typename T, int HALF>
+__device__ __forceinline__ void gi_write(const GiArgs& a, unsigned char* stage, const float* chan, int64_t row0, int64_t col0, float sa, const uint32_t* v)
 {
     constexpr int COLS = GI_PIECE / sizeof(T), PER = 16 / sizeof(T);
     const int lane = threadIdx.x & 31;
     unsigned char* const mine = stage + lane * GI_PITCH;
-    uint32_t v[COLS];
-    if (any) {
-#pragma unroll
-        for (int h = 0; h < COLS; h += 16) tc_ld_cols16(tmem + h, v + h);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-    } else {
-#pragma unroll
-        for (int j = 0; j < COLS; ++j) v[j] = 0;
-    }
 #pragma unroll
     for (int j = 0; j < COLS; j += 4) {
-        const float4 s = *reinterpret_cast<const float4*>(chan + j), b = *reinterpret_cast<const float4*>(chan + 32 + j);
+        const float4 s = *reinterpret_cast<const float4*>(chan + j), b = *reinterpret_cast<const float4*>(chan + HALF + j);
         float y[4] = {fmaf(__fmul_rn(sa, s.x), (float)(int)v[j], b.x), fmaf(__fmul_rn(sa, s.y), (float)(int)v[j + 1], b.y),
                       fmaf(__fmul_rn(sa, s.z), (float)(int)v[j + 2], b.z), fmaf(__fmul_rn(sa, s.w), (float)(int)v[j + 3], b.w)};
         if (a.relu) {
@@ -201,26 +192,37 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
         static_assert(HALF % COLS == 0 && COLS <= 32, "pieces of half a tile's rows");
         const int e = warp - 2, quarter = warp & 3, half = e >> 2;
         unsigned char* const stage = smem + Cfg::OFF_OUT + e * 32 * GI_PITCH;
-        float* const chan = reinterpret_cast<float*>(smem + Cfg::OFF_SCALE) + e * 64;
+        float* const chan = reinterpret_cast<float*>(smem + Cfg::OFF_SCALE) + e * BN;
         int t = 0;
         for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++t) {
             int tm, tn;
             gi_tile(tile, a.m_tiles, a.n_tiles, tm, tn);
             const int acc = t & 1;
-            const int64_t row0 = (int64_t)tm * 128 + quarter * 32;
+            const int64_t row0 = (int64_t)tm * 128 + quarter * 32, first = (int64_t)tn * BN + half * HALF;
             const float sa = row0 + lane < a.m ? a.a_scale[row0 + lane] : 0.0f;
+#pragma unroll
+            for (int u = lane; u < HALF; u += 32) {
+                chan[u] = first + u < a.n ? __ldg(a.b_scale + first + u) : 0.0f;
+                chan[HALF + u] = a.bias && first + u < a.n ? __ldg(a.bias + first + u) : 0.0f;
+            }
+            __syncwarp();
             if (a.kblocks > 0 && !tc_wait(bar(Cfg::DONE + acc), (uint32_t)(t / 2) & 1u, abort_flag, a.status, 73)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            for (int c = half * HALF; c < (half + 1) * HALF; c += COLS) {
-                const int64_t col0 = (int64_t)tn * BN + c;
-                if (row0 >= a.m || col0 >= a.n) break;   // (the same for the warp)
-                if (lane < COLS) {
-                    const int64_t col = col0 + lane;
-                    chan[lane] = col < a.n ? __ldg(a.b_scale + col) : 0.0f;
-                    chan[32 + lane] = a.bias && col < a.n ? __ldg(a.bias + col) : 0.0f;
-                }
-                __syncwarp();
-                gi_write<T>(a, stage, chan, row0, col0, sa, tmem + (uint32_t)(acc * BN + c) + ((uint32_t)quarter << 21), a.kblocks > 0);
+            const uint32_t at = tmem + (uint32_t)(acc * BN + half * HALF) + ((uint32_t)quarter << 21);
+            const int cols = row0 >= a.m ? 0 : (int)min((int64_t)HALF, a.n - first);   // (the same for the warp)
+            uint32_t next[COLS] = {};
+            const auto fetch = [&](int c) {
+#pragma unroll
+                for (int h = 0; h < COLS; h += 16) tc_ld_cols16(at + (uint32_t)(c + h), next + h);
+            };
+            if (cols > 0 && a.kblocks > 0) fetch(0);
+            for (int c = 0; c < cols; c += COLS) {
+                uint32_t v[COLS];
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                for (int j = 0; j < COLS; ++j) v[j] = next[j];
+                if (c + COLS < cols && a.kblocks > 0) fetch(c + COLS);
+                gi_write<T, HALF>(a, stage, chan + c, row0, first + c, sa, v);
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (lane == 0) tc_mbar_arrive(bar(Cfg::READ + acc));

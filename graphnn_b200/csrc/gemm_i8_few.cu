@@ -318,19 +318,27 @@ __global__ void __launch_bounds__(GS_THREADS) gemm_i8_split_kernel(const __grid_
         for (int c = 0; c < 8; ++c)
             if (c < a.ctas) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from[c]) : "r"(smem_u32(mine + row)), "r"(c));
         const int t0 = rank * NT / a.ctas, t1 = (rank + 1) * NT / a.ctas;
-        for (int t = t0; t < t1; ++t) {
-            const int64_t token = (int64_t)tm * NT + t;
-            if (token >= a.m) break;
-            int sum = 0;
+        constexpr int G = NT < 32 ? 2 : 8;   // tokens whose sums are on their way at once (a load from another CTA takes as long as one from L2)
+        for (int t = t0; t < t1; t += G) {
+            int part[G][8];
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-                if (c < a.ctas) {
-                    int p;
-                    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(p) : "r"(from[c] + (uint32_t)t * 512u) : "memory");
-                    sum += p;
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    part[g][c] = 0;
+                    if (c < a.ctas && t + g < t1) asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(part[g][c]) : "r"(from[c] + (uint32_t)(t + g) * 512u) : "memory");
                 }
-            const float v = fmaf(__fmul_rn(a.a_scale[token], sw), (float)sum, b);
-            if (col < a.n) static_cast<T*>(a.C)[token * a.ldc + col] = from_f32<T>(a.relu ? relu_ref(v) : v);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const int64_t token = (int64_t)tm * NT + t + g;
+                int sum = 0;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) sum += part[g][c];
+                if (t + g < t1 && token < a.m && col < a.n) {
+                    const float v = fmaf(__fmul_rn(a.a_scale[token], sw), (float)sum, b);
+                    static_cast<T*>(a.C)[token * a.ldc + col] = from_f32<T>(a.relu ? relu_ref(v) : v);
+                }
+            }
         }
     }
     __syncwarp();
