@@ -14,15 +14,15 @@ namespace
 
 constexpr int GI_EPI = 8;                              // epilogue warps
 constexpr int GI_THREADS = 32 * (2 + GI_EPI);
-constexpr int GI_PIECE = 64, GI_PITCH = 80;             // bytes of a row that an epilogue warp stages at a time; bytes between the staged rows (no bank conflicts)
+constexpr int GI_PIECE = 64, GI_BOX = 32 * GI_PIECE;    // bytes of a row that an epilogue warp hands over at a time; of its 32 rows
 
 template <int BN> struct GiCfg {
     static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 5 : 7, BOXES = BN == 256 ? 1 : 2;   // boxes of an epilogue warp
     static constexpr uint32_t TM_COLS = 2 * BN;
     static constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);   // s32 <- s8 x s8, M = 128, N = BN
-    static constexpr uint32_t OFF_OUT = STAGES * STAGE;                       // per epilogue warp: 32 rows
-    static constexpr uint32_t OFF_SCALE = OFF_OUT + GI_EPI * 32 * GI_PITCH;   // per epilogue warp: the scales of half a tile's channels, then their biases
+    static constexpr uint32_t OFF_OUT = STAGES * STAGE;                       // per epilogue warp: its boxes
+    static constexpr uint32_t OFF_SCALE = OFF_OUT + GI_EPI * BOXES * GI_BOX;   // per epilogue warp: the scales of half a tile's channels, then their biases
     static constexpr uint32_t OFF_BAR = OFF_SCALE + GI_EPI * BN * 4;
     enum { FULL = 0, EMPTY = FULL + STAGES, DONE = EMPTY + STAGES, READ = DONE + 2, BARS = READ + 2 };
     static constexpr uint32_t OFF_MISC = OFF_BAR + 8 * BARS;
@@ -38,7 +38,7 @@ struct GiArgs {
     const float* b_scale;
     const float* bias;
     void* C;
-    int relu, wide;                 // wide: 16-byte stores of whole rows' pieces are aligned
+    int relu, boxes;                // boxes: the output has a tensor map (16-byte aligned rows)
     s2v_device_status* status;
 };
 
@@ -61,49 +61,46 @@ __device__ __forceinline__ void gi_tile(int tile, int m_tiles, int n_tiles, int&
     tn = at / rows;
 }
 
-// The outputs of 32 rows (lanes) by COLS columns, staged so that the store instructions write whole sectors.
+// The outputs of 32 rows (lanes) by COLS columns: into a box in shared memory (64-byte rows, their 16-byte pieces exchanged by the 64-byte swizzle,
+// which also keeps the stores free of bank conflicts), and from there by one copy that leaves out what the matrix does not have.  (Written by the
+// warp's own loads and stores, a product with few sums an output was bound by that: 491,520 x 256 outputs of fp32 over k = 128 158 us.)
 template <typename T, int HALF>
-__device__ __forceinline__ void gi_write(const GiArgs& a, unsigned char* stage, const float* chan, int64_t row0, int64_t col0, float sa, const uint32_t* v)
+__device__ __forceinline__ void gi_write(const GiArgs& a, const CUtensorMap* map, unsigned char* box, const float* chan, int64_t row0, int64_t col0, float sa, const uint32_t* v)
 {
     constexpr int COLS = GI_PIECE / sizeof(T), PER = 16 / sizeof(T);
     const int lane = threadIdx.x & 31;
-    unsigned char* const mine = stage + lane * GI_PITCH;
+    const auto piece = [&](int row, int i) { return box + row * GI_PIECE + 16 * (i ^ (row >> 1 & 3)); };
 #pragma unroll
-    for (int j = 0; j < COLS; j += 4) {
-        const float4 s = *reinterpret_cast<const float4*>(chan + j), b = *reinterpret_cast<const float4*>(chan + HALF + j);
-        float y[4] = {fmaf(__fmul_rn(sa, s.x), (float)(int)v[j], b.x), fmaf(__fmul_rn(sa, s.y), (float)(int)v[j + 1], b.y),
-                      fmaf(__fmul_rn(sa, s.z), (float)(int)v[j + 2], b.z), fmaf(__fmul_rn(sa, s.w), (float)(int)v[j + 3], b.w)};
+    for (int j = 0; j < COLS; j += PER) {
+        float y[PER];
+#pragma unroll
+        for (int u = 0; u < PER; u += 4) {
+            const float4 s = *reinterpret_cast<const float4*>(chan + j + u), b = *reinterpret_cast<const float4*>(chan + HALF + j + u);
+            y[u] = fmaf(__fmul_rn(sa, s.x), (float)(int)v[j + u], b.x), y[u + 1] = fmaf(__fmul_rn(sa, s.y), (float)(int)v[j + u + 1], b.y);
+            y[u + 2] = fmaf(__fmul_rn(sa, s.z), (float)(int)v[j + u + 2], b.z), y[u + 3] = fmaf(__fmul_rn(sa, s.w), (float)(int)v[j + u + 3], b.w);
+        }
         if (a.relu) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) y[u] = relu_ref(y[u]);
+            for (int u = 0; u < PER; ++u) y[u] = relu_ref(y[u]);
         }
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(mine + 4 * j) = make_float4(y[0], y[1], y[2], y[3]);
-        else *reinterpret_cast<uint2*>(mine + 2 * j) = make_uint2(pack_16bit<T>(y[0], y[1]), pack_16bit<T>(y[2], y[3]));
+        *reinterpret_cast<uint4*>(piece(lane, j / PER)) = pack_piece(y, T());
     }
-    __syncwarp();
-    T* const C = static_cast<T*>(a.C);
-    const int seg = lane & 3;
-    const int64_t c = col0 + seg * PER;
-#pragma unroll
-    for (int it = 0; it < 4; ++it) {
-        const int r = it * 8 + (lane >> 2);
-        if (row0 + r < a.m && c < a.n) {
-            const T* const from = reinterpret_cast<const T*>(stage + r * GI_PITCH + 16 * seg);
-            T* const to = C + (row0 + r) * a.ldc + c;
-            if (a.wide && c + PER <= a.n) {
-                *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
-            } else {
-#pragma unroll
-                for (int u = 0; u < PER; ++u)
-                    if (c + u < a.n) to[u] = from[u];
-            }
+    if (a.boxes) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) tma_store_2d(map, (int)col0, (int)row0, smem_u32(box));
+    } else {
+        __syncwarp();
+        T* const C = static_cast<T*>(a.C);
+        for (int e = lane; e < 32 * COLS; e += 32) {
+            const int r = e / COLS, c = e % COLS;
+            if (row0 + r < a.m && col0 + c < a.n) C[(row0 + r) * a.ldc + col0 + c] = reinterpret_cast<const T*>(piece(r, c / PER))[c % PER];
         }
     }
-    __syncwarp();
 }
 
 template <typename T, int BN>
-__global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GiArgs a)
+__global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c, const GiArgs a)
 {
     using Cfg = GiCfg<BN>;
     constexpr int STAGES = Cfg::STAGES;
@@ -191,7 +188,8 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
         constexpr int COLS = GI_PIECE / sizeof(T), HALF = BN / 2;
         static_assert(HALF % COLS == 0 && COLS <= 32, "pieces of half a tile's rows");
         const int e = warp - 2, quarter = warp & 3, half = e >> 2;
-        unsigned char* const stage = smem + Cfg::OFF_OUT + e * 32 * GI_PITCH;
+        unsigned char* const boxes = smem + Cfg::OFF_OUT + e * Cfg::BOXES * GI_BOX;
+        int turn = 0;
         float* const chan = reinterpret_cast<float*>(smem + Cfg::OFF_SCALE) + e * BN;
         int t = 0;
         for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++t) {
@@ -222,12 +220,18 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
 #pragma unroll
                 for (int j = 0; j < COLS; ++j) v[j] = next[j];
                 if (c + COLS < cols && a.kblocks > 0) fetch(c + COLS);
-                gi_write<T, HALF>(a, stage, chan + c, row0, first + c, sa, v);
+                // the copy that last read this box has done so
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(Cfg::BOXES - 1) : "memory");
+                __syncwarp();
+                gi_write<T, HALF>(a, &map_c, boxes + turn * GI_BOX, chan + c, row0, first + c, sa, v);
+                turn = (turn + 1) % Cfg::BOXES;
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (lane == 0) tc_mbar_arrive(bar(Cfg::READ + acc));
             __syncwarp();
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -238,7 +242,7 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
 template <typename T, int BN> int gi_launch(s2v_ctx* ctx, cudaStream_t st, const s2v_gemm_i8_args& g, bool dependent)
 {
     using Cfg = GiCfg<BN>;
-    CUtensorMap map_a, map_b;
+    CUtensorMap map_a, map_b, map_c;
     if (g.k > 0) {
         // (the leading dimension of a single row is not the caller's to get right)
         const int64_t up = (g.k + 15) / 16 * 16;
@@ -256,7 +260,10 @@ template <typename T, int BN> int gi_launch(s2v_ctx* ctx, cudaStream_t st, const
     if (mt * nt > INT32_MAX / 2) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, "gemm_i8: more than 2^30 tiles of outputs");
     a.m_tiles = (int)mt, a.n_tiles = (int)nt;
     a.a_scale = g.a_scale, a.b_scale = g.b_scale, a.bias = g.bias, a.C = g.C, a.relu = g.relu;
-    a.wide = s2v_aligned16(g.C) && (g.m == 1 || g.ldc * (int64_t)sizeof(T) % 16 == 0);
+    const int64_t es = sizeof(T), ldc = g.m > 1 ? g.ldc : (g.n * es + 15) / 16 * 16 / es;
+    a.boxes = s2v_aligned16(g.C) && ldc * es % 16 == 0;
+    if (!a.boxes) memset(&map_c, 0, sizeof(map_c));
+    else if (!s2v_output_map(&map_c, g.c_type, g.C, g.m, g.n, ldc)) return s2v_fail(ctx, S2V_ERR_CUDA, "gemm_i8: the driver did not take the output's tensor map");
     a.status = ctx->dstatus_dev;
     S2V_CUDA_OK(ctx, s2v_allow_shared(gemm_i8_kernel<T, BN>, Cfg::SMEM));
     const int64_t tiles = mt * nt;
@@ -271,7 +278,7 @@ template <typename T, int BN> int gi_launch(s2v_ctx* ctx, cudaStream_t st, const
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = dependent ? 1 : 0;
-    S2V_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, gemm_i8_kernel<T, BN>, map_a, map_b, a));
+    S2V_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, gemm_i8_kernel<T, BN>, map_a, map_b, map_c, a));
     S2V_CHECK_LAUNCH(ctx, "gemm_i8_kernel");
     return S2V_OK;
 }

@@ -45,7 +45,7 @@ __device__ __forceinline__ void gv_add(int (&acc)[R][M], const uint4 (&w)[R], co
 }
 
 template <typename TX, typename TY, int M, int R>
-__global__ void __launch_bounds__(GV_THREADS, 3) gemv_i8_kernel(const GvArgs a)
+__global__ void __launch_bounds__(GV_THREADS, 4) gemv_i8_kernel(const GvArgs a)
 {
     extern __shared__ __align__(16) int8_t xs[];   // [M][kp]
     __shared__ float sx[M];
@@ -158,10 +158,7 @@ template <typename TX> int gv_by_size(s2v_ctx* ctx, cudaStream_t st, int y_type,
 {
     return s2v_by_dtype(y_type, [&](auto type) {
         using TY = decltype(type);
-        if (a.m == 1) return gv_launch<TX, TY, 1, 1>(ctx, st, a);
-        if (a.m == 2) return gv_launch<TX, TY, 2, 1>(ctx, st, a);
-        if (a.m <= 4) return gv_launch<TX, TY, 4, 1>(ctx, st, a);
-        return gv_launch<TX, TY, 8, 1>(ctx, st, a);
+        return a.m == 1 ? gv_launch<TX, TY, 1, 1>(ctx, st, a) : gv_launch<TX, TY, 2, 1>(ctx, st, a);
     });
 }
 
@@ -183,6 +180,7 @@ template <int NT> struct GsCfg {
 struct GsArgs {
     int64_t m, n, ldc;
     int kblocks, last_steps, n_tiles, ctas;
+    uint32_t bytes;   // of a panel: the weights', and the tokens' that there are (the products of the others are not looked at)
     const float* a_scale;
     const float* b_scale;
     const float* bias;
@@ -241,7 +239,7 @@ __global__ void __launch_bounds__(GS_THREADS) gemm_i8_split_kernel(const __grid_
         const int ahead = min(STAGES, steps_k);
         if (tc_elect())
             for (int i = 0; i < ahead; ++i) {
-                mbar_expect(bar(Cfg::FULL + i), Cfg::STAGE);
+                mbar_expect(bar(Cfg::FULL + i), a.bytes);
                 tma_load_2d(smem0 + (uint32_t)i * Cfg::STAGE, &map_w, (k0 + i) * 128, tn * 128, bar(Cfg::FULL + i));
             }
         __syncwarp();
@@ -254,7 +252,7 @@ __global__ void __launch_bounds__(GS_THREADS) gemm_i8_split_kernel(const __grid_
             const int s = it % STAGES;
             if (!(done = tc_wait(bar(Cfg::EMPTY + s), (uint32_t)(it / STAGES - 1) & 1u, abort_flag, a.status, 74))) break;
             if (tc_elect()) {
-                mbar_expect(bar(Cfg::FULL + s), Cfg::STAGE);
+                mbar_expect(bar(Cfg::FULL + s), a.bytes);
                 tma_load_2d(smem0 + (uint32_t)s * Cfg::STAGE, &map_w, (k0 + it) * 128, tn * 128, bar(Cfg::FULL + s));
                 tma_load_2d(smem0 + (uint32_t)s * Cfg::STAGE + Cfg::W_BYTES, &map_x, (k0 + it) * 128, tm * NT, bar(Cfg::FULL + s));
             }
@@ -351,7 +349,8 @@ template <typename T, int NT> int gs_launch(s2v_ctx* ctx, cudaStream_t st, const
     using Cfg = GsCfg<NT>;
     CUtensorMap map_w, map_x;
     const int64_t up = (g.k + 15) / 16 * 16;
-    if (!s2v_byte_matrix_map(&map_w, g.B, g.n, g.k, g.n > 1 ? g.ldb : up, 128) || !s2v_byte_matrix_map(&map_x, g.A, g.m, g.k, g.m > 1 ? g.lda : up, NT))
+    const int box = (int)(g.m < NT ? g.m : NT);   // (rows of zeros that the copy makes up take longer than none: 8 tokens 9.9 us)
+    if (!s2v_byte_matrix_map(&map_w, g.B, g.n, g.k, g.n > 1 ? g.ldb : up, 128) || !s2v_byte_matrix_map(&map_x, g.A, g.m, g.k, g.m > 1 ? g.lda : up, box))
         return s2v_fail(ctx, S2V_ERR_CUDA, "gemm_i8: the driver did not take a matrix's tensor map");
     const int64_t nt = (g.n + 127) / 128, tiles = nt * ((g.m + NT - 1) / NT);
     if (tiles * ctas > INT32_MAX / 2) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, "gemm_i8: more than 2^30 tiles of outputs");
@@ -359,7 +358,7 @@ template <typename T, int NT> int gs_launch(s2v_ctx* ctx, cudaStream_t st, const
     a.m = g.m, a.n = g.n, a.ldc = g.ldc;
     a.kblocks = (int)((g.k + 127) / 128);
     a.last_steps = (int)((g.k - 128 * (int64_t)(a.kblocks - 1) + 31) / 32);
-    a.n_tiles = (int)nt, a.ctas = ctas;
+    a.n_tiles = (int)nt, a.ctas = ctas, a.bytes = Cfg::W_BYTES + (uint32_t)box * 128;
     a.a_scale = g.a_scale, a.b_scale = g.b_scale, a.bias = g.bias, a.C = g.C, a.relu = g.relu;
     a.status = ctx->dstatus_dev;
     S2V_CUDA_OK(ctx, s2v_allow_shared(gemm_i8_split_kernel<T, NT>, Cfg::SMEM));
@@ -385,7 +384,7 @@ template <typename T, int NT> int gs_launch(s2v_ctx* ctx, cudaStream_t st, const
 
 bool s2v_gemv_i8_takes(int64_t m, int64_t n, int64_t k)
 {
-    return m <= 8 && k > 0 && n > 0 && (m <= 2 ? m : m <= 4 ? 4 : 8) * ((k + 15) / 16 * 16) <= (int64_t)GV_SMEM;
+    return m <= 2 && k > 0 && n > 0 && m * ((k + 15) / 16 * 16) <= (int64_t)GV_SMEM;
 }
 
 int s2v_launch_gemv_i8(s2v_ctx* ctx, cudaStream_t st, int x_type, const s2v_gemm_i8_args& g)

@@ -55,21 +55,59 @@ __global__ void __launch_bounds__(QR_CTA) quantize_rows_kernel(int64_t rows, int
     }
 }
 
+// Short rows: LANES lanes a row with NV pieces each, so that what a row needs once (its place, the reduction, the divisions) is done for 32 / LANES
+// rows by the same instructions.
+template <typename T, int LANES, int NV>
+__global__ void __launch_bounds__(QR_CTA) quantize_short_rows_kernel(int64_t rows, int64_t cols, const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q,
+                                                                     int64_t ldq, float* __restrict__ scale)
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (a product behind this kernel waits for its end by itself)
+    constexpr int N = PIECE<T>, GROUPS = QR_CTA / LANES;
+    static_assert(LANES >= N - 1, "the columns of the head, or of the tail, have a lane each");
+    const int at = threadIdx.x % LANES;
+    for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < rows; first += (int64_t)gridDim.x * GROUPS) {
+        const int64_t r = min(first + threadIdx.x / LANES, rows - 1);   // (the last row, several times over, where there are no more)
+        const T* const xr = x + r * ldx;
+        int8_t* const qr = q + r * ldq;
+        const row_pieces<T> row(xr, cols);
+        const uint4* const xp = reinterpret_cast<const uint4*>(xr + row.head) + at;
+        uint4 v[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) v[j] = j * LANES + at < row.pieces ? __ldg(xp + j * LANES) : make_uint4(0, 0, 0, 0);
+        const float x0 = at < row.head ? to_f32(xr[at]) : 0.0f, x1 = at < row.tail ? to_f32(xr[cols - row.tail + at]) : 0.0f;
+        uint32_t a = max(__float_as_uint(x0) & 0x7fffffffu, __float_as_uint(x1) & 0x7fffffffu);   // the largest magnitude's bit pattern
+#pragma unroll
+        for (int j = 0; j < NV; ++j) a = max(a, q_largest<T>(v[j]));
+#pragma unroll
+        for (int o = LANES / 2; o; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+        const q_row k(a);
+        int8_t* const qp = qr + row.head;
+        const bool whole = (reinterpret_cast<uintptr_t>(qp) & (N - 1)) == 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * LANES + at < row.pieces) q_store<T>(qp + (j * LANES + at) * N, whole, v[j], k);
+        if (at < row.head) qr[at] = (int8_t)k.integer(x0);
+        if (at < row.tail) qr[cols - row.tail + at] = (int8_t)k.integer(x1);
+        if (at == 0) scale[r] = k.scale;
+    }
+}
+
 template <typename T> int quantize_launch(s2v_ctx* ctx, cudaStream_t st, int64_t rows, int64_t cols, const T* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale)
 {
     const int64_t pieces = cols / PIECE<T>;
-    const auto go = [&](auto kernel, int64_t blocks) {
-        const int64_t cap = (int64_t)1 << 20;
+    const auto go = [&](auto kernel, int64_t per_block) {
+        const int64_t blocks = (rows + per_block - 1) / per_block, cap = (int64_t)1 << 20;
         kernel<<<(unsigned)(blocks < cap ? blocks : cap), QR_CTA, 0, st>>>(rows, cols, x, ldx, q, ldq, scale);
         S2V_CHECK_LAUNCH(ctx, "quantize_rows_kernel");
         return (int)S2V_OK;
     };
-    const int64_t per_warp = (rows + QR_CTA / 32 - 1) / (QR_CTA / 32);
-    if (pieces <= 32) return go(quantize_rows_kernel<T, 1, 32>, per_warp);
-    if (pieces <= 128) return go(quantize_rows_kernel<T, 4, 32>, per_warp);
-    if (pieces <= 2 * QR_CTA) return go(quantize_rows_kernel<T, 2, QR_CTA>, rows);
-    if (pieces <= 4 * QR_CTA) return go(quantize_rows_kernel<T, 4, QR_CTA>, rows);
-    return go(quantize_rows_kernel<T, 8, QR_CTA>, rows);
+    if (pieces <= 8) return go(quantize_short_rows_kernel<T, 8, 1>, QR_CTA / 8);
+    if (pieces <= 32) return go(quantize_short_rows_kernel<T, 8, 4>, QR_CTA / 8);
+    if (pieces <= 64) return go(quantize_short_rows_kernel<T, 8, 8>, QR_CTA / 8);
+    if (pieces <= 128) return go(quantize_rows_kernel<T, 4, 32>, QR_CTA / 32);
+    if (pieces <= 2 * QR_CTA) return go(quantize_rows_kernel<T, 2, QR_CTA>, 1);
+    if (pieces <= 4 * QR_CTA) return go(quantize_rows_kernel<T, 4, QR_CTA>, 1);
+    return go(quantize_rows_kernel<T, 8, QR_CTA>, 1);
 }
 
 int check_quantize(s2v_ctx* ctx, const char* name, int64_t rows, int64_t cols, int x_type, const void* x, int64_t ldx)

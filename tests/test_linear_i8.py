@@ -107,7 +107,7 @@ def test_no_context_and_workspace_sizes():
 # ---------------------------------------------------------------- quantised rows
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,cols,pad", [(1, 1, 0), (1, 1000, 0), (3, 17, 0), (7, 128, 1), (64, 128, 0), (300, 82, 3), (5, 4099, 2), (2, 70001, 0), (2500, 256, 8), (37, 8192, 0)])
+@pytest.mark.parametrize("rows,cols,pad", [(1, 1, 0), (1, 1000, 0), (3, 17, 0), (7, 128, 1), (64, 128, 0), (300, 82, 3), (5, 4099, 2), (2, 70001, 0), (2500, 256, 8), (37, 8192, 0), (90, 29, 0), (1111, 63, 1), (500, 129, 0), (64, 254, 3)])
 def test_quantized_rows(gpu_ctx, dtype, rows, cols, pad):
     gen = generator(rows * 7 + cols)
     x, _ = matrix(rows, cols, cols + pad, gen, TYPES[dtype])
