@@ -1,6 +1,8 @@
 // C = act((a_scale x b_scale) * (A B^T) + bias) for 8-bit A [m x k] and B [n x k]: tcgen05 matrix instructions with 32-bit integer accumulators.
 //
-// A persistent CTA per SM walks over tiles of 128 x BN outputs.  One warp copies panels of 128 bytes along k (tensor maps, 128-byte swizzle; zeros
+// A persistent CTA per SM walks over tiles of 128 x BN outputs, or a pair of CTAs over tiles of 256 x 256: each keeps 128 rows of A and 128 of B,
+// and one instruction multiplies all of A by all of B into both tensor memories.  (A CTA by itself needs 384 rows a tile: 94 bytes a cycle and SM from
+// L2, more than it gives, and the tensor cores were busy 71 % of the time.)  One warp copies panels of 128 bytes along k (tensor maps, 128-byte swizzle; zeros
 // outside the matrices) into a ring, one issues the products, eight take finished accumulators out of tensor memory, of which there are two, so
 // that a tile's outputs are written under the next tile's products.
 #include <cstring>
@@ -16,11 +18,12 @@ constexpr int GI_EPI = 8;                              // epilogue warps
 constexpr int GI_THREADS = 32 * (2 + GI_EPI);
 constexpr int GI_PIECE = 64, GI_BOX = 32 * GI_PIECE;    // bytes of a row that an epilogue warp hands over at a time; of its 32 rows
 
-template <int BN> struct GiCfg {
-    static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 5 : 7, BOXES = BN == 256 ? 1 : 2;   // boxes of an epilogue warp
+template <int BN, bool PAIR> struct GiCfg {
+    static constexpr int B_ROWS = PAIR ? BN / 2 : BN;   // of B, in this CTA's shared memory
+    static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = B_ROWS * 128, STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = PAIR ? 6 : BN == 256 ? 4 : BN == 128 ? 5 : 7, BOXES = BN == 256 ? 1 : 2;   // boxes of an epilogue warp
     static constexpr uint32_t TM_COLS = 2 * BN;
-    static constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);   // s32 <- s8 x s8, M = 128, N = BN
+    static constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);   // s32 <- s8 x s8, M = 128 or 256, N = BN
     static constexpr uint32_t OFF_OUT = STAGES * STAGE;                       // per epilogue warp: its boxes
     static constexpr uint32_t OFF_SCALE = OFF_OUT + GI_EPI * BOXES * GI_BOX;   // per epilogue warp: the scales of half a tile's channels, then their biases
     static constexpr uint32_t OFF_BAR = OFF_SCALE + GI_EPI * BN * 4;
@@ -42,16 +45,64 @@ struct GiArgs {
     s2v_device_status* status;
 };
 
-__device__ __forceinline__ void gi_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+template <bool PAIR> __device__ __forceinline__ void gi_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
 {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-        :
-        : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+            :
+            : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+            :
+            : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+            : "memory");
 }
+// the barrier of this CTA, or of both of the pair, once all products issued so far are done
+template <bool PAIR> __device__ __forceinline__ void gi_commit(uint32_t bar)
+{
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// tc_wait for barriers on which the other CTA of the pair arrives too
+__device__ __forceinline__ bool gi_wait_pair(uint32_t bar, uint32_t parity, volatile int* abort_flag, s2v_device_status* status, int site)
+{
+    int spins = 0;
+    bool ok = true;
+    for (;;) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done)
+                     : "r"(bar), "r"(parity), "r"(TC_SUSPEND_NS)
+                     : "memory");
+        if (done) break;
+        if (*abort_flag) { ok = false; break; }
+        if (++spins > TC_WAIT_LIMIT) {
+            *abort_flag = 1;
+            status->code = S2V_ERR_DEVICE_TIMEOUT;
+            status->where = site;
+            ok = false;
+            break;
+        }
+    }
+    return __all_sync(0xffffffffu, ok);
+}
+// the address of a barrier in the pair's first CTA
+__device__ __forceinline__ uint32_t gi_first(uint32_t bar)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(bar));
+    return r;
+}
+
 // Tiles in columns of 16 row tiles, so that the tiles of one moment share panels of both matrices in L2.
 __device__ __forceinline__ void gi_tile(int tile, int m_tiles, int n_tiles, int& tm, int& tn)
 {
@@ -99,11 +150,11 @@ __device__ __forceinline__ void gi_write(const GiArgs& a, const CUtensorMap* map
     }
 }
 
-template <typename T, int BN>
+template <typename T, int BN, bool PAIR>
 __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c, const GiArgs a)
 {
-    using Cfg = GiCfg<BN>;
-    constexpr int STAGES = Cfg::STAGES;
+    using Cfg = GiCfg<BN, PAIR>;
+    constexpr int STAGES = Cfg::STAGES, CTAS = PAIR ? 2 : 1;
     extern __shared__ unsigned char gi_raw[];
     unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(gi_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t smem0 = smem_u32(smem);
@@ -111,20 +162,26 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + Cfg::OFF_MISC);
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_MISC + 8);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tiles = a.m_tiles * a.n_tiles;
+    const int tiles = a.m_tiles * a.n_tiles, rank = PAIR ? (int)(blockIdx.x & 1) : 0, unit = (int)blockIdx.x / CTAS, units = (int)gridDim.x / CTAS;
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) tc_mbar_init(bar(Cfg::FULL + i), 1), tc_mbar_init(bar(Cfg::EMPTY + i), 1);
-        for (int i = 0; i < 2; ++i) tc_mbar_init(bar(Cfg::DONE + i), 1), tc_mbar_init(bar(Cfg::READ + i), GI_EPI);
+        for (int i = 0; i < 2; ++i) tc_mbar_init(bar(Cfg::DONE + i), 1), tc_mbar_init(bar(Cfg::READ + i), GI_EPI * CTAS);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         if (a.kblocks > 0) tma_prefetch_map(&map_a), tma_prefetch_map(&map_b);
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(Cfg::TM_COLS) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(Cfg::TM_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(Cfg::TM_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if constexpr (PAIR) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // both CTAs' barriers are there
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
 
@@ -132,53 +189,67 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
     if (warp == 0) {   // copies
         int it = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+        for (int tile = unit; ok && tile < tiles; tile += units) {
             int tm, tn;
             gi_tile(tile, a.m_tiles, a.n_tiles, tm, tn);
             for (int kb = 0; kb < a.kblocks; ++kb, ++it) {
                 const int s = it % STAGES;
                 if (it >= STAGES && !(ok = tc_wait(bar(Cfg::EMPTY + s), (uint32_t)(it / STAGES - 1) & 1u, abort_flag, a.status, 70))) break;
                 if (tc_elect()) {
-                    const uint32_t at = smem0 + (uint32_t)s * Cfg::STAGE, b = bar(Cfg::FULL + s);
-                    mbar_expect(b, Cfg::STAGE);
-                    tma_load_2d(at, &map_a, kb * 128, tm * 128, b);
-                    tma_load_2d(at + Cfg::A_BYTES, &map_b, kb * 128, tn * BN, b);
+                    const uint32_t at = smem0 + (uint32_t)s * Cfg::STAGE;
+                    if constexpr (PAIR) {   // both CTAs' copies count on the first one's barrier, where the products are issued
+                        if (rank == 0) mbar_expect(bar(Cfg::FULL + s), 2 * Cfg::STAGE);
+                        const uint32_t b = gi_first(bar(Cfg::FULL + s));
+                        tma_load_2d_pair(at, &map_a, kb * 128, tm * 256 + rank * 128, b);
+                        tma_load_2d_pair(at + Cfg::A_BYTES, &map_b, kb * 128, tn * BN + rank * Cfg::B_ROWS, b);
+                    } else {
+                        const uint32_t b = bar(Cfg::FULL + s);
+                        mbar_expect(b, Cfg::STAGE);
+                        tma_load_2d(at, &map_a, kb * 128, tm * 128, b);
+                        tma_load_2d(at + Cfg::A_BYTES, &map_b, kb * 128, tn * BN, b);
+                    }
                 }
                 __syncwarp();
             }
         }
-        // no copy may arrive once the CTA has gone: where a wait gave up, the ones under way are waited for here (bounded like every wait)
-        if (!ok || *abort_flag)
+        if constexpr (PAIR)   // nor an arrival of the products', which the pair's first CTA sends to both
+            for (int i = max(0, it - STAGES); ok && i < it; ++i) ok = tc_wait(bar(Cfg::EMPTY + i % STAGES), (uint32_t)(i / STAGES) & 1u, abort_flag, a.status, 70);
+        // No copy may arrive once the CTA has gone: where a wait gave up, the ones under way are waited for here (bounded like every wait; those of a pair
+        // by its first CTA, and neither leaves before the other).
+        if (rank == 0 && (!ok || *abort_flag))
             for (int i = max(0, it - STAGES); i < it; ++i) {
                 int spins = 0;
                 while (!tc_mbar_try(bar(Cfg::FULL + i % STAGES), (uint32_t)(i / STAGES) & 1u))
                     if (++spins > TC_WAIT_LIMIT) break;
             }
-    } else if (warp == 1) {   // products
+    } else if (warp == 1) {   // products, by the first CTA of a pair for both
         int it = 0, t = 0;
-        bool ok = true;
-        for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++t) {
+        bool ok = rank == 0;
+        for (int tile = unit; ok && tile < tiles; tile += units, ++t) {
             const int acc = t & 1;
-            if (t >= 2 && !(ok = tc_wait(bar(Cfg::READ + acc), (uint32_t)(t / 2 - 1) & 1u, abort_flag, a.status, 71))) break;
+            if (t >= 2 && !(ok = PAIR ? gi_wait_pair(bar(Cfg::READ + acc), (uint32_t)(t / 2 - 1) & 1u, abort_flag, a.status, 71)
+                                      : tc_wait(bar(Cfg::READ + acc), (uint32_t)(t / 2 - 1) & 1u, abort_flag, a.status, 71)))
+                break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (int kb = 0; kb < a.kblocks; ++kb, ++it) {
                 const int s = it % STAGES;
-                if (!(ok = tc_wait(bar(Cfg::FULL + s), (uint32_t)(it / STAGES) & 1u, abort_flag, a.status, 72))) break;
+                if (!(ok = PAIR ? gi_wait_pair(bar(Cfg::FULL + s), (uint32_t)(it / STAGES) & 1u, abort_flag, a.status, 72)
+                                : tc_wait(bar(Cfg::FULL + s), (uint32_t)(it / STAGES) & 1u, abort_flag, a.status, 72)))
+                    break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (tc_elect()) {
                     const uint64_t da = tc_b_desc(smem0 + (uint32_t)s * Cfg::STAGE), db = tc_b_desc(smem0 + (uint32_t)s * Cfg::STAGE + Cfg::A_BYTES);
                     const int steps = kb + 1 == a.kblocks ? a.last_steps : 4;
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks)
-                        if (ks < steps) gi_mma(tmem + (uint32_t)(acc * BN), da + 2u * ks, db + 2u * ks, Cfg::IDESC, kb > 0 || ks > 0);
-                    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar(Cfg::EMPTY + s)) : "memory");
-                    if (kb + 1 == a.kblocks)
-                        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar(Cfg::DONE + acc)) : "memory");
+                        if (ks < steps) gi_mma<PAIR>(tmem + (uint32_t)(acc * BN), da + 2u * ks, db + 2u * ks, Cfg::IDESC, kb > 0 || ks > 0);
+                    gi_commit<PAIR>(bar(Cfg::EMPTY + s));
+                    if (kb + 1 == a.kblocks) gi_commit<PAIR>(bar(Cfg::DONE + acc));
                 }
                 __syncwarp();
             }
         }
-        if (!ok || *abort_flag)   // products under way read shared memory and write tensor memory
+        if (rank == 0 && (!ok || *abort_flag))   // products under way read shared memory and write tensor memory
             for (int i = max(0, it - STAGES); i < it; ++i) {
                 int spins = 0;
                 while (!tc_mbar_try(bar(Cfg::EMPTY + i % STAGES), (uint32_t)(i / STAGES) & 1u))
@@ -192,11 +263,11 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
         int turn = 0;
         float* const chan = reinterpret_cast<float*>(smem + Cfg::OFF_SCALE) + e * BN;
         int t = 0;
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++t) {
+        for (int tile = unit; tile < tiles; tile += units, ++t) {
             int tm, tn;
             gi_tile(tile, a.m_tiles, a.n_tiles, tm, tn);
             const int acc = t & 1;
-            const int64_t row0 = (int64_t)tm * 128 + quarter * 32, first = (int64_t)tn * BN + half * HALF;
+            const int64_t row0 = (int64_t)tm * (128 * CTAS) + rank * 128 + quarter * 32, first = (int64_t)tn * BN + half * HALF;
             const float sa = row0 + lane < a.m ? a.a_scale[row0 + lane] : 0.0f;
 #pragma unroll
             for (int u = lane; u < HALF; u += 32) {
@@ -204,7 +275,9 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
                 chan[HALF + u] = a.bias && first + u < a.n ? __ldg(a.bias + first + u) : 0.0f;
             }
             __syncwarp();
-            if (a.kblocks > 0 && !tc_wait(bar(Cfg::DONE + acc), (uint32_t)(t / 2) & 1u, abort_flag, a.status, 73)) break;
+            if (a.kblocks > 0 && !(PAIR ? gi_wait_pair(bar(Cfg::DONE + acc), (uint32_t)(t / 2) & 1u, abort_flag, a.status, 73)
+                                        : tc_wait(bar(Cfg::DONE + acc), (uint32_t)(t / 2) & 1u, abort_flag, a.status, 73)))
+                break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t at = tmem + (uint32_t)(acc * BN + half * HALF) + ((uint32_t)quarter << 21);
             const int cols = row0 >= a.m ? 0 : (int)min((int64_t)HALF, a.n - first);   // (the same for the warp)
@@ -227,7 +300,10 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
                 turn = (turn + 1) % Cfg::BOXES;
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            if (lane == 0) tc_mbar_arrive(bar(Cfg::READ + acc));
+            if (lane == 0) {
+                if constexpr (PAIR) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(gi_first(bar(Cfg::READ + acc))) : "memory");
+                else tc_mbar_arrive(bar(Cfg::READ + acc));
+            }
             __syncwarp();
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -235,18 +311,23 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if constexpr (PAIR) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // (the other one's arrivals and copies)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::TM_COLS) : "memory");
+    if (warp == 1) {
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::TM_COLS) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::TM_COLS) : "memory");
+    }
 }
 
-template <typename T, int BN> int gi_launch(s2v_ctx* ctx, cudaStream_t st, const s2v_gemm_i8_args& g, bool dependent)
+template <typename T, int BN, bool PAIR> int gi_launch(s2v_ctx* ctx, cudaStream_t st, const s2v_gemm_i8_args& g, bool dependent)
 {
-    using Cfg = GiCfg<BN>;
+    using Cfg = GiCfg<BN, PAIR>;
+    constexpr int ROWS = PAIR ? 256 : 128;
     CUtensorMap map_a, map_b, map_c;
     if (g.k > 0) {
         // (the leading dimension of a single row is not the caller's to get right)
         const int64_t up = (g.k + 15) / 16 * 16;
-        if (!s2v_byte_matrix_map(&map_a, g.A, g.m, g.k, g.m > 1 ? g.lda : up, 128) || !s2v_byte_matrix_map(&map_b, g.B, g.n, g.k, g.n > 1 ? g.ldb : up, BN))
+        if (!s2v_byte_matrix_map(&map_a, g.A, g.m, g.k, g.m > 1 ? g.lda : up, 128) || !s2v_byte_matrix_map(&map_b, g.B, g.n, g.k, g.n > 1 ? g.ldb : up, Cfg::B_ROWS))
             return s2v_fail(ctx, S2V_ERR_CUDA, "gemm_i8: the driver did not take a matrix's tensor map");
     } else {
         memset(&map_a, 0, sizeof(map_a));
@@ -256,7 +337,7 @@ template <typename T, int BN> int gi_launch(s2v_ctx* ctx, cudaStream_t st, const
     a.m = g.m, a.n = g.n, a.ldc = g.ldc;
     a.kblocks = (int)((g.k + 127) / 128);
     a.last_steps = g.k > 0 ? (int)((g.k - 128 * (int64_t)(a.kblocks - 1) + 31) / 32) : 0;
-    const int64_t mt = (g.m + 127) / 128, nt = (g.n + BN - 1) / BN;
+    const int64_t mt = (g.m + ROWS - 1) / ROWS, nt = (g.n + BN - 1) / BN;
     if (mt * nt > INT32_MAX / 2) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, "gemm_i8: more than 2^30 tiles of outputs");
     a.m_tiles = (int)mt, a.n_tiles = (int)nt;
     a.a_scale = g.a_scale, a.b_scale = g.b_scale, a.bias = g.bias, a.C = g.C, a.relu = g.relu;
@@ -265,20 +346,23 @@ template <typename T, int BN> int gi_launch(s2v_ctx* ctx, cudaStream_t st, const
     if (!a.boxes) memset(&map_c, 0, sizeof(map_c));
     else if (!s2v_output_map(&map_c, g.c_type, g.C, g.m, g.n, ldc)) return s2v_fail(ctx, S2V_ERR_CUDA, "gemm_i8: the driver did not take the output's tensor map");
     a.status = ctx->dstatus_dev;
-    S2V_CUDA_OK(ctx, s2v_allow_shared(gemm_i8_kernel<T, BN>, Cfg::SMEM));
-    const int64_t tiles = mt * nt;
-    const unsigned grid = (unsigned)(tiles < ctx->sm_count ? tiles : ctx->sm_count);
+    S2V_CUDA_OK(ctx, s2v_allow_shared(gemm_i8_kernel<T, BN, PAIR>, Cfg::SMEM));
+    const int64_t tiles = mt * nt, units = ctx->sm_count / (PAIR ? 2 : 1);
+    const unsigned grid = (unsigned)(tiles < units ? tiles : units) * (PAIR ? 2 : 1);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(GI_THREADS);
     cfg.dynamicSmemBytes = Cfg::SMEM;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = PAIR ? 2 : 1;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = dependent ? 1 : 0;
-    S2V_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, gemm_i8_kernel<T, BN>, map_a, map_b, map_c, a));
+    cfg.numAttrs = dependent ? 2 : 1;
+    S2V_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, gemm_i8_kernel<T, BN, PAIR>, map_a, map_b, map_c, a));
     S2V_CHECK_LAUNCH(ctx, "gemm_i8_kernel");
     return S2V_OK;
 }
@@ -292,8 +376,9 @@ int s2v_launch_gemm_i8(s2v_ctx* ctx, cudaStream_t st, const s2v_gemm_i8_args& g,
     if (g.k > 0 && (g.m <= 64 || mt * ((g.n + 63) / 64) < ctx->sm_count)) return s2v_launch_gemm_i8_split(ctx, st, g, dependent);
     return s2v_by_dtype(g.c_type, [&](auto type) {
         using T = decltype(type);
-        if (mt * ((g.n + 255) / 256) >= ctx->sm_count) return gi_launch<T, 256>(ctx, st, g, dependent);
-        if (mt * ((g.n + 127) / 128) >= ctx->sm_count) return gi_launch<T, 128>(ctx, st, g, dependent);
-        return gi_launch<T, 64>(ctx, st, g, dependent);
+        if (mt * ((g.n + 255) / 256) >= ctx->sm_count && g.k > 512 && ctx->sm_count >= 2) return gi_launch<T, 256, true>(ctx, st, g, dependent);
+        if (mt * ((g.n + 255) / 256) >= ctx->sm_count) return gi_launch<T, 256, false>(ctx, st, g, dependent);
+        if (mt * ((g.n + 127) / 128) >= ctx->sm_count) return gi_launch<T, 128, false>(ctx, st, g, dependent);
+        return gi_launch<T, 64, false>(ctx, st, g, dependent);
     });
 }

@@ -25,7 +25,7 @@ def quantized(x):
 
 def product(a, sa, b, sb, bias, relu):
     """In 64 bits, and the size of what was added up for the tolerance."""
-    acc = a.double().cpu() @ b.double().cpu().t()
+    acc = (a.to(b.device).double() @ b.double().t()).cpu()     # whole numbers below 2^31: exact in any order
     y = sa.double().cpu()[:, None] * sb.double().cpu()[None, :] * acc
     size = y.abs()
     if bias is not None:
@@ -163,7 +163,8 @@ def test_quantized_rows_without_columns(gpu_ctx):
 # ---------------------------------------------------------------- the product
 SHAPES = [(1, 1, 1), (1, 8, 16), (1, 333, 4096), (2, 1000, 100), (3, 17, 33), (5, 4096, 1024), (8, 129, 2047), (9, 250, 640), (16, 2048, 4096), (17, 640, 129),
           (33, 500, 1000), (64, 1536, 512), (65, 257, 8192), (100, 100, 100), (127, 127, 127), (128, 256, 128), (129, 255, 257), (300, 1021, 1504), (513, 770, 200),
-          (1000, 24, 4096), (2049, 264, 96), (1500, 1500, 1500), (4100, 513, 64)]
+          (1000, 24, 4096), (2049, 264, 96), (1500, 1500, 1500), (4100, 513, 64),
+          (2100, 2304, 640), (4000, 1300, 1000), (129, 38000, 520), (5000, 1025, 513)]
 
 
 @gpu
