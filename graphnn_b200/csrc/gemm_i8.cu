@@ -5,6 +5,7 @@
 // L2, more than it gives, and the tensor cores were busy 71 % of the time.)  One warp copies panels of 128 bytes along k (tensor maps, 128-byte swizzle; zeros
 // outside the matrices) into a ring, one issues the products, eight take finished accumulators out of tensor memory, of which there are two, so
 // that a tile's outputs are written under the next tile's products.
+#include <cmath>
 #include <cstring>
 
 #include "gemm_i8.cuh"
@@ -21,7 +22,7 @@ constexpr int GI_PIECE = 64, GI_BOX = 32 * GI_PIECE;    // bytes of a row that a
 template <int BN, bool PAIR> struct GiCfg {
     static constexpr int B_ROWS = PAIR ? BN / 2 : BN;   // of B, in this CTA's shared memory
     static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = B_ROWS * 128, STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = PAIR ? 6 : BN == 256 ? 4 : BN == 128 ? 5 : 7, BOXES = BN == 256 ? 1 : 2;   // boxes of an epilogue warp
+    static constexpr int STAGES = PAIR ? (BN == 256 ? 6 : 7) : BN == 256 ? 4 : BN == 128 ? 5 : 7, BOXES = BN == 256 ? 1 : 2;   // boxes of an epilogue warp
     static constexpr uint32_t TM_COLS = 2 * BN;
     static constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);   // s32 <- s8 x s8, M = 128 or 256, N = BN
     static constexpr uint32_t OFF_OUT = STAGES * STAGE;                       // per epilogue warp: its boxes
@@ -42,6 +43,7 @@ struct GiArgs {
     const float* bias;
     void* C;
     int relu, boxes;                // boxes: the output has a tensor map (16-byte aligned rows)
+    uint32_t bytes;                 // of a panel of this CTA
     s2v_device_status* status;
 };
 
@@ -141,12 +143,38 @@ __device__ __forceinline__ void gi_write(const GiArgs& a, const CUtensorMap* map
         __syncwarp();
         if (lane == 0) tma_store_2d(map, (int)col0, (int)row0, smem_u32(box));
     } else {
+        // Rows that start anywhere: 16 lanes a row, a word of four bytes each.  In a row of 16-bit numbers at an odd place a lane writes the second half of
+        // its word with the first half of its neighbour's, the first lane the first number and the last lane the last one.
         __syncwarp();
-        T* const C = static_cast<T*>(a.C);
-        for (int e = lane; e < 32 * COLS; e += 32) {
-            const int r = e / COLS, c = e % COLS;
-            if (row0 + r < a.m && col0 + c < a.n) C[(row0 + r) * a.ldc + col0 + c] = reinterpret_cast<const T*>(piece(r, c / PER))[c % PER];
+        const int l = lane & 15, hi = lane >> 4;
+        T* const to = static_cast<T*>(a.C) + (row0 + hi) * a.ldc + col0;
+        const int cols = (int)min((int64_t)COLS, a.n - col0), rows = (int)min((int64_t)32, a.m - row0);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const unsigned char* const from = box + hi * GI_PIECE + u * 2 * GI_PIECE + 16 * ((l >> 2) ^ u) + 4 * (l & 3);   // (rows of this u have the same swizzle)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = hi + 2 * u + 8 * i;
+                T* const at = to + (2 * u + 8 * i) * a.ldc;
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(from + i * 8 * GI_PIECE);
+                if constexpr (sizeof(T) == 4) {
+                    if (r < rows && l < cols) *reinterpret_cast<uint32_t*>(at + l) = w;
+                } else {
+                    uint16_t* const h = reinterpret_cast<uint16_t*>(at) + 2 * l;
+                    const uint32_t next = __shfl_down_sync(0xffffffffu, w, 1);
+                    if (r >= rows) continue;
+                    if ((reinterpret_cast<uintptr_t>(h) & 2) == 0) {
+                        if (2 * l + 1 < cols) *reinterpret_cast<uint32_t*>(h) = w;
+                        else if (2 * l < cols) h[0] = (uint16_t)w;
+                    } else {
+                        if (l < 15 && 2 * l + 2 < cols) *reinterpret_cast<uint32_t*>(h + 1) = __byte_perm(w, next, 0x5432);
+                        else if (2 * l + 1 < cols) h[1] = (uint16_t)(w >> 16);
+                        if (l == 0) h[0] = (uint16_t)w;
+                    }
+                }
+            }
         }
+        __syncwarp();
     }
 }
 
@@ -198,13 +226,13 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
                 if (tc_elect()) {
                     const uint32_t at = smem0 + (uint32_t)s * Cfg::STAGE;
                     if constexpr (PAIR) {   // both CTAs' copies count on the first one's barrier, where the products are issued
-                        if (rank == 0) mbar_expect(bar(Cfg::FULL + s), 2 * Cfg::STAGE);
+                        if (rank == 0) mbar_expect(bar(Cfg::FULL + s), 2 * a.bytes);
                         const uint32_t b = gi_first(bar(Cfg::FULL + s));
                         tma_load_2d_pair(at, &map_a, kb * 128, tm * 256 + rank * 128, b);
                         tma_load_2d_pair(at + Cfg::A_BYTES, &map_b, kb * 128, tn * BN + rank * Cfg::B_ROWS, b);
                     } else {
                         const uint32_t b = bar(Cfg::FULL + s);
-                        mbar_expect(b, Cfg::STAGE);
+                        mbar_expect(b, a.bytes);
                         tma_load_2d(at, &map_a, kb * 128, tm * 128, b);
                         tma_load_2d(at + Cfg::A_BYTES, &map_b, kb * 128, tn * BN, b);
                     }
@@ -323,11 +351,13 @@ template <typename T, int BN, bool PAIR> int gi_launch(s2v_ctx* ctx, cudaStream_
 {
     using Cfg = GiCfg<BN, PAIR>;
     constexpr int ROWS = PAIR ? 256 : 128;
+    // (a box with many rows outside the matrix takes longer than a full one: 27 rows of 128, 22 us instead of 16)
+    const int box_a = (int)(g.m < 128 ? g.m : 128), box_b = (int)(g.n < Cfg::B_ROWS ? g.n : Cfg::B_ROWS);
     CUtensorMap map_a, map_b, map_c;
     if (g.k > 0) {
         // (the leading dimension of a single row is not the caller's to get right)
         const int64_t up = (g.k + 15) / 16 * 16;
-        if (!s2v_byte_matrix_map(&map_a, g.A, g.m, g.k, g.m > 1 ? g.lda : up, 128) || !s2v_byte_matrix_map(&map_b, g.B, g.n, g.k, g.n > 1 ? g.ldb : up, Cfg::B_ROWS))
+        if (!s2v_byte_matrix_map(&map_a, g.A, g.m, g.k, g.m > 1 ? g.lda : up, box_a) || !s2v_byte_matrix_map(&map_b, g.B, g.n, g.k, g.n > 1 ? g.ldb : up, box_b))
             return s2v_fail(ctx, S2V_ERR_CUDA, "gemm_i8: the driver did not take a matrix's tensor map");
     } else {
         memset(&map_a, 0, sizeof(map_a));
@@ -339,7 +369,7 @@ template <typename T, int BN, bool PAIR> int gi_launch(s2v_ctx* ctx, cudaStream_
     a.last_steps = g.k > 0 ? (int)((g.k - 128 * (int64_t)(a.kblocks - 1) + 31) / 32) : 0;
     const int64_t mt = (g.m + ROWS - 1) / ROWS, nt = (g.n + BN - 1) / BN;
     if (mt * nt > INT32_MAX / 2) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, "gemm_i8: more than 2^30 tiles of outputs");
-    a.m_tiles = (int)mt, a.n_tiles = (int)nt;
+    a.m_tiles = (int)mt, a.n_tiles = (int)nt, a.bytes = (uint32_t)(box_a + box_b) * 128;
     a.a_scale = g.a_scale, a.b_scale = g.b_scale, a.bias = g.bias, a.C = g.C, a.relu = g.relu;
     const int64_t es = sizeof(T), ldc = g.m > 1 ? g.ldc : (g.n * es + 15) / 16 * 16 / es;
     a.boxes = s2v_aligned16(g.C) && ldc * es % 16 == 0;
@@ -367,18 +397,47 @@ template <typename T, int BN, bool PAIR> int gi_launch(s2v_ctx* ctx, cudaStream_
     return S2V_OK;
 }
 
+// What a call takes by each form, in us, fitted to times of 148 SMs (16-bit outputs, every form at k = 128 to 14336, n = 256 to 14336, m = 16 to
+// 20000; mostly within 15 %): `fixed` with the first tile's outputs, `first` and `next` for 128 columns of k in the first and in further tiles of a CTA
+// (the further ones share L2 with everybody), `out` for a further tile's outputs where they take longer than that.  Measured sides of some choices:
+//                          256 x 256 pair  256 x 128 pair  128 x 256  128 x 128  128 x 64   split
+//     4096 x 4096 x 4096        47              79             56         97                             (m x n x k)
+//     1024 x 4096 x 4096        17.5            22.7           18.5       25.8       42.8
+//      512 x 4096 x 4096        16.5            14.4           17.4       15.6       23.7       22
+//      200 x  256 x 4096        15.4            12.8           16.3       13.9       12.9        8.0
+//       64 x 4096 x  512         8.0             6.5            7.2        5.7        5.1        7.2
+//       27 x 4096 x 4096        15.3            13.0           16.2       14.0       13.2        7.2
+//    20000 x 4096 x  128        72              94             57         67         89
+struct GiForm {
+    int rows, bn;
+    float fixed, first, next, out;
+};
+constexpr GiForm GI_PAIR_256{256, 256, 6.6f, .33f, .335f, 3.9f}, GI_PAIR_128{256, 128, 5.3f, .28f, .28f, 2.6f}, GI_256{128, 256, 5.8f, .40f, .42f, 3.15f},
+    GI_128{128, 128, 4.4f, .33f, .345f, 1.9f}, GI_64{128, 64, 3.8f, .30f, .31f, 1.26f};
+
+float gi_cost(const s2v_ctx* ctx, const s2v_gemm_i8_args& g, const GiForm& f)
+{
+    const int64_t units = ctx->sm_count / (f.rows / 128);
+    if (units == 0) return INFINITY;
+    const float panels = (float)((g.k + 127) / 128), waves = (float)((((g.m + f.rows - 1) / f.rows) * ((g.n + f.bn - 1) / f.bn) + units - 1) / units);
+    const float out = f.out * (g.c_type == S2V_F32 ? 1.45f : 1.0f), next = f.next * panels;
+    return f.fixed + out - f.out + f.first * panels + (waves - 1.0f) * (out > next ? out : next);
+}
+
 }  // namespace
 
 int s2v_launch_gemm_i8(s2v_ctx* ctx, cudaStream_t st, const s2v_gemm_i8_args& g, bool dependent)
 {
     if (s2v_gemv_i8_takes(g.m, g.n, g.k)) return s2v_launch_gemv_i8(ctx, st, -1, g);
-    const int64_t mt = (g.m + 127) / 128;
-    if (g.k > 0 && (g.m <= 64 || mt * ((g.n + 63) / 64) < ctx->sm_count)) return s2v_launch_gemm_i8_split(ctx, st, g, dependent);
+    const GiForm* best = &GI_64;
+    float least = gi_cost(ctx, g, GI_64);
+    for (const GiForm* f : {&GI_128, &GI_256, &GI_PAIR_128, &GI_PAIR_256})
+        if (const float c = gi_cost(ctx, g, *f); g.k > 0 && c < least) best = f, least = c;
+    if (g.k > 0 && s2v_gemm_i8_split_cost(ctx, g) < least) return s2v_launch_gemm_i8_split(ctx, st, g, dependent);
     return s2v_by_dtype(g.c_type, [&](auto type) {
         using T = decltype(type);
-        if (mt * ((g.n + 255) / 256) >= ctx->sm_count && g.k > 512 && ctx->sm_count >= 2) return gi_launch<T, 256, true>(ctx, st, g, dependent);
-        if (mt * ((g.n + 255) / 256) >= ctx->sm_count) return gi_launch<T, 256, false>(ctx, st, g, dependent);
-        if (mt * ((g.n + 127) / 128) >= ctx->sm_count) return gi_launch<T, 128, false>(ctx, st, g, dependent);
-        return gi_launch<T, 64, false>(ctx, st, g, dependent);
+        return best == &GI_PAIR_256 ? gi_launch<T, 256, true>(ctx, st, g, dependent) : best == &GI_PAIR_128 ? gi_launch<T, 128, true>(ctx, st, g, dependent)
+             : best == &GI_256      ? gi_launch<T, 256, false>(ctx, st, g, dependent) : best == &GI_128      ? gi_launch<T, 128, false>(ctx, st, g, dependent)
+                                                                                                            : gi_launch<T, 64, false>(ctx, st, g, dependent);
     });
 }

@@ -19,4 +19,5 @@ int s2v_launch_gemm_i8(s2v_ctx* ctx, cudaStream_t st, const s2v_gemm_i8_args& a,
 bool s2v_gemv_i8_takes(int64_t m, int64_t n, int64_t k);
 int s2v_launch_gemv_i8(s2v_ctx* ctx, cudaStream_t st, int x_type, const s2v_gemm_i8_args& a);
 // gemm_i8_few.cu: outputs of few tiles, k > 0
+float s2v_gemm_i8_split_cost(const s2v_ctx* ctx, const s2v_gemm_i8_args& a);   // us, about
 int s2v_launch_gemm_i8_split(s2v_ctx* ctx, cudaStream_t st, const s2v_gemm_i8_args& a, bool dependent);

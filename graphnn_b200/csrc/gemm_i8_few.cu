@@ -1,5 +1,7 @@
 // Products with few tokens, where reading the weights once is everything: a kernel without matrix instructions for up to 8 tokens (which also
 // quantises them on the way), and one that splits k among the CTAs of a cluster for outputs of few tiles.
+#include <cmath>
+
 #include "gemm_i8.cuh"
 #include "quantize.cuh"
 #include "tcgen05.cuh"
@@ -165,13 +167,14 @@ template <typename TX> int gv_by_size(s2v_ctx* ctx, cudaStream_t st, int y_type,
 // ---------------------------------------------------------------- few tiles of outputs: k split among a cluster
 // A CTA multiplies 128 weight rows (the rows of the accumulator) by NT tokens over its share of k; the integers of the shares are added through
 // the cluster's shared memory, each CTA finishing an equal part of the tokens.  (Integer sums: the order does not matter.)
-constexpr int GS_THREADS = 32 * 6;
+constexpr int GS_EPI = 8, GS_THREADS = 32 * (2 + GS_EPI);   // epilogue warps: two for each quarter of the weight rows, sharing the tokens
 template <int NT> struct GsCfg {
     static constexpr uint32_t W_BYTES = 128 * 128, STAGE = W_BYTES + NT * 128;
     static constexpr int STAGES = NT <= 32 ? 5 : NT == 64 ? 4 : 3;   // about 100 KB: two CTAs an SM
     static constexpr uint32_t TM_COLS = NT < 32 ? 32 : NT;
     static constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);   // s32 <- s8 x s8, M = 128, N = NT
-    static constexpr uint32_t OFF_BAR = STAGES * STAGE;
+    static constexpr uint32_t OFF_SCALE = STAGES * STAGE;          // of the tokens
+    static constexpr uint32_t OFF_BAR = OFF_SCALE + NT * 4;
     enum { FULL = 0, EMPTY = FULL + STAGES, DONE = EMPTY + STAGES, BARS = DONE + 1 };
     static constexpr uint32_t OFF_MISC = OFF_BAR + 8 * BARS;
     static constexpr uint32_t SMEM = OFF_MISC + 16 + 1024;
@@ -233,7 +236,18 @@ __global__ void __launch_bounds__(GS_THREADS) gemm_i8_split_kernel(const __grid_
     const int row = (warp & 3) * 32 + lane;                     // epilogue: this thread's weight row
     const int64_t col = (int64_t)tn * 128 + row;
     int* const mine = reinterpret_cast<int*>(smem);             // [NT][128]
+    float* const token_scale = reinterpret_cast<float*>(smem + Cfg::OFF_SCALE);
+    float sw = 0.0f, bias = 0.0f;
     bool done = true;
+    const int half = (warp - 2) >> 2;
+    const int tokens = (int)min((int64_t)NT, a.m - (int64_t)tm * NT);
+    T* const out = static_cast<T*>(a.C) + (int64_t)tm * NT * a.ldc + col;
+    const float least = a.relu ? 0.0f : -INFINITY;
+    const auto put = [&](int t, int sum) {
+        float v = fmaf(__fmul_rn(token_scale[t], sw), (float)sum, bias);
+        v = v < least ? least : v;   // (NaN stays)
+        if (t < tokens && col < a.n) out[t * a.ldc] = from_f32<T>(v);
+    };
 
     if (warp == 0) {   // copies: the first weights before the tokens, which a kernel in front may still be writing
         const int ahead = min(STAGES, steps_k);
@@ -289,16 +303,24 @@ __global__ void __launch_bounds__(GS_THREADS) gemm_i8_split_kernel(const __grid_
                     if (++spins > TC_WAIT_LIMIT) break;
             }
     } else {
+        asm volatile("griddepcontrol.wait;" ::: "memory");   // the tokens' scales
+        for (int t = (int)threadIdx.x - 64; t < NT; t += 32 * GS_EPI) token_scale[t] = (int64_t)tm * NT + t < a.m ? a.a_scale[(int64_t)tm * NT + t] : 0.0f;
+        if (col < a.n) sw = __ldg(a.b_scale + col), bias = a.bias ? __ldg(a.bias + col) : 0.0f;
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * GS_EPI) : "memory");
         done = tc_wait(bar(Cfg::DONE), 0, abort_flag, a.status, 76);
         if (done) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-            for (int h = 0; h < NT; h += 16) {
+            for (int h = 16 * half; h < NT; h += 32) {
                 uint32_t v[16];
                 tc_ld_cols16(tmem + (uint32_t)h + ((uint32_t)(warp & 3) << 21), v);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                if (a.ctas == 1) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) mine[(h + j) * 128 + row] = (int)v[j];   // (every panel has been read)
+                    for (int j = 0; j < 16; ++j) put(h + j, (int)v[j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) mine[(h + j) * 128 + row] = (int)v[j];   // (every panel has been read)
+                }
             }
         }
     }
@@ -308,15 +330,13 @@ __global__ void __launch_bounds__(GS_THREADS) gemm_i8_split_kernel(const __grid_
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::TM_COLS) : "memory");
-    if (warp >= 2 && done) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");   // the tokens' scales
-        const float sw = col < a.n ? __ldg(a.b_scale + col) : 0.0f, b = a.bias && col < a.n ? __ldg(a.bias + col) : 0.0f;
+    if (warp >= 2 && done && a.ctas > 1) {
         uint32_t from[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c)
             if (c < a.ctas) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from[c]) : "r"(smem_u32(mine + row)), "r"(c));
-        const int t0 = rank * NT / a.ctas, t1 = (rank + 1) * NT / a.ctas;
-        constexpr int G = NT < 32 ? 2 : 8;   // tokens whose sums are on their way at once (a load from another CTA takes as long as one from L2)
+        const int share = NT / a.ctas / 2, t0 = rank * 2 * share + half * share, t1 = t0 + share;
+        constexpr int G = NT < 32 ? 2 : NT < 128 ? 4 : 8;   // tokens whose sums are on their way at once (a load from another CTA takes as long as one from L2)
         for (int t = t0; t < t1; t += G) {
             int part[G][8];
 #pragma unroll
@@ -328,14 +348,10 @@ __global__ void __launch_bounds__(GS_THREADS) gemm_i8_split_kernel(const __grid_
                 }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                const int64_t token = (int64_t)tm * NT + t + g;
                 int sum = 0;
 #pragma unroll
                 for (int c = 0; c < 8; ++c) sum += part[g][c];
-                if (t + g < t1 && token < a.m && col < a.n) {
-                    const float v = fmaf(__fmul_rn(a.a_scale[token], sw), (float)sum, b);
-                    static_cast<T*>(a.C)[token * a.ldc + col] = from_f32<T>(a.relu ? relu_ref(v) : v);
-                }
+                if (t + g < t1) put(t + g, sum);
             }
         }
     }
@@ -394,12 +410,36 @@ int s2v_launch_gemv_i8(s2v_ctx* ctx, cudaStream_t st, int x_type, const s2v_gemm
     return s2v_by_dtype(x_type, [&](auto type) { return gv_by_size<decltype(type)>(ctx, st, g.c_type, a); });
 }
 
+// the split form for a call: tokens of a tile, tiles, and CTAs that share a tile's k
+struct GsPlan {
+    int nt, ctas;
+    int64_t tiles, kblocks;
+    GsPlan(const s2v_ctx* ctx, const s2v_gemm_i8_args& g)
+    {
+        nt = g.m <= 16 ? 16 : g.m <= 32 ? 32 : g.m <= 64 ? 64 : 128;
+        tiles = (g.n + 127) / 128 * ((g.m + nt - 1) / nt);
+        kblocks = (g.k + 127) / 128;
+        // A CTA an SM, two where k is long (16 tokens, n = 4096: k = 4096 6.7 us with four CTAs a tile, 8.3 with eight; 4096 tokens of k = 14336 the same, 14336 x 14336 40.5 with
+        // one CTA a tile, 36.5 with two)
+        const int64_t most = ctx->sm_count * (kblocks >= 64 ? 2 : 1);
+        ctas = 1;
+        while (ctas < 8 && tiles * ctas * 2 <= most && kblocks >= 4 * ctas) ctas *= 2;
+    }
+};
+
+float s2v_gemm_i8_split_cost(const s2v_ctx* ctx, const s2v_gemm_i8_args& g)
+{
+    const GsPlan p(ctx, g);
+    const float each = (float)p.kblocks / p.ctas, waves = (float)((p.tiles * p.ctas + ctx->sm_count - 1) / ctx->sm_count);
+    if (g.m > 64 && p.tiles > ctx->sm_count) return INFINITY;   // (nothing to gain: there are enough tiles)
+    const float fixed = p.nt <= 32 ? 4.0f : p.nt == 64 ? 4.5f : 5.6f, panel = p.nt <= 32 ? .34f : p.nt == 64 ? .38f : .46f, outputs = (p.ctas > 1 ? .05f : .012f) * p.nt / p.ctas;
+    return fixed + outputs + panel * each * (1.0f + .7f * (waves - 1.0f)) + outputs * (waves - 1.0f);
+}
+
 int s2v_launch_gemm_i8_split(s2v_ctx* ctx, cudaStream_t st, const s2v_gemm_i8_args& g, bool dependent)
 {
-    const int NT = g.m <= 16 ? 16 : g.m <= 32 ? 32 : g.m <= 64 ? 64 : 128;
-    const int64_t tiles = (g.n + 127) / 128 * ((g.m + NT - 1) / NT), kblocks = (g.k + 127) / 128;
-    int ctas = 1;
-    while (ctas < 8 && tiles * ctas * 2 <= 2 * ctx->sm_count && kblocks >= 4 * ctas) ctas *= 2;
+    const GsPlan p(ctx, g);
+    const int NT = p.nt, ctas = p.ctas;
     return s2v_by_dtype(g.c_type, [&](auto type) {
         using T = decltype(type);
         if (NT == 16) return gs_launch<T, 16>(ctx, st, g, ctas, dependent);
