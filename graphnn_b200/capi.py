@@ -219,8 +219,8 @@ def _matrix(name: str, t, device: int, rows: int, cols: int, dtype) -> int:
 
 
 def _vector(name: str, t, device: int, length: int):
-    """Checks an fp32 device vector (or None)."""
-    if t is not None and not (t.dtype is torch.float32 and t.get_device() == device and t.shape == (length,) and t.is_contiguous()):
+    """Checks an fp32 device vector."""
+    if not (t.dtype is torch.float32 and t.get_device() == device and t.shape == (length,) and t.is_contiguous()):
         _refuse(f"{name} is no contiguous fp32 vector of {length} on cuda:{device}, but {tuple(t.shape)} of {t.dtype} on {t.device}")
 
 
@@ -323,7 +323,8 @@ class Context:
 
     def call(self, name: str, *args):
         rc = getattr(self.lib, name)(self.h, *args)
-        self.check(rc)
+        if rc != 0:
+            self.check(rc)
 
     @property
     def stream(self) -> int:
@@ -427,8 +428,10 @@ class Context:
         lda, ldb, ldc = _matrix("A", A, dev, m, k, torch.int8), _matrix("B", B, dev, n, k, torch.int8), _matrix("C_out", C_out, dev, m, n, dtype)
         _vector("a_scale", a_scale, dev, m)
         _vector("b_scale", b_scale, dev, n)
-        _vector("bias", bias, dev, n)
-        self.call("s2v_gemm_i8", stream, m, n, k, A.data_ptr(), lda, a_scale.data_ptr(), B.data_ptr(), ldb, b_scale.data_ptr(), _ptr(bias),
+        if bias is not None:
+            _vector("bias", bias, dev, n)
+            bias = bias.data_ptr()
+        self.call("s2v_gemm_i8", stream, m, n, k, A.data_ptr(), lda, a_scale.data_ptr(), B.data_ptr(), ldb, b_scale.data_ptr(), bias,
                   1 if relu else 0, _DTYPES[dtype], C_out.data_ptr(), ldc)
         return C_out
 
@@ -440,38 +443,50 @@ class Context:
         (m, k, xtype), (rows, n, ytype), dev = _sizes("x", x), _sizes("y", y), self.device
         ldx, ldw, ldy = _matrix("x", x, dev, m, k, xtype), _matrix("W", W, dev, n, k, torch.int8), _matrix("y", y, dev, m, n, ytype)
         _vector("w_scale", w_scale, dev, n)
-        _vector("bias", bias, dev, n)
+        if bias is not None:
+            _vector("bias", bias, dev, n)
+            bias = bias.data_ptr()
         if workspace.get_device() != dev or not workspace.is_contiguous():
             _refuse("workspace is not contiguous or on another device")
-        self.call("s2v_linear_i8", stream, m, n, k, _DTYPES[xtype], x.data_ptr(), ldx, W.data_ptr(), ldw, w_scale.data_ptr(), _ptr(bias), 1 if relu else 0,
-                  workspace.data_ptr(), workspace.numel() * workspace.element_size(), _DTYPES[ytype], y.data_ptr(), ldy)
+        self.call("s2v_linear_i8", stream, m, n, k, _DTYPES[xtype], x.data_ptr(), ldx, W.data_ptr(), ldw, w_scale.data_ptr(), bias, 1 if relu else 0,
+                  workspace.data_ptr(), workspace.nbytes, _DTYPES[ytype], y.data_ptr(), ldy)
         return y
 
     # -- distillation from a teacher's top logits
-    def _distill_args(self, z, idx, t, temperature, t_lse, row_weight, stats, dz):
+    def _distill_args(self, z, idx, t, temperature, t_lse, row_weight, loss, stats, dz):
         (rows, cols, dtype), (_, top, ttype), dev = _sizes("z", z), _sizes("t", t), self.device
         ldz, ldt = _matrix("z", z, dev, rows, cols, dtype), _matrix("t", t, dev, rows, top, ttype)
         if _matrix("idx", idx, dev, rows, top, torch.int32) != ldt and rows > 1:
             _refuse("idx and t need the same leading dimension")
-        _vector("t_lse", t_lse, dev, rows)
-        _vector("row_weight", row_weight, dev, rows)
-        if stats is not None and _matrix("stats", stats, dev, rows, 4, torch.float32) != 4 and rows > 1:
-            _refuse("stats is not contiguous")
-        lddz = 0 if dz is None else _matrix("dz", dz, dev, rows, cols, dtype)
-        return (rows, cols, _DTYPES[dtype], z.data_ptr(), ldz, top, idx.data_ptr(), _DTYPES[ttype], t.data_ptr(), ldt, _ptr(t_lse), temperature, _ptr(row_weight)), lddz
+        if t_lse is not None:
+            _vector("t_lse", t_lse, dev, rows)
+            t_lse = t_lse.data_ptr()
+        if row_weight is not None:
+            _vector("row_weight", row_weight, dev, rows)
+            row_weight = row_weight.data_ptr()
+        if loss is not None:
+            _vector("loss", loss, dev, rows)
+        if stats is not None:
+            if _matrix("stats", stats, dev, rows, 4, torch.float32) != 4 and rows > 1:
+                _refuse("stats is not contiguous")
+            stats = stats.data_ptr()
+        lddz = 0
+        if dz is not None:
+            lddz = _matrix("dz", dz, dev, rows, cols, dtype)
+            dz = dz.data_ptr()
+        return (rows, cols, _DTYPES[dtype], z.data_ptr(), ldz, top, idx.data_ptr(), _DTYPES[ttype], t.data_ptr(), ldt, t_lse, temperature, row_weight), (stats, dz, lddz)
 
     def distill_topk(self, z, idx, t, loss, temperature=1.0, t_lse=None, row_weight=None, stats=None, dz=None, stream=None):
         """s2v_distill_topk: loss[i] = row_weight[i] * KL(teacher's top logits || student's row z[i]); dz (may be z): its gradient;
         stats: float [rows x 4] kept for distill_topk_grad."""
-        args, lddz = self._distill_args(z, idx, t, temperature, t_lse, row_weight, stats, dz)
-        _vector("loss", loss, self.device, args[0])
-        self.call("s2v_distill_topk", stream, *args, loss.data_ptr(), _ptr(stats), _ptr(dz), lddz)
+        args, out = self._distill_args(z, idx, t, temperature, t_lse, row_weight, loss, stats, dz)
+        self.call("s2v_distill_topk", stream, *args, loss.data_ptr(), *out)
         return loss
 
     def distill_topk_grad(self, z, idx, t, stats, dz, temperature=1.0, t_lse=None, row_weight=None, stream=None):
         """s2v_distill_topk_grad: the gradient of sum(row_weight * KL) from the stats of distill_topk."""
-        args, lddz = self._distill_args(z, idx, t, temperature, t_lse, row_weight, stats, dz)
-        self.call("s2v_distill_topk_grad", stream, *args, _ptr(stats), _ptr(dz), lddz)
+        args, out = self._distill_args(z, idx, t, temperature, t_lse, row_weight, None, stats, dz)
+        self.call("s2v_distill_topk_grad", stream, *args, *out)
         return dz
 
     def segment_sum(self, seg_ptr, H, Y, stream=None, average=False):

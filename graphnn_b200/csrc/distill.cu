@@ -289,9 +289,9 @@ __device__ __forceinline__ float dt_loss(const DtArgs& a, const DtList& l, const
     return (float)(kl * weight);
 }
 
-// ---------------------------------------------------------------- rows of up to 256 pieces: a warp each
-// The row stays in registers between the sums and the gradient.
-constexpr int DW_WARPS = 4, DW_PIECES = 8;   // pieces a lane
+// ---------------------------------------------------------------- rows of up to 512 pieces: a warp each
+// The row stays in registers between the sums and the gradient.  (16384 x 2500 bf16 by CTAs of 128 threads: 153 us.)
+constexpr int DW_WARPS = 4, DW_PIECES = 16;   // pieces a lane, at most
 struct DwShared {
     double P[DT_TOP];
     float z[DT_TOP];
@@ -715,7 +715,8 @@ __global__ void __launch_bounds__(DC_THREADS, CTAS_SM) distill_cluster_kernel(co
 }
 
 // The gradient from kept sums: nothing to wait for but the list.
-// (A CTA of 512 threads a long row: 4096 x 131072 bf16 345 us, 6.2 TB/s; with clusters of four such CTAs 454.)
+// (A CTA a row, of 128 threads up to 4096 pieces, else 256: 16384 x 9000 bf16 128 us, with 256 threads 177 and with 512 282; 4096 x 131072 bf16 349 us,
+// 6.2 TB/s, with 128 threads 364, and 454 where four CTAs shared a row.)
 template <typename T, int DG_THREADS> __global__ void __launch_bounds__(DG_THREADS, 1024 / DG_THREADS) distill_grad_kernel(const DtArgs a, int ctas)
 {
     __shared__ DcShared s;
@@ -815,15 +816,15 @@ template <typename T, bool GRAD_ONLY> int dt_launch_type(s2v_ctx* ctx, cudaStrea
 {
     const int64_t pieces = a.cols / PIECE<T>;
     if (pieces <= 32) return dw_launch<T, 1, GRAD_ONLY>(ctx, st, a);
+    if (pieces <= 32 * 8) return dw_launch<T, 8, GRAD_ONLY>(ctx, st, a);
     if (pieces <= 32 * DW_PIECES) return dw_launch<T, DW_PIECES, GRAD_ONLY>(ctx, st, a);
     int ctas = 1;
-    const bool small = pieces <= DC_SHORT && a.top <= 128;
     if constexpr (GRAD_ONLY) {
         while (ctas < DC_CTAS && a.rows * ctas < 2 * ctx->sm_count && pieces >= (int64_t)ctas * 1024) ctas *= 2;
-        return small ? dg_launch<T, 128>(ctx, st, a, ctas) : dg_launch<T, 512>(ctx, st, a, ctas);
+        return pieces <= 2 * DC_SHORT && a.top <= 128 ? dg_launch<T, 128>(ctx, st, a, ctas) : dg_launch<T, 256>(ctx, st, a, ctas);
     } else {
         while (ctas < DC_CTAS && (pieces > (int64_t)ctas * DC_RUN || (a.rows * ctas < 2 * ctx->sm_count && pieces >= (int64_t)ctas * 512))) ctas *= 2;
-        return small ? dc_launch<T, 128, 6>(ctx, st, a, ctas) : dc_launch<T, 256, 3>(ctx, st, a, ctas);
+        return pieces <= DC_SHORT && a.top <= 128 ? dc_launch<T, 128, 6>(ctx, st, a, ctas) : dc_launch<T, 256, 3>(ctx, st, a, ctas);
     }
 }
 int dt_launch(s2v_ctx* ctx, s2v_stream stream, int z_type, bool grad_only, const DtArgs& a)
