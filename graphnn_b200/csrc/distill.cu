@@ -4,8 +4,8 @@
 // S_out the same over the rest.  With M the larger maximum and total = S_in exp((M_in - M) / T) + S_out exp((M_out - M) / T),
 //     log q_j = (z_j - M) / T - log total,     log s = -log(1 + exp(d)),  d = log(S_in / S_out) + (M_in - M_out) / T.
 // Taking one sum from the other's total would lose s (or 1 - s) where the student gives nearly everything (or nothing) to the list, and one
-// maximum for both would lose the smaller sum where they are far apart (logits masked with the type's lowest value).  Whatever exists once per
-// row or per entry is computed in 64 bits, the sums over columns in fp32.
+// maximum for both would lose the smaller sum where they are far apart (logits masked with the type's lowest value).  The loss is put together in 64
+// bits (it is a difference of larger numbers), the sums over columns and the gradient in fp32.
 #include "elem_types.cuh"
 
 namespace
@@ -251,7 +251,7 @@ __device__ __forceinline__ DtCoef dt_coefficients(const DtArgs& a, double Z, con
     const float total = m == -INFINITY ? NAN : in.s * e_in + out.s * e_out;
     float given, rest;
     if (a.t_lse) {
-        given = (float)Z;
+        given = (float)(Z + (Z - Z));     // (infinite: NaN)
         rest = Z > 1.0 ? 0.0f : (float)(1.0 - Z);
         k.p_scale = 1.0f;
     } else {
@@ -262,7 +262,7 @@ __device__ __forceinline__ DtCoef dt_coefficients(const DtArgs& a, double Z, con
     k.scale = weight * inv_t;
     const float both = __fdividef(given + rest, total);
     k.inner = k.scale * both;
-    k.outer = k.scale * (out.s == 0.0f && total == total ? 0.0f : both * e_out - __fdividef(rest, out.s));
+    k.outer = k.scale * (out.s == 0.0f && both == both ? 0.0f : both * e_out - __fdividef(rest, out.s));
     return k;
 }
 // (A warp's work, all lanes with the same arguments: its logarithms are taken side by side in three lanes.)
@@ -285,7 +285,7 @@ __device__ __forceinline__ float dt_loss(const DtArgs& a, const DtList& l, const
         if (out.s != 0.0f) kl += rest * (log_z + minus_log_s);
         else if (rest > 1.0 / 65536.0) kl = INFINITY;
     }
-    if (mf == -INFINITY) kl = NAN;
+    if (mf == -INFINITY || !(l.Z < INFINITY)) kl = NAN;
     return (float)(kl * weight);
 }
 
@@ -450,7 +450,7 @@ constexpr int DC_SLOTS = 512;                        // of the table that finds 
 struct DcShared {
     float P[DT_TOP], t[DT_TOP], z[DT_TOP];
     int id[DT_TOP], slot[DC_SLOTS];
-    float4 peer[2][DC_CTAS];   // outer and inner sums of the cluster's CTAs, two rows by turns
+    float4 peer[DC_CTAS];      // outer and inner sums of the cluster's CTAs
     float2 outer[16], inner[DC_LISTERS];
     float Z[DC_LISTERS], tmax[DC_LISTERS];
     int has[DC_LISTERS];       // bit 0: an entry; bit 1: a column that is listed twice
@@ -473,14 +473,13 @@ struct DcHead {
 // What every thread with an entry knows of it, before z is looked at.  P in fp32: the gradient's rest, 1 - sum P, is off by 2^-23 at most.
 struct DcEntry {
     float t, tmax, P;
-    int slot;     // its column's place in the table
     bool twice;   // whether another entry of this column was there first
 };
 __device__ __forceinline__ DcEntry dc_entry(const DtArgs& a, const DcHead& h, DcShared& s)
 {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const bool lister = warp * 32 < a.top;   // warps with entries
-    DcEntry e{h.id >= 0 ? h.t : -INFINITY, -INFINITY, 0.0f, 0, false};
+    DcEntry e{h.id >= 0 ? h.t : -INFINITY, -INFINITY, 0.0f, false};
     if (!a.t_lse) {
         if (lister) {
             const float m = dt_warp_max(e.t);
@@ -492,8 +491,8 @@ __device__ __forceinline__ DcEntry dc_entry(const DtArgs& a, const DcHead& h, Dc
     if (lister) {
         if (h.id >= 0) {
             e.P = expf(a.t_lse ? e.t * a.inv_t - h.t_lse : (e.t - dt_finite_or_zero(e.tmax)) * a.inv_t);
-            int was;
-            for (e.slot = h.id & (DC_SLOTS - 1); (was = atomicCAS(&s.slot[e.slot], -1, h.id)) != -1 && was != h.id; e.slot = (e.slot + 1) & (DC_SLOTS - 1)) {}
+            int was, at = h.id & (DC_SLOTS - 1);   // (twice as many places as entries)
+            while ((was = atomicCAS(&s.slot[at], -1, h.id)) != -1 && was != h.id) at = (at + 1) & (DC_SLOTS - 1);
             e.twice = was == h.id;
         }
         s.id[tid] = h.id;
@@ -571,48 +570,113 @@ __global__ void __launch_bounds__(DC_THREADS, CTAS_SM) distill_cluster_kernel(co
     for (int w = tid; w < (most - held + 3) / 4; w += DC_THREADS) marks[w] = 0;
     for (int w = tid; w < DC_SLOTS; w += DC_THREADS) s.slot[w] = -1;
     if (tid < DC_LISTERS) s.inner[tid] = make_float2(-INFINITY, 0.0f);   // (of the warps without entries, once and for all)
-    int turn = 0;
-    for (int64_t r = blockIdx.x / (unsigned)ctas; r < a.rows; r += gridDim.x / (unsigned)ctas) {
-        const T* const z = static_cast<const T*>(a.z) + r * a.ldz;
-        T* const dz = a.dz ? static_cast<T*>(a.dz) + r * a.lddz : nullptr;
-        const DcHead head(a, r);
-        const float weight = head.weight;
-        const DcRun<T> my(z, a.cols, rank, ctas);
-        const uint4* const zp = reinterpret_cast<const uint4*>(z + my.row.head) + my.first;
-        const bool skip_weight = weight == 0.0f && !a.stats;
-        const int kept = min(held, my.pieces);
-        if (!skip_weight)
-            for (int p = tid; p < kept; p += DC_THREADS) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(run + p)), "l"(zp + p) : "memory");
-        const DcEntry e = dc_entry(a, head, s);
-        int at;
-        const bool here = my.has(head.id, rank, ctas, at), held_entry = here && at >= 0 && at < held * N;
-        bool mine = here && !e.twice;
-        float P_all = e.P, zk = (here && !held_entry) || (rank == 0 && head.id >= 0) ? to_f32(z[head.id]) : -INFINITY;
-        if (here && at >= held * N) atomicOr(&marks[(at / N - held) >> 2], 1u << (8 * ((at / N - held) & 3) + at % N));
-        // the scalar columns: the head's to the first CTA, the tail's to the last
-        const bool in_head = rank == 0 && tid < my.row.head, in_tail = rank == ctas - 1 && tid >= 32 && tid < 32 + my.row.tail;
-        const int edge_at = in_head ? tid : (int)a.cols - my.row.tail + tid - 32;
-        const float edge = in_head || in_tail ? to_f32(z[edge_at]) : -INFINITY;
-        __syncthreads();
-        const int has = dc_has(a, e, s);
-        if (skip_weight || !(has & 1)) {   // (the same for all CTAs of the row)
-            if (rank == 0) {
-                if (tid == 0) a.loss[r] = 0.0f;
-                if (a.stats && tid < 4) a.stats[4 * r + tid] = 0.0f;
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            __syncthreads();   // (dz may be z)
-            if (head.id >= 0) s.slot[e.slot] = -1;
-            if (here && at >= held * N) marks[(at / N - held) >> 2] = 0;
-            if (dz) dt_zero_row(dz, a.cols, rank * DC_THREADS + tid, ctas * DC_THREADS);
-            continue;
+    const int64_t r = blockIdx.x / (unsigned)ctas;
+    const T* const z = static_cast<const T*>(a.z) + r * a.ldz;
+    T* const dz = a.dz ? static_cast<T*>(a.dz) + r * a.lddz : nullptr;
+    const DcHead head(a, r);
+    const float weight = head.weight;
+    const DcRun<T> my(z, a.cols, rank, ctas);
+    const uint4* const zp = reinterpret_cast<const uint4*>(z + my.row.head) + my.first;
+    const bool skip_weight = weight == 0.0f && !a.stats;
+    const int kept = min(held, my.pieces);
+    if (!skip_weight)
+        for (int p = tid; p < kept; p += DC_THREADS) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(run + p)), "l"(zp + p) : "memory");
+    __syncthreads();   // the table and the marks are empty
+    const DcEntry e = dc_entry(a, head, s);
+    int at;
+    const bool here = my.has(head.id, rank, ctas, at), held_entry = here && at >= 0 && at < held * N;
+    bool mine = here && !e.twice;
+    float P_all = e.P, zk = (here && !held_entry) || (rank == 0 && head.id >= 0) ? to_f32(z[head.id]) : -INFINITY;
+    if (here && at >= held * N) atomicOr(&marks[(at / N - held) >> 2], 1u << (8 * ((at / N - held) & 3) + at % N));
+    // the scalar columns: the head's to the first CTA, the tail's to the last
+    const bool in_head = rank == 0 && tid < my.row.head, in_tail = rank == ctas - 1 && tid >= 32 && tid < 32 + my.row.tail;
+    const int edge_at = in_head ? tid : (int)a.cols - my.row.tail + tid - 32;
+    const float edge = in_head || in_tail ? to_f32(z[edge_at]) : -INFINITY;
+    __syncthreads();
+    const int has = dc_has(a, e, s);
+    if (skip_weight || !(has & 1)) {   // (the same for all CTAs of the row)
+        if (rank == 0) {
+            if (tid == 0) a.loss[r] = 0.0f;
+            if (a.stats && tid < 4) a.stats[4 * r + tid] = 0.0f;
         }
-        bool edge_out = in_head || in_tail;   // not listed
-        if (edge_out)
-            for (int k = 0; k < a.top; ++k) edge_out &= s.id[k] != edge_at;
-        if ((has & 2) && here) mine = dc_first(a, head.id, s, P_all);
-        DtSum outer{-INFINITY, 0.0f}, inner{-INFINITY, 0.0f};
-        // what is not held, while the rest is on its way
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();   // (dz may be z)
+        if (dz) dt_zero_row(dz, a.cols, rank * DC_THREADS + tid, ctas * DC_THREADS);
+        return;
+    }
+    bool edge_out = in_head || in_tail;   // not listed
+    if (edge_out)
+        for (int k = 0; k < a.top; ++k) edge_out &= s.id[k] != edge_at;
+    if ((has & 2) && here) mine = dc_first(a, head.id, s, P_all);
+    DtSum outer{-INFINITY, 0.0f}, inner{-INFINITY, 0.0f};
+    // what is not held, while the rest is on its way
+    for (int p = held + tid; p < my.pieces; p += 4 * DC_THREADS) {
+        uint4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (p + j * DC_THREADS < my.pieces) v[j] = zp[p + j * DC_THREADS];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (p + j * DC_THREADS < my.pieces)
+                if (const uint32_t listed = mark[p + j * DC_THREADS]) dt_take_out<T>(v[j], listed);
+        outer.template add_pieces<T, 4>(v, p, DC_THREADS, my.pieces, c);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    if (mine && held_entry) {   // (one thread an element)
+        T* const element = reinterpret_cast<T*>(run) + at;
+        zk = to_f32(*element);
+        *element = from_f32<T>(-INFINITY);
+    }
+    if (warp * 32 < a.top) {
+        s.z[tid] = zk;
+        // (a listed z of -infinity adds nothing, +infinity and NaN make the sum NaN)
+        if (mine) inner = DtSum{zk, zk < INFINITY ? zk > -INFINITY ? 1.0f : 0.0f : NAN};
+        inner.template join<32>(c);
+        if (lane == 0) s.inner[warp] = make_float2(inner.m, inner.s);
+    }
+    __syncthreads();
+    for (int p = tid; p < kept; p += 4 * DC_THREADS) {
+        uint4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (p + j * DC_THREADS < kept) v[j] = run[p + j * DC_THREADS];
+        outer.template add_pieces<T, 4>(v, p, DC_THREADS, kept, c);
+    }
+    if (edge_out) outer.add_one(edge, c);
+    outer.template join<32>(c);
+    if (lane == 0) s.outer[warp] = make_float2(outer.m, outer.s);
+    __syncthreads();
+    if (warp == 0) {   // the CTA's sums: lanes 0 to 15 the outer ones, 16 to 23 the inner ones
+        const float2 o = lane < DC_WARPS ? s.outer[lane] : lane >= 16 && lane < 16 + DC_LISTERS ? s.inner[lane - 16] : make_float2(-INFINITY, 0.0f);
+        DtSum d{o.x, o.y};
+        d.template join<16>(c);
+        const float m_in = __shfl_sync(0xffffffffu, d.m, 16), s_in = __shfl_sync(0xffffffffu, d.s, 16);
+        if (lane < ctas) {
+            uint32_t to;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&s.peer[rank])), "r"(lane));
+            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(d.m), "f"(d.s), "f"(m_in), "f"(s_in) : "memory");
+        }
+        __syncwarp();
+    }
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    else __syncthreads();
+    {
+        const float4 o = (lane & 7) < ctas ? s.peer[lane & 7] : make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
+        DtSum d = lane & 8 ? DtSum{o.z, o.w} : DtSum{o.x, o.y};
+        d.template join<8>(c);
+        outer = DtSum{__shfl_sync(0xffffffffu, d.m, 0), __shfl_sync(0xffffffffu, d.s, 0)};
+        inner = DtSum{__shfl_sync(0xffffffffu, d.m, 8), __shfl_sync(0xffffffffu, d.s, 8)};
+    }
+    if (a.stats && rank == 0 && tid == DC_THREADS - 1) reinterpret_cast<float4*>(a.stats)[r] = make_float4(outer.m, outer.s, inner.m, inner.s);
+    if (dz && weight == 0.0f) {   // (for the stats alone; the cluster has read the row)
+        dt_zero_row(dz, a.cols, rank * DC_THREADS + tid, ctas * DC_THREADS);
+    } else if (dz) {
+        const DtCoef k = dt_coefficients(a, dc_Z(a, s), inner, outer, weight, inv_t, c);
+        const float base = dt_finite_or_zero(outer.m);
+        const uint64_t base2 = dt_two(-base, -base), outer2 = dt_two(k.outer, k.outer), c2 = dt_two(c, c);
+        T* const dp = dz + my.row.head + (int64_t)my.first * N;
+        const bool whole = (reinterpret_cast<uintptr_t>(dp) & 15) == 0;
         for (int p = held + tid; p < my.pieces; p += 4 * DC_THREADS) {
             uint4 v[4];
 #pragma unroll
@@ -620,97 +684,25 @@ __global__ void __launch_bounds__(DC_THREADS, CTAS_SM) distill_cluster_kernel(co
                 if (p + j * DC_THREADS < my.pieces) v[j] = zp[p + j * DC_THREADS];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (p + j * DC_THREADS < my.pieces)
-                    if (const uint32_t listed = mark[p + j * DC_THREADS]) dt_take_out<T>(v[j], listed);
-            outer.template add_pieces<T, 4>(v, p, DC_THREADS, my.pieces, c);
+                if (p + j * DC_THREADS < my.pieces) dt_store(dp + (p + j * DC_THREADS) * N, whole, v[j], base2, outer2, c2);
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncthreads();
-        if (mine && held_entry) {   // (one thread an element)
-            T* const element = reinterpret_cast<T*>(run) + at;
-            zk = to_f32(*element);
-            *element = from_f32<T>(-INFINITY);
-        }
-        if (warp * 32 < a.top) {
-            s.z[tid] = zk;
-            // (a listed z of -infinity adds nothing, +infinity and NaN make the sum NaN)
-            if (mine) inner = DtSum{zk, zk < INFINITY ? zk > -INFINITY ? 1.0f : 0.0f : NAN};
-            inner.template join<32>(c);
-            if (lane == 0) s.inner[warp] = make_float2(inner.m, inner.s);
-        }
-        __syncthreads();
-        for (int p = tid; p < kept; p += 4 * DC_THREADS) {
-            uint4 v[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (p + j * DC_THREADS < kept) v[j] = run[p + j * DC_THREADS];
-            outer.template add_pieces<T, 4>(v, p, DC_THREADS, kept, c);
-        }
-        if (edge_out) outer.add_one(edge, c);
-        outer.template join<32>(c);
-        if (lane == 0) s.outer[warp] = make_float2(outer.m, outer.s);
-        __syncthreads();
-        if (warp == 0) {   // the CTA's sums: lanes 0 to 15 the outer ones, 16 to 23 the inner ones
-            const float2 o = lane < DC_WARPS ? s.outer[lane] : lane >= 16 && lane < 16 + DC_LISTERS ? s.inner[lane - 16] : make_float2(-INFINITY, 0.0f);
-            DtSum d{o.x, o.y};
-            d.template join<16>(c);
-            const float m_in = __shfl_sync(0xffffffffu, d.m, 16), s_in = __shfl_sync(0xffffffffu, d.s, 16);
-            if (lane < ctas) {
-                uint32_t to;
-                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&s.peer[turn][rank])), "r"(lane));
-                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(d.m), "f"(d.s), "f"(m_in), "f"(s_in) : "memory");
-            }
-            __syncwarp();
-        }
-        if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-        else __syncthreads();
-        {
-            const float4 o = (lane & 7) < ctas ? s.peer[turn][lane & 7] : make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
-            DtSum d = lane & 8 ? DtSum{o.z, o.w} : DtSum{o.x, o.y};
-            d.template join<8>(c);
-            outer = DtSum{__shfl_sync(0xffffffffu, d.m, 0), __shfl_sync(0xffffffffu, d.s, 0)};
-            inner = DtSum{__shfl_sync(0xffffffffu, d.m, 8), __shfl_sync(0xffffffffu, d.s, 8)};
-        }
-        turn ^= 1;
-        if (a.stats && rank == 0 && tid == DC_THREADS - 1) reinterpret_cast<float4*>(a.stats)[r] = make_float4(outer.m, outer.s, inner.m, inner.s);
-        if (dz && weight == 0.0f) {   // (for the stats alone; the cluster has read the row)
-            dt_zero_row(dz, a.cols, rank * DC_THREADS + tid, ctas * DC_THREADS);
-        } else if (dz) {
-            const DtCoef k = dt_coefficients(a, dc_Z(a, s), inner, outer, weight, inv_t, c);
-            const float base = dt_finite_or_zero(outer.m);
-            const uint64_t base2 = dt_two(-base, -base), outer2 = dt_two(k.outer, k.outer), c2 = dt_two(c, c);
-            T* const dp = dz + my.row.head + (int64_t)my.first * N;
-            const bool whole = (reinterpret_cast<uintptr_t>(dp) & 15) == 0;
-            for (int p = held + tid; p < my.pieces; p += 4 * DC_THREADS) {
-                uint4 v[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (p + j * DC_THREADS < my.pieces) v[j] = zp[p + j * DC_THREADS];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (p + j * DC_THREADS < my.pieces) dt_store(dp + (p + j * DC_THREADS) * N, whole, v[j], base2, outer2, c2);
-            }
-            if (whole) {
+        if (whole) {
 #pragma unroll 4
-                for (int p = tid; p < kept; p += DC_THREADS) dt_store(dp + p * N, true, run[p], base2, outer2, c2);
-            } else {
-                for (int p = tid; p < kept; p += DC_THREADS) dt_store(dp + p * N, false, run[p], base2, outer2, c2);
-            }
-            if (edge_out) dz[edge_at] = from_f32<T>(dt_exp2((edge - base) * c) * k.outer);
-            __syncthreads();   // the listed columns have been written as the others
-            if (mine) dz[head.id] = from_f32<T>(k.inner * expf((zk - k.M) * inv_t) - k.scale * (P_all * k.p_scale));
+            for (int p = tid; p < kept; p += DC_THREADS) dt_store(dp + p * N, true, run[p], base2, outer2, c2);
+        } else {
+            for (int p = tid; p < kept; p += DC_THREADS) dt_store(dp + p * N, false, run[p], base2, outer2, c2);
         }
-        if (rank == 0 && warp == 0) {
-            DtList l{0.0, 0.0, 0.0, (double)inner.s, inner.m};
-            for (int k = lane; k < a.top; k += 32)
-                if (s.id[k] >= 0) dt_count(a, l, s.t[k], e.tmax, (double)head.t_lse, s.z[k], inv);
-            l.Z = dt_warp_sum(l.Z), l.A = dt_warp_sum(l.A), l.B = dt_warp_sum(l.B);
-            const float loss = dt_loss(a, l, outer, weight, inv, c);
-            if (lane == 0) a.loss[r] = weight == 0.0f ? 0.0f : loss;
-        }
-        __syncthreads();
-        if (head.id >= 0) s.slot[e.slot] = -1;
-        if (here && at >= held * N) marks[(at / N - held) >> 2] = 0;   // (a whole word, by each of its entries)
+        if (edge_out) dz[edge_at] = from_f32<T>(dt_exp2((edge - base) * c) * k.outer);
+        __syncthreads();   // the listed columns have been written as the others
+        if (mine) dz[head.id] = from_f32<T>(k.inner * expf((zk - k.M) * inv_t) - k.scale * (P_all * k.p_scale));
+    }
+    if (rank == 0 && warp == 0) {
+        DtList l{0.0, 0.0, 0.0, (double)inner.s, inner.m};
+        for (int k = lane; k < a.top; k += 32)
+            if (s.id[k] >= 0) dt_count(a, l, s.t[k], e.tmax, (double)head.t_lse, s.z[k], inv);
+        l.Z = dt_warp_sum(l.Z), l.A = dt_warp_sum(l.A), l.B = dt_warp_sum(l.B);
+        const float loss = dt_loss(a, l, outer, weight, inv, c);
+        if (lane == 0) a.loss[r] = weight == 0.0f ? 0.0f : loss;
     }
 }
 
@@ -725,63 +717,60 @@ template <typename T, int DG_THREADS> __global__ void __launch_bounds__(DG_THREA
     const int rank = (int)(blockIdx.x % (unsigned)ctas);
     const float inv_t = a.inv_t, c = a.c;
     for (int w = tid; w < DC_SLOTS; w += DG_THREADS) s.slot[w] = -1;
-    for (int64_t r = blockIdx.x / (unsigned)ctas; r < a.rows; r += gridDim.x / (unsigned)ctas) {
-        const T* const z = static_cast<const T*>(a.z) + r * a.ldz;
-        T* const dz = static_cast<T*>(a.dz) + r * a.lddz;
-        const DcHead head(a, r);
-        const float weight = head.weight;
-        const float4 st = __ldg(reinterpret_cast<const float4*>(a.stats) + r);
-        const DcRun<T> my(z, a.cols, rank, ctas);
-        const DcEntry e = dc_entry(a, head, s);
-        int at;
-        const bool here = my.has(head.id, rank, ctas, at);
-        bool mine = here && !e.twice;
-        float P_all = e.P;
-        const float zk = here ? to_f32(z[head.id]) : 0.0f;
-        const bool in_head = rank == 0 && tid < my.row.head, in_tail = rank == ctas - 1 && tid >= 32 && tid < 32 + my.row.tail;
-        const int edge_at = in_head ? tid : (int)a.cols - my.row.tail + tid - 32;
-        const float edge = in_head || in_tail ? to_f32(z[edge_at]) : 0.0f;
-        // (the barrier also stands between the reads of listed columns and the writes: dz may be z)
-        __syncthreads();
-        const int has = dc_has(a, e, s);
-        if ((has & 2) && here) mine = dc_first(a, head.id, s, P_all);
-        if (head.id >= 0) s.slot[e.slot] = -1;
-        if (weight == 0.0f || !(has & 1)) {
-            dt_zero_row(dz, a.cols, rank * DG_THREADS + tid, ctas * DG_THREADS);
-            __syncthreads();
-            continue;
-        }
-        const DtSum outer{st.x, st.y}, inner{st.z, st.w};
-        const DtCoef k = dt_coefficients(a, dc_Z(a, s), inner, outer, weight, inv_t, c);
-        const float base = dt_finite_or_zero(outer.m);
-        const uint64_t base2 = dt_two(-base, -base), outer2 = dt_two(k.outer, k.outer), c2 = dt_two(c, c);
-        const uint4* const zp = reinterpret_cast<const uint4*>(z + my.row.head) + my.first;
-        T* const dp = dz + my.row.head + (int64_t)my.first * N;
-        const bool whole = (reinterpret_cast<uintptr_t>(dp) & 15) == 0;
-        for (int p = tid; p < my.pieces; p += 4 * DG_THREADS) {
-            uint4 v[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (p + j * DG_THREADS < my.pieces) v[j] = zp[p + j * DG_THREADS];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (p + j * DG_THREADS < my.pieces) dt_store(dp + (p + j * DG_THREADS) * N, whole, v[j], base2, outer2, c2);
-        }
-        if (in_head || in_tail) dz[edge_at] = from_f32<T>(dt_exp2((edge - base) * c) * k.outer);
-        __syncthreads();   // the listed columns have been written as the others
-        if (mine) dz[head.id] = from_f32<T>(k.inner * expf((zk - k.M) * inv_t) - k.scale * (P_all * k.p_scale));
-        __syncthreads();
+    const int64_t r = blockIdx.x / (unsigned)ctas;
+    const T* const z = static_cast<const T*>(a.z) + r * a.ldz;
+    T* const dz = static_cast<T*>(a.dz) + r * a.lddz;
+    const DcHead head(a, r);
+    const float weight = head.weight;
+    const float4 st = __ldg(reinterpret_cast<const float4*>(a.stats) + r);
+    const DcRun<T> my(z, a.cols, rank, ctas);
+    __syncthreads();   // the table is empty
+    const DcEntry e = dc_entry(a, head, s);
+    int at;
+    const bool here = my.has(head.id, rank, ctas, at);
+    bool mine = here && !e.twice;
+    float P_all = e.P;
+    const float zk = here ? to_f32(z[head.id]) : 0.0f;
+    const bool in_head = rank == 0 && tid < my.row.head, in_tail = rank == ctas - 1 && tid >= 32 && tid < 32 + my.row.tail;
+    const int edge_at = in_head ? tid : (int)a.cols - my.row.tail + tid - 32;
+    const float edge = in_head || in_tail ? to_f32(z[edge_at]) : 0.0f;
+    // (the barrier also stands between the reads of listed columns and the writes: dz may be z)
+    __syncthreads();
+    const int has = dc_has(a, e, s);
+    if ((has & 2) && here) mine = dc_first(a, head.id, s, P_all);
+    if (weight == 0.0f || !(has & 1)) {
+        dt_zero_row(dz, a.cols, rank * DG_THREADS + tid, ctas * DG_THREADS);
+        return;
     }
+    const DtSum outer{st.x, st.y}, inner{st.z, st.w};
+    const DtCoef k = dt_coefficients(a, dc_Z(a, s), inner, outer, weight, inv_t, c);
+    const float base = dt_finite_or_zero(outer.m);
+    const uint64_t base2 = dt_two(-base, -base), outer2 = dt_two(k.outer, k.outer), c2 = dt_two(c, c);
+    const uint4* const zp = reinterpret_cast<const uint4*>(z + my.row.head) + my.first;
+    T* const dp = dz + my.row.head + (int64_t)my.first * N;
+    const bool whole = (reinterpret_cast<uintptr_t>(dp) & 15) == 0;
+    for (int p = tid; p < my.pieces; p += 4 * DG_THREADS) {
+        uint4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (p + j * DG_THREADS < my.pieces) v[j] = zp[p + j * DG_THREADS];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (p + j * DG_THREADS < my.pieces) dt_store(dp + (p + j * DG_THREADS) * N, whole, v[j], base2, outer2, c2);
+    }
+    if (in_head || in_tail) dz[edge_at] = from_f32<T>(dt_exp2((edge - base) * c) * k.outer);
+    __syncthreads();   // the listed columns have been written as the others
+    if (mine) dz[head.id] = from_f32<T>(k.inner * expf((zk - k.M) * inv_t) - k.scale * (P_all * k.p_scale));
 }
 
 template <typename T, int THREADS, int CTAS_SM> int dc_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a, int ctas)
 {
-    const int64_t most = (a.cols / PIECE<T> + ctas - 1) / ctas, rows = a.rows < (1 << 20) ? a.rows : 1 << 20;   // (clusters; further rows by turns)
+    const int64_t most = (a.cols / PIECE<T> + ctas - 1) / ctas;
     const int held = (int)(most < DC_HELD ? most : DC_HELD);
     const auto kernel = distill_cluster_kernel<T, THREADS, CTAS_SM>;
     S2V_CUDA_OK(ctx, s2v_allow_shared(kernel, DC_SMEM));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * ctas));
+    cfg.gridDim = dim3((unsigned)(a.rows * ctas));
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = (size_t)(held * 16 + (most - held + 3) / 4 * 4);
     cfg.stream = st;
@@ -797,8 +786,7 @@ template <typename T, int THREADS, int CTAS_SM> int dc_launch(s2v_ctx* ctx, cuda
 }
 template <typename T, int THREADS> int dg_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a, int ctas)
 {
-    const int64_t rows = a.rows < (1 << 20) ? a.rows : 1 << 20;
-    distill_grad_kernel<T, THREADS><<<(unsigned)(rows * ctas), THREADS, 0, st>>>(a, ctas);
+    distill_grad_kernel<T, THREADS><<<(unsigned)(a.rows * ctas), THREADS, 0, st>>>(a, ctas);
     S2V_CHECK_LAUNCH(ctx, "distill_grad_kernel");
     return S2V_OK;
 }
@@ -818,6 +806,7 @@ template <typename T, bool GRAD_ONLY> int dt_launch_type(s2v_ctx* ctx, cudaStrea
     if (pieces <= 32) return dw_launch<T, 1, GRAD_ONLY>(ctx, st, a);
     if (pieces <= 32 * 8) return dw_launch<T, 8, GRAD_ONLY>(ctx, st, a);
     if (pieces <= 32 * DW_PIECES) return dw_launch<T, DW_PIECES, GRAD_ONLY>(ctx, st, a);
+    if (a.rows * DC_CTAS > INT32_MAX) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, "distill_topk: more than 2^28 rows of this length");
     int ctas = 1;
     if constexpr (GRAD_ONLY) {
         while (ctas < DC_CTAS && a.rows * ctas < 2 * ctx->sm_count && pieces >= (int64_t)ctas * 1024) ctas *= 2;

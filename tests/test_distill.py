@@ -271,6 +271,40 @@ def test_rows_that_masks_leave_empty_and_values_that_are_not_finite(gpu_ctx, col
 
 
 @gpu
+@pytest.mark.parametrize("cols", [12, 700, 6000, 40000])
+@pytest.mark.parametrize("tail", [False, True])
+def test_teachers_that_are_not_finite(gpu_ctx, cols, tail):
+    z, idx, t, lse, w = inputs(6, cols, 5, "f32", cols, tail, 1.0, ragged=False)
+    w.fill_(0.5)
+    t[0, 1], t[1, 4], t[2, 0] = INF, float("nan"), -INF
+    idx[3, 2], t[3, 2] = -1, float("nan")               # an entry that is not there
+    if tail:
+        lse[4] = float("nan")
+    loss, dz = both_ways(gpu_ctx, z, idx, t, 1.0, lse, w)
+    for i in (0, 1, 4) if tail else (0, 1):
+        assert math.isnan(loss[i]) and bool(dz[i].isnan().all()), i
+    rows = [2, 3, 5]
+    assert_matches(loss[rows], dz[rows], z[rows], idx[rows], t[rows].nan_to_num(nan=0.0, neginf=-INF), 1.0, None if lse is None else lse[rows], w[rows])
+
+
+@gpu
+@pytest.mark.parametrize("cols", [40, 2000, 9000, 70000])
+@pytest.mark.parametrize("tail", [False, True])
+def test_lists_of_one_class_over_and_over(gpu_ctx, cols, tail):
+    """Every place of a full list names one of three classes, many rows at once: each class is counted once, with all its entries' p."""
+    rows, top = 300, 256
+    z, idx, t, lse, w = inputs(rows, cols, top, "f32", cols, tail, 1.0, ragged=False)
+    t.copy_(torch.randn(t.shape, device="cuda"))
+    idx.copy_((torch.arange(top, device="cuda")[None, :] * 7 + torch.arange(rows, device="cuda")[:, None]) % 3 * (cols // 3 - 1))
+    if tail:
+        lse.copy_(torch.logsumexp(t, 1) + 0.7)
+    loss, dz = both_ways(gpu_ctx, z, idx, t, 1.0, lse, w)
+    some = torch.arange(0, rows, 23)
+    at = some.cuda()
+    assert_matches(loss[at], dz[at], z[at], idx[at], t[at], 1.0, None if lse is None else lse[at], w[at])
+
+
+@gpu
 @pytest.mark.parametrize("cols", [10, 900, 30000])
 def test_a_class_outside_the_row_is_reported_and_left_out(gpu_ctx, cols):
     z, idx, t, lse, w = inputs(6, cols, 5, "f32", cols, True, 1.0, ragged=False)
