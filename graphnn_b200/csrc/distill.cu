@@ -827,21 +827,21 @@ int dt_launch(s2v_ctx* ctx, s2v_stream stream, int z_type, bool grad_only, const
 
 int dt_check(s2v_ctx* ctx, const char* name, int z_type, const DtArgs& a)
 {
-    const std::string who(name);
-    if (a.rows < 0 || a.cols <= 0 || a.top <= 0) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": negative or empty size");
-    if (!s2v_dtype_ok(z_type) || !s2v_dtype_ok(a.t_type)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": unknown element type");
-    if (!(a.temperature >= 1e-30f && a.temperature <= 1e30f)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": temperature outside [1e-30, 1e30]");
+    const auto bad = [&](int status, const char* what) { return s2v_fail(ctx, status, std::string(name) + ": " + what); };
+    if (a.rows < 0 || a.cols <= 0 || a.top <= 0) return bad(S2V_ERR_INVALID_ARG, "negative or empty size");
+    if (!s2v_dtype_ok(z_type) || !s2v_dtype_ok(a.t_type)) return bad(S2V_ERR_INVALID_ARG, "unknown element type");
+    if (!(a.temperature >= 1e-30f && a.temperature <= 1e30f)) return bad(S2V_ERR_INVALID_ARG, "temperature outside [1e-30, 1e30]");
     if (a.rows == 0) return S2V_OK;
-    if (!a.z || !a.idx || !a.t) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": NULL pointer");
-    if (a.top > DT_TOP) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, who + ": more than 256 entries a row");
-    if (a.cols * (int64_t)s2v_dtype_bytes(z_type) > DT_ROW_BYTES) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, who + ": rows of more than 1,048,576 bytes");
+    if (!a.z || !a.idx || !a.t) return bad(S2V_ERR_INVALID_ARG, "NULL pointer");
+    if (a.top > DT_TOP) return bad(S2V_ERR_UNSUPPORTED, "more than 256 entries a row");
+    if (a.cols * (int64_t)s2v_dtype_bytes(z_type) > DT_ROW_BYTES) return bad(S2V_ERR_UNSUPPORTED, "rows of more than 1,048,576 bytes");
     if (a.rows > 1 && (a.ldz < a.cols || a.ldt < a.top || (a.dz && a.lddz < a.cols)))
-        return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": leading dimension below the number of columns");
+        return bad(S2V_ERR_INVALID_ARG, "leading dimension below the number of columns");
     const size_t es = s2v_dtype_bytes(z_type);
     if (reinterpret_cast<uintptr_t>(a.z) % es || reinterpret_cast<uintptr_t>(a.dz) % es || reinterpret_cast<uintptr_t>(a.t) % s2v_dtype_bytes(a.t_type))
-        return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": misaligned pointer");
-    if (!s2v_aligned16(a.stats)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": stats must be 16-byte aligned");
-    if (a.dz == a.z && a.rows > 1 && a.lddz != a.ldz) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": dz in the place of z needs the same leading dimension");
+        return bad(S2V_ERR_INVALID_ARG, "misaligned pointer");
+    if (!s2v_aligned16(a.stats)) return bad(S2V_ERR_INVALID_ARG, "stats must be 16-byte aligned");
+    if (a.dz == a.z && a.rows > 1 && a.lddz != a.ldz) return bad(S2V_ERR_INVALID_ARG, "dz in the place of z needs the same leading dimension");
     return S2V_OK;
 }
 

@@ -115,7 +115,7 @@ __device__ __forceinline__ void gi_tile(int tile, int m_tiles, int n_tiles, int&
 }
 
 // The outputs of 32 rows (lanes) by COLS columns: into a box in shared memory (64-byte rows, their 16-byte pieces exchanged by the 64-byte swizzle,
-// which also keeps the stores free of bank conflicts), and from there by one copy that leaves out what the matrix does not have.  (Written by the
+// which also keeps the stores free of bank conflicts), and from there by one copy that leaves out rows and 16-byte pieces which the matrix does not have.  (Written by the
 // warp's own loads and stores, a product with few sums an output was bound by that: 491,520 x 256 outputs of fp32 over k = 128 158 us.)
 template <typename T, int HALF>
 __device__ __forceinline__ void gi_write(const GiArgs& a, const CUtensorMap* map, unsigned char* box, const float* chan, int64_t row0, int64_t col0, float sa, const uint32_t* v)
@@ -138,7 +138,8 @@ __device__ __forceinline__ void gi_write(const GiArgs& a, const CUtensorMap* map
         }
         *reinterpret_cast<uint4*>(piece(lane, j / PER)) = pack_piece(y, T());
     }
-    if (a.boxes) {
+    // (a copy that meets the end of a row inside 16 bytes writes zeros behind it, into what may be somebody else's)
+    if (a.boxes && (col0 + COLS <= a.n || a.n % PER == 0)) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) tma_store_2d(map, (int)col0, (int)row0, smem_u32(box));

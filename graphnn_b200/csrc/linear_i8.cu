@@ -112,14 +112,14 @@ template <typename T> int quantize_launch(s2v_ctx* ctx, cudaStream_t st, int64_t
 
 int check_quantize(s2v_ctx* ctx, const char* name, int64_t rows, int64_t cols, int x_type, const void* x, int64_t ldx)
 {
-    const std::string who(name);
-    if (rows < 0 || cols < 0) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": negative size");
-    if (!s2v_dtype_ok(x_type)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": unknown element type");
+    const auto bad = [&](int status, const char* what) { return s2v_fail(ctx, status, std::string(name) + ": " + what); };
+    if (rows < 0 || cols < 0) return bad(S2V_ERR_INVALID_ARG, "negative size");
+    if (!s2v_dtype_ok(x_type)) return bad(S2V_ERR_INVALID_ARG, "unknown element type");
     if (rows == 0) return S2V_OK;
-    if (cols > INT32_MAX) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, who + ": more than 2^31 - 1 columns");
-    if (cols > 0 && !x) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": NULL pointer");
-    if (rows > 1 && ldx < cols) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": leading dimension below the number of columns");
-    if (reinterpret_cast<uintptr_t>(x) % s2v_dtype_bytes(x_type)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": misaligned x");
+    if (cols > INT32_MAX) return bad(S2V_ERR_UNSUPPORTED, "more than 2^31 - 1 columns");
+    if (cols > 0 && !x) return bad(S2V_ERR_INVALID_ARG, "NULL pointer");
+    if (rows > 1 && ldx < cols) return bad(S2V_ERR_INVALID_ARG, "leading dimension below the number of columns");
+    if (reinterpret_cast<uintptr_t>(x) % s2v_dtype_bytes(x_type)) return bad(S2V_ERR_INVALID_ARG, "misaligned x");
     return S2V_OK;
 }
 
@@ -131,17 +131,17 @@ size_t workspace_scale_offset(int64_t m, int64_t k)
 int check_gemm(s2v_ctx* ctx, const char* name, int64_t m, int64_t n, int64_t k, const int8_t* B, int64_t ldb, const float* b_scale, int c_type, const void* C,
                int64_t ldc)
 {
-    const std::string who(name);
-    if (m < 0 || n < 0 || k < 0) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": negative size");
-    if (!s2v_dtype_ok(c_type)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": unknown element type");
+    const auto bad = [&](int status, const char* what) { return s2v_fail(ctx, status, std::string(name) + ": " + what); };
+    if (m < 0 || n < 0 || k < 0) return bad(S2V_ERR_INVALID_ARG, "negative size");
+    if (!s2v_dtype_ok(c_type)) return bad(S2V_ERR_INVALID_ARG, "unknown element type");
     if (m == 0 || n == 0) return S2V_OK;
-    if (!b_scale || !C || (k > 0 && !B)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": NULL pointer");
-    if (k > 131071) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, who + ": k beyond 131,071, where 32-bit sums can overflow");
-    if (m > INT32_MAX || n > INT32_MAX) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, who + ": more than 2^31 - 1 rows");
+    if (!b_scale || !C || (k > 0 && !B)) return bad(S2V_ERR_INVALID_ARG, "NULL pointer");
+    if (k > 131071) return bad(S2V_ERR_UNSUPPORTED, "k beyond 131,071, where 32-bit sums can overflow");
+    if (m > INT32_MAX || n > INT32_MAX) return bad(S2V_ERR_UNSUPPORTED, "more than 2^31 - 1 rows");
     if ((n > 1 && k > 0 && (ldb < k || ldb % 16 != 0)) || (m > 1 && ldc < n))
-        return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": leading dimension too small, or of an 8-bit matrix no multiple of 16");
-    if (!s2v_aligned16(B)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": 8-bit matrices must be 16-byte aligned");
-    if (reinterpret_cast<uintptr_t>(C) % s2v_dtype_bytes(c_type)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, who + ": misaligned output");
+        return bad(S2V_ERR_INVALID_ARG, "leading dimension too small, or of an 8-bit matrix no multiple of 16");
+    if (!s2v_aligned16(B)) return bad(S2V_ERR_INVALID_ARG, "8-bit matrices must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(C) % s2v_dtype_bytes(c_type)) return bad(S2V_ERR_INVALID_ARG, "misaligned output");
     return S2V_OK;
 }
 

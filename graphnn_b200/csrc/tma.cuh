@@ -61,7 +61,8 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
                  "r"(bar)
                  : "memory");
 }
-// a box to the matrix (what lies outside is left out); x times the element size a multiple of 16.  One of the thread's bulk groups.
+// a box to the matrix (rows outside are left out; of a row's end every 16 bytes that hold one of its numbers are written, with zeros behind it); x times the
+// element size a multiple of 16.  One of the thread's bulk groups.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src)
 {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
