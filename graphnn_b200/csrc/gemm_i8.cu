@@ -22,13 +22,14 @@ constexpr int GI_PIECE = 64, GI_BOX = 32 * GI_PIECE;    // bytes of a row that a
 template <int BN, bool PAIR> struct GiCfg {
     static constexpr int B_ROWS = PAIR ? BN / 2 : BN;   // of B, in this CTA's shared memory
     static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = B_ROWS * 128, STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = PAIR ? (BN == 256 ? 6 : 7) : BN == 256 ? 4 : BN == 128 ? 5 : 7, BOXES = BN == 256 ? 1 : 2;   // boxes of an epilogue warp
-    static constexpr uint32_t TM_COLS = 2 * BN;
+    static constexpr int STAGES = PAIR ? (BN == 256 ? 5 : 7) : BN == 256 ? 3 : BN == 128 ? 5 : 7, BOXES = 2;   // boxes of an epilogue warp
+    static constexpr int ACCS = 2;   // accumulators (four of 128 columns: no faster)
+    static constexpr uint32_t TM_COLS = ACCS * BN;
     static constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);   // s32 <- s8 x s8, M = 128 or 256, N = BN
     static constexpr uint32_t OFF_OUT = STAGES * STAGE;                       // per epilogue warp: its boxes
     static constexpr uint32_t OFF_SCALE = OFF_OUT + GI_EPI * BOXES * GI_BOX;   // per epilogue warp: the scales of half a tile's channels, then their biases
     static constexpr uint32_t OFF_BAR = OFF_SCALE + GI_EPI * BN * 4;
-    enum { FULL = 0, EMPTY = FULL + STAGES, DONE = EMPTY + STAGES, READ = DONE + 2, BARS = READ + 2 };
+    enum { FULL = 0, EMPTY = FULL + STAGES, DONE = EMPTY + STAGES, READ = DONE + ACCS, BARS = READ + ACCS };
     static constexpr uint32_t OFF_MISC = OFF_BAR + 8 * BARS;
     static constexpr uint32_t SMEM = OFF_MISC + 16 + 1024;                    // + slack to align the base to 1024 bytes
     static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -74,17 +75,25 @@ template <bool PAIR> __device__ __forceinline__ void gi_commit(uint32_t bar)
     else
         asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-// tc_wait for barriers on which the other CTA of the pair arrives too
-__device__ __forceinline__ bool gi_wait_pair(uint32_t bar, uint32_t parity, volatile int* abort_flag, s2v_device_status* status, int site)
+// tc_wait for barriers on which the other CTA of the pair arrives too.  Where all that a barrier orders is accumulators in tensor memory, which tcgen05.fence
+// takes care of, its arrivals and waits are relaxed (released and acquired at the cluster's scope they cost pairs of 256 x 128 a third of their time at
+// k = 128, and a microsecond of 18 at 200 x 14336 x 4096).
+template <bool ACQUIRE> __device__ __forceinline__ bool gi_wait_pair(uint32_t bar, uint32_t parity, volatile int* abort_flag, s2v_device_status* status, int site)
 {
     int spins = 0;
     bool ok = true;
     for (;;) {
         uint32_t done;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(done)
-                     : "r"(bar), "r"(parity), "r"(TC_SUSPEND_NS)
-                     : "memory");
+        if constexpr (ACQUIRE)
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                         : "=r"(done)
+                         : "r"(bar), "r"(parity), "r"(TC_SUSPEND_NS)
+                         : "memory");
+        else
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                         : "=r"(done)
+                         : "r"(bar), "r"(parity), "r"(TC_SUSPEND_NS)
+                         : "memory");
         if (done) break;
         if (*abort_flag) { ok = false; break; }
         if (++spins > TC_WAIT_LIMIT) {
@@ -114,30 +123,94 @@ __device__ __forceinline__ void gi_tile(int tile, int m_tiles, int n_tiles, int&
     tn = at / rows;
 }
 
-// The outputs of 32 rows (lanes) by COLS columns: into a box in shared memory (64-byte rows, their 16-byte pieces exchanged by the 64-byte swizzle,
-// which also keeps the stores free of bank conflicts), and from there by one copy that leaves out rows and 16-byte pieces which the matrix does not have.  (Written by the
-// warp's own loads and stores, a product with few sums an output was bound by that: 491,520 x 256 outputs of fp32 over k = 128 158 us.)
+// Accumulators that tcgen05.ld was asked for: no use of them comes before the wait.
+template <int N> __device__ __forceinline__ void gi_wait_loads(uint32_t (&v)[N])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < N; j += 8)
+        asm volatile("" : "+r"(v[j]), "+r"(v[j + 1]), "+r"(v[j + 2]), "+r"(v[j + 3]), "+r"(v[j + 4]), "+r"(v[j + 5]), "+r"(v[j + 6]), "+r"(v[j + 7]));
+}
+// fma(sa * s, v, b) of two accumulators, in packed fp32 arithmetic
+__device__ __forceinline__ void gi_two(uint64_t sa, uint64_t s, uint64_t b, uint32_t v0, uint32_t v1, float& y0, float& y1)
+{
+    asm("{\n\t.reg .b64 v, s;\n\t"
+        "mov.b64 v, {%5, %6};\n\t"
+        "mul.rn.f32x2 s, %2, %3;\n\t"
+        "fma.rn.f32x2 v, s, v, %4;\n\t"
+        "mov.b64 {%0, %1}, v;\n\t}"
+        : "=f"(y0), "=f"(y1)
+        : "l"(sa), "l"(s), "l"(b), "f"((float)(int)v0), "f"((float)(int)v1));
+}
+// The accumulators of 32 rows by 64 bytes of outputs, COLS columns, as matrices of 8 rows by 16 bytes of outputs: lane l has word l % 4 of
+// row l / 4 of each, which is as stmatrix wants it.
+template <typename T> __device__ __forceinline__ void gi_fetch(uint32_t at, uint32_t* v)
+{
+#pragma unroll
+    for (int h = 0; h < 2; ++h, at += 16u << 16) {
+        if constexpr (sizeof(T) == 4)
+            asm volatile("tcgen05.ld.sync.aligned.16x128b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                         : "=r"(v[8 * h]), "=r"(v[8 * h + 1]), "=r"(v[8 * h + 2]), "=r"(v[8 * h + 3]), "=r"(v[8 * h + 4]), "=r"(v[8 * h + 5]), "=r"(v[8 * h + 6]), "=r"(v[8 * h + 7])
+                         : "r"(at)
+                         : "memory");
+        else
+            asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                         : "=r"(v[16 * h]), "=r"(v[16 * h + 1]), "=r"(v[16 * h + 2]), "=r"(v[16 * h + 3]), "=r"(v[16 * h + 4]), "=r"(v[16 * h + 5]), "=r"(v[16 * h + 6]), "=r"(v[16 * h + 7]),
+                           "=r"(v[16 * h + 8]), "=r"(v[16 * h + 9]), "=r"(v[16 * h + 10]), "=r"(v[16 * h + 11]), "=r"(v[16 * h + 12]), "=r"(v[16 * h + 13]), "=r"(v[16 * h + 14]), "=r"(v[16 * h + 15])
+                         : "r"(at)
+                         : "memory");
+    }
+}
+// Where a column of half a tile stands in the table of scales: a lane's columns of one piece side by side.
+template <typename T> __device__ __forceinline__ int gi_place(int c)
+{
+    if constexpr (sizeof(T) == 4) return (c & ~15) + 4 * (c & 3) + (c >> 2 & 3);
+    else return (c & ~31) + 8 * (c >> 1 & 3) + 2 * (c >> 3 & 3) + (c & 1);
+}
+// The outputs, as 64-byte rows of a box whose 16-byte pieces are exchanged by the 64-byte swizzle, which keeps the stores free of bank conflicts.
+// (With a row a lane every lane reads every scale and bias, 16 bytes for four columns of one row, and shared memory is what such an epilogue waits for:
+// 491,520 x 256 outputs over k = 128 106 us in fp32 and 81 us in bf16.)
+template <typename T, int HALF, bool RELU> __device__ __forceinline__ void gi_fill(unsigned char* box, const float* chan, const uint64_t* sa, const uint32_t* v)
+{
+    constexpr int PAIRS = 8 / sizeof(T), VALUES = 2 * PAIRS;   // of a lane's columns
+    const int lane = threadIdx.x & 31;
+    ulonglong2 s[PAIRS / 2], b[PAIRS / 2];
+#pragma unroll
+    for (int j = 0; j < PAIRS / 2; ++j)
+        s[j] = reinterpret_cast<const ulonglong2*>(chan + VALUES * (lane & 3))[j], b[j] = reinterpret_cast<const ulonglong2*>(chan + HALF + VALUES * (lane & 3))[j];
+    const uint32_t to = smem_u32(box) + (lane & 7) * GI_PIECE + 16 * ((lane >> 3) ^ (lane >> 1 & 3));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {   // 8 rows
+        float y[VALUES];
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < PAIRS; ++j) {
+            const uint32_t* const from = v + r / 2 * (PAIRS * 4) + (sizeof(T) == 4 ? 4 * j + r % 2 : 4 * j + 2 * (r % 2));
+            gi_two(sa[r], j & 1 ? s[j / 2].y : s[j / 2].x, j & 1 ? b[j / 2].y : b[j / 2].x, from[0], from[sizeof(T) == 4 ? 2 : 1], y[2 * j], y[2 * j + 1]);
+        }
+        if constexpr (RELU) {
+#pragma unroll
+            for (int u = 0; u < VALUES; ++u) y[u] = relu_ref(y[u]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(y[j]);
+            else w[j] = pack_16bit<T>(y[2 * j], y[2 * j + 1]);
+        }
+        asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(to + r * 8 * GI_PIECE), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+    }
+}
+
+// The outputs of 32 rows by COLS columns: into a box in shared memory, and from there by one copy that leaves out rows and 16-byte pieces which the
+// matrix does not have.  (Written by the warp's own loads and stores, a product with few sums an output was bound by that: 491,520 x 256 outputs of fp32
+// over k = 128 158 us.)
 template <typename T, int HALF>
-__device__ __forceinline__ void gi_write(const GiArgs& a, const CUtensorMap* map, unsigned char* box, const float* chan, int64_t row0, int64_t col0, float sa, const uint32_t* v)
+__device__ __forceinline__ void gi_write(const GiArgs& a, const CUtensorMap* map, unsigned char* box, const float* chan, int64_t row0, int64_t col0, const uint64_t* sa, const uint32_t* v)
 {
     constexpr int COLS = GI_PIECE / sizeof(T), PER = 16 / sizeof(T);
     const int lane = threadIdx.x & 31;
-    const auto piece = [&](int row, int i) { return box + row * GI_PIECE + 16 * (i ^ (row >> 1 & 3)); };
-#pragma unroll
-    for (int j = 0; j < COLS; j += PER) {
-        float y[PER];
-#pragma unroll
-        for (int u = 0; u < PER; u += 4) {
-            const float4 s = *reinterpret_cast<const float4*>(chan + j + u), b = *reinterpret_cast<const float4*>(chan + HALF + j + u);
-            y[u] = fmaf(__fmul_rn(sa, s.x), (float)(int)v[j + u], b.x), y[u + 1] = fmaf(__fmul_rn(sa, s.y), (float)(int)v[j + u + 1], b.y);
-            y[u + 2] = fmaf(__fmul_rn(sa, s.z), (float)(int)v[j + u + 2], b.z), y[u + 3] = fmaf(__fmul_rn(sa, s.w), (float)(int)v[j + u + 3], b.w);
-        }
-        if (a.relu) {
-#pragma unroll
-            for (int u = 0; u < PER; ++u) y[u] = relu_ref(y[u]);
-        }
-        *reinterpret_cast<uint4*>(piece(lane, j / PER)) = pack_piece(y, T());
-    }
+    if (a.relu) gi_fill<T, HALF, true>(box, chan, sa, v);
+    else gi_fill<T, HALF, false>(box, chan, sa, v);
     // (a copy that meets the end of a row inside 16 bytes writes zeros behind it, into what may be somebody else's)
     if (a.boxes && (col0 + COLS <= a.n || a.n % PER == 0)) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -183,7 +256,7 @@ template <typename T, int BN, bool PAIR>
 __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c, const GiArgs a)
 {
     using Cfg = GiCfg<BN, PAIR>;
-    constexpr int STAGES = Cfg::STAGES, CTAS = PAIR ? 2 : 1;
+    constexpr int STAGES = Cfg::STAGES, ACCS = Cfg::ACCS, CTAS = PAIR ? 2 : 1;
     extern __shared__ unsigned char gi_raw[];
     unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(gi_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t smem0 = smem_u32(smem);
@@ -194,7 +267,7 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
     const int tiles = a.m_tiles * a.n_tiles, rank = PAIR ? (int)(blockIdx.x & 1) : 0, unit = (int)blockIdx.x / CTAS, units = (int)gridDim.x / CTAS;
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) tc_mbar_init(bar(Cfg::FULL + i), 1), tc_mbar_init(bar(Cfg::EMPTY + i), 1);
-        for (int i = 0; i < 2; ++i) tc_mbar_init(bar(Cfg::DONE + i), 1), tc_mbar_init(bar(Cfg::READ + i), GI_EPI * CTAS);
+        for (int i = 0; i < ACCS; ++i) tc_mbar_init(bar(Cfg::DONE + i), 1), tc_mbar_init(bar(Cfg::READ + i), GI_EPI * CTAS);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         if (a.kblocks > 0) tma_prefetch_map(&map_a), tma_prefetch_map(&map_b);
@@ -255,14 +328,14 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
         int it = 0, t = 0;
         bool ok = rank == 0;
         for (int tile = unit; ok && tile < tiles; tile += units, ++t) {
-            const int acc = t & 1;
-            if (t >= 2 && !(ok = PAIR ? gi_wait_pair(bar(Cfg::READ + acc), (uint32_t)(t / 2 - 1) & 1u, abort_flag, a.status, 71)
-                                      : tc_wait(bar(Cfg::READ + acc), (uint32_t)(t / 2 - 1) & 1u, abort_flag, a.status, 71)))
+            const int acc = t % ACCS;
+            if (t >= ACCS && !(ok = PAIR ? gi_wait_pair<false>(bar(Cfg::READ + acc), (uint32_t)(t / ACCS - 1) & 1u, abort_flag, a.status, 71)
+                                      : tc_wait(bar(Cfg::READ + acc), (uint32_t)(t / ACCS - 1) & 1u, abort_flag, a.status, 71)))
                 break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (int kb = 0; kb < a.kblocks; ++kb, ++it) {
                 const int s = it % STAGES;
-                if (!(ok = PAIR ? gi_wait_pair(bar(Cfg::FULL + s), (uint32_t)(it / STAGES) & 1u, abort_flag, a.status, 72)
+                if (!(ok = PAIR ? gi_wait_pair<true>(bar(Cfg::FULL + s), (uint32_t)(it / STAGES) & 1u, abort_flag, a.status, 72)
                                 : tc_wait(bar(Cfg::FULL + s), (uint32_t)(it / STAGES) & 1u, abort_flag, a.status, 72)))
                     break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -291,46 +364,61 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
         unsigned char* const boxes = smem + Cfg::OFF_OUT + e * Cfg::BOXES * GI_BOX;
         int turn = 0;
         float* const chan = reinterpret_cast<float*>(smem + Cfg::OFF_SCALE) + e * BN;
-        int t = 0;
-        for (int tile = unit; tile < tiles; tile += units, ++t) {
+        // A tile's scales and biases are fetched a tile ahead.
+        float sa[4] = {}, s[HALF / 32] = {}, bias[HALF / 32] = {};   // (of a lane's four rows; of its columns)
+        int64_t row0 = 0, first = 0;
+        const auto fetch_scales = [&](int tile) {
             int tm, tn;
             gi_tile(tile, a.m_tiles, a.n_tiles, tm, tn);
-            const int acc = t & 1;
-            const int64_t row0 = (int64_t)tm * (128 * CTAS) + rank * 128 + quarter * 32, first = (int64_t)tn * BN + half * HALF;
-            const float sa = row0 + lane < a.m ? a.a_scale[row0 + lane] : 0.0f;
+            row0 = (int64_t)tm * (128 * CTAS) + rank * 128 + quarter * 32, first = (int64_t)tn * BN + half * HALF;
 #pragma unroll
-            for (int u = lane; u < HALF; u += 32) {
-                chan[u] = first + u < a.n ? __ldg(a.b_scale + first + u) : 0.0f;
-                chan[HALF + u] = a.bias && first + u < a.n ? __ldg(a.bias + first + u) : 0.0f;
+            for (int r = 0; r < 4; ++r) {
+                const int64_t row = row0 + 8 * r + (lane >> 2);
+                sa[r] = row < a.m ? a.a_scale[row] : 0.0f;
             }
+#pragma unroll
+            for (int u = 0; u < HALF / 32; ++u) {
+                const int64_t c = first + u * 32 + lane;
+                s[u] = c < a.n ? __ldg(a.b_scale + c) : 0.0f;
+                bias[u] = a.bias && c < a.n ? __ldg(a.bias + c) : 0.0f;
+            }
+        };
+        int t = 0;
+        if (unit < tiles) fetch_scales(unit);
+        for (int tile = unit; tile < tiles; tile += units, ++t) {
+            const int acc = t % ACCS;
+            const int64_t to_row = row0, to_col = first;
+            uint64_t sa2[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) asm("mov.b64 %0, {%1, %1};" : "=l"(sa2[r]) : "f"(sa[r]));
             __syncwarp();
-            if (a.kblocks > 0 && !(PAIR ? gi_wait_pair(bar(Cfg::DONE + acc), (uint32_t)(t / 2) & 1u, abort_flag, a.status, 73)
-                                        : tc_wait(bar(Cfg::DONE + acc), (uint32_t)(t / 2) & 1u, abort_flag, a.status, 73)))
+#pragma unroll
+            for (int u = 0; u < HALF / 32; ++u) chan[gi_place<T>(u * 32 + lane)] = s[u], chan[HALF + gi_place<T>(u * 32 + lane)] = bias[u];
+            __syncwarp();
+            if (tile + units < tiles) fetch_scales(tile + units);
+            if (a.kblocks > 0 && !(PAIR ? gi_wait_pair<false>(bar(Cfg::DONE + acc), (uint32_t)(t / ACCS) & 1u, abort_flag, a.status, 73)
+                                        : tc_wait(bar(Cfg::DONE + acc), (uint32_t)(t / ACCS) & 1u, abort_flag, a.status, 73)))
                 break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t at = tmem + (uint32_t)(acc * BN + half * HALF) + ((uint32_t)quarter << 21);
-            const int cols = row0 >= a.m ? 0 : (int)min((int64_t)HALF, a.n - first);   // (the same for the warp)
-            uint32_t next[COLS] = {};
-            const auto fetch = [&](int c) {
+            const int cols = to_row >= a.m ? 0 : (int)min((int64_t)HALF, a.n - to_col);   // (the same for the warp)
+            uint32_t v[2][COLS] = {};
+            if (cols > 0 && a.kblocks > 0) gi_fetch<T>(at, v[0]);
 #pragma unroll
-                for (int h = 0; h < COLS; h += 16) tc_ld_cols16(at + (uint32_t)(c + h), next + h);
-            };
-            if (cols > 0 && a.kblocks > 0) fetch(0);
-            for (int c = 0; c < cols; c += COLS) {
-                uint32_t v[COLS];
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                for (int j = 0; j < COLS; ++j) v[j] = next[j];
-                if (c + COLS < cols && a.kblocks > 0) fetch(c + COLS);
+            for (int c = 0; c < HALF; c += COLS) {
+                if (c >= cols) break;
+                uint32_t(&now)[COLS] = v[c / COLS & 1];
+                gi_wait_loads(now);
+                if (c + COLS < cols && a.kblocks > 0) gi_fetch<T>(at + (uint32_t)(c + COLS), v[~(c / COLS) & 1]);
                 // the copy that last read this box has done so
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(Cfg::BOXES - 1) : "memory");
                 __syncwarp();
-                gi_write<T, HALF>(a, &map_c, boxes + turn * GI_BOX, chan + c, row0, first + c, sa, v);
+                gi_write<T, HALF>(a, &map_c, boxes + turn * GI_BOX, chan + c, to_row, to_col + c, sa2, now);
                 turn = (turn + 1) % Cfg::BOXES;
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (lane == 0) {
-                if constexpr (PAIR) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(gi_first(bar(Cfg::READ + acc))) : "memory");
+                if constexpr (PAIR) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(gi_first(bar(Cfg::READ + acc))) : "memory");
                 else tc_mbar_arrive(bar(Cfg::READ + acc));
             }
             __syncwarp();
@@ -413,8 +501,8 @@ struct GiForm {
     int rows, bn;
     float fixed, first, next, out;
 };
-constexpr GiForm GI_PAIR_256{256, 256, 6.6f, .33f, .335f, 3.9f}, GI_PAIR_128{256, 128, 5.3f, .28f, .28f, 2.6f}, GI_256{128, 256, 5.8f, .40f, .42f, 3.15f},
-    GI_128{128, 128, 4.4f, .33f, .345f, 1.9f}, GI_64{128, 64, 3.8f, .30f, .31f, 1.26f};
+constexpr GiForm GI_PAIR_256{256, 256, 5.6f, .35f, .305f, 2.55f}, GI_PAIR_128{256, 128, 5.3f, .258f, .268f, 1.42f}, GI_256{128, 256, 4.7f, .45f, .44f, 2.55f},
+    GI_128{128, 128, 4.55f, .329f, .334f, 1.45f}, GI_64{128, 64, 4.2f, .255f, .333f, .89f};
 
 float gi_cost(const s2v_ctx* ctx, const s2v_gemm_i8_args& g, const GiForm& f)
 {
