@@ -440,10 +440,12 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
 // memory; the others' are named by a byte per piece.  Their gradients are written over what the loops over the run wrote.  The first CTA's first
 // warp adds up the loss while the others write the gradient.
 constexpr int DC_CTAS = 8, DC_LISTERS = DT_TOP / 32;
-// Rows of up to DC_SHORT pieces: six CTAs of 128 threads an SM (the steps of a row are a chain of latencies: 16384 rows of 9000 bf16 199 us, with
-// CTAs of 256 threads 311), lists of more than 128 entries apart.  Longer ones: three of 256 (4096 rows of 131072 bf16 490 us; six of 128
-// 562, two of 512 620 to 650, all pieces held by a cluster of four 504).
-constexpr int DC_SHORT = 2048, DC_HELD = 4000, DC_RUN = 8192;   // pieces: of a short row; held, and of a run, at most
+// Rows of up to DC_SHORT pieces: six CTAs of 128 threads an SM (the steps of a row are a chain of latencies: 16384 rows of 9000 bf16 with their gradients
+// 168 us, with CTAs of 256 threads 311), lists of more than 128 entries apart.  Longer ones: three of 256 (4096 rows of 26000 bf16 113 us, 122 by CTAs of
+// 128; of 23000 110 and 99; of 131072 470 and 562, by two of 512 620 to 650, all pieces held by a cluster of four 504).
+// The loss alone, of rows of more than DC_ONCE pieces and more of them than run at a time, needs a row once: nothing is held, eight CTAs of 128 threads or
+// six of 256 an SM (4096 rows of 131072 bf16 202 us, 5.3 TB/s, held 282; of 20000 57 and 76; 8192 of 16384 89 and 96, of 14000 87 and 82).
+constexpr int DC_SHORT = 3000, DC_ONCE = 1900, DC_HELD = 4000, DC_RUN = 8192;   // pieces: of short rows; of rows held all the same; held, and of a run, at most
 constexpr int DC_SMEM = 72 << 10;
 static_assert(DC_HELD * 16 + (DC_RUN - DC_HELD) <= DC_SMEM && DC_SHORT <= DC_HELD, "a byte for each piece that is not held");
 constexpr int DC_SLOTS = 512;                        // of the table that finds columns listed twice
@@ -553,41 +555,42 @@ template <typename T> struct DcRun {
     }
 };
 
-template <typename T, int DC_THREADS, int CTAS_SM>
+template <typename T, int DC_THREADS, int CTAS_SM, bool LOSS>
 __global__ void __launch_bounds__(DC_THREADS, CTAS_SM) distill_cluster_kernel(const DtArgs a, int ctas, int held)
 {
     extern __shared__ __align__(16) unsigned char dc_raw[];
     __shared__ DcShared s;
     constexpr int N = PIECE<T>, DC_WARPS = DC_THREADS / 32;
     uint4* const run = reinterpret_cast<uint4*>(dc_raw);
-    uint32_t* const marks = reinterpret_cast<uint32_t*>(run + held);           // a byte for each piece behind the held ones
-    const uint8_t* const mark = reinterpret_cast<const uint8_t*>(marks) - held;
+    const int unmarked = LOSS ? 0 : held;
+    uint32_t* const marks = reinterpret_cast<uint32_t*>(run + unmarked);       // a byte for each piece behind those
+    const uint8_t* const mark = reinterpret_cast<const uint8_t*>(marks) - unmarked;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)(blockIdx.x % (unsigned)ctas);
     const double inv = a.inv;
     const float inv_t = a.inv_t, c = a.c;
     const int most = (int)((a.cols / N + ctas - 1) / ctas);
-    for (int w = tid; w < (most - held + 3) / 4; w += DC_THREADS) marks[w] = 0;
+    for (int w = tid; w < (most - unmarked + 3) / 4; w += DC_THREADS) marks[w] = 0;
     for (int w = tid; w < DC_SLOTS; w += DC_THREADS) s.slot[w] = -1;
     if (tid < DC_LISTERS) s.inner[tid] = make_float2(-INFINITY, 0.0f);   // (of the warps without entries, once and for all)
     const int64_t r = blockIdx.x / (unsigned)ctas;
     const T* const z = static_cast<const T*>(a.z) + r * a.ldz;
-    T* const dz = a.dz ? static_cast<T*>(a.dz) + r * a.lddz : nullptr;
+    T* const dz = !LOSS && a.dz ? static_cast<T*>(a.dz) + r * a.lddz : nullptr;
     const DcHead head(a, r);
     const float weight = head.weight;
     const DcRun<T> my(z, a.cols, rank, ctas);
     const uint4* const zp = reinterpret_cast<const uint4*>(z + my.row.head) + my.first;
     const bool skip_weight = weight == 0.0f && !a.stats;
     const int kept = min(held, my.pieces);
-    if (!skip_weight)
+    if (!LOSS && !skip_weight)
         for (int p = tid; p < kept; p += DC_THREADS) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(run + p)), "l"(zp + p) : "memory");
     __syncthreads();   // the table and the marks are empty
     const DcEntry e = dc_entry(a, head, s);
     int at;
-    const bool here = my.has(head.id, rank, ctas, at), held_entry = here && at >= 0 && at < held * N;
+    const bool here = my.has(head.id, rank, ctas, at), held_entry = !LOSS && here && at >= 0 && at < held * N;
     bool mine = here && !e.twice;
     float P_all = e.P, zk = (here && !held_entry) || (rank == 0 && head.id >= 0) ? to_f32(z[head.id]) : -INFINITY;
-    if (here && at >= held * N) atomicOr(&marks[(at / N - held) >> 2], 1u << (8 * ((at / N - held) & 3) + at % N));
+    if (here && at >= unmarked * N) atomicOr(&marks[(at / N - unmarked) >> 2], 1u << (8 * ((at / N - unmarked) & 3) + at % N));
     // the scalar columns: the head's to the first CTA, the tail's to the last
     const bool in_head = rank == 0 && tid < my.row.head, in_tail = rank == ctas - 1 && tid >= 32 && tid < 32 + my.row.tail;
     const int edge_at = in_head ? tid : (int)a.cols - my.row.tail + tid - 32;
@@ -609,18 +612,21 @@ __global__ void __launch_bounds__(DC_THREADS, CTAS_SM) distill_cluster_kernel(co
         for (int k = 0; k < a.top; ++k) edge_out &= s.id[k] != edge_at;
     if ((has & 2) && here) mine = dc_first(a, head.id, s, P_all);
     DtSum outer{-INFINITY, 0.0f}, inner{-INFINITY, 0.0f};
-    // what is not held, while the rest is on its way
-    for (int p = held + tid; p < my.pieces; p += 4 * DC_THREADS) {
-        uint4 v[4];
+    const auto add = [&](int from, int n) {
+        for (int p = from + tid; p < n; p += 4 * DC_THREADS) {
+            uint4 v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (p + j * DC_THREADS < my.pieces) v[j] = zp[p + j * DC_THREADS];
+            for (int j = 0; j < 4; ++j)
+                if (p + j * DC_THREADS < n) v[j] = zp[p + j * DC_THREADS];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (p + j * DC_THREADS < my.pieces)
-                if (const uint32_t listed = mark[p + j * DC_THREADS]) dt_take_out<T>(v[j], listed);
-        outer.template add_pieces<T, 4>(v, p, DC_THREADS, my.pieces, c);
-    }
+            for (int j = 0; j < 4; ++j)
+                if (p + j * DC_THREADS < n)
+                    if (const uint32_t listed = mark[p + j * DC_THREADS]) dt_take_out<T>(v[j], listed);
+            outer.template add_pieces<T, 4>(v, p, DC_THREADS, n, c);
+        }
+    };
+    add(held, my.pieces);   // what is not held, while the rest is on its way
+    if constexpr (LOSS) add(0, kept);   // (in the same order, and the same loss to the last bit, as with a gradient)
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     if (mine && held_entry) {   // (one thread an element)
@@ -636,7 +642,7 @@ __global__ void __launch_bounds__(DC_THREADS, CTAS_SM) distill_cluster_kernel(co
         if (lane == 0) s.inner[warp] = make_float2(inner.m, inner.s);
     }
     __syncthreads();
-    for (int p = tid; p < kept; p += 4 * DC_THREADS) {
+    for (int p = tid; !LOSS && p < kept; p += 4 * DC_THREADS) {
         uint4 v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -763,16 +769,16 @@ template <typename T, int DG_THREADS> __global__ void __launch_bounds__(DG_THREA
     if (mine) dz[head.id] = from_f32<T>(k.inner * expf((zk - k.M) * inv_t) - k.scale * (P_all * k.p_scale));
 }
 
-template <typename T, int THREADS, int CTAS_SM> int dc_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a, int ctas)
+template <typename T, int THREADS, int CTAS_SM, bool LOSS> int dc_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a, int ctas)
 {
     const int64_t most = (a.cols / PIECE<T> + ctas - 1) / ctas;
     const int held = (int)(most < DC_HELD ? most : DC_HELD);
-    const auto kernel = distill_cluster_kernel<T, THREADS, CTAS_SM>;
+    const auto kernel = distill_cluster_kernel<T, THREADS, CTAS_SM, LOSS>;
     S2V_CUDA_OK(ctx, s2v_allow_shared(kernel, DC_SMEM));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.rows * ctas));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = (size_t)(held * 16 + (most - held + 3) / 4 * 4);
+    cfg.dynamicSmemBytes = LOSS ? (size_t)(most + 3) / 4 * 4 : (size_t)(held * 16 + (most - held + 3) / 4 * 4);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -813,7 +819,9 @@ template <typename T, bool GRAD_ONLY> int dt_launch_type(s2v_ctx* ctx, cudaStrea
         return pieces <= 2 * DC_SHORT && a.top <= 128 ? dg_launch<T, 128>(ctx, st, a, ctas) : dg_launch<T, 256>(ctx, st, a, ctas);
     } else {
         while (ctas < DC_CTAS && (pieces > (int64_t)ctas * DC_RUN || (a.rows * ctas < 2 * ctx->sm_count && pieces >= (int64_t)ctas * 512))) ctas *= 2;
-        return pieces <= DC_SHORT && a.top <= 128 ? dc_launch<T, 128, 6>(ctx, st, a, ctas) : dc_launch<T, 256, 3>(ctx, st, a, ctas);
+        const bool once = !a.dz && pieces > DC_ONCE && a.rows * ctas >= 3 * ctx->sm_count;
+        if (pieces <= DC_SHORT && a.top <= 128) return once ? dc_launch<T, 128, 8, true>(ctx, st, a, ctas) : dc_launch<T, 128, 6, false>(ctx, st, a, ctas);
+        return once ? dc_launch<T, 256, 6, true>(ctx, st, a, ctas) : dc_launch<T, 256, 3, false>(ctx, st, a, ctas);
     }
 }
 int dt_launch(s2v_ctx* ctx, s2v_stream stream, int z_type, bool grad_only, const DtArgs& a)
