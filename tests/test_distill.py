@@ -349,6 +349,34 @@ def test_many_rows(gpu_ctx, rows, cols):
 
 
 @gpu
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype,cols,top", [("f32", 8203, 9), ("f16", 17001, 128), ("bf16", 17001, 200), ("f32", 33001, 64), ("bf16", 131077, 30)])
+def test_losses_of_many_long_rows(gpu_ctx, dtype, cols, top, tail):
+    """The loss alone, of more long rows than run at a time: the same to the last bit as with a gradient, with columns listed twice, masked and NaN."""
+    z, idx, t, lse, w = inputs(50, cols, top, dtype, cols + top, tail, 1.0)
+    idx[3, 1] = idx[3, 0]
+    z[4, : cols // 2] = -math.inf
+    z[5, idx[5].clamp(min=0).long()] = torch.finfo(z.dtype).min
+    torch.cuda.synchronize()
+    loss50, dz50 = both_ways(gpu_ctx, z, idx, t, 1.0, lse, w)
+    assert_matches(loss50, dz50, z, idx, t, 1.0, lse, w)
+    z[6, 77] = math.nan
+    many = [None if v is None else v.repeat(9, *([1] * (v.dim() - 1))) for v in (z, idx, t, lse, w)]
+    more = {"t_lse": many[3], "row_weight": many[4]}
+    loss, alone, kept, dz, stats = *(torch.empty(450, device="cuda") for _ in range(3)), torch.empty_like(many[0]), torch.empty((450, 4), device="cuda")
+    torch.cuda.synchronize()
+    gpu_ctx.distill_topk(*many[:3], loss, dz=dz, **more)
+    gpu_ctx.distill_topk(*many[:3], alone, **more)
+    gpu_ctx.distill_topk(*many[:3], kept, stats=stats, **more)
+    gpu_ctx.synchronize()
+    same = lambda a, b: torch.equal(a.nan_to_num(nan=12345.0), b.nan_to_num(nan=12345.0))  # noqa: E731
+    assert same(loss, alone) and same(loss, kept) and bool(loss.view(9, 50)[:, 6].isnan().all())
+    loss50[6] = math.nan
+    rel = 2 * relative(cols, 1.0, z.nan_to_num(nan=0.0))
+    assert torch.allclose(loss, loss50.repeat(9), rtol=2.0 ** -22, atol=2 * rel, equal_nan=True)
+
+
+@gpu
 def test_captured_replayed_and_on_another_stream(gpu_ctx):
     for rows, cols in ((64, 6), (40, 3000), (12, 60000)):
         z, idx, t, lse, w = inputs(rows, cols, 5, "f16", rows, True, 1.0)
