@@ -713,7 +713,7 @@ __global__ void __launch_bounds__(DC_THREADS, CTAS_SM) distill_cluster_kernel(co
 }
 
 // The gradient from kept sums: nothing to wait for but the list.
-// (A CTA a row, of 128 threads up to 4096 pieces, else 256: 16384 x 9000 bf16 128 us, with 256 threads 177 and with 512 282; 4096 x 131072 bf16 349 us,
+// (A CTA a row, of 128 threads up to 4096 pieces, else 256: 16384 x 9000 bf16 116 us, with 256 threads 177 and with 512 282; 4096 x 131072 bf16 347 us,
 // 6.2 TB/s, with 128 threads 364, and 454 where four CTAs shared a row.)
 template <typename T, int DG_THREADS> __global__ void __launch_bounds__(DG_THREADS, 1024 / DG_THREADS) distill_grad_kernel(const DtArgs a, int ctas)
 {

@@ -22,6 +22,7 @@ constexpr int GI_PIECE = 64, GI_BOX = 32 * GI_PIECE;    // bytes of a row that a
 template <int BN, bool PAIR> struct GiCfg {
     static constexpr int B_ROWS = PAIR ? BN / 2 : BN;   // of B, in this CTA's shared memory
     static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = B_ROWS * 128, STAGE = A_BYTES + B_BYTES;
+    // (128 x 256 with four stages and one box: 491,520 x 256 outputs of bf16 over k = 128 85 us, with three and two 65; 300 x 11000 x 4096 18.9 and 19.7)
     static constexpr int STAGES = PAIR ? (BN == 256 ? 5 : 7) : BN == 256 ? 3 : BN == 128 ? 5 : 7, BOXES = 2;   // boxes of an epilogue warp
     static constexpr int ACCS = 2;   // accumulators (four of 128 columns: no faster)
     static constexpr uint32_t TM_COLS = ACCS * BN;
@@ -169,7 +170,7 @@ template <typename T> __device__ __forceinline__ int gi_place(int c)
 }
 // The outputs, as 64-byte rows of a box whose 16-byte pieces are exchanged by the 64-byte swizzle, which keeps the stores free of bank conflicts.
 // (With a row a lane every lane reads every scale and bias, 16 bytes for four columns of one row, and shared memory is what such an epilogue waits for:
-// 491,520 x 256 outputs over k = 128 106 us in fp32 and 81 us in bf16.)
+// 491,520 x 256 outputs over k = 128 105 us in fp32 and 80 us in bf16; so 103 and 65.)
 template <typename T, int HALF, bool RELU> __device__ __forceinline__ void gi_fill(unsigned char* box, const float* chan, const uint64_t* sa, const uint32_t* v)
 {
     constexpr int PAIRS = 8 / sizeof(T), VALUES = 2 * PAIRS;   // of a lane's columns
@@ -490,13 +491,14 @@ template <typename T, int BN, bool PAIR> int gi_launch(s2v_ctx* ctx, cudaStream_
 // 20000; mostly within 15 %): `fixed` with the first tile's outputs, `first` and `next` for 128 columns of k in the first and in further tiles of a CTA
 // (the further ones share L2 with everybody), `out` for a further tile's outputs where they take longer than that.  Measured sides of some choices:
 //                          256 x 256 pair  256 x 128 pair  128 x 256  128 x 128  128 x 64   split
-//     4096 x 4096 x 4096        47              79             56         97                             (m x n x k)
-//     1024 x 4096 x 4096        17.5            22.7           18.5       25.8       42.8
-//      512 x 4096 x 4096        16.5            14.4           17.4       15.6       23.7       22
-//      200 x  256 x 4096        15.4            12.8           16.3       13.9       12.9        8.0
-//       64 x 4096 x  512         8.0             6.5            7.2        5.7        5.1        7.2
-//       27 x 4096 x 4096        15.3            13.0           16.2       14.0       13.2        7.2
-//    20000 x 4096 x  128        72              94             57         67         89
+//     4096 x 4096 x 4096        46              63             58         78        137                  (m x n x k)
+//     1024 x 4096 x 4096        16.3            21.7           17.3       25.0       42.5
+//      512 x 4096 x 4096        15.4            13.5           16.5       14.8       23.4       22
+//      200 x  256 x 4096        14.6            12.2           15.7       13.8       12.7        8.1
+//       64 x 4096 x  512         7.1             5.8            6.6        5.3        4.7        7.2
+//       27 x 4096 x 4096        14.7            12.6           15.6       13.8       12.9        7.2
+//     5000 x 4096 x 1024        20.1            27.8           23.7       31.0       51.1
+//    20000 x 4096 x  128        47.6            54.5           44.2       52.6       65.3
 struct GiForm {
     int rows, bn;
     float fixed, first, next, out;
