@@ -15,7 +15,7 @@ struct s2v_gemm_i8_args {
 };
 // `dependent`: the kernel in front writes A and a_scale and has told the next launch to start (griddepcontrol.launch_dependents)
 int s2v_launch_gemm_i8(s2v_ctx* ctx, cudaStream_t st, const s2v_gemm_i8_args& a, bool dependent);
-// gemm_i8_few.cu: up to 8 tokens that fit shared memory as 8-bit integers; x_type < 0: A is 8-bit with scales, else it is quantised on the way
+// gemm_i8_few.cu: one or two tokens that fit shared memory as 8-bit integers; x_type < 0: A is 8-bit with scales, else it is quantised on the way
 bool s2v_gemv_i8_takes(int64_t m, int64_t n, int64_t k);
 int s2v_launch_gemv_i8(s2v_ctx* ctx, cudaStream_t st, int x_type, const s2v_gemm_i8_args& a);
 // gemm_i8_few.cu: outputs of few tiles, k > 0

@@ -1,4 +1,4 @@
-// Products with few tokens, where reading the weights once is everything: a kernel without matrix instructions for up to 8 tokens (which also
+// Products with few tokens, where reading the weights once is everything: a kernel without matrix instructions for one or two tokens (which also
 // quantises them on the way), and one that splits k among the CTAs of a cluster for outputs of few tiles.
 #include <cmath>
 
@@ -10,7 +10,7 @@
 namespace
 {
 
-// ---------------------------------------------------------------- up to 8 tokens
+// ---------------------------------------------------------------- one or two tokens
 // A warp per weight row: 32 lanes read 512 bytes of it at a time, eight such loads on their way at once, before the tokens are even looked at.  The
 // tokens lie in shared memory as 8-bit integers, quantised by every CTA for itself (they are few; a launch in front would take as long as this
 // one).  dp4a adds up four products; a lane's sums are joined at the end.
@@ -29,50 +29,38 @@ struct GvArgs {
     void* y;
 };
 
-template <int M, int R>
-__device__ __forceinline__ void gv_add(int (&acc)[R][M], const uint4 (&w)[R], const int8_t* xs, int kp, int off)
+template <int M> __device__ __forceinline__ void gv_add(int (&acc)[M], const uint4& w, const int8_t* xs, int kp, int off)
 {
 #pragma unroll
     for (int t = 0; t < M; ++t) {
         const uint4 x = *reinterpret_cast<const uint4*>(xs + t * kp + off);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            int s = acc[r][t];
-            s = __dp4a((int)w[r].x, (int)x.x, s);
-            s = __dp4a((int)w[r].y, (int)x.y, s);
-            s = __dp4a((int)w[r].z, (int)x.z, s);
-            acc[r][t] = __dp4a((int)w[r].w, (int)x.w, s);
-        }
+        int s = acc[t];
+        s = __dp4a((int)w.x, (int)x.x, s);
+        s = __dp4a((int)w.y, (int)x.y, s);
+        s = __dp4a((int)w.z, (int)x.z, s);
+        acc[t] = __dp4a((int)w.w, (int)x.w, s);
     }
 }
 
-template <typename TX, typename TY, int M, int R>
+template <typename TX, typename TY, int M>
 __global__ void __launch_bounds__(GV_THREADS, 4) gemv_i8_kernel(const GvArgs a)
 {
     extern __shared__ __align__(16) int8_t xs[];   // [M][kp]
     __shared__ float sx[M];
     __shared__ uint32_t part[GV_WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t groups = (a.n + GV_WARPS * R - 1) / (GV_WARPS * R);
+    const int64_t groups = (a.n + GV_WARPS - 1) / GV_WARPS;
     const int kp = a.kp, chunks = ((int)a.k + 511) / 512;
-    uint4 w[GV_AHEAD][R];
-    const int8_t* wr[R];
+    uint4 w[GV_AHEAD];
+    const int8_t* wr;
     const int k16 = (int)a.k & ~15, rest = (int)a.k & 15;   // whole pieces; the last bytes are multiplied one by one (a matrix may end with its last row)
-    const auto rows_of = [&](int64_t g) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int64_t row = min((g * GV_WARPS + warp) * R + r, a.n - 1);   // (rows behind the last are computed as the last and not written)
-            wr[r] = a.W + row * a.ldw;
-        }
-    };
+    const auto row_of = [&](int64_t g) { return min(g * GV_WARPS + warp, a.n - 1); };   // (rows behind the last are computed as the last and not written)
     const auto fetch = [&](int c0) {
 #pragma unroll
         for (int c = 0; c < GV_AHEAD; ++c)
-#pragma unroll
-            for (int r = 0; r < R; ++r) 
-                if (const int off = (c0 + c) * 512 + lane * 16; off < k16) w[c][r] = __ldcs(reinterpret_cast<const uint4*>(wr[r] + off));
+            if (const int off = (c0 + c) * 512 + lane * 16; off < k16) w[c] = __ldcs(reinterpret_cast<const uint4*>(wr + off));
     };
-    rows_of(blockIdx.x);
+    wr = a.W + row_of(blockIdx.x) * a.ldw;
     fetch(0);
     // the tokens: GV_WARPS / M warps each
     if constexpr (std::is_same<TX, int8_t>::value) {
@@ -108,51 +96,40 @@ __global__ void __launch_bounds__(GV_THREADS, 4) gemv_i8_kernel(const GvArgs a)
     }
     __syncthreads();
     for (int64_t g = blockIdx.x; g < groups; g += gridDim.x) {
-        int acc[R][M] = {};
-        float ws[R], b[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int64_t row = min((g * GV_WARPS + warp) * R + r, a.n - 1);
-            ws[r] = __ldg(a.w_scale + row);
-            b[r] = a.bias ? __ldg(a.bias + row) : 0.0f;
-        }
+        int acc[M] = {};
+        const int64_t row = row_of(g);
+        const float ws = __ldg(a.w_scale + row), b = a.bias ? __ldg(a.bias + row) : 0.0f;
         for (int c0 = 0; c0 < chunks; c0 += GV_AHEAD) {
             if (c0 > 0) fetch(c0);
 #pragma unroll
             for (int c = 0; c < GV_AHEAD; ++c)
-                if (const int off = (c0 + c) * 512 + lane * 16; off < k16) gv_add<M, R>(acc, w[c], xs, kp, off);
+                if (const int off = (c0 + c) * 512 + lane * 16; off < k16) gv_add<M>(acc, w[c], xs, kp, off);
         }
         if (lane < rest) {
+            const int wb = wr[k16 + lane];
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int wb = wr[r][k16 + lane];
-#pragma unroll
-                for (int t = 0; t < M; ++t) acc[r][t] += wb * xs[t * kp + k16 + lane];
-            }
+            for (int t = 0; t < M; ++t) acc[t] += wb * xs[t * kp + k16 + lane];
         }
         if (g + gridDim.x < groups) {
-            rows_of(g + gridDim.x);
+            wr = a.W + row_of(g + gridDim.x) * a.ldw;
             fetch(0);
         }
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int t = 0; t < M; ++t) {
-                const int sum = __reduce_add_sync(0xffffffffu, acc[r][t]);
-                const int64_t row = (g * GV_WARPS + warp) * R + r;
-                if (lane == r * M + t && t < a.m && row < a.n) {
-                    const float v = fmaf(__fmul_rn(sx[t], ws[r]), (float)sum, b[r]);
-                    static_cast<TY*>(a.y)[t * a.ldy + row] = from_f32<TY>(a.relu ? relu_ref(v) : v);
-                }
+        for (int t = 0; t < M; ++t) {
+            const int sum = __reduce_add_sync(0xffffffffu, acc[t]);
+            if (lane == t && g * GV_WARPS + warp < a.n) {
+                const float v = fmaf(__fmul_rn(sx[t], ws), (float)sum, b);
+                static_cast<TY*>(a.y)[t * a.ldy + row] = from_f32<TY>(a.relu ? relu_ref(v) : v);
             }
+        }
     }
 }
 
-template <typename TX, typename TY, int M, int R> int gv_launch(s2v_ctx* ctx, cudaStream_t st, const GvArgs& a)
+template <typename TX, typename TY, int M> int gv_launch(s2v_ctx* ctx, cudaStream_t st, const GvArgs& a)
 {
-    const int64_t groups = (a.n + GV_WARPS * R - 1) / (GV_WARPS * R), cap = (int64_t)ctx->sm_count * 4;
-    S2V_CUDA_OK(ctx, s2v_allow_shared(gemv_i8_kernel<TX, TY, M, R>, GV_SMEM));
-    gemv_i8_kernel<TX, TY, M, R><<<(unsigned)(groups < cap ? groups : cap), GV_THREADS, (size_t)M * a.kp, st>>>(a);
+    const int64_t groups = (a.n + GV_WARPS - 1) / GV_WARPS, cap = (int64_t)ctx->sm_count * 4;
+    S2V_CUDA_OK(ctx, s2v_allow_shared(gemv_i8_kernel<TX, TY, M>, GV_SMEM));
+    gemv_i8_kernel<TX, TY, M><<<(unsigned)(groups < cap ? groups : cap), GV_THREADS, (size_t)M * a.kp, st>>>(a);
     S2V_CHECK_LAUNCH(ctx, "gemv_i8_kernel");
     return S2V_OK;
 }
@@ -160,7 +137,7 @@ template <typename TX> int gv_by_size(s2v_ctx* ctx, cudaStream_t st, int y_type,
 {
     return s2v_by_dtype(y_type, [&](auto type) {
         using TY = decltype(type);
-        return a.m == 1 ? gv_launch<TX, TY, 1, 1>(ctx, st, a) : gv_launch<TX, TY, 2, 1>(ctx, st, a);
+        return a.m == 1 ? gv_launch<TX, TY, 1>(ctx, st, a) : gv_launch<TX, TY, 2>(ctx, st, a);
     });
 }
 
