@@ -6,6 +6,8 @@
 // Taking one sum from the other's total would lose s (or 1 - s) where the student gives nearly everything (or nothing) to the list, and one
 // maximum for both would lose the smaller sum where they are far apart (logits masked with the type's lowest value).  The loss is put together in 64
 // bits (it is a difference of larger numbers), the sums over columns and the gradient in fp32.
+#include <algorithm>
+
 #include "elem_types.cuh"
 
 namespace
@@ -435,14 +437,16 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
 }
 
 // ---------------------------------------------------------------- longer rows: a CTA or a cluster of CTAs each
-// Every CTA has an equal run of the row's pieces.  The first DC_HELD of them lie in shared memory between the sums and the gradient, the others are
+// Every CTA has an equal run of the row's pieces.  The first `held` of them lie in shared memory between the sums and the gradient, the others are
 // read once more, from L2.  Several CTAs share an SM, so that some move data while others join sums or wait.  Listed columns become -infinity in shared
 // memory; the others' are named by a byte per piece.  Their gradients are written over what the loops over the run wrote.  The first CTA's first
 // warp adds up the loss while the others write the gradient.
 constexpr int DC_CTAS = 8, DC_LISTERS = DT_TOP / 32;
-// Rows of up to DC_SHORT pieces: six CTAs of 128 threads an SM (the steps of a row are a chain of latencies: 16384 rows of 9000 bf16 with their gradients
-// 168 us, with CTAs of 256 threads 311), lists of more than 128 entries apart.  Longer ones: three of 256 (4096 rows of 26000 bf16 113 us, 122 by CTAs of
-// 128; of 23000 110 and 99; of 131072 470 and 562, by two of 512 620 to 650, all pieces held by a cluster of four 504).
+// Rows of up to DC_SHORT pieces: six CTAs of 128 threads an SM, all held (the steps of a row are a chain of latencies: 16384 rows of 9000 bf16 with their
+// gradients 168 us, with CTAs of 256 threads 311), lists of more than 128 entries apart.  Longer ones, where a CTA takes a row and there are more of them than
+// run at a time: six of 256 threads, nothing held (8192 rows of 32768 bf16 217 us; three that hold 4000 pieces 245).  Rows of more than DC_RUN pieces, and
+// few rows: three of 256 that hold 4000 pieces (4096 rows of 131072 bf16 470 us; six that hold none 483, six of 128 562, two of 512 620 to 650, all
+// pieces held by a cluster of four 504).
 // The loss alone, of rows of more than DC_ONCE pieces and more of them than run at a time, needs a row once: nothing is held, eight CTAs of 128 threads or
 // six of 256 an SM (4096 rows of 131072 bf16 202 us, 5.3 TB/s, held 282; of 20000 57 and 76; 8192 of 16384 89 and 96, of 14000 87 and 82).
 constexpr int DC_SHORT = 3000, DC_ONCE = 1900, DC_HELD = 4000, DC_RUN = 8192;   // pieces: of short rows; of rows held all the same; held, and of a run, at most
@@ -567,6 +571,7 @@ __global__ void __launch_bounds__(DC_THREADS, CTAS_SM) distill_cluster_kernel(co
     const uint8_t* const mark = reinterpret_cast<const uint8_t*>(marks) - unmarked;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)(blockIdx.x % (unsigned)ctas);
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // (this CTA has started: the others may write its shared memory)
     const double inv = a.inv;
     const float inv_t = a.inv_t, c = a.c;
     const int most = (int)((a.cols / N + ctas - 1) / ctas);
@@ -596,6 +601,7 @@ __global__ void __launch_bounds__(DC_THREADS, CTAS_SM) distill_cluster_kernel(co
     const int edge_at = in_head ? tid : (int)a.cols - my.row.tail + tid - 32;
     const float edge = in_head || in_tail ? to_f32(z[edge_at]) : -INFINITY;
     __syncthreads();
+    if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     const int has = dc_has(a, e, s);
     if (skip_weight || !(has & 1)) {   // (the same for all CTAs of the row)
         if (rank == 0) {
@@ -769,10 +775,9 @@ template <typename T, int DG_THREADS> __global__ void __launch_bounds__(DG_THREA
     if (mine) dz[head.id] = from_f32<T>(k.inner * expf((zk - k.M) * inv_t) - k.scale * (P_all * k.p_scale));
 }
 
-template <typename T, int THREADS, int CTAS_SM, bool LOSS> int dc_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a, int ctas)
+template <typename T, int THREADS, int CTAS_SM, bool LOSS> int dc_launch(s2v_ctx* ctx, cudaStream_t st, const DtArgs& a, int ctas, int held)
 {
     const int64_t most = (a.cols / PIECE<T> + ctas - 1) / ctas;
-    const int held = (int)(most < DC_HELD ? most : DC_HELD);
     const auto kernel = distill_cluster_kernel<T, THREADS, CTAS_SM, LOSS>;
     S2V_CUDA_OK(ctx, s2v_allow_shared(kernel, DC_SMEM));
     cudaLaunchConfig_t cfg = {};
@@ -819,9 +824,11 @@ template <typename T, bool GRAD_ONLY> int dt_launch_type(s2v_ctx* ctx, cudaStrea
         return pieces <= 2 * DC_SHORT && a.top <= 128 ? dg_launch<T, 128>(ctx, st, a, ctas) : dg_launch<T, 256>(ctx, st, a, ctas);
     } else {
         while (ctas < DC_CTAS && (pieces > (int64_t)ctas * DC_RUN || (a.rows * ctas < 2 * ctx->sm_count && pieces >= (int64_t)ctas * 512))) ctas *= 2;
-        const bool once = !a.dz && pieces > DC_ONCE && a.rows * ctas >= 3 * ctx->sm_count;
-        if (pieces <= DC_SHORT && a.top <= 128) return once ? dc_launch<T, 128, 8, true>(ctx, st, a, ctas) : dc_launch<T, 128, 6, false>(ctx, st, a, ctas);
-        return once ? dc_launch<T, 256, 6, true>(ctx, st, a, ctas) : dc_launch<T, 256, 3, false>(ctx, st, a, ctas);
+        const bool many = a.rows * ctas >= 3 * ctx->sm_count, once = !a.dz && pieces > DC_ONCE && many;
+        const int held = (int)std::min<int64_t>(DC_HELD, (pieces + ctas - 1) / ctas);
+        if (pieces <= DC_SHORT && a.top <= 128) return once ? dc_launch<T, 128, 8, true>(ctx, st, a, ctas, held) : dc_launch<T, 128, 6, false>(ctx, st, a, ctas, held);
+        if (many && ctas == 1) return once ? dc_launch<T, 256, 6, true>(ctx, st, a, 1, 0) : dc_launch<T, 256, 6, false>(ctx, st, a, 1, 0);
+        return once ? dc_launch<T, 256, 6, true>(ctx, st, a, ctas, held) : dc_launch<T, 256, 3, false>(ctx, st, a, ctas, held);
     }
 }
 int dt_launch(s2v_ctx* ctx, s2v_stream stream, int z_type, bool grad_only, const DtArgs& a)
