@@ -719,8 +719,8 @@ __global__ void __launch_bounds__(DC_THREADS, CTAS_SM) distill_cluster_kernel(co
 }
 
 // The gradient from kept sums: nothing to wait for but the list.
-// (A CTA a row, of 128 threads up to 4096 pieces, else 256: 16384 x 9000 bf16 116 us, with 256 threads 177 and with 512 282; 4096 x 131072 bf16 347 us,
-// 6.2 TB/s, with 128 threads 364, and 454 where four CTAs shared a row.)
+// (CTAs of 128 threads up to 4096 pieces a row, else of 256: 16384 x 9000 bf16 116 us, with 256 threads 177 and with 512 282.  Long rows in several runs:
+// 4096 x 131072 bf16 337 us, 6.4 TB/s, a CTA a row 347, four CTAs 454; 483 x 186542 fp32 121 and 140; 1300 x 131072 fp32 215 and 232.)
 template <typename T, int DG_THREADS> __global__ void __launch_bounds__(DG_THREADS, 1024 / DG_THREADS) distill_grad_kernel(const DtArgs a, int ctas)
 {
     __shared__ DcShared s;
@@ -820,7 +820,9 @@ template <typename T, bool GRAD_ONLY> int dt_launch_type(s2v_ctx* ctx, cudaStrea
     if (a.rows * DC_CTAS > INT32_MAX) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, "distill_topk: more than 2^28 rows of this length");
     int ctas = 1;
     if constexpr (GRAD_ONLY) {
-        while (ctas < DC_CTAS && a.rows * ctas < 2 * ctx->sm_count && pieces >= (int64_t)ctas * 1024) ctas *= 2;
+        // CTAs for all SMs; and eight times as many as run at a time of long rows, so that none is left with the last ones
+        const auto runs = [&](int64_t waves, int64_t each) { return a.rows * ctas < waves * ctx->sm_count && pieces >= ctas * each; };
+        while (ctas < DC_CTAS && (runs(2, 1024) || runs(32, 8192))) ctas *= 2;
         return pieces <= 2 * DC_SHORT && a.top <= 128 ? dg_launch<T, 128>(ctx, st, a, ctas) : dg_launch<T, 256>(ctx, st, a, ctas);
     } else {
         while (ctas < DC_CTAS && (pieces > (int64_t)ctas * DC_RUN || (a.rows * ctas < 2 * ctx->sm_count && pieces >= (int64_t)ctas * 512))) ctas *= 2;
