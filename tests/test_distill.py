@@ -377,6 +377,36 @@ def test_losses_of_many_long_rows(gpu_ctx, dtype, cols, top, tail):
 
 
 @gpu
+@pytest.mark.parametrize("rows,dtype,cols,top", [(450, "f16", 17001, 128), (450, "bf16", 17001, 200), (460, "f32", 24001, 64), (310, "bf16", 70001, 30), (310, "f32", 140001, 150)])
+def test_gradients_of_many_long_rows_in_place(gpu_ctx, rows, dtype, cols, top):
+    """dz in the place of z gives what dz beside it gives, with rows wider than their columns and columns listed twice."""
+    some, idx, t, lse, w = inputs(31, cols, top, dtype, cols, True, 1.0)
+    idx[3, 1] = idx[3, 0]
+    n = -(-rows // 31)
+    idx, t, lse, w = (v.repeat(n, *([1] * (v.dim() - 1)))[:rows].contiguous() for v in (idx, t, lse, w))
+    wide = torch.full((rows, cols + 3), 9.0, dtype=some.dtype, device="cuda")
+    z = wide[:, :cols]
+    z.copy_(some.repeat(n, 1)[:rows])
+    loss, loss2, dz, stats = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda"), torch.empty_like(wide)[:, :cols], torch.empty((rows, 4), device="cuda")
+    more = {"t_lse": lse, "row_weight": w}
+    torch.cuda.synchronize()
+    gpu_ctx.distill_topk(z, idx, t, loss, dz=dz, **more)
+    gpu_ctx.distill_topk(z, idx, t, loss2, stats=stats, **more)
+    gpu_ctx.synchronize()
+    assert torch.equal(loss, loss2)
+    assert_matches(loss[:31], dz[:31], z[:31], idx[:31], t[:31], 1.0, lse[:31], w[:31])
+    kept = wide.clone()
+    later = torch.empty_like(wide)[:, :cols]
+    torch.cuda.synchronize()
+    gpu_ctx.distill_topk_grad(z, idx, t, stats, later, **more)
+    gpu_ctx.distill_topk(z, idx, t, loss2, dz=z, **more)
+    gpu_ctx.distill_topk_grad(kept[:, :cols], idx, t, stats, kept[:, :cols], **more)
+    gpu_ctx.synchronize()
+    assert torch.equal(loss, loss2) and torch.equal(z, dz) and torch.equal(kept[:, :cols], later)
+    assert bool((wide[:, cols:] == 9).all() and (kept[:, cols:] == 9).all())
+
+
+@gpu
 def test_captured_replayed_and_on_another_stream(gpu_ctx):
     for rows, cols in ((64, 6), (40, 3000), (12, 60000)):
         z, idx, t, lse, w = inputs(rows, cols, 5, "f16", rows, True, 1.0)

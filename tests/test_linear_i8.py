@@ -219,6 +219,25 @@ def test_outputs_inside_a_wider_matrix(gpu_ctx, m, n, k, ld, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(9999, 257, 33), (9999, 513, 129), (47001, 129, 129), (9999, 1025, 257), (15001, 257, 520), (15001, 257, 1001), (47001, 129, 1001), (47001, 129, 2050)])
+def test_product_of_many_tiles(gpu_ctx, m, n, k, dtype):
+    """Several tiles a CTA, with rows of outputs that start anywhere and on 16 bytes."""
+    gen = generator(m + n + k)
+    up = (k + 15) // 16 * 16
+    a, b = matrix(m, k, up, gen, torch.int8)[0], matrix(n, k, up, gen, torch.int8)[0]
+    sa, sb, bias = torch.rand(m, generator=gen, device="cuda") * 1e-2, torch.rand(n, generator=gen, device="cuda") * 1e-2, torch.randn(n, generator=gen, device="cuda")
+    want, size = product(a, sa, b, sb, bias, True)
+    for ld in (n, (n + 15) // 16 * 16):
+        buf = torch.full((m, ld), 3.0, dtype=TYPES[dtype], device="cuda")
+        torch.cuda.synchronize()
+        gpu_ctx.gemm_i8(a, sa, b, sb, buf[:, :n], bias=bias, relu=True)
+        gpu_ctx.synchronize()
+        assert_product(buf[:, :n], want, size)
+        assert bool((buf[:, n:] == 3).all())
+
+
+@gpu
 @pytest.mark.parametrize("m", [1, 5, 40, 200])
 def test_product_sums_are_exact_at_the_longest_rows(gpu_ctx, m):
     k, n = 131071, 70
@@ -323,6 +342,45 @@ def test_layer_captured_and_on_another_stream(gpu_ctx, m, n, k):
             assert torch.equal(y, first)
         q, s = quantized(x)
         assert_product(y, *product(torch.from_numpy(q), torch.from_numpy(s), w, sw, None, False))
+    gpu_ctx.synchronize()
+
+
+@gpu
+def test_two_layers_at_once(gpu_ctx):
+    """Calls on two streams, each with its own workspace, and graphs of them that replay side by side."""
+    gen = generator(11)
+    w, _ = matrix(700, 520, 528, gen, torch.int8)
+    sw = torch.rand(700, generator=gen, device="cuda")
+    calls = []
+    for m in (2000, 40):
+        x, y = torch.randn((m, 520), generator=gen, device="cuda"), torch.empty((m, 700), device="cuda")
+        calls.append((x, y, torch.empty(gpu_ctx.linear_i8_workspace_bytes(m, 520), dtype=torch.uint8, device="cuda"), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    first = []
+    for x, y, ws, _ in calls:
+        gpu_ctx.linear_i8(x, w, sw, y, ws)
+        gpu_ctx.synchronize()
+        first.append(y.clone())
+    graphs = []
+    for x, y, ws, side in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            for _ in range(4):
+                gpu_ctx.linear_i8(x, w, sw, y, ws, stream=side.cuda_stream)
+        graphs.append(graph)
+    for replayed in (False, True):
+        for _, y, _, _ in calls:
+            y.fill_(-1)
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for (x, y, ws, side), graph in zip(calls, graphs):
+                if replayed:
+                    with torch.cuda.stream(side):
+                        graph.replay()
+                else:
+                    gpu_ctx.linear_i8(x, w, sw, y, ws, stream=side.cuda_stream)
+        torch.cuda.synchronize()
+        assert all(torch.equal(c[1], f) for c, f in zip(calls, first))
     gpu_ctx.synchronize()
 
 
