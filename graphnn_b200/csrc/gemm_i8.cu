@@ -249,6 +249,8 @@ __device__ __forceinline__ void gi_write(const GiArgs& a, const CUtensorMap* map
                 }
             }
         }
+        // a piece is a bulk group in any case: the wait before a box is filled counts groups, and this one's turn is over like a copy's
+        if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         __syncwarp();
     }
 }
@@ -411,7 +413,7 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
                 uint32_t(&now)[COLS] = v[c / COLS & 1];
                 gi_wait_loads(now);
                 if (c + COLS < cols && a.kblocks > 0) gi_fetch<T>(at + (uint32_t)(c + COLS), v[~(c / COLS) & 1]);
-                // the copy that last read this box has done so
+                // the copy that last read this box has done so: of the groups since then, one a piece, as many may be under way as there are other boxes
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(Cfg::BOXES - 1) : "memory");
                 __syncwarp();
                 gi_write<T, HALF>(a, &map_c, boxes + turn * GI_BOX, chan + c, to_row, to_col + c, sa2, now);

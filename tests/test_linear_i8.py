@@ -238,6 +238,26 @@ def test_product_of_many_tiles(gpu_ctx, m, n, k, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,ld,k", [(20000, 1021, 1024, 64), (20000, 1021, 1024, 128), (30011, 2041, 2048, 128), (20000, 2041, 2048, 64), (60000, 253, 256, 32), (9000, 1021, 1040, 300)])
+def test_many_tiles_whose_rows_end_inside_16_bytes(gpu_ctx, m, n, ld, k, dtype):
+    """Few sums an output and a CTA's tiles one right behind the other; a tile's last columns leave by stores, those in front of them and the next tile's by
+    copies.  Scales of powers of two: every output is exact before its only rounding, so that all of them are equal, in every one of many calls."""
+    gen = generator(m + n + k)
+    a, b = matrix(m, k, (k + 15) // 16 * 16, gen, torch.int8)[0], matrix(n, k, (k + 15) // 16 * 16, gen, torch.int8)[0]
+    sa, sb = (torch.exp2(torch.randint(-6, 0, (r,), generator=gen, device="cuda").float()) for r in (m, n))
+    want = torch.cat([(part.double() @ b.double().t()).float() for part in a.split(10000)]) * sa[:, None] * sb[None, :]
+    want = want.to(TYPES[dtype])
+    c = torch.empty((m, ld), dtype=TYPES[dtype], device="cuda")
+    for _ in range(12):
+        c.fill_(3)
+        torch.cuda.synchronize()
+        gpu_ctx.gemm_i8(a, sa, b, sb, c[:, :n])
+        gpu_ctx.synchronize()
+        assert torch.equal(c[:, :n], want) and bool((c[:, n:] == 3).all())
+
+
+@gpu
 @pytest.mark.parametrize("m", [1, 5, 40, 200])
 def test_product_sums_are_exact_at_the_longest_rows(gpu_ctx, m):
     k, n = 131071, 70
