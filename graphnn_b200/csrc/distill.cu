@@ -54,6 +54,19 @@ __device__ __forceinline__ float dt_warp_max(float v)
     for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
+// The largest of the teacher's logits: NaN where one of them is, so that a list of NaN is none whose every t is -infinity.
+__device__ __forceinline__ float dt_nan_max(float a, float b)
+{
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+__device__ __forceinline__ float dt_warp_nan_max(float v)
+{
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = dt_nan_max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
 
 // ---------------------------------------------------------------- sums and gradients of pieces of 16 bytes
 __device__ __forceinline__ uint64_t dt_two(float a, float b)
@@ -326,10 +339,10 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
             s.id[k] = id;
             if (id < 0) continue;
             some = true;
-            tmax = fmaxf(tmax, dt_load_t(a, r, k));
+            tmax = dt_nan_max(tmax, dt_load_t(a, r, k));
         }
         some = __any_sync(0xffffffffu, some);
-        tmax = dt_warp_max(tmax);
+        tmax = dt_warp_nan_max(tmax);
         if (!some || (!a.t_lse && tmax == -INFINITY) || (weight == 0.0f && (GRAD_ONLY || !a.stats))) {
             if (!GRAD_ONLY && lane == 0) a.loss[r] = 0.0f;
             if (!GRAD_ONLY && a.stats && lane < 4) a.stats[4 * r + lane] = 0.0f;
@@ -488,11 +501,11 @@ __device__ __forceinline__ DcEntry dc_entry(const DtArgs& a, const DcHead& h, Dc
     DcEntry e{h.id >= 0 ? h.t : -INFINITY, -INFINITY, 0.0f, false};
     if (!a.t_lse) {
         if (lister) {
-            const float m = dt_warp_max(e.t);
+            const float m = dt_warp_nan_max(e.t);
             if (lane == 0) s.tmax[warp] = m;
         }
         __syncthreads();
-        for (int w = 0; w * 32 < a.top; ++w) e.tmax = fmaxf(e.tmax, s.tmax[w]);
+        for (int w = 0; w * 32 < a.top; ++w) e.tmax = dt_nan_max(e.tmax, s.tmax[w]);
     }
     if (lister) {
         if (h.id >= 0) {

@@ -288,6 +288,45 @@ def test_teachers_that_are_not_finite(gpu_ctx, cols, tail):
 
 
 @gpu
+@pytest.mark.parametrize("rows,cols,dtype,top", [(9, 12, "f32", 5), (9, 700, "f16", 5), (9, 2050, "f32", 40), (9, 6000, "bf16", 7), (9, 40000, "f32", 130), (460, 8203, "f32", 5), (460, 20001, "bf16", 129)])
+@pytest.mark.parametrize("tail", [False, True])
+def test_teachers_without_a_number(gpu_ctx, rows, cols, dtype, top, tail):
+    """A list of NaN alone, or of NaN and -infinity, gives NaN; only one where every t is -infinity is a teacher without mass."""
+    z, idx, t, lse, _ = inputs(9, cols, top, dtype, cols, tail, 1.0, ragged=False)
+    w = torch.ones(9, device="cuda")
+    nan = float("nan")
+    t[0] = nan
+    t[1], t[1, top - 1] = -INF, nan
+    t[2], idx[2, 1:] = nan, -1                          # a list of one entry
+    t[3] = -INF
+    t[4], idx[4, 0], t[4, 0] = -INF, -1, nan            # the NaN is at an entry that is not there
+    t[5], w[5] = nan, 0.0                               # a padded row
+    t[6], t[6, 0], t[6, 1] = -INF, nan, 0.5
+    n = -(-rows // 9)
+    z, idx, t, w = (v.repeat(n, *([1] * (v.dim() - 1)))[:rows].contiguous() for v in (z, idx, t, w))
+    lse = None if lse is None else lse.repeat(n)[:rows].contiguous()
+    loss, dz = torch.full((rows,), 5.0, device="cuda"), torch.full_like(z, 5.0)
+    alone, kept, later, stats = loss.clone(), loss.clone(), dz.clone(), torch.empty((rows, 4), device="cuda")
+    more = {"t_lse": lse, "row_weight": w}
+    torch.cuda.synchronize()
+    gpu_ctx.distill_topk(z, idx, t, loss, dz=dz, **more)
+    gpu_ctx.distill_topk(z, idx, t, alone, **more)
+    gpu_ctx.distill_topk(z, idx, t, kept, stats=stats, **more)
+    gpu_ctx.distill_topk_grad(z, idx, t, stats, later, **more)
+    gpu_ctx.synchronize()
+    i = torch.arange(rows, device="cuda") % 9
+    for of_nan in (0, 1, 2, 6):
+        at = i == of_nan
+        assert all(bool(v[at].isnan().all()) for v in (loss, alone, kept, dz, later)), of_nan
+    empty = (i == 5) | ((i == 3) | (i == 4)) & (not tail)
+    assert not any(bool(v[empty].any()) for v in (loss, alone, kept, dz, later))
+    rest = [j for j in (3, 4, 5, 7, 8) if j < rows]
+    t = t.nan_to_num(nan=0.0, neginf=-INF)
+    for got, grad in ((loss, dz), (alone, None), (kept, later)):
+        assert_matches(got[rest], None if grad is None else grad[rest], z[rest], idx[rest], t[rest], 1.0, None if lse is None else lse[rest], w[rest])
+
+
+@gpu
 @pytest.mark.parametrize("cols", [40, 2000, 9000, 70000])
 @pytest.mark.parametrize("tail", [False, True])
 def test_lists_of_one_class_over_and_over(gpu_ctx, cols, tail):
