@@ -5,7 +5,7 @@
 //     log q_j = (z_j - M) / T - log total,     log s = -log(1 + exp(d)),  d = log(S_in / S_out) + (M_in - M_out) / T.
 // Taking one sum from the other's total would lose s (or 1 - s) where the student gives nearly everything (or nothing) to the list, and one
 // maximum for both would lose the smaller sum where they are far apart (logits masked with the type's lowest value).  The loss is put together in 64
-// bits (it is a difference of larger numbers), the sums over columns and the gradient in fp32.
+// bits (it is a difference of larger numbers), and so are the list's p, of whose sum little may be left; the sums over columns and the gradient in fp32.
 #include <algorithm>
 
 #include "elem_types.cuh"
@@ -239,9 +239,9 @@ __device__ __forceinline__ double dt_log_p(const DtArgs& a, float tv, float tmax
 }
 
 // an entry's part of Z, A and B (B relative to l.m, the largest listed z)
-__device__ __forceinline__ void dt_count(const DtArgs& a, DtList& l, float tv, float tmax, double t_lse, float zk, double inv_t)
+__device__ __forceinline__ void dt_count(const DtArgs& a, DtList& l, double P, float tv, float tmax, double t_lse, float zk, double inv_t)
 {
-    const double lp = dt_log_p(a, tv, tmax, t_lse, inv_t), P = exp(lp);
+    const double lp = dt_log_p(a, tv, tmax, t_lse, inv_t);
     l.Z += P;
     if (P != 0.0) {
         l.A += P * lp;
@@ -257,6 +257,7 @@ struct DtCoef {
     float outer;        // any other's: outer * exp((z - m_out) / T)
     float scale;        // row_weight / T
 };
+// 1 - sum P is taken in 64 bits; what is made of it in fp32 are factors, each off by a few 2^-24 of itself (outer: of its larger term, both are parts of the gradient).
 __device__ __forceinline__ DtCoef dt_coefficients(const DtArgs& a, double Z, const DtSum& in, const DtSum& out, float weight, float inv_t, float c)
 {
     DtCoef k;
@@ -467,11 +468,16 @@ constexpr int DC_SMEM = 72 << 10;
 static_assert(DC_HELD * 16 + (DC_RUN - DC_HELD) <= DC_SMEM && DC_SHORT <= DC_HELD, "a byte for each piece that is not held");
 constexpr int DC_SLOTS = 512;                        // of the table that finds columns listed twice
 struct DcShared {
-    float P[DT_TOP], t[DT_TOP], z[DT_TOP];
-    int id[DT_TOP], slot[DC_SLOTS];
+    double P[DT_TOP], Z[DC_LISTERS];
+    union {
+        int slot[DC_SLOTS];
+        float z[DT_TOP];   // (once the table has been used)
+    };
+    float t[DT_TOP];
+    int id[DT_TOP];
     float4 peer[DC_CTAS];      // outer and inner sums of the cluster's CTAs
     float2 outer[16], inner[DC_LISTERS];
-    float Z[DC_LISTERS], tmax[DC_LISTERS];
+    float tmax[DC_LISTERS];
     int has[DC_LISTERS];       // bit 0: an entry; bit 1: a column that is listed twice
 };
 
@@ -489,16 +495,17 @@ struct DcHead {
         }
     }
 };
-// What every thread with an entry knows of it, before z is looked at.  P in fp32: the gradient's rest, 1 - sum P, is off by 2^-23 at most.
+// What every thread with an entry knows of it, before z is looked at.
 struct DcEntry {
-    float t, tmax, P;
+    float t, tmax;
+    double P;
     bool twice;   // whether another entry of this column was there first
 };
 __device__ __forceinline__ DcEntry dc_entry(const DtArgs& a, const DcHead& h, DcShared& s)
 {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const bool lister = warp * 32 < a.top;   // warps with entries
-    DcEntry e{h.id >= 0 ? h.t : -INFINITY, -INFINITY, 0.0f, false};
+    DcEntry e{h.id >= 0 ? h.t : -INFINITY, -INFINITY, 0.0, false};
     if (!a.t_lse) {
         if (lister) {
             const float m = dt_warp_nan_max(e.t);
@@ -509,19 +516,30 @@ __device__ __forceinline__ DcEntry dc_entry(const DtArgs& a, const DcHead& h, Dc
     }
     if (lister) {
         if (h.id >= 0) {
-            e.P = expf(a.t_lse ? e.t * a.inv_t - h.t_lse : (e.t - dt_finite_or_zero(e.tmax)) * a.inv_t);
             int was, at = h.id & (DC_SLOTS - 1);   // (twice as many places as entries)
             while ((was = atomicCAS(&s.slot[at], -1, h.id)) != -1 && was != h.id) at = (at + 1) & (DC_SLOTS - 1);
             e.twice = was == h.id;
         }
         s.id[tid] = h.id;
         s.t[tid] = e.t;
-        s.P[tid] = e.P;
-        const float Z = dt_warp_sum(e.P);
         const int has = (__any_sync(0xffffffffu, h.id >= 0) ? 1 : 0) | (__any_sync(0xffffffffu, e.twice) ? 2 : 0);
-        if (lane == 0) s.Z[warp] = Z, s.has[warp] = has;
+        if (lane == 0) s.has[warp] = has;
     }
     return e;
+}
+// The entries' P and their sum, in 64 bits: where the list has nearly everything, the gradient goes by 1 - sum P, and t / T - t_lse in fp32 is off by 2^-24 of |t / T|
+// and more (T = 1.5, t around 200, a rest of 1e-4: the gradient of what is not listed by some hundredths of itself).
+__device__ __forceinline__ void dc_weigh(const DtArgs& a, const DcHead& h, DcEntry& e, DcShared& s)
+{
+    if ((threadIdx.x & ~31) >= a.top) return;
+    // Nothing of this is done ahead of the row's other loads: converted to 64 bits where it is loaded, the normaliser made every thread wait for it before it asked for
+    // the rest (16384 x 9000 bf16 loss 127 us instead of 114, with gradient 169 and 157).
+    float t_lse = h.t_lse;
+    asm volatile("" : "+f"(t_lse), "+f"(e.t));
+    if (h.id >= 0) e.P = exp(dt_log_p(a, e.t, e.tmax, (double)t_lse, a.inv));
+    s.P[threadIdx.x] = e.P;
+    const double Z = dt_warp_sum(e.P);
+    if ((threadIdx.x & 31) == 0) s.Z[threadIdx.x >> 5] = Z;
 }
 // (after a barrier) bit 0: the row's list has an entry that counts; bit 1: a column is listed twice
 __device__ __forceinline__ int dc_has(const DtArgs& a, const DcEntry& e, const DcShared& s)
@@ -534,17 +552,18 @@ __device__ __forceinline__ int dc_has(const DtArgs& a, const DcEntry& e, const D
 __device__ __forceinline__ bool dc_first(const DtArgs& a, int id, const DcShared& s, float& P)
 {
     bool first = true;
-    P = 0.0f;
+    double sum = 0.0;
     for (int k = 0; k < a.top; ++k)
         if (s.id[k] == id) {
-            P += s.P[k];
+            sum += s.P[k];
             if (k < (int)threadIdx.x) first = false;
         }
+    P = (float)sum;
     return first;
 }
-__device__ __forceinline__ float dc_Z(const DtArgs& a, const DcShared& s)
+__device__ __forceinline__ double dc_Z(const DtArgs& a, const DcShared& s)
 {
-    float Z = 0.0f;
+    double Z = 0.0;
     for (int w = 0; w * 32 < a.top; ++w) Z += s.Z[w];
     return Z;
 }
@@ -603,11 +622,12 @@ __global__ void __launch_bounds__(DC_THREADS, CTAS_SM) distill_cluster_kernel(co
     if (!LOSS && !skip_weight)
         for (int p = tid; p < kept; p += DC_THREADS) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(run + p)), "l"(zp + p) : "memory");
     __syncthreads();   // the table and the marks are empty
-    const DcEntry e = dc_entry(a, head, s);
+    DcEntry e = dc_entry(a, head, s);
+    dc_weigh(a, head, e, s);
     int at;
     const bool here = my.has(head.id, rank, ctas, at), held_entry = !LOSS && here && at >= 0 && at < held * N;
     bool mine = here && !e.twice;
-    float P_all = e.P, zk = (here && !held_entry) || (rank == 0 && head.id >= 0) ? to_f32(z[head.id]) : -INFINITY;
+    float P_all = (float)e.P, zk = (here && !held_entry) || (rank == 0 && head.id >= 0) ? to_f32(z[head.id]) : -INFINITY;
     if (here && at >= unmarked * N) atomicOr(&marks[(at / N - unmarked) >> 2], 1u << (8 * ((at / N - unmarked) & 3) + at % N));
     // the scalar columns: the head's to the first CTA, the tail's to the last
     const bool in_head = rank == 0 && tid < my.row.head, in_tail = rank == ctas - 1 && tid >= 32 && tid < 32 + my.row.tail;
@@ -724,7 +744,7 @@ __global__ void __launch_bounds__(DC_THREADS, CTAS_SM) distill_cluster_kernel(co
     if (rank == 0 && warp == 0) {
         DtList l{0.0, 0.0, 0.0, (double)inner.s, inner.m};
         for (int k = lane; k < a.top; k += 32)
-            if (s.id[k] >= 0) dt_count(a, l, s.t[k], e.tmax, (double)head.t_lse, s.z[k], inv);
+            if (s.id[k] >= 0) dt_count(a, l, s.P[k], s.t[k], e.tmax, (double)head.t_lse, s.z[k], inv);
         l.Z = dt_warp_sum(l.Z), l.A = dt_warp_sum(l.A), l.B = dt_warp_sum(l.B);
         const float loss = dt_loss(a, l, outer, weight, inv, c);
         if (lane == 0) a.loss[r] = weight == 0.0f ? 0.0f : loss;
@@ -749,16 +769,17 @@ template <typename T, int DG_THREADS> __global__ void __launch_bounds__(DG_THREA
     const float weight = head.weight;
     const float4 st = __ldg(reinterpret_cast<const float4*>(a.stats) + r);
     const DcRun<T> my(z, a.cols, rank, ctas);
-    __syncthreads();   // the table is empty
-    const DcEntry e = dc_entry(a, head, s);
     int at;
     const bool here = my.has(head.id, rank, ctas, at);
-    bool mine = here && !e.twice;
-    float P_all = e.P;
-    const float zk = here ? to_f32(z[head.id]) : 0.0f;
+    const float zk = here ? to_f32(z[head.id]) : 0.0f;   // (on its way under the exponentials)
     const bool in_head = rank == 0 && tid < my.row.head, in_tail = rank == ctas - 1 && tid >= 32 && tid < 32 + my.row.tail;
     const int edge_at = in_head ? tid : (int)a.cols - my.row.tail + tid - 32;
     const float edge = in_head || in_tail ? to_f32(z[edge_at]) : 0.0f;
+    __syncthreads();   // the table is empty
+    DcEntry e = dc_entry(a, head, s);
+    dc_weigh(a, head, e, s);
+    bool mine = here && !e.twice;
+    float P_all = (float)e.P;
     // (the barrier also stands between the reads of listed columns and the writes: dz may be z)
     __syncthreads();
     const int has = dc_has(a, e, s);

@@ -327,6 +327,35 @@ def test_teachers_without_a_number(gpu_ctx, rows, cols, dtype, top, tail):
 
 
 @gpu
+@pytest.mark.parametrize("rows,cols,top", [(5, 700, 64), (5, 5000, 64), (5, 40003, 200), (450, 8203, 64)])
+@pytest.mark.parametrize("temp,offset", [(1.5, 20.0), (1.5, 200.0), (3.0, 60.0), (0.7, -150.0)])
+def test_small_rests_at_temperatures_that_are_no_powers_of_two(gpu_ctx, rows, cols, top, temp, offset):
+    """A teacher that gives the list all but 1e-4, far from zero, and a student that does nearly the same: the gradient of what is not listed goes by rest / s."""
+    temp = float(torch.tensor(temp))     # as the call takes it: 0.7 in fp32
+    gen = torch.Generator().manual_seed(cols + top)
+    idx = torch.stack([torch.randperm(cols, generator=gen)[:top] for _ in range(5)]).to(torch.int32)
+    t = (offset + 3 * torch.randn((5, top), generator=gen)).float()
+    # (t_lse as fp32 has it is the definition's: the rest is what it leaves, anywhere around 1e-4)
+    lse = (torch.logsumexp(t.double() / temp, 1) - math.log1p(-1e-4)).float()
+    z = 0.5 * temp * torch.randn((5, cols), generator=gen)
+    z.scatter_(1, idx.long(), temp * (torch.randn((5, top), generator=gen) + math.log(cols / top) + 9.0))
+    n = rows // 5
+    z, idx, t, lse = (v.repeat(n, *([1] * (v.dim() - 1))).cuda() for v in (z, idx, t, lse))
+    w = torch.full((rows,), 0.75, device="cuda")
+    loss, dz = torch.empty(rows, device="cuda"), torch.empty_like(z)
+    later, stats = torch.empty_like(z), torch.empty((rows, 4), device="cuda")
+    torch.cuda.synchronize()
+    more = {"temperature": temp, "t_lse": lse, "row_weight": w}
+    gpu_ctx.distill_topk(z, idx, t, loss, dz=dz, **more)
+    gpu_ctx.distill_topk(z, idx, t, loss, stats=stats, **more)
+    gpu_ctx.distill_topk_grad(z, idx, t, stats, later, **more)
+    gpu_ctx.synchronize()
+    for grad in (dz, later):
+        assert_matches(loss[:5], grad[:5], z[:5], idx[:5], t[:5], temp, lse[:5], w[:5])
+        assert torch.equal(grad.view(n, 5, cols)[0], grad.view(n, 5, cols)[(n - 1) // 4 * 4])     # (rows that lie alike)
+
+
+@gpu
 @pytest.mark.parametrize("cols", [40, 2000, 9000, 70000])
 @pytest.mark.parametrize("tail", [False, True])
 def test_lists_of_one_class_over_and_over(gpu_ctx, cols, tail):
