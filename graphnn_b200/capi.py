@@ -10,7 +10,6 @@ import ctypes as C
 import os
 
 import numpy as np
-import torch
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libs2v_b200.so")
@@ -199,8 +198,8 @@ def validate_csr_host(m: int, k: int, row_ptr: np.ndarray, col_idx: np.ndarray) 
     return lib.s2v_validate_csr_host(m, k, int(ci.shape[0]), _ptr(rp), _ptr(ci))
 
 
-# s2v_dtype
-_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+# s2v_dtype by torch's types.  torch is imported by the methods that check its tensors, not by this module: the host-side functions need numpy alone.
+_DTYPES = {}
 
 
 def _refuse(text: str):
@@ -220,12 +219,16 @@ def _matrix(name: str, t, device: int, rows: int, cols: int, dtype) -> int:
 
 def _vector(name: str, t, device: int, length: int):
     """Checks an fp32 device vector."""
+    import torch
     if not (t.dtype is torch.float32 and t.get_device() == device and t.shape == (length,) and t.is_contiguous()):
         _refuse(f"{name} is no contiguous fp32 vector of {length} on cuda:{device}, but {tuple(t.shape)} of {t.dtype} on {t.device}")
 
 
 def _sizes(name: str, t):
     """Rows, columns and element type of a matrix that the others go by."""
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
     if len(t.shape) != 2 or t.dtype not in _DTYPES:
         _refuse(f"{name} is no matrix of fp32, fp16 or bf16 numbers, but {tuple(t.shape)} of {t.dtype}")
     return (*t.shape, t.dtype)
@@ -414,6 +417,7 @@ class Context:
     # -- dense layers with 8-bit weights (types: fp32, fp16, bf16; matrices may have a leading dimension of their own)
     def quantize_rows_i8(self, x, q, scale, stream=None):
         """s2v_quantize_rows_i8: rows of x to int8 q and fp32 scale, x ~ scale[:, None] * q."""
+        import torch
         rows, cols, dtype = _sizes("x", x)
         dev = self.device
         ldx, ldq = _matrix("x", x, dev, rows, cols, dtype), _matrix("q", q, dev, rows, cols, torch.int8)
@@ -423,6 +427,7 @@ class Context:
 
     def gemm_i8(self, A, a_scale, B, b_scale, C_out, bias=None, relu=False, stream=None):
         """s2v_gemm_i8: C = act((a_scale x b_scale) * (A B^T) + bias) with int8 A [m x k] and B [n x k], rows on 16-byte boundaries."""
+        import torch
         m, n, dtype = _sizes("C_out", C_out)
         k, dev = A.shape[-1], self.device
         lda, ldb, ldc = _matrix("A", A, dev, m, k, torch.int8), _matrix("B", B, dev, n, k, torch.int8), _matrix("C_out", C_out, dev, m, n, dtype)
@@ -440,6 +445,7 @@ class Context:
 
     def linear_i8(self, x, W, w_scale, y, workspace, bias=None, relu=False, stream=None):
         """s2v_linear_i8: y = act(x W^T + bias) with x quantised row by row on the way; W int8 [n x k] with a scale per row."""
+        import torch
         (m, k, xtype), (rows, n, ytype), dev = _sizes("x", x), _sizes("y", y), self.device
         ldx, ldw, ldy = _matrix("x", x, dev, m, k, xtype), _matrix("W", W, dev, n, k, torch.int8), _matrix("y", y, dev, m, n, ytype)
         _vector("w_scale", w_scale, dev, n)
@@ -454,6 +460,7 @@ class Context:
 
     # -- distillation from a teacher's top logits
     def _distill_args(self, z, idx, t, temperature, t_lse, row_weight, loss, stats, dz):
+        import torch
         (rows, cols, dtype), (_, top, ttype), dev = _sizes("z", z), _sizes("t", t), self.device
         ldz, ldt = _matrix("z", z, dev, rows, cols, dtype), _matrix("t", t, dev, rows, top, ttype)
         if _matrix("idx", idx, dev, rows, top, torch.int32) != ldt and rows > 1:

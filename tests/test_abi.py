@@ -3,6 +3,8 @@ its host-only entry points work without a GPU."""
 import ctypes
 import os
 import re
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -164,3 +166,14 @@ def test_levels_pass_their_entry_count():
         ctx.h = None   # (nothing to close)
     assert [(n, a[:4]) for n, a in calls] == [("s2v_level_nnz_f32", (4, 7, 10, 32)), ("s2v_level_rp64_f32", (4, 7, 32, calls[1][1][3])),
                                               ("s2v_level_lookup_nnz_f32", (4, 7, 10, 32)), ("s2v_level_nnz_f32", (4, 7, 0, 32))]
+
+
+def test_host_functions_need_no_torch(lib):
+    """The binding's host-side part is imported and used where torch is not installed."""
+    code = ("import sys; sys.modules['torch'] = None\n"
+            "import numpy as np\n"
+            "from graphnn_b200 import capi\n"
+            "rp, ci, _ = capi.build_n2n_csr_host(3, np.array([0, 1], np.int32), np.array([1, 2], np.int32))\n"
+            "assert capi.validate_csr_host(3, 3, rp, ci) == 0\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=REPO, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
