@@ -851,7 +851,7 @@ template <typename T, bool GRAD_ONLY> int dt_launch_type(s2v_ctx* ctx, cudaStrea
     if (pieces <= 32) return dw_launch<T, 1, GRAD_ONLY>(ctx, st, a);
     if (pieces <= 32 * 8) return dw_launch<T, 8, GRAD_ONLY>(ctx, st, a);
     if (pieces <= 32 * DW_PIECES) return dw_launch<T, DW_PIECES, GRAD_ONLY>(ctx, st, a);
-    if (a.rows * DC_CTAS > INT32_MAX) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, "distill_topk: more than 2^28 rows of this length");
+    if (a.rows > INT32_MAX / DC_CTAS) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, "distill_topk: more than 2^28 rows of this length");
     int ctas = 1;
     if constexpr (GRAD_ONLY) {
         // CTAs for all SMs; and eight times as many as run at a time of long rows, so that none is left with the last ones
@@ -885,7 +885,7 @@ int dt_check(s2v_ctx* ctx, const char* name, int z_type, const DtArgs& a)
     if (a.rows == 0) return S2V_OK;
     if (!a.z || !a.idx || !a.t) return bad(S2V_ERR_INVALID_ARG, "NULL pointer");
     if (a.top > DT_TOP) return bad(S2V_ERR_UNSUPPORTED, "more than 256 entries a row");
-    if (a.cols * (int64_t)s2v_dtype_bytes(z_type) > DT_ROW_BYTES) return bad(S2V_ERR_UNSUPPORTED, "rows of more than 1,048,576 bytes");
+    if (a.cols > DT_ROW_BYTES / (int64_t)s2v_dtype_bytes(z_type)) return bad(S2V_ERR_UNSUPPORTED, "rows of more than 1,048,576 bytes");
     if (a.rows > 1 && (a.ldz < a.cols || a.ldt < a.top || (a.dz && a.lddz < a.cols)))
         return bad(S2V_ERR_INVALID_ARG, "leading dimension below the number of columns");
     const size_t es = s2v_dtype_bytes(z_type);

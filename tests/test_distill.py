@@ -524,6 +524,18 @@ def test_refusals(gpu_ctx):
     assert not f.any()
 
 
+@gpu
+@pytest.mark.parametrize("cols", [1 << 61, 1 << 62, (1 << 63) - 1, (1 << 62) + 8, (1 << 32) + 5])
+def test_refusal_of_rows_whose_bytes_pass_64_bits(gpu_ctx, cols):
+    f, i = torch.zeros(64, device="cuda"), torch.zeros(8, dtype=torch.int32, device="cuda")
+    p, ip = f.data_ptr(), i.data_ptr()
+    for zt in (0, 1, 2):
+        assert gpu_ctx.lib.s2v_distill_topk(gpu_ctx.h, None, 1, cols, zt, p, cols, 1, ip, 0, p, 1, None, 1.0, None, p, None, None, 0) == -2
+        assert gpu_ctx.lib.s2v_distill_topk_grad(gpu_ctx.h, None, 1, cols, zt, p, cols, 1, ip, 0, p, 1, None, 1.0, None, p, p, cols) == -2
+    gpu_ctx.synchronize()
+    assert not f.any()
+
+
 # ---------------------------------------------------------------- together, as they are used
 @gpu
 def test_an_8_bit_student_of_the_readout(gpu_ctx):
