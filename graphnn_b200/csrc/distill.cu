@@ -889,7 +889,8 @@ int dt_check(s2v_ctx* ctx, const char* name, int z_type, const DtArgs& a)
     if (a.rows > 1 && (a.ldz < a.cols || a.ldt < a.top || (a.dz && a.lddz < a.cols)))
         return bad(S2V_ERR_INVALID_ARG, "leading dimension below the number of columns");
     const size_t es = s2v_dtype_bytes(z_type);
-    if (reinterpret_cast<uintptr_t>(a.z) % es || reinterpret_cast<uintptr_t>(a.dz) % es || reinterpret_cast<uintptr_t>(a.t) % s2v_dtype_bytes(a.t_type))
+    if (reinterpret_cast<uintptr_t>(a.z) % es || reinterpret_cast<uintptr_t>(a.dz) % es || reinterpret_cast<uintptr_t>(a.t) % s2v_dtype_bytes(a.t_type) ||
+        !s2v_aligned4(a.idx, a.t_lse, a.row_weight, a.loss))
         return bad(S2V_ERR_INVALID_ARG, "misaligned pointer");
     if (!s2v_aligned16(a.stats)) return bad(S2V_ERR_INVALID_ARG, "stats must be 16-byte aligned");
     if (a.dz == a.z && a.rows > 1 && a.lddz != a.ldz) return bad(S2V_ERR_INVALID_ARG, "dz in the place of z needs the same leading dimension");

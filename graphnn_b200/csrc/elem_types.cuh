@@ -16,6 +16,11 @@ inline size_t s2v_dtype_bytes(int t)
 {
     return t == S2V_F32 ? 4 : 2;
 }
+// whether arrays of 32-bit numbers (NULL ones among them) lie as a kernel's loads and stores need them
+template <typename... P> inline bool s2v_aligned4(const P*... p)
+{
+    return ((reinterpret_cast<uintptr_t>(p) | ...) & 3u) == 0;
+}
 
 #ifdef __CUDACC__
 namespace

@@ -129,8 +129,8 @@ size_t workspace_scale_offset(int64_t m, int64_t k)
     return (size_t)m * (size_t)((k + 15) / 16 * 16);
 }
 
-int check_gemm(s2v_ctx* ctx, const char* name, int64_t m, int64_t n, int64_t k, const int8_t* B, int64_t ldb, const float* b_scale, int c_type, const void* C,
-               int64_t ldc)
+int check_gemm(s2v_ctx* ctx, const char* name, int64_t m, int64_t n, int64_t k, const int8_t* B, int64_t ldb, const float* b_scale, const float* bias, int c_type,
+               const void* C, int64_t ldc)
 {
     const auto bad = [&](int status, const char* what) { return s2v_fail(ctx, status, std::string(name) + ": " + what); };
     if (m < 0 || n < 0 || k < 0) return bad(S2V_ERR_INVALID_ARG, "negative size");
@@ -143,6 +143,7 @@ int check_gemm(s2v_ctx* ctx, const char* name, int64_t m, int64_t n, int64_t k, 
         return bad(S2V_ERR_INVALID_ARG, "leading dimension too small, or of an 8-bit matrix no multiple of 16");
     if (!s2v_aligned16(B)) return bad(S2V_ERR_INVALID_ARG, "8-bit matrices must be 16-byte aligned");
     if (reinterpret_cast<uintptr_t>(C) % s2v_dtype_bytes(c_type)) return bad(S2V_ERR_INVALID_ARG, "misaligned output");
+    if (!s2v_aligned4(b_scale, bias)) return bad(S2V_ERR_INVALID_ARG, "misaligned scales or bias");
     return S2V_OK;
 }
 
@@ -157,6 +158,7 @@ int s2v_quantize_rows_i8(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t 
     const int rc = check_quantize(ctx, "quantize_rows", rows, cols, x_type, x, ldx);
     if (rc != S2V_OK || rows == 0) return rc;
     if (!scale || (cols > 0 && !q)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "quantize_rows: NULL pointer");
+    if (!s2v_aligned4(scale)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "quantize_rows: misaligned scale");
     if (rows > 1 && ldq < cols) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "quantize_rows: leading dimension below the number of columns");
     cudaStream_t st = s2v_pick_stream(ctx, stream);
     return s2v_by_dtype(x_type, [&](auto type) {
@@ -169,11 +171,12 @@ int s2v_gemm_i8(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, int64_t k
                 int64_t ldb, const float* b_scale, const float* bias, int relu, int c_type, void* C, int64_t ldc)
 {
     S2V_ENTER(ctx);
-    const int rc = check_gemm(ctx, "gemm_i8", m, n, k, B, ldb, b_scale, c_type, C, ldc);
+    const int rc = check_gemm(ctx, "gemm_i8", m, n, k, B, ldb, b_scale, bias, c_type, C, ldc);
     if (rc != S2V_OK || m == 0 || n == 0) return rc;
     if (!a_scale || (k > 0 && !A)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "gemm_i8: NULL pointer");
     if (m > 1 && k > 0 && (lda < k || lda % 16 != 0)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "gemm_i8: lda below k or no multiple of 16");
     if (!s2v_aligned16(A)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "gemm_i8: 8-bit matrices must be 16-byte aligned");
+    if (!s2v_aligned4(a_scale)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "gemm_i8: misaligned scales");
     const s2v_gemm_i8_args g{m, n, k, lda, ldb, ldc, A, B, a_scale, b_scale, bias, relu, c_type, C};
     return s2v_launch_gemm_i8(ctx, s2v_pick_stream(ctx, stream), g, false);
 }
@@ -188,7 +191,7 @@ int s2v_linear_i8(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, int64_t
                   const float* w_scale, const float* bias, int relu, void* workspace, size_t workspace_bytes, int y_type, void* y, int64_t ldy)
 {
     S2V_ENTER(ctx);
-    const int rc = check_gemm(ctx, "linear_i8", m, n, k, W, ldw, w_scale, y_type, y, ldy);
+    const int rc = check_gemm(ctx, "linear_i8", m, n, k, W, ldw, w_scale, bias, y_type, y, ldy);
     if (rc != S2V_OK || m == 0 || n == 0) return rc;
     if (!s2v_dtype_ok(x_type)) return s2v_fail(ctx, S2V_ERR_INVALID_ARG, "linear_i8: unknown element type");
     if (!workspace || workspace_bytes < s2v_linear_i8_workspace_bytes(m, k)) return s2v_fail(ctx, S2V_ERR_WORKSPACE, "linear_i8: workspace too small");

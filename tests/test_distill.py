@@ -536,6 +536,22 @@ def test_refusal_of_rows_whose_bytes_pass_64_bits(gpu_ctx, cols):
     assert not f.any()
 
 
+@gpu
+def test_refusals_of_misaligned_lists_and_rows(gpu_ctx):
+    lib, h = gpu_ctx.lib, gpu_ctx.h
+    f, i = torch.zeros(4096, device="cuda"), torch.zeros(64, dtype=torch.int32, device="cuda")
+    p = f.data_ptr()
+    good = {"idx": i.data_ptr(), "lse": p, "weight": p, "loss": p, "stats": p}
+    for name in ("idx", "lse", "weight", "loss"):
+        for off in (1, 2, 3):
+            a = dict(good, **{name: good[name] + off})
+            assert lib.s2v_distill_topk(h, None, 4, 10, 0, p, 10, 3, a["idx"], 0, p, 3, a["lse"], 1.0, a["weight"], a["loss"], None, p + 4096, 10) == -1, name
+            if name != "loss":
+                assert lib.s2v_distill_topk_grad(h, None, 4, 10, 0, p, 10, 3, a["idx"], 0, p, 3, a["lse"], 1.0, a["weight"], a["stats"], p + 4096, 10) == -1, name
+    gpu_ctx.synchronize()
+    assert not f.any()
+
+
 # ---------------------------------------------------------------- together, as they are used
 @gpu
 def test_an_8_bit_student_of_the_readout(gpu_ctx):

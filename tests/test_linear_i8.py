@@ -433,3 +433,20 @@ def test_refusals(gpu_ctx):
     for got in (quant(rows=1, ldx=0, ldq=0), quant(rows=0, x=None), gemm(m=1, lda=0, ldc=0), gemm(m=0, a=None), gemm(n=0, w=None), layer(m=0, wsp=None, wsb=0)):
         assert got == 0    # leading dimensions of single rows are not read; empty calls do nothing
     gpu_ctx.synchronize()
+
+
+@gpu
+def test_refusals_of_misaligned_scales_and_biases(gpu_ctx):
+    lib, h = gpu_ctx.lib, gpu_ctx.h
+    f, i8 = torch.zeros(4096, device="cuda"), torch.zeros(8192, dtype=torch.int8, device="cuda")
+    p, b = f.data_ptr(), i8.data_ptr()
+    ws = gpu_ctx.linear_i8_workspace_bytes(4, 32)
+    for off in (1, 2, 3):
+        assert lib.s2v_quantize_rows_i8(h, None, 4, 32, 0, p, 32, b, 32, p + off) == -1
+        for sa, sb, bias in ((p + off, p, p), (p, p + off, p), (p, p, p + off)):
+            assert lib.s2v_gemm_i8(h, None, 4, 4, 32, b, 32, sa, b, 32, sb, bias, 0, 0, p, 4) == -1
+        for m in (1, 4):
+            for sw, bias in ((p + off, p), (p, p + off)):
+                assert lib.s2v_linear_i8(h, None, m, 4, 32, 0, p, 32, b, 32, sw, bias, 0, b, ws, 0, p, 4) == -1
+    gpu_ctx.synchronize()
+    assert not f.any() and not i8.any()
