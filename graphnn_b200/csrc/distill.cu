@@ -456,9 +456,10 @@ __global__ void __launch_bounds__(32 * DW_WARPS) distill_warp_kernel(const DtArg
 // memory; the others' are named by a byte per piece.  Their gradients are written over what the loops over the run wrote.  The first CTA's first
 // warp adds up the loss while the others write the gradient.
 constexpr int DC_CTAS = 8, DC_LISTERS = DT_TOP / 32;
-// Rows of up to DC_SHORT pieces: six CTAs of 128 threads an SM, all held (the steps of a row are a chain of latencies: 16384 rows of 9000 bf16 with their
-// gradients 168 us, with CTAs of 256 threads 311), lists of more than 128 entries apart.  Longer ones, where a CTA takes a row and there are more of them than
-// run at a time: six of 256 threads, nothing held (8192 rows of 32768 bf16 217 us; three that hold 4000 pieces 245).  Rows of more than DC_RUN pieces, and
+// Rows of up to DC_SHORT pieces: CTAs of 128 threads, all held; six an SM up to 1,950 pieces, beyond as many as its shared memory takes, four at DC_SHORT (the steps of
+// a row are a chain of latencies, which more CTAs cover better than more threads: 16384 rows of 9000 bf16 with their gradients 159 us, by six CTAs of 256 that hold
+// nothing 232, 8192 of 20000 159 and 162; the two meet at 2,800 pieces, 8192 of 23900 188 and 178).  Lists of more than 128 entries apart.  Longer ones,
+// where a CTA takes a row and there are more of them than run at a time: six of 256 threads, nothing held (8192 rows of 32768 bf16 217 us; three that hold 4000 pieces 245).  Rows of more than DC_RUN pieces, and
 // few rows: three of 256 that hold 4000 pieces (4096 rows of 131072 bf16 470 us; six that hold none 483, six of 128 562, two of 512 620 to 650, all
 // pieces held by a cluster of four 504).
 // The loss alone, of rows of more than DC_ONCE pieces and more of them than run at a time, needs a row once: nothing is held, eight CTAs of 128 threads or
