@@ -88,6 +88,14 @@ def load_library():
         "s2v_linear_i8": (i32, [vp, vp, i64, i64, i64, i32, vp, i64, vp, i64, vp, vp, i32, vp, C.c_size_t, i32, vp, i64]),
         "s2v_distill_topk": (i32, [vp, vp, i64, i64, i32, vp, i64, i32, vp, i32, vp, i64, vp, f32, vp, vp, vp, vp, i64]),
         "s2v_distill_topk_grad": (i32, [vp, vp, i64, i64, i32, vp, i64, i32, vp, i32, vp, i64, vp, f32, vp, vp, vp, i64]),
+        "s2v_layer_norm": (i32, [vp, vp, i64, i64, i32, vp, i64, vp, vp, f32, vp, i64, vp, vp, i64, vp]),
+        "s2v_layer_norm_grad_workspace_bytes": (C.c_size_t, [i64, i64]),
+        "s2v_layer_norm_grad": (i32, [vp, vp, i64, i64, i32, vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, C.c_size_t, vp, i64, vp, vp]),
+        "s2v_linear_i8_grad_workspace_bytes": (C.c_size_t, [i64, i64, i64, i32]),
+        "s2v_linear_i8_grad": (i32, [vp, vp, i64, i64, i64, i32, vp, i64, vp, i64, vp, vp, C.c_size_t, vp, i64, vp]),
+        "s2v_linear_cross_entropy_workspace_bytes": (C.c_size_t, [i64, i64, i64, i32, i32]),
+        "s2v_linear_cross_entropy": (i32, [vp, vp, i64, i64, i64, i32, vp, i64, vp, i64, vp, vp, vp, C.c_size_t, vp, vp]),
+        "s2v_linear_cross_entropy_grad": (i32, [vp, vp, i64, i64, i64, i32, vp, i64, vp, i64, vp, vp, vp, vp, C.c_size_t, vp, i64, vp, i64]),
         "s2v_segment_sum_f32": (i32, [vp, vp, i64, i32, vp, vp, vp]),
         "s2v_segment_pool_f32": (i32, [vp, vp, i64, i32, vp, vp, i32, vp]),
         "s2v_readout_f32": (i32, [vp, vp, i64, i32, i32, i32, vp, vp, vp, vp, vp, vp]),
@@ -224,11 +232,40 @@ def _vector(name: str, t, device: int, length: int):
         _refuse(f"{name} is no contiguous fp32 vector of {length} on cuda:{device}, but {tuple(t.shape)} of {t.dtype} on {t.device}")
 
 
-def _sizes(name: str, t):
-    """Rows, columns and element type of a matrix that the others go by."""
+def _dtypes():
     if not _DTYPES:
         import torch
         _DTYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    return _DTYPES
+
+
+def _optional(name: str, t, device: int, length: int):
+    """The address of an fp32 vector that may be None."""
+    if t is None:
+        return None
+    _vector(name, t, device, length)
+    return t.data_ptr()
+
+
+def _pairs(name: str, t, device: int, rows: int):
+    """The address of a contiguous fp32 [rows x 2] matrix that may be None."""
+    if t is None:
+        return None
+    import torch
+    if _matrix(name, t, device, rows, 2, torch.float32) != 2 and rows > 1:
+        _refuse(f"{name} is not contiguous")
+    return t.data_ptr()
+
+
+def _workspace(t, device: int):
+    if t.get_device() != device or not t.is_contiguous():
+        _refuse("workspace is not contiguous or on another device")
+    return t.data_ptr(), t.nbytes
+
+
+def _sizes(name: str, t):
+    """Rows, columns and element type of a matrix that the others go by."""
+    _dtypes()
     if len(t.shape) != 2 or t.dtype not in _DTYPES:
         _refuse(f"{name} is no matrix of fp32, fp16 or bf16 numbers, but {tuple(t.shape)} of {t.dtype}")
     return (*t.shape, t.dtype)
@@ -457,6 +494,99 @@ class Context:
         self.call("s2v_linear_i8", stream, m, n, k, _DTYPES[xtype], x.data_ptr(), ldx, W.data_ptr(), ldw, w_scale.data_ptr(), bias, 1 if relu else 0,
                   workspace.data_ptr(), workspace.nbytes, _DTYPES[ytype], y.data_ptr(), ldy)
         return y
+
+    def linear_i8_grad_workspace_bytes(self, m: int, n: int, k: int, dtype) -> int:
+        return int(self.lib.s2v_linear_i8_grad_workspace_bytes(m, n, k, _dtypes()[dtype]))
+
+    def linear_i8_grad(self, dy, q, q_scale, dW, workspace, dbias=None, stream=None):
+        """s2v_linear_i8_grad: dW = dy^T (q_scale[:, None] * q), dbias = column sums of dy, for a layer whose input was kept as 8-bit rows."""
+        import torch
+        (m, n, dtype), k, dev = _sizes("dy", dy), q.shape[-1], self.device
+        lddy, ldq, lddw = _matrix("dy", dy, dev, m, n, dtype), _matrix("q", q, dev, m, k, torch.int8), _matrix("dW", dW, dev, n, k, dtype)
+        _vector("q_scale", q_scale, dev, m)
+        dbias = _optional("dbias", dbias, dev, n)
+        self.call("s2v_linear_i8_grad", stream, m, n, k, _DTYPES[dtype], dy.data_ptr(), lddy, q.data_ptr(), ldq, q_scale.data_ptr(), *_workspace(workspace, dev),
+                  dW.data_ptr(), lddw, dbias)
+        return dW
+
+    # -- layer norm
+    def layer_norm(self, x, y, weight=None, bias=None, eps=1e-5, stats=None, q=None, q_scale=None, stream=None):
+        """s2v_layer_norm: y (may be x) = the normalised rows of x, times weight, plus bias; kept for the gradient where given: stats, float [rows x 2], and
+        the rows of x in 8 bits, q and q_scale, as quantize_rows_i8 gives them."""
+        import torch
+        (rows, cols, dtype), dev = _sizes("x", x), self.device
+        ldx, ldy = _matrix("x", x, dev, rows, cols, dtype), _matrix("y", y, dev, rows, cols, dtype)
+        ldq = 0
+        if (q is None) != (q_scale is None):
+            _refuse("q and q_scale go together")
+        if q is not None:
+            ldq = _matrix("q", q, dev, rows, cols, torch.int8)
+            q = q.data_ptr()
+        weight, bias, q_scale = _optional("weight", weight, dev, cols), _optional("bias", bias, dev, cols), _optional("q_scale", q_scale, dev, rows)
+        self.call("s2v_layer_norm", stream, rows, cols, _DTYPES[dtype], x.data_ptr(), ldx, weight, bias, eps, y.data_ptr(), ldy, _pairs("stats", stats, dev, rows), q, ldq,
+                  q_scale)
+        return y
+
+    def layer_norm_grad_workspace_bytes(self, rows: int, cols: int) -> int:
+        return int(self.lib.s2v_layer_norm_grad_workspace_bytes(rows, cols))
+
+    def layer_norm_grad(self, dy, stats, dx, workspace=None, x=None, q=None, q_scale=None, weight=None, dweight=None, dbias=None, stream=None):
+        """s2v_layer_norm_grad: dx (may be dy), dweight and dbias from x, or from the 8-bit rows q and q_scale, and the stats that layer_norm kept; the workspace is
+        needed for dweight and dbias alone."""
+        import torch
+        (rows, cols, dtype), dev = _sizes("dy", dy), self.device
+        if (x is None) == (q is None) or (q is None) != (q_scale is None):
+            _refuse("takes x, or q and q_scale")
+        lddy, lddx = _matrix("dy", dy, dev, rows, cols, dtype), _matrix("dx", dx, dev, rows, cols, dtype)
+        ldx = ldq = 0
+        if x is not None:
+            ldx = _matrix("x", x, dev, rows, cols, dtype)
+            x = x.data_ptr()
+        else:
+            ldq = _matrix("q", q, dev, rows, cols, torch.int8)
+            q = q.data_ptr()
+            q_scale = _optional("q_scale", q_scale, dev, rows)
+        if stats is None:
+            _refuse("stats is None")
+        space = (None, 0) if workspace is None else _workspace(workspace, dev)
+        weight, dweight, dbias = _optional("weight", weight, dev, cols), _optional("dweight", dweight, dev, cols), _optional("dbias", dbias, dev, cols)
+        self.call("s2v_layer_norm_grad", stream, rows, cols, _DTYPES[dtype], dy.data_ptr(), lddy, x, ldx, q, ldq, q_scale, _pairs("stats", stats, dev, rows), weight, *space,
+                  dx.data_ptr(), lddx, dweight, dbias)
+        return dx
+
+    # -- the loss over a vocabulary, from embeddings
+    def linear_cross_entropy_workspace_bytes(self, rows: int, vocab: int, k: int, dtype, grad: bool = True) -> int:
+        return int(self.lib.s2v_linear_cross_entropy_workspace_bytes(rows, vocab, k, _dtypes()[dtype], 1 if grad else 0))
+
+    def _cross_entropy_args(self, x, W, target, row_weight):
+        import torch
+        (rows, k, dtype), (vocab, _, _), dev = _sizes("x", x), _sizes("W", W), self.device
+        ldx, ldw = _matrix("x", x, dev, rows, k, dtype), _matrix("W", W, dev, vocab, k, dtype)
+        if not (target.dtype is torch.int32 and target.get_device() == dev and target.shape == (rows,) and target.is_contiguous()):
+            _refuse(f"target is no contiguous int32 vector of {rows} on cuda:{dev}, but {tuple(target.shape)} of {target.dtype} on {target.device}")
+        return (rows, vocab, k, _DTYPES[dtype], x.data_ptr(), ldx, W.data_ptr(), ldw, target.data_ptr(), _optional("row_weight", row_weight, dev, rows))
+
+    def linear_cross_entropy(self, x, W, target, loss, workspace, row_weight=None, stats=None, stream=None):
+        """s2v_linear_cross_entropy: loss[i] = row_weight[i] * (log-sum-exp of x[i] W^T - the logit of class target[i]); stats: float [rows x 2] kept for
+        linear_cross_entropy_grad."""
+        args = self._cross_entropy_args(x, W, target, row_weight)
+        _vector("loss", loss, self.device, x.shape[0])
+        self.call("s2v_linear_cross_entropy", stream, *args, *_workspace(workspace, self.device), loss.data_ptr(), _pairs("stats", stats, self.device, x.shape[0]))
+        return loss
+
+    def linear_cross_entropy_grad(self, x, W, target, stats, workspace, dx=None, dW=None, row_weight=None, stream=None):
+        """s2v_linear_cross_entropy_grad: the gradients dx and dW (either may be None) of sum(loss) from the stats of linear_cross_entropy."""
+        args, dev = self._cross_entropy_args(x, W, target, row_weight), self.device
+        if stats is None:
+            _refuse("stats is None")
+        lddx = lddw = 0
+        if dx is not None:
+            lddx = _matrix("dx", dx, dev, *x.shape, x.dtype)
+            dx = dx.data_ptr()
+        if dW is not None:
+            lddw = _matrix("dW", dW, dev, *W.shape, x.dtype)
+            dW = dW.data_ptr()
+        self.call("s2v_linear_cross_entropy_grad", stream, *args, _pairs("stats", stats, dev, x.shape[0]), *_workspace(workspace, dev), dx, lddx, dW, lddw)
 
     # -- distillation from a teacher's top logits
     def _distill_args(self, z, idx, t, temperature, t_lse, row_weight, loss, stats, dz):

@@ -1,0 +1,541 @@
+// Layer norm of rows, its gradient, and the 8-bit rows that a training step keeps between the two instead of its input.
+//
+// Forward: a row by 8 lanes, a warp or a CTA, held in registers between its moments and its outputs.  Deviations are summed around each thread's own mean and
+// the moments of threads joined by  M2 = M2a + M2b + (mb - ma)^2 na nb / (na + nb),  so that one exchange among a row's threads gives both moments without the
+// cancellation of E x^2 - (E x)^2.
+// Gradient: the same places of a row in every turn of a thread, which so sums its columns of the weight's and the bias's gradient in registers over all
+// the rows that it takes; a CTA leaves one line of sums, and a second kernel adds the lines in their order.
+#include "quantize.cuh"
+
+namespace
+{
+
+constexpr int LN_CTA = 256;
+constexpr int LN_MAX_LINES = 1024;   // CTAs of the gradient, each with a line of column sums in the workspace
+
+// Pieces of a row: 16 bytes where every row lies on a 16-byte boundary, else single elements.
+template <typename T, bool VEC> struct ln_piece {
+    static constexpr int N = VEC ? 16 / (int)sizeof(T) : 1;
+    using raw = typename std::conditional<VEC, uint4, T>::type;
+    static __device__ __forceinline__ raw load(const T* row, int64_t p) { return __ldcs(reinterpret_cast<const raw*>(row) + p); }
+    static __device__ __forceinline__ raw load_again(const T* row, int64_t p) { return reinterpret_cast<const raw*>(row)[p]; }
+    static __device__ __forceinline__ void unpack(const raw& v, float* x)
+    {
+        if constexpr (VEC) unpack_piece(v, x, T());
+        else x[0] = to_f32(v);
+    }
+    static __device__ __forceinline__ void store(T* row, int64_t p, const float* y)
+    {
+        if constexpr (VEC) reinterpret_cast<uint4*>(row)[p] = pack_piece(y, T());
+        else row[p] = from_f32<T>(y[0]);
+    }
+    static __device__ __forceinline__ void columns(const float* v, int64_t p, float otherwise, float* w)   // of a vector of fp32, NULL: one value everywhere
+    {
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = otherwise;
+        if (!v) return;
+        if constexpr (VEC) {
+            if ((reinterpret_cast<uintptr_t>(v) & 15) == 0) {
+#pragma unroll
+                for (int e = 0; e < N; e += 4) {
+                    const float4 f = __ldg(reinterpret_cast<const float4*>(v + p * N + e));
+                    w[e] = f.x, w[e + 1] = f.y, w[e + 2] = f.z, w[e + 3] = f.w;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) w[e] = __ldg(v + p * N + e);
+            }
+        } else w[0] = __ldg(v + p);
+    }
+    static __device__ __forceinline__ uint32_t largest(const raw& v)
+    {
+        if constexpr (VEC) return q_largest<T>(v);
+        else return __float_as_uint(to_f32(v)) & 0x7fffffffu;
+    }
+    static __device__ __forceinline__ void quantize(int8_t* row, int64_t p, bool whole, const raw& v, const q_row& k)
+    {
+        if constexpr (VEC) q_store<T>(row + p * N, whole, v, k);
+        else row[p] = (int8_t)k.integer(to_f32(v));
+    }
+    // 8-bit numbers of a piece
+    using raw8 = typename std::conditional<VEC, typename std::conditional<N == 8, uint2, uint32_t>::type, int8_t>::type;
+    static __device__ __forceinline__ raw8 load8(const int8_t* row, int64_t p) { return __ldcs(reinterpret_cast<const raw8*>(row) + p); }
+    static __device__ __forceinline__ void unpack8(const raw8& v, float* x)
+    {
+        if constexpr (!VEC) x[0] = (float)v;
+        else {
+            uint32_t w[N / 4];
+            if constexpr (N == 8) w[0] = v.x, w[1] = v.y;
+            else w[0] = v;
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = (float)(int8_t)(w[e / 4] >> (8 * (e & 3)));
+        }
+    }
+};
+
+// n numbers with their mean and the sum of their squared deviations from it
+struct ln_moments {
+    float n, mean, m2;
+    __device__ __forceinline__ void join(float nb, float mb, float m2b)
+    {
+        const float sum = n + nb;
+        if (nb == 0.0f) return;
+        const float share = nb / sum, d = mb - mean;
+        mean = n == 0.0f ? mb : fmaf(d, share, mean);
+        m2 = m2 + m2b + (n == 0.0f ? 0.0f : d * d * (n * share));
+        n = sum;
+    }
+    template <int LANES> __device__ __forceinline__ void join_lanes()
+    {
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) {
+            // both sides compute the same numbers: the lower lane's come first
+            const float nb = __shfl_xor_sync(0xffffffffu, n, o), mb = __shfl_xor_sync(0xffffffffu, mean, o), qb = __shfl_xor_sync(0xffffffffu, m2, o);
+            const bool second = threadIdx.x & o;
+            ln_moments a{second ? nb : n, second ? mb : mean, second ? qb : m2};
+            a.join(second ? n : nb, second ? mean : mb, second ? m2 : qb);
+            *this = a;
+        }
+    }
+};
+
+// THREADS threads a row (8, 32 or a CTA of THREADS), NV pieces of each in registers; a longer row's others (CTAs alone) are read again.
+template <typename T, bool VEC, int NV, int THREADS>
+__global__ void __launch_bounds__(THREADS < LN_CTA ? LN_CTA : THREADS)
+    layer_norm_kernel(int64_t rows, int64_t cols, const T* x, int64_t ldx, const float* __restrict__ weight, const float* __restrict__ bias, float eps, T* y, int64_t ldy,
+                      float2* __restrict__ stats, int8_t* __restrict__ q, int64_t ldq, float* __restrict__ q_scale)   // (y may be x)
+{
+    using P = ln_piece<T, VEC>;
+    constexpr int N = P::N, CTA = THREADS < LN_CTA ? LN_CTA : THREADS, WARPS = THREADS / 32, GROUPS = CTA / THREADS;
+    __shared__ float4 part[WARPS > 1 ? 2 * WARPS : 1];
+    const int at = threadIdx.x % THREADS;
+    const int64_t pieces = cols / N;
+    int turn = 0;
+    for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < rows; first += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
+        // (groups behind the last row take it too, but leave nothing: all lanes of a warp exchange)
+        const int64_t own = first + threadIdx.x / THREADS, r = min(own, rows - 1);
+        const bool mine = own < rows;
+        const T* const xr = x + r * ldx;
+        typename P::raw v[NV];
+        float sum = 0.0f;
+        int count = 0;
+        uint32_t a = 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * THREADS + at < pieces) v[j] = P::load_again(xr, j * THREADS + at);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * THREADS + at < pieces) {
+                float f[N];
+                P::unpack(v[j], f);
+#pragma unroll
+                for (int e = 0; e < N; ++e) sum += f[e];
+                count += N;
+            }
+        if constexpr (WARPS > 1)
+            for (int64_t p = NV * THREADS + at; p < pieces; p += THREADS) {
+                float f[N];
+                P::unpack(P::load_again(xr, p), f);
+#pragma unroll
+                for (int e = 0; e < N; ++e) sum += f[e];
+                count += N;
+            }
+        ln_moments m{(float)count, count ? sum / (float)count : 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * THREADS + at < pieces) {
+                float f[N];
+                P::unpack(v[j], f);
+#pragma unroll
+                for (int e = 0; e < N; ++e) m.m2 = fmaf(f[e] - m.mean, f[e] - m.mean, m.m2);
+                if (q) a = max(a, P::largest(v[j]));
+            }
+        if constexpr (WARPS > 1)
+            for (int64_t p = NV * THREADS + at; p < pieces; p += THREADS) {
+                const typename P::raw w = P::load_again(xr, p);
+                float f[N];
+                P::unpack(w, f);
+#pragma unroll
+                for (int e = 0; e < N; ++e) m.m2 = fmaf(f[e] - m.mean, f[e] - m.mean, m.m2);
+                if (q) a = max(a, P::largest(w));
+            }
+        m.template join_lanes<(THREADS < 32 ? THREADS : 32)>();
+        if (q) {
+            if constexpr (THREADS < 32) {
+#pragma unroll
+                for (int o = THREADS / 2; o; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+            } else a = __reduce_max_sync(0xffffffffu, a);
+        }
+        if constexpr (WARPS > 1) {   // (two turns' places: one barrier a row)
+            if ((at & 31) == 0) part[turn * WARPS + (at >> 5)] = make_float4(m.n, m.mean, m.m2, __uint_as_float(a));
+            __syncthreads();
+            m = ln_moments{0.0f, 0.0f, 0.0f};
+            a = 0;
+#pragma unroll
+            for (int i = 0; i < WARPS; ++i) {
+                const float4 o = part[turn * WARPS + i];
+                m.join(o.x, o.y, o.z);
+                a = max(a, __float_as_uint(o.w));
+            }
+        }
+        const float rstd = 1.0f / sqrtf(m.m2 / m.n + eps);
+        if (mine && at == 0 && stats) stats[r] = make_float2(m.mean, rstd);
+        if (!mine) continue;
+        T* const yr = y + r * ldy;
+        const q_row k(a);
+        int8_t* const qr = q + r * ldq;
+        const bool whole = VEC && (reinterpret_cast<uintptr_t>(qr) & (N - 1)) == 0;
+        const auto leave = [&](int64_t p, const typename P::raw& w) {
+            float f[N], g[N], b[N];
+            P::unpack(w, f);
+            P::columns(weight, p, 1.0f, g);
+            P::columns(bias, p, 0.0f, b);
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[e] = fmaf((f[e] - m.mean) * rstd, g[e], b[e]);
+            if (q) P::quantize(qr, p, whole, w, k);
+            P::store(yr, p, f);
+        };
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * THREADS + at < pieces) leave(j * THREADS + at, v[j]);
+        if constexpr (WARPS > 1)
+            for (int64_t p = NV * THREADS + at; p < pieces; p += THREADS) leave(p, P::load_again(xr, p));
+        if (q && at == 0) q_scale[r] = k.scale;
+    }
+}
+
+// What the gradient takes its normalised rows from: x, or 8-bit rows with scales.
+struct LnGrad {
+    int64_t rows, cols, lddy, ldx, lddx;
+    const void* dy;
+    const void* x;          // or
+    const int8_t* q;
+    const float* q_scale;
+    const float2* stats;
+    const float* weight;
+    void* dx;
+    float* lines;           // [CTAs][2][cols]: sums of dy xh and of dy
+    int columns;            // whether these are wanted
+};
+
+template <typename T, bool VEC, int NV, int THREADS, bool FROM8>
+__global__ void __launch_bounds__(THREADS < LN_CTA ? LN_CTA : THREADS) layer_norm_grad_kernel(const LnGrad a)
+{
+    using P = ln_piece<T, VEC>;
+    constexpr int N = P::N, CTA = THREADS < LN_CTA ? LN_CTA : THREADS, WARPS = THREADS / 32, GROUPS = CTA / THREADS;
+    __shared__ float2 part[WARPS > 1 ? 2 * WARPS : 1];
+    extern __shared__ float ln_lines[];   // GROUPS > 1: a line of sums at a time
+    const int at = threadIdx.x % THREADS;
+    const int pieces = (int)(a.cols / N);
+    float sum_w[NV * N] = {}, sum_b[NV * N] = {};
+    int turn = 0;
+    for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < a.rows; first += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
+        const int64_t own = first + threadIdx.x / THREADS, r = min(own, a.rows - 1);
+        const bool mine = own < a.rows;
+        const T* const dyr = static_cast<const T*>(a.dy) + r * a.lddy;
+        const float2 st = a.stats[r];
+        const float s = FROM8 ? a.q_scale[r] : 1.0f;
+        typename P::raw dv[NV];
+        typename std::conditional<FROM8, typename P::raw8, typename P::raw>::type xv[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * THREADS + at < pieces) {
+                dv[j] = P::load(dyr, j * THREADS + at);
+                if constexpr (FROM8) xv[j] = P::load8(a.q + r * a.ldx, j * THREADS + at);
+                else xv[j] = P::load(static_cast<const T*>(a.x) + r * a.ldx, j * THREADS + at);
+            }
+        const auto normalised = [&](int j, float* h) {
+            if constexpr (FROM8) P::unpack8(xv[j], h);
+            else P::unpack(xv[j], h);
+#pragma unroll
+            for (int e = 0; e < N; ++e) h[e] = FROM8 ? fmaf(h[e], s, -st.x) * st.y : (h[e] - st.x) * st.y;
+        };
+        float g0 = 0.0f, g1 = 0.0f;   // sums of g = dy w and of g xh
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * THREADS + at < pieces) {
+                float d[N], h[N], w[N];
+                P::unpack(dv[j], d);
+                normalised(j, h);
+                P::columns(a.weight, j * THREADS + at, 1.0f, w);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const float g = d[e] * w[e];
+                    g0 += g;
+                    g1 = fmaf(g, h[e], g1);
+                    if (mine) sum_w[j * N + e] = fmaf(d[e], h[e], sum_w[j * N + e]), sum_b[j * N + e] += d[e];
+                }
+            }
+#pragma unroll
+        for (int o = (THREADS < 32 ? THREADS : 32) / 2; o; o >>= 1) g0 += __shfl_xor_sync(0xffffffffu, g0, o), g1 += __shfl_xor_sync(0xffffffffu, g1, o);
+        if constexpr (WARPS > 1) {
+            if ((at & 31) == 0) part[turn * WARPS + (at >> 5)] = make_float2(g0, g1);
+            __syncthreads();
+            g0 = g1 = 0.0f;
+#pragma unroll
+            for (int i = 0; i < WARPS; ++i) g0 += part[turn * WARPS + i].x, g1 += part[turn * WARPS + i].y;
+        }
+        if (!mine) continue;
+        const float inv = 1.0f / (float)a.cols, m0 = g0 * inv, m1 = g1 * inv;
+        T* const dxr = static_cast<T*>(a.dx) + r * a.lddx;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * THREADS + at < pieces) {
+                float d[N], h[N], w[N];
+                P::unpack(dv[j], d);
+                normalised(j, h);
+                P::columns(a.weight, j * THREADS + at, 1.0f, w);
+#pragma unroll
+                for (int e = 0; e < N; ++e) d[e] = st.y * (fmaf(d[e], w[e], -m0) - h[e] * m1);
+                P::store(dxr, j * THREADS + at, d);
+            }
+    }
+    if (!a.columns) return;
+    float* const line = a.lines + (int64_t)blockIdx.x * 2 * a.cols;
+    if constexpr (GROUPS == 1) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * THREADS + at < pieces)
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    line[(int64_t)(j * THREADS + at) * N + e] = sum_w[j * N + e];
+                    line[a.cols + (int64_t)(j * THREADS + at) * N + e] = sum_b[j * N + e];
+                }
+    } else {   // groups of a warp by shuffles, warps through shared memory
+#pragma unroll
+        for (int i = 0; i < NV * N; ++i)
+#pragma unroll
+            for (int o = THREADS; o < 32; o <<= 1) sum_w[i] += __shfl_xor_sync(0xffffffffu, sum_w[i], o), sum_b[i] += __shfl_xor_sync(0xffffffffu, sum_b[i], o);
+        constexpr int LINE = NV * N * THREADS, CW = CTA / 32;
+        for (int half = 0; half < 2; ++half) {
+            if ((threadIdx.x & 31) < THREADS) {
+#pragma unroll
+                for (int i = 0; i < NV * N; ++i) ln_lines[(threadIdx.x >> 5) * LINE + (i / N * THREADS + at) * N + i % N] = half ? sum_b[i] : sum_w[i];
+            }
+            __syncthreads();
+            for (int c = threadIdx.x; c < a.cols; c += CTA) {
+                float t = 0.0f;
+                for (int w = 0; w < CW; ++w) t += ln_lines[w * LINE + c];
+                line[half * a.cols + c] = t;
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// Rows longer than a CTA's registers: read twice, and a second kernel for the columns' sums.
+template <typename T, bool FROM8> __global__ void __launch_bounds__(512) layer_norm_grad_long_kernel(const LnGrad a)
+{
+    __shared__ float2 part[2 * 16];
+    int turn = 0;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x, turn ^= 1) {
+        const T* const dyr = static_cast<const T*>(a.dy) + r * a.lddy;
+        T* const dxr = static_cast<T*>(a.dx) + r * a.lddx;
+        const float2 st = a.stats[r];
+        const float s = FROM8 ? a.q_scale[r] : 1.0f;
+        const auto normalised = [&](int64_t c) { return FROM8 ? fmaf((float)a.q[r * a.ldx + c], s, -st.x) * st.y : (to_f32(static_cast<const T*>(a.x)[r * a.ldx + c]) - st.x) * st.y; };
+        float g0 = 0.0f, g1 = 0.0f;
+        for (int64_t c = threadIdx.x; c < a.cols; c += 512) {
+            const float g = to_f32(dyr[c]) * (a.weight ? __ldg(a.weight + c) : 1.0f);
+            g0 += g;
+            g1 = fmaf(g, normalised(c), g1);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) g0 += __shfl_xor_sync(0xffffffffu, g0, o), g1 += __shfl_xor_sync(0xffffffffu, g1, o);
+        if ((threadIdx.x & 31) == 0) part[turn * 16 + (threadIdx.x >> 5)] = make_float2(g0, g1);
+        __syncthreads();
+        g0 = g1 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) g0 += part[turn * 16 + i].x, g1 += part[turn * 16 + i].y;
+        const float m0 = g0 / (float)a.cols, m1 = g1 / (float)a.cols;
+        for (int64_t c = threadIdx.x; c < a.cols; c += 512)
+            dxr[c] = from_f32<T>(st.y * (fmaf(to_f32(dyr[c]), a.weight ? __ldg(a.weight + c) : 1.0f, -m0) - normalised(c) * m1));
+    }
+}
+// a column a thread, a share of the rows a CTA
+template <typename T, bool FROM8> __global__ void __launch_bounds__(LN_CTA) layer_norm_columns_kernel(const LnGrad a, int64_t share)
+{
+    const int64_t c = (int64_t)blockIdx.x * LN_CTA + threadIdx.x, from = blockIdx.y * share, to = min(a.rows, from + share);
+    if (c >= a.cols) return;
+    float w = 0.0f, b = 0.0f;
+    for (int64_t r = from; r < to; ++r) {
+        const float d = to_f32(static_cast<const T*>(a.dy)[r * a.lddy + c]);
+        const float2 st = a.stats[r];
+        const float h = FROM8 ? fmaf((float)a.q[r * a.ldx + c], a.q_scale[r], -st.x) * st.y : (to_f32(static_cast<const T*>(a.x)[r * a.ldx + c]) - st.x) * st.y;
+        w = fmaf(d, h, w);
+        b += d;
+    }
+    float* const line = a.lines + (int64_t)blockIdx.y * 2 * a.cols;
+    line[c] = w, line[a.cols + c] = b;
+}
+// the lines of the gradient's CTAs, added in their order by 8 threads a column
+__global__ void __launch_bounds__(LN_CTA) layer_norm_lines_kernel(int lines, int64_t cols, const float* __restrict__ from, float* __restrict__ dweight, float* __restrict__ dbias)
+{
+    __shared__ float part[8][33];
+    const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+    const int g = threadIdx.x >> 5;
+    float t = 0.0f;
+    if (c < 2 * cols)
+        for (int l = g; l < lines; l += 8) t += from[(int64_t)l * 2 * cols + c];
+    part[g][threadIdx.x & 31] = t;
+    __syncthreads();
+    if (g || c >= 2 * cols) return;
+    t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t += part[i][threadIdx.x & 31];
+    if (c < cols) {
+        if (dweight) dweight[c] = t;
+    } else if (dbias) dbias[c - cols] = t;
+}
+
+template <typename T, bool VEC>
+int ln_launch(s2v_ctx* ctx, cudaStream_t st, int64_t rows, int64_t cols, const T* x, int64_t ldx, const float* weight, const float* bias, float eps, T* y, int64_t ldy,
+              float2* stats, int8_t* q, int64_t ldq, float* q_scale)
+{
+    const int64_t pieces = cols / ln_piece<T, VEC>::N;
+    const auto go = [&](auto kernel, int threads) {
+        const int per = threads < LN_CTA ? LN_CTA / threads : 1;
+        const int64_t blocks = (rows + per - 1) / per, cap = (int64_t)1 << 20;
+        kernel<<<(unsigned)(blocks < cap ? blocks : cap), threads < LN_CTA ? LN_CTA : threads, 0, st>>>(rows, cols, x, ldx, weight, bias, eps, y, ldy, stats, q, ldq, q_scale);
+        S2V_CHECK_LAUNCH(ctx, "layer_norm_kernel");
+        return (int)S2V_OK;
+    };
+    if (pieces <= 8) return go(layer_norm_kernel<T, VEC, 1, 8>, 8);
+    if (pieces <= 32) return go(layer_norm_kernel<T, VEC, 4, 8>, 8);
+    if (pieces <= 128) return go(layer_norm_kernel<T, VEC, 4, 32>, 32);
+    if (pieces <= 512) return go(layer_norm_kernel<T, VEC, 2, 256>, 256);
+    if (pieces <= 1024) return go(layer_norm_kernel<T, VEC, 4, 256>, 256);
+    return go(layer_norm_kernel<T, VEC, 8, 256>, 256);
+}
+
+int ln_ctas(const s2v_ctx* ctx, int64_t rows, int per)
+{
+    const int64_t turns = (rows + per - 1) / per, most = 4 * (int64_t)ctx->sm_count;
+    return (int)(turns < most ? turns : most < LN_MAX_LINES ? most : LN_MAX_LINES);
+}
+
+template <typename T, bool FROM8> int ln_grad_launch(s2v_ctx* ctx, cudaStream_t st, const LnGrad& a, bool vec, float* dweight, float* dbias)
+{
+    int lines = 0;
+    const auto go = [&](auto kernel, int threads, int line) {
+        const int per = threads < LN_CTA ? LN_CTA / threads : 1;
+        lines = ln_ctas(ctx, a.rows, per);
+        kernel<<<lines, threads < LN_CTA ? LN_CTA : threads, threads < LN_CTA ? LN_CTA / 32 * line * sizeof(float) : 0, st>>>(a);
+        S2V_CHECK_LAUNCH(ctx, "layer_norm_grad_kernel");
+        return (int)S2V_OK;
+    };
+    const auto by_size = [&](auto vector) {
+        constexpr bool VEC = decltype(vector)::value;
+        constexpr int N = ln_piece<T, VEC>::N;
+        const int64_t pieces = a.cols / N;
+        if (pieces <= 8) return go(layer_norm_grad_kernel<T, VEC, 1, 8, FROM8>, 8, 8 * N);
+        if (pieces <= 32) return go(layer_norm_grad_kernel<T, VEC, VEC ? 1 : 4, VEC ? 32 : 8, FROM8>, VEC ? 32 : 8, 32 * N);
+        if (pieces <= 128) return go(layer_norm_grad_kernel<T, VEC, 4, 32, FROM8>, 32, 128 * N);
+        if (pieces <= 512) return go(layer_norm_grad_kernel<T, VEC, 2, 256, FROM8>, 256, 0);
+        if (pieces <= 1024) return go(layer_norm_grad_kernel<T, VEC, 2, 512, FROM8>, 512, 0);
+        if (pieces <= 2048) return go(layer_norm_grad_kernel<T, VEC, 4, 512, FROM8>, 512, 0);
+        if constexpr (N < 8) {
+            if (pieces <= 4096) return go(layer_norm_grad_kernel<T, VEC, 8, 512, FROM8>, 512, 0);
+        }
+        if (a.columns) {   // (first: dx may lie over dy)
+            const int64_t blocks = (a.cols + LN_CTA - 1) / LN_CTA;
+            if (blocks > INT32_MAX) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, "layer_norm_grad: too many columns");
+            lines = ln_ctas(ctx, a.rows, 16);
+            const int64_t share = (a.rows + lines - 1) / lines;
+            lines = (int)((a.rows + share - 1) / share);
+            layer_norm_columns_kernel<T, FROM8><<<dim3((unsigned)blocks, lines), LN_CTA, 0, st>>>(a, share);
+            S2V_CHECK_LAUNCH(ctx, "layer_norm_columns_kernel");
+        }
+        const int64_t cap = (int64_t)1 << 20;
+        layer_norm_grad_long_kernel<T, FROM8><<<(unsigned)(a.rows < cap ? a.rows : cap), 512, 0, st>>>(a);
+        S2V_CHECK_LAUNCH(ctx, "layer_norm_grad_long_kernel");
+        return (int)S2V_OK;
+    };
+    const int rc = vec ? by_size(std::true_type()) : by_size(std::false_type());
+    if (rc != S2V_OK || !a.columns) return rc;
+    layer_norm_lines_kernel<<<(unsigned)((2 * a.cols + 31) / 32), LN_CTA, 0, st>>>(lines, a.cols, a.lines, dweight, dbias);
+    S2V_CHECK_LAUNCH(ctx, "layer_norm_lines_kernel");
+    return S2V_OK;
+}
+
+// Whether every row of a matrix lies on a boundary of `bytes`.
+bool rows_aligned(const void* p, int64_t rows, int64_t ld, int64_t es, int64_t bytes)
+{
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && (rows <= 1 || ld * es % bytes == 0);
+}
+
+}  // namespace
+
+extern "C" {
+
+int s2v_layer_norm(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t cols, int x_type, const void* x, int64_t ldx, const float* weight, const float* bias, float eps,
+                   void* y, int64_t ldy, float* stats, int8_t* q, int64_t ldq, float* q_scale)
+{
+    S2V_ENTER(ctx);
+    const auto bad = [&](int status, const char* what) { return s2v_fail(ctx, status, std::string("layer_norm: ") + what); };
+    if (rows < 0 || cols < 1) return bad(S2V_ERR_INVALID_ARG, "negative size or no columns");
+    if (!s2v_dtype_ok(x_type)) return bad(S2V_ERR_INVALID_ARG, "unknown element type");
+    if (!(eps >= 0.0f) || eps > 1e30f) return bad(S2V_ERR_INVALID_ARG, "eps outside 0 to 1e30");
+    if (rows == 0) return S2V_OK;
+    if (cols > INT32_MAX) return bad(S2V_ERR_UNSUPPORTED, "more than 2^31 - 1 columns");
+    if (!x || !y || (q == nullptr) != (q_scale == nullptr)) return bad(S2V_ERR_INVALID_ARG, "NULL pointer");
+    if (rows > 1 && (ldx < cols || ldy < cols || (q && ldq < cols))) return bad(S2V_ERR_INVALID_ARG, "leading dimension below the number of columns");
+    if (x == y && rows > 1 && ldx != ldy) return bad(S2V_ERR_INVALID_ARG, "in place with another leading dimension");
+    const int64_t es = (int64_t)s2v_dtype_bytes(x_type);
+    if (reinterpret_cast<uintptr_t>(x) % es || reinterpret_cast<uintptr_t>(y) % es || reinterpret_cast<uintptr_t>(stats) % 8 || !s2v_aligned4(weight, bias, q_scale))
+        return bad(S2V_ERR_INVALID_ARG, "misaligned pointer");
+    cudaStream_t st = s2v_pick_stream(ctx, stream);
+    const bool vec = cols % (16 / es) == 0 && rows_aligned(x, rows, ldx, es, 16) && rows_aligned(y, rows, ldy, es, 16);
+    return s2v_by_dtype(x_type, [&](auto type) {
+        using T = decltype(type);
+        const auto go = [&](auto vector) {
+            return ln_launch<T, decltype(vector)::value>(ctx, st, rows, cols, static_cast<const T*>(x), ldx, weight, bias, eps, static_cast<T*>(y), ldy,
+                                                         reinterpret_cast<float2*>(stats), q, ldq, q_scale);
+        };
+        return vec ? go(std::true_type()) : go(std::false_type());
+    });
+}
+
+size_t s2v_layer_norm_grad_workspace_bytes(int64_t rows, int64_t cols)
+{
+    if (rows <= 0 || cols <= 0 || cols > INT32_MAX) return 0;
+    return (size_t)(rows < LN_MAX_LINES ? rows : LN_MAX_LINES) * 2 * (size_t)cols * sizeof(float);
+}
+
+int s2v_layer_norm_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t cols, int type, const void* dy, int64_t lddy, const void* x, int64_t ldx, const int8_t* q,
+                        int64_t ldq, const float* q_scale, const float* stats, const float* weight, void* workspace, size_t workspace_bytes, void* dx, int64_t lddx,
+                        float* dweight, float* dbias)
+{
+    S2V_ENTER(ctx);
+    const auto bad = [&](int status, const char* what) { return s2v_fail(ctx, status, std::string("layer_norm_grad: ") + what); };
+    if (rows < 0 || cols < 1) return bad(S2V_ERR_INVALID_ARG, "negative size or no columns");
+    if (!s2v_dtype_ok(type)) return bad(S2V_ERR_INVALID_ARG, "unknown element type");
+    if (cols > INT32_MAX) return bad(S2V_ERR_UNSUPPORTED, "more than 2^31 - 1 columns");
+    if (!s2v_aligned4(weight, q_scale, dweight, dbias) || reinterpret_cast<uintptr_t>(stats) % 8) return bad(S2V_ERR_INVALID_ARG, "misaligned pointer");
+    cudaStream_t st = s2v_pick_stream(ctx, stream);
+    if (rows == 0) {   // empty sums
+        if (dweight) S2V_CUDA_OK(ctx, cudaMemsetAsync(dweight, 0, (size_t)cols * sizeof(float), st));
+        if (dbias) S2V_CUDA_OK(ctx, cudaMemsetAsync(dbias, 0, (size_t)cols * sizeof(float), st));
+        return S2V_OK;
+    }
+    if (!dy || !dx || !stats) return bad(S2V_ERR_INVALID_ARG, "NULL pointer");
+    if ((x == nullptr) == (q == nullptr) || (q == nullptr) != (q_scale == nullptr)) return bad(S2V_ERR_INVALID_ARG, "takes x, or q and its scales");
+    if (rows > 1 && (lddy < cols || lddx < cols || (x ? ldx : ldq) < cols)) return bad(S2V_ERR_INVALID_ARG, "leading dimension below the number of columns");
+    if (dx == dy && rows > 1 && lddx != lddy) return bad(S2V_ERR_INVALID_ARG, "in place with another leading dimension");
+    const int64_t es = (int64_t)s2v_dtype_bytes(type);
+    if (reinterpret_cast<uintptr_t>(dy) % es || reinterpret_cast<uintptr_t>(x) % es || reinterpret_cast<uintptr_t>(dx) % es) return bad(S2V_ERR_INVALID_ARG, "misaligned pointer");
+    if (dweight || dbias) {
+        if (!workspace || workspace_bytes < s2v_layer_norm_grad_workspace_bytes(rows, cols)) return bad(S2V_ERR_WORKSPACE, "workspace too small");
+        if (!s2v_aligned16(workspace)) return bad(S2V_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
+    }
+    LnGrad a{rows, cols, lddy, x ? ldx : ldq, lddx, dy, x, q, q_scale, reinterpret_cast<const float2*>(stats), weight, dx, static_cast<float*>(workspace), dweight || dbias};
+    const int64_t n = 16 / es;
+    const bool vec = cols % n == 0 && rows_aligned(dy, rows, lddy, es, 16) && rows_aligned(dx, rows, lddx, es, 16) &&
+                     (x ? rows_aligned(x, rows, ldx, es, 16) : rows_aligned(q, rows, ldq, 1, n));
+    return s2v_by_dtype(type, [&](auto t) {
+        using T = decltype(t);
+        return q ? ln_grad_launch<T, true>(ctx, st, a, vec, dweight, dbias) : ln_grad_launch<T, false>(ctx, st, a, vec, dweight, dbias);
+    });
+}
+
+}  // extern "C"

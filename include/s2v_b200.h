@@ -258,6 +258,54 @@ int s2v_distill_topk_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t
                           const int32_t* idx, int t_type, const void* t, int64_t ldt, const float* t_lse, float temperature,
                           const float* row_weight, const float* stats, void* dz, int64_t lddz);
 
+/* ---- training a model's head: layer norm, activations kept in 8 bits, the loss over a vocabulary (no counterpart in the reference; they stand
+ * beside the 8-bit layers above and s2v_cross_entropy_f32, which takes logits) ----
+ * Matrices and leading dimensions as above; rows may start anywhere that an element may.  Workspaces are 16-byte aligned; calls that share one must be
+ * ordered, those inside captured graphs among them.  Every sum has a fixed order: the same call gives the same bits. */
+/* Layer norm of every row of x : [rows x cols] of x_type:
+ *     mean_i = sum_j x_ij / cols;  rstd_i = 1 / sqrt(sum_j (x_ij - mean_i)^2 / cols + eps);  y_ij = (x_ij - mean_i) rstd_i weight_j + bias_j
+ * in fp32, rounded once to x_type.  weight, bias : fp32 [cols] or NULL (1 and 0); eps 0 to 1e30; y : [rows x cols] of x_type, may be x itself (with
+ * ldy = ldx).  What a training step keeps: stats : float [rows x 2], 8-byte aligned, or NULL: mean and rstd; q : int8 [rows x cols] with q_scale : [rows], or
+ * both NULL: the rows of x in 8 bits, exactly as s2v_quantize_rows_i8 gives them, written in the same pass over x.  With eps = 0 a row of equal numbers gives NaN; so
+ * does, whatever eps is, a row with an infinity or NaN (its 8-bit rows: q = 0, q_scale = NaN).  The sum of squares is an fp32 number: deviations of about
+ * 1e19 and more overflow it (rstd = 0). */
+int s2v_layer_norm(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t cols, int x_type, const void* x, int64_t ldx, const float* weight,
+                   const float* bias, float eps, void* y, int64_t ldy, float* stats, int8_t* q, int64_t ldq, float* q_scale);
+/* The gradients, from dy : [rows x cols] of `type`, stats, and either x (then q and q_scale are NULL) or the 8-bit rows (then x is NULL), in which case
+ * q_scale_i q_ij stands for x_ij:
+ *     h_ij = (x_ij - mean_i) rstd_i;  g_ij = dy_ij weight_j;  dx_ij = rstd_i (g_ij - (sum_j g_ij + h_ij sum_j g_ij h_ij) / cols)
+ *     dweight_j = sum_i dy_ij h_ij;  dbias_j = sum_i dy_ij
+ * dx : [rows x cols] of `type`, may be dy itself (with lddx = lddy); dweight, dbias : fp32 [cols] or NULL; the workspace is needed for these alone.
+ * No rows: zeros in dweight and dbias. */
+size_t s2v_layer_norm_grad_workspace_bytes(int64_t rows, int64_t cols);
+int s2v_layer_norm_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t cols, int type, const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                        const int8_t* q, int64_t ldq, const float* q_scale, const float* stats, const float* weight, void* workspace,
+                        size_t workspace_bytes, void* dx, int64_t lddx, float* dweight, float* dbias);
+/* The weight gradient of a dense layer y = x W^T + bias whose input was kept as 8-bit rows, x_ij = q_scale_i q_ij (s2v_quantize_rows_i8, s2v_layer_norm,
+ * or what s2v_linear_i8 multiplied):
+ *     dW_jl = sum_i dy_ij q_scale_i q_il;   dbias_j = sum_i dy_ij
+ * dy : [m x n] of dy_type; q : int8 [m x k]; dW : [n x k] of dy_type; dbias : fp32 [n] or NULL.  With m = 0 they are zeros. */
+size_t s2v_linear_i8_grad_workspace_bytes(int64_t m, int64_t n, int64_t k, int dy_type);
+int s2v_linear_i8_grad(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, int64_t k, int dy_type, const void* dy, int64_t lddy, const int8_t* q,
+                       int64_t ldq, const float* q_scale, void* workspace, size_t workspace_bytes, void* dW, int64_t lddw, float* dbias);
+/* Softmax cross entropy of the logits z = x W^T against one class a row; z is never in memory as a whole:
+ *     loss_i = row_weight_i (log sum_j exp z_ij - z_it),  t = target_i
+ * x : [rows x k], W : [vocab x k] (a class a row), both of `type`; target : int32 [rows]; row_weight : [rows] or NULL (1).  A row whose target lies outside
+ * [0, vocab), or whose row_weight is 0, is left out: loss 0 and gradient 0, whatever x holds there.  A row with an infinity or NaN among its logits
+ * has NaN as its loss (logits of -infinity, which only overflowing products give, among them where they meet).  loss : [rows]; stats : float [rows x 2], 8-byte aligned, or NULL, for the gradient.
+ * `grad` of the workspace's size: whether it has to do for s2v_linear_cross_entropy_grad too. */
+size_t s2v_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t vocab, int64_t k, int type, int grad);
+int s2v_linear_cross_entropy(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t vocab, int64_t k, int type, const void* x, int64_t ldx,
+                             const void* W, int64_t ldw, const int32_t* target, const float* row_weight, void* workspace, size_t workspace_bytes,
+                             float* loss, float* stats);
+/* The gradients of sum_i loss_i, from the `stats` that s2v_linear_cross_entropy wrote for the same x, W and target; row_weight is that of this call (the
+ * gradient that arrives at each row's loss):
+ *     G_ij = row_weight_i (exp z_ij / sum_j exp z_ij - [j = t]);   dx = G W;   dW = G^T x
+ * dx : [rows x k], dW : [vocab x k] of `type`; either may be NULL; they overlap no input and not each other. */
+int s2v_linear_cross_entropy_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t vocab, int64_t k, int type, const void* x, int64_t ldx,
+                                  const void* W, int64_t ldw, const int32_t* target, const float* row_weight, const float* stats, void* workspace,
+                                  size_t workspace_bytes, void* dx, int64_t lddx, void* dW, int64_t lddw);
+
 /* ---- graph pooling: Y[g,:] = sum of H[n,:] over n in [seg_ptr[g], seg_ptr[g+1]).
  * Replaces MatMul(SubgraphMsgPass CSR, H) (kernel_mean_field.cpp:44,
  * src/nn/msg_pass.cpp:156-177) for the batcher's layout, where graph g owns a

@@ -1,0 +1,238 @@
+"""Weight gradients of dense layers from 8-bit rows, against the formula in 64 bits; and a head in training as its calls follow each other."""
+import pytest
+import torch
+
+from graphnn_b200 import capi
+
+gpu = pytest.mark.gpu
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+U = 2.0 ** -24   # half a step of fp32
+
+
+def inputs(m, n, k, dtype, seed=1):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed)
+    dy = (torch.randn((m, n), generator=gen, device="cuda") * (0.2 + torch.rand((m, 1), generator=gen, device="cuda"))).to(TYPES[dtype])
+    q = torch.randint(-127, 128, (m, k), generator=gen, device="cuda", dtype=torch.int8)
+    scale = 0.01 * (0.1 + torch.rand(m, generator=gen, device="cuda"))
+    if m > 3:
+        scale[m // 2], q[m // 2] = 0.0, 0
+    return dy, q, scale
+
+
+def check(dy, q, scale, dW, dbias):
+    m = dy.shape[0]
+    d, x = dy.double(), q.double() * scale.double()[:, None]
+    f = torch.finfo(dy.dtype)
+    if dW is not None and dW.numel():
+        want, size = d.t() @ x, d.abs().t() @ x.abs()
+        # dy times the row's scale is rounded to 16 bits for the product where dy has 16 (fp16: in steps of 2^-24 of the column's largest below the normal range), to three 16-bit
+        # parts where it has 32; a rounding (or a cut, twice as much) for each term of the sum
+        rounding = f.eps / 2 if dy.dtype is not torch.float32 else 2 * U
+        floor = 2.0 ** -24 * (d.abs() * scale.double()[:, None]).amax(0)[:, None] * q.double().abs().sum(0) if m else 0.0
+        tol = (rounding + 2 * U * (m + 8)) * size + (floor if dy.dtype is torch.float16 else 0.0)
+        tol = tol + f.eps / 2 * (want.abs() + tol) + f.smallest_normal * f.eps
+        beyond = want.abs() > f.max * (1 + f.eps / 4)        # nearer to infinity than to the type's largest number: infinite, or the largest, within the tolerance
+        assert bool((dW.double()[beyond] * want[beyond].sign() >= (want.abs() - tol)[beyond].clamp(max=f.max)).all())
+        err = (dW.double() - want).abs()[~beyond & (want.abs() + tol < f.max)]
+        tol = tol[~beyond & (want.abs() + tol < f.max)]
+        assert bool((err <= tol).all()), f"dW off by up to {float((err / tol).max() if err.numel() else 0):.3g} of the tolerance"
+    if dbias is not None:
+        err, tol = (dbias.double() - d.sum(0)).abs(), U * (m + 40) * d.abs().sum(0) + 1e-44
+        assert bool((err <= tol).all()), f"dbias off by up to {float((err / tol).max()):.3g} of the tolerance"
+
+
+def space(ctx, m, n, k, dtype):
+    return torch.full((max(16, ctx.linear_i8_grad_workspace_bytes(m, n, k, dtype)),), 255, dtype=torch.uint8, device="cuda")   # (NaN, as floats of any type)
+
+
+def run(ctx, dy, q, scale, bias=True, stream=None):
+    (m, n), k = dy.shape, q.shape[1]
+    dW, dbias = torch.full((n, k), 5.0, dtype=dy.dtype, device="cuda"), torch.full((n,), 5.0, device="cuda") if bias else None
+    ws = space(ctx, m, n, k, dy.dtype)
+    torch.cuda.synchronize()
+    ctx.linear_i8_grad(dy, q, scale, dW, ws, dbias=dbias, stream=stream)
+    torch.cuda.synchronize()
+    ctx.stream_status(stream)
+    return dW, dbias
+
+
+# ---------------------------------------------------------------- without a GPU
+def test_workspace_sizes_without_a_gpu():
+    size = capi.load_library().s2v_linear_i8_grad_workspace_bytes
+    for bad in ((0, 5, 5, 0), (5, 0, 5, 0), (-1, 5, 5, 0), (5, 5, 5, 3), (5, 5, 5, -1)):
+        assert size(*bad) == 0
+    for t in (0, 1, 2):
+        assert size(100, 40, 60, t) < 1 << 24
+
+
+def test_binding_refuses_what_the_library_cannot_see():
+    ctx = capi.Context.__new__(capi.Context)
+    ctx.h, ctx.device, ctx.lib = None, -1, capi.load_library()   # (torch gives -1 as the device of CPU tensors)
+    made = []
+    ctx.call = lambda name, *a: made.append((name, a))
+    dy, q, s, dW, ws = torch.zeros(4, 6), torch.zeros((4, 9), dtype=torch.int8), torch.zeros(4), torch.zeros(6, 9), torch.zeros(64)
+    ctx.linear_i8_grad(dy, q, s, dW, ws, dbias=torch.zeros(6))
+    assert len(made) == 1 and made[0][1][1:4] == (4, 6, 9)
+    for make in (lambda: ctx.linear_i8_grad(dy.double(), q, s, dW, ws), lambda: ctx.linear_i8_grad(dy, q.float(), s, dW, ws), lambda: ctx.linear_i8_grad(dy, q[:3], s, dW, ws), lambda: ctx.linear_i8_grad(dy, q, s[:3], dW, ws),
+                 lambda: ctx.linear_i8_grad(dy, q, s, dW.half(), ws), lambda: ctx.linear_i8_grad(dy, q, s, dW.t(), ws), lambda: ctx.linear_i8_grad(dy, q, s, dW, ws[::2]),
+                 lambda: ctx.linear_i8_grad(dy, q, s, dW, ws, dbias=torch.zeros(9)), lambda: ctx.linear_i8_grad(dy, q.t().contiguous().t(), s, dW, ws)):
+        with pytest.raises(capi.S2VError):
+            make()
+    assert len(made) == 1
+
+
+# ---------------------------------------------------------------- values
+SHAPES = [(1, 1, 1), (2, 3, 5), (64, 6, 128), (1, 300, 500), (100, 128, 128), (65, 129, 257), (1000, 40, 24), (333, 256, 1021), (2000, 300, 130), (5000, 17, 72), (129, 1500, 700), (4099, 256, 128)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_weight_and_bias_gradients(gpu_ctx, shape, dtype):
+    dy, q, scale = inputs(*shape, dtype)
+    check(dy, q, scale, *run(gpu_ctx, dy, q, scale))
+    dW, _ = run(gpu_ctx, dy, q, scale, bias=False)
+    check(dy, q, scale, dW, None)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("extra,lead", [(16, 0), (3, 0), (16, 1), (5, 3)])
+def test_rows_anywhere_and_nothing_else_written(gpu_ctx, extra, lead, dtype):
+    def spaced(m):
+        base = torch.full((m.shape[0] * (m.shape[1] + extra) + lead + extra,), 7, dtype=m.dtype, device="cuda")
+        view = torch.as_strided(base, m.shape, (m.shape[1] + extra, 1), lead)
+        view.copy_(m)
+        return view, base
+    for m, n, k in ((200, 48, 160), (77, 300, 64)):
+        dy, q, scale = inputs(m, n, k, dtype, seed=3)
+        (dys, _), (qs, _), (dW, dWb) = spaced(dy), spaced(q), spaced(torch.zeros((n, k), dtype=dy.dtype, device="cuda"))
+        dbias, ws = torch.empty(n, device="cuda"), space(gpu_ctx, m, n, k, dy.dtype)
+        torch.cuda.synchronize()
+        gpu_ctx.linear_i8_grad(dys, qs, scale, dW, ws, dbias=dbias)
+        gpu_ctx.synchronize()
+        check(dy, q, scale, dW, dbias)
+        mask = torch.ones_like(dWb, dtype=torch.bool)
+        torch.as_strided(mask, dW.shape, dW.stride(), lead).fill_(False)
+        assert bool((dWb[mask] == 7).all())
+
+
+@gpu
+def test_columns_and_scales_of_very_different_sizes(gpu_ctx):
+    for dtype in TYPES:
+        dy, q, scale = inputs(300, 80, 96, dtype, seed=4)
+        scale *= torch.logspace(-3, 3, 300, device="cuda")[torch.randperm(300, device="cuda")]
+        dy = (dy.float() * torch.logspace(-2, 2, 80, device="cuda")).to(dy.dtype)
+        check(dy, q, scale, *run(gpu_ctx, dy, q, scale))
+        # rows of a scale of NaN (they held no numbers) and of a gradient of infinity reach every weight they touch, and no others
+        scale[5] = float("nan")
+        dW, dbias = run(gpu_ctx, dy, q, scale)
+        assert bool(dW.isnan().all()) and bool(dbias.isfinite().all())
+
+
+@gpu
+def test_same_bits_again_and_empty_sums(gpu_ctx):
+    for dtype in TYPES:
+        dy, q, scale = inputs(6001, 70, 90, dtype, seed=5)
+        first, again = run(gpu_ctx, dy, q, scale), run(gpu_ctx, dy, q, scale, stream=torch.cuda.Stream().cuda_stream)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+        side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        dW, dbias, ws = torch.zeros_like(first[0]), torch.zeros_like(first[1]), space(gpu_ctx, 6001, 70, 90, dy.dtype)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            gpu_ctx.linear_i8_grad(dy, q, scale, dW, ws, dbias=dbias, stream=side.cuda_stream)
+        for _ in range(2):
+            dW.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(dW, first[0]) and torch.equal(dbias, first[1])
+        dW, dbias = run(gpu_ctx, dy[:0], q[:0], scale[:0])
+        assert not dW.any() and not dbias.any()
+
+
+@gpu
+def test_refusals(gpu_ctx):
+    lib, h = gpu_ctx.lib, gpu_ctx.h
+    f = torch.zeros(1 << 18, device="cuda")
+    p, half = f.data_ptr(), f.nbytes // 2
+
+    def call(m=4, n=10, k=8, t=0, dy=p, lddy=10, q=p, ldq=8, s=p, ws=p + half, size=half, dW=p + 4096, lddw=8, db=p + 8192):
+        return lib.s2v_linear_i8_grad(h, None, m, n, k, t, dy, lddy, q, ldq, s, ws, size, dW, lddw, db)
+    for got, want in [(call(m=-1), -1), (call(n=-1), -1), (call(k=-1), -1), (call(t=3), -1), (call(dy=None), -1), (call(q=None), -1), (call(s=None), -1), (call(dW=None), -1), (call(lddy=9), -1), (call(ldq=7), -1),
+                      (call(lddw=7), -1), (call(dy=p + 2), -1), (call(dW=p + 1, t=2), -1), (call(s=p + 2), -1), (call(db=p + 1), -1), (call(ws=None), -5), (call(size=8), -5), (call(ws=p + half + 4), -1), (call(m=1 << 31), -2),
+                      (call(n=1 << 31, lddy=1 << 31), -2), (call(k=1 << 31, ldq=1 << 31, lddw=1 << 31), -2)]:
+        assert got == want, lib.s2v_last_error(h)
+    assert call(n=0) == 0
+    gpu_ctx.synchronize()
+    assert not f.any()
+
+
+# ---------------------------------------------------------------- together, as they are used
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_head_in_training(gpu_ctx, dtype):
+    """Embeddings -> layer norm (kept in 8 bits) -> dense layer (its input kept in 8 bits) -> loss over the classes, and all gradients, against the same chain in
+    64 bits with the 8-bit rows as they are kept."""
+    rows, d, hidden, vocab = 600, 128, 256, 777
+    T, gen = TYPES[dtype], torch.Generator(device="cuda")
+    gen.manual_seed(11)
+
+    def rand(*shape, size=1.0):
+        return torch.randn(shape, generator=gen, device="cuda") * size
+    x, gamma, beta = rand(rows, d, size=2.0).to(T), 1 + 0.2 * rand(d), 0.1 * rand(d)
+    W1, W2 = rand(hidden, d, size=d ** -0.5).to(T), rand(vocab, hidden, size=hidden ** -0.5).to(T)
+    target = torch.randint(0, vocab, (rows,), generator=gen, device="cuda", dtype=torch.int32)
+    target[5::50] = -1
+    weight = torch.full((rows,), 1.0 / int((target >= 0).sum()), device="cuda")
+    xq, xs, stats = torch.empty((rows, d), dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda"), torch.empty((rows, 2), device="cuda")
+    y, hq, hs = torch.empty_like(x), torch.empty((rows, d), dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+    w8, w8s, h = torch.empty((hidden, d), dtype=torch.int8, device="cuda"), torch.empty(hidden, device="cuda"), torch.empty((rows, hidden), dtype=T, device="cuda")
+    loss, kept = torch.empty(rows, device="cuda"), torch.empty((rows, 2), device="cuda")
+    dh, dW2, dW1, db1 = torch.empty_like(h), torch.empty_like(W2), torch.empty_like(W1), torch.empty(hidden, device="cuda")
+    dx, dgamma, dbeta = torch.empty_like(x), torch.empty(d, device="cuda"), torch.empty(d, device="cuda")
+    ws = torch.empty(max(gpu_ctx.linear_cross_entropy_workspace_bytes(rows, vocab, hidden, T), gpu_ctx.linear_i8_grad_workspace_bytes(rows, hidden, d, T),
+                         gpu_ctx.layer_norm_grad_workspace_bytes(rows, d)), dtype=torch.uint8, device="cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        at = s.cuda_stream
+        gpu_ctx.quantize_rows_i8(W1, w8, w8s, stream=at)
+        gpu_ctx.layer_norm(x, y, gamma, beta, 1e-5, stats, xq, xs, stream=at)
+        gpu_ctx.quantize_rows_i8(y, hq, hs, stream=at)
+        gpu_ctx.gemm_i8(hq, hs, w8, w8s, h, relu=True, stream=at)
+        gpu_ctx.linear_cross_entropy(h, W2, target, loss, ws, row_weight=weight, stats=kept, stream=at)
+        gpu_ctx.linear_cross_entropy_grad(h, W2, target, kept, ws, dx=dh, dW=dW2, row_weight=weight, stream=at)
+        dz = torch.where(h > 0, dh, 0.0)                       # back through ReLU
+        gpu_ctx.linear_i8_grad(dz, hq, hs, dW1, ws, dbias=db1, stream=at)
+        dy = dz @ W1
+        gpu_ctx.layer_norm_grad(dy, stats, dx, ws, q=xq, q_scale=xs, weight=gamma, dweight=dgamma, dbias=dbeta, stream=at)
+    s.synchronize()
+    gpu_ctx.stream_status(at)
+    # each step in 64 bits from what the step before handed over
+    live = target >= 0
+    z = h.double() @ W2.double().t()
+    t = torch.where(live, target.long(), 0)[:, None]
+    want = torch.where(live, (z.logsumexp(1) - z.gather(1, t)[:, 0]) * weight.double(), 0.0)
+    assert float((loss.double() - want).abs().max()) < 1e-5 * float(want.max())
+    G = z.softmax(1).scatter_add(1, t, torch.full_like(z[:, :1], -1.0)) * torch.where(live, weight.double(), 0.0)[:, None]
+    eps = torch.finfo(T).eps
+
+    def close(got, want, size):     # operands and results of eps / 2 each, sums of some hundred terms
+        assert bool(((got.double() - want).abs() <= (1.5 * eps + 2 * U * 900) * size + eps / 2 * want.abs()).all())
+    close(dh, G @ W2.double(), G.abs() @ W2.double().abs())
+    close(dW2, G.t() @ h.double(), G.abs().t() @ h.double().abs())
+    check(dz, hq, hs, dW1, db1)
+    kept_x = xq.double() * xs.double()[:, None]
+    hat = (kept_x - stats[:, :1].double()) * stats[:, 1:].double()
+    g = dy.double() * gamma.double()
+    want = stats[:, 1:].double() * (g - g.mean(1, keepdim=True) - hat * (g * hat).mean(1, keepdim=True))
+    assert float((dx.double() - want).abs().max()) <= (eps + 1e-5) * float(want.abs().max())
+    assert float((dgamma.double() - (dy.double() * hat).sum(0)).abs().max()) < 1e-5 * float((dy.double() * hat).abs().sum(0).max())
+    assert float((dbeta.double() - dy.double().sum(0)).abs().max()) < 1e-5 * float(dy.double().abs().sum(0).max())
+    # and the 8-bit rows are worth keeping: gradients of the norm from them point where those from x itself do
+    dx_full = torch.empty_like(x)
+    torch.cuda.synchronize()
+    gpu_ctx.layer_norm_grad(dy, stats, dx_full, ws, x=x, weight=gamma)
+    gpu_ctx.synchronize()
+    assert float(torch.nn.functional.cosine_similarity(dx.double().flatten(), dx_full.double().flatten(), dim=0)) > 0.999
