@@ -2,14 +2,19 @@
 //     loss_i = w_i log sum_j exp(z_ij - z_it),   G_ij = w_i (exp(z_ij - lse_i) - [j = t_i]),   dx = G W,   dW = G^T x.
 // A pass over W leaves, for every row and tile of classes, the largest logit m and l = sum exp(z - m) of the classes other than the row's own, and the row's own
 // logit; joined, they give log sum_j exp(z_ij - z_it) = log1p(sum of the others relative to the own class), which keeps its digits where the own class has
-// nearly all of the probability.  The gradient computes the logits again, a piece of the vocabulary at a time, and multiplies the piece's G.
-#include "product_simt.cuh"
+// nearly all of the probability.  The gradient computes the logits again, a piece of the vocabulary at a time, leaves the piece's G in memory in 16 bits
+// (what the tensor cores multiply; three parts of it where x and W are fp32) and multiplies it.  G in 16 bits is off by half a step of them, as x and W are.
+#include <algorithm>
+
+#include "mm16.cuh"
 
 namespace
 {
 
-constexpr int XE_TILE = PS_TILE;                  // classes of a partial sum
-constexpr size_t XE_PIECE = (size_t)64 << 20;     // bytes of G, about
+constexpr size_t XE_G_BYTES = (size_t)256 << 20;      // of a piece's G
+constexpr size_t XE_W_BYTES = (size_t)128 << 20;      // of a piece of W that has to be copied
+constexpr size_t XE_PART_BYTES = (size_t)256 << 20;   // of a piece's partial sums
+constexpr int64_t XE_TILE = 256;                      // pieces are multiples of it
 
 // a sum of exponentials, l * exp(m)
 struct xe_sum {
@@ -36,124 +41,131 @@ struct xe_rows {
     }
 };
 
-// rows of x, zeros where the row is left out
-template <typename T> struct xe_x_across_k {
-    static constexpr bool K_FAST = false;
-    const T* p;
-    int64_t ld;
-    xe_rows rows;
-    __device__ __forceinline__ float operator()(int64_t i, int64_t k) const { return rows.own(k) < 0 ? 0.0f : to_f32(p[k * ld + i]); }
-};
-
-struct xe_partials {   // 16 threads a row of the tile
-    int64_t rows_n, vocab;
-    xe_rows rows;
-    float2* part;      // [tiles of classes][rows]
-    float* mine;       // [rows]: the own class's logit
-    __device__ __forceinline__ void operator()(int64_t r0, int64_t c0, const float (&acc)[4][4]) const
-    {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int64_t i = r0 + r, own = i < rows_n ? rows.own(i) : -1;
-            xe_sum s{-INFINITY, 0.0f};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int64_t j = c0 + c;
-                if (j >= vocab) continue;
-                if (j == own) mine[i] = acc[r][c];
-                else s.join(acc[r][c], 1.0f);
-            }
-#pragma unroll
-            for (int o = 1; o < 16; o <<= 1) {
-                const float mb = __shfl_xor_sync(0xffffffffu, s.m, o), lb = __shfl_xor_sync(0xffffffffu, s.l, o);
-                s.join(mb, lb);
-            }
-            if (i < rows_n && (threadIdx.x & 15) == 0) part[c0 / XE_TILE * rows_n + i] = make_float2(s.m, s.l);
-        }
-    }
-};
-
-__global__ void __launch_bounds__(128) xe_join_kernel(int64_t rows_n, int tiles, xe_rows rows, const float2* __restrict__ part, const float* __restrict__ mine, float* __restrict__ loss,
-                                                      float2* __restrict__ stats)
+// The partial sums of a piece, THREADS threads a row, onto what the pieces before gave (`run`, [rows]; first: nothing yet); after the last piece the loss.
+template <int THREADS>
+__global__ void __launch_bounds__(256) xe_join_kernel(int64_t rows_n, int lines, xe_rows rows, const float2* __restrict__ part, const float* __restrict__ mine, float2* __restrict__ run, int first,
+                                                      int last, float* __restrict__ loss, float2* __restrict__ stats)
 {
-    const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
-    if (i >= rows_n) return;
+    constexpr int ROWS = 256 / THREADS;
+    __shared__ float2 of[THREADS][ROWS];
+    const int at = threadIdx.x % ROWS, g = threadIdx.x / ROWS;
+    const int64_t i = (int64_t)blockIdx.x * ROWS + at;
+    xe_sum s{-INFINITY, 0.0f};
+    if (i < rows_n)
+        for (int t = g; t < lines; t += 4 * THREADS) {
+            float2 p[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) p[u] = t + u * THREADS < lines ? part[(int64_t)(t + u * THREADS) * rows_n + i] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) s.join(p[u].x, p[u].y);
+        }
+    of[g][at] = make_float2(s.m, s.l);
+    __syncthreads();
+#pragma unroll
+    for (int o = THREADS / 2; o; o >>= 1) {
+        if (g < o) {
+            s.join(of[g + o][at].x, of[g + o][at].y);
+            of[g][at] = make_float2(s.m, s.l);
+        }
+        __syncthreads();
+    }
+    if (g || i >= rows_n) return;
+    if (!first) s.join(run[i].x, run[i].y);
+    if (!last) {
+        run[i] = make_float2(s.m, s.l);
+        return;
+    }
     if (rows.own(i) < 0) {
         loss[i] = 0.0f;
         if (stats) stats[i] = make_float2(0.0f, 0.0f);
         return;
     }
-    xe_sum s{-INFINITY, 0.0f};
-    for (int t = 0; t < tiles; ++t) {
-        const float2 p = part[(int64_t)t * rows_n + i];
-        s.join(p.x, p.y);
-    }
-    // log(1 + l exp(m - z_t)), from whichever side is the larger
+    // log(1 + l exp(m - z_t)), from whichever side is the larger; alone in the vocabulary a class loses nothing
     const double d = (double)s.m - (double)mine[i];
-    const double one = s.m == -INFINITY && s.l == 0.0f ? (mine[i] - mine[i]) : d > 0 ? d + log((double)s.l + exp(-d)) : log1p((double)s.l * exp(d));
+    const double one = s.m == -INFINITY && s.l == 0.0f ? (double)(mine[i] - mine[i]) : d > 0 ? d + log((double)s.l + exp(-d)) : log1p((double)s.l * exp(d));
     loss[i] = (float)(one * (rows.weight ? (double)rows.weight[i] : 1.0));
     if (stats) stats[i] = make_float2((float)(one + (double)mine[i]), (float)expm1(-one));
 }
+int xe_join(s2v_ctx* ctx, cudaStream_t st, int64_t rows_n, int lines, xe_rows rows, const float2* part, const float* mine, float2* run, bool first, bool last, float* loss, float* stats)
+{
+    const auto go = [&](auto kernel, int threads) {
+        const int64_t per = 256 / threads;
+        kernel<<<(unsigned)((rows_n + per - 1) / per), 256, 0, st>>>(rows_n, lines, rows, part, mine, run, first, last, loss, reinterpret_cast<float2*>(stats));
+        S2V_CHECK_LAUNCH(ctx, "xe_join_kernel");
+        return (int)S2V_OK;
+    };
+    return rows_n >= 2048 || lines <= 32 ? go(xe_join_kernel<8>, 8) : go(xe_join_kernel<64>, 64);
+}
 
-struct xe_gradient {   // a piece's G
-    int64_t rows_n, cols, first;   // the piece's classes: first to first + cols
-    xe_rows rows;
-    const float2* stats;
-    float* g;
-    int64_t ldg;
-    __device__ __forceinline__ void operator()(int64_t r0, int64_t c0, const float (&acc)[4][4]) const
-    {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int64_t i = r0 + r;
-            if (i >= rows_n) continue;
-            const int64_t own = rows.own(i);
-            const float w = own < 0 ? 0.0f : rows.weight ? rows.weight[i] : 1.0f;
-            const float2 st = stats[i];
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (c0 + c < cols) g[i * ldg + c0 + c] = own < 0 ? 0.0f : w * (first + c0 + c == own ? st.y : expf(acc[r][c] - st.x));
+// G in 16 bits of fp16 is scaled by a power of two that puts the largest row weight's binade at 2^14: its steps are then 2^-38 of that and less.
+// factor[0], and factor[1] = 1 / factor[0].
+__global__ void __launch_bounds__(1024) xe_factor_kernel(int64_t rows_n, xe_rows rows, float* factor)
+{
+    __shared__ uint32_t part[32];
+    uint32_t top = 0;
+    for (int64_t i = threadIdx.x; i < rows_n; i += 1024)
+        if (rows.own(i) >= 0) {
+            const uint32_t w = rows.weight ? __float_as_uint(rows.weight[i]) & 0x7fffffffu : 0x3f800000u;
+            if (w < 0x7f800000u) top = max(top, w);
         }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    top = __reduce_max_sync(0xffffffffu, part[threadIdx.x]);
+    if (threadIdx.x == 0) {
+        const int e = min(max((int)(top >> 23) - 127, -100), 127);   // (weights below 2^-100 are not scaled up further)
+        factor[0] = exp2f((float)(14 - e)), factor[1] = exp2f((float)(e - 14));
     }
-};
+}
 
-// outputs added to those of the pieces before
-template <typename T> struct xe_add_outputs {
-    float* sum;
-    T* p;   // NULL before the last piece
-    int64_t ld, m, n;
-    int start;
-    __device__ __forceinline__ void operator()(int64_t r0, int64_t c0, const float (&acc)[4][4]) const
-    {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (r0 + r < m && c0 + c < n) {
-                    float* const s = sum + (r0 + r) * n + c0 + c;
-                    const float v = start ? acc[r][c] : *s + acc[r][c];
-                    if (p) p[(r0 + r) * ld + c0 + c] = from_f32<T>(v);
-                    else *s = v;
-                }
+// What a row's G is multiplied by before it is rounded to 16 bits, and what the rounding takes from the own class's, a row's largest number by far: dx gets that
+// times the class's row of W back, in fp32 (400 rows, 5000 classes, fp16: 1.4e-4 off from the rounding of G without it, relative, 2e-5 with it; bf16 1.0e-3 and 1.6e-4).
+template <typename H> __global__ void __launch_bounds__(256) xe_row_scale_kernel(int64_t rows_n, xe_rows rows, const float2* __restrict__ stats, const float* __restrict__ factor,
+                                                                                 float* __restrict__ scale, float* __restrict__ fix)
+{
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows_n) return;
+    float s = 0.0f, f = 0.0f;
+    if (rows.own(i) >= 0) {
+        s = (rows.weight ? rows.weight[i] : 1.0f) * (factor ? factor[0] : 1.0f);
+        const float own = s * stats[i].y;
+        f = (own - to_f32(from_f32<H>(own))) * (factor ? factor[1] : 1.0f);
     }
-};
+    scale[i] = s, fix[i] = f;
+}
 
-// Where things lie in the workspace.
+// Where things lie in the workspace, and how many classes a piece has.  `copied`: whether W has to be copied (fp32, or rows that don't lie on 16-byte boundaries).
 struct xe_space {
-    size_t part = 0, mine = 0, g = 0, sum = 0, bytes = 0;
-    int64_t piece = 0;
-    xe_space(int64_t rows, int64_t vocab, int64_t k, bool grad)
+    size_t mine = 0, run = 0, part = 0, x16 = 0, w16 = 0, factor = 0, scale = 0, g = 0, sum = 0, lines = 0, bytes = 0;
+    int64_t piece = 0, ld16 = 0, ldg = 0, parts = 0;
+    xe_space(int64_t rows, int64_t vocab, int64_t k, int type, bool grad, bool copied)
     {
         const auto take = [&](size_t& at, size_t n) { at = bytes, bytes += (n + 255) / 256 * 256; };
-        if (!grad) {
+        parts = type == S2V_F32 ? 3 : 1;
+        ld16 = (k + 7) / 8 * 8;
+        const auto of = [&](size_t all, size_t each) { return std::max((int64_t)(all / each) / XE_TILE * XE_TILE, XE_TILE); };
+        piece = vocab;
+        if (copied) piece = std::min(piece, of(XE_W_BYTES, (size_t)ld16 * 2 * parts));
+        if (grad) {
+            piece = std::min(piece, of(XE_G_BYTES, (size_t)rows * 2 * parts));
+            ldg = (piece + 63) / 64 * 64;
+            take(factor, 2 * sizeof(float));
+            take(scale, 2 * (size_t)rows * sizeof(float));
+            take(g, (size_t)rows * ldg * 2 * parts);
+            take(sum, (size_t)rows * mm16_pitch(k) * sizeof(float));
+            const int products = parts == 3 ? 6 : 1;
+            const int64_t last = vocab - (vocab - 1) / piece * piece;   // (fewer tiles, which may have more shares)
+            take(lines, (size_t)std::max({mm16_split_floats_most(rows, k, piece, products), mm16_split_floats_most(piece, k, rows, products), mm16_split_floats_most(last, k, rows, products)}) *
+                            sizeof(float));
+        } else {
+            piece = std::min(piece, of(XE_PART_BYTES, (size_t)rows * sizeof(float2)) * 64);   // (a line for every 64 classes at most)
             take(mine, (size_t)rows * sizeof(float));
-            take(part, (size_t)rows * (size_t)((vocab + XE_TILE - 1) / XE_TILE) * sizeof(float2));
-            return;
+            take(run, (size_t)rows * sizeof(float2));
+            take(part, (size_t)rows * mm16_sum_lines_most(piece) * sizeof(float2));
         }
-        piece = (int64_t)(XE_PIECE / sizeof(float)) / rows / XE_TILE * XE_TILE;
-        piece = piece < XE_TILE ? XE_TILE : piece > vocab ? vocab : piece;
-        take(g, (size_t)rows * (size_t)piece * sizeof(float));
-        take(sum, (size_t)rows * (size_t)k * sizeof(float));
+        if (copied) take(w16, (size_t)piece * ld16 * 2 * parts);
+        take(x16, (size_t)rows * ld16 * 2 * parts);
     }
 };
 
@@ -172,6 +184,38 @@ int check(s2v_ctx* ctx, const char* name, int64_t rows, int64_t vocab, int64_t k
     return S2V_OK;
 }
 
+// What both calls hand to the products: x and W in 16-bit parts, where they lie or copied.
+struct xe_call {
+    s2v_ctx* ctx;
+    cudaStream_t st;
+    bool copy_x, copy_w;
+    xe_space space;
+    xe_rows rows;
+    mm16_args args;
+    const unsigned char* W;
+    int64_t ldw;
+    int type;
+    unsigned char* w16;
+    static bool lies(int type, const void* p, int64_t rows, int64_t ld) { return type != S2V_F32 && s2v_aligned16(p) && (rows <= 1 || ld % 8 == 0); }
+    xe_call(s2v_ctx* ctx_, cudaStream_t st_, int64_t n, int64_t vocab, int64_t k, int type_, const void* x, int64_t ldx, const void* W_, int64_t ldw_, const int32_t* target, const float* weight,
+            unsigned char* ws, bool grad)
+        : ctx(ctx_), st(st_), copy_x(grad || !lies(type_, x, n, ldx)), copy_w(!lies(type_, W_, vocab, ldw_)), space(n, vocab, k, type_, grad, copy_w), rows{target, weight, vocab},
+          W(static_cast<const unsigned char*>(W_)), ldw(ldw_), type(type_), w16(ws + space.w16)
+    {
+        args.type = type == S2V_F16 ? S2V_F16 : S2V_BF16;
+        args.m = n, args.k = k;
+        args.a.p = copy_x ? ws + space.x16 : x, args.a.rows = n, args.a.cols = k, args.a.ld = copy_x ? space.ld16 : ldx, args.a.part = n * space.ld16, args.a.parts = (int)space.parts;
+        args.target = target, args.weight = weight, args.vocab = vocab;
+    }
+    int piece_of_w(mm16_operand& b, int64_t first, int64_t cols) const
+    {
+        const unsigned char* const from = W + (size_t)first * (rows.vocab > 1 ? ldw : 0) * s2v_dtype_bytes(type);
+        b.rows = cols, b.cols = args.k, b.parts = (int)space.parts;
+        b.p = copy_w ? w16 : from, b.ld = copy_w ? space.ld16 : ldw, b.part = cols * space.ld16;
+        return copy_w ? mm16_pack(ctx, st, cols, args.k, type, from, ldw, nullptr, nullptr, 0, w16, space.ld16, b.part) : S2V_OK;
+    }
+};
+
 }  // namespace
 
 extern "C" {
@@ -179,9 +223,10 @@ extern "C" {
 size_t s2v_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t vocab, int64_t k, int type, int grad)
 {
     if (rows <= 0 || vocab <= 0 || k <= 0 || rows > INT32_MAX || vocab > INT32_MAX || k > INT32_MAX || !s2v_dtype_ok(type)) return 0;
-    const size_t loss = xe_space(rows, vocab, k, false).bytes;
-    const size_t both = grad ? xe_space(rows, vocab, k, true).bytes : 0;
-    return loss > both ? loss : both;
+    size_t most = 0;   // wherever the matrices lie
+    for (int form = 0; form < (grad ? 4 : 2); ++form)
+        if ((form & 1) || type != S2V_F32) most = std::max(most, xe_space(rows, vocab, k, type, form & 2, form & 1).bytes);
+    return most;
 }
 
 int s2v_linear_cross_entropy(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t vocab, int64_t k, int type, const void* x, int64_t ldx, const void* W, int64_t ldw,
@@ -193,23 +238,25 @@ int s2v_linear_cross_entropy(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int6
     const auto bad = [&](int status, const char* what) { return s2v_fail(ctx, status, std::string("linear_cross_entropy: ") + what); };
     if (!loss) return bad(S2V_ERR_INVALID_ARG, "NULL pointer");
     if (!s2v_aligned4(loss) || reinterpret_cast<uintptr_t>(stats) % 8) return bad(S2V_ERR_INVALID_ARG, "misaligned pointer");
-    const xe_space space(rows, vocab, k, false);
     if (!workspace || workspace_bytes < s2v_linear_cross_entropy_workspace_bytes(rows, vocab, k, type, 0)) return bad(S2V_ERR_WORKSPACE, "workspace too small");
     if (!s2v_aligned16(workspace)) return bad(S2V_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
     cudaStream_t st = s2v_pick_stream(ctx, stream);
     unsigned char* const ws = static_cast<unsigned char*>(workspace);
-    float2* const part = reinterpret_cast<float2*>(ws + space.part);
-    float* const mine = reinterpret_cast<float*>(ws + space.mine);
-    const xe_rows r{target, row_weight, vocab};
-    const int done = s2v_by_dtype(type, [&](auto t) {
-        using T = decltype(t);
-        return product_simt(ctx, st, "linear_cross_entropy", rows, vocab, k, along_k<T>{static_cast<const T*>(x), ldx}, along_k<T>{static_cast<const T*>(W), ldw},
-                            xe_partials{rows, vocab, r, part, mine});
-    });
-    if (done != S2V_OK) return done;
-    xe_join_kernel<<<(unsigned)((rows + 127) / 128), 128, 0, st>>>(rows, (int)((vocab + XE_TILE - 1) / XE_TILE), r, part, mine, loss, reinterpret_cast<float2*>(stats));
-    S2V_CHECK_LAUNCH(ctx, "xe_join_kernel");
-    return S2V_OK;
+    const xe_call c(ctx, st, rows, vocab, k, type, x, ldx, W, ldw, target, row_weight, ws, false);
+    const xe_space& space = c.space;
+    mm16_args a = c.args;
+    int done = S2V_OK;
+    if (c.copy_x) done = mm16_pack(ctx, st, rows, k, type, x, ldx, nullptr, nullptr, 0, ws + space.x16, space.ld16, rows * space.ld16);
+    a.part = reinterpret_cast<float2*>(ws + space.part), a.mine = reinterpret_cast<float*>(ws + space.mine);
+    for (int64_t first = 0; done == S2V_OK && first < vocab; first += space.piece) {
+        const int64_t cols = std::min(space.piece, vocab - first);
+        done = c.piece_of_w(a.b, first, cols);
+        a.n = cols, a.first = first;
+        if (done == S2V_OK) done = mm16_launch(ctx, st, MM16_SUMS, a);
+        if (done == S2V_OK)
+            done = xe_join(ctx, st, rows, mm16_sum_lines(ctx, rows, cols), c.rows, a.part, a.mine, reinterpret_cast<float2*>(ws + space.run), first == 0, first + cols == vocab, loss, stats);
+    }
+    return done;
 }
 
 int s2v_linear_cross_entropy_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t vocab, int64_t k, int type, const void* x, int64_t ldx, const void* W, int64_t ldw,
@@ -230,31 +277,58 @@ int s2v_linear_cross_entropy_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows,
     }
     if (!stats) return bad(S2V_ERR_INVALID_ARG, "NULL pointer");
     if (!dx && !dW) return S2V_OK;
-    const xe_space space(rows, vocab, k, true);
     if (!workspace || workspace_bytes < s2v_linear_cross_entropy_workspace_bytes(rows, vocab, k, type, 1)) return bad(S2V_ERR_WORKSPACE, "workspace too small");
     if (!s2v_aligned16(workspace)) return bad(S2V_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
     unsigned char* const ws = static_cast<unsigned char*>(workspace);
-    float* const g = reinterpret_cast<float*>(ws + space.g);
-    float* const sum = reinterpret_cast<float*>(ws + space.sum);
-    const xe_rows r{target, row_weight, vocab};
-    return s2v_by_dtype(type, [&](auto t) {
-        using T = decltype(t);
-        const T* const xt = static_cast<const T*>(x);
-        const T* const wt = static_cast<const T*>(W);
-        for (int64_t first = 0; first < vocab; first += space.piece) {
-            const int64_t cols = space.piece < vocab - first ? space.piece : vocab - first;
-            int done = product_simt(ctx, st, "linear_cross_entropy_grad", rows, cols, k, along_k<T>{xt, ldx}, along_k<T>{wt + first * ldw, ldw},
-                                    xe_gradient{rows, cols, first, r, reinterpret_cast<const float2*>(stats), g, space.piece});
-            if (done == S2V_OK && dx)
-                done = product_simt(ctx, st, "linear_cross_entropy_grad", rows, k, cols, along_k<float>{g, space.piece}, across_k<T>{wt + first * ldw, ldw},
-                                    xe_add_outputs<T>{sum, first + cols == vocab ? static_cast<T*>(dx) : nullptr, lddx, rows, k, first == 0});
-            if (done == S2V_OK && dW)
-                done = product_simt(ctx, st, "linear_cross_entropy_grad", cols, k, rows, across_k<float>{g, space.piece}, xe_x_across_k<T>{xt, ldx, r},
-                                    store_outputs<T>{static_cast<T*>(dW) + first * lddw, lddw, cols, k});
-            if (done != S2V_OK) return done;
+    const xe_call c(ctx, st, rows, vocab, k, type, x, ldx, W, ldw, target, row_weight, ws, true);
+    const xe_space& space = c.space;
+    // x with zeros in the rows that are left out, whatever these hold: their zeros of G meet zeros in dW
+    int done = mm16_pack(ctx, st, rows, k, type, x, ldx, target, row_weight, vocab, ws + space.x16, space.ld16, rows * space.ld16);
+    float* factor = nullptr;
+    if (done == S2V_OK && type == S2V_F16) {
+        factor = reinterpret_cast<float*>(ws + space.factor);
+        xe_factor_kernel<<<1, 1024, 0, st>>>(rows, c.rows, factor);
+        S2V_CHECK_LAUNCH(ctx, "xe_factor_kernel");
+    }
+    float* const scale = reinterpret_cast<float*>(ws + space.scale);
+    const float2* const kept = reinterpret_cast<const float2*>(stats);
+    if (done == S2V_OK) {
+        const auto kernel = type == S2V_F32 ? xe_row_scale_kernel<float> : type == S2V_F16 ? xe_row_scale_kernel<__half> : xe_row_scale_kernel<__nv_bfloat16>;
+        kernel<<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(rows, c.rows, kept, factor, scale, scale + rows);
+        S2V_CHECK_LAUNCH(ctx, "xe_row_scale_kernel");
+    }
+    mm16_args z = c.args;   // the logits again
+    z.stats = kept, z.row_scale = scale;
+    z.g = ws + space.g, z.ldg = space.ldg, z.g_part = rows * space.ldg, z.g_parts = (int)space.parts;
+    for (int64_t first = 0; done == S2V_OK && first < vocab; first += space.piece) {
+        const int64_t cols = std::min(space.piece, vocab - first);
+        done = c.piece_of_w(z.b, first, cols);
+        z.n = cols, z.first = first;
+        if (done == S2V_OK) done = mm16_launch(ctx, st, MM16_SOFTMAX_GRAD, z);
+        mm16_args p;
+        p.type = z.type;
+        p.a.p = z.g, p.a.rows = rows, p.a.cols = cols, p.a.ld = space.ldg, p.a.part = z.g_part, p.a.parts = (int)space.parts;
+        p.alpha = factor ? factor + 1 : nullptr;
+        p.lines = reinterpret_cast<float*>(ws + space.lines);
+        p.out_type = type, p.n = k;
+        if (done == S2V_OK && dx) {
+            mm16_args q = p;
+            q.b = z.b, q.m = rows, q.k = cols;
+            q.sum = reinterpret_cast<float*>(ws + space.sum), q.add = first > 0;
+            if (first + cols == vocab) {
+                q.out = dx, q.ldo = lddx;
+                if (type != S2V_F32) q.fix = scale + rows, q.target = target, q.vocab = vocab, q.fix_w = W, q.fix_ld = ldw;
+            }
+            done = mm16_launch(ctx, st, MM16_OUT, q);
         }
-        return (int)S2V_OK;
-    });
+        if (done == S2V_OK && dW) {
+            mm16_args q = p;
+            q.b = z.a, q.m = cols, q.k = rows;
+            q.out = static_cast<unsigned char*>(dW) + (size_t)first * (vocab > 1 ? lddw : k) * es, q.ldo = lddw;
+            done = mm16_launch(ctx, st, MM16_OUT_ACROSS, q);
+        }
+    }
+    return done;
 }
 
 }  // extern "C"

@@ -9,7 +9,7 @@
 #include <cstring>
 
 #include "gemm_i8.cuh"
-#include "tcgen05.cuh"
+#include "tcgen05_pair.cuh"
 #include "tma.cuh"
 
 namespace
@@ -67,70 +67,6 @@ template <bool PAIR> __device__ __forceinline__ void gi_mma(uint32_t d_tmem, uin
             :
             : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
             : "memory");
-}
-// the barrier of this CTA, or of both of the pair, once all products issued so far are done
-template <bool PAIR> __device__ __forceinline__ void gi_commit(uint32_t bar)
-{
-    if constexpr (PAIR)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
-    else
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-// tc_wait for barriers on which the other CTA of the pair arrives too.  Where all that a barrier orders is accumulators in tensor memory, which tcgen05.fence
-// takes care of, its arrivals and waits are relaxed (released and acquired at the cluster's scope they cost pairs of 256 x 128 a third of their time at
-// k = 128, and a microsecond of 18 at 200 x 14336 x 4096).
-template <bool ACQUIRE> __device__ __forceinline__ bool gi_wait_pair(uint32_t bar, uint32_t parity, volatile int* abort_flag, s2v_device_status* status, int site)
-{
-    int spins = 0;
-    bool ok = true;
-    for (;;) {
-        uint32_t done;
-        if constexpr (ACQUIRE)
-            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                         : "=r"(done)
-                         : "r"(bar), "r"(parity), "r"(TC_SUSPEND_NS)
-                         : "memory");
-        else
-            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                         : "=r"(done)
-                         : "r"(bar), "r"(parity), "r"(TC_SUSPEND_NS)
-                         : "memory");
-        if (done) break;
-        if (*abort_flag) { ok = false; break; }
-        if (++spins > TC_WAIT_LIMIT) {
-            *abort_flag = 1;
-            status->code = S2V_ERR_DEVICE_TIMEOUT;
-            status->where = site;
-            ok = false;
-            break;
-        }
-    }
-    return __all_sync(0xffffffffu, ok);
-}
-// the address of a barrier in the pair's first CTA
-__device__ __forceinline__ uint32_t gi_first(uint32_t bar)
-{
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(bar));
-    return r;
-}
-
-// Tiles in columns of 16 row tiles, so that the tiles of one moment share panels of both matrices in L2.
-__device__ __forceinline__ void gi_tile(int tile, int m_tiles, int n_tiles, int& tm, int& tn)
-{
-    constexpr int G = 16;
-    const int per = G * n_tiles, g = tile / per, first = g * G, rows = min(G, m_tiles - first), at = tile - g * per;
-    tm = first + at % rows;
-    tn = at / rows;
-}
-
-// Accumulators that tcgen05.ld was asked for: no use of them comes before the wait.
-template <int N> __device__ __forceinline__ void gi_wait_loads(uint32_t (&v)[N])
-{
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int j = 0; j < N; j += 8)
-        asm volatile("" : "+r"(v[j]), "+r"(v[j + 1]), "+r"(v[j + 2]), "+r"(v[j + 3]), "+r"(v[j + 4]), "+r"(v[j + 5]), "+r"(v[j + 6]), "+r"(v[j + 7]));
 }
 // fma(sa * s, v, b) of two accumulators, in packed fp32 arithmetic
 __device__ __forceinline__ void gi_two(uint64_t sa, uint64_t s, uint64_t b, uint32_t v0, uint32_t v1, float& y0, float& y1)
@@ -297,7 +233,7 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
         bool ok = true;
         for (int tile = unit; ok && tile < tiles; tile += units) {
             int tm, tn;
-            gi_tile(tile, a.m_tiles, a.n_tiles, tm, tn);
+            tc_tile(tile, a.m_tiles, a.n_tiles, tm, tn);
             for (int kb = 0; kb < a.kblocks; ++kb, ++it) {
                 const int s = it % STAGES;
                 if (it >= STAGES && !(ok = tc_wait(bar(Cfg::EMPTY + s), (uint32_t)(it / STAGES - 1) & 1u, abort_flag, a.status, 70))) break;
@@ -305,7 +241,7 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
                     const uint32_t at = smem0 + (uint32_t)s * Cfg::STAGE;
                     if constexpr (PAIR) {   // both CTAs' copies count on the first one's barrier, where the products are issued
                         if (rank == 0) mbar_expect(bar(Cfg::FULL + s), 2 * a.bytes);
-                        const uint32_t b = gi_first(bar(Cfg::FULL + s));
+                        const uint32_t b = tc_pair_first(bar(Cfg::FULL + s));
                         tma_load_2d_pair(at, &map_a, kb * 128, tm * 256 + rank * 128, b);
                         tma_load_2d_pair(at + Cfg::A_BYTES, &map_b, kb * 128, tn * BN + rank * Cfg::B_ROWS, b);
                     } else {
@@ -333,13 +269,13 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
         bool ok = rank == 0;
         for (int tile = unit; ok && tile < tiles; tile += units, ++t) {
             const int acc = t % ACCS;
-            if (t >= ACCS && !(ok = PAIR ? gi_wait_pair<false>(bar(Cfg::READ + acc), (uint32_t)(t / ACCS - 1) & 1u, abort_flag, a.status, 71)
+            if (t >= ACCS && !(ok = PAIR ? tc_wait_pair<false>(bar(Cfg::READ + acc), (uint32_t)(t / ACCS - 1) & 1u, abort_flag, a.status, 71)
                                       : tc_wait(bar(Cfg::READ + acc), (uint32_t)(t / ACCS - 1) & 1u, abort_flag, a.status, 71)))
                 break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (int kb = 0; kb < a.kblocks; ++kb, ++it) {
                 const int s = it % STAGES;
-                if (!(ok = PAIR ? gi_wait_pair<true>(bar(Cfg::FULL + s), (uint32_t)(it / STAGES) & 1u, abort_flag, a.status, 72)
+                if (!(ok = PAIR ? tc_wait_pair<true>(bar(Cfg::FULL + s), (uint32_t)(it / STAGES) & 1u, abort_flag, a.status, 72)
                                 : tc_wait(bar(Cfg::FULL + s), (uint32_t)(it / STAGES) & 1u, abort_flag, a.status, 72)))
                     break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -349,8 +285,8 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks)
                         if (ks < steps) gi_mma<PAIR>(tmem + (uint32_t)(acc * BN), da + 2u * ks, db + 2u * ks, Cfg::IDESC, kb > 0 || ks > 0);
-                    gi_commit<PAIR>(bar(Cfg::EMPTY + s));
-                    if (kb + 1 == a.kblocks) gi_commit<PAIR>(bar(Cfg::DONE + acc));
+                    tc_commit<PAIR>(bar(Cfg::EMPTY + s));
+                    if (kb + 1 == a.kblocks) tc_commit<PAIR>(bar(Cfg::DONE + acc));
                 }
                 __syncwarp();
             }
@@ -373,7 +309,7 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
         int64_t row0 = 0, first = 0;
         const auto fetch_scales = [&](int tile) {
             int tm, tn;
-            gi_tile(tile, a.m_tiles, a.n_tiles, tm, tn);
+            tc_tile(tile, a.m_tiles, a.n_tiles, tm, tn);
             row0 = (int64_t)tm * (128 * CTAS) + rank * 128 + quarter * 32, first = (int64_t)tn * BN + half * HALF;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -400,7 +336,7 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
             for (int u = 0; u < HALF / 32; ++u) chan[gi_place<T>(u * 32 + lane)] = s[u], chan[HALF + gi_place<T>(u * 32 + lane)] = bias[u];
             __syncwarp();
             if (tile + units < tiles) fetch_scales(tile + units);
-            if (a.kblocks > 0 && !(PAIR ? gi_wait_pair<false>(bar(Cfg::DONE + acc), (uint32_t)(t / ACCS) & 1u, abort_flag, a.status, 73)
+            if (a.kblocks > 0 && !(PAIR ? tc_wait_pair<false>(bar(Cfg::DONE + acc), (uint32_t)(t / ACCS) & 1u, abort_flag, a.status, 73)
                                         : tc_wait(bar(Cfg::DONE + acc), (uint32_t)(t / ACCS) & 1u, abort_flag, a.status, 73)))
                 break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -412,7 +348,7 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
             for (int c = 0; c < HALF; c += COLS) {
                 if (c >= cols) break;
                 uint32_t(&now)[COLS] = v[c / COLS & 1];
-                gi_wait_loads(now);
+                tc_wait_loads(now);
                 if (c + COLS < cols && a.kblocks > 0) gi_fetch<T>(at + (uint32_t)(c + COLS), v[~(c / COLS) & 1]);
                 // the copy that last read this box has done so: of the groups since then, one a piece, as many may be under way as there are other boxes
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(Cfg::BOXES - 1) : "memory");
@@ -422,7 +358,7 @@ __global__ void __launch_bounds__(GI_THREADS, 1) gemm_i8_kernel(const __grid_con
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (lane == 0) {
-                if constexpr (PAIR) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(gi_first(bar(Cfg::READ + acc))) : "memory");
+                if constexpr (PAIR) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(tc_pair_first(bar(Cfg::READ + acc))) : "memory");
                 else tc_mbar_arrive(bar(Cfg::READ + acc));
             }
             __syncwarp();

@@ -284,7 +284,8 @@ int s2v_layer_norm_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t c
 /* The weight gradient of a dense layer y = x W^T + bias whose input was kept as 8-bit rows, x_ij = q_scale_i q_ij (s2v_quantize_rows_i8, s2v_layer_norm,
  * or what s2v_linear_i8 multiplied):
  *     dW_jl = sum_i dy_ij q_scale_i q_il;   dbias_j = sum_i dy_ij
- * dy : [m x n] of dy_type; q : int8 [m x k]; dW : [n x k] of dy_type; dbias : fp32 [n] or NULL.  With m = 0 they are zeros. */
+ * dy : [m x n] of dy_type; q : int8 [m x k]; dW : [n x k] of dy_type; dbias : fp32 [n] or NULL.  With m = 0 they are zeros.  k is 1 or more.
+ * An infinity or NaN in dy or q_scale makes the sums that it is part of infinite or NaN. */
 size_t s2v_linear_i8_grad_workspace_bytes(int64_t m, int64_t n, int64_t k, int dy_type);
 int s2v_linear_i8_grad(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, int64_t k, int dy_type, const void* dy, int64_t lddy, const int8_t* q,
                        int64_t ldq, const float* q_scale, void* workspace, size_t workspace_bytes, void* dW, int64_t lddw, float* dbias);

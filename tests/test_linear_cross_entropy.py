@@ -265,9 +265,10 @@ def test_gradients_against_differences(gpu_ctx):
 
 @gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-def test_many_pieces_of_the_vocabulary(gpu_ctx, dtype):
-    # rows enough that a piece's gradient of the logits is a small part of the vocabulary
-    x, W, target, weight = inputs(9000, 20011, 48, dtype, seed=8)
+@pytest.mark.parametrize("rows,vocab", [(9000, 20011), (9000, 15000), (70000, 1850), (70000, 3800)])
+def test_many_pieces_of_the_vocabulary(gpu_ctx, rows, vocab, dtype):
+    # rows enough that a piece's gradient of the logits is a part of the vocabulary, with small and large last pieces
+    x, W, target, weight = inputs(rows, vocab, 48, dtype, seed=8)
     loss, dx, dW = both(gpu_ctx, x, W, target, weight)
     ref = Reference(x, W, target, weight)
     ref.check_loss(loss)
