@@ -155,9 +155,7 @@ struct xe_space {
             take(g, (size_t)rows * ldg * 2 * parts);
             take(sum, (size_t)rows * mm16_pitch(k) * sizeof(float));
             const int products = parts == 3 ? 6 : 1;
-            const int64_t last = vocab - (vocab - 1) / piece * piece;   // (fewer tiles, which may have more shares)
-            take(lines, (size_t)std::max({mm16_split_floats_most(rows, k, piece, products), mm16_split_floats_most(piece, k, rows, products), mm16_split_floats_most(last, k, rows, products)}) *
-                            sizeof(float));
+            take(lines, std::max(mm16_lines_bytes(piece, products), mm16_lines_bytes(rows, products)));
         } else {
             piece = std::min(piece, of(XE_PART_BYTES, (size_t)rows * sizeof(float2)) * 64);   // (a line for every 64 classes at most)
             take(mine, (size_t)rows * sizeof(float));

@@ -135,7 +135,7 @@ struct LgSpace {
         take(q, (size_t)m * ldk * 2);
         take(columns, (size_t)LG_SLABS * n * sizeof(float));
         take(factor, (size_t)n * 2 * sizeof(float));
-        take(lines, (size_t)mm16_split_floats_most(n, k, m, (int)parts) * sizeof(float));
+        take(lines, mm16_lines_bytes(m, (int)parts));
     }
 };
 

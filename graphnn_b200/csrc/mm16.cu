@@ -7,7 +7,12 @@
 //
 // The matrix instructions cut what they add to an accumulator instead of rounding it: over a long k a sum comes out too small by half a step of fp32 an
 // instruction (loss of a token over k = 4096: 4.7e-6 off, relative; 2.7e-7 with fp32 units).  So an accumulator takes MM_CHUNK panels only, and the
-// epilogue warps, which would wait otherwise, add them up in registers, rounded.
+// epilogue warps, which would wait otherwise, add them up in registers, rounded.  The tensor cores go on with the next tile's first two accumulators while a tile's
+// outputs leave: with four panels each that is too short for 256 x 256 of them (4096 x 131072 x 2048, sums: 1.81 ms; eight panels 1.70, sixteen 1.66).
+//
+// Tiles that are left over when every unit has had its last full turn are cut along k, so that all units share them; their parts' sums go through memory
+// and a second kernel.
+#include <algorithm>
 #include <cstring>
 
 #include "mm16.cuh"
@@ -23,7 +28,8 @@ constexpr int MM_THREADS = 32 * (4 + MM_EPI);
 // 128 * (40 + 2 * 232) = 384 * 168.
 constexpr int MM_REGS = 168;
 constexpr int MM_K = 64;                       // numbers along k of a panel
-constexpr int MM_CHUNK = 4;                    // panels that an accumulator takes
+constexpr int MM_CHUNK = 8, MM_CHUNK_16 = 32;   // panels that an accumulator takes; where the outputs are 16-bit numbers
+constexpr int MM_PIECE = 64, MM_BOX = 32 * MM_PIECE, MM_BOXES = 2;   // bytes of an output row that an epilogue warp hands over at a time; of its 32 rows; boxes of a warp
 constexpr uint32_t MM_BLOCK = 64 * 128;        // bytes of 64 rows of k by 64 numbers across
 
 template <int BN, bool PAIR> struct MmCfg {
@@ -32,14 +38,15 @@ template <int BN, bool PAIR> struct MmCfg {
     static constexpr int STAGES = 6, ACCS = 2;
     static constexpr uint32_t TM_COLS = ACCS * BN;
     enum { FULL = 0, EMPTY = FULL + STAGES, DONE = EMPTY + STAGES, READ = DONE + ACCS, BARS = READ + ACCS };
-    static constexpr uint32_t OFF_BAR = STAGES * STAGE, OFF_MISC = OFF_BAR + 8 * BARS, SMEM = OFF_MISC + 16 + 1024;   // + slack to align the base to 1024 bytes
+    static constexpr uint32_t OFF_OUT = STAGES * STAGE, OFF_BAR = OFF_OUT + MM_EPI * MM_BOXES * MM_BOX, OFF_MISC = OFF_BAR + 8 * BARS, SMEM = OFF_MISC + 16 + 1024;   // + slack to align the base to 1024 bytes
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
 struct MmArgs {
     int64_t m, n;
-    int m_tiles, n_tiles, splits;
-    int steps, per_split;               // panels of a tile, all parts' products; of a share
+    int m_tiles, n_tiles;
+    int full, rest, splits;             // tiles by one unit each; the others, and the shares of k of each of them
+    int steps, per_split, chunk;        // panels of a tile, all parts' products; of a share; of an accumulator
     int products, last_mmas;            // products of parts; instructions of a panel at the end of k
     uint32_t a_parts, b_parts;          // four bits a product
     int a_boxes, b_boxes;               // boxes of an operand that lies across
@@ -64,9 +71,9 @@ struct MmArgs {
     const float* fix;
     const void* fix_w;
     int64_t fix_ld;
-    int fix_wide;
+    int fix_wide;                       // rows of fix_w lie on 16-byte boundaries
     int64_t ldo;
-    int out_type, wide;                 // wide: rows of `out` (fix_wide: of fix_w) lie on 16-byte boundaries
+    int out_type, boxes;                // boxes: the output has a tensor map (rows on 16-byte boundaries)
     s2v_device_status* status;
 };
 
@@ -169,28 +176,64 @@ template <typename T> __device__ __forceinline__ void mm_add_row(const T* p, flo
         }
     }
 }
-template <typename T> __device__ __forceinline__ void mm_store_row(T* p, const float* y, int cols, bool wide)
+// 32 outputs of each of the warp's 32 rows, a row a lane, as boxes of 64-byte rows whose 16-byte pieces are exchanged by the 64-byte swizzle (which keeps the
+// stores free of bank conflicts), and from there by one copy, or, where rows don't lie on 16-byte boundaries, by 16 lanes a row.  (A lane's own stores along
+// its row: 50021 x 1021 of fp16 over 1531 rows, rows at odd places, 569 us.)
+template <typename T> __device__ __forceinline__ void mm_write(const MmArgs& a, const CUtensorMap* map, unsigned char* boxes, int& turn, int64_t row0, int64_t col, int n, const float* y)
 {
-    constexpr int N = PIECE<T>;
-    if (wide) {
+    constexpr int COLS = MM_PIECE / sizeof(T), PER = 16 / sizeof(T);
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-        for (int c = 0; c < 32; c += N) {
-            if (c + N <= cols) *reinterpret_cast<uint4*>(p + c) = pack_piece(y + c, T());
-            else {
+    for (int c = 0; c < 32; c += COLS) {
+        if (c >= n) break;
+        unsigned char* const box = boxes + turn * MM_BOX;
+        turn = (turn + 1) % MM_BOXES;
+        // the copy that last read this box has done so: of the groups since then, one a box, as many may be under way as there are other boxes
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(MM_BOXES - 1) : "memory");
+        __syncwarp();
 #pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (c + e < cols) p[c + e] = from_f32<T>(y[c + e]);
+        for (int p = 0; p < 4; ++p) *reinterpret_cast<uint4*>(box + lane * MM_PIECE + 16 * (p ^ (lane >> 1 & 3))) = pack_piece(y + c + p * PER, T());
+        // (a copy that meets the end of a row inside 16 bytes writes zeros behind it, into what may be somebody else's)
+        if (a.boxes && (col + c + COLS <= a.n || a.n % PER == 0)) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tma_store_2d(map, (int)(col + c), (int)row0, smem_u32(box));
+        } else {
+            // a word of four bytes a lane; in a row of 16-bit numbers at an odd place a lane writes the second half of its word with the first half of its
+            // neighbour's, the first lane the first number and the last lane the last one
+            __syncwarp();
+            const int l = lane & 15, hi = lane >> 4;
+            const int cols = (int)min((int64_t)COLS, a.n - col - c), rows = (int)min((int64_t)32, a.m - row0);
+#pragma unroll 4
+            for (int r = hi; r < 32; r += 2) {
+                T* const at = static_cast<T*>(a.out) + (row0 + r) * a.ldo + col + c;
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(box + r * MM_PIECE + 16 * ((l >> 2) ^ (r >> 1 & 3)) + 4 * (l & 3));
+                if constexpr (sizeof(T) == 4) {
+                    if (r < rows && l < cols) *reinterpret_cast<uint32_t*>(at + l) = w;
+                } else {
+                    uint16_t* const h = reinterpret_cast<uint16_t*>(at) + 2 * l;
+                    const uint32_t next = __shfl_down_sync(0xffffffffu, w, 1);
+                    if (r < rows) {
+                        if ((reinterpret_cast<uintptr_t>(h) & 2) == 0) {
+                            if (2 * l + 1 < cols) *reinterpret_cast<uint32_t*>(h) = w;
+                            else if (2 * l < cols) h[0] = (uint16_t)w;
+                        } else {
+                            if (l < 15 && 2 * l + 2 < cols) *reinterpret_cast<uint32_t*>(h + 1) = __byte_perm(w, next, 0x5432);
+                            else if (2 * l + 1 < cols) h[1] = (uint16_t)(w >> 16);
+                            if (l == 0) h[0] = (uint16_t)w;
+                        }
+                    }
+                }
             }
+            // among copies a piece is a bulk group in any case: the wait before a box is filled counts groups, and this one's turn is over like a copy's
+            if (a.boxes && lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            __syncwarp();
         }
-    } else {
-#pragma unroll
-        for (int c = 0; c < 32; ++c)
-            if (c < cols) p[c] = from_f32<T>(y[c]);
     }
 }
 
 template <int KIND, int BN, bool PAIR>
-__global__ void __launch_bounds__(MM_THREADS, 1) mm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const MmArgs a)
+__global__ void __launch_bounds__(MM_THREADS, 1) mm16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c, const MmArgs a)
 {
     using Cfg = MmCfg<BN, PAIR>;
     constexpr int STAGES = Cfg::STAGES, ACCS = Cfg::ACCS, CTAS = PAIR ? 2 : 1;
@@ -202,7 +245,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) mm16_kernel(const __grid_consta
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + Cfg::OFF_MISC);
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_MISC + 8);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tiles = a.m_tiles * a.n_tiles, items = tiles * a.splits;
+    const int items = a.full + a.rest * a.splits;
     const int rank = PAIR ? (int)(blockIdx.x & 1) : 0, unit = (int)blockIdx.x / CTAS, units = (int)gridDim.x / CTAS;
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) tc_mbar_init(bar(Cfg::FULL + i), 1), tc_mbar_init(bar(Cfg::EMPTY + i), 1);
@@ -225,11 +268,11 @@ __global__ void __launch_bounds__(MM_THREADS, 1) mm16_kernel(const __grid_consta
     if constexpr (PAIR) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // both CTAs' barriers are there
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
-    // an item: a tile and a share [from, to) of its panels
+    // an item: a tile and all of its panels, or a share [from, to) of them
     const auto item_of = [&](int item, int& tm, int& tn, int& from, int& to) {
-        const int split = item / tiles;
-        tc_tile(item - split * tiles, a.m_tiles, a.n_tiles, tm, tn);
-        from = split * a.per_split, to = min(a.steps, from + a.per_split);
+        const int over = item - a.full, split = over < 0 ? 0 : over / a.rest;
+        tc_tile(over < 0 ? item : a.full + over - split * a.rest, a.m_tiles, a.n_tiles, tm, tn);
+        from = over < 0 ? 0 : split * a.per_split, to = over < 0 ? a.steps : min(a.steps, from + a.per_split);
     };
 
     if (warp < 4) {
@@ -279,7 +322,8 @@ __global__ void __launch_bounds__(MM_THREADS, 1) mm16_kernel(const __grid_consta
             int tm, tn, from, to;
             item_of(item, tm, tn, from, to);
             for (int step = from, acc = 0; step < to; ++step, ++it) {
-                const bool first = (step - from) % MM_CHUNK == 0, last = (step - from) % MM_CHUNK == MM_CHUNK - 1 || step + 1 == to;   // of an accumulator
+                const int at = (step - from) & (a.chunk - 1);
+                const bool first = at == 0, last = at + 1 == a.chunk || step + 1 == to;   // of an accumulator
                 if (first) {
                     acc = t % ACCS;
                     if (t >= ACCS && !(ok = PAIR ? tc_wait_pair<false>(bar(Cfg::READ + acc), (uint32_t)(t / ACCS - 1) & 1u, abort_flag, a.status, 81)
@@ -319,7 +363,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) mm16_kernel(const __grid_consta
         if constexpr (PAIR) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
         constexpr int HALF = BN / 2;
         const int quarter = warp & 3, half = (warp - 4) >> 2;
-        int t = 0;
+        int t = 0, turn = 0;
         bool ok = true;
         for (int item = unit; ok && item < items; item += units) {
             int tm, tn, from, to;
@@ -334,7 +378,9 @@ __global__ void __launch_bounds__(MM_THREADS, 1) mm16_kernel(const __grid_consta
             const int64_t left = row - lane >= a.m ? 0 : a.n - col0;
             const int cols = left < 0 ? 0 : left < HALF ? (int)left : HALF;   // (the same for the warp)
             float y[HALF];
-            for (int step = from; step < to; step += MM_CHUNK, ++t) {
+#pragma unroll
+            for (int j = 0; j < HALF; ++j) y[j] = 0.0f;
+            for (int step = from; step < to; step += a.chunk, ++t) {
                 const int acc = t % ACCS;
                 if (!(ok = PAIR ? tc_wait_pair<false>(bar(Cfg::DONE + acc), (uint32_t)(t / ACCS) & 1u, abort_flag, a.status, 83)
                                 : tc_wait(bar(Cfg::DONE + acc), (uint32_t)(t / ACCS) & 1u, abort_flag, a.status, 83)))
@@ -350,7 +396,10 @@ __global__ void __launch_bounds__(MM_THREADS, 1) mm16_kernel(const __grid_consta
                     tc_wait_loads(now);
                     if (c + 16 < cols) tc_ld_cols16(at + (uint32_t)(c + 16), v[~(c / 16) & 1]);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) y[c + j] = step > from ? y[c + j] + __uint_as_float(now[j]) : __uint_as_float(now[j]);
+                    for (int j = 0; j < 16; j += 2)
+                        asm("{\n\t.reg .b64 s, v;\n\tmov.b64 s, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tadd.rn.f32x2 s, s, v;\n\tmov.b64 {%0, %1}, s;\n\t}"
+                            : "+f"(y[c + j]), "+f"(y[c + j + 1])
+                            : "f"(__uint_as_float(now[j])), "f"(__uint_as_float(now[j + 1])));
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
@@ -405,37 +454,52 @@ __global__ void __launch_bounds__(MM_THREADS, 1) mm16_kernel(const __grid_consta
                                 mm_store32(to_g + p * a.g_part, h), mm_store32(to_g + p * a.g_part + 16, h + 8);
                             }
                     }
-                } else if (row < a.m) {
-                    const bool finished = a.splits == 1;
-                    const float alpha = finished && a.alpha ? a.alpha[a.alpha_rows ? row : 0] : 1.0f;
+                } else {
+                    const bool whole = item < a.full;
+                    if (whole) {
+                        if (row < a.m) {
+                            const float alpha = a.alpha ? a.alpha[a.alpha_rows ? row : 0] : 1.0f;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) now[j] *= alpha;
-                    float* const s = finished ? a.sum + row * a.pitch + col0 + c : a.lines + ((int64_t)(item / tiles) * a.m + row) * a.pitch + col0 + c;
-                    if (finished && a.add) {
+                            for (int j = 0; j < 32; ++j) now[j] *= alpha;
+                            if (a.add) {
+                                const float* const s = a.sum + row * a.pitch + col0 + c;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (j < n) now[j] += s[j];
-                    }
-                    if (finished && a.fix) {
-                        const float f = a.fix[row];
-                        if (f != 0.0f) {   // (of a row that is left out it is 0)
-                            const int64_t from = a.target[row] * a.fix_ld + col0 + c;
-                            if (a.out_type == S2V_F16) mm_add_row(static_cast<const __half*>(a.fix_w) + from, f, now, n, a.fix_wide);
-                            else mm_add_row(static_cast<const __nv_bfloat16*>(a.fix_w) + from, f, now, n, a.fix_wide);
+                                for (int j = 0; j < 32; j += 4)
+                                    if (j < n) {
+                                        const float4 f = *reinterpret_cast<const float4*>(s + j);   // (rows of a multiple of 8)
+                                        now[j] += f.x, now[j + 1] += f.y, now[j + 2] += f.z, now[j + 3] += f.w;
+                                    }
+                            }
+                            if (a.fix) {
+                                const float f = a.fix[row];
+                                if (f != 0.0f) {   // (of a row that is left out it is 0)
+                                    const int64_t from_w = a.target[row] * a.fix_ld + col0 + c;
+                                    if (a.out_type == S2V_F16) mm_add_row(static_cast<const __half*>(a.fix_w) + from_w, f, now, n, a.fix_wide);
+                                    else mm_add_row(static_cast<const __nv_bfloat16*>(a.fix_w) + from_w, f, now, n, a.fix_wide);
+                                }
+                            }
+                        }
+                        if (a.out) {
+                            unsigned char* const boxes = smem + Cfg::OFF_OUT + (warp - 4) * MM_BOXES * MM_BOX;
+                            if (a.out_type == S2V_F32) mm_write<float>(a, &map_c, boxes, turn, row - lane, col0 + c, n, now);
+                            else if (a.out_type == S2V_F16) mm_write<__half>(a, &map_c, boxes, turn, row - lane, col0 + c, n, now);
+                            else mm_write<__nv_bfloat16>(a, &map_c, boxes, turn, row - lane, col0 + c, n, now);
                         }
                     }
-                    if (!finished || !a.out) {
+                    if (row < a.m && (!whole || !a.out)) {
+                        float* const s = whole ? a.sum + row * a.pitch + col0 + c
+                                               : a.lines + ((int64_t)(item - a.full) * Cfg::ROWS + (rank * 128 + quarter * 32 + lane)) * BN + half * HALF + c;
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4)
-                            if (j < n) *reinterpret_cast<float4*>(s + j) = make_float4(now[j], now[j + 1], now[j + 2], now[j + 3]);   // (rows of a multiple of 8)
-                    } else if (a.out_type == S2V_F32) mm_store_row(static_cast<float*>(a.out) + row * a.ldo + col0 + c, now, n, a.wide);
-                    else if (a.out_type == S2V_F16) mm_store_row(static_cast<__half*>(a.out) + row * a.ldo + col0 + c, now, n, a.wide);
-                    else mm_store_row(static_cast<__nv_bfloat16*>(a.out) + row * a.ldo + col0 + c, now, n, a.wide);
+                        for (int j = 0; j < 32; j += 8)
+                            if (j < n) mm_store32(s + j, reinterpret_cast<const uint32_t*>(now + j));
+                    }
                 }
             }
             if constexpr (KIND == MM16_SUMS)
                 if (row < a.m) a.part[(int64_t)(2 * tn + half) * a.m + row] = make_float2(sums.m, sums.l);
         }
+        if (B_ACROSS && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -447,36 +511,36 @@ __global__ void __launch_bounds__(MM_THREADS, 1) mm16_kernel(const __grid_consta
     }
 }
 
-// out (or sum) = alpha * the lines of shares of k, added in their order (+ sum)
-__global__ void __launch_bounds__(256) mm16_lines_kernel(const MmArgs a)
+// The tiles that were cut along k: out (or sum) = alpha * the shares' sums, added in their order (+ sum, and what fix gives)
+template <int ROWS, int BN> __global__ void __launch_bounds__(256) mm16_lines_kernel(const MmArgs a)
 {
-    const int64_t per_row = a.pitch / 4, all = a.m * per_row, step = a.m * a.pitch;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / per_row, col = (i - row * per_row) * 4;
-        if (col >= a.n) continue;
-        const float* const from = a.lines + row * a.pitch + col;
-        float y[4] = {};
-        for (int s = 0; s < a.splits; ++s) {
-            const float4 f = *reinterpret_cast<const float4*>(from + s * step);
-            y[0] += f.x, y[1] += f.y, y[2] += f.z, y[3] += f.w;
-        }
-        const float alpha = a.alpha ? a.alpha[a.alpha_rows ? row : 0] : 1.0f;
-        float* const s = a.sum + row * a.pitch + col;
+    constexpr int PER_TILE = ROWS * BN / 4 / 256;   // CTAs
+    const int over = (int)blockIdx.x / PER_TILE, at = ((int)blockIdx.x % PER_TILE * 256 + (int)threadIdx.x) * 4;
+    int tm, tn;
+    tc_tile(a.full + over, a.m_tiles, a.n_tiles, tm, tn);
+    const int64_t row = (int64_t)tm * ROWS + at / BN, col = (int64_t)tn * BN + at % BN;
+    if (row >= a.m || col >= a.n) return;
+    const float* const from = a.lines + (int64_t)over * ROWS * BN + at;
+    float y[4] = {};
+    for (int s = 0; s < a.splits; ++s) {
+        const float4 f = *reinterpret_cast<const float4*>(from + (int64_t)s * a.rest * ROWS * BN);
+        y[0] += f.x, y[1] += f.y, y[2] += f.z, y[3] += f.w;
+    }
+    const float alpha = a.alpha ? a.alpha[a.alpha_rows ? row : 0] : 1.0f, fix = a.fix ? a.fix[row] : 0.0f;
+    float* const s = a.sum + row * a.pitch + col;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (col + e >= a.n) break;
-            y[e] = alpha * y[e] + (a.add ? s[e] : 0.0f);
-            if (a.fix) {
-                const float f = a.fix[row];
-                const int64_t from = f != 0.0f ? a.target[row] * a.fix_ld + col + e : 0;
-                if (f != 0.0f) y[e] = fmaf(f, a.out_type == S2V_F16 ? to_f32(static_cast<const __half*>(a.fix_w)[from]) : to_f32(static_cast<const __nv_bfloat16*>(a.fix_w)[from]), y[e]);
-            }
-            const int64_t at = row * a.ldo + col + e;
-            if (!a.out) s[e] = y[e];
-            else if (a.out_type == S2V_F32) static_cast<float*>(a.out)[at] = y[e];
-            else if (a.out_type == S2V_F16) static_cast<__half*>(a.out)[at] = from_f32<__half>(y[e]);
-            else static_cast<__nv_bfloat16*>(a.out)[at] = from_f32<__nv_bfloat16>(y[e]);
+    for (int e = 0; e < 4; ++e) {
+        if (col + e >= a.n) break;
+        y[e] = alpha * y[e] + (a.add ? s[e] : 0.0f);
+        if (fix != 0.0f) {
+            const int64_t w = a.target[row] * a.fix_ld + col + e;
+            y[e] = fmaf(fix, a.out_type == S2V_F16 ? to_f32(static_cast<const __half*>(a.fix_w)[w]) : to_f32(static_cast<const __nv_bfloat16*>(a.fix_w)[w]), y[e]);
         }
+        const int64_t to = row * a.ldo + col + e;
+        if (!a.out) s[e] = y[e];
+        else if (a.out_type == S2V_F32) static_cast<float*>(a.out)[to] = y[e];
+        else if (a.out_type == S2V_F16) static_cast<__half*>(a.out)[to] = from_f32<__half>(y[e]);
+        else static_cast<__nv_bfloat16*>(a.out)[to] = from_f32<__nv_bfloat16>(y[e]);
     }
 }
 
@@ -546,13 +610,25 @@ bool mm_map(CUtensorMap* map, const mm16_operand& o, int box_rows)
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Whether pairs of CTAs on tiles of 256 x 256: where their tiles fill at least half of the pairs, and either matrix more than half of a tile.
-bool mm_pairs(const s2v_ctx* ctx, int64_t m, int64_t n)
-{
-    const int64_t pairs = ctx->sm_count / 2;
-    return pairs > 0 && m > 128 && n > 128 && ((m + 255) / 256) * ((n + 255) / 256) * 2 >= pairs;
-}
 int mm_products(const mm16_args& a) { return a.a.parts == 1 ? (a.b.parts == 1 ? 1 : 3) : a.b.parts == 1 ? 3 : 6; }
+
+// Whether pairs of CTAs on tiles of 256 x 256: both matrices more than half of a tile, and half of the pairs busy, or enough panels to share out among them.
+bool mm_pairs(const s2v_ctx* ctx, int64_t m, int64_t n, int64_t steps)
+{
+    const int64_t pairs = ctx->sm_count / 2, tiles = ((m + 255) / 256) * ((n + 255) / 256);
+    return pairs > 0 && m > 128 && n > 128 && (tiles * 2 >= pairs || tiles * steps >= 32 * pairs);
+}
+// How the tiles are shared out: the last, incomplete turn in `splits` shares of k each, none below 16 panels (8 where there is no other turn).
+struct MmShares {
+    int64_t full, rest, splits;
+    MmShares(int64_t units, int64_t tiles, int64_t steps)
+    {
+        rest = tiles % units, full = tiles - rest, splits = 1;
+        if (rest) splits = std::min(units / rest, steps / (full ? 16 : 8));
+        if (splits < 2) full = tiles, rest = 0, splits = 1;
+    }
+};
+int64_t mm_steps(const mm16_args& a) { return (a.k + MM_K - 1) / MM_K * mm_products(a); }
 
 template <int KIND, int BN, bool PAIR> int mm_launch(s2v_ctx* ctx, cudaStream_t st, const mm16_args& g)
 {
@@ -566,17 +642,22 @@ template <int KIND, int BN, bool PAIR> int mm_launch(s2v_ctx* ctx, cudaStream_t 
     MmArgs a = {};
     a.m = g.m, a.n = g.n;
     const int64_t mt = (g.m + Cfg::ROWS - 1) / Cfg::ROWS, nt = (g.n + BN - 1) / BN;
-    a.splits = B_ACROSS ? mm16_splits(ctx, g) : 1;
-    if (mt * nt > INT32_MAX / 2 / a.splits) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, "more than 2^30 tiles of outputs");
+    if (mt * nt > INT32_MAX / 2) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, "more than 2^30 tiles of outputs");
     a.m_tiles = (int)mt, a.n_tiles = (int)nt;
     const int64_t kblocks = (g.k + MM_K - 1) / MM_K;
     a.products = mm_products(g);
     // small parts first would gain nothing: the accumulator holds a rounding of its own size either way
     a.a_parts = g.a.parts == 1 ? 0u : g.b.parts == 1 ? 0x210u : 0x201100u;
     a.b_parts = g.b.parts == 1 ? 0u : g.a.parts == 1 ? 0x210u : 0x021010u;
+    if (kblocks * a.products > INT32_MAX / 2) return s2v_fail(ctx, S2V_ERR_UNSUPPORTED, "more than 2^30 panels of k");
     a.steps = (int)kblocks * a.products;
-    a.per_split = (a.steps + a.splits - 1) / a.splits;
+    const int64_t units = std::min(ctx->sm_count, 148) / (PAIR ? 2 : 1);
+    MmShares shares(units, mt * nt, a.steps);
+    if (!B_ACROSS) shares.full = mt * nt, shares.rest = 0, shares.splits = 1;
+    a.full = (int)shares.full, a.rest = (int)shares.rest;
+    a.per_split = (int)((a.steps + shares.splits - 1) / shares.splits);
     a.splits = (a.steps + a.per_split - 1) / a.per_split;
+    a.chunk = KIND == MM16_SUMS || a.products > 1 || (B_ACROSS && g.out_type == S2V_F32) ? MM_CHUNK : MM_CHUNK_16;
     a.last_mmas = (int)((g.k - MM_K * (kblocks - 1) + 15) / 16);
     a.a_boxes = A_ACROSS ? boxes(PAIR || g.m > 128 ? 128 : g.m) : 0, a.b_boxes = B_ACROSS ? boxes(PAIR || g.n > 128 ? 128 : g.n) : 0;
     a.bytes = (A_ACROSS ? (uint32_t)a.a_boxes * MM_BLOCK : (uint32_t)box_a * 128) + (B_ACROSS ? (uint32_t)a.b_boxes * MM_BLOCK : (uint32_t)box_b * 128);
@@ -587,7 +668,11 @@ template <int KIND, int BN, bool PAIR> int mm_launch(s2v_ctx* ctx, cudaStream_t 
     a.g = g.g, a.ldg = g.ldg, a.g_part = g.g_part, a.g_type = g.type, a.g_parts = g.g_parts;
     a.alpha = g.alpha, a.alpha_rows = g.alpha_rows, a.sum = g.sum, a.pitch = mm16_pitch(g.n), a.add = g.add, a.lines = g.lines;
     a.out = g.out, a.ldo = g.ldo, a.out_type = g.out_type;
-    a.wide = s2v_aligned16(g.out) && (g.m <= 1 || g.ldo * (int64_t)s2v_dtype_bytes(g.out_type) % 16 == 0);
+    CUtensorMap map_c;
+    const int64_t es = (int64_t)s2v_dtype_bytes(g.out_type), ldo = g.m > 1 ? g.ldo : (g.n * es + 15) / 16 * 16 / es;
+    a.boxes = g.out && s2v_aligned16(g.out) && ldo * es % 16 == 0;
+    if (!a.boxes) memset(&map_c, 0, sizeof(map_c));
+    else if (!s2v_output_map(&map_c, g.out_type, g.out, g.m, g.n, ldo)) return s2v_fail(ctx, S2V_ERR_CUDA, "the driver did not take the output's tensor map");
     a.fix = g.fix, a.fix_w = g.fix_w, a.fix_ld = g.vocab > 1 ? g.fix_ld : 0;
     a.fix_wide = s2v_aligned16(g.fix_w) && (g.vocab <= 1 || g.fix_ld % 8 == 0);
     a.status = ctx->dstatus_dev;
@@ -599,7 +684,7 @@ template <int KIND, int BN, bool PAIR> int mm_launch(s2v_ctx* ctx, cudaStream_t 
         }();
         if (regs != MM_REGS) return s2v_fail(ctx, S2V_ERR_CUDA, "mm16_kernel was not compiled for the registers that it shares out");
     }
-    const int64_t items = mt * nt * a.splits, units = ctx->sm_count / (PAIR ? 2 : 1);
+    const int64_t items = a.full + (int64_t)a.rest * a.splits;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(items < units ? items : units) * (PAIR ? 2 : 1));
     cfg.blockDim = dim3(MM_THREADS);
@@ -611,11 +696,10 @@ template <int KIND, int BN, bool PAIR> int mm_launch(s2v_ctx* ctx, cudaStream_t 
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    S2V_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, mm16_kernel<KIND, BN, PAIR>, map_a, map_b, a));
+    S2V_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, mm16_kernel<KIND, BN, PAIR>, map_a, map_b, map_c, a));
     S2V_CHECK_LAUNCH(ctx, "mm16_kernel");
-    if (a.splits > 1) {
-        const int64_t blocks = (g.m * (a.pitch / 4) + 255) / 256, cap = 16 * (int64_t)ctx->sm_count;
-        mm16_lines_kernel<<<(unsigned)(blocks < cap ? blocks : cap), 256, 0, st>>>(a);
+    if (a.rest) {
+        mm16_lines_kernel<Cfg::ROWS, BN><<<(unsigned)(a.rest * (Cfg::ROWS * BN / 4 / 256)), 256, 0, st>>>(a);
         S2V_CHECK_LAUNCH(ctx, "mm16_lines_kernel");
     }
     return S2V_OK;
@@ -625,34 +709,21 @@ template <int KIND, int BN, bool PAIR> int mm_launch(s2v_ctx* ctx, cudaStream_t 
 
 int mm16_sum_lines(const s2v_ctx* ctx, int64_t m, int64_t n)
 {
-    const int64_t bn = mm_pairs(ctx, m, n) ? 256 : 128;
+    const int64_t bn = mm_pairs(ctx, m, n, 0) ? 256 : 128;
     return (int)(2 * ((n + bn - 1) / bn));
 }
 int64_t mm16_sum_lines_most(int64_t n) { return 2 * ((n + 127) / 128); }
 
-// Shares of k: as many as there are idle units, none below eight panels.
-int mm16_splits(const s2v_ctx* ctx, const mm16_args& a)
+size_t mm16_lines_bytes(int64_t k, int products)
 {
-    const bool pairs = mm_pairs(ctx, a.m, a.n);
-    const int64_t side = pairs ? 256 : 128, units = pairs ? ctx->sm_count / 2 : ctx->sm_count;
-    const int64_t tiles = ((a.m + side - 1) / side) * ((a.n + side - 1) / side), steps = (a.k + MM_K - 1) / MM_K * mm_products(a);
-    int64_t s = (units < MM16_SPLITS_MOST ? units : MM16_SPLITS_MOST) / tiles;
-    s = s < steps / 8 ? s : steps / 8;
-    return (int)(s < 1 ? 1 : s < MM16_SPLITS_MOST ? s : MM16_SPLITS_MOST);
-}
-int64_t mm16_split_floats_most(int64_t m, int64_t n, int64_t k, int products)
-{
-    const auto tiles = [&](int64_t side) { return ((m + side - 1) / side) * ((n + side - 1) / side); };
-    const int64_t single = MM16_SPLITS_MOST / tiles(128), pairs = MM16_SPLITS_MOST / 2 / tiles(256), steps = (k + MM_K - 1) / MM_K * products / 8;
-    int64_t s = single > pairs ? single : pairs;   // of either form
-    s = s < steps ? s : steps;
-    return s > 1 ? s * m * mm16_pitch(n) : 0;
+    // a share of a tile of 256 x 256 for each of 74 pairs (as much as of 128 x 128 for each of 148 CTAs, twice over); none where k is too short to be shared out
+    return (k + MM_K - 1) / MM_K * products < 16 ? 0 : (size_t)74 * 256 * 256 * sizeof(float);
 }
 
 int mm16_launch(s2v_ctx* ctx, cudaStream_t st, mm16_kind kind, const mm16_args& a)
 {
     if (a.m == 0 || a.n == 0) return S2V_OK;
-    const bool pairs = mm_pairs(ctx, a.m, a.n);
+    const bool pairs = mm_pairs(ctx, a.m, a.n, kind == MM16_OUT || kind == MM16_OUT_ACROSS ? mm_steps(a) : 0);
     switch (kind) {
         case MM16_SUMS: return pairs ? mm_launch<MM16_SUMS, 256, true>(ctx, st, a) : mm_launch<MM16_SUMS, 128, false>(ctx, st, a);
         case MM16_SOFTMAX_GRAD: return pairs ? mm_launch<MM16_SOFTMAX_GRAD, 256, true>(ctx, st, a) : mm_launch<MM16_SOFTMAX_GRAD, 128, false>(ctx, st, a);

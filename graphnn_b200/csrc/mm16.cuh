@@ -39,7 +39,7 @@ struct mm16_args {
     const float* fix = nullptr;         // [m] or NULL: out gets fix_i times row target_i of fix_w ([vocab x n], of out_type) too
     const void* fix_w = nullptr;
     int64_t fix_ld = 0;
-    float* lines = nullptr;             // [splits][m x mm16_pitch(n)] where k is shared out
+    float* lines = nullptr;             // mm16_lines_bytes(): sums of shares of k
     int out_type = S2V_F32;
     void* out = nullptr;
     int64_t ldo = 0;
@@ -49,9 +49,7 @@ enum mm16_kind { MM16_SUMS, MM16_SOFTMAX_GRAD, MM16_OUT, MM16_OUT_ACROSS };   //
 inline int64_t mm16_pitch(int64_t n) { return (n + 7) / 8 * 8; }
 int mm16_sum_lines(const s2v_ctx* ctx, int64_t m, int64_t n);                     // as the launch will write them
 int64_t mm16_sum_lines_most(int64_t n);                                           // the most of any launch
-constexpr int MM16_SPLITS_MOST = 148;
-int mm16_splits(const s2v_ctx* ctx, const mm16_args& a);                          // shares of k (MM16_OUT, MM16_OUT_ACROSS)
-int64_t mm16_split_floats_most(int64_t m, int64_t n, int64_t k, int products);    // of `lines`; products: of parts, 1, 3 or 6
+size_t mm16_lines_bytes(int64_t k, int products);                                 // of `lines`; products: of parts, 1, 3 or 6
 int mm16_launch(s2v_ctx* ctx, cudaStream_t st, mm16_kind kind, const mm16_args& a);
 
 // Rows of x as 16-bit parts (1 or 3), zeros where a target leaves the row out (target NULL: none); columns up to the next multiple of 8 are filled with zeros.
