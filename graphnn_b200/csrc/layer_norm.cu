@@ -6,6 +6,8 @@
 // Gradient: the same places of a row in every turn of a thread, which so sums its columns of the weight's and the bias's gradient in registers over all
 // the rows that it takes; a CTA leaves one line of sums, and a second kernel adds the lines in their order.
 #include "quantize.cuh"
+#include "tcgen05.cuh"
+#include "tma.cuh"
 
 namespace
 {
@@ -204,6 +206,147 @@ __global__ void __launch_bounds__(THREADS < LN_CTA ? LN_CTA : THREADS)
     }
 }
 
+// ---- rows through a ring in shared memory
+constexpr int LN_STAGES = 8;   // at most
+
+struct ln_ring {
+    uint32_t base, full;       // shared addresses: stages, barriers
+    unsigned char* at;
+    volatile int* abort_flag;
+    int stages, bytes;         // of a stage
+    __device__ __forceinline__ ln_ring(unsigned char* raw, int stages_, int bytes_) : stages(stages_), bytes(bytes_)
+    {
+        at = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 127) & ~(uintptr_t)127);
+        base = smem_u32(at), full = base + (uint32_t)(stages * bytes);
+        abort_flag = reinterpret_cast<volatile int*>(at + stages * bytes + 8 * LN_STAGES);
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < stages; ++i) tc_mbar_init(full + 8 * i, 1);
+            *abort_flag = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncthreads();
+    }
+    // by one thread: `n` bytes (a multiple of 16) to a stage, behind `offset`
+    __device__ __forceinline__ void copy(int stage, int offset, const void* from, int n) const
+    {
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(base + (uint32_t)(stage * bytes + offset)), "l"(from), "r"(n),
+                     "r"(full + 8 * stage)
+                     : "memory");
+    }
+    __device__ __forceinline__ bool wait(int turn, s2v_device_status* status) const { return tc_wait(full + 8 * (turn % stages), (uint32_t)(turn / stages) & 1u, abort_flag, status, 90); }
+    // where a wait gave up: copies under way, before the CTA goes
+    __device__ __forceinline__ void drain(int from, int to) const
+    {
+        if (threadIdx.x == 0)
+            for (int i = from; i < to; ++i) {
+                int spins = 0;
+                while (!tc_mbar_try(full + 8 * (i % stages), (uint32_t)(i / stages) & 1u))
+                    if (++spins > TC_WAIT_LIMIT) break;
+            }
+    }
+    static size_t shared(int stages, int bytes) { return 128 + (size_t)stages * bytes + 8 * LN_STAGES + 16; }
+};
+
+struct LnNorm {
+    int64_t rows, cols, ldx, ldy, ldq;
+    const void* x;
+    const float* weight;
+    const float* bias;
+    float eps;
+    void* y;
+    float2* stats;
+    int8_t* q;
+    float* q_scale;
+    int stages, bytes;
+    s2v_device_status* status;
+};
+
+// A row a CTA, NV pieces a thread; one barrier a row, behind which the stage of the row before is free.
+template <typename T, int NV, int THREADS, int CTAS> __global__ void __launch_bounds__(THREADS, CTAS) layer_norm_ring_kernel(const LnNorm a)
+{
+    using P = ln_piece<T, true>;
+    constexpr int N = P::N, WARPS = THREADS / 32;
+    __shared__ float4 part[2][WARPS];
+    extern __shared__ unsigned char ln_raw[];
+    const ln_ring ring(ln_raw, a.stages, a.bytes);
+    const int at = threadIdx.x, pieces = (int)(a.cols / N), row_bytes = (int)(a.cols * (int64_t)sizeof(T));
+    const int turns = (int)((a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x);
+    const auto fetch = [&](int turn) {
+        if (turn < turns) {
+            mbar_expect(ring.full + 8 * (turn % a.stages), (uint32_t)row_bytes);
+            ring.copy(turn % a.stages, 0, static_cast<const T*>(a.x) + ((int64_t)blockIdx.x + (int64_t)turn * gridDim.x) * a.ldx, row_bytes);
+        }
+    };
+    if (at == 0)
+        for (int i = 0; i < a.stages; ++i) fetch(i);
+    float w[NV * N], b[NV * N];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        if (j * THREADS + at < pieces) P::columns(a.weight, j * THREADS + at, 1.0f, w + j * N), P::columns(a.bias, j * THREADS + at, 0.0f, b + j * N);
+    }
+    int i = 0;
+    bool failed = false;
+    for (; i < turns; ++i) {
+        const int64_t r = (int64_t)blockIdx.x + (int64_t)i * gridDim.x;
+        const bool ok = ring.wait(i, a.status);
+        const uint4* const row = reinterpret_cast<const uint4*>(ring.at + (i % a.stages) * a.bytes);
+        float f[NV * N], sum = 0.0f;
+        int count = 0;
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * THREADS + at < pieces) {
+                const uint4 v = row[j * THREADS + at];
+                P::unpack(v, f + j * N);
+                if (a.q) top = max(top, P::largest(v));
+#pragma unroll
+                for (int e = 0; e < N; ++e) sum += f[j * N + e];
+                count += N;
+            }
+        ln_moments m{(float)count, count ? sum / (float)count : 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * THREADS + at < pieces)
+#pragma unroll
+                for (int e = 0; e < N; ++e) m.m2 = fmaf(f[j * N + e] - m.mean, f[j * N + e] - m.mean, m.m2);
+        m.join_lanes<32>();
+        top = __reduce_max_sync(0xffffffffu, top);
+        if ((at & 31) == 0) part[i & 1][at >> 5] = make_float4(m.n, m.mean, m.m2, __uint_as_float(top));
+        if (__syncthreads_or(!ok)) {
+            failed = true;
+            break;
+        }
+        if (at == 0 && i > 0) fetch(i - 1 + a.stages);
+        m = ln_moments{0.0f, 0.0f, 0.0f};
+        top = 0;
+#pragma unroll
+        for (int k = 0; k < WARPS; ++k) {
+            const float4 o = part[i & 1][k];
+            m.join(o.x, o.y, o.z);
+            top = max(top, __float_as_uint(o.w));
+        }
+        const float rstd = 1.0f / sqrtf(m.m2 / m.n + a.eps);
+        const q_row k(top);
+        T* const yr = static_cast<T*>(a.y) + r * a.ldy;
+        int8_t* const qr = a.q + r * a.ldq;
+        const bool whole = (reinterpret_cast<uintptr_t>(qr) & (N - 1)) == 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * THREADS + at < pieces) {
+                if (a.q) P::quantize(qr, j * THREADS + at, whole, row[j * THREADS + at], k);
+                float o[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) o[e] = fmaf((f[j * N + e] - m.mean) * rstd, w[j * N + e], b[j * N + e]);
+                P::store(yr, j * THREADS + at, o);
+            }
+        if (at == 0) {
+            if (a.stats) a.stats[r] = make_float2(m.mean, rstd);
+            if (a.q) a.q_scale[r] = k.scale;
+        }
+    }
+    if (failed) ring.drain(i, min(turns, max(i, 1) - 1 + a.stages));
+}
+
 // What the gradient takes its normalised rows from: x, or 8-bit rows with scales.
 struct LnGrad {
     int64_t rows, cols, lddy, ldx, lddx;
@@ -216,6 +359,8 @@ struct LnGrad {
     void* dx;
     float* lines;           // [CTAs][2][cols]: sums of dy xh and of dy
     int columns;            // whether these are wanted
+    int stages, bytes;      // of the ring
+    s2v_device_status* status;
 };
 
 template <typename T, bool VEC, int NV, int THREADS, bool FROM8>
@@ -323,6 +468,106 @@ __global__ void __launch_bounds__(THREADS < LN_CTA ? LN_CTA : THREADS) layer_nor
     }
 }
 
+// The same through the ring, a row a CTA: a stage holds the row's dy and, behind it, x or the 8-bit row.
+template <typename T, int NV, int THREADS, int CTAS, bool FROM8> __global__ void __launch_bounds__(THREADS, CTAS) layer_norm_grad_ring_kernel(const LnGrad a)
+{
+    using P = ln_piece<T, true>;
+    constexpr int N = P::N, WARPS = THREADS / 32;
+    __shared__ float2 part[2][WARPS];
+    extern __shared__ unsigned char ln_raw[];
+    const ln_ring ring(ln_raw, a.stages, a.bytes);
+    const int at = threadIdx.x, pieces = (int)(a.cols / N), row_bytes = (int)(a.cols * (int64_t)sizeof(T)), x_bytes = FROM8 ? (int)a.cols : row_bytes;
+    const int turns = (int)((a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x);
+    const auto fetch = [&](int turn) {
+        if (turn < turns) {
+            const int64_t r = (int64_t)blockIdx.x + (int64_t)turn * gridDim.x;
+            mbar_expect(ring.full + 8 * (turn % a.stages), (uint32_t)(row_bytes + x_bytes));
+            ring.copy(turn % a.stages, 0, static_cast<const T*>(a.dy) + r * a.lddy, row_bytes);
+            if constexpr (FROM8) ring.copy(turn % a.stages, row_bytes, a.q + r * a.ldx, x_bytes);
+            else ring.copy(turn % a.stages, row_bytes, static_cast<const T*>(a.x) + r * a.ldx, x_bytes);
+        }
+    };
+    if (at == 0)
+        for (int i = 0; i < a.stages; ++i) fetch(i);
+    float sum_w[NV * N] = {}, sum_b[NV * N] = {};
+    const float inv = 1.0f / (float)a.cols;
+    int i = 0;
+    bool failed = false;
+    float2 next_st = a.stats[blockIdx.x];
+    float next_s = FROM8 ? a.q_scale[blockIdx.x] : 1.0f;
+    for (; i < turns; ++i) {
+        const int64_t r = (int64_t)blockIdx.x + (int64_t)i * gridDim.x;
+        const float2 st = next_st;
+        const float s = next_s;
+        if (i + 1 < turns) {
+            next_st = a.stats[r + gridDim.x];
+            if (FROM8) next_s = a.q_scale[r + gridDim.x];
+        }
+        const bool ok = ring.wait(i, a.status);
+        const uint4* const dyr = reinterpret_cast<const uint4*>(ring.at + (i % a.stages) * a.bytes);
+        const void* const xr = ring.at + (i % a.stages) * a.bytes + row_bytes;
+        const auto load = [&](int p, float* d, float* h, float* w) {   // dy, normalised row and weight of a piece
+            P::unpack(dyr[p], d);
+            if constexpr (FROM8) P::unpack8(static_cast<const typename P::raw8*>(xr)[p], h);
+            else P::unpack(static_cast<const uint4*>(xr)[p], h);
+#pragma unroll
+            for (int e = 0; e < N; ++e) h[e] = FROM8 ? fmaf(h[e], s, -st.x) * st.y : (h[e] - st.x) * st.y;
+            P::columns(a.weight, p, 1.0f, w);
+        };
+        float g0 = 0.0f, g1 = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * THREADS + at < pieces) {
+                float d[N], h[N], w[N];
+                load(j * THREADS + at, d, h, w);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const float g = d[e] * w[e];
+                    g0 += g;
+                    g1 = fmaf(g, h[e], g1);
+                    sum_w[j * N + e] = fmaf(d[e], h[e], sum_w[j * N + e]), sum_b[j * N + e] += d[e];
+                }
+            }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) g0 += __shfl_xor_sync(0xffffffffu, g0, o), g1 += __shfl_xor_sync(0xffffffffu, g1, o);
+        if ((at & 31) == 0) part[i & 1][at >> 5] = make_float2(g0, g1);
+        if (__syncthreads_or(!ok)) {
+            failed = true;
+            break;
+        }
+        if (at == 0 && i > 0) fetch(i - 1 + a.stages);
+        g0 = g1 = 0.0f;
+#pragma unroll
+        for (int k = 0; k < WARPS; ++k) g0 += part[i & 1][k].x, g1 += part[i & 1][k].y;
+        const float m0 = g0 * inv, m1 = g1 * inv;
+        T* const dxr = static_cast<T*>(a.dx) + r * a.lddx;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j * THREADS + at < pieces) {
+                float d[N], h[N], w[N];
+                load(j * THREADS + at, d, h, w);
+#pragma unroll
+                for (int e = 0; e < N; ++e) d[e] = st.y * (fmaf(d[e], w[e], -m0) - h[e] * m1);
+                P::store(dxr, j * THREADS + at, d);
+            }
+    }
+    if (failed) {
+        ring.drain(i, min(turns, max(i, 1) - 1 + a.stages));
+        return;
+    }
+    if (!a.columns) return;
+    float* const line = a.lines + (int64_t)blockIdx.x * 2 * a.cols;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+        if (j * THREADS + at < pieces)
+#pragma unroll
+            for (int e = 0; e < N; e += 4) {
+                const int c = (j * THREADS + at) * N + e;
+                *reinterpret_cast<float4*>(line + c) = make_float4(sum_w[j * N + e], sum_w[j * N + e + 1], sum_w[j * N + e + 2], sum_w[j * N + e + 3]);
+                *reinterpret_cast<float4*>(line + a.cols + c) = make_float4(sum_b[j * N + e], sum_b[j * N + e + 1], sum_b[j * N + e + 2], sum_b[j * N + e + 3]);
+            }
+}
+
 // Rows longer than a CTA's registers: read twice, and a second kernel for the columns' sums.
 template <typename T, bool FROM8> __global__ void __launch_bounds__(512) layer_norm_grad_long_kernel(const LnGrad a)
 {
@@ -368,24 +613,45 @@ template <typename T, bool FROM8> __global__ void __launch_bounds__(LN_CTA) laye
     float* const line = a.lines + (int64_t)blockIdx.y * 2 * a.cols;
     line[c] = w, line[a.cols + c] = b;
 }
-// the lines of the gradient's CTAs, added in their order by 8 threads a column
-__global__ void __launch_bounds__(LN_CTA) layer_norm_lines_kernel(int lines, int64_t cols, const float* __restrict__ from, float* __restrict__ dweight, float* __restrict__ dbias)
+// The lines of the gradient's CTAs, added in a fixed order: V columns a thread, 8 threads' shares of the lines.
+template <int V> __global__ void __launch_bounds__(LN_CTA) layer_norm_lines_kernel(int lines, int64_t cols, const float* __restrict__ from, float* __restrict__ dweight, float* __restrict__ dbias)
 {
-    __shared__ float part[8][33];
-    const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+    __shared__ float part[8][32 * V];
+    const int64_t c = ((int64_t)blockIdx.x * 32 + (threadIdx.x & 31)) * V;
     const int g = threadIdx.x >> 5;
-    float t = 0.0f;
-    if (c < 2 * cols)
-        for (int l = g; l < lines; l += 8) t += from[(int64_t)l * 2 * cols + c];
-    part[g][threadIdx.x & 31] = t;
-    __syncthreads();
-    if (g || c >= 2 * cols) return;
-    t = 0.0f;
+    float t[V] = {};
+    if (c < 2 * cols) {
+#pragma unroll 4
+        for (int l = g; l < lines; l += 8) {
+            if constexpr (V == 4) {
+                const float4 f = __ldcs(reinterpret_cast<const float4*>(from + (int64_t)l * 2 * cols + c));
+                t[0] += f.x, t[1] += f.y, t[2] += f.z, t[3] += f.w;
+            } else t[0] += from[(int64_t)l * 2 * cols + c];
+        }
+    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t += part[i][threadIdx.x & 31];
-    if (c < cols) {
-        if (dweight) dweight[c] = t;
-    } else if (dbias) dbias[c - cols] = t;
+    for (int e = 0; e < V; ++e) part[g][(threadIdx.x & 31) * V + e] = t[e];
+    __syncthreads();
+    if (threadIdx.x >= 32 * V) return;
+    const int64_t k = (int64_t)blockIdx.x * 32 * V + threadIdx.x;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += part[i][threadIdx.x];
+    if (k < cols) {
+        if (dweight) dweight[k] = s;
+    } else if (k < 2 * cols && dbias) dbias[k - cols] = s;
+}
+
+// Stages of a ring for `ctas` CTAs on an SM: what fits, LN_STAGES at most.
+constexpr int LN_RING_ROW = 65536;   // bytes of a row
+constexpr size_t LN_RING_SHARED = 222 * 1024;
+template <typename K, typename A> int ln_ring_stages(s2v_ctx* ctx, K kernel, A& a, int ctas)
+{
+    const size_t fixed = ln_ring::shared(0, 0) + 1024 + 512;   // (what a CTA takes besides, and the kernel's own)
+    a.stages = (int)((LN_RING_SHARED / ctas - fixed) / a.bytes);
+    a.stages = a.stages < LN_STAGES ? a.stages : LN_STAGES;
+    S2V_CUDA_OK(ctx, s2v_allow_shared(kernel, LN_RING_SHARED));
+    return S2V_OK;
 }
 
 template <typename T, bool VEC>
@@ -400,6 +666,25 @@ int ln_launch(s2v_ctx* ctx, cudaStream_t st, int64_t rows, int64_t cols, const T
         S2V_CHECK_LAUNCH(ctx, "layer_norm_kernel");
         return (int)S2V_OK;
     };
+    if constexpr (VEC) {
+        if (pieces > 128 && pieces * 16 <= LN_RING_ROW && rows <= INT32_MAX) {
+            LnNorm a{rows, cols, ldx, ldy, ldq, x, weight, bias, eps, y, stats, q, q_scale, 0, (int)((pieces * 16 + 127) / 128 * 128), ctx->dstatus_dev};
+            const auto ring = [&](auto kernel, int threads, int ctas) {
+                const int rc = ln_ring_stages(ctx, kernel, a, ctas);
+                if (rc != S2V_OK) return rc;
+                const int64_t most = (int64_t)ctas * ctx->sm_count;
+                kernel<<<(unsigned)(rows < most ? rows : most), threads, ln_ring::shared(a.stages, a.bytes), st>>>(a);
+                S2V_CHECK_LAUNCH(ctx, "layer_norm_ring_kernel");
+                return (int)S2V_OK;
+            };
+            constexpr int N = ln_piece<T, true>::N;
+            if (pieces <= 256) return ring(layer_norm_ring_kernel<T, 1, 256, 5>, 256, 5);
+            if (pieces <= 512) return ring(layer_norm_ring_kernel<T, 2, 256, 3>, 256, 3);
+            if (pieces <= 1024) return ring(layer_norm_ring_kernel<T, 4, 256, 2>, 256, 2);
+            if (pieces <= 2048) return ring(layer_norm_ring_kernel<T, 4, 512, 1>, 512, 1);
+            if constexpr (N == 4) return ring(layer_norm_ring_kernel<T, 8, 512, 1>, 512, 1);
+        }
+    }
     if (pieces <= 8) return go(layer_norm_kernel<T, VEC, 1, 8>, 8);
     if (pieces <= 32) return go(layer_norm_kernel<T, VEC, 4, 8>, 8);
     if (pieces <= 128) return go(layer_norm_kernel<T, VEC, 4, 32>, 32);
@@ -424,12 +709,34 @@ template <typename T, bool FROM8> int ln_grad_launch(s2v_ctx* ctx, cudaStream_t 
         S2V_CHECK_LAUNCH(ctx, "layer_norm_grad_kernel");
         return (int)S2V_OK;
     };
+    const auto ring = [&](auto kernel, int threads, int ctas) {
+        LnGrad r = a;
+        r.bytes = (int)((a.cols * (int64_t)(sizeof(T) + (FROM8 ? 1 : sizeof(T))) + 127) / 128 * 128), r.status = ctx->dstatus_dev;
+        const int rc = ln_ring_stages(ctx, kernel, r, ctas);
+        if (rc != S2V_OK) return rc;
+        const int64_t most = (int64_t)ctas * ctx->sm_count;
+        lines = (int)(a.rows < most ? a.rows : most);
+        kernel<<<lines, threads, ln_ring::shared(r.stages, r.bytes), st>>>(r);
+        S2V_CHECK_LAUNCH(ctx, "layer_norm_grad_ring_kernel");
+        return (int)S2V_OK;
+    };
     const auto by_size = [&](auto vector) {
         constexpr bool VEC = decltype(vector)::value;
         constexpr int N = ln_piece<T, VEC>::N;
         const int64_t pieces = a.cols / N;
+        if constexpr (VEC) {
+            // (at least two rows of a CTA in the ring; the 8-bit rows on 16-byte boundaries too)
+            const bool whole = !FROM8 || (a.cols % 16 == 0 && s2v_aligned16(a.q) && (a.rows <= 1 || a.ldx % 16 == 0));
+            if (pieces > 128 && pieces <= 2048 * 8 / N && whole && a.rows <= INT32_MAX && a.cols * (int64_t)(sizeof(T) + (FROM8 ? 1 : sizeof(T))) <= LN_RING_ROW) {
+                if (pieces <= 256) return ring(layer_norm_grad_ring_kernel<T, 1, 256, 4, FROM8>, 256, 4);
+                if (pieces <= 512) return ring(layer_norm_grad_ring_kernel<T, 2, 256, 3, FROM8>, 256, 3);
+                if (pieces <= 1024) return ring(layer_norm_grad_ring_kernel<T, 4, 256, 2, FROM8>, 256, 2);
+                if (pieces <= 2048) return ring(layer_norm_grad_ring_kernel<T, 4, 512, 1, FROM8>, 512, 1);
+                if constexpr (N == 4) return ring(layer_norm_grad_ring_kernel<T, 8, 512, 1, FROM8>, 512, 1);
+            }
+        }
         if (pieces <= 8) return go(layer_norm_grad_kernel<T, VEC, 1, 8, FROM8>, 8, 8 * N);
-        if (pieces <= 32) return go(layer_norm_grad_kernel<T, VEC, VEC ? 1 : 4, VEC ? 32 : 8, FROM8>, VEC ? 32 : 8, 32 * N);
+        if (pieces <= 32) return go(layer_norm_grad_kernel<T, VEC, 4, 8, FROM8>, 8, 32 * N);
         if (pieces <= 128) return go(layer_norm_grad_kernel<T, VEC, 4, 32, FROM8>, 32, 128 * N);
         if (pieces <= 512) return go(layer_norm_grad_kernel<T, VEC, 2, 256, FROM8>, 256, 0);
         if (pieces <= 1024) return go(layer_norm_grad_kernel<T, VEC, 2, 512, FROM8>, 512, 0);
@@ -453,7 +760,8 @@ template <typename T, bool FROM8> int ln_grad_launch(s2v_ctx* ctx, cudaStream_t 
     };
     const int rc = vec ? by_size(std::true_type()) : by_size(std::false_type());
     if (rc != S2V_OK || !a.columns) return rc;
-    layer_norm_lines_kernel<<<(unsigned)((2 * a.cols + 31) / 32), LN_CTA, 0, st>>>(lines, a.cols, a.lines, dweight, dbias);
+    if (a.cols % 2 == 0) layer_norm_lines_kernel<4><<<(unsigned)((2 * a.cols + 127) / 128), LN_CTA, 0, st>>>(lines, a.cols, a.lines, dweight, dbias);
+    else layer_norm_lines_kernel<1><<<(unsigned)((2 * a.cols + 31) / 32), LN_CTA, 0, st>>>(lines, a.cols, a.lines, dweight, dbias);
     S2V_CHECK_LAUNCH(ctx, "layer_norm_lines_kernel");
     return S2V_OK;
 }
@@ -528,7 +836,7 @@ int s2v_layer_norm_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t c
         if (!workspace || workspace_bytes < s2v_layer_norm_grad_workspace_bytes(rows, cols)) return bad(S2V_ERR_WORKSPACE, "workspace too small");
         if (!s2v_aligned16(workspace)) return bad(S2V_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
     }
-    LnGrad a{rows, cols, lddy, x ? ldx : ldq, lddx, dy, x, q, q_scale, reinterpret_cast<const float2*>(stats), weight, dx, static_cast<float*>(workspace), dweight || dbias};
+    LnGrad a{rows, cols, lddy, x ? ldx : ldq, lddx, dy, x, q, q_scale, reinterpret_cast<const float2*>(stats), weight, dx, static_cast<float*>(workspace), dweight || dbias, 0, 0, nullptr};
     const int64_t n = 16 / es;
     const bool vec = cols % n == 0 && rows_aligned(dy, rows, lddy, es, 16) && rows_aligned(dx, rows, lddx, es, 16) &&
                      (x ? rows_aligned(x, rows, ldx, es, 16) : rows_aligned(q, rows, ldq, 1, n));
