@@ -1,10 +1,11 @@
 // Layer norm of rows, its gradient, and the 8-bit rows that a training step keeps between the two instead of its input.
 //
-// Forward: a row by 8 lanes, a warp or a CTA, held in registers between its moments and its outputs.  Deviations are summed around each thread's own mean and
-// the moments of threads joined by  M2 = M2a + M2b + (mb - ma)^2 na nb / (na + nb),  so that one exchange among a row's threads gives both moments without the
+// Forward: a row by 8 lanes, a warp or a CTA, held in registers between its moments and its outputs.  Deviations are summed around the mean of the lanes or the warp,
+// and a CTA's warps joined by  sum (x - mean)^2 = sum over warps of (M2_w + n_w (mean_w - mean)^2),  so that one barrier a row gives both moments, without the
 // cancellation of E x^2 - (E x)^2.
 // Gradient: the same places of a row in every turn of a thread, which so sums its columns of the weight's and the bias's gradient in registers over all
 // the rows that it takes; a CTA leaves one line of sums, and a second kernel adds the lines in their order.
+#include "f32x2.cuh"
 #include "quantize.cuh"
 #include "tcgen05.cuh"
 #include "tma.cuh"
@@ -75,31 +76,25 @@ template <typename T, bool VEC> struct ln_piece {
     }
 };
 
-// n numbers with their mean and the sum of their squared deviations from it
-struct ln_moments {
-    float n, mean, m2;
-    __device__ __forceinline__ void join(float nb, float mb, float m2b)
-    {
-        const float sum = n + nb;
-        if (nb == 0.0f) return;
-        const float share = nb / sum, d = mb - mean;
-        mean = n == 0.0f ? mb : fmaf(d, share, mean);
-        m2 = m2 + m2b + (n == 0.0f ? 0.0f : d * d * (n * share));
-        n = sum;
-    }
-    template <int LANES> __device__ __forceinline__ void join_lanes()
-    {
+template <int LANES> __device__ __forceinline__ float ln_lanes_sum(float v)
+{
 #pragma unroll
-        for (int o = 1; o < LANES; o <<= 1) {
-            // both sides compute the same numbers: the lower lane's come first
-            const float nb = __shfl_xor_sync(0xffffffffu, n, o), mb = __shfl_xor_sync(0xffffffffu, mean, o), qb = __shfl_xor_sync(0xffffffffu, m2, o);
-            const bool second = threadIdx.x & o;
-            ln_moments a{second ? nb : n, second ? mb : mean, second ? qb : m2};
-            a.join(second ? n : nb, second ? mean : mb, second ? m2 : qb);
-            *this = a;
-        }
+    for (int o = LANES / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// Mean and sum of squared deviations of a row from its warps' (sum, sum of squared deviations from the warp's mean, 1 / count, count).
+template <int WARPS> __device__ __forceinline__ void ln_join(const float2* part, const float2* counts, float inv, float& mean, float& m2)
+{
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) sum += part[i].x;
+    mean = sum * inv, m2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+        const float d = fmaf(part[i].x, counts[i].x, -mean);
+        m2 += fmaf(d * counts[i].y, d, part[i].y);
     }
-};
+}
 
 // THREADS threads a row (8, 32 or a CTA of THREADS), NV pieces of each in registers; a longer row's others (CTAs alone) are read again.
 template <typename T, bool VEC, int NV, int THREADS>
@@ -109,9 +104,18 @@ __global__ void __launch_bounds__(THREADS < LN_CTA ? LN_CTA : THREADS)
 {
     using P = ln_piece<T, VEC>;
     constexpr int N = P::N, CTA = THREADS < LN_CTA ? LN_CTA : THREADS, WARPS = THREADS / 32, GROUPS = CTA / THREADS;
-    __shared__ float4 part[WARPS > 1 ? 2 * WARPS : 1];
+    constexpr int LANES = THREADS < 32 ? THREADS : 32;
+    __shared__ float2 part[WARPS > 1 ? 2 * WARPS : 1], counts[WARPS > 1 ? WARPS : 1];   // of two turns, so that there is one barrier a row
+    __shared__ uint32_t tops[WARPS > 1 ? 2 * WARPS : 1];
     const int at = threadIdx.x % THREADS;
     const int64_t pieces = cols / N;
+    const float inv = 1.0f / (float)cols;
+    float inv_warp = inv;   // 1 / numbers of the lanes that sum around one mean
+    if constexpr (WARPS > 1) {
+        const float n = ln_lanes_sum<32>((float)((pieces - at + THREADS - 1) / THREADS * N));
+        inv_warp = n > 0.0f ? 1.0f / n : 0.0f;
+        if ((at & 31) == 0) counts[at >> 5] = make_float2(inv_warp, n);   // (the first row's barrier is before their first use)
+    }
     int turn = 0;
     for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < rows; first += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
         // (groups behind the last row take it too, but leave nothing: all lanes of a warp exchange)
@@ -119,69 +123,53 @@ __global__ void __launch_bounds__(THREADS < LN_CTA ? LN_CTA : THREADS)
         const bool mine = own < rows;
         const T* const xr = x + r * ldx;
         typename P::raw v[NV];
-        float sum = 0.0f;
-        int count = 0;
+        float sum = 0.0f, m2 = 0.0f;
         uint32_t a = 0;
+        const auto add = [&](const typename P::raw& w) {
+            float f[N];
+            P::unpack(w, f);
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum += f[e];
+        };
 #pragma unroll
         for (int j = 0; j < NV; ++j)
             if (j * THREADS + at < pieces) v[j] = P::load_again(xr, j * THREADS + at);
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-            if (j * THREADS + at < pieces) {
-                float f[N];
-                P::unpack(v[j], f);
-#pragma unroll
-                for (int e = 0; e < N; ++e) sum += f[e];
-                count += N;
-            }
+            if (j * THREADS + at < pieces) add(v[j]);
         if constexpr (WARPS > 1)
-            for (int64_t p = NV * THREADS + at; p < pieces; p += THREADS) {
-                float f[N];
-                P::unpack(P::load_again(xr, p), f);
+            for (int64_t p = NV * THREADS + at; p < pieces; p += THREADS) add(P::load_again(xr, p));
+        sum = ln_lanes_sum<LANES>(sum);
+        float mean = sum * inv_warp;
+        const auto deviate = [&](const typename P::raw& w) {
+            float f[N];
+            P::unpack(w, f);
 #pragma unroll
-                for (int e = 0; e < N; ++e) sum += f[e];
-                count += N;
-            }
-        ln_moments m{(float)count, count ? sum / (float)count : 0.0f, 0.0f};
+            for (int e = 0; e < N; ++e) m2 = fmaf(f[e] - mean, f[e] - mean, m2);
+            if (q) a = max(a, P::largest(w));
+        };
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-            if (j * THREADS + at < pieces) {
-                float f[N];
-                P::unpack(v[j], f);
-#pragma unroll
-                for (int e = 0; e < N; ++e) m.m2 = fmaf(f[e] - m.mean, f[e] - m.mean, m.m2);
-                if (q) a = max(a, P::largest(v[j]));
-            }
+            if (j * THREADS + at < pieces) deviate(v[j]);
         if constexpr (WARPS > 1)
-            for (int64_t p = NV * THREADS + at; p < pieces; p += THREADS) {
-                const typename P::raw w = P::load_again(xr, p);
-                float f[N];
-                P::unpack(w, f);
-#pragma unroll
-                for (int e = 0; e < N; ++e) m.m2 = fmaf(f[e] - m.mean, f[e] - m.mean, m.m2);
-                if (q) a = max(a, P::largest(w));
-            }
-        m.template join_lanes<(THREADS < 32 ? THREADS : 32)>();
+            for (int64_t p = NV * THREADS + at; p < pieces; p += THREADS) deviate(P::load_again(xr, p));
+        m2 = ln_lanes_sum<LANES>(m2);
         if (q) {
             if constexpr (THREADS < 32) {
 #pragma unroll
                 for (int o = THREADS / 2; o; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
             } else a = __reduce_max_sync(0xffffffffu, a);
         }
-        if constexpr (WARPS > 1) {   // (two turns' places: one barrier a row)
-            if ((at & 31) == 0) part[turn * WARPS + (at >> 5)] = make_float4(m.n, m.mean, m.m2, __uint_as_float(a));
+        if constexpr (WARPS > 1) {
+            if ((at & 31) == 0) part[turn * WARPS + (at >> 5)] = make_float2(sum, m2), tops[turn * WARPS + (at >> 5)] = a;
             __syncthreads();
-            m = ln_moments{0.0f, 0.0f, 0.0f};
+            ln_join<WARPS>(part + turn * WARPS, counts, inv, mean, m2);
             a = 0;
 #pragma unroll
-            for (int i = 0; i < WARPS; ++i) {
-                const float4 o = part[turn * WARPS + i];
-                m.join(o.x, o.y, o.z);
-                a = max(a, __float_as_uint(o.w));
-            }
+            for (int i = 0; i < WARPS; ++i) a = max(a, tops[turn * WARPS + i]);
         }
-        const float rstd = 1.0f / sqrtf(m.m2 / m.n + eps);
-        if (mine && at == 0 && stats) stats[r] = make_float2(m.mean, rstd);
+        const float rstd = 1.0f / sqrtf(fmaf(m2, inv, eps));
+        if (mine && at == 0 && stats) stats[r] = make_float2(mean, rstd);
         if (!mine) continue;
         T* const yr = y + r * ldy;
         const q_row k(a);
@@ -193,7 +181,7 @@ __global__ void __launch_bounds__(THREADS < LN_CTA ? LN_CTA : THREADS)
             P::columns(weight, p, 1.0f, g);
             P::columns(bias, p, 0.0f, b);
 #pragma unroll
-            for (int e = 0; e < N; ++e) f[e] = fmaf((f[e] - m.mean) * rstd, g[e], b[e]);
+            for (int e = 0; e < N; ++e) f[e] = fmaf((f[e] - mean) * rstd, g[e], b[e]);
             if (q) P::quantize(qr, p, whole, w, k);
             P::store(yr, p, f);
         };
@@ -203,6 +191,31 @@ __global__ void __launch_bounds__(THREADS < LN_CTA ? LN_CTA : THREADS)
         if constexpr (WARPS > 1)
             for (int64_t p = NV * THREADS + at; p < pieces; p += THREADS) leave(p, P::load_again(xr, p));
         if (q && at == 0) q_scale[r] = k.scale;
+    }
+}
+
+// a piece's 8-bit integers from its numbers (of which `largest` is the row's: the same as q_store)
+template <int N> __device__ __forceinline__ void q_store_pairs(int8_t* q, bool whole, const uint64_t* x, const q_row& k)
+{
+    // (the products by single instructions: a packed one and a packed addition behind it are made a multiply-add, whose one rounding gives other integers)
+    const uint64_t up = f2_of(12582912.0f, 12582912.0f);
+    const auto two = [&](uint64_t v) {
+        const float2 f = f2_get(v);
+        return f2_get(f2_add(f2_of(__fmul_rn(f.x, k.factor), __fmul_rn(f.y, k.factor)), up));
+    };
+    uint32_t w[N / 4];
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+        const float2 a = two(x[2 * i]), b = two(x[2 * i + 1]);
+        w[i] = __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040), __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
+        if (k.factor == 0.0f) w[i] = 0;
+    }
+    if (whole) {
+        if constexpr (N == 4) *reinterpret_cast<uint32_t*>(q) = w[0];
+        else *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) q[e] = (int8_t)(w[e / 4] >> (8 * (e & 3)));
     }
 }
 
@@ -266,7 +279,8 @@ template <typename T, int NV, int THREADS, int CTAS> __global__ void __launch_bo
 {
     using P = ln_piece<T, true>;
     constexpr int N = P::N, WARPS = THREADS / 32;
-    __shared__ float4 part[2][WARPS];
+    __shared__ float2 part[2][WARPS], counts[WARPS];
+    __shared__ uint32_t tops[2][WARPS];
     extern __shared__ unsigned char ln_raw[];
     const ln_ring ring(ln_raw, a.stages, a.bytes);
     const int at = threadIdx.x, pieces = (int)(a.cols / N), row_bytes = (int)(a.cols * (int64_t)sizeof(T));
@@ -279,70 +293,79 @@ template <typename T, int NV, int THREADS, int CTAS> __global__ void __launch_bo
     };
     if (at == 0)
         for (int i = 0; i < a.stages; ++i) fetch(i);
-    float w[NV * N], b[NV * N];
+    uint64_t w[NV * N / 2], b[NV * N / 2];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        if (j * THREADS + at < pieces) P::columns(a.weight, j * THREADS + at, 1.0f, w + j * N), P::columns(a.bias, j * THREADS + at, 0.0f, b + j * N);
+        float u[N], v[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) u[e] = v[e] = 0.0f;
+        if (j * THREADS + at < pieces) P::columns(a.weight, j * THREADS + at, 1.0f, u), P::columns(a.bias, j * THREADS + at, 0.0f, v);
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) w[j * N / 2 + e] = f2_of(u[2 * e], u[2 * e + 1]), b[j * N / 2 + e] = f2_of(v[2 * e], v[2 * e + 1]);
     }
+    const float inv = 1.0f / (float)a.cols, n_warp = ln_lanes_sum<32>((float)(max(0, pieces - at + THREADS - 1) / THREADS * N)), inv_warp = n_warp > 0.0f ? 1.0f / n_warp : 0.0f;
+    if ((at & 31) == 0) counts[at >> 5] = make_float2(inv_warp, n_warp);   // (the first row's barrier is before their first use)
     int i = 0;
     bool failed = false;
     for (; i < turns; ++i) {
         const int64_t r = (int64_t)blockIdx.x + (int64_t)i * gridDim.x;
         const bool ok = ring.wait(i, a.status);
         const uint4* const row = reinterpret_cast<const uint4*>(ring.at + (i % a.stages) * a.bytes);
-        float f[NV * N], sum = 0.0f;
-        int count = 0;
+        uint64_t f[NV * N / 2], s = 0;   // (two zeros)
         uint32_t top = 0;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
             if (j * THREADS + at < pieces) {
                 const uint4 v = row[j * THREADS + at];
-                P::unpack(v, f + j * N);
+                f2_unpack<T>(v, f + j * N / 2);
                 if (a.q) top = max(top, P::largest(v));
 #pragma unroll
-                for (int e = 0; e < N; ++e) sum += f[j * N + e];
-                count += N;
+                for (int e = 0; e < N / 2; ++e) s = f2_add(s, f[j * N / 2 + e]);
             }
-        ln_moments m{(float)count, count ? sum / (float)count : 0.0f, 0.0f};
+        const float sum = ln_lanes_sum<32>(f2_sum(s)), near = -sum * inv_warp;
+        const uint64_t near2 = f2_of(near, near);
+        s = 0;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
             if (j * THREADS + at < pieces)
 #pragma unroll
-                for (int e = 0; e < N; ++e) m.m2 = fmaf(f[j * N + e] - m.mean, f[j * N + e] - m.mean, m.m2);
-        m.join_lanes<32>();
-        top = __reduce_max_sync(0xffffffffu, top);
-        if ((at & 31) == 0) part[i & 1][at >> 5] = make_float4(m.n, m.mean, m.m2, __uint_as_float(top));
+                for (int e = 0; e < N / 2; ++e) {
+                    const uint64_t d = f2_add(f[j * N / 2 + e], near2);
+                    s = f2_fma(d, d, s);
+                }
+        float m2 = ln_lanes_sum<32>(f2_sum(s)), mean;
+        if (a.q) top = __reduce_max_sync(0xffffffffu, top);
+        if ((at & 31) == 0) part[i & 1][at >> 5] = make_float2(sum, m2), tops[i & 1][at >> 5] = top;
         if (__syncthreads_or(!ok)) {
             failed = true;
             break;
         }
         if (at == 0 && i > 0) fetch(i - 1 + a.stages);
-        m = ln_moments{0.0f, 0.0f, 0.0f};
-        top = 0;
+        ln_join<WARPS>(part[i & 1], counts, inv, mean, m2);
+        const float rstd = 1.0f / sqrtf(fmaf(m2, inv, a.eps));
+        const uint64_t mean2 = f2_of(-mean, -mean), rstd2 = f2_of(rstd, rstd);
+        if (a.q) {
+            top = 0;
 #pragma unroll
-        for (int k = 0; k < WARPS; ++k) {
-            const float4 o = part[i & 1][k];
-            m.join(o.x, o.y, o.z);
-            top = max(top, __float_as_uint(o.w));
+            for (int k = 0; k < WARPS; ++k) top = max(top, tops[i & 1][k]);
+            const q_row k(top);
+            int8_t* const qr = a.q + r * a.ldq;
+            const bool whole = (reinterpret_cast<uintptr_t>(qr) & (N - 1)) == 0;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (j * THREADS + at < pieces) q_store_pairs<N>(qr + (j * THREADS + at) * N, whole, f + j * N / 2, k);
+            if (at == 0) a.q_scale[r] = k.scale;
         }
-        const float rstd = 1.0f / sqrtf(m.m2 / m.n + a.eps);
-        const q_row k(top);
         T* const yr = static_cast<T*>(a.y) + r * a.ldy;
-        int8_t* const qr = a.q + r * a.ldq;
-        const bool whole = (reinterpret_cast<uintptr_t>(qr) & (N - 1)) == 0;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
             if (j * THREADS + at < pieces) {
-                if (a.q) P::quantize(qr, j * THREADS + at, whole, row[j * THREADS + at], k);
-                float o[N];
+                uint64_t o[N / 2];
 #pragma unroll
-                for (int e = 0; e < N; ++e) o[e] = fmaf((f[j * N + e] - m.mean) * rstd, w[j * N + e], b[j * N + e]);
-                P::store(yr, j * THREADS + at, o);
+                for (int e = 0; e < N / 2; ++e) o[e] = f2_fma(f2_mul(f2_add(f[j * N / 2 + e], mean2), rstd2), w[j * N / 2 + e], b[j * N / 2 + e]);
+                reinterpret_cast<uint4*>(yr)[j * THREADS + at] = f2_piece<T>(o);
             }
-        if (at == 0) {
-            if (a.stats) a.stats[r] = make_float2(m.mean, rstd);
-            if (a.q) a.q_scale[r] = k.scale;
-        }
+        if (at == 0 && a.stats) a.stats[r] = make_float2(mean, rstd);
     }
     if (failed) ring.drain(i, min(turns, max(i, 1) - 1 + a.stages));
 }
@@ -489,7 +512,7 @@ template <typename T, int NV, int THREADS, int CTAS, bool FROM8> __global__ void
     };
     if (at == 0)
         for (int i = 0; i < a.stages; ++i) fetch(i);
-    float sum_w[NV * N] = {}, sum_b[NV * N] = {};
+    uint64_t sum_w[NV * N / 2] = {}, sum_b[NV * N / 2] = {};   // (zeros)
     const float inv = 1.0f / (float)a.cols;
     int i = 0;
     bool failed = false;
@@ -506,30 +529,36 @@ template <typename T, int NV, int THREADS, int CTAS, bool FROM8> __global__ void
         const bool ok = ring.wait(i, a.status);
         const uint4* const dyr = reinterpret_cast<const uint4*>(ring.at + (i % a.stages) * a.bytes);
         const void* const xr = ring.at + (i % a.stages) * a.bytes + row_bytes;
-        const auto load = [&](int p, float* d, float* h, float* w) {   // dy, normalised row and weight of a piece
-            P::unpack(dyr[p], d);
-            if constexpr (FROM8) P::unpack8(static_cast<const typename P::raw8*>(xr)[p], h);
-            else P::unpack(static_cast<const uint4*>(xr)[p], h);
+        const uint64_t mean2 = f2_of(-st.x, -st.x), rstd2 = f2_of(st.y, st.y), s2 = f2_of(s, s);
+        const auto load = [&](int p, uint64_t* d, uint64_t* h, uint64_t* w) {   // dy, normalised row and weight of a piece
+            f2_unpack<T>(dyr[p], d);
+            if constexpr (FROM8) {
+                const typename P::raw8 v = static_cast<const typename P::raw8*>(xr)[p];
+                if constexpr (N == 8) f2_unpack8(v.x, h), f2_unpack8(v.y, h + 2);
+                else f2_unpack8(v, h);
+            } else f2_unpack<T>(static_cast<const uint4*>(xr)[p], h);
+            float u[N];
+            P::columns(a.weight, p, 1.0f, u);
 #pragma unroll
-            for (int e = 0; e < N; ++e) h[e] = FROM8 ? fmaf(h[e], s, -st.x) * st.y : (h[e] - st.x) * st.y;
-            P::columns(a.weight, p, 1.0f, w);
+            for (int e = 0; e < N / 2; ++e) {
+                h[e] = f2_mul(FROM8 ? f2_fma(h[e], s2, mean2) : f2_add(h[e], mean2), rstd2);
+                w[e] = f2_of(u[2 * e], u[2 * e + 1]);
+            }
         };
-        float g0 = 0.0f, g1 = 0.0f;
+        uint64_t s0 = 0, s1 = 0;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
             if (j * THREADS + at < pieces) {
-                float d[N], h[N], w[N];
+                uint64_t d[N / 2], h[N / 2], w[N / 2];
                 load(j * THREADS + at, d, h, w);
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const float g = d[e] * w[e];
-                    g0 += g;
-                    g1 = fmaf(g, h[e], g1);
-                    sum_w[j * N + e] = fmaf(d[e], h[e], sum_w[j * N + e]), sum_b[j * N + e] += d[e];
+                for (int e = 0; e < N / 2; ++e) {
+                    const uint64_t g = f2_mul(d[e], w[e]);
+                    s0 = f2_add(s0, g), s1 = f2_fma(g, h[e], s1);
+                    sum_w[j * N / 2 + e] = f2_fma(d[e], h[e], sum_w[j * N / 2 + e]), sum_b[j * N / 2 + e] = f2_add(sum_b[j * N / 2 + e], d[e]);
                 }
             }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) g0 += __shfl_xor_sync(0xffffffffu, g0, o), g1 += __shfl_xor_sync(0xffffffffu, g1, o);
+        float g0 = ln_lanes_sum<32>(f2_sum(s0)), g1 = ln_lanes_sum<32>(f2_sum(s1));
         if ((at & 31) == 0) part[i & 1][at >> 5] = make_float2(g0, g1);
         if (__syncthreads_or(!ok)) {
             failed = true;
@@ -539,16 +568,16 @@ template <typename T, int NV, int THREADS, int CTAS, bool FROM8> __global__ void
         g0 = g1 = 0.0f;
 #pragma unroll
         for (int k = 0; k < WARPS; ++k) g0 += part[i & 1][k].x, g1 += part[i & 1][k].y;
-        const float m0 = g0 * inv, m1 = g1 * inv;
+        const uint64_t m0 = f2_of(-g0 * inv, -g0 * inv), m1 = f2_of(-g1 * inv, -g1 * inv);
         T* const dxr = static_cast<T*>(a.dx) + r * a.lddx;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
             if (j * THREADS + at < pieces) {
-                float d[N], h[N], w[N];
+                uint64_t d[N / 2], h[N / 2], w[N / 2];
                 load(j * THREADS + at, d, h, w);
 #pragma unroll
-                for (int e = 0; e < N; ++e) d[e] = st.y * (fmaf(d[e], w[e], -m0) - h[e] * m1);
-                P::store(dxr, j * THREADS + at, d);
+                for (int e = 0; e < N / 2; ++e) d[e] = f2_mul(rstd2, f2_fma(h[e], m1, f2_fma(d[e], w[e], m0)));
+                reinterpret_cast<uint4*>(dxr)[j * THREADS + at] = f2_piece<T>(d);
             }
     }
     if (failed) {
@@ -563,8 +592,8 @@ template <typename T, int NV, int THREADS, int CTAS, bool FROM8> __global__ void
 #pragma unroll
             for (int e = 0; e < N; e += 4) {
                 const int c = (j * THREADS + at) * N + e;
-                *reinterpret_cast<float4*>(line + c) = make_float4(sum_w[j * N + e], sum_w[j * N + e + 1], sum_w[j * N + e + 2], sum_w[j * N + e + 3]);
-                *reinterpret_cast<float4*>(line + a.cols + c) = make_float4(sum_b[j * N + e], sum_b[j * N + e + 1], sum_b[j * N + e + 2], sum_b[j * N + e + 3]);
+                *reinterpret_cast<ulonglong2*>(line + c) = make_ulonglong2(sum_w[(j * N + e) / 2], sum_w[(j * N + e) / 2 + 1]);
+                *reinterpret_cast<ulonglong2*>(line + a.cols + c) = make_ulonglong2(sum_b[(j * N + e) / 2], sum_b[(j * N + e) / 2 + 1]);
             }
 }
 
@@ -678,7 +707,7 @@ int ln_launch(s2v_ctx* ctx, cudaStream_t st, int64_t rows, int64_t cols, const T
                 return (int)S2V_OK;
             };
             constexpr int N = ln_piece<T, true>::N;
-            if (pieces <= 256) return ring(layer_norm_ring_kernel<T, 1, 256, 5>, 256, 5);
+            if (pieces <= 256) return ring(layer_norm_ring_kernel<T, 1, 256, 4>, 256, 4);
             if (pieces <= 512) return ring(layer_norm_ring_kernel<T, 2, 256, 3>, 256, 3);
             if (pieces <= 1024) return ring(layer_norm_ring_kernel<T, 4, 256, 2>, 256, 2);
             if (pieces <= 2048) return ring(layer_norm_ring_kernel<T, 4, 512, 1>, 512, 1);
