@@ -82,18 +82,13 @@ template <int LANES> __device__ __forceinline__ float ln_lanes_sum(float v)
     for (int o = LANES / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-// Mean and sum of squared deviations of a row from its warps' (sum, sum of squared deviations from the warp's mean, 1 / count, count).
+// Mean and sum of squared deviations of a row from its warps' (sum, sum of squared deviations from the warp's mean) and (1 / count, count): a warp's part a lane.
 template <int WARPS> __device__ __forceinline__ void ln_join(const float2* part, const float2* counts, float inv, float& mean, float& m2)
 {
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) sum += part[i].x;
-    mean = sum * inv, m2 = 0.0f;
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) {
-        const float d = fmaf(part[i].x, counts[i].x, -mean);
-        m2 += fmaf(d * counts[i].y, d, part[i].y);
-    }
+    const float2 p = part[threadIdx.x & (WARPS - 1)], c = counts[threadIdx.x & (WARPS - 1)];
+    mean = ln_lanes_sum<WARPS>(p.x) * inv;
+    const float d = fmaf(p.x, c.x, -mean);
+    m2 = ln_lanes_sum<WARPS>(fmaf(d * c.y, d, p.y));
 }
 
 // THREADS threads a row (8, 32 or a CTA of THREADS), NV pieces of each in registers; a longer row's others (CTAs alone) are read again.
@@ -164,11 +159,9 @@ __global__ void __launch_bounds__(THREADS < LN_CTA ? LN_CTA : THREADS)
             if ((at & 31) == 0) part[turn * WARPS + (at >> 5)] = make_float2(sum, m2), tops[turn * WARPS + (at >> 5)] = a;
             __syncthreads();
             ln_join<WARPS>(part + turn * WARPS, counts, inv, mean, m2);
-            a = 0;
-#pragma unroll
-            for (int i = 0; i < WARPS; ++i) a = max(a, tops[turn * WARPS + i]);
+            if (q) a = __reduce_max_sync(0xffffffffu, tops[turn * WARPS + (threadIdx.x & (WARPS - 1))]);
         }
-        const float rstd = 1.0f / sqrtf(fmaf(m2, inv, eps));
+        const float rstd = rsqrtf(fmaf(m2, inv, eps));
         if (mine && at == 0 && stats) stats[r] = make_float2(mean, rstd);
         if (!mine) continue;
         T* const yr = y + r * ldy;
@@ -274,7 +267,7 @@ struct LnNorm {
     s2v_device_status* status;
 };
 
-// A row a CTA, NV pieces a thread; one barrier a row, behind which the stage of the row before is free.
+// A row a CTA, NV pieces a thread; one barrier a row, behind which its stage is free.
 template <typename T, int NV, int THREADS, int CTAS> __global__ void __launch_bounds__(THREADS, CTAS) layer_norm_ring_kernel(const LnNorm a)
 {
     using P = ln_piece<T, true>;
@@ -340,15 +333,12 @@ template <typename T, int NV, int THREADS, int CTAS> __global__ void __launch_bo
             failed = true;
             break;
         }
-        if (at == 0 && i > 0) fetch(i - 1 + a.stages);
+        if (at == 0) fetch(i + a.stages);   // (the row is in registers)
         ln_join<WARPS>(part[i & 1], counts, inv, mean, m2);
-        const float rstd = 1.0f / sqrtf(fmaf(m2, inv, a.eps));
+        const float rstd = rsqrtf(fmaf(m2, inv, a.eps));
         const uint64_t mean2 = f2_of(-mean, -mean), rstd2 = f2_of(rstd, rstd);
         if (a.q) {
-            top = 0;
-#pragma unroll
-            for (int k = 0; k < WARPS; ++k) top = max(top, tops[i & 1][k]);
-            const q_row k(top);
+            const q_row k(__reduce_max_sync(0xffffffffu, tops[i & 1][at & (WARPS - 1)]));
             int8_t* const qr = a.q + r * a.ldq;
             const bool whole = (reinterpret_cast<uintptr_t>(qr) & (N - 1)) == 0;
 #pragma unroll
@@ -367,7 +357,7 @@ template <typename T, int NV, int THREADS, int CTAS> __global__ void __launch_bo
             }
         if (at == 0 && a.stats) a.stats[r] = make_float2(mean, rstd);
     }
-    if (failed) ring.drain(i, min(turns, max(i, 1) - 1 + a.stages));
+    if (failed) ring.drain(i, min(turns, i + a.stages));
 }
 
 // What the gradient takes its normalised rows from: x, or 8-bit rows with scales.
@@ -491,97 +481,139 @@ __global__ void __launch_bounds__(THREADS < LN_CTA ? LN_CTA : THREADS) layer_nor
     }
 }
 
-// The same through the ring, a row a CTA: a stage holds the row's dy and, behind it, x or the 8-bit row.
-template <typename T, int NV, int THREADS, int CTAS, bool FROM8> __global__ void __launch_bounds__(THREADS, CTAS) layer_norm_grad_ring_kernel(const LnGrad a)
+// The same through the ring, R rows a turn of a CTA: a stage holds a row's dy and, behind it, x or the 8-bit row.  With the rows' raw numbers and the weight in
+// registers a number is read from shared memory once, and R rows share a barrier (dy and 8-bit rows read twice and the weight twice a row through L1: 8192 x 8192
+// bf16 105 us).
+template <typename T, int NV, int R, int THREADS, int CTAS, bool FROM8> __global__ void __launch_bounds__(THREADS, CTAS) layer_norm_grad_ring_kernel(const LnGrad a)
 {
     using P = ln_piece<T, true>;
+    using raw_x = typename std::conditional<FROM8, typename P::raw8, uint4>::type;
     constexpr int N = P::N, WARPS = THREADS / 32;
-    __shared__ float2 part[2][WARPS];
+    __shared__ float2 part[2][R][WARPS];
     extern __shared__ unsigned char ln_raw[];
     const ln_ring ring(ln_raw, a.stages, a.bytes);
     const int at = threadIdx.x, pieces = (int)(a.cols / N), row_bytes = (int)(a.cols * (int64_t)sizeof(T)), x_bytes = FROM8 ? (int)a.cols : row_bytes;
-    const int turns = (int)((a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x);
-    const auto fetch = [&](int turn) {
-        if (turn < turns) {
-            const int64_t r = (int64_t)blockIdx.x + (int64_t)turn * gridDim.x;
-            mbar_expect(ring.full + 8 * (turn % a.stages), (uint32_t)(row_bytes + x_bytes));
-            ring.copy(turn % a.stages, 0, static_cast<const T*>(a.dy) + r * a.lddy, row_bytes);
-            if constexpr (FROM8) ring.copy(turn % a.stages, row_bytes, a.q + r * a.ldx, x_bytes);
-            else ring.copy(turn % a.stages, row_bytes, static_cast<const T*>(a.x) + r * a.ldx, x_bytes);
+    const int mine = (int)((a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x);   // rows of this CTA
+    const auto fetch = [&](int i) {
+        if (i < mine) {
+            const int64_t r = (int64_t)blockIdx.x + (int64_t)i * gridDim.x;
+            mbar_expect(ring.full + 8 * (i % a.stages), (uint32_t)(row_bytes + x_bytes));
+            ring.copy(i % a.stages, 0, static_cast<const T*>(a.dy) + r * a.lddy, row_bytes);
+            if constexpr (FROM8) ring.copy(i % a.stages, row_bytes, a.q + r * a.ldx, x_bytes);
+            else ring.copy(i % a.stages, row_bytes, static_cast<const T*>(a.x) + r * a.ldx, x_bytes);
         }
     };
     if (at == 0)
         for (int i = 0; i < a.stages; ++i) fetch(i);
-    uint64_t sum_w[NV * N / 2] = {}, sum_b[NV * N / 2] = {};   // (zeros)
+    uint64_t w[NV * N / 2], sum_w[NV * N / 2] = {}, sum_b[NV * N / 2] = {};   // (zeros)
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        float u[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) u[e] = 0.0f;
+        if (j * THREADS + at < pieces) P::columns(a.weight, j * THREADS + at, 1.0f, u);
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) w[j * N / 2 + e] = f2_of(u[2 * e], u[2 * e + 1]);
+    }
     const float inv = 1.0f / (float)a.cols;
     int i = 0;
     bool failed = false;
-    float2 next_st = a.stats[blockIdx.x];
-    float next_s = FROM8 ? a.q_scale[blockIdx.x] : 1.0f;
-    for (; i < turns; ++i) {
-        const int64_t r = (int64_t)blockIdx.x + (int64_t)i * gridDim.x;
-        const float2 st = next_st;
-        const float s = next_s;
-        if (i + 1 < turns) {
-            next_st = a.stats[r + gridDim.x];
-            if (FROM8) next_s = a.q_scale[r + gridDim.x];
-        }
-        const bool ok = ring.wait(i, a.status);
-        const uint4* const dyr = reinterpret_cast<const uint4*>(ring.at + (i % a.stages) * a.bytes);
-        const void* const xr = ring.at + (i % a.stages) * a.bytes + row_bytes;
-        const uint64_t mean2 = f2_of(-st.x, -st.x), rstd2 = f2_of(st.y, st.y), s2 = f2_of(s, s);
-        const auto load = [&](int p, uint64_t* d, uint64_t* h, uint64_t* w) {   // dy, normalised row and weight of a piece
-            f2_unpack<T>(dyr[p], d);
-            if constexpr (FROM8) {
-                const typename P::raw8 v = static_cast<const typename P::raw8*>(xr)[p];
-                if constexpr (N == 8) f2_unpack8(v.x, h), f2_unpack8(v.y, h + 2);
-                else f2_unpack8(v, h);
-            } else f2_unpack<T>(static_cast<const uint4*>(xr)[p], h);
-            float u[N];
-            P::columns(a.weight, p, 1.0f, u);
+    float2 next_st[R];
+    float next_s[R];
+    const auto ask = [&](int from) {   // the rows' numbers, a turn ahead
 #pragma unroll
-            for (int e = 0; e < N / 2; ++e) {
-                h[e] = f2_mul(FROM8 ? f2_fma(h[e], s2, mean2) : f2_add(h[e], mean2), rstd2);
-                w[e] = f2_of(u[2 * e], u[2 * e + 1]);
+        for (int u = 0; u < R; ++u)
+            if (from + u < mine) {
+                const int64_t r = (int64_t)blockIdx.x + (int64_t)(from + u) * gridDim.x;
+                next_st[u] = a.stats[r], next_s[u] = FROM8 ? a.q_scale[r] : 1.0f;
             }
+    };
+    ask(0);
+    for (; i < mine; i += R) {
+        float2 st[R];
+        float s[R];
+#pragma unroll
+        for (int u = 0; u < R; ++u) st[u] = next_st[u], s[u] = next_s[u];
+        ask(i + R);
+        uint4 dv[R][NV];
+        raw_x xv[R][NV];
+        // normalised numbers of a piece
+        const auto normalise = [&](int u, const raw_x& v, uint64_t* h) {
+            const uint64_t mean2 = f2_of(-st[u].x, -st[u].x), rstd2 = f2_of(st[u].y, st[u].y), s2 = f2_of(s[u], s[u]);
+            if constexpr (!FROM8) f2_unpack<T>(v, h);
+            else if constexpr (N == 8) f2_unpack8(v.x, h), f2_unpack8(v.y, h + 2);
+            else f2_unpack8(v, h);
+#pragma unroll
+            for (int e = 0; e < N / 2; ++e) h[e] = f2_mul(FROM8 ? f2_fma(h[e], s2, mean2) : f2_add(h[e], mean2), rstd2);
         };
-        uint64_t s0 = 0, s1 = 0;
+        bool ok = true;
+        float g0[R], g1[R];
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-            if (j * THREADS + at < pieces) {
-                uint64_t d[N / 2], h[N / 2], w[N / 2];
-                load(j * THREADS + at, d, h, w);
+        for (int u = 0; u < R; ++u) {
+            uint64_t s0 = 0, s1 = 0;
+            if (i + u < mine) {
+                ok = ok && ring.wait(i + u, a.status);
+                const unsigned char* const stage = ring.at + ((i + u) % a.stages) * a.bytes;
 #pragma unroll
-                for (int e = 0; e < N / 2; ++e) {
-                    const uint64_t g = f2_mul(d[e], w[e]);
-                    s0 = f2_add(s0, g), s1 = f2_fma(g, h[e], s1);
-                    sum_w[j * N / 2 + e] = f2_fma(d[e], h[e], sum_w[j * N / 2 + e]), sum_b[j * N / 2 + e] = f2_add(sum_b[j * N / 2 + e], d[e]);
-                }
+                for (int j = 0; j < NV; ++j)
+                    if (j * THREADS + at < pieces) {
+                        dv[u][j] = reinterpret_cast<const uint4*>(stage)[j * THREADS + at];
+                        xv[u][j] = reinterpret_cast<const raw_x*>(stage + row_bytes)[j * THREADS + at];
+                        uint64_t d[N / 2], h[N / 2];
+                        f2_unpack<T>(dv[u][j], d);
+                        normalise(u, xv[u][j], h);
+#pragma unroll
+                        for (int e = 0; e < N / 2; ++e) {
+                            const int c = j * N / 2 + e;
+                            const uint64_t g = f2_mul(d[e], w[c]);
+                            s1 = f2_fma(g, h[e], s1), s0 = f2_fma(d[e], w[c], s0);
+                            sum_w[c] = f2_fma(d[e], h[e], sum_w[c]), sum_b[c] = f2_add(sum_b[c], d[e]);
+                        }
+                    }
             }
-        float g0 = ln_lanes_sum<32>(f2_sum(s0)), g1 = ln_lanes_sum<32>(f2_sum(s1));
-        if ((at & 31) == 0) part[i & 1][at >> 5] = make_float2(g0, g1);
+            g0[u] = f2_sum(s0), g1[u] = f2_sum(s1);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1)
+#pragma unroll
+            for (int u = 0; u < R; ++u) g0[u] += __shfl_xor_sync(0xffffffffu, g0[u], o), g1[u] += __shfl_xor_sync(0xffffffffu, g1[u], o);
+        const int turn = i / R & 1;
+        if ((at & 31) == 0) {
+#pragma unroll
+            for (int u = 0; u < R; ++u) part[turn][u][at >> 5] = make_float2(g0[u], g1[u]);
+        }
         if (__syncthreads_or(!ok)) {
             failed = true;
             break;
         }
-        if (at == 0 && i > 0) fetch(i - 1 + a.stages);
-        g0 = g1 = 0.0f;
+        if (at == 0) {   // (the rows are in registers)
 #pragma unroll
-        for (int k = 0; k < WARPS; ++k) g0 += part[i & 1][k].x, g1 += part[i & 1][k].y;
-        const uint64_t m0 = f2_of(-g0 * inv, -g0 * inv), m1 = f2_of(-g1 * inv, -g1 * inv);
-        T* const dxr = static_cast<T*>(a.dx) + r * a.lddx;
+            for (int u = 0; u < R; ++u) fetch(i + u + a.stages);
+        }
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-            if (j * THREADS + at < pieces) {
-                uint64_t d[N / 2], h[N / 2], w[N / 2];
-                load(j * THREADS + at, d, h, w);
+        for (int u = 0; u < R; ++u) {
+            const float2 p = part[turn][u][at & (WARPS - 1)];
+            g0[u] = ln_lanes_sum<WARPS>(p.x), g1[u] = ln_lanes_sum<WARPS>(p.y);
+        }
 #pragma unroll
-                for (int e = 0; e < N / 2; ++e) d[e] = f2_mul(rstd2, f2_fma(h[e], m1, f2_fma(d[e], w[e], m0)));
-                reinterpret_cast<uint4*>(dxr)[j * THREADS + at] = f2_piece<T>(d);
-            }
+        for (int u = 0; u < R; ++u) {
+            if (i + u >= mine) break;
+            const uint64_t m0 = f2_of(-g0[u] * inv, -g0[u] * inv), m1 = f2_of(-g1[u] * inv, -g1[u] * inv), rstd2 = f2_of(st[u].y, st[u].y);
+            uint4* const dxr = reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + ((int64_t)blockIdx.x + (int64_t)(i + u) * gridDim.x) * a.lddx);
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (j * THREADS + at < pieces) {
+                    uint64_t d[N / 2], h[N / 2];
+                    f2_unpack<T>(dv[u][j], d);
+                    normalise(u, xv[u][j], h);
+#pragma unroll
+                    for (int e = 0; e < N / 2; ++e) d[e] = f2_mul(rstd2, f2_fma(h[e], m1, f2_fma(d[e], w[j * N / 2 + e], m0)));
+                    dxr[j * THREADS + at] = f2_piece<T>(d);
+                }
+        }
     }
     if (failed) {
-        ring.drain(i, min(turns, max(i, 1) - 1 + a.stages));
+        ring.drain(i, min(mine, i + a.stages));
         return;
     }
     if (!a.columns) return;
@@ -590,10 +622,10 @@ template <typename T, int NV, int THREADS, int CTAS, bool FROM8> __global__ void
     for (int j = 0; j < NV; ++j)
         if (j * THREADS + at < pieces)
 #pragma unroll
-            for (int e = 0; e < N; e += 4) {
-                const int c = (j * THREADS + at) * N + e;
-                *reinterpret_cast<ulonglong2*>(line + c) = make_ulonglong2(sum_w[(j * N + e) / 2], sum_w[(j * N + e) / 2 + 1]);
-                *reinterpret_cast<ulonglong2*>(line + a.cols + c) = make_ulonglong2(sum_b[(j * N + e) / 2], sum_b[(j * N + e) / 2 + 1]);
+            for (int e = 0; e < N / 2; e += 2) {
+                const int c = (j * THREADS + at) * N + 2 * e;
+                *reinterpret_cast<ulonglong2*>(line + c) = make_ulonglong2(sum_w[j * N / 2 + e], sum_w[j * N / 2 + e + 1]);
+                *reinterpret_cast<ulonglong2*>(line + a.cols + c) = make_ulonglong2(sum_b[j * N / 2 + e], sum_b[j * N / 2 + e + 1]);
             }
 }
 
@@ -642,30 +674,31 @@ template <typename T, bool FROM8> __global__ void __launch_bounds__(LN_CTA) laye
     float* const line = a.lines + (int64_t)blockIdx.y * 2 * a.cols;
     line[c] = w, line[a.cols + c] = b;
 }
-// The lines of the gradient's CTAs, added in a fixed order: V columns a thread, 8 threads' shares of the lines.
-template <int V> __global__ void __launch_bounds__(LN_CTA) layer_norm_lines_kernel(int lines, int64_t cols, const float* __restrict__ from, float* __restrict__ dweight, float* __restrict__ dbias)
+// The lines of the gradient's CTAs, added in a fixed order: V columns a thread, LANES threads side by side, the others a share of the lines each.
+template <int V, int LANES> __global__ void __launch_bounds__(LN_CTA) layer_norm_lines_kernel(int lines, int64_t cols, const float* __restrict__ from, float* __restrict__ dweight, float* __restrict__ dbias)
 {
-    __shared__ float part[8][32 * V];
-    const int64_t c = ((int64_t)blockIdx.x * 32 + (threadIdx.x & 31)) * V;
-    const int g = threadIdx.x >> 5;
+    constexpr int SHARES = LN_CTA / LANES;
+    __shared__ float part[SHARES][LANES * V];
+    const int at = threadIdx.x % LANES, g = threadIdx.x / LANES;
+    const int64_t c = ((int64_t)blockIdx.x * LANES + at) * V;
     float t[V] = {};
     if (c < 2 * cols) {
-#pragma unroll 4
-        for (int l = g; l < lines; l += 8) {
+#pragma unroll 8
+        for (int l = g; l < lines; l += SHARES) {
             if constexpr (V == 4) {
                 const float4 f = __ldcs(reinterpret_cast<const float4*>(from + (int64_t)l * 2 * cols + c));
                 t[0] += f.x, t[1] += f.y, t[2] += f.z, t[3] += f.w;
-            } else t[0] += from[(int64_t)l * 2 * cols + c];
+            } else t[0] += __ldcs(from + (int64_t)l * 2 * cols + c);
         }
     }
 #pragma unroll
-    for (int e = 0; e < V; ++e) part[g][(threadIdx.x & 31) * V + e] = t[e];
+    for (int e = 0; e < V; ++e) part[g][at * V + e] = t[e];
     __syncthreads();
-    if (threadIdx.x >= 32 * V) return;
-    const int64_t k = (int64_t)blockIdx.x * 32 * V + threadIdx.x;
+    if (threadIdx.x >= LANES * V) return;
+    const int64_t k = (int64_t)blockIdx.x * LANES * V + threadIdx.x;
     float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s += part[i][threadIdx.x];
+#pragma unroll 8
+    for (int i = 0; i < SHARES; ++i) s += part[i][threadIdx.x];
     if (k < cols) {
         if (dweight) dweight[k] = s;
     } else if (k < 2 * cols && dbias) dbias[k - cols] = s;
@@ -756,12 +789,13 @@ template <typename T, bool FROM8> int ln_grad_launch(s2v_ctx* ctx, cudaStream_t 
         if constexpr (VEC) {
             // (at least two rows of a CTA in the ring; the 8-bit rows on 16-byte boundaries too)
             const bool whole = !FROM8 || (a.cols % 16 == 0 && s2v_aligned16(a.q) && (a.rows <= 1 || a.ldx % 16 == 0));
-            if (pieces > 128 && pieces <= 2048 * 8 / N && whole && a.rows <= INT32_MAX && a.cols * (int64_t)(sizeof(T) + (FROM8 ? 1 : sizeof(T))) <= LN_RING_ROW) {
-                if (pieces <= 256) return ring(layer_norm_grad_ring_kernel<T, 1, 256, 4, FROM8>, 256, 4);
-                if (pieces <= 512) return ring(layer_norm_grad_ring_kernel<T, 2, 256, 3, FROM8>, 256, 3);
-                if (pieces <= 1024) return ring(layer_norm_grad_ring_kernel<T, 4, 256, 2, FROM8>, 256, 2);
-                if (pieces <= 2048) return ring(layer_norm_grad_ring_kernel<T, 4, 512, 1, FROM8>, 512, 1);
-                if constexpr (N == 4) return ring(layer_norm_grad_ring_kernel<T, 8, 512, 1, FROM8>, 512, 1);
+            if (pieces > 128 && whole && a.rows <= INT32_MAX && a.cols * (int64_t)(sizeof(T) + (FROM8 ? 1 : sizeof(T))) <= LN_RING_ROW) {
+                if (pieces <= 256) return ring(layer_norm_grad_ring_kernel<T, 1, 2, 256, 3, FROM8>, 256, 3);
+                if (pieces <= 512) return ring(layer_norm_grad_ring_kernel<T, 2, 2, 256, 2, FROM8>, 256, 2);
+                if (pieces <= 1024) return ring(layer_norm_grad_ring_kernel<T, 2, 2, 512, 1, FROM8>, 512, 1);
+                if constexpr (N == 4) {
+                    if (pieces <= 2048) return ring(layer_norm_grad_ring_kernel<T, 4, 1, 512, 1, FROM8>, 512, 1);
+                }
             }
         }
         if (pieces <= 8) return go(layer_norm_grad_kernel<T, VEC, 1, 8, FROM8>, 8, 8 * N);
@@ -789,8 +823,10 @@ template <typename T, bool FROM8> int ln_grad_launch(s2v_ctx* ctx, cudaStream_t 
     };
     const int rc = vec ? by_size(std::true_type()) : by_size(std::false_type());
     if (rc != S2V_OK || !a.columns) return rc;
-    if (a.cols % 2 == 0) layer_norm_lines_kernel<4><<<(unsigned)((2 * a.cols + 127) / 128), LN_CTA, 0, st>>>(lines, a.cols, a.lines, dweight, dbias);
-    else layer_norm_lines_kernel<1><<<(unsigned)((2 * a.cols + 31) / 32), LN_CTA, 0, st>>>(lines, a.cols, a.lines, dweight, dbias);
+    // (eight threads side by side where columns are few: 592 lines of 2 x 128 columns by two CTAs of 32 took 22 us)
+    const auto add = [&](auto kernel, int64_t per) { kernel<<<(unsigned)((2 * a.cols + per - 1) / per), LN_CTA, 0, st>>>(lines, a.cols, a.lines, dweight, dbias); };
+    if (a.cols % 2 == 0) a.cols >= 4096 ? add(layer_norm_lines_kernel<4, 16>, 64) : add(layer_norm_lines_kernel<4, 4>, 16);
+    else a.cols >= 4096 ? add(layer_norm_lines_kernel<1, 32>, 32) : add(layer_norm_lines_kernel<1, 8>, 8);
     S2V_CHECK_LAUNCH(ctx, "layer_norm_lines_kernel");
     return S2V_OK;
 }
