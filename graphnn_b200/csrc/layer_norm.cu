@@ -239,7 +239,11 @@ struct ln_ring {
                      "r"(full + 8 * stage)
                      : "memory");
     }
-    __device__ __forceinline__ bool wait(int turn, s2v_device_status* status) const { return tc_wait(full + 8 * (turn % stages), (uint32_t)(turn / stages) & 1u, abort_flag, status, 90); }
+    __device__ __forceinline__ bool wait(int stage, uint32_t phase, s2v_device_status* status) const
+    {
+        const uint32_t bar = full + 8 * stage;
+        return __all_sync(0xffffffffu, tc_mbar_try(bar, phase)) || tc_wait(bar, phase, abort_flag, status, 90);
+    }
     // where a wait gave up: copies under way, before the CTA goes
     __device__ __forceinline__ void drain(int from, int to) const
     {
@@ -267,7 +271,9 @@ struct LnNorm {
     s2v_device_status* status;
 };
 
-// A row a CTA, NV pieces a thread; one barrier a row, behind which its stage is free.
+// A row a CTA, NV pieces a thread; one barrier a row, behind which its stage is free.  What a row costs a thread besides its numbers is some 200 instructions, so
+// threads are few and pieces many; weight and bias are in registers for all rows.  (8192 x 8192 bf16 with 8-bit rows, threads x pieces x CTAs an SM: 512 x 2 x 1
+// 107 us, 256 x 4 x 2 70; 128 x 8 x 5 with weight and bias from L1 92.)
 template <typename T, int NV, int THREADS, int CTAS> __global__ void __launch_bounds__(THREADS, CTAS) layer_norm_ring_kernel(const LnNorm a)
 {
     using P = ln_piece<T, true>;
@@ -277,15 +283,17 @@ template <typename T, int NV, int THREADS, int CTAS> __global__ void __launch_bo
     extern __shared__ unsigned char ln_raw[];
     const ln_ring ring(ln_raw, a.stages, a.bytes);
     const int at = threadIdx.x, pieces = (int)(a.cols / N), row_bytes = (int)(a.cols * (int64_t)sizeof(T));
-    const int turns = (int)((a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x);
-    const auto fetch = [&](int turn) {
-        if (turn < turns) {
-            mbar_expect(ring.full + 8 * (turn % a.stages), (uint32_t)row_bytes);
-            ring.copy(turn % a.stages, 0, static_cast<const T*>(a.x) + ((int64_t)blockIdx.x + (int64_t)turn * gridDim.x) * a.ldx, row_bytes);
+    const int mine = (int)((a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x);   // rows of this CTA
+    const auto fetch = [&](int i, int stage) {
+        if (i < mine) {
+            mbar_expect(ring.full + 8 * stage, (uint32_t)row_bytes);
+            ring.copy(stage, 0, static_cast<const T*>(a.x) + ((int64_t)blockIdx.x + (int64_t)i * gridDim.x) * a.ldx, row_bytes);
         }
     };
     if (at == 0)
-        for (int i = 0; i < a.stages; ++i) fetch(i);
+        for (int i = 0; i < a.stages; ++i) fetch(i, i);
+    const float inv = 1.0f / (float)a.cols, n_warp = ln_lanes_sum<32>((float)(max(0, pieces - at + THREADS - 1) / THREADS * N)), inv_warp = n_warp > 0.0f ? 1.0f / n_warp : 0.0f;
+    if ((at & 31) == 0) counts[at >> 5] = make_float2(inv_warp, n_warp);   // (the first row's barrier is before their first use)
     uint64_t w[NV * N / 2], b[NV * N / 2];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -296,36 +304,40 @@ template <typename T, int NV, int THREADS, int CTAS> __global__ void __launch_bo
 #pragma unroll
         for (int e = 0; e < N / 2; ++e) w[j * N / 2 + e] = f2_of(u[2 * e], u[2 * e + 1]), b[j * N / 2 + e] = f2_of(v[2 * e], v[2 * e + 1]);
     }
-    const float inv = 1.0f / (float)a.cols, n_warp = ln_lanes_sum<32>((float)(max(0, pieces - at + THREADS - 1) / THREADS * N)), inv_warp = n_warp > 0.0f ? 1.0f / n_warp : 0.0f;
-    if ((at & 31) == 0) counts[at >> 5] = make_float2(inv_warp, n_warp);   // (the first row's barrier is before their first use)
-    int i = 0;
+    int i = 0, stage = 0;
+    uint32_t phase = 0;
     bool failed = false;
-    for (; i < turns; ++i) {
+    for (; i < mine; ++i) {
         const int64_t r = (int64_t)blockIdx.x + (int64_t)i * gridDim.x;
-        const bool ok = ring.wait(i, a.status);
-        const uint4* const row = reinterpret_cast<const uint4*>(ring.at + (i % a.stages) * a.bytes);
-        uint64_t f[NV * N / 2], s = 0;   // (two zeros)
+        const bool ok = ring.wait(stage, phase, a.status);
+        const uint4* const row = reinterpret_cast<const uint4*>(ring.at + stage * a.bytes);
+        uint4 v[NV];
+        uint64_t s = 0;   // (two zeros)
         uint32_t top = 0;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
             if (j * THREADS + at < pieces) {
-                const uint4 v = row[j * THREADS + at];
-                f2_unpack<T>(v, f + j * N / 2);
-                if (a.q) top = max(top, P::largest(v));
+                v[j] = row[j * THREADS + at];
+                uint64_t f[N / 2];
+                f2_unpack<T>(v[j], f);
+                if (a.q) top = max(top, P::largest(v[j]));
 #pragma unroll
-                for (int e = 0; e < N / 2; ++e) s = f2_add(s, f[j * N / 2 + e]);
+                for (int e = 0; e < N / 2; ++e) s = f2_add(s, f[e]);
             }
         const float sum = ln_lanes_sum<32>(f2_sum(s)), near = -sum * inv_warp;
         const uint64_t near2 = f2_of(near, near);
         s = 0;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-            if (j * THREADS + at < pieces)
+            if (j * THREADS + at < pieces) {
+                uint64_t f[N / 2];
+                f2_unpack<T>(v[j], f);
 #pragma unroll
                 for (int e = 0; e < N / 2; ++e) {
-                    const uint64_t d = f2_add(f[j * N / 2 + e], near2);
+                    const uint64_t d = f2_add(f[e], near2);
                     s = f2_fma(d, d, s);
                 }
+            }
         float m2 = ln_lanes_sum<32>(f2_sum(s)), mean;
         if (a.q) top = __reduce_max_sync(0xffffffffu, top);
         if ((at & 31) == 0) part[i & 1][at >> 5] = make_float2(sum, m2), tops[i & 1][at >> 5] = top;
@@ -333,31 +345,31 @@ template <typename T, int NV, int THREADS, int CTAS> __global__ void __launch_bo
             failed = true;
             break;
         }
-        if (at == 0) fetch(i + a.stages);   // (the row is in registers)
+        if (at == 0) fetch(i + a.stages, stage);   // (the row is in registers)
+        if (++stage == a.stages) stage = 0, phase ^= 1;
         ln_join<WARPS>(part[i & 1], counts, inv, mean, m2);
         const float rstd = rsqrtf(fmaf(m2, inv, a.eps));
         const uint64_t mean2 = f2_of(-mean, -mean), rstd2 = f2_of(rstd, rstd);
-        if (a.q) {
-            const q_row k(__reduce_max_sync(0xffffffffu, tops[i & 1][at & (WARPS - 1)]));
-            int8_t* const qr = a.q + r * a.ldq;
-            const bool whole = (reinterpret_cast<uintptr_t>(qr) & (N - 1)) == 0;
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-                if (j * THREADS + at < pieces) q_store_pairs<N>(qr + (j * THREADS + at) * N, whole, f + j * N / 2, k);
-            if (at == 0) a.q_scale[r] = k.scale;
-        }
         T* const yr = static_cast<T*>(a.y) + r * a.ldy;
+        int8_t* const qr = a.q + r * a.ldq;
+        const bool whole = (reinterpret_cast<uintptr_t>(qr) & (N - 1)) == 0;
+        const q_row scale(a.q ? __reduce_max_sync(0xffffffffu, tops[i & 1][at & (WARPS - 1)]) : 0u);
 #pragma unroll
         for (int j = 0; j < NV; ++j)
             if (j * THREADS + at < pieces) {
-                uint64_t o[N / 2];
+                uint64_t f[N / 2];
+                f2_unpack<T>(v[j], f);
+                if (a.q) q_store_pairs<N>(qr + (j * THREADS + at) * N, whole, f, scale);
 #pragma unroll
-                for (int e = 0; e < N / 2; ++e) o[e] = f2_fma(f2_mul(f2_add(f[j * N / 2 + e], mean2), rstd2), w[j * N / 2 + e], b[j * N / 2 + e]);
-                reinterpret_cast<uint4*>(yr)[j * THREADS + at] = f2_piece<T>(o);
+                for (int e = 0; e < N / 2; ++e) f[e] = f2_fma(f2_mul(f2_add(f[e], mean2), rstd2), w[j * N / 2 + e], b[j * N / 2 + e]);
+                reinterpret_cast<uint4*>(yr)[j * THREADS + at] = f2_piece<T>(f);
             }
-        if (at == 0 && a.stats) a.stats[r] = make_float2(mean, rstd);
+        if (at == 0) {
+            if (a.stats) a.stats[r] = make_float2(mean, rstd);
+            if (a.q) a.q_scale[r] = scale.scale;
+        }
     }
-    if (failed) ring.drain(i, min(turns, i + a.stages));
+    if (failed) ring.drain(i, min(mine, i + a.stages));
 }
 
 // What the gradient takes its normalised rows from: x, or 8-bit rows with scales.
@@ -482,8 +494,9 @@ __global__ void __launch_bounds__(THREADS < LN_CTA ? LN_CTA : THREADS) layer_nor
 }
 
 // The same through the ring, R rows a turn of a CTA: a stage holds a row's dy and, behind it, x or the 8-bit row.  With the rows' raw numbers and the weight in
-// registers a number is read from shared memory once, and R rows share a barrier (dy and 8-bit rows read twice and the weight twice a row through L1: 8192 x 8192
-// bf16 105 us).
+// registers a number is read from shared memory once, and R rows share a barrier.  (8192 x 8192 bf16, 83 us: the instructions, some 20 a number, half of them what a
+// row costs a thread; 32 numbers a thread of two CTAs an SM, with dy and 8-bit rows read twice and the weight twice a row through L1 105, with g = dy w kept in
+// registers, some of them spilled, 119; before the ring was kept count of without divisions 97.)
 template <typename T, int NV, int R, int THREADS, int CTAS, bool FROM8> __global__ void __launch_bounds__(THREADS, CTAS) layer_norm_grad_ring_kernel(const LnGrad a)
 {
     using P = ln_piece<T, true>;
@@ -494,17 +507,17 @@ template <typename T, int NV, int R, int THREADS, int CTAS, bool FROM8> __global
     const ln_ring ring(ln_raw, a.stages, a.bytes);
     const int at = threadIdx.x, pieces = (int)(a.cols / N), row_bytes = (int)(a.cols * (int64_t)sizeof(T)), x_bytes = FROM8 ? (int)a.cols : row_bytes;
     const int mine = (int)((a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x);   // rows of this CTA
-    const auto fetch = [&](int i) {
+    const auto fetch = [&](int i, int stage) {
         if (i < mine) {
             const int64_t r = (int64_t)blockIdx.x + (int64_t)i * gridDim.x;
-            mbar_expect(ring.full + 8 * (i % a.stages), (uint32_t)(row_bytes + x_bytes));
-            ring.copy(i % a.stages, 0, static_cast<const T*>(a.dy) + r * a.lddy, row_bytes);
-            if constexpr (FROM8) ring.copy(i % a.stages, row_bytes, a.q + r * a.ldx, x_bytes);
-            else ring.copy(i % a.stages, row_bytes, static_cast<const T*>(a.x) + r * a.ldx, x_bytes);
+            mbar_expect(ring.full + 8 * stage, (uint32_t)(row_bytes + x_bytes));
+            ring.copy(stage, 0, static_cast<const T*>(a.dy) + r * a.lddy, row_bytes);
+            if constexpr (FROM8) ring.copy(stage, row_bytes, a.q + r * a.ldx, x_bytes);
+            else ring.copy(stage, row_bytes, static_cast<const T*>(a.x) + r * a.ldx, x_bytes);
         }
     };
     if (at == 0)
-        for (int i = 0; i < a.stages; ++i) fetch(i);
+        for (int i = 0; i < a.stages; ++i) fetch(i, i);
     uint64_t w[NV * N / 2], sum_w[NV * N / 2] = {}, sum_b[NV * N / 2] = {};   // (zeros)
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -516,7 +529,8 @@ template <typename T, int NV, int R, int THREADS, int CTAS, bool FROM8> __global
         for (int e = 0; e < N / 2; ++e) w[j * N / 2 + e] = f2_of(u[2 * e], u[2 * e + 1]);
     }
     const float inv = 1.0f / (float)a.cols;
-    int i = 0;
+    int i = 0, stage = 0;
+    uint32_t phase = 0;
     bool failed = false;
     float2 next_st[R];
     float next_s[R];
@@ -548,17 +562,19 @@ template <typename T, int NV, int R, int THREADS, int CTAS, bool FROM8> __global
         };
         bool ok = true;
         float g0[R], g1[R];
+        int at_stage[R];
 #pragma unroll
         for (int u = 0; u < R; ++u) {
             uint64_t s0 = 0, s1 = 0;
+            at_stage[u] = stage;
             if (i + u < mine) {
-                ok = ok && ring.wait(i + u, a.status);
-                const unsigned char* const stage = ring.at + ((i + u) % a.stages) * a.bytes;
+                ok = ok && ring.wait(stage, phase, a.status);
+                const unsigned char* const from = ring.at + stage * a.bytes;
 #pragma unroll
                 for (int j = 0; j < NV; ++j)
                     if (j * THREADS + at < pieces) {
-                        dv[u][j] = reinterpret_cast<const uint4*>(stage)[j * THREADS + at];
-                        xv[u][j] = reinterpret_cast<const raw_x*>(stage + row_bytes)[j * THREADS + at];
+                        dv[u][j] = reinterpret_cast<const uint4*>(from)[j * THREADS + at];
+                        xv[u][j] = reinterpret_cast<const raw_x*>(from + row_bytes)[j * THREADS + at];
                         uint64_t d[N / 2], h[N / 2];
                         f2_unpack<T>(dv[u][j], d);
                         normalise(u, xv[u][j], h);
@@ -571,6 +587,7 @@ template <typename T, int NV, int R, int THREADS, int CTAS, bool FROM8> __global
                         }
                     }
             }
+            if (++stage == a.stages) stage = 0, phase ^= 1;
             g0[u] = f2_sum(s0), g1[u] = f2_sum(s1);
         }
 #pragma unroll
@@ -588,7 +605,7 @@ template <typename T, int NV, int R, int THREADS, int CTAS, bool FROM8> __global
         }
         if (at == 0) {   // (the rows are in registers)
 #pragma unroll
-            for (int u = 0; u < R; ++u) fetch(i + u + a.stages);
+            for (int u = 0; u < R; ++u) fetch(i + u + a.stages, at_stage[u]);
         }
 #pragma unroll
         for (int u = 0; u < R; ++u) {
@@ -705,12 +722,13 @@ template <int V, int LANES> __global__ void __launch_bounds__(LN_CTA) layer_norm
 }
 
 // Stages of a ring for `ctas` CTAs on an SM: what fits, LN_STAGES at most.
-constexpr int LN_RING_ROW = 65536;   // bytes of a row
-constexpr size_t LN_RING_SHARED = 222 * 1024;
+constexpr int LN_RING_ROW = 65536;   // bytes of a stage
+constexpr size_t LN_RING_SHARED = 222 * 1024, LN_RING_LESS = 168 * 1024;   // of an SM; where the smaller has room for two stages, the rest is L1's
 template <typename K, typename A> int ln_ring_stages(s2v_ctx* ctx, K kernel, A& a, int ctas)
 {
     const size_t fixed = ln_ring::shared(0, 0) + 1024 + 512;   // (what a CTA takes besides, and the kernel's own)
-    a.stages = (int)((LN_RING_SHARED / ctas - fixed) / a.bytes);
+    const auto stages = [&](size_t shared) { return (int)((shared / ctas - fixed) / a.bytes); };
+    a.stages = stages(LN_RING_LESS) >= 2 ? stages(LN_RING_LESS) : stages(LN_RING_SHARED);
     a.stages = a.stages < LN_STAGES ? a.stages : LN_STAGES;
     S2V_CUDA_OK(ctx, s2v_allow_shared(kernel, LN_RING_SHARED));
     return S2V_OK;
@@ -729,7 +747,7 @@ int ln_launch(s2v_ctx* ctx, cudaStream_t st, int64_t rows, int64_t cols, const T
         return (int)S2V_OK;
     };
     if constexpr (VEC) {
-        if (pieces > 128 && pieces * 16 <= LN_RING_ROW && rows <= INT32_MAX) {
+        if (pieces > 128 && cols <= 16384 && rows <= INT32_MAX) {
             LnNorm a{rows, cols, ldx, ldy, ldq, x, weight, bias, eps, y, stats, q, q_scale, 0, (int)((pieces * 16 + 127) / 128 * 128), ctx->dstatus_dev};
             const auto ring = [&](auto kernel, int threads, int ctas) {
                 const int rc = ln_ring_stages(ctx, kernel, a, ctas);
@@ -740,11 +758,10 @@ int ln_launch(s2v_ctx* ctx, cudaStream_t st, int64_t rows, int64_t cols, const T
                 return (int)S2V_OK;
             };
             constexpr int N = ln_piece<T, true>::N;
-            if (pieces <= 256) return ring(layer_norm_ring_kernel<T, 1, 256, 4>, 256, 4);
-            if (pieces <= 512) return ring(layer_norm_ring_kernel<T, 2, 256, 3>, 256, 3);
-            if (pieces <= 1024) return ring(layer_norm_ring_kernel<T, 4, 256, 2>, 256, 2);
-            if (pieces <= 2048) return ring(layer_norm_ring_kernel<T, 4, 512, 1>, 512, 1);
-            if constexpr (N == 4) return ring(layer_norm_ring_kernel<T, 8, 512, 1>, 512, 1);
+            if (cols <= 2048) return ring(layer_norm_ring_kernel<T, 32 / N, 64, 8>, 64, 8);
+            if (cols <= 4096) return ring(layer_norm_ring_kernel<T, 32 / N, 128, 4>, 128, 4);
+            if (cols <= 8192) return ring(layer_norm_ring_kernel<T, 32 / N, 256, 2>, 256, 2);
+            if (cols <= 16384) return ring(layer_norm_ring_kernel<T, 32 / N, 512, 1>, 512, 1);
         }
     }
     if (pieces <= 8) return go(layer_norm_kernel<T, VEC, 1, 8>, 8);
@@ -790,7 +807,7 @@ template <typename T, bool FROM8> int ln_grad_launch(s2v_ctx* ctx, cudaStream_t 
             // (at least two rows of a CTA in the ring; the 8-bit rows on 16-byte boundaries too)
             const bool whole = !FROM8 || (a.cols % 16 == 0 && s2v_aligned16(a.q) && (a.rows <= 1 || a.ldx % 16 == 0));
             if (pieces > 128 && whole && a.rows <= INT32_MAX && a.cols * (int64_t)(sizeof(T) + (FROM8 ? 1 : sizeof(T))) <= LN_RING_ROW) {
-                if (pieces <= 256) return ring(layer_norm_grad_ring_kernel<T, 1, 2, 256, 3, FROM8>, 256, 3);
+                if (pieces <= 256) return ring(layer_norm_grad_ring_kernel<T, 2, 2, 128, 4, FROM8>, 128, 4);
                 if (pieces <= 512) return ring(layer_norm_grad_ring_kernel<T, 2, 2, 256, 2, FROM8>, 256, 2);
                 if (pieces <= 1024) return ring(layer_norm_grad_ring_kernel<T, 2, 2, 512, 1, FROM8>, 512, 1);
                 if constexpr (N == 4) {
