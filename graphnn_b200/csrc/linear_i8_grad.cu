@@ -3,9 +3,11 @@
 // The rows' scales go to dy, in fp32:  dW_jl = sum_i (dy_ij scale_i) q_il.  8-bit integers are exact in 16 bits, so one rounding is left, that of dy_ij scale_i to
 // the 16 bits that the tensor cores multiply: half a step of bf16 or fp16, as dy itself has; fp32 goes as three bf16 numbers.  For fp16 a column is
 // first scaled by a power of two that puts its largest product's binade at 2^14, since scale_i can take dy_ij out of fp16's normal range; dW's row is scaled back.
+// Where dW is small and the rows are many, that and the products are one kernel (linear_i8_direct.cu); else both matrices are written in 16 bits first, which many
+// tiles then read.
 #include <algorithm>
 
-#include "mm16.cuh"
+#include "linear_i8_grad.cuh"
 
 namespace
 {
@@ -123,19 +125,25 @@ template <typename H> __global__ void __launch_bounds__(256) grad_q_kernel(int64
     }
 }
 
+// Where things lie in the workspace.  Matrices in 16 bits are made for a piece of the rows at a time, dW's sums of several pieces kept in fp32.
+constexpr size_t LG_BYTES = (size_t)256 << 20;   // of a piece, about
 struct LgSpace {
-    size_t dy = 0, q = 0, columns = 0, factor = 0, lines = 0, bytes = 0;
-    int64_t ldn = 0, ldk = 0, parts = 0;
-    LgSpace(int64_t m, int64_t n, int64_t k, int type)
+    size_t dy = 0, q = 0, columns = 0, factor = 0, lines = 0, sum = 0, bytes = 0;
+    int64_t ldn = 0, ldk = 0, parts = 0, piece = 0, pieces = 1, slabs = LG_SLABS;   // slabs: of a piece
+    LgSpace(int64_t m, int64_t n, int64_t k, int type, bool direct)
     {
         const auto take = [&](size_t& at, size_t size) { at = bytes, bytes += (size + 255) / 256 * 256; };
         parts = type == S2V_F32 ? 3 : 1;
         ldn = (n + 7) / 8 * 8, ldk = (k + 7) / 8 * 8;
-        take(dy, (size_t)m * ldn * 2 * parts);
-        take(q, (size_t)m * ldk * 2);
-        take(columns, (size_t)LG_SLABS * n * sizeof(float));
+        if (!direct) {
+            piece = std::min(m, std::max<int64_t>(4096, (int64_t)(LG_BYTES / (size_t)(ldn * 2 * parts + ldk * 2)) / 64 * 64)), pieces = (m + piece - 1) / piece;
+            slabs = std::max<int64_t>(1, LG_SLABS / pieces);
+            take(dy, (size_t)piece * ldn * 2 * parts), take(q, (size_t)piece * ldk * 2);
+            if (pieces > 1) take(sum, (size_t)n * mm16_pitch(k) * sizeof(float));
+        }
+        take(columns, (size_t)std::max<int64_t>(pieces * slabs, LG_SLABS) * n * sizeof(float));
         take(factor, (size_t)n * 2 * sizeof(float));
-        take(lines, mm16_lines_bytes(m, (int)parts));
+        take(lines, direct ? linear_i8_direct_floats(m, n, k) * sizeof(float) : mm16_lines_bytes(piece, (int)parts));
     }
 };
 
@@ -146,7 +154,8 @@ extern "C" {
 size_t s2v_linear_i8_grad_workspace_bytes(int64_t m, int64_t n, int64_t k, int dy_type)
 {
     if (m <= 0 || n <= 0 || k <= 0 || m > INT32_MAX || n > INT32_MAX || k > INT32_MAX || !s2v_dtype_ok(dy_type)) return 0;
-    return LgSpace(m, n, k, dy_type).bytes;
+    // (rows that don't lie on 16-byte boundaries take the other way)
+    return std::max(LgSpace(m, n, k, dy_type, false).bytes, linear_i8_direct_takes(m, n, k, dy_type) ? LgSpace(m, n, k, dy_type, true).bytes : 0);
 }
 
 int s2v_linear_i8_grad(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, int64_t k, int dy_type, const void* dy, int64_t lddy, const int8_t* q, int64_t ldq,
@@ -171,50 +180,68 @@ int s2v_linear_i8_grad(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, in
         return S2V_OK;
     }
     unsigned char* const ws = static_cast<unsigned char*>(workspace);
-    const LgSpace space(m, n, k, dy_type);
+    const bool direct = linear_i8_direct_takes(m, n, k, dy_type) && linear_i8_direct_lies(m, dy_type, dy, lddy, q, ldq);
+    const LgSpace space(m, n, k, dy_type, direct);
     float* const columns = reinterpret_cast<float*>(ws + space.columns);
     float* const factor = dy_type == S2V_F16 ? reinterpret_cast<float*>(ws + space.factor) : nullptr;
-    LgRows r{m, n, lddy, 0, dy, q_scale, nullptr, s2v_aligned16(dy) && (m <= 1 || lddy * es % 16 == 0), 1, reinterpret_cast<uint16_t*>(ws + space.dy), space.ldn, m * space.ldn, columns};
+    LgRows r{m, n, lddy, 0, dy, q_scale, nullptr, s2v_aligned16(dy) && (m <= 1 || lddy * es % 16 == 0), 1, reinterpret_cast<uint16_t*>(ws + space.dy), space.ldn, space.piece * space.ldn, columns};
     while (r.groups < 32 && r.groups * 8 < n) r.groups *= 2;
     const int64_t blocks = (n + r.groups * 8 - 1) / (r.groups * 8), lanes = LG_THREADS / r.groups;
-    const int64_t slabs = std::max<int64_t>(1, std::min({(int64_t)LG_SLABS, (8 * (int64_t)ctx->sm_count + blocks - 1) / blocks, (m + 4 * lanes - 1) / (4 * lanes)}));
-    r.share = (m + slabs - 1) / slabs;
-    const dim3 grid((unsigned)blocks, (unsigned)((m + r.share - 1) / r.share));
-    const auto lines = [&](auto kernel, float* out) {
-        kernel<<<(unsigned)((n + 31) / 32), 256, 0, st>>>((int)grid.y, n, columns, out);
+    // `rows` of r in at most `most` shares; how many there are
+    const auto shared_out = [&](int64_t rows, int64_t most) {
+        const int64_t slabs = std::max<int64_t>(1, std::min({most, (8 * (int64_t)ctx->sm_count + blocks - 1) / blocks, (rows + 4 * lanes - 1) / (4 * lanes)}));
+        r.m = rows, r.share = (rows + slabs - 1) / slabs;
+        return (rows + r.share - 1) / r.share;
+    };
+    const auto lines = [&](auto kernel, int64_t count, float* out) {
+        kernel<<<(unsigned)((n + 31) / 32), 256, 0, st>>>((int)count, n, columns, out);
         S2V_CHECK_LAUNCH(ctx, "grad_lines_kernel");
         return (int)S2V_OK;
     };
-    int done = s2v_by_dtype(dy_type, [&](auto type) {
-        using T = decltype(type);
-        if (factor) {
-            grad_rows_kernel<T, false><<<grid, LG_THREADS, 0, st>>>(r);
-            S2V_CHECK_LAUNCH(ctx, "grad_rows_kernel");
-            const int rc = lines(grad_lines_kernel<false>, factor);
-            if (rc != S2V_OK) return rc;
-            r.factor = factor;
-        }
-        grad_rows_kernel<T, true><<<grid, LG_THREADS, 0, st>>>(r);
+    if (factor) {
+        const int64_t slabs = shared_out(m, LG_SLABS);
+        grad_rows_kernel<__half, false><<<dim3((unsigned)blocks, (unsigned)slabs), LG_THREADS, 0, st>>>(r);
         S2V_CHECK_LAUNCH(ctx, "grad_rows_kernel");
-        return dbias ? lines(grad_lines_kernel<true>, dbias) : (int)S2V_OK;
-    });
-    if (done != S2V_OK) return done;
-    {
-        const int64_t all = (m * (space.ldk / 8) + 255) / 256, cap = 32 * (int64_t)ctx->sm_count;
-        const int wide = reinterpret_cast<uintptr_t>(q) % 8 == 0 && (m <= 1 || ldq % 8 == 0);
-        const auto kernel = dy_type == S2V_F16 ? grad_q_kernel<__half> : grad_q_kernel<__nv_bfloat16>;
-        kernel<<<(unsigned)(all < cap ? all : cap), 256, 0, st>>>(m, k, q, ldq, wide, reinterpret_cast<uint16_t*>(ws + space.q), space.ldk);
-        S2V_CHECK_LAUNCH(ctx, "grad_q_kernel");
+        const int rc = lines(grad_lines_kernel<false>, slabs, factor);
+        if (rc != S2V_OK) return rc;
+        r.factor = factor;
+    }
+    if (direct) {
+        const linear_i8_grad_args d{m, n, k, lddy, ldq, lddw, dy_type, dy, q, q_scale, factor, factor ? factor + n : nullptr, dW};
+        int shares = 0;
+        const int rc = linear_i8_direct(ctx, st, d, reinterpret_cast<float*>(ws + space.lines), dbias ? columns : nullptr, &shares);
+        return rc == S2V_OK && dbias ? lines(grad_lines_kernel<true>, shares, dbias) : rc;
     }
     mm16_args g;
     g.type = dy_type == S2V_F16 ? S2V_F16 : S2V_BF16;
-    g.a.p = ws + space.dy, g.a.rows = m, g.a.cols = n, g.a.ld = space.ldn, g.a.part = r.part, g.a.parts = (int)space.parts;
-    g.b.p = ws + space.q, g.b.rows = m, g.b.cols = k, g.b.ld = space.ldk;
-    g.m = n, g.n = k, g.k = m;
+    g.a.p = ws + space.dy, g.a.cols = n, g.a.ld = space.ldn, g.a.part = r.part, g.a.parts = (int)space.parts;
+    g.b.p = ws + space.q, g.b.cols = k, g.b.ld = space.ldk;
+    g.m = n, g.n = k;
     g.alpha = factor ? factor + n : nullptr, g.alpha_rows = 1;
-    g.lines = reinterpret_cast<float*>(ws + space.lines);
-    g.out = dW, g.out_type = dy_type, g.ldo = lddw;
-    return mm16_launch(ctx, st, MM16_OUT_ACROSS, g);
+    g.lines = reinterpret_cast<float*>(ws + space.lines), g.sum = reinterpret_cast<float*>(ws + space.sum);
+    g.out_type = dy_type, g.ldo = lddw;
+    int64_t all_lines = 0;
+    for (int64_t first = 0; first < m; first += space.piece) {
+        const int64_t rows = std::min(space.piece, m - first), slabs = shared_out(rows, space.slabs);
+        r.dy = static_cast<const unsigned char*>(dy) + (size_t)first * (m > 1 ? lddy : 0) * es, r.scale = q_scale + first, r.lines = columns + all_lines * n;
+        all_lines += slabs;
+        int rc = s2v_by_dtype(dy_type, [&](auto type) {
+            grad_rows_kernel<decltype(type), true><<<dim3((unsigned)blocks, (unsigned)slabs), LG_THREADS, 0, st>>>(r);
+            S2V_CHECK_LAUNCH(ctx, "grad_rows_kernel");
+            return (int)S2V_OK;
+        });
+        if (rc != S2V_OK) return rc;
+        const int64_t units = (rows * (space.ldk / 8) + 255) / 256, cap = 32 * (int64_t)ctx->sm_count;
+        const int wide = reinterpret_cast<uintptr_t>(q) % 8 == 0 && (m <= 1 || ldq % 8 == 0);
+        const auto kernel = dy_type == S2V_F16 ? grad_q_kernel<__half> : grad_q_kernel<__nv_bfloat16>;
+        kernel<<<(unsigned)(units < cap ? units : cap), 256, 0, st>>>(rows, k, q + (size_t)first * (m > 1 ? ldq : 0), ldq, wide, reinterpret_cast<uint16_t*>(ws + space.q), space.ldk);
+        S2V_CHECK_LAUNCH(ctx, "grad_q_kernel");
+        g.a.rows = g.b.rows = g.k = rows, g.add = first > 0;
+        if (first + rows == m) g.out = dW;
+        rc = mm16_launch(ctx, st, MM16_OUT_ACROSS, g);
+        if (rc != S2V_OK) return rc;
+    }
+    return dbias ? lines(grad_lines_kernel<true>, all_lines, dbias) : (int)S2V_OK;
 }
 
 }  // extern "C"

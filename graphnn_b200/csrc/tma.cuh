@@ -30,6 +30,19 @@ inline bool s2v_byte_matrix_map(CUtensorMap* map, const void* base, int64_t rows
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// A [rows x cols] matrix of `es`-byte numbers, rows `ld` numbers apart (a multiple of 16 bytes), copied in boxes of `box_rows` rows of `box_cols` numbers (256 at most) as they
+// lie; columns and rows outside the matrix arrive as zeros.
+inline bool s2v_matrix_map(CUtensorMap* map, int es, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_cols, int box_rows)
+{
+    const auto encode = s2v_tensor_map_encoder();
+    if (!encode) return false;
+    const int64_t pitch = rows > 1 ? ld * es : (cols * es + 15) / 16 * 16;   // (the leading dimension of a single row is not the caller's to get right)
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, step[2] = {1, 1};
+    return encode(map, es == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : es == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims,
+                  strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // A row-major output of `es`-byte numbers (S2V_F32, S2V_F16, S2V_BF16), written in boxes of 32 rows of 64 bytes that lie in the 64-byte swizzle.
 inline bool s2v_output_map(CUtensorMap* map, int dtype, void* base, int64_t rows, int64_t cols, int64_t ld)
 {
