@@ -6,6 +6,7 @@
 // (what the tensor cores multiply; three parts of it where x and W are fp32) and multiplies it.  G in 16 bits is off by half a step of them, as x and W are.
 #include <algorithm>
 
+#include "cross_entropy_few.cuh"
 #include "mm16.cuh"
 
 namespace
@@ -94,7 +95,8 @@ int xe_join(s2v_ctx* ctx, cudaStream_t st, int64_t rows_n, int lines, xe_rows ro
         S2V_CHECK_LAUNCH(ctx, "xe_join_kernel");
         return (int)S2V_OK;
     };
-    return rows_n >= 2048 || lines <= 32 ? go(xe_join_kernel<8>, 8) : go(xe_join_kernel<64>, 64);
+    // (one row of 2048 lines by 64 threads 10 us)
+    return rows_n >= 2048 || lines <= 32 ? go(xe_join_kernel<8>, 8) : rows_n > 64 ? go(xe_join_kernel<64>, 64) : go(xe_join_kernel<256>, 256);
 }
 
 // G in 16 bits of fp16 is scaled by a power of two that puts the largest row weight's binade at 2^14: its steps are then 2^-38 of that and less.
@@ -221,6 +223,7 @@ extern "C" {
 size_t s2v_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t vocab, int64_t k, int type, int grad)
 {
     if (rows <= 0 || vocab <= 0 || k <= 0 || rows > INT32_MAX || vocab > INT32_MAX || k > INT32_MAX || !s2v_dtype_ok(type)) return 0;
+    if (xe_few_takes(rows, vocab, k)) return xe_few_bytes(rows, vocab);
     size_t most = 0;   // wherever the matrices lie
     for (int form = 0; form < (grad ? 4 : 2); ++form)
         if ((form & 1) || type != S2V_F32) most = std::max(most, xe_space(rows, vocab, k, type, form & 2, form & 1).bytes);
@@ -239,6 +242,7 @@ int s2v_linear_cross_entropy(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int6
     if (!workspace || workspace_bytes < s2v_linear_cross_entropy_workspace_bytes(rows, vocab, k, type, 0)) return bad(S2V_ERR_WORKSPACE, "workspace too small");
     if (!s2v_aligned16(workspace)) return bad(S2V_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
     cudaStream_t st = s2v_pick_stream(ctx, stream);
+    if (xe_few_takes(rows, vocab, k)) return xe_few_loss(ctx, st, rows, vocab, k, type, x, ldx, W, ldw, target, row_weight, loss, stats);
     unsigned char* const ws = static_cast<unsigned char*>(workspace);
     const xe_call c(ctx, st, rows, vocab, k, type, x, ldx, W, ldw, target, row_weight, ws, false);
     const xe_space& space = c.space;
@@ -277,6 +281,7 @@ int s2v_linear_cross_entropy_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows,
     if (!dx && !dW) return S2V_OK;
     if (!workspace || workspace_bytes < s2v_linear_cross_entropy_workspace_bytes(rows, vocab, k, type, 1)) return bad(S2V_ERR_WORKSPACE, "workspace too small");
     if (!s2v_aligned16(workspace)) return bad(S2V_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
+    if (xe_few_takes(rows, vocab, k)) return xe_few_grad(ctx, st, rows, vocab, k, type, x, ldx, W, ldw, target, row_weight, stats, workspace, dx, lddx, dW, lddw);
     unsigned char* const ws = static_cast<unsigned char*>(workspace);
     const xe_call c(ctx, st, rows, vocab, k, type, x, ldx, W, ldw, target, row_weight, ws, true);
     const xe_space& space = c.space;
