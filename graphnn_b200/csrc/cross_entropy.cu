@@ -175,7 +175,8 @@ int check(s2v_ctx* ctx, const char* name, int64_t rows, int64_t vocab, int64_t k
     const auto bad = [&](int status, const char* what) { return s2v_fail(ctx, status, std::string(name) + ": " + what); };
     if (rows < 0 || vocab < 1 || k < 1) return bad(S2V_ERR_INVALID_ARG, "negative size, or no classes or no columns");
     if (!s2v_dtype_ok(type)) return bad(S2V_ERR_INVALID_ARG, "unknown element type");
-    if (rows > INT32_MAX || vocab > INT32_MAX || k > INT32_MAX) return bad(S2V_ERR_UNSUPPORTED, "a size above 2^31 - 1");
+    if (rows > INT32_MAX || vocab > INT32_MAX || k > INT32_MAX || !mm16_size_ok(rows, k) || !mm16_size_ok(vocab, k))
+        return bad(S2V_ERR_UNSUPPORTED, "a size above 2^31 - 1, or a matrix above 2^56 numbers");
     if (rows == 0) return S2V_OK;
     if (!x || !W || !target) return bad(S2V_ERR_INVALID_ARG, "NULL pointer");
     if ((rows > 1 && ldx < k) || (vocab > 1 && ldw < k)) return bad(S2V_ERR_INVALID_ARG, "leading dimension below the number of columns");
@@ -223,11 +224,12 @@ extern "C" {
 size_t s2v_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t vocab, int64_t k, int type, int grad)
 {
     if (rows <= 0 || vocab <= 0 || k <= 0 || rows > INT32_MAX || vocab > INT32_MAX || k > INT32_MAX || !s2v_dtype_ok(type)) return 0;
+    if (!mm16_size_ok(rows, k) || !mm16_size_ok(vocab, k)) return 0;
     if (xe_few_takes(rows, vocab, k)) return xe_few_bytes(rows, vocab);
     size_t most = 0;   // wherever the matrices lie
     for (int form = 0; form < (grad ? 4 : 2); ++form)
         if ((form & 1) || type != S2V_F32) most = std::max(most, xe_space(rows, vocab, k, type, form & 2, form & 1).bytes);
-    return most;
+    return most + MM16_SLACK;
 }
 
 int s2v_linear_cross_entropy(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t vocab, int64_t k, int type, const void* x, int64_t ldx, const void* W, int64_t ldw,
@@ -243,7 +245,7 @@ int s2v_linear_cross_entropy(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int6
     if (!s2v_aligned16(workspace)) return bad(S2V_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
     cudaStream_t st = s2v_pick_stream(ctx, stream);
     if (xe_few_takes(rows, vocab, k)) return xe_few_loss(ctx, st, rows, vocab, k, type, x, ldx, W, ldw, target, row_weight, loss, stats);
-    unsigned char* const ws = static_cast<unsigned char*>(workspace);
+    unsigned char* const ws = mm16_space(workspace);
     const xe_call c(ctx, st, rows, vocab, k, type, x, ldx, W, ldw, target, row_weight, ws, false);
     const xe_space& space = c.space;
     mm16_args a = c.args;
@@ -282,7 +284,7 @@ int s2v_linear_cross_entropy_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows,
     if (!workspace || workspace_bytes < s2v_linear_cross_entropy_workspace_bytes(rows, vocab, k, type, 1)) return bad(S2V_ERR_WORKSPACE, "workspace too small");
     if (!s2v_aligned16(workspace)) return bad(S2V_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
     if (xe_few_takes(rows, vocab, k)) return xe_few_grad(ctx, st, rows, vocab, k, type, x, ldx, W, ldw, target, row_weight, stats, workspace, dx, lddx, dW, lddw);
-    unsigned char* const ws = static_cast<unsigned char*>(workspace);
+    unsigned char* const ws = mm16_space(workspace);
     const xe_call c(ctx, st, rows, vocab, k, type, x, ldx, W, ldw, target, row_weight, ws, true);
     const xe_space& space = c.space;
     // x with zeros in the rows that are left out, whatever these hold: their zeros of G meet zeros in dW

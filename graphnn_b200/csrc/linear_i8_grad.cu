@@ -154,8 +154,9 @@ extern "C" {
 size_t s2v_linear_i8_grad_workspace_bytes(int64_t m, int64_t n, int64_t k, int dy_type)
 {
     if (m <= 0 || n <= 0 || k <= 0 || m > INT32_MAX || n > INT32_MAX || k > INT32_MAX || !s2v_dtype_ok(dy_type)) return 0;
+    if (!mm16_size_ok(m, n) || !mm16_size_ok(m, k) || !mm16_size_ok(n, k)) return 0;
     // (rows that don't lie on 16-byte boundaries take the other way)
-    return std::max(LgSpace(m, n, k, dy_type, false).bytes, linear_i8_direct_takes(m, n, k, dy_type) ? LgSpace(m, n, k, dy_type, true).bytes : 0);
+    return std::max(LgSpace(m, n, k, dy_type, false).bytes, linear_i8_direct_takes(m, n, k, dy_type) ? LgSpace(m, n, k, dy_type, true).bytes : 0) + MM16_SLACK;
 }
 
 int s2v_linear_i8_grad(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, int64_t k, int dy_type, const void* dy, int64_t lddy, const int8_t* q, int64_t ldq,
@@ -166,7 +167,8 @@ int s2v_linear_i8_grad(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, in
     if (m < 0 || n < 0 || k < 1) return bad(S2V_ERR_INVALID_ARG, "negative size or no columns");
     if (!s2v_dtype_ok(dy_type)) return bad(S2V_ERR_INVALID_ARG, "unknown element type");
     if (n == 0) return S2V_OK;
-    if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX) return bad(S2V_ERR_UNSUPPORTED, "a size above 2^31 - 1");
+    if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX || !mm16_size_ok(m, n) || !mm16_size_ok(m, k) || !mm16_size_ok(n, k))
+        return bad(S2V_ERR_UNSUPPORTED, "a size above 2^31 - 1, or a matrix above 2^56 numbers");
     const int64_t es = (int64_t)s2v_dtype_bytes(dy_type);
     if (!dW || (m > 0 && (!dy || !q || !q_scale))) return bad(S2V_ERR_INVALID_ARG, "NULL pointer");
     if ((m > 1 && (lddy < n || ldq < k)) || (n > 1 && lddw < k)) return bad(S2V_ERR_INVALID_ARG, "leading dimension below the number of columns");
@@ -179,7 +181,7 @@ int s2v_linear_i8_grad(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, in
         if (dbias) S2V_CUDA_OK(ctx, cudaMemsetAsync(dbias, 0, (size_t)n * sizeof(float), st));
         return S2V_OK;
     }
-    unsigned char* const ws = static_cast<unsigned char*>(workspace);
+    unsigned char* const ws = mm16_space(workspace);
     const bool direct = linear_i8_direct_takes(m, n, k, dy_type) && linear_i8_direct_lies(m, dy_type, dy, lddy, q, ldq);
     const LgSpace space(m, n, k, dy_type, direct);
     float* const columns = reinterpret_cast<float*>(ws + space.columns);

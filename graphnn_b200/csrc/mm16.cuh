@@ -46,6 +46,11 @@ struct mm16_args {
 };
 enum mm16_kind { MM16_SUMS, MM16_SOFTMAX_GRAD, MM16_OUT, MM16_OUT_ACROSS };   // ... with B across; with A and B across
 
+// Places in a workspace are 256 bytes apart, from its first such boundary on (outputs leave 32 bytes at a time; callers promise 16): what to add to its size.
+constexpr size_t MM16_SLACK = 240;
+inline unsigned char* mm16_space(void* workspace) { return reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~(uintptr_t)255); }
+// whether the bytes of a matrix of 16 or fewer bytes a number are far from passing 64 bits
+inline bool mm16_size_ok(int64_t rows, int64_t cols) { return cols == 0 || rows <= ((int64_t)1 << 56) / cols; }
 inline int64_t mm16_pitch(int64_t n) { return (n + 7) / 8 * 8; }
 int mm16_sum_lines(const s2v_ctx* ctx, int64_t m, int64_t n);                     // as the launch will write them
 int64_t mm16_sum_lines_most(int64_t n);                                           // the most of any launch

@@ -284,7 +284,7 @@ int s2v_layer_norm_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t c
 /* The weight gradient of a dense layer y = x W^T + bias whose input was kept as 8-bit rows, x_ij = q_scale_i q_ij (s2v_quantize_rows_i8, s2v_layer_norm,
  * or what s2v_linear_i8 multiplied):
  *     dW_jl = sum_i dy_ij q_scale_i q_il;   dbias_j = sum_i dy_ij
- * dy : [m x n] of dy_type; q : int8 [m x k]; dW : [n x k] of dy_type; dbias : fp32 [n] or NULL.  With m = 0 they are zeros.  k is 1 or more.
+ * in fp32 sums, with dy q_scale rounded to dy_type once more where that has 16 bits.  dy : [m x n] of dy_type; q : int8 [m x k]; dW : [n x k] of dy_type; dbias : fp32 [n] or NULL.  With m = 0 they are zeros.  k is 1 or more.
  * An infinity or NaN in dy or q_scale makes the sums that it is part of infinite or NaN. */
 size_t s2v_linear_i8_grad_workspace_bytes(int64_t m, int64_t n, int64_t k, int dy_type);
 int s2v_linear_i8_grad(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, int64_t k, int dy_type, const void* dy, int64_t lddy, const int8_t* q,
@@ -292,8 +292,9 @@ int s2v_linear_i8_grad(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, in
 /* Softmax cross entropy of the logits z = x W^T against one class a row; z is never in memory as a whole:
  *     loss_i = row_weight_i (log sum_j exp z_ij - z_it),  t = target_i
  * x : [rows x k], W : [vocab x k] (a class a row), both of `type`; target : int32 [rows]; row_weight : [rows] or NULL (1).  A row whose target lies outside
- * [0, vocab), or whose row_weight is 0, is left out: loss 0 and gradient 0, whatever x holds there.  A row with an infinity or NaN among its logits
- * has NaN as its loss (logits of -infinity, which only overflowing products give, among them where they meet).  loss : [rows]; stats : float [rows x 2], 8-byte aligned, or NULL, for the gradient.
+ * [0, vocab), or whose row_weight is 0, is left out: loss 0 and gradient 0, whatever x holds there.  A row with NaN or +infinity among its logits has NaN as its
+ * loss, and makes dW NaN.  The loss keeps its digits where the own class has nearly all of the probability.  Logits are fp32 sums (of fp32 operands as three bf16 numbers each, off by
+ * some 2^-24 of sum |x W|); fp32 matrices with an infinity give NaN.  loss : [rows]; stats : float [rows x 2], 8-byte aligned, or NULL, for the gradient.
  * `grad` of the workspace's size: whether it has to do for s2v_linear_cross_entropy_grad too. */
 size_t s2v_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t vocab, int64_t k, int type, int grad);
 int s2v_linear_cross_entropy(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t vocab, int64_t k, int type, const void* x, int64_t ldx,
@@ -302,7 +303,8 @@ int s2v_linear_cross_entropy(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int6
 /* The gradients of sum_i loss_i, from the `stats` that s2v_linear_cross_entropy wrote for the same x, W and target; row_weight is that of this call (the
  * gradient that arrives at each row's loss):
  *     G_ij = row_weight_i (exp z_ij / sum_j exp z_ij - [j = t]);   dx = G W;   dW = G^T x
- * dx : [rows x k], dW : [vocab x k] of `type`; either may be NULL; they overlap no input and not each other. */
+ * dx : [rows x k], dW : [vocab x k] of `type`; either may be NULL; they overlap no input and not each other.  Where `type` has 16 bits, G is rounded to it for the
+ * products (half a step of it, as x and W have; the own class's part of dx is not), with fp32 sums. */
 int s2v_linear_cross_entropy_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t vocab, int64_t k, int type, const void* x, int64_t ldx,
                                   const void* W, int64_t ldw, const int32_t* target, const float* row_weight, const float* stats, void* workspace,
                                   size_t workspace_bytes, void* dx, int64_t lddx, void* dW, int64_t lddw);

@@ -104,7 +104,7 @@ def both(ctx, x, W, target, weight, stream=None):
 # ---------------------------------------------------------------- without a GPU
 def test_workspace_sizes_without_a_gpu():
     size = capi.load_library().s2v_linear_cross_entropy_workspace_bytes
-    for bad in ((0, 5, 5, 0, 1), (5, 0, 5, 0, 1), (5, 5, 0, 0, 1), (-1, 5, 5, 0, 1), (5, 5, 5, 3, 1), (5, 5, 5, -1, 0), (1 << 31, 5, 5, 0, 0), (5, 1 << 40, 5, 0, 0)):
+    for bad in ((0, 5, 5, 0, 1), (5, 0, 5, 0, 1), (5, 5, 0, 0, 1), (-1, 5, 5, 0, 1), (5, 5, 5, 3, 1), (5, 5, 5, -1, 0), (1 << 31, 5, 5, 0, 0), (5, 1 << 40, 5, 0, 0), (1 << 30, 5, 1 << 30, 0, 0), (5, 1 << 30, 1 << 30, 2, 1)):
         assert size(*bad) == 0
     for t in (0, 1, 2):
         assert 0 < size(64, 6, 128, t, 0) <= size(64, 6, 128, t, 1) < 1 << 22
@@ -307,6 +307,26 @@ def test_same_bits_again_other_streams_and_a_graph(gpu_ctx, dtype):
         torch.cuda.synchronize()
         for loss, _, dx, dW in outs:
             assert torch.equal(loss, first[0]) and torch.equal(dx, first[1]) and torch.equal(dW, first[2])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_workspaces_on_any_16_byte_boundary(gpu_ctx, dtype):
+    for shape in ((200, 700, 136), (64, 6, 128), (300, 40, 2000)):
+        x, W, target, weight = inputs(*shape, dtype, seed=10)
+        want = both(gpu_ctx, x, W, target, weight)
+        rows, vocab, k = shape
+        size = gpu_ctx.linear_cross_entropy_workspace_bytes(rows, vocab, k, W.dtype)
+        for off in (16, 48, 240):
+            around = torch.full((size + 512,), 7, dtype=torch.uint8, device="cuda")
+            ws = around[off:off + size]
+            loss, stats, dx, dW = torch.empty(rows, device="cuda"), torch.empty((rows, 2), device="cuda"), torch.empty_like(x), torch.empty_like(W)
+            torch.cuda.synchronize()
+            gpu_ctx.linear_cross_entropy(x, W, target, loss, ws, row_weight=weight, stats=stats)
+            gpu_ctx.linear_cross_entropy_grad(x, W, target, stats, ws, dx=dx, dW=dW, row_weight=weight)
+            gpu_ctx.synchronize()
+            assert torch.equal(loss, want[0]) and torch.equal(dx, want[1]) and torch.equal(dW, want[2])
+            assert bool((around[:off] == 7).all()) and bool((around[off + size:] == 7).all())
 
 
 @gpu

@@ -60,10 +60,11 @@ def run(ctx, dy, q, scale, bias=True, stream=None):
 # ---------------------------------------------------------------- without a GPU
 def test_workspace_sizes_without_a_gpu():
     size = capi.load_library().s2v_linear_i8_grad_workspace_bytes
-    for bad in ((0, 5, 5, 0), (5, 0, 5, 0), (-1, 5, 5, 0), (5, 5, 5, 3), (5, 5, 5, -1)):
+    for bad in ((0, 5, 5, 0), (5, 0, 5, 0), (-1, 5, 5, 0), (5, 5, 5, 3), (5, 5, 5, -1), (5, 5, 0, 0), (1 << 30, 1 << 30, 5, 0), (1 << 30, 5, 1 << 30, 2), (1 << 31, 5, 5, 1)):
         assert size(*bad) == 0
     for t in (0, 1, 2):
         assert size(100, 40, 60, t) < 1 << 24
+        assert size(1 << 24, 256, 128, t) < 1 << 29     # does not grow with the rows for good
 
 
 def test_binding_refuses_what_the_library_cannot_see():
@@ -151,6 +152,42 @@ def test_same_bits_again_and_empty_sums(gpu_ctx):
             assert torch.equal(dW, first[0]) and torch.equal(dbias, first[1])
         dW, dbias = run(gpu_ctx, dy[:0], q[:0], scale[:0])
         assert not dW.any() and not dbias.any()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_workspaces_on_any_16_byte_boundary(gpu_ctx, dtype):
+    for m, n, k in ((300, 200, 136), (6000, 256, 128), (5000, 64, 48), (3000, 129, 130)):
+        dy, q, scale = inputs(m, n, k, dtype, seed=6)
+        want = run(gpu_ctx, dy, q, scale)
+        size = gpu_ctx.linear_i8_grad_workspace_bytes(m, n, k, dy.dtype)
+        for off in (16, 48, 240):
+            around = torch.full((size + 512,), 7, dtype=torch.uint8, device="cuda")
+            dW, dbias = torch.empty_like(want[0]), torch.empty_like(want[1])
+            torch.cuda.synchronize()
+            gpu_ctx.linear_i8_grad(dy, q, scale, dW, around[off:off + size], dbias=dbias)
+            gpu_ctx.synchronize()
+            assert torch.equal(dW, want[0]) and torch.equal(dbias, want[1])
+            assert bool((around[:off] == 7).all()) and bool((around[off + size:] == 7).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_pieces_of_the_rows(gpu_ctx, dtype):
+    # rows enough for several pieces of the 16-bit copies, the last one small; an odd number of columns keeps the direct form out of it
+    m, n, k = (70001, 1001, 31) if dtype == "f32" else (140001, 901, 63)
+    dy, q, scale = inputs(m, n, k, dtype, seed=7)
+    dW, dbias = run(gpu_ctx, dy, q, scale)
+    d, x = dy.double(), q.double() * scale.double()[:, None]
+    want, size = d.t() @ x, d.abs().t() @ x.abs()
+    f = torch.finfo(dy.dtype)
+    # (sums of 64 rows and eight panels in the matrix units, cut, then rounded additions, one for 512 terms)
+    tol = ((f.eps / 2 if dtype != "f32" else 2 * U) + 2 * U * (64 * 3 * 32 / 16 + 3 * m / 512 + 8)) * size + f.eps / 2 * want.abs() * 1.01 + f.smallest_normal
+    if dtype == "f16":
+        tol = tol + 2.0 ** -24 * (d.abs() * scale.double()[:, None]).amax(0)[:, None] * q.double().abs().sum(0)
+    inside = want.abs() + tol < f.max
+    assert bool(((dW.double() - want).abs() <= tol)[inside].all())
+    assert bool(((dbias.double() - d.sum(0)).abs() <= U * (m / 500 + 700) * d.abs().sum(0)).all())
 
 
 @gpu
