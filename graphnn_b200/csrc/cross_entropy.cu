@@ -4,6 +4,8 @@
 // logit; joined, they give log sum_j exp(z_ij - z_it) = log1p(sum of the others relative to the own class), which keeps its digits where the own class has
 // nearly all of the probability.  The gradient computes the logits again, a piece of the vocabulary at a time, leaves the piece's G in memory in 16 bits
 // (what the tensor cores multiply; three parts of it where x and W are fp32) and multiplies it.  G in 16 bits is off by half a step of them, as x and W are.
+//
+// Where the logits are few and their sums long, tiles of logits would leave most of the GPU idle: then k is shared out, and the logits, a few MB of fp32, go through memory.
 #include <algorithm>
 
 #include "cross_entropy_few.cuh"
@@ -41,6 +43,16 @@ struct xe_rows {
         return t < 0 || t >= vocab || (weight && weight[i] == 0.0f) ? -1 : t;
     }
 };
+
+// A row's loss and what is kept of it, from the largest logit m and l = sum exp(z - m) of the other classes and the own one's logit:
+// log(1 + l exp(m - z_t)), from whichever side is the larger; alone in the vocabulary a class loses nothing.
+__device__ __forceinline__ void xe_finish(const xe_rows& rows, int64_t i, float m, float l, float mine, float* loss, float2* stats)
+{
+    const double d = (double)m - (double)mine;
+    const double one = m == -INFINITY && l == 0.0f ? (double)(mine - mine) : d > 0 ? d + log((double)l + exp(-d)) : log1p((double)l * exp(d));
+    loss[i] = (float)(one * (rows.weight ? (double)rows.weight[i] : 1.0));
+    if (stats) stats[i] = make_float2((float)(one + (double)mine), (float)expm1(-one));
+}
 
 // The partial sums of a piece, THREADS threads a row, onto what the pieces before gave (`run`, [rows]; first: nothing yet); after the last piece the loss.
 template <int THREADS>
@@ -81,11 +93,7 @@ __global__ void __launch_bounds__(256) xe_join_kernel(int64_t rows_n, int lines,
         if (stats) stats[i] = make_float2(0.0f, 0.0f);
         return;
     }
-    // log(1 + l exp(m - z_t)), from whichever side is the larger; alone in the vocabulary a class loses nothing
-    const double d = (double)s.m - (double)mine[i];
-    const double one = s.m == -INFINITY && s.l == 0.0f ? (double)(mine[i] - mine[i]) : d > 0 ? d + log((double)s.l + exp(-d)) : log1p((double)s.l * exp(d));
-    loss[i] = (float)(one * (rows.weight ? (double)rows.weight[i] : 1.0));
-    if (stats) stats[i] = make_float2((float)(one + (double)mine[i]), (float)expm1(-one));
+    xe_finish(rows, i, s.m, s.l, mine[i], loss, stats);
 }
 int xe_join(s2v_ctx* ctx, cudaStream_t st, int64_t rows_n, int lines, xe_rows rows, const float2* part, const float* mine, float2* run, bool first, bool last, float* loss, float* stats)
 {
@@ -137,15 +145,86 @@ template <typename H> __global__ void __launch_bounds__(256) xe_row_scale_kernel
     scale[i] = s, fix[i] = f;
 }
 
+// Few logits, long sums: at most half of 148 tiles, and 32 panels or more of each (86 x 38 x 3206 fp32, a step: 270 us with whole tiles).
+bool xe_keeps(int64_t rows, int64_t vocab, int64_t k, int parts)
+{
+    return ((rows + 127) / 128) * ((vocab + 127) / 128) <= 74 && (k + 63) / 64 * (parts == 3 ? 6 : 1) >= 32;
+}
+// The loss from a row of logits, a row a CTA
+__global__ void __launch_bounds__(256) xe_kept_loss_kernel(xe_rows rows, const float* __restrict__ z, int64_t ldz, float* __restrict__ loss, float2* __restrict__ stats)
+{
+    __shared__ float of[2][8];
+    const int64_t i = blockIdx.x, own = rows.own(i);
+    if (own < 0) {
+        if (threadIdx.x == 0) {
+            loss[i] = 0.0f;
+            if (stats) stats[i] = make_float2(0.0f, 0.0f);
+        }
+        return;
+    }
+    const float* const row = z + i * ldz;
+    float top = -INFINITY;   // of the other classes
+    for (int64_t j = threadIdx.x; j < rows.vocab; j += 256)
+        if (j != own) top = fmaxf(top, row[j]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((threadIdx.x & 31) == 0) of[0][threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) top = fmaxf(top, of[0][w]);
+    const float from = fabsf(top) == INFINITY ? 0.0f : top;
+    float l = 0.0f;
+    for (int64_t j = threadIdx.x; j < rows.vocab; j += 256)
+        if (j != own) l += top == INFINITY ? NAN : expf(row[j] - from);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if ((threadIdx.x & 31) == 0) of[1][threadIdx.x >> 5] = l;
+    __syncthreads();
+    if (threadIdx.x) return;
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) l += of[1][w];
+    xe_finish(rows, i, top, l, row[own], loss, stats);
+}
+// A piece's G from kept logits, in 16-bit parts, eight classes a thread
+template <typename H> __global__ void __launch_bounds__(256) xe_kept_grad_kernel(int64_t rows_n, int64_t cols, int64_t first, xe_rows rows, const float* __restrict__ z, int64_t ldz,
+                                                                                 const float2* __restrict__ stats, const float* __restrict__ row_scale, uint16_t* __restrict__ g, int64_t ldg,
+                                                                                 int64_t part, int parts)
+{
+    const int64_t per_row = (cols + 7) / 8, all = rows_n * per_row;
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < all; at += (int64_t)gridDim.x * 256) {
+        const int64_t i = at / per_row, c = (at - i * per_row) * 8, own = rows.own(i) - first;
+        const float w = row_scale[i];
+        const float2 st = stats[i];
+        const float* const row = z + i * ldz + first + c;
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = w == 0.0f || c + e >= cols ? 0.0f : w * (c + e == own ? st.y : expf(row[e] - st.x));
+        for (int p = 0; p < parts; ++p) {
+            uint32_t h[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                h[j] = pack_16bit<H>(y[2 * j], y[2 * j + 1]);
+                if constexpr (std::is_same<H, __nv_bfloat16>::value) y[2 * j] -= __uint_as_float(h[j] << 16), y[2 * j + 1] -= __uint_as_float(h[j] & 0xffff0000u);
+            }
+            *reinterpret_cast<uint4*>(g + p * part + i * ldg + c) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+    }
+}
+
 // Where things lie in the workspace, and how many classes a piece has.  `copied`: whether W has to be copied (fp32, or rows that don't lie on 16-byte boundaries).
 struct xe_space {
-    size_t mine = 0, run = 0, part = 0, x16 = 0, w16 = 0, factor = 0, scale = 0, g = 0, sum = 0, lines = 0, bytes = 0;
-    int64_t piece = 0, ld16 = 0, ldg = 0, parts = 0;
+    size_t mine = 0, run = 0, part = 0, x16 = 0, w16 = 0, factor = 0, scale = 0, g = 0, sum = 0, lines = 0, z = 0, bytes = 0;
+    bool keeps;
+    int64_t ldz = 0, piece = 0, ld16 = 0, ldg = 0, parts = 0;
     xe_space(int64_t rows, int64_t vocab, int64_t k, int type, bool grad, bool copied)
     {
         const auto take = [&](size_t& at, size_t n) { at = bytes, bytes += (n + 255) / 256 * 256; };
         parts = type == S2V_F32 ? 3 : 1;
-        ld16 = (k + 7) / 8 * 8;
+        ld16 = (k + 7) / 8 * 8, ldz = mm16_pitch(vocab);
+        keeps = xe_keeps(rows, vocab, k, (int)parts);
+        const int products = parts == 3 ? 6 : 1;
+        if (keeps) take(z, (size_t)rows * ldz * sizeof(float));
         const auto of = [&](size_t all, size_t each) { return std::max((int64_t)(all / each) / XE_TILE * XE_TILE, XE_TILE); };
         piece = vocab;
         if (copied) piece = std::min(piece, of(XE_W_BYTES, (size_t)ld16 * 2 * parts));
@@ -156,10 +235,10 @@ struct xe_space {
             take(scale, 2 * (size_t)rows * sizeof(float));
             take(g, (size_t)rows * ldg * 2 * parts);
             take(sum, (size_t)rows * mm16_pitch(k) * sizeof(float));
-            const int products = parts == 3 ? 6 : 1;
-            take(lines, std::max(mm16_lines_bytes(piece, products), mm16_lines_bytes(rows, products)));
+            take(lines, std::max({mm16_lines_bytes(piece, products), mm16_lines_bytes(rows, products), keeps ? mm16_lines_bytes(k, products) : 0}));
         } else {
             piece = std::min(piece, of(XE_PART_BYTES, (size_t)rows * sizeof(float2)) * 64);   // (a line for every 64 classes at most)
+            if (keeps) take(lines, mm16_lines_bytes(k, products));
             take(mine, (size_t)rows * sizeof(float));
             take(run, (size_t)rows * sizeof(float2));
             take(part, (size_t)rows * mm16_sum_lines_most(piece) * sizeof(float2));
@@ -196,17 +275,25 @@ struct xe_call {
     const unsigned char* W;
     int64_t ldw;
     int type;
+    unsigned char* ws;
     unsigned char* w16;
     static bool lies(int type, const void* p, int64_t rows, int64_t ld) { return type != S2V_F32 && s2v_aligned16(p) && (rows <= 1 || ld % 8 == 0); }
     xe_call(s2v_ctx* ctx_, cudaStream_t st_, int64_t n, int64_t vocab, int64_t k, int type_, const void* x, int64_t ldx, const void* W_, int64_t ldw_, const int32_t* target, const float* weight,
-            unsigned char* ws, bool grad)
+            unsigned char* ws_, bool grad)
         : ctx(ctx_), st(st_), copy_x(grad || !lies(type_, x, n, ldx)), copy_w(!lies(type_, W_, vocab, ldw_)), space(n, vocab, k, type_, grad, copy_w), rows{target, weight, vocab},
-          W(static_cast<const unsigned char*>(W_)), ldw(ldw_), type(type_), w16(ws + space.w16)
+          W(static_cast<const unsigned char*>(W_)), ldw(ldw_), type(type_), ws(ws_), w16(ws + space.w16)
     {
         args.type = type == S2V_F16 ? S2V_F16 : S2V_BF16;
         args.m = n, args.k = k;
         args.a.p = copy_x ? ws + space.x16 : x, args.a.rows = n, args.a.cols = k, args.a.ld = copy_x ? space.ld16 : ldx, args.a.part = n * space.ld16, args.a.parts = (int)space.parts;
         args.target = target, args.weight = weight, args.vocab = vocab;
+    }
+    // a piece's logits to memory
+    int logits(mm16_args a, int64_t first) const
+    {
+        a.lines = reinterpret_cast<float*>(ws + space.lines);
+        a.out = reinterpret_cast<float*>(ws + space.z) + first, a.out_type = S2V_F32, a.ldo = space.ldz;
+        return mm16_launch(ctx, st, MM16_OUT_ALONG, a);
     }
     int piece_of_w(mm16_operand& b, int64_t first, int64_t cols) const
     {
@@ -256,9 +343,17 @@ int s2v_linear_cross_entropy(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int6
         const int64_t cols = std::min(space.piece, vocab - first);
         done = c.piece_of_w(a.b, first, cols);
         a.n = cols, a.first = first;
+        if (space.keeps) {
+            if (done == S2V_OK) done = c.logits(a, first);
+            continue;
+        }
         if (done == S2V_OK) done = mm16_launch(ctx, st, MM16_SUMS, a);
         if (done == S2V_OK)
             done = xe_join(ctx, st, rows, mm16_sum_lines(ctx, rows, cols), c.rows, a.part, a.mine, reinterpret_cast<float2*>(ws + space.run), first == 0, first + cols == vocab, loss, stats);
+    }
+    if (done == S2V_OK && space.keeps) {
+        xe_kept_loss_kernel<<<(unsigned)rows, 256, 0, st>>>(c.rows, reinterpret_cast<const float*>(ws + space.z), space.ldz, loss, reinterpret_cast<float2*>(stats));
+        S2V_CHECK_LAUNCH(ctx, "xe_kept_loss_kernel");
     }
     return done;
 }
@@ -309,7 +404,14 @@ int s2v_linear_cross_entropy_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows,
         const int64_t cols = std::min(space.piece, vocab - first);
         done = c.piece_of_w(z.b, first, cols);
         z.n = cols, z.first = first;
-        if (done == S2V_OK) done = mm16_launch(ctx, st, MM16_SOFTMAX_GRAD, z);
+        if (done == S2V_OK) done = space.keeps ? c.logits(z, first) : mm16_launch(ctx, st, MM16_SOFTMAX_GRAD, z);
+        if (done == S2V_OK && space.keeps) {
+            const int64_t blocks = (rows * ((cols + 7) / 8) + 255) / 256;
+            const auto kernel = type == S2V_F16 ? xe_kept_grad_kernel<__half> : xe_kept_grad_kernel<__nv_bfloat16>;
+            kernel<<<(unsigned)blocks, 256, 0, st>>>(rows, cols, first, c.rows, reinterpret_cast<const float*>(ws + space.z), space.ldz, kept, scale, static_cast<uint16_t*>(z.g), space.ldg,
+                                                     z.g_part, z.g_parts);
+            S2V_CHECK_LAUNCH(ctx, "xe_kept_grad_kernel");
+        }
         mm16_args p;
         p.type = z.type;
         p.a.p = z.g, p.a.rows = rows, p.a.cols = cols, p.a.ld = space.ldg, p.a.part = z.g_part, p.a.parts = (int)space.parts;

@@ -125,6 +125,48 @@ template <typename H> __global__ void __launch_bounds__(256) grad_q_kernel(int64
     }
 }
 
+// Few rows: fp32 arithmetic and one launch.  64 rows of dW by 256 columns a CTA, 8 x 8 a thread with its columns 32 apart, so that reads of q and writes of dW are a
+// warp's neighbours wherever rows lie.
+constexpr int LG_FEW = 32;   // rows
+// ... and up to so many multiply-adds: a call of 4 x 177 x 137 fp32 takes 19 us, 25 by the other forms' four launches or five; of 32 x 4096 x 4096 bf16 (2^29) 60 and 32
+constexpr int64_t LG_FEW_PRODUCTS = (int64_t)1 << 26;
+template <typename T>
+__global__ void __launch_bounds__(256) grad_few_kernel(int m, int64_t n, int64_t k, const T* __restrict__ dy, int64_t lddy, const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale,
+                                                       T* __restrict__ dW, int64_t lddw, float* __restrict__ dbias)
+{
+    __shared__ __align__(16) float of[LG_FEW][64];   // dy times the rows' scales
+    const int64_t row0 = (int64_t)blockIdx.y * 64, col0 = (int64_t)blockIdx.x * 256 + (threadIdx.x & 31);
+    for (int i = threadIdx.x; i < m * 64; i += 256) {
+        const int64_t j = row0 + (i & 63);
+        of[i >> 6][i & 63] = j < n ? to_f32(dy[(i >> 6) * lddy + j]) * scale[i >> 6] : 0.0f;
+    }
+    if (dbias && blockIdx.x == 0 && threadIdx.x < 64 && row0 + threadIdx.x < n) {
+        float t = 0.0f;
+        for (int i = 0; i < m; ++i) t += to_f32(dy[i * lddy + row0 + threadIdx.x]);
+        dbias[row0 + threadIdx.x] = t;
+    }
+    __syncthreads();
+    const int r0 = (threadIdx.x >> 5) * 8;
+    float acc[8][8] = {};
+#pragma unroll 2
+    for (int i = 0; i < m; ++i) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = col0 + 32 * e < k ? (float)q[i * ldq + col0 + 32 * e] : 0.0f;
+        const float4 a = *reinterpret_cast<const float4*>(&of[i][r0]), b = *reinterpret_cast<const float4*>(&of[i][r0 + 4]);
+        const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[r][e] = fmaf(y[r], x[e], acc[r][e]);
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (row0 + r0 + r < n && col0 + 32 * e < k) dW[(row0 + r0 + r) * lddw + col0 + 32 * e] = from_f32<T>(acc[r][e]);
+}
+
 // Where things lie in the workspace.  Matrices in 16 bits are made for a piece of the rows at a time, dW's sums of several pieces kept in fp32.
 constexpr size_t LG_BYTES = (size_t)256 << 20;   // of a piece, about
 struct LgSpace {
@@ -181,6 +223,14 @@ int s2v_linear_i8_grad(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, in
         if (dbias) S2V_CUDA_OK(ctx, cudaMemsetAsync(dbias, 0, (size_t)n * sizeof(float), st));
         return S2V_OK;
     }
+    if (m <= LG_FEW && n <= LG_FEW_PRODUCTS / m / k && (n + 63) / 64 <= 65535)
+        return s2v_by_dtype(dy_type, [&](auto type) {
+            using T = decltype(type);
+            grad_few_kernel<T><<<dim3((unsigned)((k + 255) / 256), (unsigned)((n + 63) / 64)), 256, 0, st>>>((int)m, n, k, static_cast<const T*>(dy), lddy, q, ldq, q_scale, static_cast<T*>(dW),
+                                                                                                            lddw, dbias);
+            S2V_CHECK_LAUNCH(ctx, "grad_few_kernel");
+            return (int)S2V_OK;
+        });
     unsigned char* const ws = mm16_space(workspace);
     const bool direct = linear_i8_direct_takes(m, n, k, dy_type) && linear_i8_direct_lies(m, dy_type, dy, lddy, q, ldq);
     const LgSpace space(m, n, k, dy_type, direct);

@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) mm16_kernel(const __grid_consta
 {
     using Cfg = MmCfg<BN, PAIR>;
     constexpr int STAGES = Cfg::STAGES, ACCS = Cfg::ACCS, CTAS = PAIR ? 2 : 1;
-    constexpr bool A_ACROSS = KIND == MM16_OUT_ACROSS, B_ACROSS = KIND == MM16_OUT || KIND == MM16_OUT_ACROSS;
+    constexpr bool A_ACROSS = KIND == MM16_OUT_ACROSS, B_ACROSS = KIND == MM16_OUT || KIND == MM16_OUT_ACROSS, OUT = KIND >= MM16_OUT;
     extern __shared__ unsigned char mm_raw[];
     unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(mm_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t smem0 = smem_u32(smem);
@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) mm16_kernel(const __grid_consta
             if constexpr (KIND == MM16_SUMS)
                 if (row < a.m) a.part[(int64_t)(2 * tn + half) * a.m + row] = make_float2(sums.m, sums.l);
         }
-        if (B_ACROSS && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        if (OUT && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         __syncwarp();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -633,7 +633,7 @@ int64_t mm_steps(const mm16_args& a) { return (a.k + MM_K - 1) / MM_K * mm_produ
 template <int KIND, int BN, bool PAIR> int mm_launch(s2v_ctx* ctx, cudaStream_t st, const mm16_args& g)
 {
     using Cfg = MmCfg<BN, PAIR>;
-    constexpr bool A_ACROSS = KIND == MM16_OUT_ACROSS, B_ACROSS = KIND == MM16_OUT || KIND == MM16_OUT_ACROSS;
+    constexpr bool A_ACROSS = KIND == MM16_OUT_ACROSS, B_ACROSS = KIND == MM16_OUT || KIND == MM16_OUT_ACROSS, OUT = KIND >= MM16_OUT;
     const auto boxes = [](int64_t rows) { return rows <= 64 ? 1 : rows <= 128 ? 2 : 4; };
     // (a box with many rows outside the matrix takes longer than a full one)
     const int box_a = A_ACROSS ? 64 : (int)(g.m < 128 ? g.m : 128), box_b = B_ACROSS ? 64 : (int)(g.n < Cfg::B_ROWS ? g.n : Cfg::B_ROWS);
@@ -653,11 +653,11 @@ template <int KIND, int BN, bool PAIR> int mm_launch(s2v_ctx* ctx, cudaStream_t 
     a.steps = (int)kblocks * a.products;
     const int64_t units = std::min(ctx->sm_count, 148) / (PAIR ? 2 : 1);
     MmShares shares(units, mt * nt, a.steps);
-    if (!B_ACROSS) shares.full = mt * nt, shares.rest = 0, shares.splits = 1;
+    if (!OUT) shares.full = mt * nt, shares.rest = 0, shares.splits = 1;
     a.full = (int)shares.full, a.rest = (int)shares.rest;
     a.per_split = (int)((a.steps + shares.splits - 1) / shares.splits);
     a.splits = (a.steps + a.per_split - 1) / a.per_split;
-    a.chunk = KIND == MM16_SUMS || a.products > 1 || (B_ACROSS && g.out_type == S2V_F32) ? MM_CHUNK : MM_CHUNK_16;
+    a.chunk = KIND == MM16_SUMS || a.products > 1 || (OUT && g.out_type == S2V_F32) ? MM_CHUNK : MM_CHUNK_16;
     a.last_mmas = (int)((g.k - MM_K * (kblocks - 1) + 15) / 16);
     a.a_boxes = A_ACROSS ? boxes(PAIR || g.m > 128 ? 128 : g.m) : 0, a.b_boxes = B_ACROSS ? boxes(PAIR || g.n > 128 ? 128 : g.n) : 0;
     a.bytes = (A_ACROSS ? (uint32_t)a.a_boxes * MM_BLOCK : (uint32_t)box_a * 128) + (B_ACROSS ? (uint32_t)a.b_boxes * MM_BLOCK : (uint32_t)box_b * 128);
@@ -723,12 +723,13 @@ size_t mm16_lines_bytes(int64_t k, int products)
 int mm16_launch(s2v_ctx* ctx, cudaStream_t st, mm16_kind kind, const mm16_args& a)
 {
     if (a.m == 0 || a.n == 0) return S2V_OK;
-    const bool pairs = mm_pairs(ctx, a.m, a.n, kind == MM16_OUT || kind == MM16_OUT_ACROSS ? mm_steps(a) : 0);
+    const bool pairs = mm_pairs(ctx, a.m, a.n, kind >= MM16_OUT ? mm_steps(a) : 0);
     switch (kind) {
         case MM16_SUMS: return pairs ? mm_launch<MM16_SUMS, 256, true>(ctx, st, a) : mm_launch<MM16_SUMS, 128, false>(ctx, st, a);
         case MM16_SOFTMAX_GRAD: return pairs ? mm_launch<MM16_SOFTMAX_GRAD, 256, true>(ctx, st, a) : mm_launch<MM16_SOFTMAX_GRAD, 128, false>(ctx, st, a);
         case MM16_OUT: return pairs ? mm_launch<MM16_OUT, 256, true>(ctx, st, a) : mm_launch<MM16_OUT, 128, false>(ctx, st, a);
-        default: return pairs ? mm_launch<MM16_OUT_ACROSS, 256, true>(ctx, st, a) : mm_launch<MM16_OUT_ACROSS, 128, false>(ctx, st, a);
+        case MM16_OUT_ACROSS: return pairs ? mm_launch<MM16_OUT_ACROSS, 256, true>(ctx, st, a) : mm_launch<MM16_OUT_ACROSS, 128, false>(ctx, st, a);
+        default: return pairs ? mm_launch<MM16_OUT_ALONG, 256, true>(ctx, st, a) : mm_launch<MM16_OUT_ALONG, 128, false>(ctx, st, a);
     }
 }
 

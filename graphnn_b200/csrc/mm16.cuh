@@ -31,7 +31,7 @@ struct mm16_args {
     void* g = nullptr;
     int64_t ldg = 0, g_part = 0;        // rows of a multiple of 64 numbers
     int g_parts = 1;
-    // MM16_OUT: out = alpha * product (+ what `sum` holds); alpha: one number, or one for each row, or NULL
+    // MM16_OUT and the others: out = alpha * product (+ what `sum` holds); alpha: one number, or one for each row, or NULL
     const float* alpha = nullptr;
     int alpha_rows = 0;
     float* sum = nullptr;               // [m x mm16_pitch(n)] fp32; outputs of the products before this one, and of this one where `out` is NULL
@@ -44,7 +44,7 @@ struct mm16_args {
     void* out = nullptr;
     int64_t ldo = 0;
 };
-enum mm16_kind { MM16_SUMS, MM16_SOFTMAX_GRAD, MM16_OUT, MM16_OUT_ACROSS };   // ... with B across; with A and B across
+enum mm16_kind { MM16_SUMS, MM16_SOFTMAX_GRAD, MM16_OUT, MM16_OUT_ACROSS, MM16_OUT_ALONG };   // outputs with B across; with A and B across; with both along k
 
 // Places in a workspace are 256 bytes apart, from its first such boundary on (outputs leave 32 bytes at a time; callers promise 16): what to add to its size.
 constexpr size_t MM16_SLACK = 240;

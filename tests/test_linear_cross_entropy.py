@@ -142,7 +142,9 @@ def test_binding_refuses_what_the_library_cannot_see(recorded):
 SHAPES = [(1, 1, 1), (1, 2, 3), (3, 1, 16), (2, 7, 5), (64, 6, 128), (5, 40, 33), (130, 129, 65), (64, 64, 64), (257, 300, 31), (100, 1000, 256), (1, 5000, 128), (7, 20000, 72), (700, 513, 200), (300, 4097, 130),
           (129, 255, 1021), (33, 900, 2048), (2100, 70, 40), (600, 2500, 512),
           # the limits of the form for a few classes, and one past each
-          (512, 64, 512), (513, 64, 512), (512, 65, 512), (512, 64, 513), (65, 33, 100)]
+          (512, 64, 512), (513, 64, 512), (512, 65, 512), (512, 64, 513), (65, 33, 100),
+          # few logits with long sums, whose logits are kept: one tile, several, odd places
+          (1, 2, 4000), (86, 38, 3206), (3, 9000, 2100), (600, 600, 2048), (1000, 1025, 2500), (130, 70, 5001)]
 
 
 @gpu

@@ -85,6 +85,8 @@ def test_binding_refuses_what_the_library_cannot_see():
 
 # ---------------------------------------------------------------- values
 SHAPES = [(1, 1, 1), (2, 3, 5), (64, 6, 128), (1, 300, 500), (100, 128, 128), (65, 129, 257), (1000, 40, 24), (333, 256, 1021), (2000, 300, 130), (5000, 17, 72), (129, 1500, 700), (4099, 256, 128),
+          # few rows
+          (32, 300, 700), (33, 300, 700), (4, 65, 257), (17, 1000, 31),
           # few outputs over many rows: every shape of the tiles that one kernel takes
           (4096, 1, 1), (5000, 64, 64), (6001, 130, 65), (20000, 256, 128), (20011, 100, 200), (4500, 128, 256), (9000, 300, 100), (4097, 20, 700), (30000, 6, 40), (7000, 512, 256)]
 
