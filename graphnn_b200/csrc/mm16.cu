@@ -199,29 +199,41 @@ template <typename T> __device__ __forceinline__ void mm_write(const MmArgs& a, 
             __syncwarp();
             if (lane == 0) tma_store_2d(map, (int)(col + c), (int)row0, smem_u32(box));
         } else {
-            // a word of four bytes a lane; in a row of 16-bit numbers at an odd place a lane writes the second half of its word with the first half of its
-            // neighbour's, the first lane the first number and the last lane the last one
+            // A word of four bytes a lane, two rows at a time; in a row of 16-bit numbers at an odd place a lane writes the second half of its word with the first half of
+            // its neighbour's, the first lane the first number and the last lane the last one.  Two rows on, a row lies as this one does, so that all of this is found once.
+            // (Found for each row: 50021 x 1021 of fp16 over 1531 rows 252 us, as many outputs of 16 bytes 124.)
             __syncwarp();
             const int l = lane & 15, hi = lane >> 4;
-            const int cols = (int)min((int64_t)COLS, a.n - col - c), rows = (int)min((int64_t)32, a.m - row0);
-#pragma unroll 4
-            for (int r = hi; r < 32; r += 2) {
-                T* const at = static_cast<T*>(a.out) + (row0 + r) * a.ldo + col + c;
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(box + r * MM_PIECE + 16 * ((l >> 2) ^ (r >> 1 & 3)) + 4 * (l & 3));
-                if constexpr (sizeof(T) == 4) {
-                    if (r < rows && l < cols) *reinterpret_cast<uint32_t*>(at + l) = w;
-                } else {
-                    uint16_t* const h = reinterpret_cast<uint16_t*>(at) + 2 * l;
-                    const uint32_t next = __shfl_down_sync(0xffffffffu, w, 1);
-                    if (r < rows) {
-                        if ((reinterpret_cast<uintptr_t>(h) & 2) == 0) {
-                            if (2 * l + 1 < cols) *reinterpret_cast<uint32_t*>(h) = w;
-                            else if (2 * l < cols) h[0] = (uint16_t)w;
-                        } else {
-                            if (l < 15 && 2 * l + 2 < cols) *reinterpret_cast<uint32_t*>(h + 1) = __byte_perm(w, next, 0x5432);
-                            else if (2 * l + 1 < cols) h[1] = (uint16_t)(w >> 16);
-                            if (l == 0) h[0] = (uint16_t)w;
-                        }
+            const int cols = (int)min((int64_t)COLS, a.n - col - c), rows = (int)min((int64_t)32, a.m - row0) - hi;
+            T* const p = static_cast<T*>(a.out) + (row0 + hi) * a.ldo + col + c;
+            const int64_t step = 2 * a.ldo;
+            uint32_t at[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) at[i] = smem_u32(box) + (uint32_t)(hi * MM_PIECE + 16 * ((l >> 2) ^ i) + 4 * (l & 3));
+            const auto word = [&](int i) {
+                uint32_t w;
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at[i & 3] + (uint32_t)(i * 2 * MM_PIECE)) : "memory");
+                return w;
+            };
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t w = word(i);
+                    if (2 * i < rows && l < cols) *reinterpret_cast<uint32_t*>(p + l + i * step) = w;
+                }
+            } else {
+                uint16_t* const h = reinterpret_cast<uint16_t*>(p) + 2 * l;
+                const bool odd = reinterpret_cast<uintptr_t>(h) & 2;
+                const bool both = odd ? l < 15 && 2 * l + 2 < cols : 2 * l + 1 < cols, low = odd ? l == 0 : 2 * l < cols && !both, high = odd && !both && 2 * l + 1 < cols;
+                const uint32_t pick = odd ? 0x5432u : 0x3210u;
+                uint16_t* const h2 = h + (odd ? 1 : 0);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t w = word(i), next = __shfl_down_sync(0xffffffffu, w, 1);
+                    if (2 * i < rows) {
+                        if (both) *reinterpret_cast<uint32_t*>(h2 + i * step) = __byte_perm(w, next, pick);
+                        if (low) h[i * step] = (uint16_t)w;
+                        if (high) h[1 + i * step] = (uint16_t)(w >> 16);
                     }
                 }
             }
