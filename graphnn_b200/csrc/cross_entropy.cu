@@ -107,9 +107,10 @@ int xe_join(s2v_ctx* ctx, cudaStream_t st, int64_t rows_n, int lines, xe_rows ro
     return rows_n >= 2048 || lines <= 32 ? go(xe_join_kernel<8>, 8) : rows_n > 64 ? go(xe_join_kernel<64>, 64) : go(xe_join_kernel<256>, 256);
 }
 
-// G in 16 bits of fp16 is scaled by a power of two that puts the largest row weight's binade at 2^14: its steps are then 2^-38 of that and less.
-// factor[0], and factor[1] = 1 / factor[0].
-__global__ void __launch_bounds__(1024) xe_factor_kernel(int64_t rows_n, xe_rows rows, float* factor)
+// G in 16 bits is held relative to the largest row weight (times `unit`, 2^14 for fp16, whose steps are then 2^-38 of that weight and less): where all rows weigh the same, which
+// is the rule, the own class's G of a row that does not know it is next to -1, and rounds to it, instead of all such rows being rounded alike by what that weight is
+// off in 16 bits (4096 x 131072 x 4096 bf16: dW 2.6e-3 off for one number of rows, 2.0e-3 for another).  factor[0], and factor[1] = 1 / factor[0].
+__global__ void __launch_bounds__(1024) xe_factor_kernel(int64_t rows_n, xe_rows rows, float unit, float* factor)
 {
     __shared__ uint32_t part[32];
     uint32_t top = 0;
@@ -124,8 +125,8 @@ __global__ void __launch_bounds__(1024) xe_factor_kernel(int64_t rows_n, xe_rows
     if (threadIdx.x >= 32) return;
     top = __reduce_max_sync(0xffffffffu, part[threadIdx.x]);
     if (threadIdx.x == 0) {
-        const int e = min(max((int)(top >> 23) - 127, -100), 127);   // (weights below 2^-100 are not scaled up further)
-        factor[0] = exp2f((float)(14 - e)), factor[1] = exp2f((float)(e - 14));
+        const float largest = fminf(fmaxf(__uint_as_float(top), 7.888609052210118e-31f), 1.2676506002282294e30f);   // (2^-100 to 2^100: weights outside are not scaled further)
+        factor[0] = unit / largest, factor[1] = largest / unit;
     }
 }
 
@@ -385,9 +386,9 @@ int s2v_linear_cross_entropy_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows,
     // x with zeros in the rows that are left out, whatever these hold: their zeros of G meet zeros in dW
     int done = mm16_pack(ctx, st, rows, k, type, x, ldx, target, row_weight, vocab, ws + space.x16, space.ld16, rows * space.ld16);
     float* factor = nullptr;
-    if (done == S2V_OK && type == S2V_F16) {
+    if (done == S2V_OK && type != S2V_F32) {
         factor = reinterpret_cast<float*>(ws + space.factor);
-        xe_factor_kernel<<<1, 1024, 0, st>>>(rows, c.rows, factor);
+        xe_factor_kernel<<<1, 1024, 0, st>>>(rows, c.rows, type == S2V_F16 ? 16384.0f : 1.0f, factor);
         S2V_CHECK_LAUNCH(ctx, "xe_factor_kernel");
     }
     float* const scale = reinterpret_cast<float*>(ws + space.scale);
