@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(THREADS < LN_CTA ? LN_CTA : THREADS) layer_nor
 }
 
 // The same through the ring, R rows a turn of a CTA: a stage holds a row's dy and, behind it, x or the 8-bit row.  With the rows' raw numbers and the weight in
-// registers a number is read from shared memory once, and R rows share a barrier.  (8192 x 8192 bf16, 83 us: the instructions, some 20 a number, half of them what a
+// registers a number is read from shared memory once, and R rows share a barrier.  (8192 x 8192 bf16, 83 us: the instructions, 27 a number, half of them what a
 // row costs a thread; 32 numbers a thread of two CTAs an SM, with dy and 8-bit rows read twice and the weight twice a row through L1 105, with g = dy w kept in
 // registers, some of them spilled, 119; before the ring was kept count of without divisions 97.)
 template <typename T, int NV, int R, int THREADS, int CTAS, bool FROM8> __global__ void __launch_bounds__(THREADS, CTAS) layer_norm_grad_ring_kernel(const LnGrad a)
