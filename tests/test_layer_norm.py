@@ -9,7 +9,9 @@ TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 U = 2.0 ** -24   # half a step of fp32
 # one row and several; widths around every form's limits, odd ones (no row but the first aligned), and rows longer than registers hold
 SHAPES = [(1, 1), (3, 2), (5, 7), (64, 128), (33, 31), (2, 256), (7, 264), (9, 129), (4, 513), (6, 1021), (5, 1024), (3, 2048), (11, 4096), (3, 4100), (2, 8192), (300, 40), (2, 8200), (3, 16384), (2, 16392), (2, 20001),
-          (1, 70000), (700, 96)]
+          (1, 70000), (700, 96),
+          # many rows of each CTA: stages and sums in turn
+          (9001, 128), (6000, 1032), (3001, 2048), (2500, 4096), (1300, 8192), (700, 16384), (1500, 1001)]
 
 
 def depth(cols):
