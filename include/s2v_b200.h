@@ -266,8 +266,8 @@ int s2v_distill_topk_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t
  *     mean_i = sum_j x_ij / cols;  rstd_i = 1 / sqrt(sum_j (x_ij - mean_i)^2 / cols + eps);  y_ij = (x_ij - mean_i) rstd_i weight_j + bias_j
  * in fp32, rounded once to x_type.  weight, bias : fp32 [cols] or NULL (1 and 0); eps 0 to 1e30; y : [rows x cols] of x_type, may be x itself (with
  * ldy = ldx).  What a training step keeps: stats : float [rows x 2], 8-byte aligned, or NULL: mean and rstd; q : int8 [rows x cols] with q_scale : [rows], or
- * both NULL: the rows of x in 8 bits, exactly as s2v_quantize_rows_i8 gives them, written in the same pass over x.  With eps = 0 a row of equal numbers gives NaN; so
- * does, whatever eps is, a row with an infinity or NaN (its 8-bit rows: q = 0, q_scale = NaN).  The sum of squares is an fp32 number: deviations of about
+ * both NULL: the rows of x in 8 bits, exactly as s2v_quantize_rows_i8 gives them, written in the same pass over x.  With eps = 0 a row of equal numbers has no
+ * defined result; a row with an infinity or NaN gives NaN (its 8-bit rows: q = 0, q_scale = NaN).  The sum of squares is an fp32 number: deviations of about
  * 1e19 and more overflow it (rstd = 0). */
 int s2v_layer_norm(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t cols, int x_type, const void* x, int64_t ldx, const float* weight,
                    const float* bias, float eps, void* y, int64_t ldy, float* stats, int8_t* q, int64_t ldq, float* q_scale);
@@ -289,7 +289,7 @@ int s2v_layer_norm_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t c
 size_t s2v_linear_i8_grad_workspace_bytes(int64_t m, int64_t n, int64_t k, int dy_type);
 int s2v_linear_i8_grad(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, int64_t k, int dy_type, const void* dy, int64_t lddy, const int8_t* q,
                        int64_t ldq, const float* q_scale, void* workspace, size_t workspace_bytes, void* dW, int64_t lddw, float* dbias);
-/* Softmax cross entropy of the logits z = x W^T against one class a row; z is never in memory as a whole:
+/* Softmax cross entropy of the logits z = x W^T against one class a row; z is not in memory as a whole (but for a few MB where it has no more):
  *     loss_i = row_weight_i (log sum_j exp z_ij - z_it),  t = target_i
  * x : [rows x k], W : [vocab x k] (a class a row), both of `type`; target : int32 [rows]; row_weight : [rows] or NULL (1).  A row whose target lies outside
  * [0, vocab), or whose row_weight is 0, is left out: loss 0 and gradient 0, whatever x holds there.  A row with NaN or +infinity among its logits has NaN as its

@@ -209,6 +209,45 @@ def test_refusals(gpu_ctx):
     assert not f.any()
 
 
+@gpu
+@pytest.mark.parametrize("reserved", [1, 75, 140, 146])
+def test_sms_left_to_others(reserved):
+    """With most SMs left to others tiles, shares and rows fall to few CTAs; results stay within the same tolerances, workspaces within their sizes."""
+    ctx = capi.Context(0)
+    try:
+        ctx.set_option(ctx.OPT_RESERVED_SMS, reserved)
+        for m, n, k, dtype in ((700, 300, 260, "bf16"), (6000, 256, 128, "f32"), (5000, 600, 130, "f16"), (4200, 40, 64, "bf16")):
+            dy, q, scale = inputs(m, n, k, dtype, seed=8)
+            (dW, dbias), size = run(ctx, dy, q, scale), ctx.linear_i8_grad_workspace_bytes(m, n, k, dy.dtype)
+            check(dy, q, scale, dW, dbias)
+            around = torch.full((size + 1024,), 7, dtype=torch.uint8, device="cuda")
+            torch.cuda.synchronize()
+            ctx.linear_i8_grad(dy, q, scale, dW, around[:size], dbias=dbias)
+            ctx.synchronize()
+            check(dy, q, scale, dW, dbias)
+            assert bool((around[size:] == 7).all())
+        from test_layer_norm import check_forward, check_grad
+        from test_linear_cross_entropy import Reference, both
+        from test_linear_cross_entropy import inputs as classes
+        for shape, dtype in (((300, 1500, 200), "bf16"), ((200, 130, 2100), "f32"), ((600, 2500, 512), "f16")):
+            x, W, target, weight = classes(*shape, dtype)
+            ref = Reference(x, W, target, weight)
+            loss, dx, dWv = both(ctx, x, W, target, weight)
+            ref.check_loss(loss)
+            ref.check_grad(dx, dWv)
+        x = torch.randn((900, 4096), device="cuda").bfloat16()
+        dy, y, dx, stats = torch.randn_like(x), torch.empty_like(x), torch.empty_like(x), torch.empty((900, 2), device="cuda")
+        dw, db, ws = torch.empty(4096, device="cuda"), torch.empty(4096, device="cuda"), torch.empty(ctx.layer_norm_grad_workspace_bytes(900, 4096), dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        ctx.layer_norm(x, y, stats=stats)
+        ctx.layer_norm_grad(dy, stats, dx, ws, x=x, dweight=dw, dbias=db)
+        ctx.synchronize()
+        check_forward(x, None, None, 1e-5, y, stats)
+        check_grad(dy, x.double(), stats, None, dx, dw, db)
+    finally:
+        ctx.close()
+
+
 # ---------------------------------------------------------------- together, as they are used
 @gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
