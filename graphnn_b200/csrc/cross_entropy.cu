@@ -9,6 +9,7 @@
 #include <algorithm>
 
 #include "cross_entropy_few.cuh"
+#include "cross_entropy_rows.cuh"
 #include "mm16.cuh"
 
 namespace
@@ -31,28 +32,6 @@ struct xe_sum {
         m = top;
     }
 };
-
-struct xe_rows {
-    const int32_t* target;
-    const float* weight;   // NULL: ones
-    int64_t vocab;
-    // the row's class, -1 if it is left out
-    __device__ __forceinline__ int64_t own(int64_t i) const
-    {
-        const int64_t t = target[i];
-        return t < 0 || t >= vocab || (weight && weight[i] == 0.0f) ? -1 : t;
-    }
-};
-
-// A row's loss and what is kept of it, from the largest logit m and l = sum exp(z - m) of the other classes and the own one's logit:
-// log(1 + l exp(m - z_t)), from whichever side is the larger; alone in the vocabulary a class loses nothing.
-__device__ __forceinline__ void xe_finish(const xe_rows& rows, int64_t i, float m, float l, float mine, float* loss, float2* stats)
-{
-    const double d = (double)m - (double)mine;
-    const double one = m == -INFINITY && l == 0.0f ? (double)(mine - mine) : d > 0 ? d + log((double)l + exp(-d)) : log1p((double)l * exp(d));
-    loss[i] = (float)(one * (rows.weight ? (double)rows.weight[i] : 1.0));
-    if (stats) stats[i] = make_float2((float)(one + (double)mine), (float)expm1(-one));
-}
 
 // The partial sums of a piece, THREADS threads a row, onto what the pieces before gave (`run`, [rows]; first: nothing yet); after the last piece the loss.
 template <int THREADS>

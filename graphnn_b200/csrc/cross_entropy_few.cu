@@ -2,6 +2,7 @@
 // A CTA has a row of x in shared memory; its warps share the classes, a logit being a sum over the lanes, and its threads the columns of dx.  What bounds it is the
 // latency of a chain of steps (a warp a row, 35 classes one after the other: 3 x 35 x 449 fp16, a step, 158 us).
 #include "cross_entropy_few.cuh"
+#include "cross_entropy_rows.cuh"
 
 namespace
 {
@@ -13,20 +14,13 @@ struct XfArgs {
     int64_t ldx, ldw, lddx, lddw;
     const void* x;
     const void* W;
-    const int32_t* target;
-    const float* weight;
+    xe_rows of;
     float* loss;
     float2* stats;
     float* g;   // [rows][vocab]
     void* dx;
     void* dW;
 };
-
-__device__ __forceinline__ int xf_own(const XfArgs& a, int i)
-{
-    const int t = a.target[i];
-    return t < 0 || t >= a.vocab || (a.weight && a.weight[i] == 0.0f) ? -1 : t;
-}
 
 // row i's logits to z[64], by the whole CTA
 template <typename T> __device__ __forceinline__ void xf_logits(const XfArgs& a, int i, float* x, float* z)
@@ -59,7 +53,7 @@ template <typename T> __device__ __forceinline__ void xf_logits(const XfArgs& a,
 template <typename T> __global__ void __launch_bounds__(XF_CTA) xe_few_loss_kernel(const XfArgs a)
 {
     __shared__ float x[XF_COLS], z[XF_CLASSES];
-    const int i = blockIdx.x, own = xf_own(a, i);
+    const int i = blockIdx.x, own = (int)a.of.own(i);
     if (own < 0) {
         if (threadIdx.x == 0) {
             a.loss[i] = 0.0f;
@@ -85,24 +79,20 @@ template <typename T> __global__ void __launch_bounds__(XF_CTA) xe_few_loss_kern
         if (j < a.vocab && j != own) l += top == INFINITY ? NAN : expf(z[j] - from);
 #pragma unroll
     for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (lane) return;
-    const double d = (double)top - (double)mine;
-    const double one = top == -INFINITY && l == 0.0f ? (double)(mine - mine) : d > 0 ? d + log((double)l + exp(-d)) : log1p((double)l * exp(d));
-    a.loss[i] = (float)(one * (a.weight ? (double)a.weight[i] : 1.0));
-    if (a.stats) a.stats[i] = make_float2((float)(one + (double)mine), (float)expm1(-one));
+    if (lane == 0) xe_finish(a.of, i, top, l, mine, a.loss, a.stats);
 }
 
 // G and dx
 template <typename T> __global__ void __launch_bounds__(XF_CTA) xe_few_grad_kernel(const XfArgs a)
 {
     __shared__ float x[XF_COLS], z[XF_CLASSES];
-    const int i = blockIdx.x, own = xf_own(a, i);
+    const int i = blockIdx.x, own = (int)a.of.own(i);
     if (own >= 0) {
         xf_logits<T>(a, i, x, z);
         if (threadIdx.x < a.vocab) {
             const float2 st = a.stats[i];
             const int j = threadIdx.x;
-            const float g = (a.weight ? a.weight[i] : 1.0f) * (j == own ? st.y : expf(z[j] - st.x));
+            const float g = (a.of.weight ? a.of.weight[i] : 1.0f) * (j == own ? st.y : expf(z[j] - st.x));
             z[j] = g, a.g[(int64_t)i * a.vocab + j] = g;
         }
         __syncthreads();
@@ -126,7 +116,7 @@ template <typename T> __global__ void __launch_bounds__(512) xe_few_weight_kerne
     float t[4] = {};
 #pragma unroll 4
     for (int i = g; i < a.rows; i += 16) {
-        const bool counts = xf_own(a, i) >= 0;   // (a row that is left out may hold anything)
+        const bool counts = a.of.own(i) >= 0;   // (a row that is left out may hold anything)
         const float x = counts && col < a.k ? to_f32(static_cast<const T*>(a.x)[i * a.ldx + col]) : 0.0f;
 #pragma unroll
         for (int c = 0; c < 4; ++c) t[c] = fmaf(a.g[(int64_t)i * a.vocab + min(j0 + c, a.vocab - 1)], x, t[c]);
@@ -149,7 +139,7 @@ size_t xe_few_bytes(int64_t rows, int64_t vocab) { return (size_t)rows * vocab *
 int xe_few_loss(s2v_ctx* ctx, cudaStream_t st, int64_t rows, int64_t vocab, int64_t k, int type, const void* x, int64_t ldx, const void* W, int64_t ldw, const int32_t* target,
                 const float* row_weight, float* loss, float* stats)
 {
-    const XfArgs a{(int)rows, (int)vocab, (int)k, ldx, ldw, 0, 0, x, W, target, row_weight, loss, reinterpret_cast<float2*>(stats), nullptr, nullptr, nullptr};
+    const XfArgs a{(int)rows, (int)vocab, (int)k, ldx, ldw, 0, 0, x, W, {target, row_weight, vocab}, loss, reinterpret_cast<float2*>(stats), nullptr, nullptr, nullptr};
     return s2v_by_dtype(type, [&](auto t) {
         xe_few_loss_kernel<decltype(t)><<<(unsigned)rows, XF_CTA, 0, st>>>(a);
         S2V_CHECK_LAUNCH(ctx, "xe_few_loss_kernel");
@@ -160,7 +150,7 @@ int xe_few_loss(s2v_ctx* ctx, cudaStream_t st, int64_t rows, int64_t vocab, int6
 int xe_few_grad(s2v_ctx* ctx, cudaStream_t st, int64_t rows, int64_t vocab, int64_t k, int type, const void* x, int64_t ldx, const void* W, int64_t ldw, const int32_t* target,
                 const float* row_weight, const float* stats, void* workspace, void* dx, int64_t lddx, void* dW, int64_t lddw)
 {
-    const XfArgs a{(int)rows, (int)vocab, (int)k, ldx, ldw, lddx, lddw, x, W, target, row_weight, nullptr, reinterpret_cast<float2*>(const_cast<float*>(stats)), static_cast<float*>(workspace), dx, dW};
+    const XfArgs a{(int)rows, (int)vocab, (int)k, ldx, ldw, lddx, lddw, x, W, {target, row_weight, vocab}, nullptr, reinterpret_cast<float2*>(const_cast<float*>(stats)), static_cast<float*>(workspace), dx, dW};
     return s2v_by_dtype(type, [&](auto t) {
         using T = decltype(t);
         xe_few_grad_kernel<T><<<(unsigned)rows, XF_CTA, 0, st>>>(a);

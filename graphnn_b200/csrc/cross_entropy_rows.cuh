@@ -1,0 +1,33 @@
+// What every form of the loss over a vocabulary makes of a row: which class is its own, and its loss.
+#pragma once
+
+#include "elem_types.cuh"
+
+namespace
+{
+
+struct xe_rows {
+    const int32_t* target;
+    const float* weight;   // NULL: ones
+    int64_t vocab;
+    // the row's class, -1 if it is left out
+    __device__ __forceinline__ int64_t own(int64_t i) const
+    {
+        const int64_t t = target[i];
+        return t < 0 || t >= vocab || (weight && weight[i] == 0.0f) ? -1 : t;
+    }
+};
+
+// A row's loss and what is kept of it, from the largest logit m and l = sum exp(z - m) of the other classes and the own one's logit:
+// log(1 + l exp(m - z_t)), from whichever side is the larger; alone in the vocabulary a class loses nothing.  An own logit of +infinity has no loss (infinity less
+// infinity), although the others are nothing beside it.
+__device__ __forceinline__ void xe_finish(const xe_rows& rows, int64_t i, float m, float l, float mine, float* loss, float2* stats)
+{
+    const double d = (double)m - (double)mine;
+    const bool alone = m == -INFINITY && l == 0.0f;
+    const double one = alone || mine == INFINITY ? (double)(mine - mine) : d > 0 ? d + log((double)l + exp(-d)) : log1p((double)l * exp(d));
+    loss[i] = (float)(one * (rows.weight ? (double)rows.weight[i] : 1.0));
+    if (stats) stats[i] = make_float2((float)(one + (double)mine), (float)expm1(-one));
+}
+
+}  // namespace

@@ -365,3 +365,27 @@ def test_refusals(gpu_ctx):
     assert loss(rows=0) == 0 and grad(dx=None, dW=None) == 0
     gpu_ctx.synchronize()
     assert not f.any()
+
+
+# ---------------------------------------------------------------- every form of the calls: a few classes, tiles of logits, kept logits
+FORMS = {"few": (48, 30, 40), "tiled": (150, 300, 136), "kept": (60, 70, 2100)}
+
+
+def with_an_infinite_weight(form, dtype):
+    """Weights of class 4 with an infinity in column 3, and every x there -1: logits of class 4 are -infinity."""
+    rows, vocab, k = FORMS[form]
+    x, W, target, weight = inputs(rows, vocab, k, dtype, seed=11, ignored=False)
+    target[target == 4] = 5
+    x[:, 3], W[4, 3] = -1.0, float("inf")
+    return x, W, target, weight
+
+
+# (fp32 operands go to the tensor cores as sums of three numbers, which infinities have none: tiled and kept forms give NaN)
+@gpu
+@pytest.mark.parametrize("form,dtype", [("few", "f32"), ("few", "f16"), ("few", "bf16"), ("tiled", "f16"), ("tiled", "bf16"), ("kept", "f16"), ("kept", "bf16")])
+def test_an_own_logit_of_infinity_has_no_loss(gpu_ctx, form, dtype):
+    x, W, target, weight = with_an_infinite_weight(form, dtype)
+    x[7, 3], target[7] = 1.0, 4            # the one row with +infinity among its logits, and that its own class's
+    loss, dx, dW = both(gpu_ctx, x, W, target, weight)
+    assert bool(loss[7].isnan()) and bool(loss[:7].isfinite().all()) and bool(loss[8:].isfinite().all())
+    assert bool(dx[7].isnan().all()) and bool(dW.isnan().all())
