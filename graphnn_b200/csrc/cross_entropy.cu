@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(256) xe_join_kernel(int64_t rows_n, int lines,
         run[i] = make_float2(s.m, s.l);
         return;
     }
-    if (rows.own(i) < 0) {
+    if (rows.its(i) < 0) {
         loss[i] = 0.0f;
         if (stats) stats[i] = make_float2(0.0f, 0.0f);
         return;
@@ -134,7 +134,7 @@ bool xe_keeps(int64_t rows, int64_t vocab, int64_t k, int parts)
 __global__ void __launch_bounds__(256) xe_kept_loss_kernel(xe_rows rows, const float* __restrict__ z, int64_t ldz, float* __restrict__ loss, float2* __restrict__ stats)
 {
     __shared__ float of[2][8];
-    const int64_t i = blockIdx.x, own = rows.own(i);
+    const int64_t i = blockIdx.x, own = stats ? rows.its(i) : rows.own(i);
     if (own < 0) {
         if (threadIdx.x == 0) {
             loss[i] = 0.0f;
@@ -316,6 +316,7 @@ int s2v_linear_cross_entropy(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int6
     const xe_call c(ctx, st, rows, vocab, k, type, x, ldx, W, ldw, target, row_weight, ws, false);
     const xe_space& space = c.space;
     mm16_args a = c.args;
+    a.weight = nullptr;   // (a row whose weight is 0 here may have another one in the gradient)
     int done = S2V_OK;
     if (c.copy_x) done = mm16_pack(ctx, st, rows, k, type, x, ldx, nullptr, nullptr, 0, ws + space.x16, space.ld16, rows * space.ld16);
     a.part = reinterpret_cast<float2*>(ws + space.part), a.mine = reinterpret_cast<float*>(ws + space.mine);

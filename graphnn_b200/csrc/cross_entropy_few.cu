@@ -53,7 +53,7 @@ template <typename T> __device__ __forceinline__ void xf_logits(const XfArgs& a,
 template <typename T> __global__ void __launch_bounds__(XF_CTA) xe_few_loss_kernel(const XfArgs a)
 {
     __shared__ float x[XF_COLS], z[XF_CLASSES];
-    const int i = blockIdx.x, own = (int)a.of.own(i);
+    const int i = blockIdx.x, own = (int)(a.stats ? a.of.its(i) : a.of.own(i));
     if (own < 0) {
         if (threadIdx.x == 0) {
             a.loss[i] = 0.0f;

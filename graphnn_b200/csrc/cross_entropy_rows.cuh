@@ -10,23 +10,26 @@ struct xe_rows {
     const int32_t* target;
     const float* weight;   // NULL: ones
     int64_t vocab;
-    // the row's class, -1 if it is left out
-    __device__ __forceinline__ int64_t own(int64_t i) const
+    // the row's class, -1 if it has none
+    __device__ __forceinline__ int64_t its(int64_t i) const
     {
         const int64_t t = target[i];
-        return t < 0 || t >= vocab || (weight && weight[i] == 0.0f) ? -1 : t;
+        return t < 0 || t >= vocab ? -1 : t;
     }
+    __device__ __forceinline__ bool counts(int64_t i) const { return !weight || weight[i] != 0.0f; }
+    // the row's class, -1 if it is left out
+    __device__ __forceinline__ int64_t own(int64_t i) const { return counts(i) ? its(i) : -1; }
 };
 
 // A row's loss and what is kept of it, from the largest logit m and l = sum exp(z - m) of the other classes and the own one's logit:
 // log(1 + l exp(m - z_t)), from whichever side is the larger; alone in the vocabulary a class loses nothing.  An own logit of +infinity has no loss (infinity less
-// infinity), although the others are nothing beside it.
+// infinity), although the others are nothing beside it.  What is kept has nothing to do with the row's weight, which the gradient's call brings along: a weight of 0 here need not be 0 there.
 __device__ __forceinline__ void xe_finish(const xe_rows& rows, int64_t i, float m, float l, float mine, float* loss, float2* stats)
 {
     const double d = (double)m - (double)mine;
     const bool alone = m == -INFINITY && l == 0.0f;
     const double one = alone || mine == INFINITY ? (double)(mine - mine) : d > 0 ? d + log((double)l + exp(-d)) : log1p((double)l * exp(d));
-    loss[i] = (float)(one * (rows.weight ? (double)rows.weight[i] : 1.0));
+    loss[i] = !rows.counts(i) ? 0.0f : (float)(one * (rows.weight ? (double)rows.weight[i] : 1.0));
     if (stats) stats[i] = make_float2((float)(one + (double)mine), (float)expm1(-one));
 }
 

@@ -389,3 +389,37 @@ def test_an_own_logit_of_infinity_has_no_loss(gpu_ctx, form, dtype):
     loss, dx, dW = both(gpu_ctx, x, W, target, weight)
     assert bool(loss[7].isnan()) and bool(loss[:7].isfinite().all()) and bool(loss[8:].isfinite().all())
     assert bool(dx[7].isnan().all()) and bool(dW.isnan().all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("form", FORMS)
+def test_a_gradient_with_other_row_weights_than_the_loss(gpu_ctx, form, dtype):
+    rows, vocab, k = FORMS[form]
+    x, W, target, weight = inputs(rows, vocab, k, dtype, seed=12)
+    other = weight.flip(0) * 1.5
+    weight[5:9], other[7:12] = 0.0, 0.0                     # in one call alone, and in both
+    x[[1, rows // 2, rows - 1, rows // 4]] = 0.0            # (rows of the helper's that one of the calls may count)
+    target[1], x[1] = -1, float("nan")                      # no class: left out in either
+    x[8] = float("nan")                                     # left out by weights of 0 in either
+    loss, stats = torch.full((rows,), 5.0, device="cuda"), torch.full((rows, 2), 5.0, device="cuda")
+    dx, dW, ws = torch.full_like(x, 5.0), torch.full_like(W, 5.0), space(gpu_ctx, rows, vocab, k, W.dtype)
+    torch.cuda.synchronize()
+    gpu_ctx.linear_cross_entropy(x, W, target, loss, ws, row_weight=weight, stats=stats)
+    gpu_ctx.linear_cross_entropy_grad(x, W, target, stats, ws, dx=dx, dW=dW, row_weight=other)
+    gpu_ctx.synchronize()
+    Reference(x, W, target, weight).check_loss(loss)
+    ref = Reference(x, W, target, other)
+    ref.check_grad(dx, dW)
+    assert not dx[~ref.live].any()
+    # the loss is the same without stats, and without a weight the gradient is that of every row with a class
+    again = torch.full((rows,), 5.0, device="cuda")
+    gpu_ctx.linear_cross_entropy(x, W, target, again, ws, row_weight=weight)
+    x[8] = 0.25
+    torch.cuda.synchronize()
+    gpu_ctx.linear_cross_entropy(x, W, target, loss, ws, row_weight=torch.zeros_like(weight), stats=stats)
+    gpu_ctx.linear_cross_entropy_grad(x, W, target, stats, ws, dx=dx, dW=dW)
+    gpu_ctx.synchronize()
+    Reference(torch.where(x.isnan(), 0.0, x), W, target, weight).check_loss(again)
+    assert not loss.any()
+    Reference(x, W, target, None).check_grad(dx, dW)
