@@ -23,14 +23,18 @@ struct xe_rows {
 
 // A row's loss and what is kept of it, from the largest logit m and l = sum exp(z - m) of the other classes and the own one's logit:
 // log(1 + l exp(m - z_t)), from whichever side is the larger; alone in the vocabulary a class loses nothing.  An own logit of +infinity has no loss (infinity less
-// infinity), although the others are nothing beside it.  What is kept has nothing to do with the row's weight, which the gradient's call brings along: a weight of 0 here need not be 0 there.
+// infinity), although the others are nothing beside it; one of -infinity loses everything, and the others' sum is what it is.  What is kept has nothing to do with the row's weight, which the gradient's call brings along: a weight of 0 here need not be 0 there.
 __device__ __forceinline__ void xe_finish(const xe_rows& rows, int64_t i, float m, float l, float mine, float* loss, float2* stats)
 {
     const double d = (double)m - (double)mine;
-    const bool alone = m == -INFINITY && l == 0.0f;
-    const double one = alone || mine == INFINITY ? (double)(mine - mine) : d > 0 ? d + log((double)l + exp(-d)) : log1p((double)l * exp(d));
+    double one, lse;
+    if ((m == -INFINITY && l == 0.0f) || mine == INFINITY) one = (double)(mine - mine), lse = one + (double)mine;
+    else if (d > 0) {
+        const double beside = log((double)l + exp(-d));   // the sum of all relative to m
+        one = d + beside, lse = (double)m + beside;
+    } else one = log1p((double)l * exp(d)), lse = one + (double)mine;
     loss[i] = !rows.counts(i) ? 0.0f : (float)(one * (rows.weight ? (double)rows.weight[i] : 1.0));
-    if (stats) stats[i] = make_float2((float)(one + (double)mine), (float)expm1(-one));
+    if (stats) stats[i] = make_float2((float)lse, (float)expm1(-one));
 }
 
 }  // namespace

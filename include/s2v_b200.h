@@ -293,7 +293,7 @@ int s2v_linear_i8_grad(s2v_ctx* ctx, s2v_stream stream, int64_t m, int64_t n, in
  *     loss_i = row_weight_i (log sum_j exp z_ij - z_it),  t = target_i
  * x : [rows x k], W : [vocab x k] (a class a row), both of `type`; target : int32 [rows]; row_weight : [rows] or NULL (1).  A row whose target lies outside
  * [0, vocab), or whose row_weight is 0, is left out: loss 0 and gradient 0, whatever x holds there.  A row with NaN or +infinity among its logits has NaN as its
- * loss, and makes dW NaN.  The loss keeps its digits where the own class has nearly all of the probability.  Logits are fp32 sums (of fp32 operands as three bf16 numbers each, off by
+ * loss, and makes dW NaN; an own logit of -infinity beside finite ones has a loss of infinity and the gradients below.  The loss keeps its digits where the own class has nearly all of the probability.  Logits are fp32 sums (of fp32 operands as three bf16 numbers each, off by
  * some 2^-24 of sum |x W|); fp32 matrices with an infinity give NaN.  loss : [rows]; stats : float [rows x 2], 8-byte aligned, or NULL, for the gradient: they do not depend
  * on row_weight (0, 0 in a row without a class).
  * `grad` of the workspace's size: whether it has to do for s2v_linear_cross_entropy_grad too. */

@@ -423,3 +423,23 @@ def test_a_gradient_with_other_row_weights_than_the_loss(gpu_ctx, form, dtype):
     Reference(torch.where(x.isnan(), 0.0, x), W, target, weight).check_loss(again)
     assert not loss.any()
     Reference(x, W, target, None).check_grad(dx, dW)
+
+
+@gpu
+@pytest.mark.parametrize("form,dtype", [("few", "f32"), ("few", "f16"), ("few", "bf16"), ("tiled", "f16"), ("tiled", "bf16"), ("kept", "f16"), ("kept", "bf16")])
+def test_an_own_logit_of_minus_infinity_leaves_the_others_their_gradients(gpu_ctx, form, dtype):
+    x, W, target, weight = with_an_infinite_weight(form, dtype)
+    target[7] = 4
+    loss, dx, dW = both(gpu_ctx, x, W, target, weight)
+    assert float(loss[7]) == float("inf") * weight[7].sign() and bool(loss[:7].isfinite().all()) and bool(loss[8:].isfinite().all())
+    # the other classes' logits as without class 4, whose G is -w in row 7 and 0 elsewhere
+    rest = torch.arange(W.shape[0], device="cuda") != 4
+    ref = Reference(x, W[rest], torch.where(target > 4, target - 1, target), weight)
+    ref.G[7] = ref.w[7] * (ref.x[7] @ ref.W.t()).softmax(0)
+    ref.p[7] = ref.G[7] / ref.w[7]
+    G, p, used = torch.zeros(x.shape[0], W.shape[0], dtype=torch.float64, device="cuda"), torch.zeros(x.shape[0], W.shape[0], dtype=torch.float64, device="cuda"), W.double()
+    G[:, rest], p[:, rest] = ref.G, ref.p
+    G[7, 4], used[4, 3] = -ref.w[7], 0.0
+    ref.G, ref.p, ref.W = G, p, used
+    dx[:, 3] = (G @ used)[:, 3].to(dx.dtype)     # (products with the infinity: infinite, or NaN as 0 times it is)
+    ref.check_grad(dx, dW)
