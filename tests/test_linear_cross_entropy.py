@@ -443,3 +443,121 @@ def test_an_own_logit_of_minus_infinity_leaves_the_others_their_gradients(gpu_ct
     ref.G, ref.p, ref.W = G, p, used
     dx[:, 3] = (G @ used)[:, 3].to(dx.dtype)     # (products with the infinity: infinite, or NaN as 0 times it is)
     ref.check_grad(dx, dW)
+
+
+# ---------------------------------------------------------------- every form at its limits: certain rows, weights far apart
+# (fp32 takes three 16-bit numbers an operand, and so six panels for one: fewer columns make its sums long)
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,vocab,k", [(40, 40, 64), (40, 300, 300), (40, 40, 2100)], ids=["few", "tiled", "kept"])
+def test_certain_rows_in_every_form(gpu_ctx, rows, vocab, k, dtype):
+    # logits of 20 to 60 in the own class and 0 in the others: losses of vocab e^-20 and far less; all logits are exact
+    W = torch.eye(vocab, k, device="cuda").to(TYPES[dtype])
+    at = torch.arange(rows, device="cuda") * (vocab // rows)
+    x = torch.zeros((rows, k), device="cuda")
+    x[torch.arange(rows), at] = torch.linspace(20, 60, rows, device="cuda")
+    x = x.to(TYPES[dtype])
+    target = at.to(torch.int32)
+    loss, dx, dW = both(gpu_ctx, x, W, target, None)
+    ref = Reference(x, W, target, None)
+    ref.check_loss(loss)
+    ref.check_grad(dx, dW)
+    # the others' exponentials are equal, and their sum in any order off by a rounding each; two steps of the exponential, the logarithm in 64 bits, the loss rounded
+    assert bool(((loss.double() / ref.loss - 1).abs() < U * (vocab + 150)).all()) and float(loss[-1]) < 1e-20
+    # dx of the own class is its G: rounded to the type, with `fix` for what 16 bits of G lose, so that the type's rounding of dx is left, and fp16's smallest step
+    own, want = dx[torch.arange(rows), at].double(), torch.expm1(-ref.one)
+    f = torch.finfo(TYPES[dtype])
+    assert bool(((own - want).abs() <= want.abs() * (f.eps / 2 + U * (vocab + 200)) + f.smallest_normal * f.eps).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,vocab,k", [(48, 30, 64), (200, 700, 136), (60, 40, 2100)], ids=["few", "tiled", "kept"])
+def test_weights_six_decades_apart_in_every_form(gpu_ctx, rows, vocab, k, dtype):
+    x, W, target, _ = inputs(rows, vocab, k, dtype, seed=13, ignored=False)
+    weight = torch.logspace(-3, 3, rows, device="cuda")[torch.randperm(rows, generator=torch.Generator().manual_seed(3))]
+    weight[::3] *= -1.0
+    loss, dx, dW = both(gpu_ctx, x, W, target, weight)
+    ref = Reference(x, W, target, weight)
+    ref.check_loss(loss)
+    ref.check_grad(dx, dW)
+
+
+# ---------------------------------------------------------------- all of fp32: sums of so few terms that a lost part of an operand shows
+def spare(rows, k, gen, low, high):
+    """[rows x k] with one number a row, of any fp32 mantissa, in column after column."""
+    x = torch.zeros((rows, k), device="cuda")
+    i = torch.arange(rows, device="cuda")
+    sign = torch.randint(0, 2, (rows,), generator=gen, device="cuda") * 2.0 - 1.0
+    x[i, i * 7 % k] = sign * (low + (high - low) * torch.rand(rows, generator=gen, device="cuda"))
+    return x
+
+
+# An operand in three bf16 numbers is off by 2^-27 of it, and six of nine products leave out 2^-26 and two of 2^-35: together below 2^-24.  Each of the six that are added to others is a
+# rounding, or a cut, twice as much; further terms of a sum are zeros and change nothing.  In units of sum |x W|, for `terms` products that are none:
+def product_tol(terms):
+    return U * (1 + 2 * 6 * terms + 2)
+
+
+@gpu
+@pytest.mark.parametrize("rows,k", [(600, 303), (600, 3207), (200, 41)], ids=["tiled", "kept", "few"])
+def test_fp32_logits_keep_all_their_digits(gpu_ctx, rows, k):
+    gen = torch.Generator(device="cuda").manual_seed(14)
+    x = spare(rows, k, gen, 3.0, 6.0).abs()
+    W = 3.0 + 3.0 * torch.rand((2, k), generator=gen, device="cuda")
+    W[0] *= -1.0
+    target = torch.zeros(rows, dtype=torch.int32, device="cuda")     # the class far behind: the loss is the two logits' difference, 18 to 72, and e^-18 and less
+    loss, _, _ = both(gpu_ctx, x, W, target, None)
+    z = x.double() @ W.double().t()
+    want = torch.nn.functional.softplus(z[:, 1] - z[:, 0], threshold=1e9)
+    # the logits are rounded as fp32 numbers, the loss too; of what the other class's exponential adds, at most e^-18, an error does not show
+    tol = (product_tol(1) + U) * z.abs().sum(1) + U * want
+    err = (loss.double() - want).abs()
+    assert bool((err <= tol).all()), f"off by up to {float((err / tol).max()):.3g} of the tolerance"
+
+
+@gpu
+@pytest.mark.parametrize("rows,k", [(600, 303), (600, 3207), (200, 41)], ids=["tiled", "kept", "few"])
+def test_fp32_gradients_keep_all_their_digits(gpu_ctx, rows, k):
+    gen = torch.Generator(device="cuda").manual_seed(15)
+    vocab = 3
+    x = spare(rows, k, gen, 0.01, 0.02)
+    W = 0.5 + torch.rand((vocab, k), generator=gen, device="cuda")
+    target = torch.randint(0, vocab, (rows,), generator=gen, device="cuda").to(torch.int32)
+    _, dx, dW = both(gpu_ctx, x, W, target, None)
+    X, V = x.double(), W.double()
+    z = X @ V.t()
+    p = z.softmax(1)
+    G = p.scatter_add(1, target.long()[:, None], torch.full((rows, 1), -1.0, dtype=torch.float64, device="cuda"))
+    # |z| < 0.03: logits are off by less than 0.03 of product_tol(1), twice in an exponent that holds the kept log-sum-exp (1.1 and less) too, with three roundings of 1.2 * log2(e);
+    # exponentials four steps, the sum of three, the product with the weight; of the own class's 1 - p, which is 0.6 and more, the same and its own rounding; three parts of G leave 2^-27
+    assert float(z.abs().max()) < 0.03
+    dg = (2 * 0.03 * product_tol(1) + U * (3 * 1.8 + 8 + 3 + 1 + 2 + 1)) * p.clamp(min=0.4) + U * G.abs()
+    for got, a, b, da, terms in ((dx, G, V, dg, vocab), (dW, G.t(), X, dg.t(), int((X != 0).sum(0).max()))):
+        want = a @ b
+        tol = da @ b.abs() + product_tol(terms) * (a.abs() @ b.abs()) + U * want.abs()
+        err = (got.double() - want).abs()
+        assert bool((err <= tol * (1 + 1e-6)).all()), f"off by up to {float((err / tol).nan_to_num(0).max()):.3g} of the tolerance"
+
+
+@gpu
+@pytest.mark.parametrize("dtype,k", [("bf16", 32768), ("f16", 32768), ("f32", 8192)])
+def test_long_sums_keep_the_losses_digits(gpu_ctx, dtype, k):
+    # One class with a logit of thousands, a sum of terms that all have one sign, beside 9,599 of 0: the loss is that logit.  So many classes are tiles of logits, for two rows.
+    gen = torch.Generator(device="cuda").manual_seed(16)
+    x = (0.5 + 0.5 * torch.rand((2, k), generator=gen, device="cuda")).to(TYPES[dtype])
+    W = torch.zeros((9600, k), dtype=TYPES[dtype], device="cuda")
+    W[1] = (0.5 + 0.5 * torch.rand(k, generator=gen, device="cuda")).to(TYPES[dtype])
+    target = torch.tensor([0, 9599], dtype=torch.int32, device="cuda")
+    loss, ws = torch.empty(2, device="cuda"), space(gpu_ctx, 2, 9600, k, W.dtype, False)
+    torch.cuda.synchronize()
+    gpu_ctx.linear_cross_entropy(x, W, target, loss, ws)
+    gpu_ctx.synchronize()
+    want = x.double() @ W[1].double()
+    # An accumulator of tensor memory takes 32 instructions, of 16 terms each; an instruction's 16 products and sum are cut in two places at most, a step of fp32 (2 U of the accumulator) each
+    # (2,048 instructions to an accumulator gave 2,900 U).
+    # Accumulators are added with a rounding each (512 numbers of k are one; six products of parts in fp32).
+    accumulators = k // 512 * (6 if dtype == "f32" else 1)
+    tol = U * (32 * 4 + accumulators + 4) * want
+    err = (loss.double() - want).abs()
+    assert bool((err <= tol).all()), f"off by up to {float((err / tol).max()):.3g} of the tolerance"
