@@ -316,3 +316,60 @@ def test_a_head_in_training(gpu_ctx, dtype):
     gpu_ctx.layer_norm_grad(dy, stats, dx_full, ws, x=x, weight=gamma)
     gpu_ctx.synchronize()
     assert float(torch.nn.functional.cosine_similarity(dx.double().flatten(), dx_full.double().flatten(), dim=0)) > 0.999
+
+
+# ---------------------------------------------------------------- infinities and NaN in dy, and all of fp32, in every form
+FORMS = {"few": (20, 70, 90), "general": (1000, 40, 90), "direct": (5000, 70, 90)}     # (one launch; 16-bit copies; straight from dy)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("form", FORMS)
+def test_infinities_and_nan_reach_what_they_are_part_of_alone(gpu_ctx, form, dtype):
+    dy, q, scale = inputs(*FORMS[form], dtype, seed=6)
+    clean = run(gpu_ctx, dy, q, scale)
+    rest = torch.arange(dy.shape[1], device="cuda") != 3
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        dy[5, 3] = bad
+        dW, dbias = run(gpu_ctx, dy, q, scale)
+        assert not dW[3].isfinite().any() and not dbias[3].isfinite().any()
+        assert torch.equal(dW[rest], clean[0][rest]) and torch.equal(dbias[rest], clean[1][rest])
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", [(20, 70, 90), (2000, 300, 130), (4099, 256, 128), (5000, 64, 64), (9000, 300, 100), (4500, 128, 256)])
+def test_fp32_keeps_all_its_digits(gpu_ctx, m, n, k):
+    # four rows of dy have a number in a column, so that few roundings hide a lost part of it
+    _, q, scale = inputs(m, n, k, "f32", seed=7)
+    scale = scale.clamp(min=1e-3)
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    dy, j = torch.zeros((m, n), device="cuda"), torch.arange(n, device="cuda")
+    for i in range(4):
+        dy[(j * 13 + i * (m // 4)) % m, j] = torch.randn(n, generator=gen, device="cuda")
+    dW, dbias = run(gpu_ctx, dy, q, scale)
+    d, x = dy.double(), q.double() * scale.double()[:, None]
+    want, size = d.t() @ x, d.abs().t() @ x.abs()
+    # dy times the scale is rounded, and is three bf16 numbers but for 2^-24 (the first cut to eight bits, the others rounded); twelve products that are none, added with a rounding, or a
+    # cut, twice as much, each; the result rounded
+    tol = U * (1 + 1 + 2 * 12 + 1) * size + 1e-44
+    err = (dW.double() - want).abs()
+    assert bool((err <= tol).all()), f"dW off by up to {float((err / tol).max()):.3g} of the tolerance"
+    assert bool(((dbias.double() - d.sum(0)).abs() <= 4 * U * d.abs().sum(0) + 1e-44).all())
+
+
+@gpu
+def test_long_sums_of_one_sign(gpu_ctx):
+    m, n, k = 1 << 22, 8, 16
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    dy, scale = 0.5 + 0.5 * torch.rand((m, n), generator=gen, device="cuda"), 0.5 + 0.5 * torch.rand(m, generator=gen, device="cuda")
+    q = torch.randint(64, 128, (m, k), generator=gen, device="cuda", dtype=torch.int8)
+    dW, _ = run(gpu_ctx, dy, q, scale)
+    want = torch.zeros((n, k), dtype=torch.float64, device="cuda")
+    for a in range(0, m, 1 << 20):
+        at = slice(a, a + (1 << 20))
+        want += dy[at].double().t() @ (q[at].double() * scale[at].double()[:, None])
+    # 148 shares of the rows at most, and 100 at least, of 1311 panels of 32 rows each; an accumulator takes five panels, 30 instructions of two cuts of a step (2 U) at most; accumulators
+    # are added with a rounding each, and the shares four at a time; operands as above
+    tol = U * (3 + 30 * 4 + 1311 / 5 + 37 + 4) * want
+    err = (dW.double() - want).abs()
+    assert bool((err <= tol).all()), f"off by up to {float((err / tol).max()):.3g} of the tolerance"
