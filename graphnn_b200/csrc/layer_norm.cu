@@ -767,8 +767,10 @@ int ln_launch(s2v_ctx* ctx, cudaStream_t st, int64_t rows, int64_t cols, const T
     if (pieces <= 8) return go(layer_norm_kernel<T, VEC, 1, 8>, 8);
     if (pieces <= 32) return go(layer_norm_kernel<T, VEC, 4, 8>, 8);
     if (pieces <= 128) return go(layer_norm_kernel<T, VEC, 4, 32>, 32);
-    if (pieces <= 512) return go(layer_norm_kernel<T, VEC, 2, 256>, 256);
-    if (pieces <= 1024) return go(layer_norm_kernel<T, VEC, 4, 256>, 256);
+    if constexpr (!VEC) {   // (pieces of 16 bytes go through the ring; of more rows than that takes there is no memory for)
+        if (pieces <= 512) return go(layer_norm_kernel<T, VEC, 2, 256>, 256);
+        if (pieces <= 1024) return go(layer_norm_kernel<T, VEC, 4, 256>, 256);
+    }
     return go(layer_norm_kernel<T, VEC, 8, 256>, 256);
 }
 
@@ -818,9 +820,14 @@ template <typename T, bool FROM8> int ln_grad_launch(s2v_ctx* ctx, cudaStream_t 
         if (pieces <= 8) return go(layer_norm_grad_kernel<T, VEC, 1, 8, FROM8>, 8, 8 * N);
         if (pieces <= 32) return go(layer_norm_grad_kernel<T, VEC, 4, 8, FROM8>, 8, 32 * N);
         if (pieces <= 128) return go(layer_norm_grad_kernel<T, VEC, 4, 32, FROM8>, 32, 128 * N);
-        if (pieces <= 512) return go(layer_norm_grad_kernel<T, VEC, 2, 256, FROM8>, 256, 0);
-        if (pieces <= 1024) return go(layer_norm_grad_kernel<T, VEC, 2, 512, FROM8>, 512, 0);
-        if (pieces <= 2048) return go(layer_norm_grad_kernel<T, VEC, 4, 512, FROM8>, 512, 0);
+        constexpr bool RING = VEC && !FROM8;   // rows of x in pieces of 16 bytes go through the ring, up to its limits; 8-bit rows may lie at other places
+        if constexpr (!RING) {
+            if (pieces <= 512) return go(layer_norm_grad_kernel<T, VEC, 2, 256, FROM8>, 256, 0);
+            if (pieces <= 1024) return go(layer_norm_grad_kernel<T, VEC, 2, 512, FROM8>, 512, 0);
+        }
+        if constexpr (!RING || N == 8) {
+            if (pieces <= 2048) return go(layer_norm_grad_kernel<T, VEC, 4, 512, FROM8>, 512, 0);
+        }
         if constexpr (N < 8) {
             if (pieces <= 4096) return go(layer_norm_grad_kernel<T, VEC, 8, 512, FROM8>, 512, 0);
         }
