@@ -216,9 +216,9 @@ struct xe_space {
             take(g, (size_t)rows * ldg * 2 * parts);
             take(sum, (size_t)rows * mm16_pitch(k) * sizeof(float));
             take(lines, std::max({mm16_lines_bytes(piece, products), mm16_lines_bytes(rows, products), keeps ? mm16_lines_bytes(k, products) : 0}));
-        } else {
+        } else if (keeps) take(lines, mm16_lines_bytes(k, products));
+        else {
             piece = std::min(piece, of(XE_PART_BYTES, (size_t)rows * sizeof(float2)) * 64);   // (a line for every 64 classes at most)
-            if (keeps) take(lines, mm16_lines_bytes(k, products));
             take(mine, (size_t)rows * sizeof(float));
             take(run, (size_t)rows * sizeof(float2));
             take(part, (size_t)rows * mm16_sum_lines_most(piece) * sizeof(float2));
