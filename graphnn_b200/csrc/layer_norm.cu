@@ -767,7 +767,7 @@ int ln_launch(s2v_ctx* ctx, cudaStream_t st, int64_t rows, int64_t cols, const T
     if (pieces <= 8) return go(layer_norm_kernel<T, VEC, 1, 8>, 8);
     if (pieces <= 32) return go(layer_norm_kernel<T, VEC, 4, 8>, 8);
     if (pieces <= 128) return go(layer_norm_kernel<T, VEC, 4, 32>, 32);
-    if constexpr (!VEC) {   // (pieces of 16 bytes go through the ring; of more rows than that takes there is no memory for)
+    if constexpr (!VEC) {   // (rows in pieces of 16 bytes go through the ring; no memory holds more rows than it takes)
         if (pieces <= 512) return go(layer_norm_kernel<T, VEC, 2, 256>, 256);
         if (pieces <= 1024) return go(layer_norm_kernel<T, VEC, 4, 256>, 256);
     }

@@ -39,27 +39,6 @@ struct LdArgs {
     s2v_device_status* status;
 };
 
-__device__ __forceinline__ uint64_t ld_desc(uint32_t smem_addr)   // an operand across k: 64-column blocks LD_BLOCK apart, 8 rows of k every 1024 bytes
-{
-    uint64_t d = 0;
-    d |= (uint64_t)((smem_addr >> 4) & 0x3fffu);
-    d |= (uint64_t)(LD_BLOCK >> 4) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
-}
-__device__ __forceinline__ void ld_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
-{
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        :
-        : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
 // ANB: blocks of dy in a panel (2 or 4); a thread has eight columns of one or two of a panel's rows.
 template <typename T, int ANB>
 __global__ void __launch_bounds__(LD_THREADS, 1) linear_i8_direct_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_q, const LdArgs a)
@@ -122,15 +101,15 @@ __global__ void __launch_bounds__(LD_THREADS, 1) linear_i8_direct_kernel(const _
         const bool last = at_in + 1 == a.chunk || p + 1 == panels;
         if (tc_elect()) {
             const uint32_t at = smem0 + (uint32_t)at_stage * stage_bytes;
-            const uint64_t db = ld_desc(at + (uint32_t)(PARTS * ANB) * LD_BLOCK);
+            const uint64_t db = tc_desc_across<LD_BLOCK>(at + (uint32_t)(PARTS * ANB) * LD_BLOCK);
 #pragma unroll
             for (int h = 0; h < HALVES; ++h)
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q) {
-                    const uint64_t da = ld_desc(at + (uint32_t)(q * ANB + 2 * h) * LD_BLOCK);
+                    const uint64_t da = tc_desc_across<LD_BLOCK>(at + (uint32_t)(q * ANB + 2 * h) * LD_BLOCK);
 #pragma unroll
                     for (int ks = 0; ks < LD_ROWS / 16; ++ks)   // 16 rows of 128 bytes
-                        ld_mma(tmem + (uint32_t)(buf * 256 + h * cols), da + 128u * ks, db + 128u * ks, a.idesc, at_in > 0 || q > 0 || ks > 0);
+                        tc_mma_f16<false>(tmem + (uint32_t)(buf * 256 + h * cols), da + 128u * ks, db + 128u * ks, a.idesc, at_in > 0 || q > 0 || ks > 0);
                 }
             tc_commit<false>(empty(at_stage));
             if (last) tc_commit<false>(done(buf));

@@ -77,25 +77,6 @@ struct MmArgs {
     s2v_device_status* status;
 };
 
-template <bool PAIR> __device__ __forceinline__ void mm_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
-{
-    if constexpr (PAIR)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-            :
-            : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-            : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-            :
-            : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-            : "memory");
-}
 template <bool PAIR> __device__ __forceinline__ void mm_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar)
 {
     if constexpr (PAIR)
@@ -105,17 +86,6 @@ template <bool PAIR> __device__ __forceinline__ void mm_load(uint32_t dst, const
     else
         asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
                      : "memory");
-}
-// shared-memory descriptor of an operand across k: blocks of 64 numbers MM_BLOCK apart, in them 8 rows of k every 1024 bytes (128-byte swizzle)
-__device__ __forceinline__ uint64_t mm_desc_across(uint32_t smem_addr)
-{
-    uint64_t d = 0;
-    d |= (uint64_t)((smem_addr >> 4) & 0x3fffu);
-    d |= (uint64_t)(MM_BLOCK >> 4) << 16;   // leading byte offset: the next 64 numbers
-    d |= (uint64_t)(1024 >> 4) << 32;       // stride byte offset: the next 8 rows of k
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
 }
 
 // ---- outputs: a row a lane, 32 columns at a time
@@ -353,11 +323,11 @@ __global__ void __launch_bounds__(MM_THREADS, 1) mm16_kernel(const __grid_consta
                     const uint32_t at_a = smem0 + (uint32_t)s * Cfg::STAGE, at_b = at_a + Cfg::A_BYTES;
                     // 16 numbers of k: 32 bytes of a row along k, 16 rows of 128 bytes across
                     constexpr uint32_t STEP_A = A_ACROSS ? 128u : 2u, STEP_B = B_ACROSS ? 128u : 2u;
-                    const uint64_t da = A_ACROSS ? mm_desc_across(at_a) : tc_b_desc(at_a), db = B_ACROSS ? mm_desc_across(at_b) : tc_b_desc(at_b);
+                    const uint64_t da = A_ACROSS ? tc_desc_across<MM_BLOCK>(at_a) : tc_b_desc(at_a), db = B_ACROSS ? tc_desc_across<MM_BLOCK>(at_b) : tc_b_desc(at_b);
                     const int mmas = step + a.products >= a.steps ? a.last_mmas : 4;
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks)
-                        if (ks < mmas) mm_mma<PAIR>(tmem + (uint32_t)(acc * BN), da + STEP_A * ks, db + STEP_B * ks, a.idesc, !first || ks > 0);
+                        if (ks < mmas) tc_mma_f16<PAIR>(tmem + (uint32_t)(acc * BN), da + STEP_A * ks, db + STEP_B * ks, a.idesc, !first || ks > 0);
                     tc_commit<PAIR>(bar(Cfg::EMPTY + s));
                     if (last) tc_commit<PAIR>(bar(Cfg::DONE + acc));
                 }

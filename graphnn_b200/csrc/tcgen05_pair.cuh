@@ -1,4 +1,4 @@
-// What kernels share whose tiles a CTA or a pair of CTAs multiplies: commits and waits of a pair, the order of tiles, loads of accumulators.
+// What kernels share whose tiles a CTA or a pair of CTAs multiplies: commits and waits of a pair, products of 16-bit operands, the order of tiles, loads of accumulators.
 #pragma once
 
 #include "tcgen05.cuh"
@@ -51,6 +51,38 @@ __device__ __forceinline__ uint32_t tc_pair_first(uint32_t bar)
     uint32_t r;
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(bar));
     return r;
+}
+
+// 16 numbers along k of 16-bit operands, by a CTA or by a pair, of which the first issues them for both.
+template <bool PAIR> __device__ __forceinline__ void tc_mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+{
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+            :
+            : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+            :
+            : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+// shared-memory descriptor of an operand across k: blocks of 64 numbers BLOCK bytes apart, in them 8 rows of k every 1024 bytes (128-byte swizzle)
+template <uint32_t BLOCK> __device__ __forceinline__ uint64_t tc_desc_across(uint32_t smem_addr)
+{
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr >> 4) & 0x3fffu);
+    d |= (uint64_t)(BLOCK >> 4) << 16;      // leading byte offset: the next 64 numbers
+    d |= (uint64_t)(1024 >> 4) << 32;       // stride byte offset: the next 8 rows of k
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
 }
 
 // Tiles in columns of 16 row tiles, so that the tiles of one moment share panels of both matrices in L2.
