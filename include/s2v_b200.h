@@ -305,7 +305,7 @@ int s2v_linear_cross_entropy(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int6
  * gradient that arrives at each row's loss):
  *     G_ij = row_weight_i (exp z_ij / sum_j exp z_ij - [j = t]);   dx = G W;   dW = G^T x
  * dx : [rows x k], dW : [vocab x k] of `type`; either may be NULL; they overlap no input and not each other.  Where `type` has 16 bits, G is rounded to it for the
- * products (half a step of it, as x and W have; the own class's part of dx is not), with fp32 sums. */
+ * products (half a step of it, as x and W have; the own class's part of dx is not), with fp32 sums; fp16 in steps of no less than 2^-38 of the largest |row_weight|. */
 int s2v_linear_cross_entropy_grad(s2v_ctx* ctx, s2v_stream stream, int64_t rows, int64_t vocab, int64_t k, int type, const void* x, int64_t ldx,
                                   const void* W, int64_t ldw, const int32_t* target, const float* row_weight, const float* stats, void* workspace,
                                   size_t workspace_bytes, void* dx, int64_t lddx, void* dW, int64_t lddw);
